@@ -118,7 +118,7 @@ def _quantise(x, fmt):
     m, e = torch.frexp(b.abs().amax(-1))
     # the exponent of the largest magnitude once that is rounded to the element's precision
     up = (m >= (0.875 if fmt == "fp4" else 1 - 2.0 ** -8)).to(e.dtype)
-    e = (e - 1 + up - (2 if fmt == "fp4" else 0)).clamp(-127, 127)
+    e = (e - 1 + up - (2 if fmt == "fp4" else 0)).clamp(-126, 127)
     v = torch.ldexp(b, -e[..., None])
     if fmt == "fp4":
         a = v.abs()
@@ -140,19 +140,19 @@ def _quantised_values(x, fmt):
 
 def _pack_fp4(x):
     """x [rows, n] in the package's layout: rows padded with zeros to a multiple of
-    128 values, two codes a byte (the lower value in the lower half), one scale
-    byte (exponent + 127) a block."""
+    128 values, two codes a byte (the lower value in the lower half); one scale
+    byte (exponent + 127, 0 for a block of zeros) a block, [n / 128][rows][4]."""
     v, e = _quantise(_pad(x.float(), 128), "fp4")
     grid = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], device=x.device)
     code = torch.bucketize(v.abs(), grid) + 8 * (v < 0)
     code = code.reshape(x.shape[0], -1, 2).to(torch.uint8)
     zero = v.reshape(x.shape[0], e.shape[1], BLOCK).abs().amax(-1) == 0
-    return Packed((code[..., 0] | (code[..., 1] << 4)).contiguous(),
-                  torch.where(zero, 0, e + 127).to(torch.uint8).contiguous())
+    scales = torch.where(zero, 0, e + 127).to(torch.uint8).reshape(x.shape[0], -1, 4)
+    return Packed((code[..., 0] | (code[..., 1] << 4)).contiguous(), scales.transpose(0, 1).contiguous())
 
 
 def _unpack_fp4(packed, n):
-    codes, scales = packed
+    codes, scales = packed.codes, packed.scales.transpose(0, 1).reshape(packed.codes.shape[0], -1)
     grid = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], device=codes.device)
     grid = torch.cat([grid, -grid])
     v = grid[torch.stack([codes & 15, codes >> 4], -1).reshape(codes.shape[0], -1).int()]
@@ -277,14 +277,17 @@ def _run_own(s):
         return s["out"]
     M, K, B, op = case["M"], case["K"], case["batch"], case["op"]
     if case["kind"] == "serve":
-        mx.build_mx_predict(M, K, B, act, dt)(s["x"], mx.MXMatrix(*s["w4"]), s["out"])
+        predict = mx.build_mx_predict(M, K, B, act, dt)
+        predict(s["x"], mx.MXMatrix(*s["w4"]), s["out"], workspace=predict.new_workspace(s["x"].device))
         return s["out"]
     if case["kind"] == "backward":
         save = mx.build_checkpoint_save(K, B, dt)
         x8 = save.new_output(s["x"].device)
         save(s["x"], x8)
-        mx.build_checkpoint_gradient(K, M, B, act, dt)(s["w"], s["e"], x8, s["grad"])
-        mx.build_checkpoint_weight_update(M, K, B, act, dt, ALPHA)(s["w"], s["e"], x8)
+        gradient = mx.build_checkpoint_gradient(K, M, B, act, dt)
+        gradient(s["w"], s["e"], x8, s["grad"], workspace=gradient.new_workspace(s["x"].device))
+        update = mx.build_checkpoint_weight_update(M, K, B, act, dt, ALPHA)
+        update(s["w"], s["e"], x8, workspace=update.new_workspace(s["x"].device))
         return {"w": s["w"], "grad": s["grad"]}
 
     def packed4(x, rows, cols, activation, axis):
@@ -347,7 +350,7 @@ def _nearest(x, fmt, dim):
     whole = torch.floor(torch.log2(top.clamp(min=2.0 ** -140)))  # log2 may be a unit off next to a power of two
     whole = whole + (top >= 2.0 ** (whole + 1)) - (top < 2.0 ** whole).double()
     limit = 7.0 / 4 if fmt == "fp4" else 255.0 / 128  # from here on the largest magnitude rounds to the next power
-    scale = 2.0 ** ((whole + (top >= limit * 2.0 ** whole).double()) - (2 if fmt == "fp4" else 0)).clamp(-127, 127)
+    scale = 2.0 ** ((whole + (top >= limit * 2.0 ** whole).double()) - (2 if fmt == "fp4" else 0)).clamp(-126, 127)
     a = b.abs() / scale
     if fmt == "fp4":
         q = torch.zeros_like(a)
