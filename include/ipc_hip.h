@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define IPC_ABI_VERSION 6
+#define IPC_ABI_VERSION 7
 
 /* status codes */
 #define IPC_OK 0
@@ -494,6 +494,67 @@ long long ipc_s16_workspace_bytes(int kind, int act, int M, int K, int B, int gr
 long long ipc_s16_workspace_bytes_tile(int kind, int act, int M, int K, int B, int groups, int tile);
 int ipc_set_s16_preactivate(int mode);
 int ipc_s16_preactivates(int kind, int act, int M, int K, int B);
+
+/*
+ * Microscaled storage (OCP MX): 32 consecutive values of a row share one
+ * power-of-two scale.  No counterpart in the reference.
+ *
+ * A packed matrix of `rows` rows of `n` values is a pair of buffers:
+ *   codes   IPC_MX_FP4: E2M1 elements (0 0.5 1 1.5 2 3 4 6 and negatives), two a
+ *           byte, the lower value in the lower half, rows padded with zeros to
+ *           a multiple of 128 values; IPC_MX_INT8: signed bytes, value = code *
+ *           2^(s - 133), rows padded to a multiple of 32.  16-byte aligned.
+ *   scales  [ceil(n / 128)][rows][4] bytes s, block scale 2^(s - 127), 0 for a
+ *           block of zeros, 255 for one that holds an infinity or NaN (all of it
+ *           reads as NaN).  4-byte aligned.
+ * A block's scale comes from its largest magnitude rounded to the element's
+ * precision, 2^-126 at the least: fp4 amax < 7 * scale, int8 amax < 2 * scale.
+ * Elements round to nearest, ties to even; the products with powers of two are
+ * exact, so a packed matrix is the same wherever it is made.
+ * ipc_mx_code_bytes / ipc_mx_scale_bytes: the buffers' sizes (0: refused).
+ */
+#define IPC_MX_FP4 0
+#define IPC_MX_INT8 1
+long long ipc_mx_code_bytes(int rows, int n, int format);
+long long ipc_mx_scale_bytes(int rows, int n);
+
+/* f(x), x [R][C], into a packed matrix: axis 1 its rows (R rows of C values),
+ * axis 0 its columns (C rows of R values, the transpose), which is how an
+ * operand whose contraction runs along the rows of x is packed.  Kept in
+ * IPC_MX_INT8 with IPC_ACT_IDENTITY this is the 8-bit checkpoint of a state. */
+int ipc_mx_quantize(const void* x, void* codes, void* scales, int R, int C, int axis, int format, int storage,
+                    int act, void* stream);
+
+/* A packed matrix of R rows of C values back into out [R][C]. */
+int ipc_mx_dequantize(const void* codes, const void* scales, void* out, int R, int C, int format, int storage,
+                      void* stream);
+
+/*
+ * The kernel families with both operands packed in IPC_MX_FP4 along the
+ * contraction (fp32 accumulation; the other tensors are of type `storage`, the
+ * epilogue runs in fp32 and rounds once):
+ *   ipc_mx_pred_err       E = X_lower - W f(X_upper)
+ *   ipc_mx_forward        OUT = W f(X_upper)
+ *       w: W [M][K] packed by rows; x: f(X_upper) [K][B] packed by columns
+ *   ipc_mx_infer_update   X += gamma (-E + f'(X) W_lower^T E_lower)
+ *       wt: W_lower [K][M] packed by columns; et: E_lower [K][B] packed by columns
+ *   ipc_mx_weight_update  W += alpha E f(X_upper)^T
+ *       e: E [M][B] packed by rows; a: f(X_upper) [K][B] packed by rows
+ */
+int ipc_mx_pred_err(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales,
+                    const void* x_lower, void* e, int M, int K, int B, int storage, void* stream);
+int ipc_mx_forward(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, void* out,
+                   int M, int K, int B, int storage, void* stream);
+int ipc_mx_infer_update(void* x, const void* e, const void* wt_codes, const void* wt_scales, const void* et_codes,
+                        const void* et_scales, int M, int K, int B, float gamma, int storage, int act, void* stream);
+int ipc_mx_weight_update(void* w, const void* e_codes, const void* e_scales, const void* a_codes,
+                         const void* a_scales, int M, int K, int B, float alpha, int storage, void* stream);
+
+/* OUT [M][B] = W f(X) with W packed in IPC_MX_FP4 by rows and the states X [K][B]
+ * in their storage type, which are not quantised: the forward pass of one
+ * sample or a few (at most 2^20).  f(X) is carried to fp32 accuracy. */
+int ipc_mx_predict(const void* x, const void* w_codes, const void* w_scales, void* out, int M, int K, int B,
+                   int storage, int act, void* stream);
 
 void ipc_plan_destroy(ipc_plan* plan);
 

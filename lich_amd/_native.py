@@ -26,6 +26,7 @@ TILE_AUTO = -1
 TILE_DMA = 3
 TILE_DMA_TILES = (3, 4, 5, 6)  # LDS-DMA kernel: 256 x 128, 128 x 256, 128 x 128, 256 x 256
 TILE_COUNT = 7
+MX_FORMATS = {"fp4": 0, "int8": 1}
 WMODE = {"gemm": 0, "outer": 1, "auto": 2}
 SPLIT_NONE, SPLIT_W, SPLIT_WX = 1, 2, 3
 PATH_AUTO, PATH_PHASED, PATH_NARROW, PATH_WIDE, PATH_RESIDENT = -1, 0, 1, 2, 3
@@ -113,6 +114,15 @@ def _declare(lib):
         "ipc_steps_noalloc": ([i, POINTER(c_int), i, POINTER(vp), POINTER(vp), POINTER(vp), i, i, i, f, f, i, i, vp],
                               i),
         "ipc_plan_destroy": ([vp], None),
+        "ipc_mx_code_bytes": ([i, i, i], c_longlong),
+        "ipc_mx_scale_bytes": ([i, i], c_longlong),
+        "ipc_mx_quantize": ([vp, vp, vp, i, i, i, i, i, i, vp], i),
+        "ipc_mx_dequantize": ([vp, vp, vp, i, i, i, i, vp], i),
+        "ipc_mx_pred_err": ([vp, vp, vp, vp, vp, vp, i, i, i, i, vp], i),
+        "ipc_mx_forward": ([vp, vp, vp, vp, vp, i, i, i, i, vp], i),
+        "ipc_mx_infer_update": ([vp, vp, vp, vp, vp, vp, i, i, i, f, i, i, vp], i),
+        "ipc_mx_weight_update": ([vp, vp, vp, vp, vp, i, i, i, f, i, vp], i),
+        "ipc_mx_predict": ([vp, vp, vp, vp, i, i, i, i, i, vp], i),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)

@@ -21,18 +21,21 @@
 #include <vector>
 
 #include "../../include/ipc_hip.h"
+#include "ipc_abi_check.h"
 #include "ipc_launch.h"
 #include "ipc_narrow.h"
 #include "ipc_wide.h"
 
 using namespace ipc;
+using namespace ipc::abi;
 
 namespace {
 
 thread_local std::string g_last_error;
 
-int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
-int fail(int code, const char* fmt, ...) {
+}  // namespace
+
+int ipc::abi::fail(int code, const char* fmt, ...) {
   char buf[512];
   va_list ap;
   va_start(ap, fmt);
@@ -42,43 +45,7 @@ int fail(int code, const char* fmt, ...) {
   return code;
 }
 
-int ok() { return IPC_OK; }
-
-const long long kMaxElems = (1LL << 31) - 1;  // per-matrix element count (32-bit tile indices)
-
-int elem_size(int dt) { return dt == IPC_DT_F32 ? 4 : 2; }
-
-int check_dtypes(int storage, int operand) {
-  if (storage < IPC_DT_F32 || storage > IPC_DT_BF16)
-    return fail(IPC_ERR_DTYPE, "unknown storage dtype %d", storage);
-  if (operand < IPC_DT_F32 || operand > IPC_DT_BF16)
-    return fail(IPC_ERR_DTYPE, "unknown operand dtype %d", operand);
-  if (storage != IPC_DT_F32 && operand != storage)
-    return fail(IPC_ERR_DTYPE, "16-bit storage (%d) requires operand dtype == storage (got %d)",
-                storage, operand);
-  return ok();
-}
-
-int check_act(int act) {
-  if (act < IPC_ACT_IDENTITY || act > IPC_ACT_GELU)
-    return fail(IPC_ERR_ACT, "unknown activation %d", act);
-  return ok();
-}
-
-int check_dims(int M, int K, int B, int groups) {
-  if (M < 1 || K < 1 || B < 1 || groups < 1)
-    return fail(IPC_ERR_SHAPE, "dimensions must be >= 1 (M=%d K=%d B=%d groups=%d)", M, K, B, groups);
-  if ((long long)M * K > kMaxElems || (long long)M * B > kMaxElems || (long long)K * B > kMaxElems)
-    return fail(IPC_ERR_SHAPE, "matrix too large (M=%d K=%d B=%d)", M, K, B);
-  return ok();
-}
-
-int check_ptr(const void* p, const char* name, int esize) {
-  if (!p) return fail(IPC_ERR_NULL, "%s is NULL", name);
-  if (reinterpret_cast<uintptr_t>(p) % esize)
-    return fail(IPC_ERR_ALIGN, "%s is not aligned to its %d-byte element", name, esize);
-  return ok();
-}
+namespace {
 
 int check_split(int split) {
   if (split < IPC_SPLIT_NONE || split > IPC_SPLIT_WX) return fail(IPC_ERR_CONFIG, "unknown split %d", split);
@@ -94,17 +61,6 @@ int check_tile(int tile) {
   if (tile < IPC_TILE_AUTO || tile >= IPC_TILE_COUNT)
     return fail(IPC_ERR_CONFIG, "unknown tile config %d", tile);
   return ok();
-}
-
-#define TRY(x)                  \
-  do {                          \
-    const int _rc = (x);        \
-    if (_rc != IPC_OK) return _rc; \
-  } while (0)
-
-// 4-element vector loads need the contiguous length and the base aligned to 4 elements.
-int vec_ok(const void* p, long long contiguous, int esize) {
-  return (contiguous % 4 == 0) && (reinterpret_cast<uintptr_t>(p) % (4 * esize) == 0);
 }
 
 // Whether the k-chunk kernel (ipc_chunk_kernel.h) can address a problem: it
@@ -202,11 +158,6 @@ int pick_tile(int tile, const GemmProblem* q, int n, bool chunk) {
   return count_tiles<128>(q, n) >= 512 ? IPC_TILE_128x128 : t64 >= 64 ? IPC_TILE_64x64 : IPC_TILE_32x32;
 }
 
-int launch_rc(hipError_t err, const char* what) {
-  if (err != hipSuccess) return fail(IPC_ERR_LAUNCH, "%s: %s", what, hipGetErrorString(err));
-  return ok();
-}
-
 GemmProblem make_pf(int kind, const void* xu, const void* w, const void* xl, void* out, int M, int K,
                     int B, int groups, int act, int esize) {
   GemmProblem p{};
@@ -270,9 +221,6 @@ OuterProblem make_outer(void* w, const void* e, const void* xu, int M, int K, in
 }
 
 constexpr int kOuterMaxB = 32;
-
-bool al16(const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; }
-bool al8(const void* q) { return q == nullptr || reinterpret_cast<uintptr_t>(q) % 8 == 0; }
 
 // The LDS-DMA kernel serves 16-bit storage whose contraction is a multiple of
 // WIDE_BK and whose operands stream in 16-byte chunks: aligned bases, row
@@ -477,13 +425,6 @@ int run_generic(const GemmProblem& p, int storage, int operand, int split, int t
   q.act_b = IPC_ACT_IDENTITY;
   q.vec_b = vec_ok(workspace, q.ldb, 2);
   return launch_rc(launch_gemm(&q, 1, storage, operand, split, run, s), what);
-}
-
-int check_workspace(const void* workspace, long long ws_bytes) {
-  if (ws_bytes < 0) return fail(IPC_ERR_SHAPE, "workspace_bytes must be >= 0");
-  if (workspace && reinterpret_cast<uintptr_t>(workspace) % 16)
-    return fail(IPC_ERR_ALIGN, "workspace must be 16-byte aligned");
-  return ok();
 }
 
 }  // namespace

@@ -1,0 +1,74 @@
+// ipc_mx.h - microscaled storage (OCP MX): layout, host structs and launchers.
+//
+// A packed matrix holds `rows` rows of `n` values, blocks of 32 consecutive
+// values of a row sharing one power-of-two scale 2^(s - 127), s the block's
+// scale byte (E8M0; 255 = the block holds an infinity or NaN and reads as NaN):
+//
+//   fp4   E2M1 elements 0 0.5 1 1.5 2 3 4 6 and their negatives, two a byte, the
+//         lower value in the lower half; rows padded with zeros to a multiple of
+//         128 values: codes [rows][mx_row_values / 2]
+//   int8  value = code * 2^(s - 133), codes -127 .. 127; rows padded to a
+//         multiple of 32 values: codes [rows][mx_row_values]
+//   scales [ceil(n / 128)][rows][4] bytes: the four blocks of 128 values of a row
+//         in one dword, the rows' dwords contiguous, so that the 32 rows a matrix
+//         instruction takes come from one or two cache lines.
+//
+// The scale of a block follows its largest magnitude once that is rounded to
+// the element's precision (so that no element exceeds the largest code by more
+// than its own rounding): fp4 amax < 7 * 2^(s-127), int8 amax < 2 * 2^(s-127); at
+// the top of the float range it stays finite and the elements saturate.
+// Elements round to nearest, ties to the even code.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace ipc {
+
+enum { MX_FP4 = 0, MX_INT8 = 1 };
+constexpr int MX_BLOCK = 32, MX_GROUP = 128;  // values per scale, per scale dword
+
+// Values of a packed row of n, padding included.
+inline long long mx_row_values(int format, int n) {
+  const int unit = format == MX_FP4 ? MX_GROUP : MX_BLOCK;
+  return ((long long)n + unit - 1) / unit * unit;
+}
+inline long long mx_row_bytes(int format, int n) {
+  return format == MX_FP4 ? mx_row_values(format, n) / 2 : mx_row_values(format, n);
+}
+__host__ __device__ inline int mx_groups(int n) { return (int)(((long long)n + MX_GROUP - 1) / MX_GROUP); }
+
+// axis 1: rows of x [R][C] are the packed rows; axis 0: its columns.
+hipError_t launch_mx_quantize(const void* x, void* codes, void* scales, int R, int C, int axis, int format,
+                              int storage, int act, hipStream_t s);
+hipError_t launch_mx_dequantize(const void* codes, const void* scales, void* out, int R, int C, int format,
+                                int storage, hipStream_t s);
+
+// C[M][N] = sum over k of A4[m][k] B4[n][k], both fp4 with rows of `groups`
+// groups of 128 values, and the epilogue of a kernel family (GemmKind).
+struct MxProblem {
+  int kind, act;
+  int M, N, groups;
+  const uint8_t* a; const uint32_t* as;  // codes [M][groups * 64], scales [groups][M]
+  const uint8_t* b; const uint32_t* bs;  // codes [N][groups * 64], scales [groups][N]
+  void* out;                             // [M][N]: E, OUT (written), X, W (updated)
+  const void* aux;                       // [M][N]: X_lower (PRED), E (INFER)
+  float scal;                            // gamma (INFER), alpha (WEIGHT)
+  int vec;                               // out / aux allow 4-element accesses
+};
+hipError_t launch_mx_product(const MxProblem& p, int storage, hipStream_t s);
+// per storage type, one translation unit each
+hipError_t launch_mx_product_f32(const MxProblem& p, hipStream_t s);
+hipError_t launch_mx_product_f16(const MxProblem& p, hipStream_t s);
+hipError_t launch_mx_product_bf16(const MxProblem& p, hipStream_t s);
+
+// OUT [M][B] = W4 f(X), X [K][B].
+struct MxPredict {
+  int M, K, B, act;
+  const void* x;
+  const uint8_t* w; const uint32_t* ws;
+  void* out;
+};
+hipError_t launch_mx_predict(const MxPredict& p, int storage, hipStream_t s);
+
+}  // namespace ipc

@@ -1,0 +1,262 @@
+"""Microscaled operators: 4-bit products and 8-bit checkpoints (HIP, gfx950).
+
+Microscaled storage (OCP MX) keeps 32 consecutive values of a row under one
+power-of-two scale.  ``fp4`` (E2M1) carries weights and product operands,
+``int8`` carries states that a backward pass reads again.  A packed matrix is an
+``MXMatrix`` of two tensors whose layout ``include/ipc_hip.h`` states; the
+quantiser's ``new_output()`` allocates one.
+
+* ``build_mx_quantize`` / ``build_mx_dequantize``: a matrix, with f applied, into
+  packed rows (``axis=1``) or packed columns (``axis=0``) and back.
+* ``build_mx_prediction_error``, ``build_mx_forward``, ``build_mx_inference_update``,
+  ``build_mx_weight_update``: the kernel families of ``lich_amd.kernels`` with
+  both operands in fp4.
+* ``build_mx_predict``: fp4 weights, states in their own type, few samples.
+
+Each builder returns a callable that validates its tensors and enqueues on
+torch's current stream, as in ``lich_amd.kernels``; nothing is allocated or
+synchronised inside a call.  The reference has no counterpart.
+"""
+from __future__ import annotations
+
+from functools import lru_cache
+from typing import NamedTuple
+
+import torch
+
+from . import _native as nat
+from .kernels import _check, _storage_dtype
+
+BLOCK, GROUP = 32, 128  # values per scale, per four scale bytes
+
+
+class MXMatrix(NamedTuple):
+    """Packed rows: ``codes`` [rows, bytes of a row], ``scales`` [groups of 128, rows, 4]."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def _format(name: str) -> str:
+    if name not in nat.MX_FORMATS:
+        raise ValueError(f"unknown microscaled format {name!r}; expected 'fp4' or 'int8'")
+    return name
+
+
+def packed_shapes(rows: int, n: int, format: str = "fp4"):
+    """Shapes of the codes and scales of ``rows`` packed rows of ``n`` values."""
+    groups = -(-n // GROUP)
+    width = groups * GROUP // 2 if _format(format) == "fp4" else -(-n // BLOCK) * BLOCK
+    return (rows, width), (groups, rows, 4)
+
+
+def new_packed(rows: int, n: int, format: str = "fp4", device=None) -> MXMatrix:
+    """An uninitialised packed matrix of ``rows`` rows of ``n`` values."""
+    codes, scales = packed_shapes(rows, n, format)
+    device = device or torch.device("cuda")
+    return MXMatrix(torch.empty(codes, dtype=torch.uint8 if format == "fp4" else torch.int8, device=device),
+                    torch.empty(scales, dtype=torch.uint8, device=device))
+
+
+class _Packed:
+    """Checks of a packed operand, made once per kernel."""
+
+    def __init__(self, name: str, rows: int, n: int, format: str = "fp4"):
+        self.name, self.format = name, _format(format)
+        self.codes, self.scales = packed_shapes(rows, n, format)
+        self.dtype = torch.uint8 if format == "fp4" else torch.int8
+
+    def __call__(self, m):
+        if not isinstance(m, tuple) or len(m) != 2:
+            raise ValueError(f"{self.name} must be an MXMatrix (codes, scales)")
+        _check(m[0], f"{self.name}.codes", self.codes, self.dtype)
+        _check(m[1], f"{self.name}.scales", self.scales, torch.uint8)
+        return m[0].data_ptr(), m[1].data_ptr()
+
+
+def _sizes(**sizes) -> None:
+    if min(sizes.values()) < 1:
+        raise ValueError("invalid shape " + " ".join(f"{k}={v}" for k, v in sizes.items()))
+
+
+class _MXKernel:
+    def __init__(self, dtype, activation: str = "identity"):
+        self.dtype = _storage_dtype(dtype)
+        self.storage = nat.dtype_code(self.dtype)
+        self.activation = str(activation).lower()
+        self.act = nat.act_code(self.activation)
+
+
+class MXQuantizeKernel(_MXKernel):
+    """``k(X[R, C], packed)``: f(X) into packed rows (axis 1) or columns (axis 0)."""
+
+    def __init__(self, R, C, activation, dtype, format, axis):
+        super().__init__(dtype, activation)
+        _sizes(R=R, C=C)
+        if axis not in (0, 1):
+            raise ValueError(f"axis must be 0 or 1 (got {axis})")
+        self.R, self.C, self.axis, self.format = int(R), int(C), int(axis), _format(format)
+        self.rows, self.length = (self.R, self.C) if axis == 1 else (self.C, self.R)
+        self._packed = _Packed("packed", self.rows, self.length, format)
+
+    def new_output(self, device=None) -> MXMatrix:
+        return new_packed(self.rows, self.length, self.format, device)
+
+    def __call__(self, x, packed):
+        _check(x, "X", (self.R, self.C), self.dtype)
+        codes, scales = self._packed(packed)
+        nat.check(nat.lib().ipc_mx_quantize(x.data_ptr(), codes, scales, self.R, self.C, self.axis,
+                                            nat.MX_FORMATS[self.format], self.storage, self.act,
+                                            nat.current_stream_handle(x.device)))
+
+
+class MXDequantizeKernel(_MXKernel):
+    """``k(packed, OUT[R, C])``: the values of R packed rows of C."""
+
+    def __init__(self, R, C, dtype, format):
+        super().__init__(dtype)
+        _sizes(R=R, C=C)
+        self.R, self.C, self.format = int(R), int(C), _format(format)
+        self._packed = _Packed("packed", self.R, self.C, format)
+
+    def __call__(self, packed, out):
+        codes, scales = self._packed(packed)
+        _check(out, "OUT", (self.R, self.C), self.dtype)
+        nat.check(nat.lib().ipc_mx_dequantize(codes, scales, out.data_ptr(), self.R, self.C,
+                                              nat.MX_FORMATS[self.format], self.storage,
+                                              nat.current_stream_handle(out.device)))
+
+
+class _MXProduct(_MXKernel):
+    def __init__(self, M, K, B, dtype, activation="identity"):
+        super().__init__(dtype, activation)
+        _sizes(M=M, K=K, B=B)
+        self.M, self.K, self.B = int(M), int(K), int(B)
+
+
+class MXPredictionErrorKernel(_MXProduct):
+    """``k(X4, W4, X_lower[M, B], E[M, B])``: ``E = X_lower - W f(X_upper)``; W [M, K]
+    packed by rows, f(X_upper) [K, B] by columns."""
+
+    def __init__(self, *a):
+        super().__init__(*a)
+        self._x, self._w = _Packed("X_upper", self.B, self.K), _Packed("W", self.M, self.K)
+
+    def __call__(self, x4, w4, x_lower, e):
+        x, w = self._x(x4), self._w(w4)
+        _check(x_lower, "X_lower", (self.M, self.B), self.dtype)
+        _check(e, "E", (self.M, self.B), self.dtype)
+        nat.check(nat.lib().ipc_mx_pred_err(*x, *w, x_lower.data_ptr(), e.data_ptr(), self.M, self.K, self.B,
+                                            self.storage, nat.current_stream_handle(e.device)))
+
+
+class MXForwardKernel(_MXProduct):
+    """``k(X4, W4, OUT[M, B])``: ``OUT = W f(X_upper)``, operands as for the prediction error."""
+
+    def __init__(self, *a):
+        super().__init__(*a)
+        self._x, self._w = _Packed("X_upper", self.B, self.K), _Packed("W", self.M, self.K)
+
+    def __call__(self, x4, w4, out):
+        x, w = self._x(x4), self._w(w4)
+        _check(out, "OUT", (self.M, self.B), self.dtype)
+        nat.check(nat.lib().ipc_mx_forward(*x, *w, out.data_ptr(), self.M, self.K, self.B, self.storage,
+                                           nat.current_stream_handle(out.device)))
+
+
+class MXInferenceUpdateKernel(_MXProduct):
+    """``k(X[M, B], E[M, B], WT4, ET4)``: ``X += gamma(-E + f'(X) W_lower^T E_lower)``;
+    W_lower [K, M] and E_lower [K, B] packed by columns."""
+
+    def __init__(self, M, K, B, activation, dtype, gamma):
+        super().__init__(M, K, B, dtype, activation)
+        self.gamma = float(gamma)
+        self._w, self._e = _Packed("W_lower", self.M, self.K), _Packed("E_lower", self.B, self.K)
+
+    def __call__(self, x, e, wt4, et4):
+        _check(x, "X", (self.M, self.B), self.dtype)
+        _check(e, "E", (self.M, self.B), self.dtype)
+        w, el = self._w(wt4), self._e(et4)
+        nat.check(nat.lib().ipc_mx_infer_update(x.data_ptr(), e.data_ptr(), *w, *el, self.M, self.K, self.B,
+                                                self.gamma, self.storage, self.act,
+                                                nat.current_stream_handle(x.device)))
+
+
+class MXWeightUpdateKernel(_MXProduct):
+    """``k(W[M, K], E4, A4)``: ``W += alpha E A^T``; E [M, B] and A = f(X_upper) [K, B]
+    packed by rows."""
+
+    def __init__(self, M, K, B, dtype, alpha):
+        super().__init__(M, K, B, dtype)
+        self.alpha = float(alpha)
+        self._e, self._a = _Packed("E", self.M, self.B), _Packed("A", self.K, self.B)
+
+    def __call__(self, w, e4, a4):
+        _check(w, "W", (self.M, self.K), self.dtype)
+        e, a = self._e(e4), self._a(a4)
+        nat.check(nat.lib().ipc_mx_weight_update(w.data_ptr(), *e, *a, self.M, self.K, self.B, self.alpha,
+                                                 self.storage, nat.current_stream_handle(w.device)))
+
+
+class MXPredictKernel(_MXProduct):
+    """``k(X[K, B], W4, OUT[M, B], *, workspace=None)``: ``OUT = W f(X)``, W [M, K] packed
+    by rows, the states not quantised."""
+
+    def __init__(self, M, K, B, activation, dtype):
+        super().__init__(M, K, B, dtype, activation)
+        self._w = _Packed("W", self.M, self.K)
+
+    workspace_bytes = 0
+
+    def new_workspace(self, device=None):
+        return None
+
+    def __call__(self, x, w4, out, *, workspace=None):
+        _check(x, "X", (self.K, self.B), self.dtype)
+        w = self._w(w4)
+        _check(out, "OUT", (self.M, self.B), self.dtype)
+        nat.check(nat.lib().ipc_mx_predict(x.data_ptr(), *w, out.data_ptr(), self.M, self.K, self.B, self.storage,
+                                           self.act, nat.current_stream_handle(out.device)))
+
+
+@lru_cache(maxsize=256)
+def build_mx_quantize(R: int, C: int, activation: str = "identity", dtype="float32", *, format: str = "fp4",
+                      axis: int = 1):
+    """f(X [R, C]) into a packed matrix: R rows of C (``axis=1``) or C rows of R (``axis=0``)."""
+    return MXQuantizeKernel(R, C, activation, dtype, format, axis)
+
+
+@lru_cache(maxsize=256)
+def build_mx_dequantize(R: int, C: int, dtype="float32", *, format: str = "fp4"):
+    """A packed matrix of R rows of C values into OUT [R, C]."""
+    return MXDequantizeKernel(R, C, dtype, format)
+
+
+@lru_cache(maxsize=256)
+def build_mx_prediction_error(M: int, K: int, B: int, dtype="float32"):
+    """``E = X_lower - W f(X_upper)`` on fp4 operands."""
+    return MXPredictionErrorKernel(M, K, B, dtype)
+
+
+@lru_cache(maxsize=256)
+def build_mx_forward(M: int, K: int, B: int, dtype="float32"):
+    """``OUT = W f(X_upper)`` on fp4 operands."""
+    return MXForwardKernel(M, K, B, dtype)
+
+
+@lru_cache(maxsize=256)
+def build_mx_inference_update(M: int, K: int, B: int, activation: str, dtype="float32", gamma: float = 0.5):
+    """``X += gamma*(-E + f'(X)*W.T@E_lower)`` on fp4 operands."""
+    return MXInferenceUpdateKernel(M, K, B, activation, dtype, gamma)
+
+
+@lru_cache(maxsize=256)
+def build_mx_weight_update(M: int, K: int, B: int, dtype="float32", alpha: float = 1e-4):
+    """``W += alpha * E @ A.T`` on fp4 operands."""
+    return MXWeightUpdateKernel(M, K, B, dtype, alpha)
+
+
+@lru_cache(maxsize=256)
+def build_mx_predict(M: int, K: int, B: int, activation: str, dtype="float32"):
+    """``OUT = W f(X)`` with fp4 weights and states in ``dtype``."""
+    return MXPredictKernel(M, K, B, activation, dtype)

@@ -1,0 +1,299 @@
+"""Microscaled operators on the GPU against their definition in 64 bits."""
+import pytest
+import torch
+
+import mx_oracle as O
+from lich_amd import microscale as mx
+
+pytestmark = pytest.mark.gpu
+DT = O.DT
+
+
+def _rand(g, *shape, size=1.0):
+    return torch.randn(shape, generator=g, dtype=torch.float64) * size
+
+
+def _dev(x, storage):
+    return x.to(DT[storage]).cuda()
+
+
+def _up(t):
+    return t.cpu().double()
+
+
+def _pack4(x):
+    """Packed rows of a host matrix, by the oracle."""
+    return mx.MXMatrix(*(t.cuda() for t in O.pack(x, "fp4")))
+
+
+# ------------------------------------------------------------------ storage
+@pytest.mark.parametrize("fmt", ["fp4", "int8"])
+@pytest.mark.parametrize("storage", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("axis", [0, 1])
+@pytest.mark.parametrize("R,C", [(1, 1), (1, 33), (33, 1), (5, 31), (32, 32), (64, 784), (65, 129), (127, 130),
+                                 (256, 200), (300, 1531), (200, 64)])
+def test_quantize_is_the_definition(R, C, axis, storage, fmt):
+    """Codes and scales equal, blocks of very different sizes among them."""
+    g = torch.Generator().manual_seed(R * 7919 + C + axis)
+    x = _rand(g, R, C) * 2.0 ** torch.randint(-12, 12, (R, C // 40 + 1), generator=g).double().repeat_interleave(40, 1)[:, :C]
+    xd = _dev(x, storage)
+    x = _up(xd)
+    k = mx.build_mx_quantize(R, C, "identity", DT[storage], format=fmt, axis=axis)
+    out = k.new_output()
+    for t in out:
+        t.fill_(77)
+    k(xd, out)
+    codes, scales = O.pack(x if axis == 1 else x.T.contiguous(), fmt)
+    assert torch.equal(out.scales.cpu(), scales)
+    got = out.codes.cpu()
+    if fmt == "fp4":  # a value that rounds to zero may keep its sign
+        got = torch.stack([got & 15, got >> 4], -1)
+        codes = torch.stack([codes & 15, codes >> 4], -1)
+        got, codes = (torch.where(t == 8, 0, t) for t in (got, codes))
+    assert torch.equal(got, codes)
+
+
+@pytest.mark.parametrize("fmt", ["fp4", "int8"])
+@pytest.mark.parametrize("axis", [0, 1])
+def test_quantize_ties_edges_and_specials(fmt, axis):
+    """Midpoints and their neighbours, the largest and smallest floats, zeros,
+    infinities and NaN, in every lane of a block."""
+    rows = []
+    step = 0.25 if fmt == "fp4" else 1 / 128
+    for base in (2.0 ** -120, 1.0, 2.0 ** 100):
+        for top in (4.0, 5.0, 6.0, 6.5, 6.99, 7.0, 7.01, 7.99):
+            v = torch.arange(32, dtype=torch.float64) * step * (1 if fmt == "fp4" else 4)
+            v = v.clamp(max=top) * torch.where(torch.arange(32) % 2 == 0, 1.0, -1.0)
+            v[int(top * 4) % 32] = top
+            rows += [v * base, (v * base * (1 + 2.0 ** -20)), (v * base * (1 - 2.0 ** -20))]
+    fmax = torch.finfo(torch.float32).max
+    for special in (0.0, -0.0, fmax, -fmax, 2.0 ** -126, 2.0 ** -149, -2.0 ** -140, 2.0 ** -124, float("inf"),
+                    float("-inf"), float("nan")):
+        for at in (0, 13, 31):
+            v = torch.zeros(32, dtype=torch.float64)
+            v[at] = special
+            rows.append(v)
+            w = torch.ones(32, dtype=torch.float64) * 2.0 ** -130
+            w[at] = special
+            rows.append(w)
+    x = torch.stack(rows).float()
+    x = torch.cat([x, x.flip(1), x.roll(5, 0), x.roll(11, 0), x], 1).contiguous()
+    R, C = x.shape
+    xin = x if axis == 1 else x.T.contiguous()
+    k = mx.build_mx_quantize(*xin.shape, "identity", torch.float32, format=fmt, axis=axis)
+    out = k.new_output()
+    k(xin.cuda(), out)
+    codes, scales = O.pack(x.double(), fmt)
+    assert torch.equal(out.scales.cpu(), scales)
+    y = torch.empty((R, C), device="cuda")
+    mx.build_mx_dequantize(R, C, torch.float32, format=fmt)(out, y)
+    want = O.quantised(x.double(), fmt)
+    got = _up(y)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    off = torch.nan_to_num(got, nan=0.0) != torch.nan_to_num(want, nan=0.0)
+    assert not bool(off.any()), [(float(x[i, j]), float(got[i, j]), float(want[i, j])) for i, j in off.nonzero()[:8]]
+
+
+@pytest.mark.parametrize("act", ["relu", "tanh", "sigmoid", "silu", "gelu"])
+@pytest.mark.parametrize("axis", [0, 1])
+def test_quantize_applies_the_activation(act, axis):
+    """Each value within half an element's step of f(x) (of 2^-20 more for f in
+    fp32), padding zero although f(0) may not be."""
+    g = torch.Generator().manual_seed(3)
+    x = _rand(g, 70, 150, size=2.0).float()
+    for fmt, step in (("fp4", 1.0), ("int8", 1 / 64)):
+        k = mx.build_mx_quantize(70, 150, act, torch.float32, format=fmt, axis=axis)
+        out = k.new_output()
+        k(x.cuda(), out)
+        y = torch.empty((k.rows, k.length), device="cuda")
+        mx.build_mx_dequantize(k.rows, k.length, torch.float32, format=fmt)(out, y)
+        want = O.f(act, x.double())
+        want = want if axis == 1 else want.T
+        scale = 2.0 ** (out.scales.cpu().transpose(0, 1).reshape(k.rows, -1).double() - 127)
+        half = (scale * step * (1.0 if fmt == "fp4" else 0.5)).repeat_interleave(32, 1)[:, :k.length]
+        assert bool(((_up(y) - want).abs() <= half + 2.0 ** -20 * (1 + want.abs())).all())
+        code = out.codes.cpu()
+        assert int(code[:, -(-k.length // 2) if fmt == "fp4" else k.length:].abs().sum() if fmt == "int8" else
+                   code[:, -(-k.length // 2):].long().sum()) == 0
+
+
+@pytest.mark.parametrize("fmt", ["fp4", "int8"])
+@pytest.mark.parametrize("storage", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("R,C", [(1, 1), (3, 37), (64, 128), (65, 200), (130, 1031)])
+def test_dequantize_every_code(R, C, storage, fmt):
+    g = torch.Generator().manual_seed(R + C)
+    (r, width), (groups, _, four) = mx.packed_shapes(R, C, fmt)
+    codes = torch.randint(0, 256, (r, width), generator=g, dtype=torch.int64)
+    codes = codes.to(torch.uint8) if fmt == "fp4" else (codes - 128).clamp(min=-127).to(torch.int8)
+    scales = torch.randint(118, 134, (groups, R, four), generator=g).to(torch.uint8)
+    out = torch.empty((R, C), dtype=DT[storage], device="cuda")
+    mx.build_mx_dequantize(R, C, DT[storage], format=fmt)(mx.MXMatrix(codes.cuda(), scales.cuda()), out)
+    byte = scales.transpose(0, 1).reshape(R, -1).long()
+    c = torch.stack([codes & 15, codes >> 4], -1).reshape(R, -1).long() if fmt == "fp4" else codes.long()
+    full = torch.zeros((R, groups * 128), dtype=torch.int64)
+    full[:, :c.shape[1]] = c
+    want = O.values(full, byte, C, fmt)
+    assert torch.equal(_up(out), want.to(DT[storage]).double())
+
+
+# ------------------------------------------------------------------ products
+SHAPES = [(1, 1, 1), (16, 10, 1), (64, 784, 128), (33, 129, 31), (100, 257, 40), (31, 500, 97), (300, 130, 200),
+          (129, 384, 1025), (1000, 300, 1531), (130, 2000, 70), (2048, 640, 1600)]
+
+
+def _close(got, want, bound, storage):
+    """Within the bound of the fp32 sum and one rounding of the result."""
+    u = O.UNIT[storage]
+    tol = bound * (1 + u) + u * (want.abs() + bound) * 1.01 + 2.0 ** -149
+    if storage == "fp16":
+        tol = tol + 2.0 ** -25
+    bad = (_up(got) - want).abs() > tol
+    assert not bool(bad.any()), (float(((_up(got) - want).abs() / tol).max()), int(bad.sum()))
+
+
+@pytest.mark.parametrize("storage", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("M,K,B", SHAPES)
+def test_forward_and_prediction_error(M, K, B, storage):
+    g = torch.Generator().manual_seed(M + K + B)
+    w, x = _rand(g, M, K, size=K ** -0.5), _rand(g, B, K)
+    xl = _up(_rand(g, M, B).to(DT[storage]))
+    w4, x4 = _pack4(w), _pack4(x)
+    wq, xq = O.quantised(w, "fp4"), O.quantised(x, "fp4").T.contiguous()
+    want, bound = wq @ xq, O.product_bound(wq, xq, K)
+    out = torch.full((M, B), 7.0, dtype=DT[storage], device="cuda")
+    mx.build_mx_forward(M, K, B, DT[storage])(x4, w4, out)
+    _close(out, want, bound, storage)
+    mx.build_mx_prediction_error(M, K, B, DT[storage])(x4, w4, _dev(xl, storage), out)
+    _close(out, xl - want, bound + 2.0 ** -23 * (xl.abs() + want.abs()), storage)
+
+
+@pytest.mark.parametrize("act", ["identity", "relu", "tanh", "sigmoid", "silu", "gelu"])
+@pytest.mark.parametrize("storage", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("M,K,B", [(1, 1, 1), (33, 129, 31), (64, 10, 128), (1100, 300, 1025), (2048, 640, 1600)])
+def test_inference_update(M, K, B, storage, act):
+    g = torch.Generator().manual_seed(M + K + B)
+    x, e = (_up(_rand(g, M, B, size=s).to(DT[storage])) for s in (1.0, 0.1))
+    wt, et = _rand(g, M, K, size=K ** -0.5), _rand(g, B, K, size=0.1)
+    wq, eq = O.quantised(wt, "fp4"), O.quantised(et, "fp4").T.contiguous()
+    up, bound = wq @ eq, O.product_bound(wq, eq, K)
+    d = O.df(act, x)
+    want = x + 0.5 * (d * up - e)
+    xd = _dev(x, storage)
+    mx.build_mx_inference_update(M, K, B, act, DT[storage], 0.5)(xd, _dev(e, storage), _pack4(wt), _pack4(et))
+    # f' in fp32: a few units of 1; four roundings of the epilogue
+    bound = 0.5 * (bound * d.abs() + 2.0 ** -20 * up.abs()) + 2.0 ** -22 * (x.abs() + e.abs() + (d * up).abs())
+    _close(xd, want, bound, storage)
+
+
+@pytest.mark.parametrize("storage", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("M,K,B", [(1, 1, 1), (10, 64, 128), (33, 31, 300), (1000, 1531, 300), (2100, 2048, 129)])
+def test_weight_update(M, K, B, storage):
+    g = torch.Generator().manual_seed(M + K + B)
+    w = _up(_rand(g, M, K, size=0.1).to(DT[storage]))
+    e, a = _rand(g, M, B, size=0.1), _rand(g, K, B)
+    eq, aq = O.quantised(e, "fp4"), O.quantised(a, "fp4").T.contiguous()
+    acc, bound = eq @ aq, O.product_bound(eq, aq, B)
+    wd = _dev(w, storage)
+    k = mx.build_mx_weight_update(M, K, B, DT[storage], 0.01)
+    alpha = float(torch.tensor(0.01, dtype=torch.float32))
+    k(wd, _pack4(e), _pack4(a))
+    _close(wd, w + alpha * acc, alpha * bound + 2.0 ** -22 * (w.abs() + alpha * acc.abs()), storage)
+
+
+def test_a_nan_block_reaches_its_row_and_column_only():
+    g = torch.Generator().manual_seed(5)
+    M, K, B = 70, 300, 90
+    w, x = _rand(g, M, K), _rand(g, B, K)
+    w[3, 40] = float("inf")
+    x[5, 299] = float("nan")
+    out = torch.empty((M, B), device="cuda")
+    mx.build_mx_forward(M, K, B)(_pack4(x), _pack4(w), out)
+    bad = torch.isnan(out).cpu()
+    want = torch.zeros((M, B), dtype=torch.bool)
+    want[3, :] = True
+    want[:, 5] = True
+    assert torch.equal(bad, want)
+    out1 = torch.empty((M, B), device="cuda")
+    mx.build_mx_predict(M, K, B, "identity")(x.T.contiguous().float().cuda(), _pack4(w), out1)
+    assert torch.equal(torch.isnan(out1).cpu(), want)
+
+
+def test_zero_rows_and_far_scales():
+    """Blocks of zeros, and scales at both ends of their range that cancel."""
+    M = K = B = 130
+    w, x = torch.zeros(M, K, dtype=torch.float64), torch.zeros(B, K, dtype=torch.float64)
+    w[1:] = 2.0 ** 90
+    x[1:] = 2.0 ** -100
+    out = torch.empty((M, B), device="cuda")
+    mx.build_mx_forward(M, K, B)(_pack4(x), _pack4(w), out)
+    want = torch.zeros(M, B, dtype=torch.float64)
+    want[1:, 1:] = K * 2.0 ** -10
+    assert torch.equal(_up(out), want)
+
+
+# ------------------------------------------------------------------ few samples
+@pytest.mark.parametrize("storage", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("M,K,B", [(1, 1, 1), (10, 64, 1), (16, 784, 3), (64, 784, 4), (33, 129, 5), (100, 1531, 16),
+                                   (47, 300, 17), (130, 2100, 33), (64, 64, 100)])
+@pytest.mark.parametrize("act", ["identity", "tanh", "sigmoid"])
+def test_predict(M, K, B, storage, act):
+    g = torch.Generator().manual_seed(M + K + B)
+    w, x = _rand(g, M, K, size=K ** -0.5), _up(_rand(g, K, B).to(DT[storage]))
+    wq, fx = O.quantised(w, "fp4"), O.f(act, x)
+    want = wq @ fx
+    out = torch.full((M, B), 7.0, dtype=DT[storage], device="cuda")
+    k = mx.build_mx_predict(M, K, B, act, DT[storage])
+    k(_dev(x, storage), _pack4(w), out, workspace=k.new_workspace())
+    # f in fp32 (4 units), its terms (2^-17 of it for 16-bit states), the sum
+    term = (2.0 ** -21 if storage == "fp32" else 2.0 ** -16) * (wq.abs() @ fx.abs())
+    _close(out, want, O.product_bound(wq, fx, 3 * K) + term, storage)
+
+
+# ------------------------------------------------------------------ streams, graphs, repeats
+def test_calls_follow_torchs_stream_and_capture():
+    """Quantiser, product and serving product in a graph, replayed between eager
+    work, each replay equal to the eager result."""
+    M, K, B = 300, 784, 128
+    g = torch.Generator().manual_seed(9)
+    w = _pack4(_rand(g, M, K))
+    x = torch.randn(K, B, device="cuda", dtype=torch.bfloat16)
+    one = torch.randn(K, 1, device="cuda", dtype=torch.bfloat16)
+    out, out1 = torch.empty(M, B, device="cuda", dtype=torch.bfloat16), torch.empty(M, 1, device="cuda", dtype=torch.bfloat16)
+    q = mx.build_mx_quantize(K, B, "relu", torch.bfloat16, axis=0)
+    x4 = q.new_output()
+    forward, predict = mx.build_mx_forward(M, K, B, torch.bfloat16), mx.build_mx_predict(M, K, 1, "relu", torch.bfloat16)
+
+    def calls():
+        q(x, x4)
+        forward(x4, w, out)
+        predict(one, w, out1)
+
+    calls()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        calls()
+    for seed in range(4):
+        x.copy_(torch.randn(K, B, generator=torch.Generator().manual_seed(seed)))
+        one.copy_(torch.randn(K, 1, generator=torch.Generator().manual_seed(seed)))
+        out.zero_(), out1.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone(), out1.clone()
+        calls()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], out) and torch.equal(got[1], out1)
+
+
+def test_refusals():
+    k = mx.build_mx_quantize(64, 96, "relu", torch.bfloat16)
+    x, out = torch.zeros(64, 96, device="cuda", dtype=torch.bfloat16), k.new_output()
+    for bad in ((x.float(), out), (x.T, out), (x[:, :95].contiguous(), out), (x.cpu(), out),
+                (x, mx.MXMatrix(out.codes[:, :-1].contiguous(), out.scales)), (x, out.codes),
+                (x, mx.MXMatrix(out.codes.to(torch.int8), out.scales)), (x, mx.MXMatrix(out.codes, out.scales.cpu()))):
+        with pytest.raises(ValueError):
+            k(*bad)
+    shifted = torch.empty(out.codes.numel() + 4, dtype=torch.uint8, device="cuda")[4:].view_as(out.codes)
+    with pytest.raises(ValueError, match="aligned"):
+        k(x, mx.MXMatrix(shifted, out.scales))
