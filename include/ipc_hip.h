@@ -556,6 +556,28 @@ int ipc_mx_weight_update(void* w, const void* e_codes, const void* e_scales, con
 int ipc_mx_predict(const void* x, const void* w_codes, const void* w_scales, void* out, int M, int K, int B,
                    int storage, int act, void* stream);
 
+/*
+ * The backward pass of a layer y = W f(X) whose state X was kept in 8 bits:
+ * X packed by rows in IPC_MX_INT8 (ipc_mx_quantize, axis 1).
+ *   ipc_ckpt_weight_update  W += alpha E f(X)^T      W [M][K], E [M][B], X [K][B]
+ *                           (f(X) itself kept: IPC_ACT_IDENTITY)
+ *   ipc_ckpt_gradient       G = f'(X) W_lower^T E_lower
+ *                           W_lower [K][M], E_lower [K][B], X and G [M][B]
+ * storage, operand: as for ipc_weight_update and ipc_infer_update; the state is
+ * widened in the kernel's loader or epilogue, exactly where the operand type is
+ * fp32 or bf16.  The largest 16-bit calls use a workspace lent by the caller
+ * (16-byte aligned) as theirs do, ipc_ckpt_workspace_bytes bytes (kind
+ * IPC_PHASE_WEIGHT or IPC_PHASE_INFER for the gradient; 0: none): f(X) widened
+ * once, or the gradient's operands transposed.
+ */
+int ipc_ckpt_weight_update(void* w, const void* e, const void* x_codes, const void* x_scales, int M, int K, int B,
+                           float alpha, int storage, int operand, int act, void* workspace,
+                           long long workspace_bytes, void* stream);
+int ipc_ckpt_gradient(const void* w_lower, const void* e_lower, const void* x_codes, const void* x_scales, void* g,
+                      int M, int K, int B, int storage, int operand, int act, void* workspace,
+                      long long workspace_bytes, void* stream);
+long long ipc_ckpt_workspace_bytes(int kind, int act, int M, int K, int B, int storage);
+
 void ipc_plan_destroy(ipc_plan* plan);
 
 #ifdef __cplusplus

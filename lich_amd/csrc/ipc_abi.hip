@@ -23,6 +23,7 @@
 #include "../../include/ipc_hip.h"
 #include "ipc_abi_check.h"
 #include "ipc_launch.h"
+#include "ipc_mx.h"
 #include "ipc_narrow.h"
 #include "ipc_wide.h"
 
@@ -616,6 +617,129 @@ int ipc_weight_update_outer(void* w, const void* e, const void* x_upper, int M, 
   TRY(check_ptr(x_upper, "x_upper", es));
   OuterProblem p = make_outer(w, e, x_upper, M, K, B, groups, alpha, recompute, act);
   return launch_rc(launch_outer(p, storage, (hipStream_t)stream), "ipc_weight_update_outer");
+}
+
+}  // extern "C"
+
+// =========================================================================== 8-bit checkpoints
+namespace {
+
+// The packed state [rows][n] of a call.
+int check_state(const void* codes, const void* scales, int rows, int n) {
+  if ((long long)rows * mx_groups(n) * MX_GROUP > kMaxElems)
+    return fail(IPC_ERR_SHAPE, "packed matrix too large (%d rows of %d values, padded to a multiple of %d)", rows, n, MX_GROUP);
+  if (!codes || !scales) return fail(IPC_ERR_NULL, "the packed state is NULL");
+  if (!al16(codes) || reinterpret_cast<uintptr_t>(scales) % 4)
+    return fail(IPC_ERR_ALIGN, "the packed state needs codes aligned to 16 bytes and scales aligned to 4");
+  return ok();
+}
+
+// Bytes of caller workspace a call uses: the weight update's f(X) widened once to
+// the storage type where the 16-bit kernels would activate it once, the state
+// gradient's transposed operands where theirs would be.
+long long ckpt_workspace_need(int kind, int act, int M, int K, int B, int storage) {
+  if (storage == IPC_DT_F32) return 0;
+  if (kind == IPC_PHASE_WEIGHT) {
+    if (!s16_preact_rule(S16_WEIGHT, act, M, K, (long long)K * B)) return 0;
+    return (long long)K * B * 2;
+  }
+  if (kind != IPC_PHASE_INFER || !dma_eligible(storage, K, {}, {M, B})) return 0;
+  if (!s16_preact_rule(S16_INFER, act, M, K, (long long)K * B)) return 0;
+  return ((long long)M * K + (long long)K * B) * 2;
+}
+
+bool ckpt_lent(long long need, const void* workspace, long long ws_bytes) {
+  return need > 0 && workspace && ws_bytes >= need;
+}
+
+// Tile of a call on the generic kernels (their rules, for a problem of its size).
+int ckpt_tile(const GemmProblem& p, int storage, int operand) {
+  return pick_tile(IPC_TILE_AUTO, &p, 1, use_chunk(&p, 1, elem_size(storage), operand == IPC_DT_F32, IPC_SPLIT_NONE));
+}
+
+}  // namespace
+
+extern "C" {
+
+long long ipc_ckpt_workspace_bytes(int kind, int act, int M, int K, int B, int storage) {
+  if (M < 1 || K < 1 || B < 1 || act < IPC_ACT_IDENTITY || act > IPC_ACT_GELU) return 0;
+  return ckpt_workspace_need(kind, act, M, K, B, storage);
+}
+
+int ipc_ckpt_weight_update(void* w, const void* e, const void* x_codes, const void* x_scales, int M, int K, int B,
+                           float alpha, int storage, int operand, int act, void* workspace,
+                           long long workspace_bytes, void* stream) {
+  TRY(check_workspace(workspace, workspace_bytes));
+  TRY(check_dtypes(storage, operand));
+  TRY(check_act(act));
+  TRY(check_dims(M, K, B, 1));
+  TRY(check_state(x_codes, x_scales, K, B));
+  const int es = elem_size(storage);
+  TRY(check_ptr(w, "w", es));
+  TRY(check_ptr(e, "e", es));
+  if (ckpt_lent(ckpt_workspace_need(IPC_PHASE_WEIGHT, act, M, K, B, storage), workspace, workspace_bytes)) {
+    TRY(launch_rc(launch_mx_dequantize(x_codes, x_scales, workspace, K, B, MX_INT8, storage, act, (hipStream_t)stream),
+                  "ipc_ckpt_weight_update"));
+    return ipc_weight_update(w, e, workspace, M, K, B, 1, alpha, 0, storage, operand, act, IPC_TILE_AUTO, stream);
+  }
+  GemmProblem p = make_wgt(w, e, x_codes, M, K, B, 1, alpha, 1, act, es);
+  p.ldb = mx_row_bytes(MX_INT8, B);
+  p.vec_b = 1;
+  p.aux = x_scales; p.ldx = K;
+  if (dma_eligible(storage, B, {e}, {B}) && !generic_before_dma(p)) {
+    WideProblem q{};
+    q.M = M; q.N = K; q.K = B;
+    q.a = e; q.lda = B; q.a_lim = M;
+    q.b = x_codes; q.ldb = p.ldb; q.b_lim = K;
+    q.out = w; q.ldo = K;
+    q.aux = x_scales;
+    q.scal = alpha;
+    q.vec = K % 4 == 0 && al8(w);
+    return launch_rc(launch_s16_ckpt(S16_WEIGHT8, q, operand, act, s16_auto_config(M, K, 1), (hipStream_t)stream),
+                     "ipc_ckpt_weight_update");
+  }
+  return launch_rc(launch_ckpt_weight(p, storage, operand, ckpt_tile(p, storage, operand), (hipStream_t)stream),
+                   "ipc_ckpt_weight_update");
+}
+
+int ipc_ckpt_gradient(const void* w_lower, const void* e_lower, const void* x_codes, const void* x_scales, void* g,
+                      int M, int K, int B, int storage, int operand, int act, void* workspace,
+                      long long workspace_bytes, void* stream) {
+  TRY(check_workspace(workspace, workspace_bytes));
+  TRY(check_dtypes(storage, operand));
+  TRY(check_act(act));
+  TRY(check_dims(M, K, B, 1));
+  TRY(check_state(x_codes, x_scales, M, B));
+  const int es = elem_size(storage);
+  TRY(check_ptr(w_lower, "w_lower", es));
+  TRY(check_ptr(e_lower, "e_lower", es));
+  TRY(check_ptr(g, "g", es));
+  hipStream_t s = (hipStream_t)stream;
+  GemmProblem p = make_inf(g, x_codes, w_lower, e_lower, nullptr, M, K, B, 1, 0.0f, act, es);
+  p.ldx = mx_row_bytes(MX_INT8, B);
+  p.out2 = const_cast<void*>(x_scales); p.ld2 = M;
+  if (dma_eligible(storage, K, {w_lower, e_lower}, {M, B}) && !generic_before_dma(p)) {
+    WideProblem q{};
+    q.M = M; q.N = B; q.K = K;
+    q.a = w_lower; q.lda = M; q.a_lim = M;
+    q.b = e_lower; q.ldb = B; q.b_lim = B;
+    q.out = g; q.ldo = B;
+    q.aux = x_codes; q.ldx = p.ldx;
+    q.h = const_cast<void*>(x_scales);
+    q.vec = B % 4 == 0 && al8(g);
+    const int cfg = s16_auto_config(M, B, 1);
+    if (ckpt_lent(ckpt_workspace_need(IPC_PHASE_INFER, act, M, K, B, storage), workspace, workspace_bytes)) {
+      char* wt = static_cast<char*>(workspace);
+      char* et = wt + (long long)M * K * 2;
+      TRY(launch_rc(launch_s16_activate_t(q.a, wt, K, M, 1, 0, operand, IPC_ACT_IDENTITY, s), "ipc_ckpt_gradient"));
+      TRY(launch_rc(launch_s16_activate_t(q.b, et, K, B, 1, 0, operand, IPC_ACT_IDENTITY, s), "ipc_ckpt_gradient"));
+      q.a = wt; q.lda = K;
+      q.b = et; q.ldb = K;
+      return launch_rc(launch_s16_ckpt(S16_GRADT, q, operand, act, cfg, s), "ipc_ckpt_gradient");
+    }
+    return launch_rc(launch_s16_ckpt(S16_GRAD, q, operand, act, cfg, s), "ipc_ckpt_gradient");
+  }
+  return launch_rc(launch_ckpt_grad(p, storage, operand, ckpt_tile(p, storage, operand), s), "ipc_ckpt_gradient");
 }
 
 }  // extern "C"

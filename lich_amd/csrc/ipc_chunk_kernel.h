@@ -223,6 +223,64 @@ __device__ __forceinline__ void infer_group(int act, float gamma, bool keep, con
   }
 }
 
+// f'(x) s of four elements.
+template <typename ST, int ACT>
+__device__ __forceinline__ void grad_as(const float (&x)[4], const float (&s)[4], ST (&o)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = cvt<ST>(dact_t<ACT>(x[i]) * s[i]);
+}
+template <typename ST>
+__device__ __forceinline__ void grad_group(int act, const float (&x)[4], const float (&s)[4], ST (&o)[4]) {
+  switch (act) {
+    case ACT_RELU: return grad_as<ST, ACT_RELU>(x, s, o);
+    case ACT_TANH: return grad_as<ST, ACT_TANH>(x, s, o);
+    case ACT_SIGMOID: return grad_as<ST, ACT_SIGMOID>(x, s, o);
+    case ACT_SILU: return grad_as<ST, ACT_SILU>(x, s, o);
+    case ACT_GELU: return grad_as<ST, ACT_GELU>(x, s, o);
+    default: return grad_as<ST, ACT_IDENTITY>(x, s, o);
+  }
+}
+
+// A state kept in 8 bits as the B operand of the weight update: KL codes of a
+// row per lane and k-step; a chunk is one group of 128 values, whose four scale
+// bytes are one dword of the row.  Rows past the matrix read zeros.
+template <int T>
+struct QRaw {
+  unsigned v[T][2];
+};
+struct QState {
+  __amdgpu_buffer_rsrc_t q, s;
+  int rows, row_bytes;
+  __device__ __forceinline__ QState(const void* codes, unsigned bytes, const void* scales, int rows_, int row_bytes_,
+                                    int n)
+      : rows(rows_), row_bytes(row_bytes_) {
+    q = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(codes), (short)0, (int)bytes, 0x00020000);
+    s = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(scales), (short)0, (int)(mx_groups(n) * (unsigned)rows * 4u),
+                                          0x00020000);
+  }
+  template <int T>
+  __device__ __forceinline__ void scales(int group, int row, unsigned (&o)[T]) const {
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+      o[t] = __builtin_amdgcn_raw_buffer_load_b32(
+          s, row + t * 16 < rows ? ((unsigned)group * (unsigned)rows + (unsigned)(row + t * 16)) * 4u : OUTSIDE, 0, 0);
+  }
+  template <int T, int KL>
+  __device__ __forceinline__ void codes(int row, int k, QRaw<T>& o) const {
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      const unsigned at = row + t * 16 < rows && k < row_bytes
+                              ? (unsigned)(row + t * 16) * (unsigned)row_bytes + (unsigned)k : OUTSIDE;
+      if constexpr (KL == 8) {
+        const U2 v = (U2)__builtin_amdgcn_raw_buffer_load_b64(q, at, 0, 0);
+        o.v[t][0] = v[0]; o.v[t][1] = v[1];
+      } else {
+        o.v[t][0] = __builtin_amdgcn_raw_buffer_load_b32(q, at, 0, 0);
+      }
+    }
+  }
+};
+
 // Fewest waves of a launch: enough for one or two epilogue groups per thread,
 // also where the contraction has fewer chunks (1792 x 16 x 448 inference, tanh,
 // 64 x 64 tiles: 26 us with one wave per tile).
@@ -233,7 +291,7 @@ constexpr int min_waves(int TM, int TN, int MAXW) {
 // NS: waves that share a chunk, each with TN / NS of the tile's columns, where
 // the contraction has fewer chunks than the workgroup waves; OCC: waves per SIMD
 // the registers leave room for, that is workgroups a CU holds (run_chunk8).
-template <typename ST, typename OT, int LAYOUT, int SPLIT, int TM, int TN, int MAXW, int NS, int OCC>
+template <typename ST, typename OT, int LAYOUT, int SPLIT, int TM, int TN, int MAXW, int NS, int OCC, bool Q8 = false>
 __global__ void __launch_bounds__(MAXW * 64, OCC) chunk_kernel(const GemmBatch batch) {
   using MM = Mma<OT>;
   typedef typename MM::operand V;
@@ -242,6 +300,8 @@ __global__ void __launch_bounds__(MAXW * 64, OCC) chunk_kernel(const GemmBatch b
   constexpr bool SA = SPLIT >= 2, SB = SPLIT >= 3;
   constexpr int LDP = TN + 4;                       // floats per row of a partial tile
   constexpr int STEPS = CHUNK_K / KS;
+  constexpr bool QB = Q8 && LAYOUT == LAYOUT_WGT;   // B is a state kept in 8 bits
+  constexpr bool QX = Q8 && LAYOUT == LAYOUT_INF;   // the epilogue's X is, and the result f'(X) C
   extern __shared__ __align__(16) float part[];     // [chunks in flight][TM][LDP]
 
   const int bid = blockIdx.x;
@@ -258,6 +318,7 @@ __global__ void __launch_bounds__(MAXW * 64, OCC) chunk_kernel(const GemmBatch b
   const int lda = (int)p.lda, ldb = (int)p.ldb;
   const Mat<ST> A(reinterpret_cast<const ST*>(p.a) + (long long)g * p.a_gs, (long long)(A_KMAJ ? M : K) * lda);
   const Mat<ST> B(reinterpret_cast<const ST*>(p.b) + (long long)g * p.b_gs, (long long)(B_KMAJ ? N : K) * ldb);
+  const QState Bq(QB ? p.b : nullptr, QB ? (unsigned)(N * ldb) : 0u, QB ? p.aux : nullptr, QB ? N : 0, ldb, K);
   ST* out = reinterpret_cast<ST*>(p.out) + (long long)g * p.o_gs;
   const ST* aux = p.aux ? reinterpret_cast<const ST*>(p.aux) + (long long)g * p.x_gs : nullptr;
   ST* out2 = p.out2 ? reinterpret_cast<ST*>(p.out2) + (long long)g * p.o2_gs : nullptr;
@@ -274,15 +335,15 @@ __global__ void __launch_bounds__(MAXW * 64, OCC) chunk_kernel(const GemmBatch b
   // PRE of them each, min_waves).  Their inputs are fetched before the
   // contraction.
   constexpr int GROUPS = TM * TN / 4, PRE = GROUPS / (64 * min_waves(TM, TN, MAXW));
-  const bool need_x = kind != KIND_FWD;
+  const bool need_x = !QX && kind != KIND_FWD;
   const ST* xin = kind == KIND_PRED ? aux : out;
   const long long ldin = kind == KIND_PRED ? ldx : ldo;
   auto aligned4 = [](const void* q, long long ld) {
     return ld % 4 == 0 && reinterpret_cast<uintptr_t>(q) % (4 * sizeof(ST)) == 0;
   };
   const bool vx = need_x && aligned4(xin, ldin);
-  const bool ve = kind == KIND_INFER && aligned4(aux, ldx);
-  const bool vo = aligned4(out, ldo), v2 = out2 && aligned4(out2, ld2);
+  const bool ve = !QX && kind == KIND_INFER && aligned4(aux, ldx);
+  const bool vo = aligned4(out, ldo), v2 = !QX && out2 && aligned4(out2, ld2);
   auto load_group = [&](const ST* src, long long ld, bool vec, int gi, float (&o)[4]) {
     const int r = gi / (TN / 4), c = (gi % (TN / 4)) * 4;
     const int m = m0 + r, n = n0 + c;
@@ -303,8 +364,14 @@ __global__ void __launch_bounds__(MAXW * 64, OCC) chunk_kernel(const GemmBatch b
   for (int i = 0; i < PRE; ++i) {
     const int gi = tid + i * nthreads;
     if (gi >= GROUPS) continue;
-    if (need_x) load_group(xin, ldin, vx, gi, xs[i]);
-    if (LAYOUT == LAYOUT_INF) load_group(aux, ldx, ve, gi, es[i]);
+    if constexpr (QX) {
+      const int m = m0 + gi / (TN / 4), n = n0 + (gi % (TN / 4)) * 4;
+      if (m < M && n < N)
+        mx::state4(reinterpret_cast<const uint8_t*>(p.aux), ldx, reinterpret_cast<const uint8_t*>(p.out2), ld2, m, n, xs[i]);
+    } else {
+      if (need_x) load_group(xin, ldin, vx, gi, xs[i]);
+      if (LAYOUT == LAYOUT_INF) load_group(aux, ldx, ve, gi, es[i]);
+    }
   }
 
   for (int c0 = 0; c0 < chunks; c0 += slots) {
@@ -325,7 +392,10 @@ __global__ void __launch_bounds__(MAXW * 64, OCC) chunk_kernel(const GemmBatch b
         constexpr int AHEAD = REGS * STEPS <= ROOM ? STEPS : REGS * STEPS <= 2 * ROOM ? STEPS / 2
                               : REGS * STEPS <= 4 * ROOM ? STEPS / 4 : 1;
         Raw<ST, RM, KL> ra[AHEAD];
-        Raw<ST, RN, KL> rb[AHEAD];
+        Raw<ST, QB ? 1 : RN, KL> rb[AHEAD];
+        QRaw<QB ? RN : 1> rq[AHEAD];
+        unsigned qs[QB ? RN : 1];
+        if constexpr (QB) Bq.scales<RN>(c, n0 + nw + lr, qs);
 #pragma unroll 1
         for (int k0 = c * CHUNK_K; k0 < kend; k0 += AHEAD * KS) {
           const bool tail = k0 + AHEAD * KS > K;
@@ -334,7 +404,8 @@ __global__ void __launch_bounds__(MAXW * 64, OCC) chunk_kernel(const GemmBatch b
             const int k = k0 + s * KS + lg * KL;
             if constexpr (A_KMAJ) load_kmaj<ST, RM, KL, ODD>(A, lda, m0, k, K, tail, lr, ra[s]);
             else load_mn<ST, RM, KL, ODD>(A, lda, m0, k, K, lr, ra[s]);
-            if constexpr (B_KMAJ) load_kmaj<ST, RN, KL, ODD>(B, ldb, n0 + nw, k, K, tail, lr, rb[s]);
+            if constexpr (QB) Bq.codes<RN, KL>(n0 + nw + lr, k, rq[s]);
+            else if constexpr (B_KMAJ) load_kmaj<ST, RN, KL, ODD>(B, ldb, n0 + nw, k, K, tail, lr, rb[s]);
             else load_mn<ST, RN, KL, ODD>(B, ldb, n0 + nw, k, K, lr, rb[s]);
           }
 #pragma unroll
@@ -356,7 +427,7 @@ __global__ void __launch_bounds__(MAXW * 64, OCC) chunk_kernel(const GemmBatch b
 #pragma unroll
             for (int j = 0; j < RN; ++j) {
               bool raw = false;
-              if constexpr (std::is_same<ST, OT>::value) {
+              if constexpr (!QB && std::is_same<ST, OT>::value) {
                 if (LAYOUT == LAYOUT_INF || act_b == ACT_IDENTITY) {
                   raw = true;
 #pragma unroll
@@ -365,8 +436,14 @@ __global__ void __launch_bounds__(MAXW * 64, OCC) chunk_kernel(const GemmBatch b
               }
               if (!raw) {
                 float f[KL];
+                if constexpr (QB) {
+                  const float unit = mx::int8_scale(qs[j] >> (8 * (((k0 & (CHUNK_K - 1)) + s * KS) >> 5)) & 255u);
 #pragma unroll
-                for (int q = 0; q < KL; ++q) f[q] = to_f32(rb[s].v[j][q]);
+                  for (int q = 0; q < KL; ++q) f[q] = (float)mx::sext8(rq[s].v[j][q >> 2], q & 3) * unit;
+                } else {
+#pragma unroll
+                  for (int q = 0; q < KL; ++q) f[q] = to_f32(rb[s].v[j][q]);
+                }
                 if (LAYOUT != LAYOUT_INF) activate<KL>(act_b, f);
                 bh[j] = round_operand<OT, KL>(f, SB ? &bl[SB ? j : 0] : nullptr);
               }
@@ -383,7 +460,7 @@ __global__ void __launch_bounds__(MAXW * 64, OCC) chunk_kernel(const GemmBatch b
         }
       };
       if constexpr (sizeof(ST) == 2) {
-        if (A.odd(lda) || B.odd(ldb)) steps(std::integral_constant<bool, true>{});
+        if (A.odd(lda) || (!QB && B.odd(ldb))) steps(std::integral_constant<bool, true>{});
         else steps(std::integral_constant<bool, false>{});
       } else {
         steps(std::integral_constant<bool, false>{});
@@ -434,7 +511,9 @@ __global__ void __launch_bounds__(MAXW * 64, OCC) chunk_kernel(const GemmBatch b
       if (m >= M || n >= N) continue;
       const float (&x)[4] = xs[u], (&e)[4] = es[u];
       ST o[4], o2[4];
-      if constexpr (LAYOUT == LAYOUT_INF) {
+      if constexpr (QX) {
+        grad_group<ST>(p.act_epi, x, s, o);
+      } else if constexpr (LAYOUT == LAYOUT_INF) {
         infer_group<ST>(p.act_epi, p.scal, out2 != nullptr, x, e, s, o, o2);
       } else {
 #pragma unroll
@@ -459,16 +538,16 @@ __global__ void __launch_bounds__(MAXW * 64, OCC) chunk_kernel(const GemmBatch b
         }
       };
       store_group(out, ldo, vo, o);
-      if (LAYOUT == LAYOUT_INF && out2) store_group(out2, ld2, v2, o2);
+      if (LAYOUT == LAYOUT_INF && !QX && out2) store_group(out2, ld2, v2, o2);
     }
     if (!last) __syncthreads();
   }
 }
 
 // Launch of one tile size over a ragged batch.
-template <typename ST, typename OT, int LAYOUT, int SPLIT, int TM, int TN, int MAXW, int NS, int OCC>
+template <typename ST, typename OT, int LAYOUT, int SPLIT, int TM, int TN, int MAXW, int NS, int OCC, bool Q8 = false>
 static hipError_t run_chunk(const GemmProblem* probs, int count, hipStream_t s) {
-  const void* fn = reinterpret_cast<const void*>(&chunk_kernel<ST, OT, LAYOUT, SPLIT, TM, TN, MAXW, NS, OCC>);
+  const void* fn = reinterpret_cast<const void*>(&chunk_kernel<ST, OT, LAYOUT, SPLIT, TM, TN, MAXW, NS, OCC, Q8>);
   constexpr int TILE_BYTES = TM * (TN + 4) * 4;
   constexpr int LDS_MAX = (MAXW / NS + 1) * TILE_BYTES;
   static_assert(LDS_MAX <= 160 * 1024, "partial tiles exceed the LDS");
@@ -517,29 +596,29 @@ static hipError_t run_chunk(const GemmProblem* probs, int count, hipStream_t s) 
 // inference 800 x 800 x 400 17.5 -> 12.3, 26.8 -> 21.0, 14.7 -> 11.4); an inference
 // update of at most one tile per CU keeps the loads instead (512 x 4096 x 512,
 // fp32, 42.7 us against 54.7).
-template <typename ST, typename OT, int LAYOUT, int SPLIT, int TM, int TN>
+template <typename ST, typename OT, int LAYOUT, int SPLIT, int TM, int TN, bool Q8 = false>
 static hipError_t run_chunk8(const GemmProblem* probs, int count, hipStream_t s) {
   constexpr bool wide = sizeof(ST) == 4;
   int kmax = 0;
   for (int i = 0; i < count; ++i) kmax = std::max(kmax, probs[i].K);
   if constexpr (LAYOUT != LAYOUT_INF && TN == 64)
-    if (kmax <= (wide ? 2 : 3) * CHUNK_K) return run_chunk<ST, OT, LAYOUT, SPLIT, TM, TN, 8, 4, 4>(probs, count, s);
+    if (kmax <= (wide ? 2 : 3) * CHUNK_K) return run_chunk<ST, OT, LAYOUT, SPLIT, TM, TN, 8, 4, 4, Q8>(probs, count, s);
   if constexpr (LAYOUT != LAYOUT_INF && (wide || (LAYOUT == LAYOUT_WGT && TN == 32)))
-    if (kmax <= 4 * CHUNK_K) return run_chunk<ST, OT, LAYOUT, SPLIT, TM, TN, 8, 2, 4>(probs, count, s);
+    if (kmax <= 4 * CHUNK_K) return run_chunk<ST, OT, LAYOUT, SPLIT, TM, TN, 8, 2, 4, Q8>(probs, count, s);
   if constexpr (TN == 32) {
     long long tiles = 0;
     for (int i = 0; i < count; ++i) tiles += ((probs[i].M + 31LL) / 32) * ((probs[i].N + 31LL) / 32) * probs[i].groups;
-    if (LAYOUT != LAYOUT_INF || tiles > 256) return run_chunk<ST, OT, LAYOUT, SPLIT, TM, TN, 8, 1, 4>(probs, count, s);
+    if (LAYOUT != LAYOUT_INF || tiles > 256) return run_chunk<ST, OT, LAYOUT, SPLIT, TM, TN, 8, 1, 4, Q8>(probs, count, s);
   }
-  return run_chunk<ST, OT, LAYOUT, SPLIT, TM, TN, 8, 1, 2>(probs, count, s);
+  return run_chunk<ST, OT, LAYOUT, SPLIT, TM, TN, 8, 1, 2, Q8>(probs, count, s);
 }
 
-template <typename ST, typename OT, int LAYOUT, int SPLIT>
+template <typename ST, typename OT, int LAYOUT, int SPLIT, bool Q8 = false>
 static hipError_t run_chunks(const GemmProblem* probs, int count, int tile, hipStream_t s) {
   switch (tile) {
-    case TILE_CHUNK_16: return run_chunk<ST, OT, LAYOUT, SPLIT, 16, 16, 16, 1, 4>(probs, count, s);
-    case TILE_CHUNK_32: return run_chunk8<ST, OT, LAYOUT, SPLIT, 32, 32>(probs, count, s);
-    default: return run_chunk8<ST, OT, LAYOUT, SPLIT, 64, 64>(probs, count, s);
+    case TILE_CHUNK_16: return run_chunk<ST, OT, LAYOUT, SPLIT, 16, 16, 16, 1, 4, Q8>(probs, count, s);
+    case TILE_CHUNK_32: return run_chunk8<ST, OT, LAYOUT, SPLIT, 32, 32, Q8>(probs, count, s);
+    default: return run_chunk8<ST, OT, LAYOUT, SPLIT, 64, 64, Q8>(probs, count, s);
   }
 }
 

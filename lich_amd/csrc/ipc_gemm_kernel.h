@@ -18,6 +18,7 @@
 
 #include "ipc_device.h"
 #include "ipc_launch.h"
+#include "ipc_mx_state.h"
 
 namespace ipc {
 
@@ -45,7 +46,7 @@ __device__ __forceinline__ void gload4(const ST* base, long long ld, int r0, int
   }
 }
 
-template <typename ST, typename OT, int LAYOUT, int SPLIT, int BM, int BN, int BK, int WGM, int WGN>
+template <typename ST, typename OT, int LAYOUT, int SPLIT, int BM, int BN, int BK, int WGM, int WGN, bool Q8 = false>
 __global__ void __launch_bounds__(WGM * WGN * 64) gemm_kernel(const GemmBatch batch) {
   constexpr int NT = WGM * WGN * 64;
   constexpr bool A_KMAJ = (LAYOUT != LAYOUT_INF);  // A global layout has k contiguous
@@ -101,7 +102,13 @@ __global__ void __launch_bounds__(WGM * WGN * 64) gemm_kernel(const GemmBatch ba
 #pragma unroll
     for (int v = 0; v < VB; ++v) {
       const int idx = tid + v * NT;
-      if (B_KMAJ) gload4<ST, BK>(Bm, p.ldb, n0, k0, N, K, p.vec_b, idx, rb[v]);
+      if constexpr (Q8 && B_KMAJ) {
+        const int n = n0 + idx / (BK / 4), k = k0 + (idx % (BK / 4)) * 4;
+        rb[v][0] = rb[v][1] = rb[v][2] = rb[v][3] = 0.0f;
+        if (n < N && k < K)
+          mx::state4(reinterpret_cast<const uint8_t*>(p.b), p.ldb, reinterpret_cast<const uint8_t*>(p.aux), p.ldx, n, k,
+                     rb[v]);
+      } else if (B_KMAJ) gload4<ST, BK>(Bm, p.ldb, n0, k0, N, K, p.vec_b, idx, rb[v]);
       else        gload4<ST, BN>(Bm, p.ldb, k0, n0, K, N, p.vec_b, idx, rb[v]);
     }
   };
@@ -239,6 +246,12 @@ __global__ void __launch_bounds__(WGM * WGN * 64) gemm_kernel(const GemmBatch ba
             } else {
               out[o] = cvt<ST>(c);
             }
+          } else if (LAYOUT == LAYOUT_INF && Q8) {
+            float x[4];
+            mx::state4(reinterpret_cast<const uint8_t*>(p.aux), p.ldx, reinterpret_cast<const uint8_t*>(p.out2), p.ld2, m,
+                       n & ~3, x);
+            const float xv = (n & 2) ? ((n & 1) ? x[3] : x[2]) : ((n & 1) ? x[1] : x[0]);
+            out[o] = cvt<ST>(act_df(act_e, xv) * c);
           } else if (LAYOUT == LAYOUT_INF) {
             // tilelang_kernels.py:227-231 / 259-262.
             const float x = to_f32(out[o]);
@@ -258,7 +271,7 @@ __global__ void __launch_bounds__(WGM * WGN * 64) gemm_kernel(const GemmBatch ba
 
 // Launch of one tile configuration over a ragged batch (count <= MAX_BATCH
 // per launch; longer lists are split).
-template <typename ST, typename OT, int LAYOUT, int SPLIT, int BM, int BN, int BK, int WGM, int WGN>
+template <typename ST, typename OT, int LAYOUT, int SPLIT, int BM, int BN, int BK, int WGM, int WGN, bool Q8 = false>
 static hipError_t run_tile(const GemmProblem* probs, int count, hipStream_t s) {
   for (int base = 0; base < count; base += MAX_BATCH) {
     GemmBatch batch;
@@ -272,7 +285,7 @@ static hipError_t run_tile(const GemmProblem* probs, int count, hipStream_t s) {
     }
     for (int i = batch.count; i <= MAX_BATCH; ++i) batch.start[i] = total;
     if (total == 0) continue;
-    hipLaunchKernelGGL((gemm_kernel<ST, OT, LAYOUT, SPLIT, BM, BN, BK, WGM, WGN>), dim3(total),
+    hipLaunchKernelGGL((gemm_kernel<ST, OT, LAYOUT, SPLIT, BM, BN, BK, WGM, WGN, Q8>), dim3(total),
                        dim3(WGM * WGN * 64), 0, s, batch);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
@@ -280,12 +293,12 @@ static hipError_t run_tile(const GemmProblem* probs, int count, hipStream_t s) {
   return hipSuccess;
 }
 
-template <typename ST, typename OT, int LAYOUT, int SPLIT>
+template <typename ST, typename OT, int LAYOUT, int SPLIT, bool Q8 = false>
 static hipError_t run_tiles(const GemmProblem* probs, int count, int tile, hipStream_t s) {
   switch (tile) {
-    case 0: return run_tile<ST, OT, LAYOUT, SPLIT, 32, 32, 32, 1, 1>(probs, count, s);
-    case 1: return run_tile<ST, OT, LAYOUT, SPLIT, 64, 64, 32, 2, 2>(probs, count, s);
-    default: return run_tile<ST, OT, LAYOUT, SPLIT, 128, 128, 32, 2, 2>(probs, count, s);
+    case 0: return run_tile<ST, OT, LAYOUT, SPLIT, 32, 32, 32, 1, 1, Q8>(probs, count, s);
+    case 1: return run_tile<ST, OT, LAYOUT, SPLIT, 64, 64, 32, 2, 2, Q8>(probs, count, s);
+    default: return run_tile<ST, OT, LAYOUT, SPLIT, 128, 128, 32, 2, 2, Q8>(probs, count, s);
   }
 }
 

@@ -15,6 +15,12 @@ enum GemmKind {
 
 enum { DT_F32 = 0, DT_F16 = 1, DT_BF16 = 2 };
 
+// Kernels built for a state kept in 8 bits (microscaled int8, ipc_mx.h; the
+// templates' Q8): KIND_WEIGHT's B is the packed state, ldb its row bytes, aux its
+// scales and ldx its rows; KIND_INFER then writes the state gradient G = f'(X)
+// W_lo^T E_lo: aux is the packed state, ldx its row bytes, out2 its scales and ld2
+// its rows.
+
 // One (possibly grouped) GEMM with fused prologue/epilogue.  Output is M x N,
 // contraction K.  Group g offsets every pointer by g * <its group stride>.
 // All strides are in elements.
@@ -71,6 +77,11 @@ hipError_t launch_chunk_pf(const GemmProblem* probs, int count, int storage, int
                            hipStream_t s);
 hipError_t launch_chunk_inf(const GemmProblem* probs, int count, int storage, int operand, int tile, hipStream_t s);
 hipError_t launch_chunk_wgt(const GemmProblem* probs, int count, int storage, int operand, int tile, hipStream_t s);
+
+// The kernels for a state kept in 8 bits (KIND_WEIGHT, KIND_INFER): the k-chunk
+// kernel's tiles from TILE_CHUNK_16 on, else the tile kernel's.
+hipError_t launch_ckpt_weight(const GemmProblem& p, int storage, int operand, int tile, hipStream_t s);
+hipError_t launch_ckpt_grad(const GemmProblem& p, int storage, int operand, int tile, hipStream_t s);
 
 // Tile geometry per tile id (shared with the host heuristics).
 struct TileShape { int bm, bn, bk, threads; };

@@ -42,7 +42,7 @@ __host__ __device__ inline int mx_groups(int n) { return (int)(((long long)n + M
 hipError_t launch_mx_quantize(const void* x, void* codes, void* scales, int R, int C, int axis, int format,
                               int storage, int act, hipStream_t s);
 hipError_t launch_mx_dequantize(const void* codes, const void* scales, void* out, int R, int C, int format,
-                                int storage, hipStream_t s);
+                                int storage, int act, hipStream_t s);  // f applied
 
 // C[M][N] = sum over k of A4[m][k] B4[n][k], both fp4 with rows of `groups`
 // groups of 128 values, and the epilogue of a kernel family (GemmKind).

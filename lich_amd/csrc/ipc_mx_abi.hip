@@ -88,7 +88,7 @@ int ipc_mx_dequantize(const void* codes, const void* scales, void* out, int R, i
   TRY(check_packed(R, C, format));
   TRY(check_codes(codes, scales, "the packed matrix"));
   TRY(check_ptr(out, "out", elem_size(storage)));
-  return launch_rc(launch_mx_dequantize(codes, scales, out, R, C, format, storage, (hipStream_t)stream),
+  return launch_rc(launch_mx_dequantize(codes, scales, out, R, C, format, storage, IPC_ACT_IDENTITY, (hipStream_t)stream),
                    "ipc_mx_dequantize");
 }
 

@@ -53,10 +53,10 @@ __device__ __forceinline__ unsigned int8_codes4(float a, float b, float c, float
   return q(a) | (q(b) << 8) | (q(c) << 16) | (q(d) << 24);
 }
 
-// Value of int8 code q (sign-extended) in a block with scale byte s.
-__device__ __forceinline__ float int8_value(int q, unsigned s) {
-  const float v = __builtin_ldexpf((float)q, (int)s - 133);
-  return s == 255u ? __builtin_nanf("") : v;
+// 2^(s - 133), the value of code 1 in an int8 block with scale byte s: code times
+// this is exact (NaN for s = 255).
+__device__ __forceinline__ float int8_scale(unsigned s) {
+  return s == 255u ? __builtin_nanf("") : __builtin_ldexpf(1.0f, (int)s - 133);
 }
 __device__ __forceinline__ int sext8(unsigned w, int byte) { return (int)(w << (24 - 8 * byte)) >> 24; }
 

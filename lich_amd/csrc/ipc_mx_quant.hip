@@ -148,11 +148,11 @@ __global__ void __launch_bounds__(256) mx_quant_cols_kernel(const ST* __restrict
   }
 }
 
-// Packed rows back into out [R][C], 8 values a lane as in mx_quant_rows_kernel.
+// f of packed rows into out [R][C], 8 values a lane as in mx_quant_rows_kernel.
 template <typename ST, int FMT>
 __global__ void __launch_bounds__(256) mx_dequant_kernel(const uint8_t* __restrict__ codes,
                                                          const uint8_t* __restrict__ scales, ST* __restrict__ out,
-                                                         int R, int C, int row_bytes, int groups) {
+                                                         int R, int C, int row_bytes, int groups, int act) {
   const int kg = blockIdx.x % groups, r0 = blockIdx.x / groups * TILE_ROWS;
   const int tid = threadIdx.x, sub = tid & 15, c = kg * MX_GROUP + sub * 8;
   if (c >= C) return;
@@ -176,11 +176,13 @@ __global__ void __launch_bounds__(256) mx_dequant_kernel(const uint8_t* __restri
     const int r = r0 + u * 16 + (tid >> 4);
     if (r >= R) continue;
     float v[8];
+    const float unit = mx::int8_scale(s[u]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if constexpr (FMT == MX_FP4) v[i] = mx::fp4_value(q[u].x >> (4 * i) & 15u, s[u]);
-      else v[i] = mx::int8_value(mx::sext8(i < 4 ? q[u].x : q[u].y, i & 3), s[u]);
+      else v[i] = (float)mx::sext8(i < 4 ? q[u].x : q[u].y, i & 3) * unit;
     }
+    activate<8>(act, v);
     ST* p = out + (long long)r * C + c;
     if (c + 8 <= C) {
       mx::store8(p, v);
@@ -210,12 +212,12 @@ hipError_t quantize(const void* x, void* codes, void* scales, int R, int C, int 
 }
 
 template <typename ST, int FMT>
-hipError_t dequantize(const void* codes, const void* scales, void* out, int R, int C, hipStream_t s) {
+hipError_t dequantize(const void* codes, const void* scales, void* out, int R, int C, int act, hipStream_t s) {
   const int groups = mx_groups(C);
   const long long blocks = (long long)groups * ((R + (long long)TILE_ROWS - 1) / TILE_ROWS);
   hipLaunchKernelGGL((mx_dequant_kernel<ST, FMT>), dim3((unsigned)blocks), dim3(256), 0, s,
                      static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), static_cast<ST*>(out), R,
-                     C, (int)mx_row_bytes(FMT, C), groups);
+                     C, (int)mx_row_bytes(FMT, C), groups, act);
   return hipGetLastError();
 }
 
@@ -238,18 +240,18 @@ hipError_t launch_mx_quantize(const void* x, void* codes, void* scales, int R, i
 }
 
 hipError_t launch_mx_dequantize(const void* codes, const void* scales, void* out, int R, int C, int format,
-                                int storage, hipStream_t s) {
+                                int storage, int act, hipStream_t s) {
   const bool four = format == MX_FP4;
   switch (storage) {
     case DT_F32:
-      return four ? dequantize<float, MX_FP4>(codes, scales, out, R, C, s)
-                  : dequantize<float, MX_INT8>(codes, scales, out, R, C, s);
+      return four ? dequantize<float, MX_FP4>(codes, scales, out, R, C, act, s)
+                  : dequantize<float, MX_INT8>(codes, scales, out, R, C, act, s);
     case DT_F16:
-      return four ? dequantize<f16, MX_FP4>(codes, scales, out, R, C, s)
-                  : dequantize<f16, MX_INT8>(codes, scales, out, R, C, s);
+      return four ? dequantize<f16, MX_FP4>(codes, scales, out, R, C, act, s)
+                  : dequantize<f16, MX_INT8>(codes, scales, out, R, C, act, s);
     default:
-      return four ? dequantize<bf16, MX_FP4>(codes, scales, out, R, C, s)
-                  : dequantize<bf16, MX_INT8>(codes, scales, out, R, C, s);
+      return four ? dequantize<bf16, MX_FP4>(codes, scales, out, R, C, act, s)
+                  : dequantize<bf16, MX_INT8>(codes, scales, out, R, C, act, s);
   }
 }
 

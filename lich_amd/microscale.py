@@ -12,6 +12,9 @@ quantiser's ``new_output()`` allocates one.
   ``build_mx_weight_update``: the kernel families of ``lich_amd.kernels`` with
   both operands in fp4.
 * ``build_mx_predict``: fp4 weights, states in their own type, few samples.
+* ``build_checkpoint_save``, ``build_checkpoint_weight_update``,
+  ``build_checkpoint_gradient``: a layer's state kept in int8 and the backward
+  pass that reads it there.
 
 Each builder returns a callable that validates its tensors and enqueues on
 torch's current stream, as in ``lich_amd.kernels``; nothing is allocated or
@@ -25,7 +28,7 @@ from typing import NamedTuple
 import torch
 
 from . import _native as nat
-from .kernels import _check, _storage_dtype
+from .kernels import _check, _Kernel, _storage_dtype
 
 BLOCK, GROUP = 32, 128  # values per scale, per four scale bytes
 
@@ -219,6 +222,57 @@ class MXPredictKernel(_MXProduct):
                                            self.act, nat.current_stream_handle(out.device)))
 
 
+class _CheckpointKernel(_Kernel):
+    """A GEMM that reads a state kept in 8 bits."""
+
+    _phase = -1
+
+    @property
+    def workspace_bytes(self) -> int:
+        return int(nat.lib().ipc_ckpt_workspace_bytes(self._phase, self.act, self.M, self.K, self.B, self.storage))
+
+
+class CheckpointWeightUpdateKernel(_CheckpointKernel):
+    """``k(W[M, K], E[M, B], X8, *, workspace=None)``: ``W += alpha E f(X)^T``, X [K, B] kept
+    in 8 bits.  ``workspace`` (optional, caller-owned, ``new_workspace()``) lets a
+    large 16-bit call evaluate f(X) once."""
+
+    _phase = 2
+
+    def __init__(self, *a, alpha, **kw):
+        super().__init__("weight", *a, **kw)
+        self.alpha = float(alpha)
+        self._x = _Packed("X", self.K, self.B, "int8")
+
+    def __call__(self, w, e, x8, *, workspace=None):
+        _check(w, "W", (self.M, self.K), self.dtype)
+        _check(e, "E", (self.M, self.B), self.dtype)
+        x = self._x(x8)
+        nat.check(nat.lib().ipc_ckpt_weight_update(
+            w.data_ptr(), e.data_ptr(), *x, self.M, self.K, self.B, self.alpha, self.storage, self.operand, self.act,
+            *self._ws(workspace), nat.current_stream_handle(w.device)))
+
+
+class CheckpointGradientKernel(_CheckpointKernel):
+    """``k(W_lower[K, M], E_lower[K, B], X8, G[M, B], *, workspace=None)``:
+    ``G = f'(X) W_lower^T E_lower``, X [M, B] kept in 8 bits."""
+
+    _phase = 1
+
+    def __init__(self, *a, **kw):
+        super().__init__("gradient", *a, **kw)
+        self._x = _Packed("X", self.M, self.B, "int8")
+
+    def __call__(self, w_lower, e_lower, x8, g, *, workspace=None):
+        _check(w_lower, "W_lower", (self.K, self.M), self.dtype)
+        _check(e_lower, "E_lower", (self.K, self.B), self.dtype)
+        x = self._x(x8)
+        _check(g, "G", (self.M, self.B), self.dtype)
+        nat.check(nat.lib().ipc_ckpt_gradient(
+            w_lower.data_ptr(), e_lower.data_ptr(), *x, g.data_ptr(), self.M, self.K, self.B, self.storage,
+            self.operand, self.act, *self._ws(workspace), nat.current_stream_handle(g.device)))
+
+
 @lru_cache(maxsize=256)
 def build_mx_quantize(R: int, C: int, activation: str = "identity", dtype="float32", *, format: str = "fp4",
                       axis: int = 1):
@@ -260,3 +314,21 @@ def build_mx_weight_update(M: int, K: int, B: int, dtype="float32", alpha: float
 def build_mx_predict(M: int, K: int, B: int, activation: str, dtype="float32"):
     """``OUT = W f(X)`` with fp4 weights and states in ``dtype``."""
     return MXPredictKernel(M, K, B, activation, dtype)
+
+
+def build_checkpoint_save(K: int, B: int, dtype="float32", activation: str = "identity"):
+    """X [K, B] (or f(X), for a weight update built with ``identity``) into an 8-bit checkpoint."""
+    return build_mx_quantize(K, B, activation, dtype, format="int8", axis=1)
+
+
+@lru_cache(maxsize=256)
+def build_checkpoint_weight_update(M: int, K: int, B: int, activation: str, dtype="float32", alpha: float = 1e-4, *,
+                                   operand_dtype=None):
+    """``W += alpha * E @ f(X).T`` with X [K, B] kept in 8 bits."""
+    return CheckpointWeightUpdateKernel(M, K, B, activation, dtype, None, operand_dtype, alpha=alpha)
+
+
+@lru_cache(maxsize=256)
+def build_checkpoint_gradient(M: int, K: int, B: int, activation: str, dtype="float32", *, operand_dtype=None):
+    """``G = f'(X) * (W_lower.T @ E_lower)`` with X [M, B] kept in 8 bits."""
+    return CheckpointGradientKernel(M, K, B, activation, dtype, None, operand_dtype)

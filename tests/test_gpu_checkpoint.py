@@ -1,0 +1,195 @@
+"""Backward pass of a state kept in 8 bits, on the GPU, against its definition in
+64 bits and against differences of the forward pass."""
+import pytest
+import torch
+
+import mx_oracle as O
+from lich_amd import _native as nat
+from lich_amd import microscale as mx
+
+pytestmark = pytest.mark.gpu
+DT = O.DT
+ACTS = ["identity", "relu", "tanh", "sigmoid", "silu", "gelu"]
+
+
+def _rand(g, *shape, size=1.0, storage="fp32"):
+    return (torch.randn(shape, generator=g, dtype=torch.float64) * size).to(DT[storage]).double()
+
+
+def _dev(x, storage):
+    return x.to(DT[storage]).cuda()
+
+
+def _close(got, want, tol):
+    d = (got.cpu().double() - want).abs()
+    assert bool((d <= tol).all()), (float((d / tol).max()), int((d > tol).sum()))
+
+
+def _keep(x, storage):
+    save = mx.build_checkpoint_save(*x.shape, DT[storage])
+    x8 = save.new_output()
+    save(_dev(x, storage), x8)
+    return x8, O.quantised(x, "int8")
+
+
+# (storage, operand, unit of the operand's rounding)
+TYPES = [("fp32", "fp32", 0.0), ("fp32", "bf16", 2.0 ** -8), ("fp32", "fp16", 2.0 ** -11), ("fp16", "fp16", 2.0 ** -11),
+         ("bf16", "bf16", 2.0 ** -8)]
+# few tiles, odd lengths, the k-chunk kernel's rows of odd length, the LDS-DMA
+# kernel's 256 x 128 and 256 x 256 tiles with ragged edges, the tile kernel's (fp32 storage)
+SHAPES = [(1, 1, 1), (10, 64, 128), (64, 784, 128), (33, 31, 65), (100, 200, 1), (130, 257, 300), (1000, 1531, 300),
+          (1100, 2050, 192), (4100, 4000, 64)]
+
+
+def _weight(M, K, B, storage, operand, unit, act, lend=False):
+    g = torch.Generator().manual_seed(M + K + B)
+    x = _rand(g, K, B, storage=storage)
+    w, e = _rand(g, M, K, size=0.1, storage=storage), _rand(g, M, B, size=0.1, storage=storage)
+    x8, xq = _keep(x, storage)
+    fx = O.f(act, xq)
+    acc = e @ fx.T
+    wd = _dev(w, storage)
+    k = mx.build_checkpoint_weight_update(M, K, B, act, DT[storage], 0.01, operand_dtype=DT[operand])
+    ws = torch.empty(max(k.workspace_bytes, 16), dtype=torch.uint8, device="cuda") if lend else None
+    k(wd, _dev(e, storage), x8, workspace=ws)
+    alpha = float(torch.tensor(0.01, dtype=torch.float32))
+    size = e.abs() @ fx.abs().T
+    # operands rounded, f in fp32 (4 units and its cancellation, 2^-21), the sum, the epilogue, the result
+    acc_tol = size * (2 * unit + unit * unit + 2.0 ** -21 + (B + 8) * 2.0 ** -23)
+    if operand == "fp16":
+        acc_tol = acc_tol + e.abs().sum(1, keepdim=True) * 2.0 ** -24
+    want = w + alpha * acc
+    tol = alpha * acc_tol + 2.0 ** -22 * (w.abs() + alpha * acc.abs())
+    _close(wd, want, tol + O.UNIT[storage] * 1.01 * (want.abs() + tol) + 2.0 ** -25 * (storage == "fp16") + 2.0 ** -149)
+
+
+def _gradient(M, K, B, storage, operand, unit, act, lend=False):
+    g = torch.Generator().manual_seed(M + K + B + 1)
+    x = _rand(g, M, B, storage=storage)
+    w, e = _rand(g, K, M, size=0.1, storage=storage), _rand(g, K, B, size=0.1, storage=storage)
+    x8, xq = _keep(x, storage)
+    up, d = w.T.contiguous() @ e, O.df(act, xq)
+    out = torch.full((M, B), 7.0, dtype=DT[storage], device="cuda")
+    k = mx.build_checkpoint_gradient(M, K, B, act, DT[storage], operand_dtype=DT[operand])
+    ws = torch.empty(max(k.workspace_bytes, 16), dtype=torch.uint8, device="cuda") if lend else None
+    k(_dev(w, storage), _dev(e, storage), x8, out, workspace=ws)
+    size = w.T.abs().contiguous() @ e.abs()
+    own = unit if storage == "fp32" else 0.0  # 16-bit tensors are operands as they are
+    acc_tol = size * (2 * own + own * own + (K + 8) * 2.0 ** -23)
+    if operand == "fp16":
+        acc_tol = acc_tol + (w.abs().sum(0)[:, None] + e.abs().sum(0)[None]) * 2.0 ** -24
+    want = d * up
+    tol = d.abs() * acc_tol + 2.0 ** -20 * (up.abs() + acc_tol)  # f' in fp32: a few units of 1
+    _close(out, want, tol + O.UNIT[storage] * 1.01 * (want.abs() + tol) + 2.0 ** -25 * (storage == "fp16") + 2.0 ** -149)
+
+
+@pytest.mark.parametrize("storage,operand,unit", TYPES)
+@pytest.mark.parametrize("M,K,B", SHAPES)
+def test_weight_update(M, K, B, storage, operand, unit):
+    _weight(M, K, B, storage, operand, unit, "tanh")
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("storage,operand,unit", TYPES)
+@pytest.mark.parametrize("M,K,B", [(33, 31, 65), (1100, 2050, 192)])
+def test_weight_update_activations(M, K, B, storage, operand, unit, act):
+    _weight(M, K, B, storage, operand, unit, act)
+
+
+@pytest.mark.parametrize("storage,operand,unit", TYPES)
+@pytest.mark.parametrize("M,K,B", SHAPES + [(4100, 64, 4000), (2048, 1088, 1096)])
+def test_gradient(M, K, B, storage, operand, unit):
+    _gradient(M, K, B, storage, operand, unit, "tanh")
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("storage,operand,unit", TYPES)
+@pytest.mark.parametrize("M,K,B", [(33, 31, 65), (2048, 192, 1096), (4104, 64, 4000)])
+def test_gradient_activations(M, K, B, storage, operand, unit, act):
+    _gradient(M, K, B, storage, operand, unit, act)
+
+
+@pytest.mark.parametrize("storage", ["fp16", "bf16"])
+@pytest.mark.parametrize("act", ["identity", "relu", "tanh", "gelu"])
+def test_lent_workspaces(storage, act):
+    """Wherever a call can use one (mode 1), the same results."""
+    lib = nat.lib()
+    unit = O.UNIT[storage]
+    try:
+        assert lib.ipc_set_s16_preactivate(1) == 0
+        for M, K, B in ((33, 31, 65), (1100, 2050, 192), (130, 257, 300)):
+            _weight(M, K, B, storage, storage, unit, act, lend=True)
+        for M, K, B in ((2048, 192, 1096), (4104, 64, 4000)):
+            k = mx.build_checkpoint_gradient(M, K, B, act, DT[storage])
+            assert k.workspace_bytes == 2 * (M * K + K * B)
+            _gradient(M, K, B, storage, storage, unit, act, lend=True)
+    finally:
+        lib.ipc_set_s16_preactivate(-1)
+
+
+@pytest.mark.parametrize("act", ACTS[2:])
+def test_against_differences(act):
+    """L = sum(E * W f(X)): <dL/dX, D> and <dL/dW, D> against central differences
+    in 64 bits, whose truncation is below h^2 times a third derivative of at
+    most 4 and whose rounding is negligible."""
+    M, K, B, h = 40, 70, 50, 1e-4
+    g = torch.Generator().manual_seed(11)
+    x = _rand(g, K, B)
+    w, e = _rand(g, M, K, size=0.2), _rand(g, M, B)
+    x8, xq = _keep(x, "fp32")
+    grad = torch.empty((K, B), device="cuda")
+    mx.build_checkpoint_gradient(K, M, B, act)(_dev(w, "fp32"), _dev(e, "fp32"), x8, grad)
+    dw = torch.zeros((M, K), device="cuda")
+    mx.build_checkpoint_weight_update(M, K, B, act, "float32", 1.0)(dw, _dev(e, "fp32"), x8)
+
+    def loss(wv, xv):
+        return float((e * (wv @ O.f(act, xv))).sum())
+
+    for seed in range(3):
+        dx, dww = _rand(torch.Generator().manual_seed(seed), K, B), _rand(torch.Generator().manual_seed(seed), M, K)
+        up = (w.T.abs().contiguous() @ e.abs())
+        fd = (loss(w, xq + h * dx) - loss(w, xq - h * dx)) / (2 * h)
+        tol = float((up * (dx.abs() ** 3 * 4 * h * h + dx.abs() * (M + 16) * 2.0 ** -21)).sum()) + 1e-6
+        assert abs(float((grad.cpu().double() * dx).sum()) - fd) <= tol
+        fd = (loss(w + h * dww, xq) - loss(w - h * dww, xq)) / (2 * h)  # linear in W
+        tol = float(((e.abs() @ O.f(act, xq).abs().T) * dww.abs()).sum()) * (B + 16) * 2.0 ** -21 + 1e-6
+        assert abs(float((dw.cpu().double() * dww).sum()) - fd) <= tol
+
+
+def test_a_lost_block_is_seen():
+    """An infinity in a kept state reads back as NaN: its weight column and its own
+    gradients are NaN, the others are not."""
+    K, M, B = 70, 40, 64
+    g = torch.Generator().manual_seed(2)
+    x = _rand(g, K, B)
+    x[5, 40] = float("inf")
+    w, e = _rand(g, M, K), _rand(g, M, B)
+    x8, _ = _keep(x, "fp32")
+    wd, grad = _dev(w, "fp32"), torch.empty((K, B), device="cuda")
+    mx.build_checkpoint_gradient(K, M, B, "tanh")(wd, _dev(e, "fp32"), x8, grad)
+    mx.build_checkpoint_weight_update(M, K, B, "tanh")(wd, _dev(e, "fp32"), x8)
+    want = torch.zeros((K, B), dtype=torch.bool)
+    want[5, 32:] = True
+    assert torch.equal(torch.isnan(grad).cpu(), want)
+    assert bool(torch.isnan(wd[:, 5]).all()) and not bool(torch.isnan(wd[:, :5]).any())
+    assert not bool(torch.isnan(wd[:, 6:]).any())
+
+
+def test_refusals():
+    update = mx.build_checkpoint_weight_update(16, 32, 64, "relu", torch.bfloat16)
+    gradient = mx.build_checkpoint_gradient(32, 16, 64, "relu", torch.bfloat16)
+    w, e = (torch.zeros(s, device="cuda", dtype=torch.bfloat16) for s in ((16, 32), (16, 64)))
+    x8, g = mx.new_packed(32, 64, "int8"), torch.empty(32, 64, device="cuda", dtype=torch.bfloat16)
+    four = mx.new_packed(32, 64, "fp4")
+    for bad in ((w.float(), e, x8), (w, e.T, x8), (w, e, four), (w, e, mx.MXMatrix(x8.codes, x8.scales[:, :-1].contiguous())),
+                (w, e, g)):
+        with pytest.raises(ValueError):
+            update(*bad)
+        with pytest.raises(ValueError):
+            gradient(*bad, g)
+    with pytest.raises(ValueError):
+        gradient(w, e, x8, g.float())
+    with pytest.raises(ValueError):
+        mx.build_checkpoint_weight_update(16, 32, 64, "relu", torch.bfloat16, operand_dtype=torch.float32)
+    with pytest.raises(ValueError, match="workspace"):
+        update(w, e, x8, workspace=torch.empty(64))

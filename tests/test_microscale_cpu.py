@@ -1,0 +1,104 @@
+"""Host side of the microscaled operators: sizes, refusals and the oracle (no GPU)."""
+import pytest
+import torch
+
+import mx_oracle as O
+from lich_amd import _native as nat
+from lich_amd import microscale as mx
+
+P = 4096  # a fake, aligned, non-null address; never dereferenced (validation fails first)
+
+
+@pytest.mark.parametrize("rows,n", [(1, 1), (3, 32), (5, 33), (64, 128), (10, 784), (7, 1531)])
+@pytest.mark.parametrize("fmt", ["fp4", "int8"])
+def test_sizes_agree_with_the_library(rows, n, fmt):
+    codes, scales = mx.packed_shapes(rows, n, fmt)
+    lib = nat.lib()
+    assert codes[0] * codes[1] == lib.ipc_mx_code_bytes(rows, n, nat.MX_FORMATS[fmt])
+    assert scales[0] * scales[1] * scales[2] == lib.ipc_mx_scale_bytes(rows, n)
+    got = O.pack(torch.randn(rows, n, dtype=torch.float64), fmt)
+    assert tuple(got[0].shape) == codes and tuple(got[1].shape) == scales
+    packed = mx.new_packed(rows, n, fmt, "cpu")
+    assert packed.codes.dtype == got[0].dtype and packed.scales.dtype == got[1].dtype
+
+
+def test_sizes_that_are_refused():
+    lib = nat.lib()
+    assert lib.ipc_mx_code_bytes(0, 5, 0) == 0 and lib.ipc_mx_code_bytes(5, 5, 2) == 0
+    assert lib.ipc_mx_code_bytes(1 << 24, 1, 0) == 0 and lib.ipc_mx_scale_bytes(1 << 24, 1) == 0  # padded: 2^31 values
+
+
+@pytest.mark.parametrize("args,code,needle", [
+    ((None, P, P, 64, 64, 1, 0, 0, 0, None), nat.ERR_NULL, "x"),
+    ((P, None, P, 64, 64, 1, 0, 0, 0, None), nat.ERR_NULL, "packed"),
+    ((P, P + 8, P, 64, 64, 1, 0, 0, 0, None), nat.ERR_ALIGN, "aligned"),
+    ((P, P, P + 2, 64, 64, 1, 0, 0, 0, None), nat.ERR_ALIGN, "aligned"),
+    ((P + 1, P, P, 64, 64, 1, 0, 1, 0, None), nat.ERR_ALIGN, "aligned"),
+    ((P, P, P, 0, 64, 1, 0, 0, 0, None), nat.ERR_SHAPE, "dimensions"),
+    ((P, P, P, 1 << 20, 4096, 1, 0, 0, 0, None), nat.ERR_SHAPE, "too large"),
+    ((P, P, P, 1, 1 << 24, 0, 0, 0, 0, None), nat.ERR_SHAPE, "too large"),
+    ((P, P, P, 64, 64, 2, 0, 0, 0, None), nat.ERR_CONFIG, "axis"),
+    ((P, P, P, 64, 64, 1, 2, 0, 0, None), nat.ERR_DTYPE, "format"),
+    ((P, P, P, 64, 64, 1, 0, 3, 0, None), nat.ERR_DTYPE, "storage"),
+    ((P, P, P, 64, 64, 1, 0, 0, 6, None), nat.ERR_ACT, "activation"),
+])
+def test_quantize_validation(args, code, needle):
+    assert nat.lib().ipc_mx_quantize(*args) == code
+    assert needle in nat.last_error()
+
+
+def test_other_entry_points_validate():
+    lib = nat.lib()
+    assert lib.ipc_mx_dequantize(P, P, None, 64, 64, 0, 0, None) == nat.ERR_NULL
+    assert lib.ipc_mx_dequantize(P, None, P, 64, 64, 0, 0, None) == nat.ERR_NULL
+    assert lib.ipc_mx_forward(P, P, P, P, None, 64, 64, 64, 0, None) == nat.ERR_NULL
+    assert lib.ipc_mx_forward(P, P, P + 4, P, P, 64, 64, 64, 0, None) == nat.ERR_ALIGN
+    assert lib.ipc_mx_forward(P, P, P, P, P, 64, -1, 64, 0, None) == nat.ERR_SHAPE
+    assert lib.ipc_mx_pred_err(P, P, P, P, None, P, 64, 64, 64, 0, None) == nat.ERR_NULL
+    assert "x_lower" in nat.last_error()
+    assert lib.ipc_mx_infer_update(P, P, P, P, P, None, 64, 64, 64, 0.5, 0, 1, None) == nat.ERR_NULL
+    assert lib.ipc_mx_infer_update(P, P, P, P, P, P, 64, 64, 64, 0.5, 0, 9, None) == nat.ERR_ACT
+    assert lib.ipc_mx_weight_update(P, P, P, P, P, 64, 1 << 20, 1 << 20, 1e-4, 0, None) == nat.ERR_SHAPE
+    assert lib.ipc_mx_predict(P, P, P, P, 1, 1, (1 << 20) + 1, 0, 0, None) == nat.ERR_SHAPE
+    assert lib.ipc_mx_predict(P, P, P, P + 1, 1, 1, 1, 1, 0, None) == nat.ERR_ALIGN
+    assert lib.ipc_ckpt_weight_update(P, P, None, P, 64, 64, 64, 1e-4, 0, 0, 1, None, 0, None) == nat.ERR_NULL
+    assert lib.ipc_ckpt_weight_update(P, P, P, P, 64, 64, 64, 1e-4, 1, 2, 1, None, 0, None) == nat.ERR_DTYPE
+    assert lib.ipc_ckpt_weight_update(P, P, P, P, 64, 64, 64, 1e-4, 0, 0, 1, P + 8, 64, None) == nat.ERR_ALIGN
+    assert lib.ipc_ckpt_weight_update(P, P, P, P, 64, 64, 64, 1e-4, 0, 0, 1, P, -1, None) == nat.ERR_SHAPE
+    assert lib.ipc_ckpt_gradient(P, P, P + 4, P, P, 64, 64, 64, 0, 0, 1, None, 0, None) == nat.ERR_ALIGN
+    assert lib.ipc_ckpt_gradient(P, P, P, P, None, 64, 64, 64, 0, 0, 1, None, 0, None) == nat.ERR_NULL
+    assert lib.ipc_ckpt_gradient(P, P, P, P, P, 1 << 24, 64, 1, 0, 0, 1, None, 0, None) == nat.ERR_SHAPE
+
+
+def test_builders_refuse():
+    with pytest.raises(ValueError):
+        mx.build_mx_quantize(4, 4, "relu", torch.float64)
+    with pytest.raises(ValueError):
+        mx.build_mx_quantize(4, 4, "relu", torch.float32, format="fp8")
+    with pytest.raises(ValueError):
+        mx.build_mx_quantize(4, 4, "softmax", torch.float32)
+    with pytest.raises(ValueError):
+        mx.build_mx_quantize(4, 0, "relu", torch.float32)
+    with pytest.raises(ValueError):
+        mx.build_mx_quantize(4, 4, "relu", torch.float32, axis=2)
+    with pytest.raises(ValueError):
+        mx.build_mx_forward(4, 4, -1)
+    k = mx.build_mx_predict(4, 4, 1, "relu")
+    with pytest.raises(ValueError, match="device"):
+        k(torch.zeros(4, 1), mx.new_packed(4, 4, device="cpu"), torch.zeros(4, 1))
+
+
+@pytest.mark.parametrize("fmt", ["fp4", "int8"])
+def test_the_oracle_rounds_to_nearest(fmt):
+    """No representable value of the block's scale is nearer."""
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(50, 64, generator=g, dtype=torch.float64) * 2.0 ** torch.randint(-20, 20, (50, 1), generator=g).double()
+    code, byte = O.quantise(x, fmt)
+    got = O.values(code, byte, 64, fmt)
+    scale = (2.0 ** (byte[:, :2].double() - 127)).repeat_interleave(32, 1)
+    grid = torch.cat([O.GRID, -O.GRID]) if fmt == "fp4" else torch.arange(-127, 128).double() / 64
+    best = (x[..., None] - grid * scale[..., None]).abs().amin(-1)
+    assert torch.equal((x - got).abs(), best)
+    # ... and no block could have had a smaller scale without saturating past half a step
+    top = x.view(50, 2, 32).abs().amax(-1) / 2.0 ** (byte[:, :2].double() - 127)
+    assert bool((top < (7 if fmt == "fp4" else 255 / 128)).all()) and bool((top >= (3.5 if fmt == "fp4" else 255 / 256)).all())
