@@ -27,17 +27,20 @@ __device__ __forceinline__ unsigned scale_byte(unsigned amax) {
 
 __device__ __forceinline__ unsigned abs_bits(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
 
-// 8 values of a block with scale byte s as a dword of E2M1 codes.  The
+// N (4 or 8) values of a block with scale byte s as E2M1 codes, 4 bits each.  The
 // conversion divides by the scale, rounds to nearest even and saturates at 6,
 // which only values the rule above lets through (6 .. 7, next to the largest float
 // 6 .. 8) reach.
-__device__ __forceinline__ unsigned fp4_codes8(const float (&v)[8], unsigned s) {
+template <int N>
+__device__ __forceinline__ unsigned fp4_codes(const float (&v)[N], unsigned s) {
   const float scale = __builtin_bit_cast(float, (s == 255u ? 0u : s) << 23);
   unsigned o = 0;
   o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, v[0], v[1], scale, 0);
   o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, v[2], v[3], scale, 1);
-  o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, v[4], v[5], scale, 2);
-  o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, v[6], v[7], scale, 3);
+  if constexpr (N == 8) {
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, v[4], v[5], scale, 2);
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, v[6], v[7], scale, 3);
+  }
   return s == 0u || s == 255u ? 0u : o;  // (a zero scale divides by nothing: all codes are 0)
 }
 
@@ -60,43 +63,42 @@ __device__ __forceinline__ float int8_scale(unsigned s) {
 }
 __device__ __forceinline__ int sext8(unsigned w, int byte) { return (int)(w << (24 - 8 * byte)) >> 24; }
 
-// Value of the E2M1 code c in a block with scale byte s: |c| below 2 is c / 2,
-// above 1 + m / 2 times 2^(e - 1); built as an integer number of halves.
-__device__ __forceinline__ float fp4_value(unsigned c, unsigned s) {
-  const unsigned e = (c >> 1) & 3u, m = c & 1u;
-  const unsigned halves = e == 0u ? m : (2u + m) << (e - 1u);
-  const float v = __builtin_ldexpf((float)halves, (int)s - 128);
-  const float r = s == 255u ? __builtin_nanf("") : v;
-  return c & 8u ? -r : r;
+// N (4 or 8) values of E2M1 codes in a block with scale byte s.
+template <int N>
+__device__ __forceinline__ void fp4_values(unsigned q, unsigned s, float (&o)[N]) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const float scale = __builtin_bit_cast(float, s << 23);
+  const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, scale, 1);
+  o[0] = a[0]; o[1] = a[1]; o[2] = b[0]; o[3] = b[1];
+  if constexpr (N == 8) {
+    const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, scale, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, scale, 3);
+    o[4] = c[0]; o[5] = c[1]; o[6] = d[0]; o[7] = d[1];
+  }
+  if (s == 255u) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = __builtin_nanf("");
+  }
 }
 
-// N consecutive elements at any element-aligned address (gfx950 global loads
-// and stores take any alignment): 16 bytes at a time.
+// N consecutive elements (16 bytes) at any element-aligned address: gfx950's
+// global loads and stores take any alignment.
 template <typename ST, int N>
 struct Run {
   typedef ST V __attribute__((ext_vector_type(N)));
   struct __attribute__((packed, aligned(sizeof(ST)))) U { V v; };
 };
-template <typename ST>
-__device__ __forceinline__ void load8(const ST* p, float (&o)[8]) {
-  constexpr int N = 16 / sizeof(ST);
+template <typename ST, int N>
+__device__ __forceinline__ void load_run(const ST* p, float (&o)[N]) {
+  const typename Run<ST, N>::V v = reinterpret_cast<const typename Run<ST, N>::U*>(p)->v;
 #pragma unroll
-  for (int h = 0; h < 8; h += N) {
-    const typename Run<ST, N>::V v = reinterpret_cast<const typename Run<ST, N>::U*>(p + h)->v;
-#pragma unroll
-    for (int i = 0; i < N; ++i) o[h + i] = to_f32(v[i]);
-  }
+  for (int i = 0; i < N; ++i) o[i] = to_f32(v[i]);
 }
-template <typename ST>
-__device__ __forceinline__ void store8(ST* p, const float (&o)[8]) {
-  constexpr int N = 16 / sizeof(ST);
+template <typename ST, int N>
+__device__ __forceinline__ void store_run(ST* p, const float (&o)[N]) {
+  typename Run<ST, N>::V v;
 #pragma unroll
-  for (int h = 0; h < 8; h += N) {
-    typename Run<ST, N>::V v;
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = cvt<ST>(o[h + i]);
-    reinterpret_cast<typename Run<ST, N>::U*>(p + h)->v = v;
-  }
+  for (int i = 0; i < N; ++i) v[i] = cvt<ST>(o[i]);
+  reinterpret_cast<typename Run<ST, N>::U*>(p)->v = v;
 }
 
 }  // namespace mx

@@ -8,84 +8,97 @@
 namespace ipc {
 namespace {
 
-constexpr int TILE_ROWS = 64;  // packed rows a workgroup of the row kernels takes, 128 values of each
+// The row kernels: a workgroup takes 256 values (two groups, so that the fp4
+// codes it stores are whole 128-byte lines) of a few rows, a lane EPL consecutive
+// ones (16 bytes), in 4 passes whose loads are issued together.
+constexpr int WIDTH = 2 * MX_GROUP, PASSES = 4;
+template <typename ST> constexpr int EPL = 16 / (int)sizeof(ST);           // values per lane
+template <typename ST> constexpr int ROW_LANES = WIDTH / EPL<ST>;          // lanes per row
+template <typename ST> constexpr int PASS_ROWS = 256 / ROW_LANES<ST>;      // rows per pass
+template <typename ST> constexpr int TILE_ROWS = PASSES * PASS_ROWS<ST>;   // rows per workgroup
 
-// Packed rows are the rows of x.  16 lanes take the 128 values of a row, 8 each
-// (16-byte loads), 4 lanes a block: its largest magnitude comes from two
-// exchanges within a quad.  The workgroup's 64 rows go through in 4 passes
-// whose loads are issued together.
+// Packed rows are the rows of x.  A block's lanes (4, or 8 of fp32) sit side by
+// side: its largest magnitude comes from exchanges within them.
 template <typename ST, int FMT>
 __global__ void __launch_bounds__(256) mx_quant_rows_kernel(const ST* __restrict__ x, uint8_t* __restrict__ codes,
                                                             uint8_t* __restrict__ scales, int R, int C,
-                                                            int row_bytes, int groups, int act) {
-  const int kg = blockIdx.x % groups, r0 = blockIdx.x / groups * TILE_ROWS;
-  const int tid = threadIdx.x, sub = tid & 15, c = kg * MX_GROUP + sub * 8;
-  constexpr int PASSES = TILE_ROWS / 16;
-  float v[PASSES][8];
+                                                            int row_bytes, int spans, int act) {
+  constexpr int E = EPL<ST>;
+  const int c = blockIdx.x % spans * WIDTH + threadIdx.x % ROW_LANES<ST> * E;
+  const int r0 = blockIdx.x / spans * TILE_ROWS<ST> + threadIdx.x / ROW_LANES<ST>;
+  const int groups = mx_groups(C), kg = c / MX_GROUP;
+  float v[PASSES][E];
 #pragma unroll
   for (int u = 0; u < PASSES; ++u) {
-    const int r = r0 + u * 16 + (tid >> 4);
+    const int r = r0 + u * PASS_ROWS<ST>;
     const ST* p = x + (long long)r * C + c;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[u][i] = 0.0f;
-    if (r < R && c + 8 <= C) {
-      mx::load8(p, v[u]);
+    for (int i = 0; i < E; ++i) v[u][i] = 0.0f;
+    if (r < R && c + E <= C) {
+      mx::load_run<ST, E>(p, v[u]);
     } else if (r < R) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < E; ++i)
         if (c + i < C) v[u][i] = to_f32(p[i]);
     }
   }
 #pragma unroll
   for (int u = 0; u < PASSES; ++u) {
-    const int r = r0 + u * 16 + (tid >> 4);
-    activate<8>(act, v[u]);
+    const int r = r0 + u * PASS_ROWS<ST>;
+    activate<E>(act, v[u]);
+    if (c + E > C) {  // (f(0) need not be 0: padding stays zero)
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (c + i >= C) v[u][i] = 0.0f;
+    }
     unsigned m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (c + i >= C) v[u][i] = 0.0f;  // (f(0) need not be 0: padding stays zero)
-      m = max(m, mx::abs_bits(v[u][i]));
-    }
-    m = max(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xf, 0xf, true));  // quad lanes 1 0 3 2
-    m = max(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0x4E, 0xf, 0xf, true));  // quad lanes 2 3 0 1
-    if (r >= R) continue;
+    for (int i = 0; i < E; ++i) m = max(m, mx::abs_bits(v[u][i]));
+    m = max(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xf, 0xf, true));   // quad lanes 1 0 3 2
+    m = max(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0x4E, 0xf, 0xf, true));   // quad lanes 2 3 0 1
+    if (E == 4) m = max(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0x141, 0xf, 0xf, true));  // lanes 7 .. 0 of 8
+    if (r >= R || kg >= groups) continue;
     const unsigned s = mx::scale_byte<FMT>(m);
     uint8_t* row = codes + (long long)r * row_bytes;
     if constexpr (FMT == MX_FP4) {
-      *reinterpret_cast<unsigned*>(row + c / 2) = mx::fp4_codes8(v[u], s);
+      if constexpr (E == 8) *reinterpret_cast<unsigned*>(row + c / 2) = mx::fp4_codes<8>(v[u], s);
+      else *reinterpret_cast<unsigned short*>(row + c / 2) = (unsigned short)mx::fp4_codes<4>(v[u], s);
     } else if (c < row_bytes) {
-      uint2 q;
-      q.x = mx::int8_codes4(v[u][0], v[u][1], v[u][2], v[u][3], s);
-      q.y = mx::int8_codes4(v[u][4], v[u][5], v[u][6], v[u][7], s);
-      *reinterpret_cast<uint2*>(row + c) = q;
+      unsigned q[E / 4];
+#pragma unroll
+      for (int h = 0; h < E / 4; ++h)
+        q[h] = mx::int8_codes4(v[u][4 * h], v[u][4 * h + 1], v[u][4 * h + 2], v[u][4 * h + 3], s);
+      if constexpr (E == 8) *reinterpret_cast<uint2*>(row + c) = make_uint2(q[0], q[1]);
+      else *reinterpret_cast<unsigned*>(row + c) = q[0];
     }
-    if ((sub & 3) == 0) scales[((long long)kg * R + r) * 4 + (sub >> 2)] = (uint8_t)s;
+    if (c % MX_BLOCK == 0) scales[((long long)kg * R + r) * 4 + (c / MX_BLOCK & 3)] = (uint8_t)s;
   }
 }
 
-// Packed rows are the columns of x [K][N].  A workgroup stages 128 k-rows of 64
-// dwords (64 fp32 or 128 16-bit columns) in LDS with 16-byte loads; then each
-// thread owns a dword column and one of the four blocks: its 32 values are in
-// its registers, so the block's scale needs no exchange, and its codes are 16
-// (fp4) or 32 bytes of a packed row, the four blocks of a row side by side.
-// Dword w of k-row k lies at w + 16 * (k / 32) (mod 64): a wave reads 16 dwords
-// of each of the 4 blocks from 64 different banks.
+// Packed rows are the columns of x [K][N].  A workgroup stages 256 k-rows of 32
+// dwords (128 bytes of a row: 32 fp32 or 64 16-bit columns) in LDS with 16-byte
+// loads; then each thread owns a dword column and one of the eight blocks: its
+// 32 values are in its registers, so the block's scale needs no exchange, and its
+// codes are 16 (fp4) or 32 bytes of a packed row, the eight blocks of a row side
+// by side.  Dword w of k-row k (block b = k / 32) lies in row k ^ (b & 1) at w + 8 (b
+// / 2) (mod 32): a wave reads 8 dwords of each of the 8 blocks from 64 different
+// banks.
 template <typename ST, int FMT>
 __global__ void __launch_bounds__(256) mx_quant_cols_kernel(const ST* __restrict__ x, uint8_t* __restrict__ codes,
                                                             uint8_t* __restrict__ scales, int K, int N,
-                                                            int row_bytes, int groups, int act) {
+                                                            int row_bytes, int spans, int act) {
   constexpr int VPD = 4 / sizeof(ST);  // columns per dword
-  constexpr int COLS = 64 * VPD, VEC = 16 / sizeof(ST);
-  __shared__ __align__(16) unsigned tile[MX_GROUP * 64];
-  const int kg = blockIdx.x % groups, n0 = blockIdx.x / groups * COLS, k0 = kg * MX_GROUP;
+  constexpr int COLS = 32 * VPD, VEC = 16 / sizeof(ST);
+  __shared__ __align__(16) unsigned tile[WIDTH * 32];
+  const int n0 = blockIdx.x / spans * COLS, k0 = blockIdx.x % spans * WIDTH;
   const int tid = threadIdx.x;
   {
     typedef typename mx::Run<ST, VEC>::V V;
-    const int j = tid & 15, n = n0 + j * VEC;
+    const int j = tid & 7, n = n0 + j * VEC;
     V v[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      const int k = k0 + u * 16 + (tid >> 4);
+      const int k = k0 + u * 32 + (tid >> 3);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) v[u][i] = (ST)0.0f;
       const ST* p = x + (long long)k * N + n;
@@ -98,17 +111,19 @@ __global__ void __launch_bounds__(256) mx_quant_cols_kernel(const ST* __restrict
       }
     }
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int k = u * 16 + (tid >> 4);
-      *reinterpret_cast<V*>(&tile[k * 64 + ((j * 4 + 16 * (k >> 5)) & 63)]) = v[u];
-    }
+    for (int u = 0; u < 8; ++u)
+      *reinterpret_cast<V*>(&tile[((u * 32 + (tid >> 3)) ^ (u & 1)) * 32 + ((j * 4 + 8 * (u >> 1)) & 31)]) = v[u];
   }
   __syncthreads();
-  const int w = tid >> 2, blk = tid & 3;
-  unsigned d[32];
-#pragma unroll
-  for (int i = 0; i < 32; ++i) d[i] = tile[(blk * 32 + i) * 64 + ((w + 16 * blk) & 63)];
+  const int w = tid >> 3, blk = tid & 7;
   const int left = K - k0 - blk * 32;  // values of this block
+  if (k0 + (blk & 4) * 32 >= K) return;  // a group past the end
+  unsigned d[32];
+  const unsigned* at = &tile[blk * 32 * 32 + ((w + 8 * (blk >> 1)) & 31)];
+  const unsigned *even = at + (blk & 1) * 32, *odd = at - (blk & 1) * 32;  // rows i and i ^ 1
+#pragma unroll
+  for (int i = 0; i < 32; ++i) d[i] = (i & 1 ? odd : even)[i * 32];
+  const int kg = (k0 + blk * 32) / MX_GROUP;
 #pragma unroll
   for (int c = 0; c < VPD; ++c) {
     const int n = n0 + w * VPD + c;
@@ -120,23 +135,22 @@ __global__ void __launch_bounds__(256) mx_quant_cols_kernel(const ST* __restrict
       else v[i] = h2f(c == 0 ? d[i] & 0xffffu : d[i] >> 16, (ST*)nullptr);
     }
     activate<32>(act, v);
+    if (left < 32) {  // (f(0) need not be 0: padding stays zero)
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i >= left) v[i] = 0.0f;
+    }
     unsigned m = 0;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      if (i >= left) v[i] = 0.0f;
-      m = max(m, mx::abs_bits(v[i]));
-    }
+    for (int i = 0; i < 32; ++i) m = max(m, mx::abs_bits(v[i]));
     const unsigned s = mx::scale_byte<FMT>(m);
-    scales[((long long)kg * N + n) * 4 + blk] = (uint8_t)s;
+    scales[((long long)kg * N + n) * 4 + (blk & 3)] = (uint8_t)s;
     uint8_t* row = codes + (long long)n * row_bytes;
     if constexpr (FMT == MX_FP4) {
       unsigned q[4];
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const float (&t)[8] = *reinterpret_cast<const float (*)[8]>(&v[h * 8]);
-        q[h] = mx::fp4_codes8(t, s);
-      }
-      *reinterpret_cast<uint4*>(row + kg * 64 + blk * 16) = make_uint4(q[0], q[1], q[2], q[3]);
+      for (int h = 0; h < 4; ++h) q[h] = mx::fp4_codes<8>(*reinterpret_cast<const float (*)[8]>(&v[h * 8]), s);
+      *reinterpret_cast<uint4*>(row + (k0 + blk * 32) / 2) = make_uint4(q[0], q[1], q[2], q[3]);
     } else if (k0 + blk * 32 < row_bytes) {
       unsigned q[8];
 #pragma unroll
@@ -148,47 +162,54 @@ __global__ void __launch_bounds__(256) mx_quant_cols_kernel(const ST* __restrict
   }
 }
 
-// f of packed rows into out [R][C], 8 values a lane as in mx_quant_rows_kernel.
+// f of packed rows into out [R][C], lanes and passes as in mx_quant_rows_kernel.
 template <typename ST, int FMT>
 __global__ void __launch_bounds__(256) mx_dequant_kernel(const uint8_t* __restrict__ codes,
                                                          const uint8_t* __restrict__ scales, ST* __restrict__ out,
-                                                         int R, int C, int row_bytes, int groups, int act) {
-  const int kg = blockIdx.x % groups, r0 = blockIdx.x / groups * TILE_ROWS;
-  const int tid = threadIdx.x, sub = tid & 15, c = kg * MX_GROUP + sub * 8;
+                                                         int R, int C, int row_bytes, int spans, int act) {
+  constexpr int E = EPL<ST>;
+  const int c = blockIdx.x % spans * WIDTH + threadIdx.x % ROW_LANES<ST> * E;
+  const int r0 = blockIdx.x / spans * TILE_ROWS<ST> + threadIdx.x / ROW_LANES<ST>;
   if (c >= C) return;
-  constexpr int PASSES = TILE_ROWS / 16;
-  uint2 q[PASSES];
-  unsigned s[PASSES];
+  unsigned q[PASSES][2], s[PASSES];
 #pragma unroll
   for (int u = 0; u < PASSES; ++u) {
-    const int r = r0 + u * 16 + (tid >> 4);
-    q[u] = make_uint2(0, 0);
-    s[u] = 0;
+    const int r = r0 + u * PASS_ROWS<ST>;
+    q[u][0] = q[u][1] = s[u] = 0;
     if (r < R) {
       const uint8_t* row = codes + (long long)r * row_bytes;
-      if constexpr (FMT == MX_FP4) q[u].x = *reinterpret_cast<const unsigned*>(row + c / 2);
-      else q[u] = *reinterpret_cast<const uint2*>(row + c);
-      s[u] = scales[((long long)kg * R + r) * 4 + (sub >> 2)];
+      if constexpr (FMT == MX_FP4 && E == 8) {
+        q[u][0] = *reinterpret_cast<const unsigned*>(row + c / 2);
+      } else if constexpr (FMT == MX_FP4) {
+        q[u][0] = *reinterpret_cast<const unsigned short*>(row + c / 2);
+      } else if constexpr (E == 8) {
+        const uint2 t = *reinterpret_cast<const uint2*>(row + c);
+        q[u][0] = t.x; q[u][1] = t.y;
+      } else {
+        q[u][0] = *reinterpret_cast<const unsigned*>(row + c);
+      }
+      s[u] = scales[((long long)(c / MX_GROUP) * R + r) * 4 + (c / MX_BLOCK & 3)];
     }
   }
 #pragma unroll
   for (int u = 0; u < PASSES; ++u) {
-    const int r = r0 + u * 16 + (tid >> 4);
+    const int r = r0 + u * PASS_ROWS<ST>;
     if (r >= R) continue;
-    float v[8];
-    const float unit = mx::int8_scale(s[u]);
+    float v[E];
+    if constexpr (FMT == MX_FP4) {
+      mx::fp4_values<E>(q[u][0], s[u], v);
+    } else {
+      const float unit = mx::int8_scale(s[u]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (FMT == MX_FP4) v[i] = mx::fp4_value(q[u].x >> (4 * i) & 15u, s[u]);
-      else v[i] = (float)mx::sext8(i < 4 ? q[u].x : q[u].y, i & 3) * unit;
+      for (int i = 0; i < E; ++i) v[i] = (float)mx::sext8(q[u][i / 4], i & 3) * unit;
     }
-    activate<8>(act, v);
+    activate<E>(act, v);
     ST* p = out + (long long)r * C + c;
-    if (c + 8 <= C) {
-      mx::store8(p, v);
+    if (c + E <= C) {
+      mx::store_run<ST, E>(p, v);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < E; ++i)
         if (c + i < C) p[i] = cvt<ST>(v[i]);
     }
   }
@@ -197,27 +218,22 @@ __global__ void __launch_bounds__(256) mx_dequant_kernel(const uint8_t* __restri
 template <typename ST, int FMT>
 hipError_t quantize(const void* x, void* codes, void* scales, int R, int C, int axis, int act, hipStream_t s) {
   const int rows = axis == 1 ? R : C, n = axis == 1 ? C : R;
-  const int groups = mx_groups(n), per = axis == 1 ? TILE_ROWS : 256 / (int)sizeof(ST);
-  const long long blocks = (long long)groups * ((rows + (long long)per - 1) / per);
+  const int spans = (mx_groups(n) + 1) / 2, per = axis == 1 ? TILE_ROWS<ST> : 128 / (int)sizeof(ST);
+  const long long blocks = (long long)spans * ((rows + (long long)per - 1) / per);
   const int row_bytes = (int)mx_row_bytes(FMT, n);
-  if (axis == 1)
-    hipLaunchKernelGGL((mx_quant_rows_kernel<ST, FMT>), dim3((unsigned)blocks), dim3(256), 0, s,
-                       static_cast<const ST*>(x), static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), R, C,
-                       row_bytes, groups, act);
-  else
-    hipLaunchKernelGGL((mx_quant_cols_kernel<ST, FMT>), dim3((unsigned)blocks), dim3(256), 0, s,
-                       static_cast<const ST*>(x), static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), R, C,
-                       row_bytes, groups, act);
+  hipLaunchKernelGGL((axis == 1 ? mx_quant_rows_kernel<ST, FMT> : mx_quant_cols_kernel<ST, FMT>),
+                     dim3((unsigned)blocks), dim3(256), 0, s, static_cast<const ST*>(x), static_cast<uint8_t*>(codes),
+                     static_cast<uint8_t*>(scales), R, C, row_bytes, spans, act);
   return hipGetLastError();
 }
 
 template <typename ST, int FMT>
 hipError_t dequantize(const void* codes, const void* scales, void* out, int R, int C, int act, hipStream_t s) {
-  const int groups = mx_groups(C);
-  const long long blocks = (long long)groups * ((R + (long long)TILE_ROWS - 1) / TILE_ROWS);
+  const int spans = (mx_groups(C) + 1) / 2;
+  const long long blocks = (long long)spans * ((R + (long long)TILE_ROWS<ST> - 1) / TILE_ROWS<ST>);
   hipLaunchKernelGGL((mx_dequant_kernel<ST, FMT>), dim3((unsigned)blocks), dim3(256), 0, s,
                      static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), static_cast<ST*>(out), R,
-                     C, (int)mx_row_bytes(FMT, C), groups, act);
+                     C, (int)mx_row_bytes(FMT, C), spans, act);
   return hipGetLastError();
 }
 

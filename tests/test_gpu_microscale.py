@@ -31,7 +31,7 @@ def _pack4(x):
 @pytest.mark.parametrize("storage", ["fp32", "fp16", "bf16"])
 @pytest.mark.parametrize("axis", [0, 1])
 @pytest.mark.parametrize("R,C", [(1, 1), (1, 33), (33, 1), (5, 31), (32, 32), (64, 784), (65, 129), (127, 130),
-                                 (256, 200), (300, 1531), (200, 64)])
+                                 (256, 200), (300, 1531), (200, 64), (400, 513), (513, 400)])
 def test_quantize_is_the_definition(R, C, axis, storage, fmt):
     """Codes and scales equal, blocks of very different sizes among them."""
     g = torch.Generator().manual_seed(R * 7919 + C + axis)
@@ -138,7 +138,8 @@ def test_dequantize_every_code(R, C, storage, fmt):
 
 # ------------------------------------------------------------------ products
 SHAPES = [(1, 1, 1), (16, 10, 1), (64, 784, 128), (33, 129, 31), (100, 257, 40), (31, 500, 97), (300, 130, 200),
-          (129, 384, 1025), (1000, 300, 1531), (130, 2000, 70), (2048, 640, 1600)]
+          (129, 384, 1025), (1000, 300, 1531), (130, 2000, 70), (2048, 640, 1600), (1601, 130, 2049),
+          (3000, 200, 3001), (3001, 400, 2900)]
 
 
 def _close(got, want, bound, storage):
@@ -169,7 +170,8 @@ def test_forward_and_prediction_error(M, K, B, storage):
 
 @pytest.mark.parametrize("act", ["identity", "relu", "tanh", "sigmoid", "silu", "gelu"])
 @pytest.mark.parametrize("storage", ["fp32", "bf16", "fp16"])
-@pytest.mark.parametrize("M,K,B", [(1, 1, 1), (33, 129, 31), (64, 10, 128), (1100, 300, 1025), (2048, 640, 1600)])
+@pytest.mark.parametrize("M,K,B", [(1, 1, 1), (33, 129, 31), (64, 10, 128), (1100, 300, 1025), (2048, 640, 1600), (1601, 130, 2049),
+                                   (3000, 200, 3001), (3001, 130, 2900)])
 def test_inference_update(M, K, B, storage, act):
     g = torch.Generator().manual_seed(M + K + B)
     x, e = (_up(_rand(g, M, B, size=s).to(DT[storage])) for s in (1.0, 0.1))
@@ -186,7 +188,7 @@ def test_inference_update(M, K, B, storage, act):
 
 
 @pytest.mark.parametrize("storage", ["fp32", "bf16", "fp16"])
-@pytest.mark.parametrize("M,K,B", [(1, 1, 1), (10, 64, 128), (33, 31, 300), (1000, 1531, 300), (2100, 2048, 129)])
+@pytest.mark.parametrize("M,K,B", [(1, 1, 1), (10, 64, 128), (33, 31, 300), (1000, 1531, 300), (2100, 2048, 129), (3000, 3001, 40)])
 def test_weight_update(M, K, B, storage):
     g = torch.Generator().manual_seed(M + K + B)
     w = _up(_rand(g, M, K, size=0.1).to(DT[storage]))
