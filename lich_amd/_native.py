@@ -125,7 +125,8 @@ def _declare(lib):
         "ipc_mx_forward": ([vp, vp, vp, vp, vp, i, i, i, i, vp], i),
         "ipc_mx_infer_update": ([vp, vp, vp, vp, vp, vp, i, i, i, f, i, i, vp], i),
         "ipc_mx_weight_update": ([vp, vp, vp, vp, vp, i, i, i, f, i, vp], i),
-        "ipc_mx_predict": ([vp, vp, vp, vp, i, i, i, i, i, vp], i),
+        "ipc_mx_predict": ([vp, vp, vp, vp, i, i, i, i, i, vp, c_longlong, vp], i),
+        "ipc_mx_predict_workspace_bytes": ([i, i, i], c_longlong),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)

@@ -68,7 +68,11 @@ struct MxPredict {
   const void* x;
   const uint8_t* w; const uint32_t* ws;
   void* out;
+  void* terms;  // workspace of mx_predict_terms_bytes bytes for f(X), or nullptr
 };
+inline long long mx_predict_terms_bytes(int K, int B, int storage) {
+  return (storage == 0 ? 3LL : 2LL) * B * mx_groups(K) * MX_GROUP * 2;
+}
 hipError_t launch_mx_predict(const MxPredict& p, int storage, hipStream_t s);
 
 }  // namespace ipc

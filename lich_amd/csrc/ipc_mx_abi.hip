@@ -31,6 +31,11 @@ int check_codes(const void* codes, const void* scales, const char* name) {
   return ok();
 }
 
+// Bytes of caller workspace that ipc_mx_predict uses: more than one sample's f(X).
+long long predict_workspace_need(int K, int B, int storage) {
+  return B == 1 ? 0 : mx_predict_terms_bytes(K, B, storage);
+}
+
 int product(int kind, const void* a, const void* as, const char* a_name, const void* b, const void* bs,
             const char* b_name, void* out, const char* out_name, const void* aux, const char* aux_name, int M, int N,
             int K, float scal, int storage, int act, void* stream, const char* what) {
@@ -116,8 +121,14 @@ int ipc_mx_weight_update(void* w, const void* e_codes, const void* e_scales, con
                  alpha, storage, IPC_ACT_IDENTITY, stream, "ipc_mx_weight_update");
 }
 
+long long ipc_mx_predict_workspace_bytes(int K, int B, int storage) {
+  if (K < 1 || B < 1 || B > (1 << 20) || storage < IPC_DT_F32 || storage > IPC_DT_BF16) return 0;
+  return predict_workspace_need(K, B, storage);
+}
+
 int ipc_mx_predict(const void* x, const void* w_codes, const void* w_scales, void* out, int M, int K, int B,
-                   int storage, int act, void* stream) {
+                   int storage, int act, void* workspace, long long workspace_bytes, void* stream) {
+  TRY(check_workspace(workspace, workspace_bytes));
   TRY(check_dtypes(storage, storage));
   TRY(check_act(act));
   TRY(check_dims(M, K, B, 1));
@@ -130,6 +141,8 @@ int ipc_mx_predict(const void* x, const void* w_codes, const void* w_scales, voi
   p.M = M; p.K = K; p.B = B; p.act = act;
   p.x = x; p.out = out;
   p.w = static_cast<const uint8_t*>(w_codes); p.ws = static_cast<const uint32_t*>(w_scales);
+  const long long need = predict_workspace_need(K, B, storage);
+  p.terms = need > 0 && workspace && workspace_bytes >= need ? workspace : nullptr;
   return launch_rc(launch_mx_predict(p, storage, (hipStream_t)stream), "ipc_mx_predict");
 }
 

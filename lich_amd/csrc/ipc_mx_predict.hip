@@ -14,6 +14,12 @@
 //
 // The k order within a group is free as long as both operands agree: product j
 // of a group takes values 8 j .. 8 j + 7 of every lane's own block.
+//
+// Two forms.  Without a workspace each workgroup evaluates f of every element it
+// needs (all of X, K x 16 samples at a time): nothing for one sample, most of the
+// time for many.  With one, f(X) is evaluated once, in a launch of its own, into its
+// terms transposed ([term][sample][k]): the operand's lanes then load their 8
+// values as they are.
 #include <algorithm>
 
 #include "ipc_launch.h"
@@ -25,26 +31,31 @@ namespace {
 constexpr int MAX_WAVES = 16;
 constexpr int XLD = MX_GROUP + 8;  // bf16 values per sample row of a staged group
 
-// NT: 16-sample tiles; NP: samples a staging pass covers, a power of two >= the
-// samples of the block (16 NT from 16 on), so that consecutive lanes take
-// consecutive samples of a k-row.
-template <typename ST, int NT, int NP>
+// Eight weights of a block, widened.
+__device__ __forceinline__ bf16x8 widen8(unsigned w, float scale) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 a0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0), a1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1);
+  const bf16x2 a2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2), a3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3);
+  return bf16x8{a0[0], a0[1], a1[0], a1[1], a2[0], a2[1], a3[0], a3[1]};
+}
+
+// NP: samples a staging pass covers, 16 or the power of two >= B below it, so that
+// consecutive lanes take consecutive samples of a k-row.
+template <typename ST, int NP>
 __global__ void __launch_bounds__(MAX_WAVES * 64) mx_predict_kernel(const MxPredict p) {
   constexpr int TERMS = sizeof(ST) == 4 ? 3 : 2;
   extern __shared__ __align__(16) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int M = p.M, K = p.K, B = p.B, G = mx_groups(K);
-  const int m0 = blockIdx.x * 16, b0 = blockIdx.y * 16 * NT, nb = B - b0 < 16 * NT ? B - b0 : 16 * NT;
+  const int m0 = blockIdx.x * 16, b0 = blockIdx.y * 16, nb = B - b0 < 16 ? B - b0 : 16;
   const int r = lane & 15, g = lane >> 4;
   const int m = m0 + r < M ? m0 + r : M - 1;  // rows past the end: never stored
   bf16* xs = reinterpret_cast<bf16*>(smem) + (size_t)wave * TERMS * NP * XLD;  // [term][sample][k], the wave's own
   const uint8_t* wr = p.w + (long long)m * G * 64 + g * 16;
   const ST* x = reinterpret_cast<const ST*>(p.x) + b0;
 
-  f32x4 acc[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 
   // a group's codes, scales and states; the next group's loads go out before this one's products
   constexpr int XI = 2 * NP;  // staged values per lane
@@ -87,32 +98,20 @@ __global__ void __launch_bounds__(MAX_WAVES * 64) mx_predict_kernel(const MxPred
     const float scale = __builtin_bit_cast(float, (sb == 255u ? 0x7fc00000u : sb << 23));
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-      bf16x8 a;
-      const bf16x2 a0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], scale, 0);
-      const bf16x2 a1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], scale, 1);
-      const bf16x2 a2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], scale, 2);
-      const bf16x2 a3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], scale, 3);
-      a[0] = a0[0]; a[1] = a0[1]; a[2] = a1[0]; a[3] = a1[1];
-      a[4] = a2[0]; a[5] = a2[1]; a[6] = a3[0]; a[7] = a3[1];
+      const bf16x8 a = widen8(w[j], scale);
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int u = 0; u < TERMS; ++u) {
-          const int n = t * 16 + r < NP ? t * 16 + r : NP - 1;  // (columns past the samples: never stored)
-          const bf16x8 b = *reinterpret_cast<const bf16x8*>(&xs[(u * NP + n) * XLD + g * 32 + j * 8]);
-          acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc[t], 0, 0, 0);
-        }
+      for (int u = 0; u < TERMS; ++u) {
+        const bf16x8 b = *reinterpret_cast<const bf16x8*>(&xs[(u * NP + (r < NP ? r : NP - 1)) * XLD + g * 32 + j * 8]);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);  // (columns past the samples: never stored)
+      }
     }
   }
-  // partial tiles [wave][16 rows][16 NT + 1 columns], over the staged states
+  // partial tiles [wave][16 rows][17], over the staged states
   __syncthreads();
   float* part = reinterpret_cast<float*>(smem);
-  constexpr int LD = 16 * NT + 1;
+  constexpr int LD = 17;
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) part[(wave * 16 + 4 * g + q) * LD + t * 16 + r] = acc[t][q];
+  for (int q = 0; q < 4; ++q) part[(wave * 16 + 4 * g + q) * LD + r] = acc[q];
   __syncthreads();
   ST* out = reinterpret_cast<ST*>(p.out);
   for (int i = tid; i < 16 * nb; i += blockDim.x) {
@@ -123,27 +122,145 @@ __global__ void __launch_bounds__(MAX_WAVES * 64) mx_predict_kernel(const MxPred
   }
 }
 
-template <typename ST, int NT, int NP>
+// f(X) [K][B] into its bf16 terms [term][sample][groups * 128], zero past K: 8
+// values of a sample per thread, samples fastest (coalesced reads).
+template <typename ST>
+__global__ void __launch_bounds__(256) mx_terms_kernel(const ST* __restrict__ x, bf16* __restrict__ out, int K, int B,
+                                                       int groups, int act) {
+  constexpr int TERMS = sizeof(ST) == 4 ? 3 : 2;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int n = (int)(i % B), k = (int)(i / B) * 8;
+  if (k >= groups * MX_GROUP) return;
+  float v[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) v[q] = k + q < K ? to_f32(x[(long long)(k + q) * B + n]) : 0.0f;
+  activate<8>(act, v);
+#pragma unroll
+  for (int t = 0; t < TERMS; ++t) {
+    bf16x8 h;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const bf16 b = cvt<bf16>(k + q < K ? v[q] : 0.0f);
+      h[q] = b;
+      v[q] = __builtin_isfinite(to_f32(b)) ? v[q] - to_f32(b) : 0.0f;  // (an infinity has no rest)
+    }
+    *reinterpret_cast<bf16x8*>(out + ((long long)t * B + n) * groups * MX_GROUP + k) = h;
+  }
+}
+
+// RM x NT tiles of 16 rows and 16 samples per workgroup, its waves splitting the
+// contraction.
+template <typename ST, int RM, int NT>
+__global__ void __launch_bounds__(MAX_WAVES * 64) mx_predict_terms_kernel(const MxPredict p) {
+  constexpr int TERMS = sizeof(ST) == 4 ? 3 : 2;
+  constexpr int LD = 16 * NT + 1;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, waves = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int M = p.M, B = p.B, G = mx_groups(p.K);
+  const int m0 = blockIdx.x * 16 * RM, b0 = blockIdx.y * 16 * NT, nb = B - b0 < 16 * NT ? B - b0 : 16 * NT;
+  const int r = lane & 15, g = lane >> 4;
+  int m[RM];
+  const bf16* xr[NT];
+#pragma unroll
+  for (int i = 0; i < RM; ++i) m[i] = m0 + i * 16 + r < M ? m0 + i * 16 + r : M - 1;  // rows past the end: never stored
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int n = b0 + t * 16 + r < B ? b0 + t * 16 + r : B - 1;  // (nor samples)
+    xr[t] = reinterpret_cast<const bf16*>(p.terms) + (long long)n * G * MX_GROUP + g * 32;
+  }
+  const long long term = (long long)B * G * MX_GROUP;
+  f32x4 acc[RM][NT];
+#pragma unroll
+  for (int i = 0; i < RM; ++i)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[i][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int kg = wave; kg < G; kg += waves) {
+    mx::u32x4 w[RM];
+    float scale[RM];
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+      w[i] = *reinterpret_cast<const mx::u32x4*>(p.w + ((long long)m[i] * G + kg) * 64 + g * 16);
+      const unsigned sb = (p.ws[(long long)kg * M + m[i]] >> (8 * g)) & 255u;
+      scale[i] = __builtin_bit_cast(float, (sb == 255u ? 0x7fc00000u : sb << 23));
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      bf16x8 a[RM];
+#pragma unroll
+      for (int i = 0; i < RM; ++i) a[i] = widen8(w[i][j], scale[i]);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < TERMS; ++u) {
+          const bf16x8 b = *reinterpret_cast<const bf16x8*>(xr[t] + u * term + (long long)kg * MX_GROUP + j * 8);
+#pragma unroll
+          for (int i = 0; i < RM; ++i) acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b, acc[i][t], 0, 0, 0);
+        }
+    }
+  }
+  float* part = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int i = 0; i < RM; ++i)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) part[((wave * RM + i) * 16 + 4 * g + q) * LD + t * 16 + r] = acc[i][t][q];
+  __syncthreads();
+  ST* out = reinterpret_cast<ST*>(p.out);
+  for (int i = tid; i < 16 * RM * 16 * NT; i += blockDim.x) {
+    const int row = i / (16 * NT), n = i % (16 * NT);
+    if (m0 + row >= M || n >= nb) continue;
+    float s = 0.0f;
+    for (int w = 0; w < waves; ++w) s += part[(w * RM * 16 + row) * LD + n];
+    out[(long long)(m0 + row) * B + b0 + n] = cvt<ST>(s);
+  }
+}
+
+template <typename ST, int NP>
 hipError_t run(const MxPredict& p, hipStream_t s) {
   constexpr int TERMS = sizeof(ST) == 4 ? 3 : 2;
-  constexpr int WAVE_BYTES = std::max(TERMS * NP * XLD * 2, 16 * (16 * NT + 1) * 4);
+  constexpr int WAVE_BYTES = std::max(TERMS * NP * XLD * 2, 16 * 17 * 4);
   constexpr int MOST = std::min(MAX_WAVES, 160 * 1024 / WAVE_BYTES);
-  const void* fn = reinterpret_cast<const void*>(&mx_predict_kernel<ST, NT, NP>);
+  const void* fn = reinterpret_cast<const void*>(&mx_predict_kernel<ST, NP>);
   static const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, MOST * WAVE_BYTES);
   if (e != hipSuccess) return e;
   const int waves = std::min(mx_groups(p.K), MOST);
   MxPredict q = p;
   void* args[] = {&q};
-  return hipLaunchKernel(fn, dim3((p.M + 15) / 16, (p.B + 16 * NT - 1) / (16 * NT)), dim3(waves * 64), args,
-                         (size_t)waves * WAVE_BYTES, s);
+  return hipLaunchKernel(fn, dim3((p.M + 15) / 16, (p.B + 15) / 16), dim3(waves * 64), args, (size_t)waves * WAVE_BYTES, s);
+}
+
+template <typename ST, int RM, int NT>
+hipError_t run_terms(const MxPredict& p, hipStream_t s) {
+  constexpr int WAVE_BYTES = RM * 16 * (16 * NT + 1) * 4;
+  constexpr int MOST = std::min(MAX_WAVES, 160 * 1024 / WAVE_BYTES);
+  const void* fn = reinterpret_cast<const void*>(&mx_predict_terms_kernel<ST, RM, NT>);
+  static const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, MOST * WAVE_BYTES);
+  if (e != hipSuccess) return e;
+  const int waves = std::min(mx_groups(p.K), MOST);
+  MxPredict q = p;
+  void* args[] = {&q};
+  return hipLaunchKernel(fn, dim3((p.M + 16 * RM - 1) / (16 * RM), (p.B + 16 * NT - 1) / (16 * NT)), dim3(waves * 64),
+                         args, (size_t)waves * WAVE_BYTES, s);
 }
 
 template <typename ST>
 hipError_t run_samples(const MxPredict& p, hipStream_t s) {
-  if (p.B == 1) return run<ST, 1, 1>(p, s);
-  if (p.B <= 4) return run<ST, 1, 4>(p, s);
-  if (p.B <= 16) return run<ST, 1, 16>(p, s);
-  return run<ST, 2, 32>(p, s);
+  if (p.terms) {
+    const int G = mx_groups(p.K);
+    const long long items = (long long)G * (MX_GROUP / 8) * p.B;
+    hipLaunchKernelGGL(mx_terms_kernel<ST>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s,
+                       static_cast<const ST*>(p.x), static_cast<bf16*>(p.terms), p.K, p.B, G, p.act);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (p.B <= 16) return p.M < 8192 ? run_terms<ST, 1, 1>(p, s) : run_terms<ST, 2, 1>(p, s);
+    if (p.B <= 32) return p.M < 8192 ? run_terms<ST, 1, 2>(p, s) : run_terms<ST, 2, 2>(p, s);
+    return p.M < 8192 ? run_terms<ST, 1, 4>(p, s) : run_terms<ST, 2, 4>(p, s);
+  }
+  if (p.B == 1) return run<ST, 1>(p, s);
+  if (p.B <= 4) return run<ST, 4>(p, s);
+  return run<ST, 16>(p, s);
 }
 
 }  // namespace

@@ -86,11 +86,11 @@ __global__ void __launch_bounds__(256) mx_quant_rows_kernel(const ST* __restrict
 template <typename ST, int FMT>
 __global__ void __launch_bounds__(256) mx_quant_cols_kernel(const ST* __restrict__ x, uint8_t* __restrict__ codes,
                                                             uint8_t* __restrict__ scales, int K, int N,
-                                                            int row_bytes, int spans, int act) {
+                                                            int row_bytes, int tiles, int act) {
   constexpr int VPD = 4 / sizeof(ST);  // columns per dword
   constexpr int COLS = 32 * VPD, VEC = 16 / sizeof(ST);
   __shared__ __align__(16) unsigned tile[WIDTH * 32];
-  const int n0 = blockIdx.x / spans * COLS, k0 = blockIdx.x % spans * WIDTH;
+  const int n0 = blockIdx.x % tiles * COLS, k0 = blockIdx.x / tiles * WIDTH;  // (whole rows at once)
   const int tid = threadIdx.x;
   {
     typedef typename mx::Run<ST, VEC>::V V;
@@ -219,11 +219,11 @@ template <typename ST, int FMT>
 hipError_t quantize(const void* x, void* codes, void* scales, int R, int C, int axis, int act, hipStream_t s) {
   const int rows = axis == 1 ? R : C, n = axis == 1 ? C : R;
   const int spans = (mx_groups(n) + 1) / 2, per = axis == 1 ? TILE_ROWS<ST> : 128 / (int)sizeof(ST);
-  const long long blocks = (long long)spans * ((rows + (long long)per - 1) / per);
+  const long long tiles = (rows + (long long)per - 1) / per, blocks = spans * tiles;
   const int row_bytes = (int)mx_row_bytes(FMT, n);
   hipLaunchKernelGGL((axis == 1 ? mx_quant_rows_kernel<ST, FMT> : mx_quant_cols_kernel<ST, FMT>),
                      dim3((unsigned)blocks), dim3(256), 0, s, static_cast<const ST*>(x), static_cast<uint8_t*>(codes),
-                     static_cast<uint8_t*>(scales), R, C, row_bytes, spans, act);
+                     static_cast<uint8_t*>(scales), R, C, row_bytes, axis == 1 ? spans : (int)tiles, act);
   return hipGetLastError();
 }
 

@@ -55,14 +55,11 @@ def packed_shapes(rows: int, n: int, format: str = "fp4"):
 
 def new_packed(rows: int, n: int, format: str = "fp4", device=None) -> MXMatrix:
     """An uninitialised packed matrix of ``rows`` rows of ``n`` values."""
-    codes, scales = packed_shapes(rows, n, format)
-    device = device or torch.device("cuda")
-    return MXMatrix(torch.empty(codes, dtype=torch.uint8 if format == "fp4" else torch.int8, device=device),
-                    torch.empty(scales, dtype=torch.uint8, device=device))
+    return _Packed("packed", rows, n, format).new(device)
 
 
 class _Packed:
-    """Checks of a packed operand, made once per kernel."""
+    """Checks of a packed operand; the call gives its pointers."""
 
     def __init__(self, name: str, rows: int, n: int, format: str = "fp4"):
         self.name, self.format = name, _format(format)
@@ -72,9 +69,21 @@ class _Packed:
     def __call__(self, m):
         if not isinstance(m, tuple) or len(m) != 2:
             raise ValueError(f"{self.name} must be an MXMatrix (codes, scales)")
-        _check(m[0], f"{self.name}.codes", self.codes, self.dtype)
-        _check(m[1], f"{self.name}.scales", self.scales, torch.uint8)
-        return m[0].data_ptr(), m[1].data_ptr()
+        return (_pointer(m[0], f"{self.name}.codes", self.codes, self.dtype),
+                _pointer(m[1], f"{self.name}.scales", self.scales, torch.uint8))
+
+    def new(self, device=None) -> MXMatrix:
+        device = device or torch.device("cuda")
+        return MXMatrix(torch.empty(self.codes, dtype=self.dtype, device=device),
+                        torch.empty(self.scales, dtype=torch.uint8, device=device))
+
+
+def _pointer(t, name: str, shape: tuple, dtype: torch.dtype) -> int:
+    """``_check`` and the tensor's address: one test where there is nothing to refuse
+    (0.25 us a tensor against 0.6, of calls that last 4)."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is dtype and t.shape == shape and t.is_contiguous()):
+        _check(t, name, shape, dtype)
+    return t.data_ptr()
 
 
 def _sizes(**sizes) -> None:
@@ -103,12 +112,12 @@ class MXQuantizeKernel(_MXKernel):
         self._packed = _Packed("packed", self.rows, self.length, format)
 
     def new_output(self, device=None) -> MXMatrix:
-        return new_packed(self.rows, self.length, self.format, device)
+        return self._packed.new(device)
 
     def __call__(self, x, packed):
-        _check(x, "X", (self.R, self.C), self.dtype)
+        x_at = _pointer(x, "X", (self.R, self.C), self.dtype)
         codes, scales = self._packed(packed)
-        nat.check(nat.lib().ipc_mx_quantize(x.data_ptr(), codes, scales, self.R, self.C, self.axis,
+        nat.check(nat.lib().ipc_mx_quantize(x_at, codes, scales, self.R, self.C, self.axis,
                                             nat.MX_FORMATS[self.format], self.storage, self.act,
                                             nat.current_stream_handle(x.device)))
 
@@ -124,8 +133,8 @@ class MXDequantizeKernel(_MXKernel):
 
     def __call__(self, packed, out):
         codes, scales = self._packed(packed)
-        _check(out, "OUT", (self.R, self.C), self.dtype)
-        nat.check(nat.lib().ipc_mx_dequantize(codes, scales, out.data_ptr(), self.R, self.C,
+        out_at = _pointer(out, "OUT", (self.R, self.C), self.dtype)
+        nat.check(nat.lib().ipc_mx_dequantize(codes, scales, out_at, self.R, self.C,
                                               nat.MX_FORMATS[self.format], self.storage,
                                               nat.current_stream_handle(out.device)))
 
@@ -147,9 +156,9 @@ class MXPredictionErrorKernel(_MXProduct):
 
     def __call__(self, x4, w4, x_lower, e):
         x, w = self._x(x4), self._w(w4)
-        _check(x_lower, "X_lower", (self.M, self.B), self.dtype)
-        _check(e, "E", (self.M, self.B), self.dtype)
-        nat.check(nat.lib().ipc_mx_pred_err(*x, *w, x_lower.data_ptr(), e.data_ptr(), self.M, self.K, self.B,
+        x_lower_at = _pointer(x_lower, "X_lower", (self.M, self.B), self.dtype)
+        e_at = _pointer(e, "E", (self.M, self.B), self.dtype)
+        nat.check(nat.lib().ipc_mx_pred_err(*x, *w, x_lower_at, e_at, self.M, self.K, self.B,
                                             self.storage, nat.current_stream_handle(e.device)))
 
 
@@ -162,8 +171,8 @@ class MXForwardKernel(_MXProduct):
 
     def __call__(self, x4, w4, out):
         x, w = self._x(x4), self._w(w4)
-        _check(out, "OUT", (self.M, self.B), self.dtype)
-        nat.check(nat.lib().ipc_mx_forward(*x, *w, out.data_ptr(), self.M, self.K, self.B, self.storage,
+        out_at = _pointer(out, "OUT", (self.M, self.B), self.dtype)
+        nat.check(nat.lib().ipc_mx_forward(*x, *w, out_at, self.M, self.K, self.B, self.storage,
                                            nat.current_stream_handle(out.device)))
 
 
@@ -177,10 +186,10 @@ class MXInferenceUpdateKernel(_MXProduct):
         self._w, self._e = _Packed("W_lower", self.M, self.K), _Packed("E_lower", self.B, self.K)
 
     def __call__(self, x, e, wt4, et4):
-        _check(x, "X", (self.M, self.B), self.dtype)
-        _check(e, "E", (self.M, self.B), self.dtype)
+        x_at = _pointer(x, "X", (self.M, self.B), self.dtype)
+        e_at = _pointer(e, "E", (self.M, self.B), self.dtype)
         w, el = self._w(wt4), self._e(et4)
-        nat.check(nat.lib().ipc_mx_infer_update(x.data_ptr(), e.data_ptr(), *w, *el, self.M, self.K, self.B,
+        nat.check(nat.lib().ipc_mx_infer_update(x_at, e_at, *w, *el, self.M, self.K, self.B,
                                                 self.gamma, self.storage, self.act,
                                                 nat.current_stream_handle(x.device)))
 
@@ -195,31 +204,31 @@ class MXWeightUpdateKernel(_MXProduct):
         self._e, self._a = _Packed("E", self.M, self.B), _Packed("A", self.K, self.B)
 
     def __call__(self, w, e4, a4):
-        _check(w, "W", (self.M, self.K), self.dtype)
+        w_at = _pointer(w, "W", (self.M, self.K), self.dtype)
         e, a = self._e(e4), self._a(a4)
-        nat.check(nat.lib().ipc_mx_weight_update(w.data_ptr(), *e, *a, self.M, self.K, self.B, self.alpha,
+        nat.check(nat.lib().ipc_mx_weight_update(w_at, *e, *a, self.M, self.K, self.B, self.alpha,
                                                  self.storage, nat.current_stream_handle(w.device)))
 
 
 class MXPredictKernel(_MXProduct):
     """``k(X[K, B], W4, OUT[M, B], *, workspace=None)``: ``OUT = W f(X)``, W [M, K] packed
-    by rows, the states not quantised."""
+    by rows, the states not quantised.  ``workspace`` (optional, caller-owned,
+    ``new_workspace()``) lets a call of several samples evaluate f(X) once."""
 
     def __init__(self, M, K, B, activation, dtype):
         super().__init__(M, K, B, dtype, activation)
         self._w = _Packed("W", self.M, self.K)
 
-    workspace_bytes = 0
+        self.workspace_bytes = int(nat.lib().ipc_mx_predict_workspace_bytes(self.K, self.B, self.storage))
 
-    def new_workspace(self, device=None):
-        return None
+    new_workspace, _ws = _Kernel.new_workspace, staticmethod(_Kernel._ws)
 
     def __call__(self, x, w4, out, *, workspace=None):
-        _check(x, "X", (self.K, self.B), self.dtype)
+        x_at = _pointer(x, "X", (self.K, self.B), self.dtype)
         w = self._w(w4)
-        _check(out, "OUT", (self.M, self.B), self.dtype)
-        nat.check(nat.lib().ipc_mx_predict(x.data_ptr(), *w, out.data_ptr(), self.M, self.K, self.B, self.storage,
-                                           self.act, nat.current_stream_handle(out.device)))
+        out_at = _pointer(out, "OUT", (self.M, self.B), self.dtype)
+        nat.check(nat.lib().ipc_mx_predict(x_at, *w, out_at, self.M, self.K, self.B, self.storage,
+                                           self.act, *self._ws(workspace), nat.current_stream_handle(out.device)))
 
 
 class _CheckpointKernel(_Kernel):
@@ -245,11 +254,11 @@ class CheckpointWeightUpdateKernel(_CheckpointKernel):
         self._x = _Packed("X", self.K, self.B, "int8")
 
     def __call__(self, w, e, x8, *, workspace=None):
-        _check(w, "W", (self.M, self.K), self.dtype)
-        _check(e, "E", (self.M, self.B), self.dtype)
+        w_at = _pointer(w, "W", (self.M, self.K), self.dtype)
+        e_at = _pointer(e, "E", (self.M, self.B), self.dtype)
         x = self._x(x8)
         nat.check(nat.lib().ipc_ckpt_weight_update(
-            w.data_ptr(), e.data_ptr(), *x, self.M, self.K, self.B, self.alpha, self.storage, self.operand, self.act,
+            w_at, e_at, *x, self.M, self.K, self.B, self.alpha, self.storage, self.operand, self.act,
             *self._ws(workspace), nat.current_stream_handle(w.device)))
 
 
@@ -264,12 +273,12 @@ class CheckpointGradientKernel(_CheckpointKernel):
         self._x = _Packed("X", self.M, self.B, "int8")
 
     def __call__(self, w_lower, e_lower, x8, g, *, workspace=None):
-        _check(w_lower, "W_lower", (self.K, self.M), self.dtype)
-        _check(e_lower, "E_lower", (self.K, self.B), self.dtype)
+        w_lower_at = _pointer(w_lower, "W_lower", (self.K, self.M), self.dtype)
+        e_lower_at = _pointer(e_lower, "E_lower", (self.K, self.B), self.dtype)
         x = self._x(x8)
-        _check(g, "G", (self.M, self.B), self.dtype)
+        g_at = _pointer(g, "G", (self.M, self.B), self.dtype)
         nat.check(nat.lib().ipc_ckpt_gradient(
-            w_lower.data_ptr(), e_lower.data_ptr(), *x, g.data_ptr(), self.M, self.K, self.B, self.storage,
+            w_lower_at, e_lower_at, *x, g_at, self.M, self.K, self.B, self.storage,
             self.operand, self.act, *self._ws(workspace), nat.current_stream_handle(g.device)))
 
 

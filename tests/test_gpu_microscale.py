@@ -236,7 +236,8 @@ def test_zero_rows_and_far_scales():
 # ------------------------------------------------------------------ few samples
 @pytest.mark.parametrize("storage", ["fp32", "fp16", "bf16"])
 @pytest.mark.parametrize("M,K,B", [(1, 1, 1), (10, 64, 1), (16, 784, 3), (64, 784, 4), (33, 129, 5), (100, 1531, 16),
-                                   (47, 300, 17), (130, 2100, 33), (64, 64, 100)])
+                                   (47, 300, 17), (130, 2100, 33), (64, 64, 100),
+                                   (8200, 300, 2), (8197, 140, 20), (8192, 130, 40)])
 @pytest.mark.parametrize("act", ["identity", "tanh", "sigmoid"])
 def test_predict(M, K, B, storage, act):
     g = torch.Generator().manual_seed(M + K + B)
@@ -245,10 +246,12 @@ def test_predict(M, K, B, storage, act):
     want = wq @ fx
     out = torch.full((M, B), 7.0, dtype=DT[storage], device="cuda")
     k = mx.build_mx_predict(M, K, B, act, DT[storage])
-    k(_dev(x, storage), _pack4(w), out, workspace=k.new_workspace())
     # f in fp32 (4 units), its terms (2^-17 of it for 16-bit states), the sum
     term = (2.0 ** -21 if storage == "fp32" else 2.0 ** -16) * (wq.abs() @ fx.abs())
-    _close(out, want, O.product_bound(wq, fx, 3 * K) + term, storage)
+    for workspace in (None, k.new_workspace()):
+        out.fill_(7.0)
+        k(_dev(x, storage), _pack4(w), out, workspace=workspace)
+        _close(out, want, O.product_bound(wq, fx, 3 * K) + term, storage)
 
 
 # ------------------------------------------------------------------ streams, graphs, repeats
