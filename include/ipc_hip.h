@@ -567,19 +567,16 @@ long long ipc_mx_predict_workspace_bytes(int K, int B, int storage);
  *   ipc_ckpt_gradient       G = f'(X) W_lower^T E_lower
  *                           W_lower [K][M], E_lower [K][B], X and G [M][B]
  * storage, operand: as for ipc_weight_update and ipc_infer_update; the state is
- * widened in the kernel's loader or epilogue, exactly where the operand type is
- * fp32 or bf16.  The largest 16-bit calls use a workspace lent by the caller
- * (16-byte aligned) as theirs do, ipc_ckpt_workspace_bytes bytes (kind
- * IPC_PHASE_WEIGHT or IPC_PHASE_INFER for the gradient; 0: none): f(X) widened
- * once, or the gradient's operands transposed.
+ * widened in the kernels, exactly where the operand type is fp32 or bf16.  Larger
+ * 16-bit weight updates use a workspace lent by the caller (16-byte aligned,
+ * ipc_ckpt_workspace_bytes bytes, 0: none), into which f(X) is widened once.
  */
 int ipc_ckpt_weight_update(void* w, const void* e, const void* x_codes, const void* x_scales, int M, int K, int B,
                            float alpha, int storage, int operand, int act, void* workspace,
                            long long workspace_bytes, void* stream);
 int ipc_ckpt_gradient(const void* w_lower, const void* e_lower, const void* x_codes, const void* x_scales, void* g,
-                      int M, int K, int B, int storage, int operand, int act, void* workspace,
-                      long long workspace_bytes, void* stream);
-long long ipc_ckpt_workspace_bytes(int kind, int act, int M, int K, int B, int storage);
+                      int M, int K, int B, int storage, int operand, int act, void* stream);
+long long ipc_ckpt_workspace_bytes(int act, int M, int K, int B, int storage);
 
 void ipc_plan_destroy(ipc_plan* plan);
 

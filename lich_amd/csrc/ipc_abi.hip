@@ -634,22 +634,24 @@ int check_state(const void* codes, const void* scales, int rows, int n) {
   return ok();
 }
 
-// Bytes of caller workspace a call uses: the weight update's f(X) widened once to
-// the storage type where the 16-bit kernels would activate it once, the state
-// gradient's transposed operands where theirs would be.
-long long ckpt_workspace_need(int kind, int act, int M, int K, int B, int storage) {
-  if (storage == IPC_DT_F32) return 0;
-  if (kind == IPC_PHASE_WEIGHT) {
-    if (!s16_preact_rule(S16_WEIGHT, act, M, K, (long long)K * B)) return 0;
-    return (long long)K * B * 2;
-  }
-  if (kind != IPC_PHASE_INFER || !dma_eligible(storage, K, {}, {M, B})) return 0;
-  if (!s16_preact_rule(S16_INFER, act, M, K, (long long)K * B)) return 0;
-  return ((long long)M * K + (long long)K * B) * 2;
+// Whether the 16-bit products of ipc_ckpt_gemm.h can run a call: operands of
+// `rows_a` rows of lda and `rows_b` of ldb elements, contraction k.
+bool ckpt_products(int storage, int k, std::initializer_list<const void*> operands, long long rows_a, long long lda,
+                   long long rows_b, long long ldb) {
+  if (storage == IPC_DT_F32 || k % 32 != 0 || lda % 8 != 0 || ldb % 8 != 0) return false;
+  for (const void* q : operands)
+    if (!al16(q)) return false;
+  return rows_a * lda < (1LL << 30) && rows_b * ldb < (1LL << 30);
 }
 
-bool ckpt_lent(long long need, const void* workspace, long long ws_bytes) {
-  return need > 0 && workspace && ws_bytes >= need;
+// The weight update's workspace: f(X) widened once to the storage type, for the
+// 16-bit products where there are outputs enough for them to win against the
+// kernels that widen in their loaders, or (lengths those products cannot take)
+// where evaluating f in every row tile costs more than that pass.
+long long ckpt_workspace_need(int act, int M, int K, int B, int storage) {
+  if (storage == IPC_DT_F32) return 0;
+  const bool products = ckpt_products(storage, B, {}, M, B, K, B) && (long long)M * K > (1 << 20);
+  return products || s16_preact_rule(S16_WEIGHT, act, M, K, (long long)K * B) ? (long long)K * B * 2 : 0;
 }
 
 // Tile of a call on the generic kernels (their rules, for a problem of its size).
@@ -661,9 +663,9 @@ int ckpt_tile(const GemmProblem& p, int storage, int operand) {
 
 extern "C" {
 
-long long ipc_ckpt_workspace_bytes(int kind, int act, int M, int K, int B, int storage) {
+long long ipc_ckpt_workspace_bytes(int act, int M, int K, int B, int storage) {
   if (M < 1 || K < 1 || B < 1 || act < IPC_ACT_IDENTITY || act > IPC_ACT_GELU) return 0;
-  return ckpt_workspace_need(kind, act, M, K, B, storage);
+  return ckpt_workspace_need(act, M, K, B, storage);
 }
 
 int ipc_ckpt_weight_update(void* w, const void* e, const void* x_codes, const void* x_scales, int M, int K, int B,
@@ -677,10 +679,20 @@ int ipc_ckpt_weight_update(void* w, const void* e, const void* x_codes, const vo
   const int es = elem_size(storage);
   TRY(check_ptr(w, "w", es));
   TRY(check_ptr(e, "e", es));
-  if (ckpt_lent(ckpt_workspace_need(IPC_PHASE_WEIGHT, act, M, K, B, storage), workspace, workspace_bytes)) {
-    TRY(launch_rc(launch_mx_dequantize(x_codes, x_scales, workspace, K, B, MX_INT8, storage, act, (hipStream_t)stream),
+  hipStream_t s = (hipStream_t)stream;
+  const long long need = ckpt_workspace_need(act, M, K, B, storage);
+  if (need > 0 && workspace && workspace_bytes >= need) {
+    TRY(launch_rc(launch_mx_dequantize(x_codes, x_scales, workspace, K, B, MX_INT8, storage, act, s),
                   "ipc_ckpt_weight_update"));
-    return ipc_weight_update(w, e, workspace, M, K, B, 1, alpha, 0, storage, operand, act, IPC_TILE_AUTO, stream);
+    if (!ckpt_products(storage, B, {e}, M, B, K, B))
+      return ipc_weight_update(w, e, workspace, M, K, B, 1, alpha, 0, storage, operand, act, IPC_TILE_AUTO, stream);
+    CkptProblem q{};
+    q.M = M; q.N = K; q.K = B;
+    q.a = e; q.lda = B;
+    q.b = workspace; q.ldb = B;
+    q.out = w; q.alpha = alpha;
+    q.vec = vec_ok(w, K, es);
+    return launch_rc(launch_ckpt_gemm(CKPT_WEIGHT, q, operand, act, s), "ipc_ckpt_weight_update");
   }
   GemmProblem p = make_wgt(w, e, x_codes, M, K, B, 1, alpha, 1, act, es);
   p.ldb = mx_row_bytes(MX_INT8, B);
@@ -695,17 +707,13 @@ int ipc_ckpt_weight_update(void* w, const void* e, const void* x_codes, const vo
     q.aux = x_scales;
     q.scal = alpha;
     q.vec = K % 4 == 0 && al8(w);
-    return launch_rc(launch_s16_ckpt(S16_WEIGHT8, q, operand, act, s16_auto_config(M, K, 1), (hipStream_t)stream),
-                     "ipc_ckpt_weight_update");
+    return launch_rc(launch_s16_weight8(q, operand, act, s16_auto_config(M, K, 1), s), "ipc_ckpt_weight_update");
   }
-  return launch_rc(launch_ckpt_weight(p, storage, operand, ckpt_tile(p, storage, operand), (hipStream_t)stream),
-                   "ipc_ckpt_weight_update");
+  return launch_rc(launch_ckpt_weight(p, storage, operand, ckpt_tile(p, storage, operand), s), "ipc_ckpt_weight_update");
 }
 
 int ipc_ckpt_gradient(const void* w_lower, const void* e_lower, const void* x_codes, const void* x_scales, void* g,
-                      int M, int K, int B, int storage, int operand, int act, void* workspace,
-                      long long workspace_bytes, void* stream) {
-  TRY(check_workspace(workspace, workspace_bytes));
+                      int M, int K, int B, int storage, int operand, int act, void* stream) {
   TRY(check_dtypes(storage, operand));
   TRY(check_act(act));
   TRY(check_dims(M, K, B, 1));
@@ -715,30 +723,19 @@ int ipc_ckpt_gradient(const void* w_lower, const void* e_lower, const void* x_co
   TRY(check_ptr(e_lower, "e_lower", es));
   TRY(check_ptr(g, "g", es));
   hipStream_t s = (hipStream_t)stream;
+  if (ckpt_products(storage, K, {w_lower, e_lower}, K, M, K, B)) {
+    CkptProblem q{};
+    q.M = M; q.N = B; q.K = K;
+    q.a = w_lower; q.lda = M;
+    q.b = e_lower; q.ldb = B;
+    q.x = x_codes; q.xs = x_scales; q.x_row = (int)mx_row_bytes(MX_INT8, B);
+    q.out = g;
+    q.vec = vec_ok(g, B, es);
+    return launch_rc(launch_ckpt_gemm(CKPT_GRAD, q, operand, act, s), "ipc_ckpt_gradient");
+  }
   GemmProblem p = make_inf(g, x_codes, w_lower, e_lower, nullptr, M, K, B, 1, 0.0f, act, es);
   p.ldx = mx_row_bytes(MX_INT8, B);
   p.out2 = const_cast<void*>(x_scales); p.ld2 = M;
-  if (dma_eligible(storage, K, {w_lower, e_lower}, {M, B}) && !generic_before_dma(p)) {
-    WideProblem q{};
-    q.M = M; q.N = B; q.K = K;
-    q.a = w_lower; q.lda = M; q.a_lim = M;
-    q.b = e_lower; q.ldb = B; q.b_lim = B;
-    q.out = g; q.ldo = B;
-    q.aux = x_codes; q.ldx = p.ldx;
-    q.h = const_cast<void*>(x_scales);
-    q.vec = B % 4 == 0 && al8(g);
-    const int cfg = s16_auto_config(M, B, 1);
-    if (ckpt_lent(ckpt_workspace_need(IPC_PHASE_INFER, act, M, K, B, storage), workspace, workspace_bytes)) {
-      char* wt = static_cast<char*>(workspace);
-      char* et = wt + (long long)M * K * 2;
-      TRY(launch_rc(launch_s16_activate_t(q.a, wt, K, M, 1, 0, operand, IPC_ACT_IDENTITY, s), "ipc_ckpt_gradient"));
-      TRY(launch_rc(launch_s16_activate_t(q.b, et, K, B, 1, 0, operand, IPC_ACT_IDENTITY, s), "ipc_ckpt_gradient"));
-      q.a = wt; q.lda = K;
-      q.b = et; q.ldb = K;
-      return launch_rc(launch_s16_ckpt(S16_GRADT, q, operand, act, cfg, s), "ipc_ckpt_gradient");
-    }
-    return launch_rc(launch_s16_ckpt(S16_GRAD, q, operand, act, cfg, s), "ipc_ckpt_gradient");
-  }
   return launch_rc(launch_ckpt_grad(p, storage, operand, ckpt_tile(p, storage, operand), s), "ipc_ckpt_gradient");
 }
 

@@ -1,0 +1,226 @@
+// ipc_ckpt_gemm.h - the backward pass of a state kept in 8 bits as 16-bit products (gfx950).
+//
+//   CKPT_GRAD     G[m][n] = f'(X)[m][n] sum_k A[k][m] B[k][n]   A = W_lower, B = E_lower
+//   CKPT_WEIGHT   W[m][n] += alpha sum_k A[m][k] B[n][k]         A = E, B = f(X) widened
+//
+// v_mfma_f32_32x32x16 tiles in the pipeline of the 4-bit product's tile kernel
+// (ipc_mx_gemm.h): four stages of LDS filled by LDS-DMA loads, here of 32 k (64
+// bytes of a k-contiguous row, or 32 k-rows of a tile's columns), one barrier a
+// stage, the loads spread between the products, the next fragments read while the
+// current products run.  A 16-bit product does a quarter of the fp4 one's work per
+// byte in the same time, so the same tile keeps the matrix units as busy.
+//
+//   * k-contiguous rows: chunk c (16 bytes) of row r at c ^ ((r >> 2) & 3), fragments
+//     are 16-byte reads;
+//   * k-rows (CKPT_GRAD): chunk c of k-row r at c ^ ((r & 3) << 2) (64 columns: ^ ((r & 2)
+//     << 1)), fragments come from
+//     two transposing reads (ds_read_b64_tr_b16), the operands are never transposed in
+//     memory;
+//
+// Reading the packed state in the weight update's own loader instead (codes to
+// registers, widened a step or two later, stored to the stage) was slower than
+// widening it once into a workspace at every size: 4096 x 4096, B = 1024, relu 59 us
+// against 40 and 5 for the widening.
+#pragma once
+
+#include "ipc_mx_gemm.h"
+
+namespace ipc {
+
+namespace mx {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+// 16 bytes a lane from byte offset v + s of a buffer into 64 consecutive places of
+// the LDS, unknown to the compiler: it would wait for every such load in flight
+// before each transposing read, whose address it cannot tell from theirs (the state
+// gradient's main loop then ran four times as long).  There is no register to wait
+// for; every wait is one of the kernel's own.
+__device__ __forceinline__ void to_lds16_unseen(i32x4 rsrc, unsigned char* lds, unsigned v, unsigned s) {
+  const unsigned at = (unsigned)(unsigned long long)(lds_void*)lds;
+  // (m0 holds the place; a wait state lies between its write and its use.  The compiler
+  // sets it anew for each instruction of its own that reads it.)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :
+               : "s"(at), "v"(v), "s"(rsrc), "s"(s)
+               : "memory");
+}
+// The buffer resource of `bytes` bytes at `base`, as words.
+__device__ __forceinline__ i32x4 rsrc_words(const void* base, unsigned bytes) {
+  const unsigned long long a = reinterpret_cast<unsigned long long>(base);
+  return i32x4{(int)(unsigned)a, (int)(unsigned)(a >> 32 & 0xffffu), (int)bytes, 0x00020000};
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+template <typename OT, int MODE, int ACT, int BM, int BN, int WGM, int WGN>
+__global__ void __launch_bounds__(WGM * WGN * 64) ckpt_gemm_kernel(const CkptProblem p) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  using MF = Mfma32<OT>;
+  typedef typename MF::operand V;
+  constexpr bool MN = MODE == CKPT_GRAD;
+  constexpr int NW = WGM * WGN, WTM = BM / WGM, WTN = BN / WGN, RM = WTM / 32, RN = WTN / 32;
+  constexpr int A_BYTES = BM * 64, B_BYTES = BN * 64, STAGE = A_BYTES + B_BYTES;
+  constexpr int IA = A_BYTES / 1024 / NW, IB = B_BYTES / 1024 / NW, LPS = IA + IB;  // LDS-DMA loads per wave and stage
+  static_assert(IA * 1024 * NW == A_BYTES && IB * 1024 * NW == B_BYTES, "tile / waves");
+
+  // consecutive tiles per XCD, in supertiles of 8 x 4 (as in mx_tile_kernel)
+  const int tn = (p.N + BN - 1) / BN, tm = (p.M + BM - 1) / BM;
+  const int b = blockIdx.x, per = gridDim.x >> 3, rem = gridDim.x & 7, xcd = b & 7;
+  const int t = xcd * per + (xcd < rem ? xcd : rem) + (b >> 3);
+  const int band = t / (8 * tn), rows = tm - band * 8 < 8 ? tm - band * 8 : 8, w8 = t - band * 8 * tn;
+  const int cs = w8 / (rows * 4), cols = tn - cs * 4 < 4 ? tn - cs * 4 : 4, w2 = w8 - cs * rows * 4;
+  const int m0 = (band * 8 + w2 / cols) * BM, n0 = (cs * 4 + w2 % cols) * BN;
+
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = w / WGN, wn = w % WGN, lr = lane & 31, lk = lane >> 5;
+  const int M = p.M, N = p.N, G = p.K / 32;  // (the host: K a multiple of 32, operands below 2^31 bytes)
+
+  const Rsrc ga(p.a, (unsigned)((MN ? (long long)p.K : (long long)M) * p.lda * 2));
+  const Rsrc gb(p.b, (unsigned)((MN ? (long long)p.K : (long long)N) * p.ldb * 2));
+  const i32x4 wa = rsrc_words(p.a, (unsigned)((long long)p.K * p.lda * 2)), wb = rsrc_words(p.b, (unsigned)((long long)p.K * p.ldb * 2));
+  // byte offset of this lane's 16 bytes of LDS-DMA instruction q of an operand (stage 0)
+  auto source = [&](int q, int edge, int e0, int lim, long long ld) -> unsigned {
+    const int slot = (q * NW + w) * 64 + lane;
+    if constexpr (MN) {  // columns past the end: the last 8 again, never stored
+      const int cpr = edge / 8, r = slot / cpr, c = (slot % cpr) ^ (edge == 64 ? (r & 2) << 1 : (r & 3) << 2);
+      const int col = e0 + c * 8 <= lim - 8 ? e0 + c * 8 : lim - 8;
+      return (unsigned)(r * ld + col) * 2u;
+    } else {
+      const int r = slot >> 2, c = (slot & 3) ^ ((r >> 2) & 3), row = e0 + r < lim ? e0 + r : lim - 1;
+      return (unsigned)(row * ld) * 2u + (unsigned)c * 16u;
+    }
+  };
+  unsigned oa[IA], ob[IB];
+#pragma unroll
+  for (int q = 0; q < IA; ++q) oa[q] = source(q, BM, m0, M, p.lda);
+#pragma unroll
+  for (int q = 0; q < IB; ++q) ob[q] = source(q, BN, n0, N, p.ldb);
+  const unsigned step_a = MN ? (unsigned)p.lda * 64u : 64u, step_b = MN ? (unsigned)p.ldb * 64u : 64u;
+  auto load = [&](int q, int kt, unsigned char* st) {
+    if constexpr (MN) {
+      if (q < IA) to_lds16_unseen(wa, st + (q * NW + w) * 1024, oa[q < IA ? q : 0], (unsigned)kt * step_a);
+      else to_lds16_unseen(wb, st + A_BYTES + ((q - IA) * NW + w) * 1024, ob[q >= IA && q - IA < IB ? q - IA : 0], (unsigned)kt * step_b);
+    } else if (q < IA) {
+      ga.to_lds16(st + (q * NW + w) * 1024, oa[q < IA ? q : 0], (unsigned)kt * step_a);
+    } else if (q < IA + IB) {
+      gb.to_lds16(st + A_BYTES + ((q - IA) * NW + w) * 1024, ob[q >= IA && q - IA < IB ? q - IA : 0], (unsigned)kt * step_b);
+    }
+  };
+
+  f32x16 acc[RM][RN];
+#pragma unroll
+  for (int i = 0; i < RM; ++i)
+#pragma unroll
+    for (int j = 0; j < RN; ++j)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
+
+  // fragments of 16 k (half s of a stage): row / column lr of a 32-wide block, k 8 lk .. + 7
+  const int g4 = lane >> 4, li = lane & 15;
+  const int tr_row = 8 * (g4 >> 1) + (li >> 2), tr_low = 2 * (g4 & 1) + ((li & 3) >> 1);
+  auto fragment = [&](const unsigned char* blk, int rowb, int e, int s) -> V {
+    if constexpr (MN) {
+      const int chunk = (((e >> 5) ^ (rowb == 128 ? li >> 3 : li >> 2)) << 2) | tr_low;
+      const unsigned char* p0 = blk + (s * 16 + tr_row) * rowb + (chunk << 4) + (li & 1) * 8;
+      const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p0));
+      const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p0 + 4 * rowb));
+      return __builtin_bit_cast(V, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      return *reinterpret_cast<const V*>(blk + (e + lr) * 64 + ((((s * 2) | lk) ^ ((lr >> 2) & 3)) << 4));
+    }
+  };
+  V fa[2][RM], fb[2][RN];
+  auto stage = [&](int kt) -> unsigned char* { return smem + (kt & (STAGES - 1)) * STAGE; };
+  auto group = [&](int kt) { return kt < G ? kt : G - 1; };  // (past the end: the last again, so that every step counts the same)
+
+  // prologue: stages 0 .. 2
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s)
+#pragma unroll
+    for (int q = 0; q < LPS; ++q) load(q, group(s), stage(s));
+  wait_loads<2 * LPS>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int j = 0; j < RN; ++j) fb[0][j] = fragment(stage(0) + A_BYTES, BN * 2, wn * WTN + j * 32, 0);
+#pragma unroll
+  for (int i = 0; i < RM; ++i) fa[0][i] = fragment(stage(0), BM * 2, wm * WTM + i * 32, 0);
+
+  // half a step: the products of set S; the fragments of the next 16 k (half S ^ 1 of
+  // `next`) and half of stage kt + 3's loads between them
+  auto half = [&](auto SV, const unsigned char* next, int kt) {
+    constexpr int S = decltype(SV)::value, O = S ^ 1;
+    constexpr int L0 = S == 0 ? 0 : (LPS + 1) / 2, L1 = S == 0 ? (LPS + 1) / 2 : LPS;
+    constexpr int NM = RM * RN, NR = RM + RN;
+#pragma unroll
+    for (int q = 0; q < NM; ++q) {
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+        if (r * NM / NR == q) {
+          if (r < RN) fb[O][r < RN ? r : 0] = fragment(next + A_BYTES, BN * 2, wn * WTN + r * 32, O);
+          else fa[O][r < RN ? 0 : r - RN] = fragment(next, BM * 2, wm * WTM + (r - RN) * 32, O);
+        }
+#pragma unroll
+      for (int l = L0; l < L1; ++l)
+        if ((l - L0) * NM / (L1 - L0) == q) load(l, group(kt + 3), stage(kt + 3));
+      const int i = q / RN, j = q % RN;
+      acc[i][j] = MF::run(fb[S][j], fa[S][i], acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+#pragma unroll 1
+  for (int kt = 0; kt < G; ++kt) {
+    // stage kt + 1 of this wave has landed (kt + 2 may be in flight), then everybody's;
+    // everybody is done with stage kt - 1, which kt + 3 takes
+    wait_loads<LPS>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    half(std::integral_constant<int, 0>{}, stage(kt), kt);
+    half(std::integral_constant<int, 1>{}, stage(kt + 1), kt);
+  }
+  wait_loads<0>();  // no load may land in the epilogue's tile
+
+  MxProblem e{};
+  e.M = M; e.N = N; e.out = p.out; e.scal = p.alpha;
+  e.aux = p.x; e.as = static_cast<const uint32_t*>(p.xs); e.groups = p.x_row;
+  float* es = reinterpret_cast<float*>(smem) + w * 32 * (WTN + 4);
+  constexpr int KIND = MODE == CKPT_GRAD ? KIND_GRAD8 : KIND_WEIGHT;
+  constexpr int EACT = MODE == CKPT_GRAD ? ACT : ACT_IDENTITY;
+  if (p.vec) tile_epilogue<OT, KIND, EACT, true, RM, RN>(e, acc, es, m0 + wm * WTM, n0 + wn * WTN);
+  else tile_epilogue<OT, KIND, EACT, false, RM, RN>(e, acc, es, m0 + wm * WTM, n0 + wn * WTN);
+}
+
+template <typename OT, int MODE, int ACT, int BM, int BN, int WGM, int WGN>
+hipError_t run_ckpt_tile(const CkptProblem& p, hipStream_t s) {
+  constexpr int epi = WGM * WGN * 32 * (BN / WGN + 4) * 4, st = STAGES * (BM + BN) * 64, smem = epi > st ? epi : st;
+  static_assert(smem <= 160 * 1024, "LDS");
+  const void* fn = reinterpret_cast<const void*>(&ckpt_gemm_kernel<OT, MODE, ACT, BM, BN, WGM, WGN>);
+  static const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != hipSuccess) return e;
+  const long long tiles = ((p.M + BM - 1LL) / BM) * ((p.N + BN - 1LL) / BN);
+  CkptProblem q = p;
+  void* args[] = {&q};
+  return hipLaunchKernel(fn, dim3((unsigned)tiles), dim3(WGM * WGN * 64), args, smem, s);
+}
+
+// The tile: the largest that gives the 256 CUs about one each.  MI355X, bf16, us, 256 /
+// 128 / 64 wide, gradient, then weight update (out rows x columns x contraction):
+//   2048 x 1024 x 1024   38 / 14.4 / 10.6   25 / 11.2 / 9.5   (128 tiles of 128 x 128)
+//   2048 x 2048 x 2048   57 / 26.1 / 30.9   44 / 24.3 / 44
+//   3200 x 3200 x 2048   59 / 56 / 67       47 / 58 / 91      (169 of 256 x 256)
+//   8192 x 2048 x 8192   205 / 235          203 / 295         (256)
+template <typename OT, int MODE, int ACT>
+hipError_t run_ckpt(const CkptProblem& p, hipStream_t s) {
+  auto tiles = [&](long long e) { return ((p.M + e - 1) / e) * ((p.N + e - 1) / e); };
+  if (tiles(256) >= (MODE == CKPT_GRAD ? 224 : 160)) return run_ckpt_tile<OT, MODE, ACT, 256, 256, 2, 2>(p, s);
+  if (tiles(128) > 128) return run_ckpt_tile<OT, MODE, ACT, 128, 128, 2, 2>(p, s);
+  return run_ckpt_tile<OT, MODE, ACT, 64, 64, 2, 2>(p, s);
+}
+
+}  // namespace mx
+}  // namespace ipc

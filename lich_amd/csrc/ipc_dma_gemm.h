@@ -80,17 +80,14 @@ __device__ __forceinline__ void wg_barrier() {
 // prediction / forward given f(X_upper)^T (S16_PREDT / S16_FWDT).  The wide
 // path keeps k-contiguous copies of every operand (WT, FT, ET next to W, F,
 // E), so all of its reads are plain 16-byte fragment reads.
-constexpr bool a_mn(int mode) { return mode == S16_INFER || mode == S16_GRAD; }
-constexpr bool b_mn(int mode) { return mode == S16_PRED || mode == S16_FWD || mode == S16_INFER || mode == S16_GRAD; }
+constexpr bool a_mn(int mode) { return mode == S16_INFER; }
+constexpr bool b_mn(int mode) { return mode == S16_PRED || mode == S16_FWD || mode == S16_INFER; }
 constexpr bool is_s16(int mode) { return mode >= S16_PRED; }
 // the standalone prediction / forward, with B as given or as f(X_upper)^T
 constexpr bool s16_pred(int mode) { return mode == S16_PRED || mode == S16_PREDT; }
 constexpr bool s16_fwd(int mode) { return mode == S16_FWD || mode == S16_FWDT; }
 // the standalone inference update, with W_lower / E_lower as given or transposed
 constexpr bool s16_infer(int mode) { return mode == S16_INFER || mode == S16_INFERT; }
-
-// the state gradient of a state kept in 8 bits
-constexpr bool s16_grad(int mode) { return mode == S16_GRAD || mode == S16_GRADT; }
 
 // chunk position of chunk c in row r
 __device__ __forceinline__ int kc_swz(int r, int c) { return c ^ ((r >> 1) & 7); }
@@ -171,9 +168,6 @@ struct Buf {
   }
   __device__ __forceinline__ void st16(unsigned short x, unsigned v, unsigned s) const {
     __builtin_amdgcn_raw_buffer_store_b16(x, r, v, s, 0);
-  }
-  __device__ __forceinline__ unsigned char ld8(unsigned v, unsigned s) const {
-    return __builtin_amdgcn_raw_buffer_load_b8(r, v, s, 0);
   }
   __device__ __forceinline__ unsigned short ld16(unsigned v, unsigned s) const {
     return __builtin_amdgcn_raw_buffer_load_b16(r, v, s, 0);
@@ -385,13 +379,6 @@ __global__ void __launch_bounds__(WGM * WGN * 64) dma_gemm_kernel(const Batch bt
     const int r = idx / (BN / 4), col = (idx % (BN / 4)) * 4;
     const int m = m0 + r, n = n0 + col;
     const int nv = (m < M && n < N) ? (N - n < 4 ? N - n : 4) : 0;
-    if constexpr (s16_grad(MODE)) {
-      o[0] = o[1] = o[2] = o[3] = 0.0f;
-      if (nv > 0)
-        mx::state4(reinterpret_cast<const unsigned char*>(p.aux), p.ldx, reinterpret_cast<const unsigned char*>(p.h), M,
-                   m, n, o);
-      return;
-    }
     if (S16) {
       const OT* src = reinterpret_cast<const OT*>(basev) + (long long)m * ld + n;
       if (vec && nv == 4) {
@@ -625,8 +612,6 @@ __global__ void __launch_bounds__(WGM * WGN * 64) dma_gemm_kernel(const Batch bt
     const Buf bh(p.h, !S16 && p.h ? (long long)M * p.ldh * (long long)sizeof(OT) : 0);
     const Buf bl(p.hl, !S16 && p.hl ? (long long)M * p.ldhl * (long long)sizeof(OT) : 0);
     const Buf b2(p.out2, p.out2 ? (long long)M * p.ld2 * ES : 0);
-    const Buf bq(p.aux, s16_grad(MODE) ? (long long)M * p.ldx : 0);                             // codes
-    const Buf bs(p.h, s16_grad(MODE) ? (long long)mx_groups(N) * M * 4 : 0);                     // scales
     auto ldin = [&](const Buf& b, unsigned v, unsigned s) -> float {
       if constexpr (S16) return to_f32(__builtin_bit_cast(OT, b.ld16(v, s)));
       else return b.ld32(v, s);
@@ -654,15 +639,6 @@ __global__ void __launch_bounds__(WGM * WGN * 64) dma_gemm_kernel(const Batch bt
         const int n = n0 + wn * WTN + (bk % RN) * 32 + elr, nn = n < N ? n : 0;
         const int mb = m0 + wm * WTM + (bk / RN) * 32 + 4 * elk;
         const unsigned vx = (unsigned)(mb * xld + nn) * ES, ve = (unsigned)(mb * p.ldx + nn) * ES;
-        if constexpr (s16_grad(MODE)) {
-          const unsigned vq = (unsigned)(mb * p.ldx + nn);
-          const unsigned vs = ((unsigned)((nn >> 7) * M) + (unsigned)mb) * 4u + (unsigned)((nn >> 5) & 3);
-#pragma unroll
-          for (int q = 0; q < 16; ++q)
-            xo[PRE ? q : 0] = (float)(int)(signed char)bq.ld8(vq, (unsigned)(qrow(q) * p.ldx)) *
-                              mx::int8_scale(bs.ld8(vs, (unsigned)qrow(q) * 4u));
-          return;
-        }
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
           if constexpr (PRE) xo[PRE ? q : 0] = ldin(bx, vx, (unsigned)(qrow(q) * xld) * ES);
@@ -688,8 +664,6 @@ __global__ void __launch_bounds__(WGM * WGN * 64) dma_gemm_kernel(const Batch bt
             hv = cvt<OT>(x - to_f32(cvt<OT>(a)));
           } else if (s16_fwd(MODE)) {
             hv = cvt<OT>(a);
-          } else if (s16_grad(MODE)) {
-            hv = cvt<OT>(dact_t<ACT>(x) * a);                          // G
           } else if (s16_infer(MODE)) {
             const float xn = x + s_scal * (-ein[cur][EIN ? q : 0] + dact_t<ACT>(x) * a);
             hv = cvt<OT>(xn);
@@ -853,8 +827,6 @@ __global__ void __launch_bounds__(WGM * WGN * 64) dma_gemm_kernel(const Batch bt
           hv[q] = cvt<OT>(x - to_f32(cvt<OT>(a)));
         } else if (s16_fwd(MODE)) {
           hv[q] = cvt<OT>(a);
-        } else if (s16_grad(MODE)) {
-          hv[q] = cvt<OT>(dact_t<ACT>(x) * a);                          // G
         } else if (s16_infer(MODE)) {
           const float xn = x + p.scal * (-ein[u][q] + dact_t<ACT>(x) * a);
           hv[q] = cvt<OT>(xn);

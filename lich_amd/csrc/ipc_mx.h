@@ -71,8 +71,26 @@ struct MxPredict {
   void* terms;  // workspace of mx_predict_terms_bytes bytes for f(X), or nullptr
 };
 inline long long mx_predict_terms_bytes(int K, int B, int storage) {
-  return (storage == 0 ? 3LL : 2LL) * B * mx_groups(K) * MX_GROUP * 2;
+  const long long rows = B < 16 ? B : (B + 15LL) / 16 * 16;
+  return (storage == 0 ? 3LL : 2LL) * rows * mx_groups(K) * MX_GROUP * 2;
 }
 hipError_t launch_mx_predict(const MxPredict& p, int storage, hipStream_t s);
+
+// The backward pass of a state kept in 8 bits as 16-bit products (ipc_ckpt_gemm.h):
+// the contraction a multiple of 32, 16-byte aligned operands and row lengths that
+// are multiples of 8, operands below 2^31 bytes.
+struct CkptProblem {
+  int M, N, K;
+  const void* a; long long lda;  // elements
+  const void* b; long long ldb;
+  const void* x;                 // CKPT_GRAD: codes, scales and row bytes of X [M][N]
+  const void* xs;
+  int x_row;
+  void* out;                     // [M][N], 16-bit
+  float alpha;
+  int vec;                       // out allows 4-element accesses
+};
+enum { CKPT_GRAD = 0, CKPT_WEIGHT = 1 };
+hipError_t launch_ckpt_gemm(int mode, const CkptProblem& p, int operand, int act, hipStream_t s);
 
 }  // namespace ipc

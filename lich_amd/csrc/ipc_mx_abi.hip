@@ -31,9 +31,12 @@ int check_codes(const void* codes, const void* scales, const char* name) {
   return ok();
 }
 
-// Bytes of caller workspace that ipc_mx_predict uses: more than one sample's f(X).
+// Bytes of caller workspace that ipc_mx_predict uses: for f(X) evaluated once, which
+// pays for its launch from five samples on.  MI355X, bf16, us, without / with: 64 x
+// 784 8 samples 6.3 / 6.0; 4096 x 4096 8 relu 13.8 / 8.8, 64 51 / 14.7; 8192 x 8192 4 relu
+// 12.1 / 15.0, gelu 16.2 / 15.3, 8 48 / 15.8, 64 191 / 40 (fp32 states the same way).
 long long predict_workspace_need(int K, int B, int storage) {
-  return B == 1 ? 0 : mx_predict_terms_bytes(K, B, storage);
+  return B > 4 ? mx_predict_terms_bytes(K, B, storage) : 0;
 }
 
 int product(int kind, const void* a, const void* as, const char* a_name, const void* b, const void* bs,

@@ -78,6 +78,10 @@ __device__ __forceinline__ void put4(ST* p, bool vec, int left, const float (&v)
   }
 }
 
+// An epilogue of the 16-bit products in ipc_ckpt_gemm.h: G = f'(X) C, X kept in 8 bits
+// (aux its codes, as its scales, groups the bytes of its rows).
+constexpr int KIND_GRAD8 = 100;
+
 // The epilogue of four elements, in fp32, each operation rounded on its own and
 // the result rounded once to the storage type.  in: X_lower (PRED), X (INFER),
 // W (WEIGHT); e: E (INFER).
@@ -87,7 +91,8 @@ __device__ __forceinline__ void finish4(const float (&c)[4], const float (&in)[4
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
 #pragma clang fp contract(off)
-    if (KIND == KIND_PRED) o[i] = in[i] - c[i];
+    if (KIND == KIND_GRAD8) o[i] = dact_t<ACT>(in[i]) * c[i];
+    else if (KIND == KIND_PRED) o[i] = in[i] - c[i];
     else if (KIND == KIND_FWD) o[i] = c[i];
     else if (KIND == KIND_INFER) o[i] = in[i] + scal * (-e[i] + dact_t<ACT>(in[i]) * c[i]);
     else o[i] = in[i] + scal * c[i];
@@ -291,6 +296,20 @@ __device__ __forceinline__ void tile_epilogue(const MxProblem& p, const f32x16 (
   Raw4<ST, VEC> in[2][IN ? PASSES : 1], e[2][E ? PASSES : 1];
   auto fetch = [&](int v, int set) {  // 16 rows
     const long long first = (mw + v * 16) * N + nw;
+    if constexpr (KIND == KIND_GRAD8) {  // four codes and their block's scale byte
+      const int row = p.groups, n = nw + ec;
+      const uint8_t* at8 = static_cast<const uint8_t*>(p.aux) + (long long)(mw + v * 16) * row;
+      const Rsrc codes(at8, mw + v * 16 < p.M ? (unsigned)min((p.M - (long long)(mw + v * 16)) * row, 0xffffff00LL) : 0u);
+      const Rsrc scales(p.as, (unsigned)mx_groups(p.N) * (unsigned)p.M * 4u);
+#pragma unroll
+      for (int u = 0; u < PASSES; ++u) {
+        const int r = u * RPP + er, m = mw + v * 16 + r;
+        in[set][u].v[0] = __builtin_amdgcn_raw_buffer_load_b32(codes.r, left > 0 ? (unsigned)(r * row + n) : 0xfffffff0u, 0, 0);
+        in[set][u].v[1] = __builtin_amdgcn_raw_buffer_load_b8(
+            scales.r, left > 0 && m < p.M ? ((unsigned)(n >> 7) * (unsigned)p.M + (unsigned)m) * 4u + ((n >> 5) & 3) : 0xfffffff0u, 0, 0);
+      }
+      return;
+    }
     if constexpr (IN) {
       const Rows<ST, VEC> src(KIND == KIND_PRED ? p.aux : p.out, first, end);
 #pragma unroll
@@ -326,7 +345,11 @@ __device__ __forceinline__ void tile_epilogue(const MxProblem& p, const f32x16 (
       const float c[4] = {t4.x, t4.y, t4.z, t4.w};
       float o[4], x[4], ev[4];
       const unsigned here = at + (unsigned)(u * RPP) * (unsigned)p.N;
-      if constexpr (IN) Rows<ST, VEC>(KIND == KIND_PRED ? p.aux : p.out, first, end).widen(in[set][IN ? u : 0], here, x);
+      if constexpr (KIND == KIND_GRAD8) {
+        const float unit = int8_scale(in[set][u].v[1]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x[q] = (float)sext8(in[set][u].v[0], q) * unit;
+      } else if constexpr (IN) Rows<ST, VEC>(KIND == KIND_PRED ? p.aux : p.out, first, end).widen(in[set][IN ? u : 0], here, x);
       if constexpr (E) Rows<ST, VEC>(p.aux, first, end).widen(e[set][E ? u : 0], here, ev);
       finish4<KIND, ACT>(c, x, ev, p.scal, o);
       dst.put(here, left, o);

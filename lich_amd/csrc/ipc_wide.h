@@ -54,11 +54,9 @@ enum {
   // S16_INFER reading W_lower^T [M][K] and E_lower^T [B][K] (both
   // k-contiguous, lda = ldb = K): the transposed copies of a caller workspace
   S16_INFERT = 10,
-  // the state X kept in 8 bits (microscaled int8, ipc_mx.h): S16_WEIGHT8 reads
-  // its B operand there (b the codes, ldb their row bytes, aux the scales),
-  // S16_GRAD / S16_GRADT are S16_INFER / S16_INFERT writing G = f'(X) W_lower^T
-  // E_lower (aux the codes, ldx their row bytes, h the scales)
-  S16_WEIGHT8 = 11, S16_GRAD = 12, S16_GRADT = 13,
+  // S16_WEIGHT whose X is kept in 8 bits (microscaled int8, ipc_mx.h): b the codes,
+  // ldb their row bytes, aux the scales
+  S16_WEIGHT8 = 11,
 };
 
 inline long long wide_pad(long long v, long long m) { return (v + m - 1) / m * m; }
@@ -104,8 +102,8 @@ struct WideReduce {
   void* t; long long ldt;
   int vec;  // 1: part, x and eps rows allow 4-element vector access
 };
-// The modes for a state kept in 8 bits: 256 x 128 tiles (cfg 0) or 256 x 256 (cfg 3).
-hipError_t launch_s16_ckpt(int mode, const WideProblem& p, int operand, int act, int cfg, hipStream_t s);
+// S16_WEIGHT8 on 256 x 128 tiles (cfg 0) or 256 x 256 (cfg 3).
+hipError_t launch_s16_weight8(const WideProblem& p, int operand, int act, int cfg, hipStream_t s);
 hipError_t launch_wide_reduce(const WideReduce& r, int operand, hipStream_t s);
 
 // Configuration index of the 64 x 64 tiles, which the plan picks for launches

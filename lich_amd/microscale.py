@@ -231,27 +231,18 @@ class MXPredictKernel(_MXProduct):
                                            self.act, *self._ws(workspace), nat.current_stream_handle(out.device)))
 
 
-class _CheckpointKernel(_Kernel):
-    """A GEMM that reads a state kept in 8 bits."""
-
-    _phase = -1
-
-    @property
-    def workspace_bytes(self) -> int:
-        return int(nat.lib().ipc_ckpt_workspace_bytes(self._phase, self.act, self.M, self.K, self.B, self.storage))
-
-
-class CheckpointWeightUpdateKernel(_CheckpointKernel):
+class CheckpointWeightUpdateKernel(_Kernel):
     """``k(W[M, K], E[M, B], X8, *, workspace=None)``: ``W += alpha E f(X)^T``, X [K, B] kept
     in 8 bits.  ``workspace`` (optional, caller-owned, ``new_workspace()``) lets a
     large 16-bit call evaluate f(X) once."""
 
-    _phase = 2
+    workspace_bytes = 0
 
     def __init__(self, *a, alpha, **kw):
         super().__init__("weight", *a, **kw)
         self.alpha = float(alpha)
         self._x = _Packed("X", self.K, self.B, "int8")
+        self.workspace_bytes = int(nat.lib().ipc_ckpt_workspace_bytes(self.act, self.M, self.K, self.B, self.storage))
 
     def __call__(self, w, e, x8, *, workspace=None):
         w_at = _pointer(w, "W", (self.M, self.K), self.dtype)
@@ -262,24 +253,24 @@ class CheckpointWeightUpdateKernel(_CheckpointKernel):
             *self._ws(workspace), nat.current_stream_handle(w.device)))
 
 
-class CheckpointGradientKernel(_CheckpointKernel):
+class CheckpointGradientKernel(_Kernel):
     """``k(W_lower[K, M], E_lower[K, B], X8, G[M, B], *, workspace=None)``:
-    ``G = f'(X) W_lower^T E_lower``, X [M, B] kept in 8 bits."""
-
-    _phase = 1
+    ``G = f'(X) W_lower^T E_lower``, X [M, B] kept in 8 bits.  It uses no workspace
+    (``new_workspace()`` is None)."""
 
     def __init__(self, *a, **kw):
         super().__init__("gradient", *a, **kw)
         self._x = _Packed("X", self.M, self.B, "int8")
 
     def __call__(self, w_lower, e_lower, x8, g, *, workspace=None):
+        self._ws(workspace)
         w_lower_at = _pointer(w_lower, "W_lower", (self.K, self.M), self.dtype)
         e_lower_at = _pointer(e_lower, "E_lower", (self.K, self.B), self.dtype)
         x = self._x(x8)
         g_at = _pointer(g, "G", (self.M, self.B), self.dtype)
         nat.check(nat.lib().ipc_ckpt_gradient(
             w_lower_at, e_lower_at, *x, g_at, self.M, self.K, self.B, self.storage,
-            self.operand, self.act, *self._ws(workspace), nat.current_stream_handle(g.device)))
+            self.operand, self.act, nat.current_stream_handle(g.device)))
 
 
 @lru_cache(maxsize=256)

@@ -35,8 +35,8 @@ def _keep(x, storage):
 # (storage, operand, unit of the operand's rounding)
 TYPES = [("fp32", "fp32", 0.0), ("fp32", "bf16", 2.0 ** -8), ("fp32", "fp16", 2.0 ** -11), ("fp16", "fp16", 2.0 ** -11),
          ("bf16", "bf16", 2.0 ** -8)]
-# few tiles, odd lengths, the k-chunk kernel's rows of odd length, the LDS-DMA
-# kernel's 256 x 128 and 256 x 256 tiles with ragged edges, the tile kernel's (fp32 storage)
+# few tiles, odd lengths, the k-chunk kernel's rows of odd length, the 16-bit products'
+# and the LDS-DMA kernel's tiles with ragged edges, the tile kernel's (fp32 storage)
 SHAPES = [(1, 1, 1), (10, 64, 128), (64, 784, 128), (33, 31, 65), (100, 200, 1), (130, 257, 300), (1000, 1531, 300),
           (1100, 2050, 192), (4100, 4000, 64)]
 
@@ -63,7 +63,7 @@ def _weight(M, K, B, storage, operand, unit, act, lend=False):
     _close(wd, want, tol + O.UNIT[storage] * 1.01 * (want.abs() + tol) + 2.0 ** -25 * (storage == "fp16") + 2.0 ** -149)
 
 
-def _gradient(M, K, B, storage, operand, unit, act, lend=False):
+def _gradient(M, K, B, storage, operand, unit, act):
     g = torch.Generator().manual_seed(M + K + B + 1)
     x = _rand(g, M, B, storage=storage)
     w, e = _rand(g, K, M, size=0.1, storage=storage), _rand(g, K, B, size=0.1, storage=storage)
@@ -71,8 +71,8 @@ def _gradient(M, K, B, storage, operand, unit, act, lend=False):
     up, d = w.T.contiguous() @ e, O.df(act, xq)
     out = torch.full((M, B), 7.0, dtype=DT[storage], device="cuda")
     k = mx.build_checkpoint_gradient(M, K, B, act, DT[storage], operand_dtype=DT[operand])
-    ws = torch.empty(max(k.workspace_bytes, 16), dtype=torch.uint8, device="cuda") if lend else None
-    k(_dev(w, storage), _dev(e, storage), x8, out, workspace=ws)
+    assert k.new_workspace() is None
+    k(_dev(w, storage), _dev(e, storage), x8, out)
     size = w.T.abs().contiguous() @ e.abs()
     own = unit if storage == "fp32" else 0.0  # 16-bit tensors are operands as they are
     acc_tol = size * (2 * own + own * own + (K + 8) * 2.0 ** -23)
@@ -97,7 +97,7 @@ def test_weight_update_activations(M, K, B, storage, operand, unit, act):
 
 
 @pytest.mark.parametrize("storage,operand,unit", TYPES)
-@pytest.mark.parametrize("M,K,B", SHAPES + [(4100, 64, 4000), (2048, 1088, 1096)])
+@pytest.mark.parametrize("M,K,B", SHAPES + [(4104, 64, 4000), (2048, 1088, 1096), (72, 32, 8), (1000, 96, 1040)])
 def test_gradient(M, K, B, storage, operand, unit):
     _gradient(M, K, B, storage, operand, unit, "tanh")
 
@@ -107,6 +107,15 @@ def test_gradient(M, K, B, storage, operand, unit):
 @pytest.mark.parametrize("M,K,B", [(33, 31, 65), (2048, 192, 1096), (4104, 64, 4000)])
 def test_gradient_activations(M, K, B, storage, operand, unit, act):
     _gradient(M, K, B, storage, operand, unit, act)
+
+
+@pytest.mark.parametrize("storage,operand,unit", TYPES[3:])
+@pytest.mark.parametrize("M,K,B", [(1032, 1100, 32), (1100, 2050, 192), (4100, 4000, 64), (3000, 4104, 96)])
+def test_weight_update_widened_once(M, K, B, storage, operand, unit):
+    """The 16-bit products on 64, 128 and 256 wide tiles."""
+    k = mx.build_checkpoint_weight_update(M, K, B, "sigmoid", DT[storage])
+    assert k.workspace_bytes == 2 * K * B
+    _weight(M, K, B, storage, operand, unit, "sigmoid", lend=True)
 
 
 @pytest.mark.parametrize("storage", ["fp16", "bf16"])
@@ -119,10 +128,6 @@ def test_lent_workspaces(storage, act):
         assert lib.ipc_set_s16_preactivate(1) == 0
         for M, K, B in ((33, 31, 65), (1100, 2050, 192), (130, 257, 300)):
             _weight(M, K, B, storage, storage, unit, act, lend=True)
-        for M, K, B in ((2048, 192, 1096), (4104, 64, 4000)):
-            k = mx.build_checkpoint_gradient(M, K, B, act, DT[storage])
-            assert k.workspace_bytes == 2 * (M * K + K * B)
-            _gradient(M, K, B, storage, storage, unit, act, lend=True)
     finally:
         lib.ipc_set_s16_preactivate(-1)
 

@@ -62,15 +62,16 @@ def test_other_entry_points_validate():
     assert lib.ipc_mx_predict(P, P, P, P, 1, 1, (1 << 20) + 1, 0, 0, None, 0, None) == nat.ERR_SHAPE
     assert lib.ipc_mx_predict(P, P, P, P + 1, 1, 1, 1, 1, 0, None, 0, None) == nat.ERR_ALIGN
     assert lib.ipc_mx_predict(P, P, P, P, 1, 1, 2, 1, 0, P + 8, 4096, None) == nat.ERR_ALIGN
-    assert lib.ipc_mx_predict_workspace_bytes(200, 1, 0) == 0
-    assert lib.ipc_mx_predict_workspace_bytes(200, 3, 0) == 3 * 3 * 256 * 2
+    need = lib.ipc_mx_predict_workspace_bytes
+    assert need(200, 1, 0) == 0 and need(200, 4, 0) == 0 and need(0, 17, 2) == 0
+    assert need(200, 5, 0) == 3 * 5 * 256 * 2 and need(200, 17, 2) == 2 * 32 * 256 * 2
     assert lib.ipc_ckpt_weight_update(P, P, None, P, 64, 64, 64, 1e-4, 0, 0, 1, None, 0, None) == nat.ERR_NULL
     assert lib.ipc_ckpt_weight_update(P, P, P, P, 64, 64, 64, 1e-4, 1, 2, 1, None, 0, None) == nat.ERR_DTYPE
     assert lib.ipc_ckpt_weight_update(P, P, P, P, 64, 64, 64, 1e-4, 0, 0, 1, P + 8, 64, None) == nat.ERR_ALIGN
     assert lib.ipc_ckpt_weight_update(P, P, P, P, 64, 64, 64, 1e-4, 0, 0, 1, P, -1, None) == nat.ERR_SHAPE
-    assert lib.ipc_ckpt_gradient(P, P, P + 4, P, P, 64, 64, 64, 0, 0, 1, None, 0, None) == nat.ERR_ALIGN
-    assert lib.ipc_ckpt_gradient(P, P, P, P, None, 64, 64, 64, 0, 0, 1, None, 0, None) == nat.ERR_NULL
-    assert lib.ipc_ckpt_gradient(P, P, P, P, P, 1 << 24, 64, 1, 0, 0, 1, None, 0, None) == nat.ERR_SHAPE
+    assert lib.ipc_ckpt_gradient(P, P, P + 4, P, P, 64, 64, 64, 0, 0, 1, None) == nat.ERR_ALIGN
+    assert lib.ipc_ckpt_gradient(P, P, P, P, None, 64, 64, 64, 0, 0, 1, None) == nat.ERR_NULL
+    assert lib.ipc_ckpt_gradient(P, P, P, P, P, 1 << 24, 64, 1, 0, 0, 1, None) == nat.ERR_SHAPE
 
 
 def test_builders_refuse():
