@@ -8,8 +8,10 @@
     python -m lich_amd.cli thermal-bench [--seconds 120 --graph] [...]
     python -m lich_amd.cli steady-state [--dims 784 64 64 10] [...]
     python -m lich_amd.cli toolchain
+    python -m lich_amd.cli compact [--synthetic 4096] [--hidden 64 --depth 2] [...]
 
-Each subcommand takes the arguments of the reference script it replaces
+``compact`` (no counterpart in the reference) trains with 8-bit states and answers
+with 4-bit weights.  Each other subcommand takes the arguments of the reference script it replaces
 (``smoke.py``, ``validate_reference.py``, ``autotune.py``, ``train_mnist.py``,
 ``train_paper_efficiency.py``, ``thermal_bench.py``,
 ``benchmark_stage2_4_steady_state.py``, ``toolchain_probe.py``).  Differences:
@@ -367,6 +369,51 @@ def toolchain_main(argv=None) -> int:
     return 0
 
 
+# ------------------------------------------------------------------ compact
+def compact_main(argv=None) -> int:
+    """Back-propagation with the states kept in 8 bits, scored with the weights
+    in 4 (``lich_amd.compact``), then one sample answered, then iPC steps on
+    4-bit operands from the trained weights."""
+    from . import compact
+    from .kernels import build_forward
+
+    p = argparse.ArgumentParser(prog="lich_amd.cli compact")
+    p.add_argument("--data", default="./data")
+    p.add_argument("--dataset", choices=["MNIST", "FashionMNIST"], default="MNIST")
+    p.add_argument("--synthetic", type=int, default=0, help="train on N seeded synthetic samples instead")
+    p.add_argument("--subset", type=int, default=0)
+    p.add_argument("--hidden", type=int, default=64)
+    p.add_argument("--depth", type=int, default=2, help="number of hidden layers")
+    p.add_argument("--batch", type=int, default=128)
+    p.add_argument("--epochs", type=int, default=8)
+    p.add_argument("--rate", type=float, default=0.01)
+    p.add_argument("--steps", type=int, default=4, help="iPC steps on 4-bit operands at the end")
+    p.add_argument("--activation", default="tanh")
+    p.add_argument("--dtype", choices=["float16", "bfloat16", "float32"], default="float32")
+    p.add_argument("--seed", type=int, default=0)
+    a = p.parse_args(argv)
+    dtype = {"float16": torch.float16, "bfloat16": torch.bfloat16, "float32": torch.float32}[a.dtype]
+    dev, data = _device(), _dataset(a, a.subset)
+    _, net = compact.train(data, hidden=a.hidden, depth=a.depth, batch=a.batch, epochs=a.epochs, rate=a.rate,
+                           activation=a.activation, dtype=dtype, seed=a.seed)
+    images, labels = next(iter(data.batches(a.batch, shuffle=False)))
+    x = images.reshape(a.batch, -1).T.contiguous().to(dev)
+    one = net.predict(x[:, :1].contiguous())
+    print(f"first sample: class {int(one.float().argmax())}, labelled {int(labels[0])}", flush=True)
+    states = [x.to(dtype)]
+    for w in reversed(net.w):
+        states.insert(0, torch.empty((w.shape[0], a.batch), dtype=dtype, device=dev))
+        build_forward(*w.shape, a.batch, a.activation, dtype)(states[1], w, states[0])
+    states[0] = torch.nn.functional.one_hot(labels, data.num_classes).T.to(dev, dtype).contiguous()
+    steps = compact.FourBitSteps(states, [w.clone() for w in net.w], a.activation)
+    energies = []
+    for _ in range(a.steps):
+        steps.step()
+        energies.append(steps.energy())
+    print("4-bit iPC energies: " + " ".join(f"{v:.4f}" for v in energies), flush=True)
+    return 0
+
+
 def _autotune(argv):
     from .autotune import main
     return main(argv)
@@ -379,7 +426,7 @@ def _train(argv):
 
 COMMANDS = {"smoke": smoke_main, "reference": reference_main, "autotune": _autotune, "train-mnist": _train,
             "efficiency": efficiency_main, "thermal-bench": thermal_main, "steady-state": steady_main,
-            "toolchain": toolchain_main}
+            "toolchain": toolchain_main, "compact": compact_main}
 
 
 def main(argv=None) -> int:

@@ -39,6 +39,8 @@ long long predict_workspace_need(int K, int B, int storage) {
   return B > 4 ? mx_predict_terms_bytes(K, B, storage) : 0;
 }
 
+constexpr int kPredictMost = 16 * 65535;  // 16 samples per grid row
+
 int product(int kind, const void* a, const void* as, const char* a_name, const void* b, const void* bs,
             const char* b_name, void* out, const char* out_name, const void* aux, const char* aux_name, int M, int N,
             int K, float scal, int storage, int act, void* stream, const char* what) {
@@ -125,7 +127,7 @@ int ipc_mx_weight_update(void* w, const void* e_codes, const void* e_scales, con
 }
 
 long long ipc_mx_predict_workspace_bytes(int K, int B, int storage) {
-  if (K < 1 || B < 1 || B > (1 << 20) || storage < IPC_DT_F32 || storage > IPC_DT_BF16) return 0;
+  if (K < 1 || B < 1 || B > kPredictMost || storage < IPC_DT_F32 || storage > IPC_DT_BF16) return 0;
   return predict_workspace_need(K, B, storage);
 }
 
@@ -136,7 +138,7 @@ int ipc_mx_predict(const void* x, const void* w_codes, const void* w_scales, voi
   TRY(check_act(act));
   TRY(check_dims(M, K, B, 1));
   TRY(check_packed(M, K, IPC_MX_FP4));
-  if (B > (1 << 20)) return fail(IPC_ERR_SHAPE, "ipc_mx_predict takes at most 2^20 samples (got %d)", B);
+  if (B > kPredictMost) return fail(IPC_ERR_SHAPE, "ipc_mx_predict takes at most %d samples (got %d)", kPredictMost, B);
   TRY(check_ptr(x, "x", elem_size(storage)));
   TRY(check_codes(w_codes, w_scales, "w"));
   TRY(check_ptr(out, "out", elem_size(storage)));

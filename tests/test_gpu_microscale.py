@@ -202,9 +202,10 @@ def test_weight_update(M, K, B, storage):
     _close(wd, w + alpha * acc, alpha * bound + 2.0 ** -22 * (w.abs() + alpha * acc.abs()), storage)
 
 
-def test_a_nan_block_reaches_its_row_and_column_only():
+@pytest.mark.parametrize("M,K,B", [(70, 300, 90), (700, 300, 600), (2048, 300, 1600), (3000, 300, 3001)])
+def test_a_nan_block_reaches_its_row_and_column_only(M, K, B):
+    """The direct kernel and the three tiles."""
     g = torch.Generator().manual_seed(5)
-    M, K, B = 70, 300, 90
     w, x = _rand(g, M, K), _rand(g, B, K)
     w[3, 40] = float("inf")
     x[5, 299] = float("nan")
@@ -220,9 +221,9 @@ def test_a_nan_block_reaches_its_row_and_column_only():
     assert torch.equal(torch.isnan(out1).cpu(), want)
 
 
-def test_zero_rows_and_far_scales():
+@pytest.mark.parametrize("M,K,B", [(130, 130, 130), (700, 130, 600), (2048, 130, 1600), (3000, 130, 3001)])
+def test_zero_rows_and_far_scales(M, K, B):
     """Blocks of zeros, and scales at both ends of their range that cancel."""
-    M = K = B = 130
     w, x = torch.zeros(M, K, dtype=torch.float64), torch.zeros(B, K, dtype=torch.float64)
     w[1:] = 2.0 ** 90
     x[1:] = 2.0 ** -100

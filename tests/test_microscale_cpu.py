@@ -59,7 +59,7 @@ def test_other_entry_points_validate():
     assert lib.ipc_mx_infer_update(P, P, P, P, P, None, 64, 64, 64, 0.5, 0, 1, None) == nat.ERR_NULL
     assert lib.ipc_mx_infer_update(P, P, P, P, P, P, 64, 64, 64, 0.5, 0, 9, None) == nat.ERR_ACT
     assert lib.ipc_mx_weight_update(P, P, P, P, P, 64, 1 << 20, 1 << 20, 1e-4, 0, None) == nat.ERR_SHAPE
-    assert lib.ipc_mx_predict(P, P, P, P, 1, 1, (1 << 20) + 1, 0, 0, None, 0, None) == nat.ERR_SHAPE
+    assert lib.ipc_mx_predict(P, P, P, P, 1, 1, (1 << 20), 0, 0, None, 0, None) == nat.ERR_SHAPE
     assert lib.ipc_mx_predict(P, P, P, P + 1, 1, 1, 1, 1, 0, None, 0, None) == nat.ERR_ALIGN
     assert lib.ipc_mx_predict(P, P, P, P, 1, 1, 2, 1, 0, P + 8, 4096, None) == nat.ERR_ALIGN
     need = lib.ipc_mx_predict_workspace_bytes
