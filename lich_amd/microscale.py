@@ -22,6 +22,7 @@ synchronised inside a call.  The reference has no counterpart.
 """
 from __future__ import annotations
 
+from ctypes import c_float, c_int
 from functools import lru_cache
 from typing import NamedTuple
 
@@ -91,6 +92,20 @@ def _sizes(**sizes) -> None:
         raise ValueError("invalid shape " + " ".join(f"{k}={v}" for k, v in sizes.items()))
 
 
+def _entry(name: str, *constants):
+    """The call ``f(pointers, device index)`` of a library entry point whose arguments
+    are pointers, then these constants (converted once), then the stream."""
+    fn = getattr(nat.lib(), name)
+    constants = tuple(c_float(v) if isinstance(v, float) else c_int(v) for v in constants)
+
+    def call(pointers, device, *rest):
+        rc = fn(*pointers, *constants, *rest, nat.current_stream_handle(device))
+        if rc:
+            nat.check(rc)
+
+    return call
+
+
 class _MXKernel:
     def __init__(self, dtype, activation: str = "identity"):
         self.dtype = _storage_dtype(dtype)
@@ -110,16 +125,14 @@ class MXQuantizeKernel(_MXKernel):
         self.R, self.C, self.axis, self.format = int(R), int(C), int(axis), _format(format)
         self.rows, self.length = (self.R, self.C) if axis == 1 else (self.C, self.R)
         self._packed = _Packed("packed", self.rows, self.length, format)
+        self._call = _entry("ipc_mx_quantize", self.R, self.C, self.axis, nat.MX_FORMATS[format], self.storage, self.act)
 
     def new_output(self, device=None) -> MXMatrix:
         return self._packed.new(device)
 
     def __call__(self, x, packed):
         x_at = _pointer(x, "X", (self.R, self.C), self.dtype)
-        codes, scales = self._packed(packed)
-        nat.check(nat.lib().ipc_mx_quantize(x_at, codes, scales, self.R, self.C, self.axis,
-                                            nat.MX_FORMATS[self.format], self.storage, self.act,
-                                            nat.current_stream_handle(x.device)))
+        self._call((x_at, *self._packed(packed)), x.get_device())
 
 
 class MXDequantizeKernel(_MXKernel):
@@ -130,13 +143,12 @@ class MXDequantizeKernel(_MXKernel):
         _sizes(R=R, C=C)
         self.R, self.C, self.format = int(R), int(C), _format(format)
         self._packed = _Packed("packed", self.R, self.C, format)
+        self._call = _entry("ipc_mx_dequantize", self.R, self.C, nat.MX_FORMATS[format], self.storage)
 
     def __call__(self, packed, out):
-        codes, scales = self._packed(packed)
+        at = self._packed(packed)
         out_at = _pointer(out, "OUT", (self.R, self.C), self.dtype)
-        nat.check(nat.lib().ipc_mx_dequantize(codes, scales, out_at, self.R, self.C,
-                                              nat.MX_FORMATS[self.format], self.storage,
-                                              nat.current_stream_handle(out.device)))
+        self._call((*at, out_at), out.get_device())
 
 
 class _MXProduct(_MXKernel):
@@ -153,13 +165,13 @@ class MXPredictionErrorKernel(_MXProduct):
     def __init__(self, *a):
         super().__init__(*a)
         self._x, self._w = _Packed("X_upper", self.B, self.K), _Packed("W", self.M, self.K)
+        self._call = _entry("ipc_mx_pred_err", self.M, self.K, self.B, self.storage)
 
     def __call__(self, x4, w4, x_lower, e):
         x, w = self._x(x4), self._w(w4)
         x_lower_at = _pointer(x_lower, "X_lower", (self.M, self.B), self.dtype)
         e_at = _pointer(e, "E", (self.M, self.B), self.dtype)
-        nat.check(nat.lib().ipc_mx_pred_err(*x, *w, x_lower_at, e_at, self.M, self.K, self.B,
-                                            self.storage, nat.current_stream_handle(e.device)))
+        self._call((*x, *w, x_lower_at, e_at), e.get_device())
 
 
 class MXForwardKernel(_MXProduct):
@@ -168,12 +180,12 @@ class MXForwardKernel(_MXProduct):
     def __init__(self, *a):
         super().__init__(*a)
         self._x, self._w = _Packed("X_upper", self.B, self.K), _Packed("W", self.M, self.K)
+        self._call = _entry("ipc_mx_forward", self.M, self.K, self.B, self.storage)
 
     def __call__(self, x4, w4, out):
         x, w = self._x(x4), self._w(w4)
         out_at = _pointer(out, "OUT", (self.M, self.B), self.dtype)
-        nat.check(nat.lib().ipc_mx_forward(*x, *w, out_at, self.M, self.K, self.B, self.storage,
-                                           nat.current_stream_handle(out.device)))
+        self._call((*x, *w, out_at), out.get_device())
 
 
 class MXInferenceUpdateKernel(_MXProduct):
@@ -184,14 +196,13 @@ class MXInferenceUpdateKernel(_MXProduct):
         super().__init__(M, K, B, dtype, activation)
         self.gamma = float(gamma)
         self._w, self._e = _Packed("W_lower", self.M, self.K), _Packed("E_lower", self.B, self.K)
+        self._call = _entry("ipc_mx_infer_update", self.M, self.K, self.B, self.gamma, self.storage, self.act)
 
     def __call__(self, x, e, wt4, et4):
         x_at = _pointer(x, "X", (self.M, self.B), self.dtype)
         e_at = _pointer(e, "E", (self.M, self.B), self.dtype)
         w, el = self._w(wt4), self._e(et4)
-        nat.check(nat.lib().ipc_mx_infer_update(x_at, e_at, *w, *el, self.M, self.K, self.B,
-                                                self.gamma, self.storage, self.act,
-                                                nat.current_stream_handle(x.device)))
+        self._call((x_at, e_at, *w, *el), x.get_device())
 
 
 class MXWeightUpdateKernel(_MXProduct):
@@ -202,12 +213,12 @@ class MXWeightUpdateKernel(_MXProduct):
         super().__init__(M, K, B, dtype)
         self.alpha = float(alpha)
         self._e, self._a = _Packed("E", self.M, self.B), _Packed("A", self.K, self.B)
+        self._call = _entry("ipc_mx_weight_update", self.M, self.K, self.B, self.alpha, self.storage)
 
     def __call__(self, w, e4, a4):
         w_at = _pointer(w, "W", (self.M, self.K), self.dtype)
         e, a = self._e(e4), self._a(a4)
-        nat.check(nat.lib().ipc_mx_weight_update(w_at, *e, *a, self.M, self.K, self.B, self.alpha,
-                                                 self.storage, nat.current_stream_handle(w.device)))
+        self._call((w_at, *e, *a), w.get_device())
 
 
 class MXPredictKernel(_MXProduct):
@@ -218,7 +229,7 @@ class MXPredictKernel(_MXProduct):
     def __init__(self, M, K, B, activation, dtype):
         super().__init__(M, K, B, dtype, activation)
         self._w = _Packed("W", self.M, self.K)
-
+        self._call = _entry("ipc_mx_predict", self.M, self.K, self.B, self.storage, self.act)
         self.workspace_bytes = int(nat.lib().ipc_mx_predict_workspace_bytes(self.K, self.B, self.storage))
 
     new_workspace, _ws = _Kernel.new_workspace, staticmethod(_Kernel._ws)
@@ -227,8 +238,7 @@ class MXPredictKernel(_MXProduct):
         x_at = _pointer(x, "X", (self.K, self.B), self.dtype)
         w = self._w(w4)
         out_at = _pointer(out, "OUT", (self.M, self.B), self.dtype)
-        nat.check(nat.lib().ipc_mx_predict(x_at, *w, out_at, self.M, self.K, self.B, self.storage,
-                                           self.act, *self._ws(workspace), nat.current_stream_handle(out.device)))
+        self._call((x_at, *w, out_at), out.get_device(), *self._ws(workspace))
 
 
 class CheckpointWeightUpdateKernel(_Kernel):
@@ -242,15 +252,13 @@ class CheckpointWeightUpdateKernel(_Kernel):
         super().__init__("weight", *a, **kw)
         self.alpha = float(alpha)
         self._x = _Packed("X", self.K, self.B, "int8")
+        self._call = _entry("ipc_ckpt_weight_update", self.M, self.K, self.B, self.alpha, self.storage, self.operand, self.act)
         self.workspace_bytes = int(nat.lib().ipc_ckpt_workspace_bytes(self.act, self.M, self.K, self.B, self.storage))
 
     def __call__(self, w, e, x8, *, workspace=None):
         w_at = _pointer(w, "W", (self.M, self.K), self.dtype)
         e_at = _pointer(e, "E", (self.M, self.B), self.dtype)
-        x = self._x(x8)
-        nat.check(nat.lib().ipc_ckpt_weight_update(
-            w_at, e_at, *x, self.M, self.K, self.B, self.alpha, self.storage, self.operand, self.act,
-            *self._ws(workspace), nat.current_stream_handle(w.device)))
+        self._call((w_at, e_at, *self._x(x8)), w.get_device(), *self._ws(workspace))
 
 
 class CheckpointGradientKernel(_Kernel):
@@ -261,6 +269,7 @@ class CheckpointGradientKernel(_Kernel):
     def __init__(self, *a, **kw):
         super().__init__("gradient", *a, **kw)
         self._x = _Packed("X", self.M, self.B, "int8")
+        self._call = _entry("ipc_ckpt_gradient", self.M, self.K, self.B, self.storage, self.operand, self.act)
 
     def __call__(self, w_lower, e_lower, x8, g, *, workspace=None):
         self._ws(workspace)
@@ -268,9 +277,7 @@ class CheckpointGradientKernel(_Kernel):
         e_lower_at = _pointer(e_lower, "E_lower", (self.K, self.B), self.dtype)
         x = self._x(x8)
         g_at = _pointer(g, "G", (self.M, self.B), self.dtype)
-        nat.check(nat.lib().ipc_ckpt_gradient(
-            w_lower_at, e_lower_at, *x, g_at, self.M, self.K, self.B, self.storage,
-            self.operand, self.act, nat.current_stream_handle(g.device)))
+        self._call((w_lower_at, e_lower_at, *x, g_at), g.get_device())
 
 
 @lru_cache(maxsize=256)
