@@ -568,7 +568,7 @@ long long ipc_mx_predict_workspace_bytes(int K, int B, int storage);
  *                           W_lower [K][M], E_lower [K][B], X and G [M][B]
  * storage, operand: as for ipc_weight_update and ipc_infer_update; the state is
  * widened in the kernels, exactly where the operand type is fp32 or bf16.  Larger
- * 16-bit weight updates use a workspace lent by the caller (16-byte aligned,
+ * weight updates use a workspace lent by the caller (16-byte aligned,
  * ipc_ckpt_workspace_bytes bytes, 0: none), into which f(X) is widened once.
  */
 int ipc_ckpt_weight_update(void* w, const void* e, const void* x_codes, const void* x_scales, int M, int K, int B,

@@ -644,12 +644,26 @@ bool ckpt_products(int storage, int k, std::initializer_list<const void*> operan
   return rows_a * lda < (1LL << 30) && rows_b * ldb < (1LL << 30);
 }
 
-// The weight update's workspace: f(X) widened once to the storage type, for the
-// 16-bit products where there are outputs enough for them to win against the
-// kernels that widen in their loaders, or (lengths those products cannot take)
-// where evaluating f in every row tile costs more than that pass.
+// Whether ipc_ckpt_gemm32.h can run a call of fp32 operands of these sizes.
+bool ckpt_products32(int storage, int operand, int M, int K, int B) {
+  const long long limit = 1LL << 29;
+  return storage == IPC_DT_F32 && operand == IPC_DT_F32 && (long long)M * K < limit && (long long)M * B < limit &&
+         (long long)K * B < limit - (long long)K * 32;
+}
+
+// The weight update's workspace: f(X) widened once to the storage type.
+// fp32: evaluating it in every row of tiles costs more than that pass (5-8 us): MI355X,
+// us, from codes / widened and read (relu; silu): 512^3 6.9; 10.3 / 6.2 + 4, 1000 x 1531 x
+// 300 16.9; 25.3 / 15.9 + 4, 2048 x 1024 x 1024 45; 87 / 41 + 5, 2048^3 162; 333 / 137 + 7.
+// 16 bits: for the 16-bit products where there are outputs enough for them to win
+// against the kernels that widen in their loaders, or (lengths those products cannot
+// take) by the same comparison.
 long long ckpt_workspace_need(int act, int M, int K, int B, int storage) {
-  if (storage == IPC_DT_F32) return 0;
+  if (storage == IPC_DT_F32) {
+    const bool cheap = act == IPC_ACT_IDENTITY || act == IPC_ACT_RELU;
+    if (!ckpt_products32(storage, IPC_DT_F32, M, K, B) || (double)M * K * B < (cheap ? 0x1p32 : 0x1p27)) return 0;
+    return K * mx_row_values(MX_INT8, B) * 4;
+  }
   const bool products = ckpt_products(storage, B, {}, M, B, K, B) && (long long)M * K > (1 << 20);
   return products || s16_preact_rule(S16_WEIGHT, act, M, K, (long long)K * B) ? (long long)K * B * 2 : 0;
 }
@@ -681,7 +695,22 @@ int ipc_ckpt_weight_update(void* w, const void* e, const void* x_codes, const vo
   TRY(check_ptr(e, "e", es));
   hipStream_t s = (hipStream_t)stream;
   const long long need = ckpt_workspace_need(act, M, K, B, storage);
-  if (need > 0 && workspace && workspace_bytes >= need) {
+  const bool lent = need > 0 && workspace && workspace_bytes >= need;
+  if (ckpt_products32(storage, operand, M, K, B)) {
+    CkptProblem q{};
+    q.M = M; q.N = K; q.K = B;
+    q.a = e; q.lda = B;
+    q.x = x_codes; q.xs = x_scales; q.x_row = (int)mx_row_bytes(MX_INT8, B);
+    if (lent) {  // (rows padded as the packed ones are)
+      const int n = (int)mx_row_values(MX_INT8, B);
+      TRY(launch_rc(launch_mx_dequantize(x_codes, x_scales, workspace, K, n, MX_INT8, storage, act, s), "ipc_ckpt_weight_update"));
+      q.b = workspace; q.ldb = n;
+    }
+    q.out = w; q.alpha = alpha;
+    q.vec = vec_ok(w, K, es);
+    return launch_rc(launch_ckpt_gemm32(CKPT_WEIGHT, q, act, s), "ipc_ckpt_weight_update");
+  }
+  if (lent && storage != IPC_DT_F32) {
     TRY(launch_rc(launch_mx_dequantize(x_codes, x_scales, workspace, K, B, MX_INT8, storage, act, s),
                   "ipc_ckpt_weight_update"));
     if (!ckpt_products(storage, B, {e}, M, B, K, B))
@@ -732,6 +761,16 @@ int ipc_ckpt_gradient(const void* w_lower, const void* e_lower, const void* x_co
     q.out = g;
     q.vec = vec_ok(g, B, es);
     return launch_rc(launch_ckpt_gemm(CKPT_GRAD, q, operand, act, s), "ipc_ckpt_gradient");
+  }
+  if (ckpt_products32(storage, operand, M, K, B)) {
+    CkptProblem q{};
+    q.M = M; q.N = B; q.K = K;
+    q.a = w_lower; q.lda = M;
+    q.b = e_lower; q.ldb = B;
+    q.x = x_codes; q.xs = x_scales; q.x_row = (int)mx_row_bytes(MX_INT8, B);
+    q.out = g;
+    q.vec = vec_ok(g, B, es);
+    return launch_rc(launch_ckpt_gemm32(CKPT_GRAD, q, act, s), "ipc_ckpt_gradient");
   }
   GemmProblem p = make_inf(g, x_codes, w_lower, e_lower, nullptr, M, K, B, 1, 0.0f, act, es);
   p.ldx = mx_row_bytes(MX_INT8, B);

@@ -83,14 +83,17 @@ struct CkptProblem {
   int M, N, K;
   const void* a; long long lda;  // elements
   const void* b; long long ldb;
-  const void* x;                 // CKPT_GRAD: codes, scales and row bytes of X [M][N]
+  const void* x;                 // codes, scales and row bytes of X (CKPT_GRAD: [M][N])
   const void* xs;
   int x_row;
-  void* out;                     // [M][N], 16-bit
+  void* out;                     // [M][N]
   float alpha;
   int vec;                       // out allows 4-element accesses
 };
 enum { CKPT_GRAD = 0, CKPT_WEIGHT = 1 };
 hipError_t launch_ckpt_gemm(int mode, const CkptProblem& p, int operand, int act, hipStream_t s);
+// On fp32 operands (ipc_ckpt_gemm32.h): rows of any length, operands below 2^31 bytes.
+// CKPT_WEIGHT: b = f(X) in fp32, or nullptr: X from its codes x, xs, x_row.
+hipError_t launch_ckpt_gemm32(int mode, const CkptProblem& p, int act, hipStream_t s);
 
 }  // namespace ipc

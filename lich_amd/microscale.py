@@ -244,7 +244,7 @@ class MXPredictKernel(_MXProduct):
 class CheckpointWeightUpdateKernel(_Kernel):
     """``k(W[M, K], E[M, B], X8, *, workspace=None)``: ``W += alpha E f(X)^T``, X [K, B] kept
     in 8 bits.  ``workspace`` (optional, caller-owned, ``new_workspace()``) lets a
-    large 16-bit call evaluate f(X) once."""
+    large call evaluate f(X) once."""
 
     workspace_bytes = 0
 

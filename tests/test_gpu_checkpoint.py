@@ -118,6 +118,56 @@ def test_weight_update_widened_once(M, K, B, storage, operand, unit):
     _weight(M, K, B, storage, operand, unit, "sigmoid", lend=True)
 
 
+@pytest.mark.parametrize("act", ["identity", "relu", "tanh", "sigmoid"])
+@pytest.mark.parametrize("M,K,B", [(300, 300, 4001), (1100, 2050, 192), (4100, 4000, 65), (4000, 4104, 300), (1000, 1531, 300)])
+def test_fp32_weight_update(M, K, B, act):
+    """fp32 products on 32, 64 and 128 wide tiles, the contraction's rests of 1 to 16, f(X)
+    widened once where the call asks for it and from the codes."""
+    k = mx.build_checkpoint_weight_update(M, K, B, act)
+    padded = 4 * K * (-(-B // 32) * 32)
+    assert k.workspace_bytes == (padded if M * K * B >= 2 ** (27 if act in ACTS[2:] else 32) else 0)
+    for lend in (False, True):
+        _weight(M, K, B, "fp32", "fp32", 0.0, act, lend=lend)
+
+
+@pytest.mark.parametrize("M,K,B", [(65, 1, 65), (1, 4000, 1), (31, 16, 33), (1531, 1000, 300), (2050, 1100, 1000),
+                                   (4001, 333, 4099), (4001, 17, 4099)])
+def test_fp32_gradient(M, K, B):
+    _gradient(M, K, B, "fp32", "fp32", 0.0, "silu")
+
+
+@pytest.mark.parametrize("storage,operand,unit", TYPES)
+@pytest.mark.parametrize("M,K,B", [(37, 50, 45), (40, 64, 72), (600, 1500, 1100), (1100, 2050, 190)])
+def test_not_a_number_stays_in_its_place(M, K, B, storage, operand, unit):
+    """A load that reaches into the next row, or clears what a stage lacks, touches no
+    other output."""
+    g = torch.Generator().manual_seed(M)
+    w, e = _rand(g, M, K, size=0.1, storage=storage), _rand(g, M, B, size=0.1, storage=storage)
+    x = _rand(g, K, B, storage=storage)
+    x8, _ = _keep(x, storage)
+    nan, bad = float("nan"), float("inf")
+    grad = mx.build_checkpoint_gradient(K, M, B, "tanh", DT[storage], operand_dtype=DT[operand])
+    plain, hit = (torch.empty((K, B), dtype=DT[storage], device="cuda") for _ in range(2))
+    grad(_dev(w, storage), _dev(e, storage), x8, plain)
+    w2, e2 = w.clone(), e.clone()
+    w2[:, 0] = nan
+    e2[:, 0] = bad
+    grad(_dev(w2, storage), _dev(e2, storage), x8, hit)
+    assert bool(hit[0].isnan().all()) and bool((~hit[:, 0].isfinite()).all())
+    assert torch.equal(hit[1:, 1:], plain[1:, 1:])
+    update = mx.build_checkpoint_weight_update(M, K, B, "tanh", DT[storage], 0.01, operand_dtype=DT[operand])
+    ws = torch.empty(max(update.workspace_bytes, 16), dtype=torch.uint8, device="cuda")
+    e2 = e.clone()
+    e2[5] = nan
+    for lent in (None, ws):
+        plain, hit = _dev(w, storage), _dev(w, storage)
+        update(plain, _dev(e, storage), x8, workspace=lent)
+        update(hit, _dev(e2, storage), x8, workspace=lent)
+        assert bool(hit[5].isnan().all())
+        keep = torch.arange(M, device="cuda") != 5
+        assert torch.equal(hit[keep], plain[keep])
+
+
 @pytest.mark.parametrize("storage", ["fp16", "bf16"])
 @pytest.mark.parametrize("act", ["identity", "relu", "tanh", "gelu"])
 def test_lent_workspaces(storage, act):
