@@ -48,7 +48,7 @@ class CompactNet:
         self._update = [mx.build_checkpoint_weight_update(d[l], d[l + 1], B, activation, dtype, float(rate) / B)
                         for l in range(L)]
         self.kept = [k.new_output(self.device) for k in self._save]  # x[l + 1] of layer l
-        most = max((k.workspace_bytes for k in self._update), default=0)
+        most = max((k.workspace_bytes for k in self._update + self._gradient), default=0)
         self._workspace = torch.empty(most, dtype=torch.uint8, device=self.device) if most else None
         self.w4 = None
 
@@ -69,7 +69,7 @@ class CompactNet:
             below = None
             if l + 1 < len(self.w):  # before W[l] changes
                 below = self._state(self.dims[l + 1], self.batch)
-                self._gradient[l](self.w[l], e, self.kept[l], below)
+                self._gradient[l](self.w[l], e, self.kept[l], below, workspace=self._workspace)
             self._update[l](self.w[l], e, self.kept[l], workspace=self._workspace)
             e = below
         return error

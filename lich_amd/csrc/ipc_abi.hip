@@ -634,15 +634,13 @@ int check_state(const void* codes, const void* scales, int rows, int n) {
   return ok();
 }
 
-// Whether the 16-bit products of ipc_ckpt_gemm.h can run a call: operands of
-// `rows_a` rows of lda and `rows_b` of ldb elements, contraction k.
-bool ckpt_products(int storage, int k, std::initializer_list<const void*> operands, long long rows_a, long long lda,
-                   long long rows_b, long long ldb) {
-  if (storage == IPC_DT_F32 || k % 32 != 0 || lda % 8 != 0 || ldb % 8 != 0) return false;
-  for (const void* q : operands)
-    if (!al16(q)) return false;
-  return rows_a * lda < (1LL << 30) && rows_b * ldb < (1LL << 30);
+// Whether the 16-bit products of ipc_ckpt_gemm.h can run a call of these sizes (rows
+// padded to a multiple of 32 for those of an odd length).
+bool ckpt_products(int storage, int M, int K, int B) {
+  const long long limit = 1LL << 30, m = M + 32LL, k = K + 32LL, b = B + 32LL;
+  return storage != IPC_DT_F32 && m * k < limit && m * b < limit && k * b < limit;
 }
+bool al4(const void* q) { return reinterpret_cast<uintptr_t>(q) % 4 == 0; }
 
 // Whether ipc_ckpt_gemm32.h can run a call of fp32 operands of these sizes.
 bool ckpt_products32(int storage, int operand, int M, int K, int B) {
@@ -664,8 +662,21 @@ long long ckpt_workspace_need(int act, int M, int K, int B, int storage) {
     if (!ckpt_products32(storage, IPC_DT_F32, M, K, B) || (double)M * K * B < (cheap ? 0x1p32 : 0x1p27)) return 0;
     return K * mx_row_values(MX_INT8, B) * 4;
   }
-  const bool products = ckpt_products(storage, B, {}, M, B, K, B) && (long long)M * K > (1 << 20);
-  return products || s16_preact_rule(S16_WEIGHT, act, M, K, (long long)K * B) ? (long long)K * B * 2 : 0;
+  const long long padded = mx_row_values(MX_INT8, B);
+  if (ckpt_products(storage, M, K, B) && (long long)M * K > (1 << 20)) return (K + (B % 2 ? (long long)M : 0LL)) * padded * 2;
+  return s16_preact_rule(S16_WEIGHT, act, M, K, (long long)K * B) ? (long long)K * B * 2 : 0;
+}
+
+// The state gradient's: rows of an odd length of W_lower [K][M] and E_lower [K][B] padded to
+// a multiple of 8 values, where that pass costs less than the 16-bit products save.  MI355X,
+// bf16, us, without / with (M x K x B): 4095 x 4093 x 1021 138 / 59, 1531 x 1000 x 300 26 / 15,
+// 4095 x 255 x 511 17 / 14; 511^3 10 / 13, 2001 x 2001 x 33 21 / 24, 8191 x 8191 x 111 88 / 108.
+bool ckpt_gradient_pads(int M, int K, int B) {
+  return (M % 2 || B % 2) && (double)M * K * B >= 0x1p28 && (M % 2 == 0 || B >= 256);
+}
+long long ckpt_gradient_need(int M, int K, int B, int storage) {
+  if (!ckpt_products(storage, M, K, B) || !ckpt_gradient_pads(M, K, B)) return 0;
+  return ((M % 2 ? K * ((M + 7LL) / 8 * 8) : 0) + (B % 2 ? K * ((B + 7LL) / 8 * 8) : 0)) * 2;
 }
 
 // Tile of a call on the generic kernels (their rules, for a problem of its size).
@@ -710,18 +721,23 @@ int ipc_ckpt_weight_update(void* w, const void* e, const void* x_codes, const vo
     q.vec = vec_ok(w, K, es);
     return launch_rc(launch_ckpt_gemm32(CKPT_WEIGHT, q, act, s), "ipc_ckpt_weight_update");
   }
-  if (lent && storage != IPC_DT_F32) {
-    TRY(launch_rc(launch_mx_dequantize(x_codes, x_scales, workspace, K, B, MX_INT8, storage, act, s),
-                  "ipc_ckpt_weight_update"));
-    if (!ckpt_products(storage, B, {e}, M, B, K, B))
-      return ipc_weight_update(w, e, workspace, M, K, B, 1, alpha, 0, storage, operand, act, IPC_TILE_AUTO, stream);
+  const bool products = ckpt_products(storage, M, K, B) && (long long)M * K > (1 << 20);
+  if (lent && products && (B % 2 || al4(e))) {  // (rows padded as the packed ones are)
+    const int n = (int)mx_row_values(MX_INT8, B);
+    void* pad = static_cast<char*>(workspace) + (long long)K * n * 2;
+    TRY(launch_rc(launch_mx_dequantize(x_codes, x_scales, workspace, K, n, MX_INT8, storage, act, s), "ipc_ckpt_weight_update"));
+    if (B % 2) TRY(launch_rc(launch_ckpt_pad(e, pad, M, B, n, nullptr, nullptr, 0, 0, 0, s), "ipc_ckpt_weight_update"));
     CkptProblem q{};
     q.M = M; q.N = K; q.K = B;
-    q.a = e; q.lda = B;
-    q.b = workspace; q.ldb = B;
+    q.a = B % 2 ? pad : e; q.lda = B % 2 ? n : B;
+    q.b = workspace; q.ldb = n;
     q.out = w; q.alpha = alpha;
     q.vec = vec_ok(w, K, es);
     return launch_rc(launch_ckpt_gemm(CKPT_WEIGHT, q, operand, act, s), "ipc_ckpt_weight_update");
+  }
+  if (lent && !products && storage != IPC_DT_F32) {
+    TRY(launch_rc(launch_mx_dequantize(x_codes, x_scales, workspace, K, B, MX_INT8, storage, act, s), "ipc_ckpt_weight_update"));
+    return ipc_weight_update(w, e, workspace, M, K, B, 1, alpha, 0, storage, operand, act, IPC_TILE_AUTO, stream);
   }
   GemmProblem p = make_wgt(w, e, x_codes, M, K, B, 1, alpha, 1, act, es);
   p.ldb = mx_row_bytes(MX_INT8, B);
@@ -741,8 +757,15 @@ int ipc_ckpt_weight_update(void* w, const void* e, const void* x_codes, const vo
   return launch_rc(launch_ckpt_weight(p, storage, operand, ckpt_tile(p, storage, operand), s), "ipc_ckpt_weight_update");
 }
 
+long long ipc_ckpt_gradient_workspace_bytes(int M, int K, int B, int storage) {
+  if (M < 1 || K < 1 || B < 1) return 0;
+  return ckpt_gradient_need(M, K, B, storage);
+}
+
 int ipc_ckpt_gradient(const void* w_lower, const void* e_lower, const void* x_codes, const void* x_scales, void* g,
-                      int M, int K, int B, int storage, int operand, int act, void* stream) {
+                      int M, int K, int B, int storage, int operand, int act, void* workspace,
+                      long long workspace_bytes, void* stream) {
+  TRY(check_workspace(workspace, workspace_bytes));
   TRY(check_dtypes(storage, operand));
   TRY(check_act(act));
   TRY(check_dims(M, K, B, 1));
@@ -752,11 +775,19 @@ int ipc_ckpt_gradient(const void* w_lower, const void* e_lower, const void* x_co
   TRY(check_ptr(e_lower, "e_lower", es));
   TRY(check_ptr(g, "g", es));
   hipStream_t s = (hipStream_t)stream;
-  if (ckpt_products(storage, K, {w_lower, e_lower}, K, M, K, B)) {
+  const long long need = ckpt_gradient_need(M, K, B, storage);
+  const bool even = M % 2 == 0 && B % 2 == 0, lent = need > 0 && workspace && workspace_bytes >= need;
+  if (ckpt_products(storage, M, K, B) && (even || lent) && (M % 2 || al4(w_lower)) && (B % 2 || al4(e_lower))) {
+    const int lda = M % 2 ? (M + 7) / 8 * 8 : M, ldb = B % 2 ? (B + 7) / 8 * 8 : B;
+    char* pw = static_cast<char*>(workspace);
+    char* pe = M % 2 ? pw + (long long)K * lda * 2 : pw;
+    if (!even)
+      TRY(launch_rc(launch_ckpt_pad(M % 2 ? w_lower : nullptr, pw, K, M, lda, B % 2 ? e_lower : nullptr, pe, K, B, ldb, s),
+                    "ipc_ckpt_gradient"));
     CkptProblem q{};
     q.M = M; q.N = B; q.K = K;
-    q.a = w_lower; q.lda = M;
-    q.b = e_lower; q.ldb = B;
+    q.a = M % 2 ? pw : w_lower; q.lda = lda;
+    q.b = B % 2 ? pe : e_lower; q.ldb = ldb;
     q.x = x_codes; q.xs = x_scales; q.x_row = (int)mx_row_bytes(MX_INT8, B);
     q.out = g;
     q.vec = vec_ok(g, B, es);

@@ -10,12 +10,16 @@
 // current products run.  A 16-bit product does a quarter of the fp4 one's work per
 // byte in the same time, so the same tile keeps the matrix units as busy.
 //
+//   * loads take 16 bytes a lane from any multiple of 4 bytes; where a row ends inside one
+//     they bring the next row's first values, which no stored output reads.  The last
+//     1 .. 32 k come first, as a stage whose rest is cleared before anything is read.
+//     Rows of an odd length are laid out once in a workspace (ckpt_pad_kernel);
 //   * k-contiguous rows: chunk c (16 bytes) of row r at c ^ ((r >> 2) & 3), fragments
 //     are 16-byte reads;
 //   * k-rows (CKPT_GRAD): chunk c of k-row r at c ^ ((r & 3) << 2) (64 columns: ^ ((r & 2)
 //     << 1)), fragments come from
 //     two transposing reads (ds_read_b64_tr_b16), the operands are never transposed in
-//     memory;
+//     memory.
 //
 // Reading the packed state in the weight update's own loader instead (codes to
 // registers, widened a step or two later, stored to the stage) was slower than
@@ -78,18 +82,19 @@ __global__ void __launch_bounds__(WGM * WGN * 64) ckpt_gemm_kernel(const CkptPro
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = w / WGN, wn = w % WGN, lr = lane & 31, lk = lane >> 5;
-  const int M = p.M, N = p.N, G = p.K / 32;  // (the host: K a multiple of 32, operands below 2^31 bytes)
+  // (the host: operands below 2^31 bytes, rows that start at multiples of 4)
+  const int M = p.M, N = p.N, K = p.K, G = (K + 31) / 32, tail = K - (G - 1) * 32;
 
   const Rsrc ga(p.a, (unsigned)((MN ? (long long)p.K : (long long)M) * p.lda * 2));
   const Rsrc gb(p.b, (unsigned)((MN ? (long long)p.K : (long long)N) * p.ldb * 2));
   const i32x4 wa = rsrc_words(p.a, (unsigned)((long long)p.K * p.lda * 2)), wb = rsrc_words(p.b, (unsigned)((long long)p.K * p.ldb * 2));
-  // byte offset of this lane's 16 bytes of LDS-DMA instruction q of an operand (stage 0)
-  auto source = [&](int q, int edge, int e0, int lim, long long ld) -> unsigned {
+  // byte offset of this lane's 16 bytes of LDS-DMA instruction q of an operand, `have` k-rows in the stage
+  auto source = [&](int q, int edge, int e0, int lim, long long ld, int have) -> unsigned {
     const int slot = (q * NW + w) * 64 + lane;
-    if constexpr (MN) {  // columns past the end: the last 8 again, never stored
+    if constexpr (MN) {  // columns past the end: the last ones again or the next row's, never stored
       const int cpr = edge / 8, r = slot / cpr, c = (slot % cpr) ^ (edge == 64 ? (r & 2) << 1 : (r & 3) << 2);
-      const int col = e0 + c * 8 <= lim - 8 ? e0 + c * 8 : lim - 8;
-      return (unsigned)(r * ld + col) * 2u;
+      const int col = e0 + c * 8 < (int)ld ? e0 + c * 8 : (int)ld - 2;
+      return (unsigned)((r < have ? r : have - 1) * ld + col) * 2u;
     } else {
       const int r = slot >> 2, c = (slot & 3) ^ ((r >> 2) & 3), row = e0 + r < lim ? e0 + r : lim - 1;
       return (unsigned)(row * ld) * 2u + (unsigned)c * 16u;
@@ -97,19 +102,15 @@ __global__ void __launch_bounds__(WGM * WGN * 64) ckpt_gemm_kernel(const CkptPro
   };
   unsigned oa[IA], ob[IB];
 #pragma unroll
-  for (int q = 0; q < IA; ++q) oa[q] = source(q, BM, m0, M, p.lda);
+  for (int q = 0; q < IA; ++q) oa[q] = source(q, BM, m0, M, p.lda, 32);
 #pragma unroll
-  for (int q = 0; q < IB; ++q) ob[q] = source(q, BN, n0, N, p.ldb);
-  const unsigned step_a = MN ? (unsigned)p.lda * 64u : 64u, step_b = MN ? (unsigned)p.ldb * 64u : 64u;
-  auto load = [&](int q, int kt, unsigned char* st) {
-    if constexpr (MN) {
-      if (q < IA) to_lds16_unseen(wa, st + (q * NW + w) * 1024, oa[q < IA ? q : 0], (unsigned)kt * step_a);
-      else to_lds16_unseen(wb, st + A_BYTES + ((q - IA) * NW + w) * 1024, ob[q >= IA && q - IA < IB ? q - IA : 0], (unsigned)kt * step_b);
-    } else if (q < IA) {
-      ga.to_lds16(st + (q * NW + w) * 1024, oa[q < IA ? q : 0], (unsigned)kt * step_a);
-    } else if (q < IA + IB) {
-      gb.to_lds16(st + A_BYTES + ((q - IA) * NW + w) * 1024, ob[q >= IA && q - IA < IB ? q - IA : 0], (unsigned)kt * step_b);
-    }
+  for (int q = 0; q < IB; ++q) ob[q] = source(q, BN, n0, N, p.ldb, 32);
+  const unsigned step_a = MN ? (unsigned)p.lda * 2u : 2u, step_b = MN ? (unsigned)p.ldb * 2u : 2u;
+  // load q of a stage: lane offset v, uniform offsets sa, sb
+  auto load = [&](int q, unsigned char* st, unsigned v, unsigned sa, unsigned sb) {
+    unsigned char* at = q < IA ? st + (q * NW + w) * 1024 : st + A_BYTES + ((q - IA) * NW + w) * 1024;
+    if constexpr (MN) to_lds16_unseen(q < IA ? wa : wb, at, v, q < IA ? sa : sb);
+    else (q < IA ? ga : gb).to_lds16(at, v, q < IA ? sa : sb);
   };
 
   f32x16 acc[RM][RN];
@@ -136,16 +137,44 @@ __global__ void __launch_bounds__(WGM * WGN * 64) ckpt_gemm_kernel(const CkptPro
   };
   V fa[2][RM], fb[2][RN];
   auto stage = [&](int kt) -> unsigned char* { return smem + (kt & (STAGES - 1)) * STAGE; };
-  auto group = [&](int kt) { return kt < G ? kt : G - 1; };  // (past the end: the last again, so that every step counts the same)
 
-  // prologue: stages 0 .. 2
+  // prologue: stages 0 .. 2.  The last 1 .. 32 k are stage 0; a load that reaches past
+  // the operand's end there has all of its offset in the lane's, which is checked.
+  if (G == 1) {  // (no other stage: its loads take the operands' first values)
 #pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s)
+    for (int q = 0; q < IA; ++q) oa[q] = 0;
 #pragma unroll
-    for (int q = 0; q < LPS; ++q) load(q, group(s), stage(s));
+    for (int q = 0; q < IB; ++q) ob[q] = 0;
+  }
+  // first k of stage kt > 0; past the end: of the last, so that every step counts the same
+  auto k_of = [&](int kt) { return (unsigned)(G == 1 ? 0 : (kt < G ? kt : G - 1) - 1) * 32u; };
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) {
+    const unsigned k = s > 0 ? k_of(s) : 0u, last = (unsigned)(K - tail);
+#pragma unroll
+    for (int q = 0; q < LPS; ++q) {
+      unsigned v = q < IA ? oa[q < IA ? q : 0] : ob[q < IA ? 0 : q - IA];
+      if (s == 0) v = q < IA ? source(q, BM, m0, M, p.lda, tail) + last * step_a : source(q - IA, BN, n0, N, p.ldb, tail) + last * step_b;
+      load(q, stage(s), v, k * step_a, k * step_b);
+    }
+  }
   wait_loads<2 * LPS>();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
+  if (tail < 32) {  // clear what stage 0 has no k for
+    uint4* o = reinterpret_cast<uint4*>(smem);
+    if constexpr (MN) {
+      for (int i = tail * (BM / 8) + tid; i < 32 * (BM / 8); i += NW * 64) o[i] = make_uint4(0, 0, 0, 0);
+      for (int i = tail * (BN / 8) + tid; i < 32 * (BN / 8); i += NW * 64) o[A_BYTES / 16 + i] = make_uint4(0, 0, 0, 0);
+    } else {  // of E (f(X) has values there)
+      unsigned short* h = reinterpret_cast<unsigned short*>(smem);
+      for (int i = tid; i < BM * 32; i += NW * 64)
+        if (((i & 31) ^ (((i >> 7) & 3) << 3)) >= tail) h[i] = 0;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  }
 #pragma unroll
   for (int j = 0; j < RN; ++j) fb[0][j] = fragment(stage(0) + A_BYTES, BN * 2, wn * WTN + j * 32, 0);
 #pragma unroll
@@ -157,6 +186,7 @@ __global__ void __launch_bounds__(WGM * WGN * 64) ckpt_gemm_kernel(const CkptPro
     constexpr int S = decltype(SV)::value, O = S ^ 1;
     constexpr int L0 = S == 0 ? 0 : (LPS + 1) / 2, L1 = S == 0 ? (LPS + 1) / 2 : LPS;
     constexpr int NM = RM * RN, NR = RM + RN;
+    const unsigned k3 = k_of(kt + 3);
 #pragma unroll
     for (int q = 0; q < NM; ++q) {
 #pragma unroll
@@ -167,7 +197,8 @@ __global__ void __launch_bounds__(WGM * WGN * 64) ckpt_gemm_kernel(const CkptPro
         }
 #pragma unroll
       for (int l = L0; l < L1; ++l)
-        if ((l - L0) * NM / (L1 - L0) == q) load(l, group(kt + 3), stage(kt + 3));
+        if ((l - L0) * NM / (L1 - L0) == q)
+          load(l, stage(kt + 3), l < IA ? oa[l < IA ? l : 0] : ob[l < IA ? 0 : l - IA], k3 * step_a, k3 * step_b);
       const int i = q / RN, j = q % RN;
       acc[i][j] = MF::run(fb[S][j], fa[S][i], acc[i][j]);
       __builtin_amdgcn_sched_barrier(0);
@@ -194,6 +225,16 @@ __global__ void __launch_bounds__(WGM * WGN * 64) ckpt_gemm_kernel(const CkptPro
   if (p.vec) tile_epilogue<OT, KIND, EACT, true, RM, RN>(e, acc, es, m0 + wm * WTM, n0 + wn * WTN);
   else tile_epilogue<OT, KIND, EACT, false, RM, RN>(e, acc, es, m0 + wm * WTM, n0 + wn * WTN);
 }
+
+// Up to two matrices of 16-bit values with their rows padded with zeros to ld, a
+// multiple of 8: one pass, 16 bytes a lane, four loads in flight.
+struct PadJob {
+  const unsigned short* src;
+  unsigned short* dst;
+  int rows, n, ld;
+};
+constexpr int PAD_CHUNKS = 4 * 256;  // of a workgroup
+inline long long pad_blocks(const PadJob& j) { return (j.rows * (long long)(j.ld / 8) + PAD_CHUNKS - 1) / PAD_CHUNKS; }
 
 template <typename OT, int MODE, int ACT, int BM, int BN, int WGM, int WGN>
 hipError_t run_ckpt_tile(const CkptProblem& p, hipStream_t s) {

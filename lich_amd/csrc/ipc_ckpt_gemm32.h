@@ -85,7 +85,8 @@ __global__ void __launch_bounds__(WGM * WGN * WK * 64) ckpt_gemm32_kernel(const 
   const int H = wk < G ? (G - wk + WK - 1) / WK : 0;  // steps of a group: stages wk, wk + WK, ...
   unsigned char* ring = smem + wk * STAGES * STAGE;
   auto place = [&](int kt) -> unsigned char* { return ring + (kt & (STAGES - 1)) * STAGE; };
-  auto k_of = [&](int g) { return g == 0 ? K - tail : (g - 1) * K32; };
+  // first k of a stage; past the end: of the last, so that every step counts the same
+  auto k_of = [&](int g) { return g == 0 || G == 1 ? K - tail : ((g < G ? g : G - 1) - 1) * K32; };
 
   // (the host: operands below 2^31 bytes)
   const long long lda = p.lda, ldb = p.ldb;
@@ -164,23 +165,29 @@ __global__ void __launch_bounds__(WGM * WGN * WK * 64) ckpt_gemm32_kernel(const 
 
   // prologue: all stages of the ring but one.  The operands' last k, where a load may
   // reach past the end, are stage 0: its whole offset is the lane's, which is checked.
+  const unsigned last_a = (unsigned)(K - tail) * step_a, last_b = (unsigned)(K - tail) * step_b;
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) {
-    const int g = s * WK + wk, k = g < G ? k_of(g) : 0;
+    const int g = s * WK + wk;
+    const bool first = g == 0 || G == 1;
+    const unsigned k = (unsigned)k_of(g);
 #pragma unroll
     for (int q = 0; q < LPS; ++q) {
       const bool of_a = q < IA, of_b = q >= IA && q < IA + IB;
       const int qb = of_b ? q - IA : 0;
       unsigned va = of_a ? oa[of_a ? q : 0] : 0u, vb = ob[qb];
-      if (MN && g == 0) {
-        if (of_a) va = source(q, BM, m0, M, lda, tail);
-        if (of_b) vb = source(qb, BN, n0, N, ldb, tail);
+      if (first) {
+        if (of_a) va = (MN ? source(q, BM, m0, M, lda, tail) : va) + last_a;
+        if (of_b) vb = (MN ? source(qb, BN, n0, N, ldb, tail) : vb) + last_b;
       }
-      // (a stage past the end: the operands' first values, so that every step counts the same)
-      const unsigned ka = (unsigned)k * step_a, kb = (unsigned)k * step_b;
-      load(q, k, place(s), g < G ? va + (g == 0 ? ka : 0u) : 0u, g == 0 ? 0u : ka, g < G ? vb + (g == 0 ? kb : 0u) : 0u,
-           g == 0 ? 0u : kb, g < G ? os : 0u);
+      load(q, (int)k, place(s), va, first ? 0u : k * step_a, vb, first ? 0u : k * step_b, os);
     }
+  }
+  if (G == 1) {  // (no other stage: its loads take the operands' first values)
+#pragma unroll
+    for (int q = 0; q < IA; ++q) oa[q] = 0;
+#pragma unroll
+    for (int q = 0; q < IB; ++q) ob[q] = 0;
   }
   wait_loads<2 * LPS>();
   if constexpr (GW > 1) __builtin_amdgcn_s_barrier();
@@ -212,9 +219,7 @@ __global__ void __launch_bounds__(WGM * WGN * WK * 64) ckpt_gemm32_kernel(const 
     wait_loads<LPS>();
     if constexpr (GW > 1) __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    const int g = kt * WK + wk, g3 = g + (STAGES - 1) * WK;
-    const bool in = g3 < G;
-    const int k3 = in ? (g3 - 1) * K32 : 0;
+    const int g = kt * WK + wk, k3 = G == 1 ? 0 : k_of(g + (STAGES - 1) * WK);
     unsigned char* fill = place(kt + STAGES - 1);
     const unsigned char* after = place(kt + 1);
     float x[RN][8];
@@ -237,8 +242,8 @@ __global__ void __launch_bounds__(WGM * WGN * WK * 64) ckpt_gemm32_kernel(const 
 #pragma unroll
       for (int l = 0; l < LPS; ++l)
         if (l * NP / LPS == q)
-          load(l, k3, fill, in && l < IA ? oa[l < IA ? l : 0] : 0u, (unsigned)k3 * step_a,
-               in && l >= IA ? ob[l >= IA && l - IA < IB ? l - IA : 0] : 0u, (unsigned)k3 * step_b, in ? os : 0u);
+          load(l, k3, fill, oa[l < IA ? l : 0], (unsigned)k3 * step_a, ob[l >= IA && l - IA < IB ? l - IA : 0],
+               (unsigned)k3 * step_b, os);
       const int kk = q / (RM * RN), i = q / RN % RM, j = q % RN;
       acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(CODES ? x[j][kk] : cur.b[CODES ? 0 : j][kk], cur.a[i][kk], acc[i][j], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);

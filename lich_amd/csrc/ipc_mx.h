@@ -77,8 +77,8 @@ inline long long mx_predict_terms_bytes(int K, int B, int storage) {
 hipError_t launch_mx_predict(const MxPredict& p, int storage, hipStream_t s);
 
 // The backward pass of a state kept in 8 bits as 16-bit products (ipc_ckpt_gemm.h):
-// the contraction a multiple of 32, 16-byte aligned operands and row lengths that
-// are multiples of 8, operands below 2^31 bytes.
+// rows that start at multiples of 4 bytes (an even lda and ldb), operands below
+// 2^31 bytes; CKPT_WEIGHT: rows of b readable and finite up to a multiple of 32.
 struct CkptProblem {
   int M, N, K;
   const void* a; long long lda;  // elements
@@ -92,6 +92,10 @@ struct CkptProblem {
 };
 enum { CKPT_GRAD = 0, CKPT_WEIGHT = 1 };
 hipError_t launch_ckpt_gemm(int mode, const CkptProblem& p, int operand, int act, hipStream_t s);
+// Rows of two 16-bit matrices (nullptr: none) padded with zeros from na, nb to lda, ldb
+// values, multiples of 8.
+hipError_t launch_ckpt_pad(const void* a, void* pa, int rows_a, int na, int lda, const void* b, void* pb, int rows_b,
+                           int nb, int ldb, hipStream_t s);
 // On fp32 operands (ipc_ckpt_gemm32.h): rows of any length, operands below 2^31 bytes.
 // CKPT_WEIGHT: b = f(X) in fp32, or nullptr: X from its codes x, xs, x_row.
 hipError_t launch_ckpt_gemm32(int mode, const CkptProblem& p, int act, hipStream_t s);

@@ -263,21 +263,23 @@ class CheckpointWeightUpdateKernel(_Kernel):
 
 class CheckpointGradientKernel(_Kernel):
     """``k(W_lower[K, M], E_lower[K, B], X8, G[M, B], *, workspace=None)``:
-    ``G = f'(X) W_lower^T E_lower``, X [M, B] kept in 8 bits.  It uses no workspace
-    (``new_workspace()`` is None)."""
+    ``G = f'(X) W_lower^T E_lower``, X [M, B] kept in 8 bits.  ``workspace`` (optional,
+    caller-owned, ``new_workspace()``) lets a 16-bit call lay out rows of an odd length once."""
+
+    workspace_bytes = 0
 
     def __init__(self, *a, **kw):
         super().__init__("gradient", *a, **kw)
         self._x = _Packed("X", self.M, self.B, "int8")
         self._call = _entry("ipc_ckpt_gradient", self.M, self.K, self.B, self.storage, self.operand, self.act)
+        self.workspace_bytes = int(nat.lib().ipc_ckpt_gradient_workspace_bytes(self.M, self.K, self.B, self.storage))
 
     def __call__(self, w_lower, e_lower, x8, g, *, workspace=None):
-        self._ws(workspace)
         w_lower_at = _pointer(w_lower, "W_lower", (self.K, self.M), self.dtype)
         e_lower_at = _pointer(e_lower, "E_lower", (self.K, self.B), self.dtype)
         x = self._x(x8)
         g_at = _pointer(g, "G", (self.M, self.B), self.dtype)
-        self._call((w_lower_at, e_lower_at, *x, g_at), g.get_device())
+        self._call((w_lower_at, e_lower_at, *x, g_at), g.get_device(), *self._ws(workspace))
 
 
 @lru_cache(maxsize=256)

@@ -69,10 +69,9 @@ def _gradient(M, K, B, storage, operand, unit, act):
     w, e = _rand(g, K, M, size=0.1, storage=storage), _rand(g, K, B, size=0.1, storage=storage)
     x8, xq = _keep(x, storage)
     up, d = w.T.contiguous() @ e, O.df(act, xq)
-    out = torch.full((M, B), 7.0, dtype=DT[storage], device="cuda")
     k = mx.build_checkpoint_gradient(M, K, B, act, DT[storage], operand_dtype=DT[operand])
-    assert k.new_workspace() is None
-    k(_dev(w, storage), _dev(e, storage), x8, out)
+    if storage == "fp32" or (M % 2 == 0 and B % 2 == 0):
+        assert k.new_workspace() is None
     size = w.T.abs().contiguous() @ e.abs()
     own = unit if storage == "fp32" else 0.0  # 16-bit tensors are operands as they are
     acc_tol = size * (2 * own + own * own + (K + 8) * 2.0 ** -23)
@@ -80,7 +79,10 @@ def _gradient(M, K, B, storage, operand, unit, act):
         acc_tol = acc_tol + (w.abs().sum(0)[:, None] + e.abs().sum(0)[None]) * 2.0 ** -24
     want = d * up
     tol = d.abs() * acc_tol + 2.0 ** -20 * (up.abs() + acc_tol)  # f' in fp32: a few units of 1
-    _close(out, want, tol + O.UNIT[storage] * 1.01 * (want.abs() + tol) + 2.0 ** -25 * (storage == "fp16") + 2.0 ** -149)
+    for workspace in (None, k.new_workspace()):
+        out = torch.full((M, B), 7.0, dtype=DT[storage], device="cuda")
+        k(_dev(w, storage), _dev(e, storage), x8, out, workspace=workspace)
+        _close(out, want, tol + O.UNIT[storage] * 1.01 * (want.abs() + tol) + 2.0 ** -25 * (storage == "fp16") + 2.0 ** -149)
 
 
 @pytest.mark.parametrize("storage,operand,unit", TYPES)
@@ -110,11 +112,13 @@ def test_gradient_activations(M, K, B, storage, operand, unit, act):
 
 
 @pytest.mark.parametrize("storage,operand,unit", TYPES[3:])
-@pytest.mark.parametrize("M,K,B", [(1032, 1100, 32), (1100, 2050, 192), (4100, 4000, 64), (3000, 4104, 96)])
+@pytest.mark.parametrize("M,K,B", [(1032, 1100, 32), (1100, 2050, 192), (4100, 4000, 64), (3000, 4104, 96), (1032, 1100, 2),
+                                   (1032, 1100, 1), (1033, 1101, 63), (1100, 2050, 191), (1100, 2051, 190), (4101, 4000, 65),
+                                   (4100, 4001, 66), (3000, 4104, 98)])
 def test_weight_update_widened_once(M, K, B, storage, operand, unit):
     """The 16-bit products on 64, 128 and 256 wide tiles."""
     k = mx.build_checkpoint_weight_update(M, K, B, "sigmoid", DT[storage])
-    assert k.workspace_bytes == 2 * K * B
+    assert k.workspace_bytes == 2 * (K + (M if B % 2 else 0)) * (-(-B // 32) * 32)
     _weight(M, K, B, storage, operand, unit, "sigmoid", lend=True)
 
 
@@ -136,8 +140,19 @@ def test_fp32_gradient(M, K, B):
     _gradient(M, K, B, "fp32", "fp32", 0.0, "silu")
 
 
+@pytest.mark.parametrize("storage,operand,unit", TYPES[3:])
+@pytest.mark.parametrize("M,K,B", [(2, 1, 2), (4, 33, 2), (65, 31, 64), (64, 40, 65), (1100, 513, 1002), (1101, 514, 1003),
+                                   (2051, 333, 1000), (4098, 47, 4006), (4097, 65, 4001)])
+def test_16_bit_gradient(M, K, B, storage, operand, unit):
+    """Rows of even and odd lengths, contractions with a rest, on 64, 128 and 256 wide tiles."""
+    pads = (M % 2 or B % 2) and M * K * B >= 2 ** 28 and (M % 2 == 0 or B >= 256)
+    need = 2 * K * ((-(-M // 8) * 8 if M % 2 else 0) + (-(-B // 8) * 8 if B % 2 else 0)) if pads else 0
+    assert mx.build_checkpoint_gradient(M, K, B, "silu", DT[storage]).workspace_bytes == need
+    _gradient(M, K, B, storage, operand, unit, "silu")
+
+
 @pytest.mark.parametrize("storage,operand,unit", TYPES)
-@pytest.mark.parametrize("M,K,B", [(37, 50, 45), (40, 64, 72), (600, 1500, 1100), (1100, 2050, 190)])
+@pytest.mark.parametrize("M,K,B", [(37, 50, 45), (40, 64, 72), (600, 1500, 1100), (1100, 2050, 190), (1101, 1201, 301)])
 def test_not_a_number_stays_in_its_place(M, K, B, storage, operand, unit):
     """A load that reaches into the next row, or clears what a stage lacks, touches no
     other output."""
@@ -148,11 +163,12 @@ def test_not_a_number_stays_in_its_place(M, K, B, storage, operand, unit):
     nan, bad = float("nan"), float("inf")
     grad = mx.build_checkpoint_gradient(K, M, B, "tanh", DT[storage], operand_dtype=DT[operand])
     plain, hit = (torch.empty((K, B), dtype=DT[storage], device="cuda") for _ in range(2))
-    grad(_dev(w, storage), _dev(e, storage), x8, plain)
+    ws = grad.new_workspace()
+    grad(_dev(w, storage), _dev(e, storage), x8, plain, workspace=ws)
     w2, e2 = w.clone(), e.clone()
     w2[:, 0] = nan
     e2[:, 0] = bad
-    grad(_dev(w2, storage), _dev(e2, storage), x8, hit)
+    grad(_dev(w2, storage), _dev(e2, storage), x8, hit, workspace=ws)
     assert bool(hit[0].isnan().all()) and bool((~hit[:, 0].isfinite()).all())
     assert torch.equal(hit[1:, 1:], plain[1:, 1:])
     update = mx.build_checkpoint_weight_update(M, K, B, "tanh", DT[storage], 0.01, operand_dtype=DT[operand])

@@ -69,9 +69,12 @@ def test_other_entry_points_validate():
     assert lib.ipc_ckpt_weight_update(P, P, P, P, 64, 64, 64, 1e-4, 1, 2, 1, None, 0, None) == nat.ERR_DTYPE
     assert lib.ipc_ckpt_weight_update(P, P, P, P, 64, 64, 64, 1e-4, 0, 0, 1, P + 8, 64, None) == nat.ERR_ALIGN
     assert lib.ipc_ckpt_weight_update(P, P, P, P, 64, 64, 64, 1e-4, 0, 0, 1, P, -1, None) == nat.ERR_SHAPE
-    assert lib.ipc_ckpt_gradient(P, P, P + 4, P, P, 64, 64, 64, 0, 0, 1, None) == nat.ERR_ALIGN
-    assert lib.ipc_ckpt_gradient(P, P, P, P, None, 64, 64, 64, 0, 0, 1, None) == nat.ERR_NULL
-    assert lib.ipc_ckpt_gradient(P, P, P, P, P, 1 << 24, 64, 1, 0, 0, 1, None) == nat.ERR_SHAPE
+    assert lib.ipc_ckpt_gradient(P, P, P + 4, P, P, 64, 64, 64, 0, 0, 1, None, 0, None) == nat.ERR_ALIGN
+    assert lib.ipc_ckpt_gradient(P, P, P, P, None, 64, 64, 64, 0, 0, 1, None, 0, None) == nat.ERR_NULL
+    assert lib.ipc_ckpt_gradient(P, P, P, P, P, 1 << 24, 64, 1, 0, 0, 1, None, 0, None) == nat.ERR_SHAPE
+    assert lib.ipc_ckpt_gradient(P, P, P, P, P, 64, 64, 64, 2, 2, 1, P + 8, 64, None) == nat.ERR_ALIGN
+    assert lib.ipc_ckpt_gradient_workspace_bytes(1001, 1000, 999, 2) == 2 * 1000 * (1008 + 1000)
+    assert lib.ipc_ckpt_gradient_workspace_bytes(1000, 999, 998, 2) == 0
 
 
 def test_builders_refuse():
