@@ -22,7 +22,7 @@ synchronised inside a call.  The reference has no counterpart.
 """
 from __future__ import annotations
 
-from ctypes import c_float, c_int
+from ctypes import c_float, c_int, c_void_p, cast
 from functools import lru_cache
 from typing import NamedTuple
 
@@ -30,6 +30,11 @@ import torch
 
 from . import _native as nat
 from .kernels import _check, _Kernel, _storage_dtype
+
+try:
+    from . import _fast_call
+except ImportError:  # not built: the calls go through ctypes
+    _fast_call = None
 
 BLOCK, GROUP = 32, 128  # values per scale, per four scale bytes
 
@@ -80,10 +85,8 @@ class _Packed:
 
 
 def _pointer(t, name: str, shape: tuple, dtype: torch.dtype) -> int:
-    """``_check`` and the tensor's address: one test where there is nothing to refuse
-    (0.25 us a tensor against 0.6, of calls that last 4)."""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is dtype and t.shape == shape and t.is_contiguous()):
-        _check(t, name, shape, dtype)
+    """The address of a tensor that passes ``_check``."""
+    _check(t, name, shape, dtype)
     return t.data_ptr()
 
 
@@ -92,21 +95,39 @@ def _sizes(**sizes) -> None:
         raise ValueError("invalid shape " + " ".join(f"{k}={v}" for k, v in sizes.items()))
 
 
-def _entry(name: str, *constants):
-    """The call ``f(pointers, device index)`` of a library entry point whose arguments
-    are pointers, then these constants (converted once), then the stream."""
-    fn = getattr(nat.lib(), name)
-    constants = tuple(c_float(v) if isinstance(v, float) else c_int(v) for v in constants)
+class _Operator:
+    """A call of a library entry point whose arguments are pointers, constants, for some a
+    lent workspace, and the stream.  ``_run(*operands[, workspace])`` makes it where
+    every operand is what it has to be and returns 0; else ``_checked`` finds out why
+    not and raises."""
 
-    def call(pointers, device, *rest):
-        rc = fn(*pointers, *constants, *rest, nat.current_stream_handle(device))
-        if rc:
+    def _bind(self, entry: str, operands: tuple, *constants, workspace: bool = False) -> None:
+        """``operands``: of each argument a ``_Packed`` or (name, shape, dtype)."""
+        self._entry, self._operands, self._lends = getattr(nat.lib(), entry), operands, workspace
+        self._constants = tuple(c_float(v) if isinstance(v, float) else c_int(v) for v in constants)
+        self._run = _no_fast_call
+        if _fast_call is not None and nat._raw_stream is not None:
+            parts = []
+            for o in operands:
+                parts += [(o.codes, o.dtype), (o.scales, torch.uint8)] if isinstance(o, _Packed) else [tuple(o[1:])]
+            self._run = _fast_call.Call(entry, cast(self._entry, c_void_p).value, tuple(parts), constants, nat._raw_stream)
+
+    def _checked(self, rc: int, *given, workspace=None) -> None:
+        if rc < 0:
             nat.check(rc)
+        pointers = []
+        for o, t in zip(self._operands, given):
+            pointers += o(t) if isinstance(o, _Packed) else (_pointer(t, *o),)
+        first = given[0] if isinstance(given[0], torch.Tensor) else given[0][0]
+        lent = _Kernel._ws(workspace) if self._lends else ()
+        nat.check(self._entry(*pointers, *self._constants, *lent, nat.current_stream_handle(first.get_device())))
 
-    return call
+
+def _no_fast_call(*_) -> int:
+    return 1
 
 
-class _MXKernel:
+class _MXKernel(_Operator):
     def __init__(self, dtype, activation: str = "identity"):
         self.dtype = _storage_dtype(dtype)
         self.storage = nat.dtype_code(self.dtype)
@@ -124,15 +145,20 @@ class MXQuantizeKernel(_MXKernel):
             raise ValueError(f"axis must be 0 or 1 (got {axis})")
         self.R, self.C, self.axis, self.format = int(R), int(C), int(axis), _format(format)
         self.rows, self.length = (self.R, self.C) if axis == 1 else (self.C, self.R)
-        self._packed = _Packed("packed", self.rows, self.length, format)
-        self._call = _entry("ipc_mx_quantize", self.R, self.C, self.axis, nat.MX_FORMATS[format], self.storage, self.act)
+        packed = _Packed("packed", self.rows, self.length, format)
+        self._bind("ipc_mx_quantize", (("X", (self.R, self.C), self.dtype), packed), self.R, self.C, self.axis,
+                   nat.MX_FORMATS[format], self.storage, self.act)
+        self._new = packed.new
+        if _fast_call is not None:
+            self._new = _fast_call.Packed(packed.codes, packed.dtype, packed.scales, torch.uint8, MXMatrix)
 
     def new_output(self, device=None) -> MXMatrix:
-        return self._packed.new(device)
+        return self._new(torch.device(device) if isinstance(device, (str, int)) else device)
 
     def __call__(self, x, packed):
-        x_at = _pointer(x, "X", (self.R, self.C), self.dtype)
-        self._call((x_at, *self._packed(packed)), x.get_device())
+        rc = self._run(x, packed)
+        if rc:
+            self._checked(rc, x, packed)
 
 
 class MXDequantizeKernel(_MXKernel):
@@ -142,13 +168,13 @@ class MXDequantizeKernel(_MXKernel):
         super().__init__(dtype)
         _sizes(R=R, C=C)
         self.R, self.C, self.format = int(R), int(C), _format(format)
-        self._packed = _Packed("packed", self.R, self.C, format)
-        self._call = _entry("ipc_mx_dequantize", self.R, self.C, nat.MX_FORMATS[format], self.storage)
+        self._bind("ipc_mx_dequantize", (_Packed("packed", self.R, self.C, format), ("OUT", (self.R, self.C), self.dtype)),
+                   self.R, self.C, nat.MX_FORMATS[format], self.storage)
 
     def __call__(self, packed, out):
-        at = self._packed(packed)
-        out_at = _pointer(out, "OUT", (self.R, self.C), self.dtype)
-        self._call((*at, out_at), out.get_device())
+        rc = self._run(packed, out)
+        if rc:
+            self._checked(rc, packed, out)
 
 
 class _MXProduct(_MXKernel):
@@ -164,14 +190,14 @@ class MXPredictionErrorKernel(_MXProduct):
 
     def __init__(self, *a):
         super().__init__(*a)
-        self._x, self._w = _Packed("X_upper", self.B, self.K), _Packed("W", self.M, self.K)
-        self._call = _entry("ipc_mx_pred_err", self.M, self.K, self.B, self.storage)
+        out = (self.M, self.B), self.dtype
+        self._bind("ipc_mx_pred_err", (_Packed("X_upper", self.B, self.K), _Packed("W", self.M, self.K), ("X_lower", *out),
+                                       ("E", *out)), self.M, self.K, self.B, self.storage)
 
     def __call__(self, x4, w4, x_lower, e):
-        x, w = self._x(x4), self._w(w4)
-        x_lower_at = _pointer(x_lower, "X_lower", (self.M, self.B), self.dtype)
-        e_at = _pointer(e, "E", (self.M, self.B), self.dtype)
-        self._call((*x, *w, x_lower_at, e_at), e.get_device())
+        rc = self._run(x4, w4, x_lower, e)
+        if rc:
+            self._checked(rc, x4, w4, x_lower, e)
 
 
 class MXForwardKernel(_MXProduct):
@@ -179,13 +205,13 @@ class MXForwardKernel(_MXProduct):
 
     def __init__(self, *a):
         super().__init__(*a)
-        self._x, self._w = _Packed("X_upper", self.B, self.K), _Packed("W", self.M, self.K)
-        self._call = _entry("ipc_mx_forward", self.M, self.K, self.B, self.storage)
+        self._bind("ipc_mx_forward", (_Packed("X_upper", self.B, self.K), _Packed("W", self.M, self.K),
+                                      ("OUT", (self.M, self.B), self.dtype)), self.M, self.K, self.B, self.storage)
 
     def __call__(self, x4, w4, out):
-        x, w = self._x(x4), self._w(w4)
-        out_at = _pointer(out, "OUT", (self.M, self.B), self.dtype)
-        self._call((*x, *w, out_at), out.get_device())
+        rc = self._run(x4, w4, out)
+        if rc:
+            self._checked(rc, x4, w4, out)
 
 
 class MXInferenceUpdateKernel(_MXProduct):
@@ -195,14 +221,15 @@ class MXInferenceUpdateKernel(_MXProduct):
     def __init__(self, M, K, B, activation, dtype, gamma):
         super().__init__(M, K, B, dtype, activation)
         self.gamma = float(gamma)
-        self._w, self._e = _Packed("W_lower", self.M, self.K), _Packed("E_lower", self.B, self.K)
-        self._call = _entry("ipc_mx_infer_update", self.M, self.K, self.B, self.gamma, self.storage, self.act)
+        out = (self.M, self.B), self.dtype
+        self._bind("ipc_mx_infer_update", (("X", *out), ("E", *out), _Packed("W_lower", self.M, self.K),
+                                           _Packed("E_lower", self.B, self.K)),
+                   self.M, self.K, self.B, self.gamma, self.storage, self.act)
 
     def __call__(self, x, e, wt4, et4):
-        x_at = _pointer(x, "X", (self.M, self.B), self.dtype)
-        e_at = _pointer(e, "E", (self.M, self.B), self.dtype)
-        w, el = self._w(wt4), self._e(et4)
-        self._call((x_at, e_at, *w, *el), x.get_device())
+        rc = self._run(x, e, wt4, et4)
+        if rc:
+            self._checked(rc, x, e, wt4, et4)
 
 
 class MXWeightUpdateKernel(_MXProduct):
@@ -212,13 +239,14 @@ class MXWeightUpdateKernel(_MXProduct):
     def __init__(self, M, K, B, dtype, alpha):
         super().__init__(M, K, B, dtype)
         self.alpha = float(alpha)
-        self._e, self._a = _Packed("E", self.M, self.B), _Packed("A", self.K, self.B)
-        self._call = _entry("ipc_mx_weight_update", self.M, self.K, self.B, self.alpha, self.storage)
+        self._bind("ipc_mx_weight_update", (("W", (self.M, self.K), self.dtype), _Packed("E", self.M, self.B),
+                                            _Packed("A", self.K, self.B)),
+                   self.M, self.K, self.B, self.alpha, self.storage)
 
     def __call__(self, w, e4, a4):
-        w_at = _pointer(w, "W", (self.M, self.K), self.dtype)
-        e, a = self._e(e4), self._a(a4)
-        self._call((w_at, *e, *a), w.get_device())
+        rc = self._run(w, e4, a4)
+        if rc:
+            self._checked(rc, w, e4, a4)
 
 
 class MXPredictKernel(_MXProduct):
@@ -228,20 +256,20 @@ class MXPredictKernel(_MXProduct):
 
     def __init__(self, M, K, B, activation, dtype):
         super().__init__(M, K, B, dtype, activation)
-        self._w = _Packed("W", self.M, self.K)
-        self._call = _entry("ipc_mx_predict", self.M, self.K, self.B, self.storage, self.act)
+        self._bind("ipc_mx_predict", (("X", (self.K, self.B), self.dtype), _Packed("W", self.M, self.K),
+                                      ("OUT", (self.M, self.B), self.dtype)),
+                   self.M, self.K, self.B, self.storage, self.act, workspace=True)
         self.workspace_bytes = int(nat.lib().ipc_mx_predict_workspace_bytes(self.K, self.B, self.storage))
 
-    new_workspace, _ws = _Kernel.new_workspace, staticmethod(_Kernel._ws)
+    new_workspace = _Kernel.new_workspace
 
     def __call__(self, x, w4, out, *, workspace=None):
-        x_at = _pointer(x, "X", (self.K, self.B), self.dtype)
-        w = self._w(w4)
-        out_at = _pointer(out, "OUT", (self.M, self.B), self.dtype)
-        self._call((x_at, *w, out_at), out.get_device(), *self._ws(workspace))
+        rc = self._run(x, w4, out, workspace)
+        if rc:
+            self._checked(rc, x, w4, out, workspace=workspace)
 
 
-class CheckpointWeightUpdateKernel(_Kernel):
+class CheckpointWeightUpdateKernel(_Operator, _Kernel):
     """``k(W[M, K], E[M, B], X8, *, workspace=None)``: ``W += alpha E f(X)^T``, X [K, B] kept
     in 8 bits.  ``workspace`` (optional, caller-owned, ``new_workspace()``) lets a
     large call evaluate f(X) once."""
@@ -251,17 +279,18 @@ class CheckpointWeightUpdateKernel(_Kernel):
     def __init__(self, *a, alpha, **kw):
         super().__init__("weight", *a, **kw)
         self.alpha = float(alpha)
-        self._x = _Packed("X", self.K, self.B, "int8")
-        self._call = _entry("ipc_ckpt_weight_update", self.M, self.K, self.B, self.alpha, self.storage, self.operand, self.act)
+        self._bind("ipc_ckpt_weight_update", (("W", (self.M, self.K), self.dtype), ("E", (self.M, self.B), self.dtype),
+                                              _Packed("X", self.K, self.B, "int8")),
+                   self.M, self.K, self.B, self.alpha, self.storage, self.operand, self.act, workspace=True)
         self.workspace_bytes = int(nat.lib().ipc_ckpt_workspace_bytes(self.act, self.M, self.K, self.B, self.storage))
 
     def __call__(self, w, e, x8, *, workspace=None):
-        w_at = _pointer(w, "W", (self.M, self.K), self.dtype)
-        e_at = _pointer(e, "E", (self.M, self.B), self.dtype)
-        self._call((w_at, e_at, *self._x(x8)), w.get_device(), *self._ws(workspace))
+        rc = self._run(w, e, x8, workspace)
+        if rc:
+            self._checked(rc, w, e, x8, workspace=workspace)
 
 
-class CheckpointGradientKernel(_Kernel):
+class CheckpointGradientKernel(_Operator, _Kernel):
     """``k(W_lower[K, M], E_lower[K, B], X8, G[M, B], *, workspace=None)``:
     ``G = f'(X) W_lower^T E_lower``, X [M, B] kept in 8 bits.  ``workspace`` (optional,
     caller-owned, ``new_workspace()``) lets a 16-bit call lay out rows of an odd length once."""
@@ -270,16 +299,15 @@ class CheckpointGradientKernel(_Kernel):
 
     def __init__(self, *a, **kw):
         super().__init__("gradient", *a, **kw)
-        self._x = _Packed("X", self.M, self.B, "int8")
-        self._call = _entry("ipc_ckpt_gradient", self.M, self.K, self.B, self.storage, self.operand, self.act)
+        self._bind("ipc_ckpt_gradient", (("W_lower", (self.K, self.M), self.dtype), ("E_lower", (self.K, self.B), self.dtype),
+                                         _Packed("X", self.M, self.B, "int8"), ("G", (self.M, self.B), self.dtype)),
+                   self.M, self.K, self.B, self.storage, self.operand, self.act, workspace=True)
         self.workspace_bytes = int(nat.lib().ipc_ckpt_gradient_workspace_bytes(self.M, self.K, self.B, self.storage))
 
     def __call__(self, w_lower, e_lower, x8, g, *, workspace=None):
-        w_lower_at = _pointer(w_lower, "W_lower", (self.K, self.M), self.dtype)
-        e_lower_at = _pointer(e_lower, "E_lower", (self.K, self.B), self.dtype)
-        x = self._x(x8)
-        g_at = _pointer(g, "G", (self.M, self.B), self.dtype)
-        self._call((w_lower_at, e_lower_at, *x, g_at), g.get_device(), *self._ws(workspace))
+        rc = self._run(w_lower, e_lower, x8, g, workspace)
+        if rc:
+            self._checked(rc, w_lower, e_lower, x8, g, workspace=workspace)
 
 
 @lru_cache(maxsize=256)

@@ -303,3 +303,57 @@ def test_refusals():
     shifted = torch.empty(out.codes.numel() + 4, dtype=torch.uint8, device="cuda")[4:].view_as(out.codes)
     with pytest.raises(ValueError, match="aligned"):
         k(x, mx.MXMatrix(shifted, out.scales))
+
+
+def test_fast_and_checked_calls_agree():
+    """The extension's calls and those through ctypes: the same results, on the stream that
+    is current; a tensor that is not what it has to be is refused either way."""
+    assert mx._fast_call is not None
+    M, K, B = 96, 200, 40
+    g = torch.Generator().manual_seed(5)
+    x, w = (torch.randn(s, generator=g).cuda() for s in ((K, B), (M, K)))
+    e = torch.randn((M, B), generator=g).cuda()
+    got = []
+    for fast in (True, False):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            def run(k, *a, **kw):
+                before, k._run = k._run, k._run if fast else mx._no_fast_call
+                try:
+                    k(*a, **kw)
+                finally:
+                    k._run = before
+
+            qx, qw, qt, qe = (mx.build_mx_quantize(K, B, "relu", axis=0), mx.build_mx_quantize(M, K), mx.build_mx_quantize(M, K, axis=0),
+                              mx.build_mx_quantize(M, B, axis=0))
+            x4, w4, wt, et = (k.new_output("cuda") for k in (qx, qw, qt, qe))
+            for k, t, o in ((qx, x, x4), (qw, w, w4), (qt, w, wt), (qe, e, et)):
+                run(k, t, o)
+            save, x8 = mx.build_checkpoint_save(K, B), mx.new_packed(K, B, "int8")
+            run(save, x, x8)
+            out = [torch.empty_like(e), torch.empty_like(e), x.clone(), w.clone(), torch.empty_like(e), w.clone(),
+                   torch.empty_like(x), torch.empty_like(x)]
+            e4, a4 = mx.build_mx_quantize(M, B), mx.build_mx_quantize(K, B)
+            er, ar = e4.new_output(), a4.new_output()
+            run(e4, e, er)
+            run(a4, x, ar)
+            run(mx.build_mx_prediction_error(M, K, B), x4, w4, e, out[0])
+            run(mx.build_mx_forward(M, K, B), x4, w4, out[1])
+            run(mx.build_mx_inference_update(K, M, B, "tanh"), out[2], x, wt, et)
+            run(mx.build_mx_weight_update(M, K, B), out[3], er, ar)
+            predict = mx.build_mx_predict(M, K, B, "silu")
+            run(predict, x, w4, out[4], workspace=predict.new_workspace())
+            run(mx.build_checkpoint_weight_update(M, K, B, "gelu"), out[5], e, x8)
+            run(mx.build_checkpoint_gradient(K, M, B, "gelu"), w, e, x8, out[6])
+            run(mx.build_mx_dequantize(K, B, format="int8"), x8, out[7])
+        side.synchronize()
+        got.append(out)
+    for a, b in zip(*got):
+        assert bool(a.isfinite().all()) and torch.equal(a, b)
+    for bad in (x.half(), x[:, :-1], x.T.contiguous().T, x.cpu(), None):
+        with pytest.raises((ValueError, TypeError)):
+            qx(bad, x4)
+    for bad in ((x4.codes, x4.scales[:1]), (x4.codes.cpu(), x4.scales), [*x4], (x4.codes,)):
+        with pytest.raises((ValueError, TypeError)):
+            qx(x, bad)

@@ -109,3 +109,23 @@ def test_the_oracle_rounds_to_nearest(fmt):
     # ... and no block could have had a smaller scale without saturating past half a step
     top = x.view(50, 2, 32).abs().amax(-1) / 2.0 ** (byte[:, :2].double() - 127)
     assert bool((top < (7 if fmt == "fp4" else 255 / 128)).all()) and bool((top >= (3.5 if fmt == "fp4" else 255 / 256)).all())
+
+
+def test_fast_calls_refuse():
+    """What is no device tensor of the right kind is left to the checks with messages."""
+    fast = pytest.importorskip("lich_amd._fast_call")
+    spec = ((2, 3), torch.float32), ((2, 64), torch.uint8), ((1, 2, 4), torch.uint8)
+    call = fast.Call("ipc_mx_quantize", 0, spec, (2, 3, 1, 0, 0, 1), lambda i: 0)
+    x, p = torch.zeros(2, 3), mx.MXMatrix(torch.zeros(2, 64, dtype=torch.uint8), torch.zeros(1, 2, 4, dtype=torch.uint8))
+    for given in ((), (x,), (x, p), (x, None), (x, (p.codes,)), (None, p), (x, p, None), (x, p, x), (p, x), (x, [*p])):
+        assert call(*given) == 1
+    assert call(x, p=p) == 1
+    for bad in (("ipc_mx_nothing", 0, spec, (2, 3, 1, 0, 0, 1), None), ("ipc_mx_quantize", 0, spec[:2], (2, 3, 1, 0, 0, 1), None),
+                ("ipc_mx_quantize", 0, spec, (2, 3, 1, 0, 0), None), ("ipc_mx_quantize", 0, spec, (2, 3, 1, 0, 0, 1.0), None),
+                ("ipc_mx_quantize", 0, (spec[0], spec[1], ((1, 2, 3, 4), torch.uint8)), (2, 3, 1, 0, 0, 1), None)):
+        with pytest.raises(ValueError):
+            fast.Call(*bad)
+    with pytest.raises(ValueError):
+        fast.Packed((2, 64), torch.uint8, (1, 2, 4), torch.uint8, list)
+    with pytest.raises(TypeError):
+        fast.Packed((2, 64), torch.uint8, (1, 2, 4), torch.uint8, mx.MXMatrix)("cuda")
