@@ -1,7 +1,10 @@
 // ipc_mx_quant.hip - matrices into microscaled storage and back (gfx950).
 //
 // Both directions are one pass over the data, bound by HBM: each value is read
-// once and each code and scale written once.
+// once and each code and scale written once.  MI355X, fp32, 4096 x 4096, fp4: columns
+// 16.3 us (76 MB, 4.7 TB/s; a copy of that size runs at 5.2), back 12.6 us; bf16, 4096 x
+// 1024, int8: rows 6.0 us, back 4.4 (13 MB, 2-3 TB/s: mostly the launch and one
+// memory latency).
 #include "ipc_launch.h"
 #include "ipc_mx_device.h"
 
