@@ -653,9 +653,13 @@ bool ckpt_products32(int storage, int operand, int M, int K, int B) {
 // fp32: evaluating it in every row of tiles costs more than that pass (5-8 us): MI355X,
 // us, from codes / widened and read (relu; silu): 512^3 6.9; 10.3 / 6.2 + 4, 1000 x 1531 x
 // 300 16.9; 25.3 / 15.9 + 4, 2048 x 1024 x 1024 45; 87 / 41 + 5, 2048^3 162; 333 / 137 + 7.
-// 16 bits: for the 16-bit products where there are outputs enough for them to win
-// against the kernels that widen in their loaders, or (lengths those products cannot
-// take) by the same comparison.
+// 16 bits: for the 16-bit products where there are outputs enough, or outputs and samples,
+// for them to win against the kernels that widen in their loaders, or (lengths those
+// products cannot take) by the same comparison.
+bool ckpt_weight_products(int M, int K, int B, int storage) {
+  const long long outputs = (long long)M * K;
+  return ckpt_products(storage, M, K, B) && (outputs > (1 << 20) || (outputs >= (1 << 18) && B >= 2048));
+}
 long long ckpt_workspace_need(int act, int M, int K, int B, int storage) {
   if (storage == IPC_DT_F32) {
     const bool cheap = act == IPC_ACT_IDENTITY || act == IPC_ACT_RELU;
@@ -663,7 +667,7 @@ long long ckpt_workspace_need(int act, int M, int K, int B, int storage) {
     return K * mx_row_values(MX_INT8, B) * 4;
   }
   const long long padded = mx_row_values(MX_INT8, B);
-  if (ckpt_products(storage, M, K, B) && (long long)M * K > (1 << 20)) return (K + (B % 2 ? (long long)M : 0LL)) * padded * 2;
+  if (ckpt_weight_products(M, K, B, storage)) return (K + (B % 2 ? (long long)M : 0LL)) * padded * 2;
   return s16_preact_rule(S16_WEIGHT, act, M, K, (long long)K * B) ? (long long)K * B * 2 : 0;
 }
 
@@ -721,7 +725,7 @@ int ipc_ckpt_weight_update(void* w, const void* e, const void* x_codes, const vo
     q.vec = vec_ok(w, K, es);
     return launch_rc(launch_ckpt_gemm32(CKPT_WEIGHT, q, act, s), "ipc_ckpt_weight_update");
   }
-  const bool products = ckpt_products(storage, M, K, B) && (long long)M * K > (1 << 20);
+  const bool products = ckpt_weight_products(M, K, B, storage);
   if (lent && products && (B % 2 || al4(e))) {  // (rows padded as the packed ones are)
     const int n = (int)mx_row_values(MX_INT8, B);
     void* pad = static_cast<char*>(workspace) + (long long)K * n * 2;

@@ -61,8 +61,60 @@ __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-template <typename OT, int MODE, int ACT, int BM, int BN, int WGM, int WGN>
-__global__ void __launch_bounds__(WGM * WGN * 64) ckpt_gemm_kernel(const CkptProblem p) {
+// The epilogue where WK groups of waves split a tile's contraction: their sums meet in
+// LDS and are added in the groups' order, every wave finishes some rows of the tile.
+template <typename ST, int KIND, int ACT, int BM, int BN, int WK, int RM, int RN>
+__device__ __forceinline__ void joined_epilogue(const MxProblem& p, const f32x16 (&acc)[RM][RN], unsigned char* smem, int wk,
+                                                int mw, int nw, int m0, int n0) {
+  constexpr int LD = BN + 4, LANES = BN / 4, THREADS = (BM / 32 / RM) * (BN / 32 / RN) * WK * 64;
+  constexpr int PASS = THREADS / LANES, PASSES = BM / PASS;
+  const int tid = threadIdx.x, lane = tid & 63, lr = lane & 31, lk = lane >> 5;
+  const int er = tid / LANES, ec = tid % LANES * 4, n = n0 + ec, left = p.N - n;
+  float in[PASSES][4];
+  ST* out = static_cast<ST*>(p.out);
+#pragma unroll
+  for (int u = 0; u < PASSES; ++u) {
+    const int m = m0 + u * PASS + er;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) in[u][i] = 0.0f;
+    if (m >= p.M || left <= 0) continue;
+    if constexpr (KIND == KIND_GRAD8) {
+      const unsigned q = *reinterpret_cast<const unsigned*>(static_cast<const uint8_t*>(p.aux) + (long long)m * p.groups + n);
+      const float unit = int8_scale(reinterpret_cast<const uint8_t*>(p.as)[((long long)(n >> 7) * p.M + m) * 4 + ((n >> 5) & 3)]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) in[u][i] = (float)sext8(q, i) * unit;
+    } else {
+      get4(out + (long long)m * p.N + n, p.vec != 0, left, in[u]);
+    }
+  }
+  float* part = reinterpret_cast<float*>(smem);
+  __syncthreads();  // every wave is done with its ring
+#pragma unroll
+  for (int i = 0; i < RM; ++i)
+#pragma unroll
+    for (int j = 0; j < RN; ++j)
+#pragma unroll
+      for (int q = 0; q < 16; q += 4)
+        *reinterpret_cast<float4*>(part + (wk * BM + mw + i * 32 + lr) * LD + nw + j * 32 + 2 * q + 4 * lk) =
+            make_float4(acc[i][j][q], acc[i][j][q + 1], acc[i][j][q + 2], acc[i][j][q + 3]);
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < PASSES; ++u) {
+    const int m = m0 + u * PASS + er;
+    if (m >= p.M || left <= 0) continue;
+    float c[4] = {}, none[4] = {}, o[4];
+#pragma unroll
+    for (int v = 0; v < WK; ++v) {
+      const float4 t4 = *reinterpret_cast<const float4*>(part + (v * BM + u * PASS + er) * LD + ec);
+      c[0] += t4.x; c[1] += t4.y; c[2] += t4.z; c[3] += t4.w;
+    }
+    finish4<KIND, ACT>(c, in[u], none, p.scal, o);
+    put4(out + (long long)m * p.N + n, p.vec != 0, left, o);
+  }
+}
+
+template <typename OT, int MODE, int ACT, int BM, int BN, int WGM, int WGN, int WK>
+__global__ void __launch_bounds__(WGM * WGN * WK * 64) ckpt_gemm_kernel(const CkptProblem p) {
   extern __shared__ __align__(16) unsigned char smem[];
   using MF = Mfma32<OT>;
   typedef typename MF::operand V;
@@ -80,8 +132,10 @@ __global__ void __launch_bounds__(WGM * WGN * 64) ckpt_gemm_kernel(const CkptPro
   const int cs = w8 / (rows * 4), cols = tn - cs * 4 < 4 ? tn - cs * 4 : 4, w2 = w8 - cs * rows * 4;
   const int m0 = (band * 8 + w2 / cols) * BM, n0 = (cs * 4 + w2 % cols) * BN;
 
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int w = wave % NW, wk = wave / NW;  // wave of its group, group
   const int wm = w / WGN, wn = w % WGN, lr = lane & 31, lk = lane >> 5;
+  unsigned char* ring = smem + wk * STAGES * STAGE;
   // (the host: operands below 2^31 bytes, rows that start at multiples of 4)
   const int M = p.M, N = p.N, K = p.K, G = (K + 31) / 32, tail = K - (G - 1) * 32;
 
@@ -136,7 +190,7 @@ __global__ void __launch_bounds__(WGM * WGN * 64) ckpt_gemm_kernel(const CkptPro
     }
   };
   V fa[2][RM], fb[2][RN];
-  auto stage = [&](int kt) -> unsigned char* { return smem + (kt & (STAGES - 1)) * STAGE; };
+  auto stage = [&](int kt) -> unsigned char* { return ring + (kt & (STAGES - 1)) * STAGE; };
 
   // prologue: stages 0 .. 2.  The last 1 .. 32 k are stage 0; a load that reaches past
   // the operand's end there has all of its offset in the lane's, which is checked.
@@ -146,15 +200,19 @@ __global__ void __launch_bounds__(WGM * WGN * 64) ckpt_gemm_kernel(const CkptPro
 #pragma unroll
     for (int q = 0; q < IB; ++q) ob[q] = 0;
   }
-  // first k of stage kt > 0; past the end: of the last, so that every step counts the same
-  auto k_of = [&](int kt) { return (unsigned)(G == 1 ? 0 : (kt < G ? kt : G - 1) - 1) * 32u; };
+  // first k of the group's stage kt (not stage 0); past the end: of the last, so that every step counts the same
+  auto k_of = [&](int kt) {
+    const int g = kt * WK + wk;
+    return (unsigned)(G == 1 ? 0 : (g < G ? g : G - 1) - 1) * 32u;
+  };
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) {
-    const unsigned k = s > 0 ? k_of(s) : 0u, last = (unsigned)(K - tail);
+    const bool first = s * WK + wk == 0;
+    const unsigned k = first ? 0u : k_of(s), last = (unsigned)(K - tail);
 #pragma unroll
     for (int q = 0; q < LPS; ++q) {
       unsigned v = q < IA ? oa[q < IA ? q : 0] : ob[q < IA ? 0 : q - IA];
-      if (s == 0) v = q < IA ? source(q, BM, m0, M, p.lda, tail) + last * step_a : source(q - IA, BN, n0, N, p.ldb, tail) + last * step_b;
+      if (first) v = q < IA ? source(q, BM, m0, M, p.lda, tail) + last * step_a : source(q - IA, BN, n0, N, p.ldb, tail) + last * step_b;
       load(q, stage(s), v, k * step_a, k * step_b);
     }
   }
@@ -162,13 +220,15 @@ __global__ void __launch_bounds__(WGM * WGN * 64) ckpt_gemm_kernel(const CkptPro
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   if (tail < 32) {  // clear what stage 0 has no k for
-    uint4* o = reinterpret_cast<uint4*>(smem);
-    if constexpr (MN) {
-      for (int i = tail * (BM / 8) + tid; i < 32 * (BM / 8); i += NW * 64) o[i] = make_uint4(0, 0, 0, 0);
-      for (int i = tail * (BN / 8) + tid; i < 32 * (BN / 8); i += NW * 64) o[A_BYTES / 16 + i] = make_uint4(0, 0, 0, 0);
+    const int at = w * 64 + lane;
+    uint4* o = reinterpret_cast<uint4*>(ring);
+    if (wk > 0) {
+    } else if constexpr (MN) {
+      for (int i = tail * (BM / 8) + at; i < 32 * (BM / 8); i += NW * 64) o[i] = make_uint4(0, 0, 0, 0);
+      for (int i = tail * (BN / 8) + at; i < 32 * (BN / 8); i += NW * 64) o[A_BYTES / 16 + i] = make_uint4(0, 0, 0, 0);
     } else {  // of E (f(X) has values there)
-      unsigned short* h = reinterpret_cast<unsigned short*>(smem);
-      for (int i = tid; i < BM * 32; i += NW * 64)
+      unsigned short* h = reinterpret_cast<unsigned short*>(ring);
+      for (int i = at; i < BM * 32; i += NW * 64)
         if (((i & 31) ^ (((i >> 7) & 3) << 3)) >= tail) h[i] = 0;
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -200,12 +260,12 @@ __global__ void __launch_bounds__(WGM * WGN * 64) ckpt_gemm_kernel(const CkptPro
         if ((l - L0) * NM / (L1 - L0) == q)
           load(l, stage(kt + 3), l < IA ? oa[l < IA ? l : 0] : ob[l < IA ? 0 : l - IA], k3 * step_a, k3 * step_b);
       const int i = q / RN, j = q % RN;
-      acc[i][j] = MF::run(fb[S][j], fa[S][i], acc[i][j]);
+      if (WK == 1 || kt * WK + wk < G) acc[i][j] = MF::run(fb[S][j], fa[S][i], acc[i][j]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
 #pragma unroll 1
-  for (int kt = 0; kt < G; ++kt) {
+  for (int kt = 0; kt < (G + WK - 1) / WK; ++kt) {
     // stage kt + 1 of this wave has landed (kt + 2 may be in flight), then everybody's;
     // everybody is done with stage kt - 1, which kt + 3 takes
     wait_loads<LPS>();
@@ -219,9 +279,14 @@ __global__ void __launch_bounds__(WGM * WGN * 64) ckpt_gemm_kernel(const CkptPro
   MxProblem e{};
   e.M = M; e.N = N; e.out = p.out; e.scal = p.alpha;
   e.aux = p.x; e.as = static_cast<const uint32_t*>(p.xs); e.groups = p.x_row;
-  float* es = reinterpret_cast<float*>(smem) + w * 32 * (WTN + 4);
   constexpr int KIND = MODE == CKPT_GRAD ? KIND_GRAD8 : KIND_WEIGHT;
   constexpr int EACT = MODE == CKPT_GRAD ? ACT : ACT_IDENTITY;
+  if constexpr (WK > 1) {
+    e.vec = p.vec;
+    joined_epilogue<OT, KIND, EACT, BM, BN, WK, RM, RN>(e, acc, smem, wk, wm * WTM, wn * WTN, m0, n0);
+    return;
+  }
+  float* es = reinterpret_cast<float*>(smem) + w * 32 * (WTN + 4);
   if (p.vec) tile_epilogue<OT, KIND, EACT, true, RM, RN>(e, acc, es, m0 + wm * WTM, n0 + wn * WTN);
   else tile_epilogue<OT, KIND, EACT, false, RM, RN>(e, acc, es, m0 + wm * WTM, n0 + wn * WTN);
 }
@@ -236,30 +301,38 @@ struct PadJob {
 constexpr int PAD_CHUNKS = 4 * 256;  // of a workgroup
 inline long long pad_blocks(const PadJob& j) { return (j.rows * (long long)(j.ld / 8) + PAD_CHUNKS - 1) / PAD_CHUNKS; }
 
-template <typename OT, int MODE, int ACT, int BM, int BN, int WGM, int WGN>
+template <typename OT, int MODE, int ACT, int BM, int BN, int WGM, int WGN, int WK = 1>
 hipError_t run_ckpt_tile(const CkptProblem& p, hipStream_t s) {
-  constexpr int epi = WGM * WGN * 32 * (BN / WGN + 4) * 4, st = STAGES * (BM + BN) * 64, smem = epi > st ? epi : st;
+  constexpr int epi = WK == 1 ? WGM * WGN * 32 * (BN / WGN + 4) * 4 : WK * BM * (BN + 4) * 4;
+  constexpr int st = WK * STAGES * (BM + BN) * 64, smem = epi > st ? epi : st;
   static_assert(smem <= 160 * 1024, "LDS");
-  const void* fn = reinterpret_cast<const void*>(&ckpt_gemm_kernel<OT, MODE, ACT, BM, BN, WGM, WGN>);
+  const void* fn = reinterpret_cast<const void*>(&ckpt_gemm_kernel<OT, MODE, ACT, BM, BN, WGM, WGN, WK>);
   static const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != hipSuccess) return e;
   const long long tiles = ((p.M + BM - 1LL) / BM) * ((p.N + BN - 1LL) / BN);
   CkptProblem q = p;
   void* args[] = {&q};
-  return hipLaunchKernel(fn, dim3((unsigned)tiles), dim3(WGM * WGN * 64), args, smem, s);
+  return hipLaunchKernel(fn, dim3((unsigned)tiles), dim3(WGM * WGN * WK * 64), args, smem, s);
 }
 
-// The tile: the largest that gives the 256 CUs about one each.  MI355X, bf16, us, 256 /
-// 128 / 64 wide, gradient, then weight update (out rows x columns x contraction):
-//   2048 x 1024 x 1024   38 / 14.4 / 10.6   25 / 11.2 / 9.5   (128 tiles of 128 x 128)
-//   2048 x 2048 x 2048   57 / 26.1 / 30.9   44 / 24.3 / 44
-//   3200 x 3200 x 2048   59 / 56 / 67       47 / 58 / 91      (169 of 256 x 256)
-//   8192 x 2048 x 8192   205 / 235          203 / 295         (256)
+// The tile: the largest that gives the 256 CUs about one each; where 64 x 64 ones do not
+// outnumber the CUs and the contraction is long, four groups of waves split it (a CU
+// then has 96 KB of loads in flight instead of 24).  MI355X, bf16, us, 256 / 128 / 64 / 64
+// wide and split, gradient, then weight update (out rows x columns x contraction):
+//   128 x 128 x 4096     86 / 30 / 20 / 13        71 / 28 / 16.4 / 12.0
+//   512 x 512 x 512      28 / 10.2 / 6.0 / 5.9    16 / 7.1 / 6.1 / 6.5
+//   1024 x 1024 x 1024   37 / 13.3 / 8.4 / 7.6    24 / 10.4 / 7.0 / 7.5
+//   1024 x 1024 x 4096   88 / 37 / 30 / 18        75 / 35 / 28 / 20     (256 tiles of 64 x 64)
+//   2048 x 1024 x 1024   38 / 14.3 / 11.3 / 14.1  25 / 11.1 / 10.4 / 13.6
+//   2048 x 2048 x 2048   56 / 25.7 / 31.5 / 40    43 / 23.8 / 41 / 40   (256 of 128 x 128)
+//   3200 x 3200 x 2048   58 / 55 / 68             48 / 59 / 92          (169 of 256 x 256)
+//   8192 x 2048 x 8192   205 / 235                203 / 295             (256)
 template <typename OT, int MODE, int ACT>
 hipError_t run_ckpt(const CkptProblem& p, hipStream_t s) {
   auto tiles = [&](long long e) { return ((p.M + e - 1) / e) * ((p.N + e - 1) / e); };
   if (tiles(256) >= (MODE == CKPT_GRAD ? 224 : 160)) return run_ckpt_tile<OT, MODE, ACT, 256, 256, 2, 2>(p, s);
   if (tiles(128) > 128) return run_ckpt_tile<OT, MODE, ACT, 128, 128, 2, 2>(p, s);
+  if (tiles(64) <= 256 && p.K > 1024) return run_ckpt_tile<OT, MODE, ACT, 64, 64, 2, 2, 4>(p, s);
   return run_ckpt_tile<OT, MODE, ACT, 64, 64, 2, 2>(p, s);
 }
 

@@ -266,50 +266,9 @@ __global__ void __launch_bounds__(WGM * WGN * WK * 64) ckpt_gemm32_kernel(const 
     float* es = reinterpret_cast<float*>(smem) + w * 32 * (WTN + 4);
     if (p.vec) tile_epilogue<float, KIND, EACT, true, RM, RN>(e, acc, es, m0 + wm * WTM, n0 + wn * WTN);
     else tile_epilogue<float, KIND, EACT, false, RM, RN>(e, acc, es, m0 + wm * WTM, n0 + wn * WTN);
-  } else {  // the groups' sums meet in LDS and are added in their order, a wave some rows of the tile
-    constexpr int LD = BN + 4, LANES = BN / 4, PASS = GW * WK * 64 / LANES, PASSES = BM / PASS;
-    const int er = tid / LANES, ec = tid % LANES * 4, n = n0 + ec;
-    float in[PASSES][4];
-    float* out = static_cast<float*>(p.out);
-#pragma unroll
-    for (int u = 0; u < PASSES; ++u) {
-      const int m = m0 + u * PASS + er;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) in[u][i] = 0.0f;
-      if (m >= M || n >= N) continue;
-      if constexpr (MN) {
-        const unsigned q = *reinterpret_cast<const unsigned*>(static_cast<const uint8_t*>(p.x) + (long long)m * p.x_row + n);
-        const float unit = int8_scale(static_cast<const uint8_t*>(p.xs)[((long long)(n >> 7) * M + m) * 4 + ((n >> 5) & 3)]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) in[u][i] = (float)sext8(q, i) * unit;
-      } else {
-        get4(out + (long long)m * N + n, p.vec != 0, N - n, in[u]);
-      }
-    }
-    float* part = reinterpret_cast<float*>(smem);
-    __syncthreads();  // every wave is done with its ring
-#pragma unroll
-    for (int i = 0; i < RM; ++i)
-#pragma unroll
-      for (int j = 0; j < RN; ++j)
-#pragma unroll
-        for (int q = 0; q < 16; q += 4)
-          *reinterpret_cast<float4*>(part + (wk * BM + wm * WTM + i * 32 + lr) * LD + wn * WTN + j * 32 + 2 * q + 4 * lk) =
-              make_float4(acc[i][j][q], acc[i][j][q + 1], acc[i][j][q + 2], acc[i][j][q + 3]);
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < PASSES; ++u) {
-      const int m = m0 + u * PASS + er;
-      if (m >= M || n >= N) continue;
-      float c[4] = {}, none[4] = {}, o[4];
-#pragma unroll
-      for (int v = 0; v < WK; ++v) {
-        const float4 t4 = *reinterpret_cast<const float4*>(part + (v * BM + u * PASS + er) * LD + ec);
-        c[0] += t4.x; c[1] += t4.y; c[2] += t4.z; c[3] += t4.w;
-      }
-      finish4<KIND, EACT>(c, in[u], none, p.alpha, o);
-      put4(out + (long long)m * N + n, p.vec != 0, N - n, o);
-    }
+  } else {
+    e.vec = p.vec;
+    joined_epilogue<float, KIND, EACT, BM, BN, WK, RM, RN>(e, acc, smem, wk, wm * WTM, wn * WTN, m0, n0);
   }
 }
 

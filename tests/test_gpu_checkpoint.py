@@ -114,7 +114,8 @@ def test_gradient_activations(M, K, B, storage, operand, unit, act):
 @pytest.mark.parametrize("storage,operand,unit", TYPES[3:])
 @pytest.mark.parametrize("M,K,B", [(1032, 1100, 32), (1100, 2050, 192), (4100, 4000, 64), (3000, 4104, 96), (1032, 1100, 2),
                                    (1032, 1100, 1), (1033, 1101, 63), (1100, 2050, 191), (1100, 2051, 190), (4101, 4000, 65),
-                                   (4100, 4001, 66), (3000, 4104, 98)])
+                                   (4100, 4001, 66), (3000, 4104, 98), (512, 512, 2048), (700, 900, 2051),
+                                   (1000, 1030, 4002)])
 def test_weight_update_widened_once(M, K, B, storage, operand, unit):
     """The 16-bit products on 64, 128 and 256 wide tiles."""
     k = mx.build_checkpoint_weight_update(M, K, B, "sigmoid", DT[storage])
@@ -142,7 +143,8 @@ def test_fp32_gradient(M, K, B):
 
 @pytest.mark.parametrize("storage,operand,unit", TYPES[3:])
 @pytest.mark.parametrize("M,K,B", [(2, 1, 2), (4, 33, 2), (65, 31, 64), (64, 40, 65), (1100, 513, 1002), (1101, 514, 1003),
-                                   (2051, 333, 1000), (4098, 47, 4006), (4097, 65, 4001)])
+                                   (2051, 333, 1000), (4098, 47, 4006), (4097, 65, 4001), (66, 1025, 34), (130, 1089, 70),
+                                   (1000, 1026, 1000), (300, 4001, 301), (1, 4000, 301), (2, 5000, 2)])
 def test_16_bit_gradient(M, K, B, storage, operand, unit):
     """Rows of even and odd lengths, contractions with a rest, on 64, 128 and 256 wide tiles."""
     pads = (M % 2 or B % 2) and M * K * B >= 2 ** 28 and (M % 2 == 0 or B >= 256)
