@@ -19,6 +19,7 @@
 #include <ATen/ops/empty.h>
 #include <torch/csrc/Device.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstring>
@@ -122,12 +123,16 @@ PyObject* call_run(PyObject* self, PyObject* const* argv, size_t nargsf, PyObjec
   c10::DeviceIndex device = -1;
   auto take = [&](PyObject* o) {
     if (got == k.pointers || !THPVariable_Check(o)) return false;
-    const at::Tensor& t = THPVariable_Unpack(o);
-    if (!c.spec[got].is(t)) return false;
-    const c10::DeviceIndex d = t.get_device();
-    if (device >= 0 && d != device) return false;
-    device = d;
-    a.p[got++] = t.data_ptr();
+    try {
+      const at::Tensor& t = THPVariable_Unpack(o);
+      if (!c.spec[got].is(t)) return false;
+      const c10::DeviceIndex d = t.get_device();
+      if (device >= 0 && d != device) return false;
+      device = d;
+      a.p[got++] = t.data_ptr();
+    } catch (const std::exception&) {  // (a tensor without strides or storage)
+      return false;
+    }
     return true;
   };
   Py_ssize_t at = 0;
@@ -146,10 +151,14 @@ PyObject* call_run(PyObject* self, PyObject* const* argv, size_t nargsf, PyObjec
     PyObject* o = argv[at++];
     if (o != Py_None) {
       if (!THPVariable_Check(o)) return refuse;
-      const at::Tensor& t = THPVariable_Unpack(o);
-      if (!t.is_cuda() || !t.is_contiguous()) return refuse;
-      a.workspace = t.data_ptr();
-      a.bytes = (long long)t.nbytes();
+      try {
+        const at::Tensor& t = THPVariable_Unpack(o);
+        if (!t.is_cuda() || !t.is_contiguous()) return refuse;
+        a.workspace = t.data_ptr();
+        a.bytes = (long long)t.nbytes();
+      } catch (const std::exception&) {
+        return refuse;
+      }
     }
   }
   if (at != n) return refuse;
@@ -236,15 +245,11 @@ PyObject* packed_run(PyObject* self, PyObject* const* argv, size_t nargsf, PyObj
     }
     device = reinterpret_cast<THPDevice*>(argv[0])->device;
   }
+  HANDLE_TH_ERRORS  // (no memory, no such device)
   at::Tensor t[2];
-  try {
-    for (int i = 0; i < 2; ++i)
-      t[i] = at::empty(at::IntArrayRef(p.part[i].size, p.part[i].dims),
-                       at::TensorOptions().dtype(p.part[i].type).device(device));
-  } catch (const std::exception& e) {  // (no memory, no such device)
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
-  }
+  for (int i = 0; i < 2; ++i)
+    t[i] = at::empty(at::IntArrayRef(p.part[i].size, p.part[i].dims),
+                     at::TensorOptions().dtype(p.part[i].type).device(device));
   PyObject *codes = THPVariable_Wrap(std::move(t[0])), *scales = codes ? THPVariable_Wrap(std::move(t[1])) : nullptr;
   PyObject* both = scales ? PyTuple_Pack(2, codes, scales) : nullptr;
   PyObject* args = both ? PyTuple_Pack(1, both) : nullptr;
@@ -254,6 +259,7 @@ PyObject* packed_run(PyObject* self, PyObject* const* argv, size_t nargsf, PyObj
   Py_XDECREF(scales);
   Py_XDECREF(codes);
   return pair;
+  END_HANDLE_TH_ERRORS
 }
 
 PyObject* packed_new(PyTypeObject* type, PyObject* args, PyObject*) {

@@ -266,3 +266,51 @@ def test_refusals():
         mx.build_checkpoint_weight_update(16, 32, 64, "relu", torch.bfloat16, operand_dtype=torch.float32)
     with pytest.raises(ValueError, match="workspace"):
         update(w, e, x8, workspace=torch.empty(64))
+
+
+def test_calls_in_a_graph():
+    """Keeping a state, its gradient and its weight update with their workspaces, captured
+    and replayed between eager work: the eager bits every time."""
+    M, K, B = 1101, 1203, 301
+    g = torch.Generator().manual_seed(9)
+    for storage in ("bf16", "fp32"):
+        x, w, e = (_dev(_rand(g, *s, storage=storage), storage) for s in ((K, B), (M, K), (M, B)))
+        save, grad = mx.build_checkpoint_save(K, B, DT[storage]), mx.build_checkpoint_gradient(K, M, B, "silu", DT[storage])
+        update = mx.build_checkpoint_weight_update(M, K, B, "silu", DT[storage], 0.01)
+        x8, out, ws = save.new_output(), torch.empty_like(x), [k.new_workspace() for k in (grad, update)]
+        assert ws[1] is not None and (ws[0] is not None) == (storage == "bf16")
+
+        def calls():
+            save(x, x8)
+            grad(w, e, x8, out, workspace=ws[0])
+            update(w, e, x8, workspace=ws[1])
+
+        start = w.clone()
+        want = []
+        for _ in range(3):
+            calls()
+            want.append((out.clone(), w.clone()))
+        w.copy_(start)
+        side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            calls()
+        for a, b in want:
+            out.zero_()
+            graph.replay()
+            assert torch.equal(out, a) and torch.equal(w, b)
+            torch.cuda.synchronize()
+            save(x * 2, mx.new_packed(K, B, "int8"))
+
+
+def test_no_storage_is_refused():
+    from torch._subclasses import FakeTensorMode
+
+    save = mx.build_checkpoint_save(64, 64)
+    x8 = save.new_output()
+    with FakeTensorMode():
+        fake = torch.empty(64, 64, device="cuda")
+    with pytest.raises((ValueError, RuntimeError)):
+        save(fake, x8)
+    with pytest.raises((ValueError, RuntimeError)):
+        save(torch.zeros(64, 64).to_sparse().cuda(), x8)
