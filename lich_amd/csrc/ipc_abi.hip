@@ -653,12 +653,17 @@ bool ckpt_products32(int storage, int operand, int M, int K, int B) {
 // fp32: evaluating it in every row of tiles costs more than that pass (5-8 us): MI355X,
 // us, from codes / widened and read (relu; silu): 512^3 6.9; 10.3 / 6.2 + 4, 1000 x 1531 x
 // 300 16.9; 25.3 / 15.9 + 4, 2048 x 1024 x 1024 45; 87 / 41 + 5, 2048^3 162; 333 / 137 + 7.
-// 16 bits: for the 16-bit products where there are outputs enough, or outputs and samples,
-// for them to win against the kernels that widen in their loaders, or (lengths those
-// products cannot take) by the same comparison.
-bool ckpt_weight_products(int M, int K, int B, int storage) {
+// 16 bits: for the 16-bit products where there are outputs enough, or outputs and samples
+// (fewer where f has an exponential), for them to win against the kernels that widen in
+// their loaders: MI355X, bf16, us, loaders / products (relu; tanh): 512^2, 512 samples
+// 6.8 / 9.0; 8.3 / 9.8, 700^2, 512 10.4 / 9.7; 12.4 / 10.6, 1024^2, 1024 12.7 / 13.6; 17.4 /
+// 14.4, 1024 x 512, 2048 19.8 / 15.1; 27.1 / 15.7, 1536 x 1024, 320 15.8 / 9.7; 19.3 / 10.6.
+// Or (lengths those products cannot take) by the comparison of fp32.
+bool ckpt_weight_products(int act, int M, int K, int B, int storage) {
   const long long outputs = (long long)M * K;
-  return ckpt_products(storage, M, K, B) && (outputs > (1 << 20) || (outputs >= (1 << 18) && B >= 2048));
+  const bool cheap = act == IPC_ACT_IDENTITY || act == IPC_ACT_RELU;
+  return ckpt_products(storage, M, K, B) && (outputs > (1 << 20) || (outputs >= (1 << 18) && B >= 2048) ||
+                                             (!cheap && outputs >= 480000 && B >= 256));
 }
 long long ckpt_workspace_need(int act, int M, int K, int B, int storage) {
   if (storage == IPC_DT_F32) {
@@ -667,7 +672,7 @@ long long ckpt_workspace_need(int act, int M, int K, int B, int storage) {
     return K * mx_row_values(MX_INT8, B) * 4;
   }
   const long long padded = mx_row_values(MX_INT8, B);
-  if (ckpt_weight_products(M, K, B, storage)) return (K + (B % 2 ? (long long)M : 0LL)) * padded * 2;
+  if (ckpt_weight_products(act, M, K, B, storage)) return (K + (B % 2 ? (long long)M : 0LL)) * padded * 2;
   return s16_preact_rule(S16_WEIGHT, act, M, K, (long long)K * B) ? (long long)K * B * 2 : 0;
 }
 
@@ -725,7 +730,7 @@ int ipc_ckpt_weight_update(void* w, const void* e, const void* x_codes, const vo
     q.vec = vec_ok(w, K, es);
     return launch_rc(launch_ckpt_gemm32(CKPT_WEIGHT, q, act, s), "ipc_ckpt_weight_update");
   }
-  const bool products = ckpt_weight_products(M, K, B, storage);
+  const bool products = ckpt_weight_products(act, M, K, B, storage);
   if (lent && products && (B % 2 || al4(e))) {  // (rows padded as the packed ones are)
     const int n = (int)mx_row_values(MX_INT8, B);
     void* pad = static_cast<char*>(workspace) + (long long)K * n * 2;

@@ -114,7 +114,7 @@ def test_gradient_activations(M, K, B, storage, operand, unit, act):
 @pytest.mark.parametrize("storage,operand,unit", TYPES[3:])
 @pytest.mark.parametrize("M,K,B", [(1032, 1100, 32), (1100, 2050, 192), (4100, 4000, 64), (3000, 4104, 96), (1032, 1100, 2),
                                    (1032, 1100, 1), (1033, 1101, 63), (1100, 2050, 191), (1100, 2051, 190), (4101, 4000, 65),
-                                   (4100, 4001, 66), (3000, 4104, 98), (512, 512, 2048), (700, 900, 2051),
+                                   (4100, 4001, 66), (3000, 4104, 98), (512, 512, 2048), (700, 900, 2051), (700, 690, 257),
                                    (1000, 1030, 4002)])
 def test_weight_update_widened_once(M, K, B, storage, operand, unit):
     """The 16-bit products on 64, 128 and 256 wide tiles."""
