@@ -2,9 +2,9 @@
 //
 // Both directions are one pass over the data, bound by HBM: each value is read
 // once and each code and scale written once.  MI355X, fp32, 4096 x 4096, fp4: columns
-// 16.3 us (76 MB, 4.7 TB/s; a copy of that size runs at 5.2), back 12.6 us; bf16, 4096 x
-// 1024, int8: rows 6.0 us, back 4.4 (13 MB, 2-3 TB/s: mostly the launch and one
-// memory latency).
+// 15.5 us (76 MB, 4.9 TB/s; a copy of that size runs at 5.2), back 12.9 us; bf16, 4096 x
+// 1024, int8: rows 4.0 us, back 3.5 (13 MB, 3-4 TB/s, launches included; one of a few
+// KB takes 2.9).
 #include "ipc_launch.h"
 #include "ipc_mx_device.h"
 
@@ -13,22 +13,22 @@ namespace {
 
 // The row kernels: a workgroup takes 256 values (two groups, so that the fp4
 // codes it stores are whole 128-byte lines) of a few rows, a lane EPL consecutive
-// ones (16 bytes), in 4 passes whose loads are issued together.
-constexpr int WIDTH = 2 * MX_GROUP, PASSES = 4;
+// ones (16 bytes), in one pass or four whose loads are issued together.
+constexpr int WIDTH = 2 * MX_GROUP;
 template <typename ST> constexpr int EPL = 16 / (int)sizeof(ST);           // values per lane
 template <typename ST> constexpr int ROW_LANES = WIDTH / EPL<ST>;          // lanes per row
 template <typename ST> constexpr int PASS_ROWS = 256 / ROW_LANES<ST>;      // rows per pass
-template <typename ST> constexpr int TILE_ROWS = PASSES * PASS_ROWS<ST>;   // rows per workgroup
+template <typename ST, int PASSES> constexpr int TILE_ROWS = PASSES * PASS_ROWS<ST>;  // rows per workgroup
 
 // Packed rows are the rows of x.  A block's lanes (4, or 8 of fp32) sit side by
 // side: its largest magnitude comes from exchanges within them.
-template <typename ST, int FMT>
+template <typename ST, int FMT, int PASSES>
 __global__ void __launch_bounds__(256) mx_quant_rows_kernel(const ST* __restrict__ x, uint8_t* __restrict__ codes,
                                                             uint8_t* __restrict__ scales, int R, int C,
                                                             int row_bytes, int spans, int act) {
   constexpr int E = EPL<ST>;
   const int c = blockIdx.x % spans * WIDTH + threadIdx.x % ROW_LANES<ST> * E;
-  const int r0 = blockIdx.x / spans * TILE_ROWS<ST> + threadIdx.x / ROW_LANES<ST>;
+  const int r0 = blockIdx.x / spans * TILE_ROWS<ST, PASSES> + threadIdx.x / ROW_LANES<ST>;
   const int groups = mx_groups(C), kg = c / MX_GROUP;
   float v[PASSES][E];
 #pragma unroll
@@ -37,7 +37,7 @@ __global__ void __launch_bounds__(256) mx_quant_rows_kernel(const ST* __restrict
     const ST* p = x + (long long)r * C + c;
 #pragma unroll
     for (int i = 0; i < E; ++i) v[u][i] = 0.0f;
-    if (r < R && c + E <= C) {
+    if (r < R && c < C && (c + E <= C || r + 1 < R)) {  // (past the row's end: the next row's, cleared below)
       mx::load_run<ST, E>(p, v[u]);
     } else if (r < R) {
 #pragma unroll
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(256) mx_quant_cols_kernel(const ST* __restrict
 #pragma unroll
       for (int i = 0; i < VEC; ++i) v[u][i] = (ST)0.0f;
       const ST* p = x + (long long)k * N + n;
-      if (k < K && n + VEC <= N) {
+      if (k < K && n < N && (n + VEC <= N || k + 1 < K)) {  // (past the row's end: the next row's, never stored)
         v[u] = reinterpret_cast<const typename mx::Run<ST, VEC>::U*>(p)->v;
       } else if (k < K) {
 #pragma unroll
@@ -165,78 +165,77 @@ __global__ void __launch_bounds__(256) mx_quant_cols_kernel(const ST* __restrict
   }
 }
 
-// f of packed rows into out [R][C], lanes and passes as in mx_quant_rows_kernel.
+// f of packed rows into out [R][C], lanes as in mx_quant_rows_kernel.
 template <typename ST, int FMT>
 __global__ void __launch_bounds__(256) mx_dequant_kernel(const uint8_t* __restrict__ codes,
                                                          const uint8_t* __restrict__ scales, ST* __restrict__ out,
                                                          int R, int C, int row_bytes, int spans, int act) {
   constexpr int E = EPL<ST>;
   const int c = blockIdx.x % spans * WIDTH + threadIdx.x % ROW_LANES<ST> * E;
-  const int r0 = blockIdx.x / spans * TILE_ROWS<ST> + threadIdx.x / ROW_LANES<ST>;
-  if (c >= C) return;
-  unsigned q[PASSES][2], s[PASSES];
-#pragma unroll
-  for (int u = 0; u < PASSES; ++u) {
-    const int r = r0 + u * PASS_ROWS<ST>;
-    q[u][0] = q[u][1] = s[u] = 0;
-    if (r < R) {
-      const uint8_t* row = codes + (long long)r * row_bytes;
-      if constexpr (FMT == MX_FP4 && E == 8) {
-        q[u][0] = *reinterpret_cast<const unsigned*>(row + c / 2);
-      } else if constexpr (FMT == MX_FP4) {
-        q[u][0] = *reinterpret_cast<const unsigned short*>(row + c / 2);
-      } else if constexpr (E == 8) {
-        const uint2 t = *reinterpret_cast<const uint2*>(row + c);
-        q[u][0] = t.x; q[u][1] = t.y;
-      } else {
-        q[u][0] = *reinterpret_cast<const unsigned*>(row + c);
-      }
-      s[u] = scales[((long long)(c / MX_GROUP) * R + r) * 4 + (c / MX_BLOCK & 3)];
+  const int r = blockIdx.x / spans * PASS_ROWS<ST> + threadIdx.x / ROW_LANES<ST>;
+  if (c >= C || r >= R) return;
+  const uint8_t* row = codes + (long long)r * row_bytes;
+  const unsigned s = scales[((long long)(c / MX_GROUP) * R + r) * 4 + (c / MX_BLOCK & 3)];
+  float v[E];
+  if constexpr (FMT == MX_FP4) {
+    unsigned q;
+    if constexpr (E == 8) q = *reinterpret_cast<const unsigned*>(row + c / 2);
+    else q = *reinterpret_cast<const unsigned short*>(row + c / 2);
+    mx::fp4_values<E>(q, s, v);
+  } else {
+    unsigned q[E / 4];
+    if constexpr (E == 8) {
+      const uint2 t = *reinterpret_cast<const uint2*>(row + c);
+      q[0] = t.x; q[1] = t.y;
+    } else {
+      q[0] = *reinterpret_cast<const unsigned*>(row + c);
     }
+    const float unit = mx::int8_scale(s);
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = (float)mx::sext8(q[i / 4], i & 3) * unit;
   }
+  activate<E>(act, v);
+  ST* p = out + (long long)r * C + c;
+  if (c + E <= C) {
+    mx::store_run<ST, E>(p, v);
+  } else {
 #pragma unroll
-  for (int u = 0; u < PASSES; ++u) {
-    const int r = r0 + u * PASS_ROWS<ST>;
-    if (r >= R) continue;
-    float v[E];
-    if constexpr (FMT == MX_FP4) {
-      mx::fp4_values<E>(q[u][0], s[u], v);
-    } else {
-      const float unit = mx::int8_scale(s[u]);
-#pragma unroll
-      for (int i = 0; i < E; ++i) v[i] = (float)mx::sext8(q[u][i / 4], i & 3) * unit;
-    }
-    activate<E>(act, v);
-    ST* p = out + (long long)r * C + c;
-    if (c + E <= C) {
-      mx::store_run<ST, E>(p, v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < E; ++i)
-        if (c + i < C) p[i] = cvt<ST>(v[i]);
-    }
+    for (int i = 0; i < E; ++i)
+      if (c + i < C) p[i] = cvt<ST>(v[i]);
   }
 }
 
+// Four passes a workgroup for large fp32 matrices, else one: shorter code, which small
+// calls spend their time to fetch, and more workgroups.  MI355X, us, one / four: fp32 fp4
+// 784 x 128 2.9 / 3.3, 2048 x 1024 3.2 / 3.3, 4096 x 2048 7.4 / 6.0; bf16 int8 784 x 128 2.9 /
+// 5.0, 4096 x 1024 4.0 / 4.8, 8192 x 8192 33 / 39.
 template <typename ST, int FMT>
 hipError_t quantize(const void* x, void* codes, void* scales, int R, int C, int axis, int act, hipStream_t s) {
   const int rows = axis == 1 ? R : C, n = axis == 1 ? C : R;
-  const int spans = (mx_groups(n) + 1) / 2, per = axis == 1 ? TILE_ROWS<ST> : 128 / (int)sizeof(ST);
-  const long long tiles = (rows + (long long)per - 1) / per, blocks = spans * tiles;
+  const int spans = (mx_groups(n) + 1) / 2;
+  const long long four = (rows + TILE_ROWS<ST, 4> - 1LL) / TILE_ROWS<ST, 4>;
+  const bool passes = sizeof(ST) == 4 && four * spans >= 1024;
+  const long long tiles = axis == 0 ? (rows * (long long)sizeof(ST) + 127) / 128
+                          : passes  ? four : (rows + TILE_ROWS<ST, 1> - 1LL) / TILE_ROWS<ST, 1>;
+  const long long blocks = spans * tiles;
   const int row_bytes = (int)mx_row_bytes(FMT, n);
-  hipLaunchKernelGGL((axis == 1 ? mx_quant_rows_kernel<ST, FMT> : mx_quant_cols_kernel<ST, FMT>),
-                     dim3((unsigned)blocks), dim3(256), 0, s, static_cast<const ST*>(x), static_cast<uint8_t*>(codes),
-                     static_cast<uint8_t*>(scales), R, C, row_bytes, axis == 1 ? spans : (int)tiles, act);
+  auto kernel = axis == 0 ? mx_quant_cols_kernel<ST, FMT> : mx_quant_rows_kernel<ST, FMT, 1>;
+  if constexpr (sizeof(ST) == 4) {
+    if (axis == 1 && passes) kernel = mx_quant_rows_kernel<ST, FMT, 4>;
+  }
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, s, static_cast<const ST*>(x),
+                     static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), R, C, row_bytes,
+                     axis == 1 ? spans : (int)tiles, act);
   return hipGetLastError();
 }
 
 template <typename ST, int FMT>
 hipError_t dequantize(const void* codes, const void* scales, void* out, int R, int C, int act, hipStream_t s) {
   const int spans = (mx_groups(C) + 1) / 2;
-  const long long blocks = (long long)spans * ((R + (long long)TILE_ROWS<ST> - 1) / TILE_ROWS<ST>);
+  const long long blocks = spans * ((R + PASS_ROWS<ST> - 1LL) / PASS_ROWS<ST>);
   hipLaunchKernelGGL((mx_dequant_kernel<ST, FMT>), dim3((unsigned)blocks), dim3(256), 0, s,
-                     static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), static_cast<ST*>(out), R,
-                     C, (int)mx_row_bytes(FMT, C), spans, act);
+                     static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), static_cast<ST*>(out), R, C,
+                     (int)mx_row_bytes(FMT, C), spans, act);
   return hipGetLastError();
 }
 
