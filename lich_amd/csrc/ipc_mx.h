@@ -37,6 +37,12 @@ inline long long mx_row_bytes(int format, int n) {
   return format == MX_FP4 ? mx_row_values(format, n) / 2 : mx_row_values(format, n);
 }
 __host__ __device__ inline int mx_groups(int n) { return (int)(((long long)n + MX_GROUP - 1) / MX_GROUP); }
+// Whether `run` values from column c of a row lie inside a matrix whose rows of n end
+// `rows_left` rows from this one on (this one counted; 0 or less: none).  A row's end may
+// be read past, into the rows after it: of narrow ones a run takes several.
+__host__ __device__ inline bool mx_run_inside(int rows_left, int n, int c, int run) {
+  return rows_left > 0 && c < n && (c + run <= n || rows_left * (long long)n >= c + run);
+}
 
 // axis 1: rows of x [R][C] are the packed rows; axis 0: its columns.
 hipError_t launch_mx_quantize(const void* x, void* codes, void* scales, int R, int C, int axis, int format,

@@ -37,7 +37,7 @@ __global__ void __launch_bounds__(256) mx_quant_rows_kernel(const ST* __restrict
     const ST* p = x + (long long)r * C + c;
 #pragma unroll
     for (int i = 0; i < E; ++i) v[u][i] = 0.0f;
-    if (r < R && c < C && (c + E <= C || r + 1 < R)) {  // (past the row's end: the next row's, cleared below)
+    if (mx_run_inside(R - r, C, c, E)) {  // (past the row's end: the next rows' values, cleared below)
       mx::load_run<ST, E>(p, v[u]);
     } else if (r < R) {
 #pragma unroll
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(256) mx_quant_cols_kernel(const ST* __restrict
 #pragma unroll
       for (int i = 0; i < VEC; ++i) v[u][i] = (ST)0.0f;
       const ST* p = x + (long long)k * N + n;
-      if (k < K && n < N && (n + VEC <= N || k + 1 < K)) {  // (past the row's end: the next row's, never stored)
+      if (mx_run_inside(K - k, N, n, VEC)) {  // (past the row's end: the next rows' values, never stored)
         v[u] = reinterpret_cast<const typename mx::Run<ST, VEC>::U*>(p)->v;
       } else if (k < K) {
 #pragma unroll

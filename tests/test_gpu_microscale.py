@@ -54,6 +54,27 @@ def test_quantize_is_the_definition(R, C, axis, storage, fmt):
 
 
 @pytest.mark.parametrize("fmt", ["fp4", "int8"])
+@pytest.mark.parametrize("storage", ["fp32", "bf16"])
+@pytest.mark.parametrize("R,C", [(10, 1), (9, 2), (257, 2), (10, 3), (66, 5), (7, 7), (129, 9)])
+def test_quantize_of_narrow_matrices(R, C, storage, fmt):
+    """A load of 16 bytes spans several rows: both axes, what comes back against the oracle."""
+    g = torch.Generator().manual_seed(R * 31 + C)
+    xd = _dev(_rand(g, R, C), storage)
+    x = _up(xd)
+    for axis in (0, 1):
+        k = mx.build_mx_quantize(R, C, "identity", DT[storage], format=fmt, axis=axis)
+        out = k.new_output()
+        k(xd, out)
+        codes, scales = O.pack(x if axis == 1 else x.T.contiguous(), fmt)
+        assert torch.equal(out.scales.cpu(), scales)
+        back, want = (torch.empty(k.rows, k.length, dtype=DT[storage], device="cuda") for _ in range(2))
+        restore = mx.build_mx_dequantize(k.rows, k.length, DT[storage], format=fmt)
+        restore(out, back)
+        restore(mx.MXMatrix(codes.cuda(), scales.cuda()), want)
+        assert torch.equal(back, want)
+
+
+@pytest.mark.parametrize("fmt", ["fp4", "int8"])
 @pytest.mark.parametrize("axis", [0, 1])
 def test_quantize_ties_edges_and_specials(fmt, axis):
     """Midpoints and their neighbours, the largest and smallest floats, zeros,

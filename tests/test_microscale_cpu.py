@@ -129,3 +129,32 @@ def test_fast_calls_refuse():
         fast.Packed((2, 64), torch.uint8, (1, 2, 4), torch.uint8, list)
     with pytest.raises(TypeError):
         fast.Packed((2, 64), torch.uint8, (1, 2, 4), torch.uint8, mx.MXMatrix)("cuda")
+
+
+def test_quantiser_run_lies_inside_the_matrix(tmp_path):
+    """The bound of the quantiser's 16-byte loads, as compiled from ipc_mx.h: no value
+    of a run lies past the matrix's last one, down to rows of a single value."""
+    import re
+    import subprocess
+    from pathlib import Path
+
+    csrc = Path(__file__).resolve().parents[1] / "lich_amd" / "csrc"
+    body = re.search(r"inline bool mx_run_inside\(.*?\n}\n", (csrc / "ipc_mx.h").read_text(), re.S).group(0)
+    assert (csrc / "ipc_mx_quant.hip").read_text().count("mx_run_inside(") == 2  # rows, columns
+    source = tmp_path / "inside.cpp"
+    source.write_text(body + """
+int main() {
+  for (int rows = 1; rows <= 20; ++rows)
+    for (int n = 1; n <= 20; ++n)
+      for (int r = -2; r < rows + 3; ++r)
+        for (int c = 0; c < 32; c += 4)
+          for (int run = 4; run <= 8; run += 4) {
+            const bool all = r >= 0 && r < rows && c < n && r * n + c + run <= rows * n;
+            if (r >= 0 && mx_run_inside(rows - r, n, c, run) != all) return 1;
+          }
+  return mx_run_inside(1 << 24, 127, 120, 8) ? 0 : 2;
+}
+""")
+    program = tmp_path / "inside"
+    subprocess.run(["g++", "-std=c++17", "-o", str(program), str(source)], check=True)
+    assert subprocess.run([str(program)]).returncode == 0
