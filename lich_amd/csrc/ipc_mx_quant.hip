@@ -2,9 +2,9 @@
 //
 // Both directions are one pass over the data, bound by HBM: each value is read
 // once and each code and scale written once.  MI355X, fp32, 4096 x 4096, fp4: columns
-// 15.5 us (76 MB, 4.9 TB/s; a copy of that size runs at 5.2), back 12.9 us; bf16, 4096 x
-// 1024, int8: rows 4.0 us, back 3.5 (13 MB, 3-4 TB/s, launches included; one of a few
-// KB takes 2.9).
+// 18.6 us from memory (76 MB, 4.1 TB/s; a copy runs at 5.2), 14.3 from the caches, back
+// 12.8; bf16, 4096 x 1024, int8: rows 4.0 us, back 3.5 (13 MB, 3-4 TB/s, launches
+// included; one of a few KB takes 2.7-2.9).
 #include "ipc_launch.h"
 #include "ipc_mx_device.h"
 
@@ -78,29 +78,32 @@ __global__ void __launch_bounds__(256) mx_quant_rows_kernel(const ST* __restrict
   }
 }
 
-// Packed rows are the columns of x [K][N].  A workgroup stages 256 k-rows of 32
+// Packed rows are the columns of x [K][N].  A workgroup stages 128 k-rows of 32
 // dwords (128 bytes of a row: 32 fp32 or 64 16-bit columns) in LDS with 16-byte
-// loads; then each thread owns a dword column and one of the eight blocks: its
-// 32 values are in its registers, so the block's scale needs no exchange, and its
-// codes are 16 (fp4) or 32 bytes of a packed row, the eight blocks of a row side
-// by side.  Dword w of k-row k (block b = k / 32) lies in row k ^ (b & 1) at w + 8 (b
-// / 2) (mod 32): a wave reads 8 dwords of each of the 8 blocks from 64 different
-// banks.
+// loads; then each thread owns a dword column and one of the eight half blocks, the
+// other half in the neighbouring lane: 8 (fp4) or 16 bytes of a packed row, the eight of
+// a row side by side.  Dword w of k-row k (half block b = k / 16) lies in row k ^ (b & 1) at
+// w + 8 (b / 2) (mod 32): a wave reads 8 dwords of each of the 8 from 64 different
+// banks.  Whole blocks a thread (no exchange, half as many workgroups, twice the LDS) were
+// slower but for the largest, us from memory, half / whole: fp4, fp32 784 x 128 2.7 / 4.6,
+// 4096 x 4096 18.6 / 20.5, bf16 4096 x 1024 5.4 / 5.9, 8192 x 2048 11.8 / 13.1, 8192 x 8192 42.5 /
+// 40.9; from the caches that one 27.8 / 32.5, and int8 35 / 42.
 template <typename ST, int FMT>
 __global__ void __launch_bounds__(256) mx_quant_cols_kernel(const ST* __restrict__ x, uint8_t* __restrict__ codes,
                                                             uint8_t* __restrict__ scales, int K, int N,
                                                             int row_bytes, int tiles, int act) {
   constexpr int VPD = 4 / sizeof(ST);  // columns per dword
   constexpr int COLS = 32 * VPD, VEC = 16 / sizeof(ST);
-  __shared__ __align__(16) unsigned tile[WIDTH * 32];
-  const int n0 = blockIdx.x % tiles * COLS, k0 = blockIdx.x / tiles * WIDTH;  // (whole rows at once)
+  constexpr int V = MX_BLOCK / 2, LOADS = MX_GROUP / 32;  // values of a thread's run, its 16-byte loads
+  __shared__ __align__(16) unsigned tile[MX_GROUP * 32];
+  const int n0 = blockIdx.x % tiles * COLS, k0 = blockIdx.x / tiles * MX_GROUP;  // (whole rows at once)
   const int tid = threadIdx.x;
   {
-    typedef typename mx::Run<ST, VEC>::V V;
+    typedef typename mx::Run<ST, VEC>::V Vec;
     const int j = tid & 7, n = n0 + j * VEC;
-    V v[8];
+    Vec v[LOADS];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
+    for (int u = 0; u < LOADS; ++u) {
       const int k = k0 + u * 32 + (tid >> 3);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) v[u][i] = (ST)0.0f;
@@ -114,53 +117,52 @@ __global__ void __launch_bounds__(256) mx_quant_cols_kernel(const ST* __restrict
       }
     }
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
-      *reinterpret_cast<V*>(&tile[((u * 32 + (tid >> 3)) ^ (u & 1)) * 32 + ((j * 4 + 8 * (u >> 1)) & 31)]) = v[u];
+    for (int u = 0; u < LOADS; ++u) {
+      const int k = u * 32 + (tid >> 3), run = k / V;
+      *reinterpret_cast<Vec*>(&tile[(k ^ (run & 1)) * 32 + ((j * 4 + 8 * (run >> 1)) & 31)]) = v[u];
+    }
   }
   __syncthreads();
-  const int w = tid >> 3, blk = tid & 7;
-  const int left = K - k0 - blk * 32;  // values of this block
-  if (k0 + (blk & 4) * 32 >= K) return;  // a group past the end
-  unsigned d[32];
-  const unsigned* at = &tile[blk * 32 * 32 + ((w + 8 * (blk >> 1)) & 31)];
-  const unsigned *even = at + (blk & 1) * 32, *odd = at - (blk & 1) * 32;  // rows i and i ^ 1
+  const int w = tid >> 3, run = tid & 7;
+  const int k = k0 + run * V, left = K - k;  // the run's first k; values of it
+  unsigned d[V];
+  const unsigned* at = &tile[run * V * 32 + ((w + 8 * (run >> 1)) & 31)];
+  const unsigned *even = at + (run & 1) * 32, *odd = at - (run & 1) * 32;  // rows i and i ^ 1
 #pragma unroll
-  for (int i = 0; i < 32; ++i) d[i] = (i & 1 ? odd : even)[i * 32];
-  const int kg = (k0 + blk * 32) / MX_GROUP;
+  for (int i = 0; i < V; ++i) d[i] = (i & 1 ? odd : even)[i * 32];
+  const int kg = k0 / MX_GROUP;
 #pragma unroll
   for (int c = 0; c < VPD; ++c) {
     const int n = n0 + w * VPD + c;
     if (n >= N) break;
-    float v[32];
+    float v[V];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
+    for (int i = 0; i < V; ++i) {
       if constexpr (VPD == 1) v[i] = __builtin_bit_cast(float, d[i]);
       else v[i] = h2f(c == 0 ? d[i] & 0xffffu : d[i] >> 16, (ST*)nullptr);
     }
-    activate<32>(act, v);
-    if (left < 32) {  // (f(0) need not be 0: padding stays zero)
+    activate<V>(act, v);
+    if (left < V) {  // (f(0) need not be 0: padding stays zero)
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
+      for (int i = 0; i < V; ++i)
         if (i >= left) v[i] = 0.0f;
     }
     unsigned m = 0;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) m = max(m, mx::abs_bits(v[i]));
+    for (int i = 0; i < V; ++i) m = max(m, mx::abs_bits(v[i]));
+    m = max(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xf, 0xf, true));  // quad lanes 1 0 3 2
     const unsigned s = mx::scale_byte<FMT>(m);
-    scales[((long long)kg * N + n) * 4 + (blk & 3)] = (uint8_t)s;
+    if (!(run & 1)) scales[((long long)kg * N + n) * 4 + (k / MX_BLOCK & 3)] = (uint8_t)s;
     uint8_t* row = codes + (long long)n * row_bytes;
     if constexpr (FMT == MX_FP4) {
+      const unsigned lo = mx::fp4_codes<8>(*reinterpret_cast<const float (*)[8]>(&v[0]), s);
+      const unsigned hi = mx::fp4_codes<8>(*reinterpret_cast<const float (*)[8]>(&v[8]), s);
+      *reinterpret_cast<uint2*>(row + k / 2) = make_uint2(lo, hi);
+    } else if (k < row_bytes) {
       unsigned q[4];
 #pragma unroll
-      for (int h = 0; h < 4; ++h) q[h] = mx::fp4_codes<8>(*reinterpret_cast<const float (*)[8]>(&v[h * 8]), s);
-      *reinterpret_cast<uint4*>(row + (k0 + blk * 32) / 2) = make_uint4(q[0], q[1], q[2], q[3]);
-    } else if (k0 + blk * 32 < row_bytes) {
-      unsigned q[8];
-#pragma unroll
-      for (int h = 0; h < 8; ++h) q[h] = mx::int8_codes4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3], s);
-      uint4* o = reinterpret_cast<uint4*>(row + k0 + blk * 32);
-      o[0] = make_uint4(q[0], q[1], q[2], q[3]);
-      o[1] = make_uint4(q[4], q[5], q[6], q[7]);
+      for (int h = 0; h < 4; ++h) q[h] = mx::int8_codes4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3], s);
+      *reinterpret_cast<uint4*>(row + k) = make_uint4(q[0], q[1], q[2], q[3]);
     }
   }
 }
@@ -212,7 +214,7 @@ __global__ void __launch_bounds__(256) mx_dequant_kernel(const uint8_t* __restri
 template <typename ST, int FMT>
 hipError_t quantize(const void* x, void* codes, void* scales, int R, int C, int axis, int act, hipStream_t s) {
   const int rows = axis == 1 ? R : C, n = axis == 1 ? C : R;
-  const int spans = (mx_groups(n) + 1) / 2;
+  const int spans = axis == 0 ? mx_groups(n) : (mx_groups(n) + 1) / 2;
   const long long four = (rows + TILE_ROWS<ST, 4> - 1LL) / TILE_ROWS<ST, 4>;
   const bool passes = sizeof(ST) == 4 && four * spans >= 1024;
   const long long tiles = axis == 0 ? (rows * (long long)sizeof(ST) + 127) / 128
