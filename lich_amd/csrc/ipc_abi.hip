@@ -649,6 +649,16 @@ bool ckpt_products32(int storage, int operand, int M, int K, int B) {
          (long long)K * B < limit - (long long)K * 32;
 }
 
+// Whether a weight update of few samples streams W past rank-B sums (ipc_outer.hip).
+// MI355X, us, the kernels below / this: bf16 8192 x 8192, 1 sample 68 / 44, 3000 x 3100, 2 14.7 /
+// 10.7, 3001 x 3101, 3 24.5 / 19.4, 1000 x 1531, 5 13.5 / 5.9, 4096 x 4096, 8 17.0 / 18.0, 16
+// 17.0 / 25.6; fp32 8192 x 8192, 1 97 / 78, 256 x 784, 4 4.1 / 3.7, 4096 x 4096, 8 28.4 / 23.4,
+// 16 28.3 / 29.2, and where W's rows are loaded value by value 3001 x 3101, 3 15.9 / 24.5.
+bool ckpt_outer(const void* w, int M, int K, int B, int storage, int operand) {
+  if (storage != operand || M > 16 * 65535) return false;  // (16 rows a grid row)
+  return storage == IPC_DT_F32 ? B <= 8 && vec_ok(w, K, 4) : B <= 5;
+}
+
 // The weight update's workspace: f(X) widened once to the storage type.
 // fp32: evaluating it in every row of tiles costs more than that pass (5-8 us): MI355X,
 // us, from codes / widened and read (relu; silu): 512^3 6.9; 10.3 / 6.2 + 4, 1000 x 1531 x
@@ -714,6 +724,11 @@ int ipc_ckpt_weight_update(void* w, const void* e, const void* x_codes, const vo
   TRY(check_ptr(w, "w", es));
   TRY(check_ptr(e, "e", es));
   hipStream_t s = (hipStream_t)stream;
+  if (ckpt_outer(w, M, K, B, storage, operand)) {
+    OuterProblem q = make_outer(w, e, x_codes, M, K, B, 1, alpha, 1, act);
+    q.x_scales = static_cast<const unsigned char*>(x_scales);
+    return launch_rc(launch_outer(q, storage, s), "ipc_ckpt_weight_update");
+  }
   const long long need = ckpt_workspace_need(act, M, K, B, storage);
   const bool lent = need > 0 && workspace && workspace_bytes >= need;
   if (ckpt_products32(storage, operand, M, K, B)) {

@@ -63,6 +63,7 @@ struct OuterProblem {
   const void* x; long long x_gs;
   float alpha;
   int act;  // ACT_IDENTITY for a saved activation
+  const unsigned char* x_scales;  // of an X kept in 8 bits, x its codes; else nullptr
 };
 
 hipError_t launch_outer(const OuterProblem& p, int storage, hipStream_t s);

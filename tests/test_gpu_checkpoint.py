@@ -92,6 +92,15 @@ def test_weight_update(M, K, B, storage, operand, unit):
 
 
 @pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("storage", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("M,K,B", [(1, 4, 1), (3, 65, 2), (64, 784, 4), (65, 260, 5), (130, 1028, 8), (2100, 1300, 3), (2101, 1303, 5)])
+def test_weight_update_of_few_samples(M, K, B, storage, act):
+    """Rank-B sums past W, operands not rounded where the samples are few enough."""
+    few = B <= 8 and K % 4 == 0 if storage == "fp32" else B <= 5
+    _weight(M, K, B, storage, storage, 0.0 if few or storage == "fp32" else O.UNIT[storage], act)
+
+
+@pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("storage,operand,unit", TYPES)
 @pytest.mark.parametrize("M,K,B", [(33, 31, 65), (1100, 2050, 192)])
 def test_weight_update_activations(M, K, B, storage, operand, unit, act):
