@@ -44,6 +44,15 @@ __host__ __device__ inline bool mx_run_inside(int rows_left, int n, int c, int r
   return rows_left > 0 && c < n && (c + run <= n || rows_left * (long long)n >= c + run);
 }
 
+// Bytes of the buffer from `mis` bytes before element `first` of a tensor to its end,
+// element `end`.  Loads take whole dwords (16-bit rows of any length), so their limit is
+// rounded up to the one that holds the last element.  A store's is exact: it is all that
+// keeps rows past the tensor's last one from the memory behind it.
+__host__ __device__ inline long long mx_rows_bytes(long long first, long long end, int element, unsigned mis, bool store) {
+  const long long bytes = end <= first ? 0 : (end - first) * element + mis;
+  return store ? bytes : (bytes + 3) & ~3LL;
+}
+
 // axis 1: rows of x [R][C] are the packed rows; axis 0: its columns.
 hipError_t launch_mx_quantize(const void* x, void* codes, void* scales, int R, int C, int axis, int format,
                               int storage, int act, hipStream_t s);

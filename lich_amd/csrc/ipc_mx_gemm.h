@@ -203,8 +203,9 @@ constexpr int tile_smem() {
 template <typename ST, bool VEC> struct Raw4 { unsigned v[sizeof(ST) == 4 ? 4 : VEC ? 2 : 3]; };
 
 // Rows of a tensor from a uniform element offset `first` on, behind a buffer
-// resource that ends with the tensor's last row: 32-bit offsets, and accesses
-// past the end give 0 or store nothing.  Buffer accesses need dwords only, so fp32
+// resource that ends with the tensor's last row (mx_rows_bytes): 32-bit offsets, loads
+// past the end give 0 or the rest of the last dword, stores past it store nothing.
+// Buffer accesses need dwords only, so fp32
 // rows of any length are read 16 bytes at a time; VEC: 16-bit rows whose length
 // and base are multiples of 4 elements.  Other 16-bit rows are read as the three
 // dwords around their 4 elements and shifted, and stored element by element.
@@ -217,10 +218,10 @@ struct Rows {
   typedef unsigned U3 __attribute__((ext_vector_type(3)));
   __amdgpu_buffer_rsrc_t r;
   unsigned mis;  // bytes from the resource's start to element `first` (0 or 2)
-  __device__ __forceinline__ Rows(const void* base, long long first, long long end) {
+  __device__ __forceinline__ Rows(const void* base, long long first, long long end, bool store = false) {
     const unsigned long long at = reinterpret_cast<unsigned long long>(static_cast<const ST*>(base) + first);
     mis = !VEC && ES == 2 ? (unsigned)(at & 2) : 0u;
-    const long long bytes = end <= first ? 0 : ((end - first) * (long long)ES + mis + (ES == 2 ? 2 : 0)) & ~3LL;
+    const long long bytes = mx_rows_bytes(first, end, ES, mis, store);
     r = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(at - mis), (short)0,
                                           (int)(unsigned)(bytes < 0xffffff00LL ? bytes : 0xffffff00LL), 0x00020000);
   }
@@ -338,7 +339,7 @@ __device__ __forceinline__ void tile_epilogue(const MxProblem& p, const f32x16 (
     // (the wave's own LDS accesses complete in order; the fence keeps the compiler from reordering them)
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     const long long first = (mw + v * 16) * N + nw;
-    const Rows<ST, VEC> dst(p.out, first, end);
+    const Rows<ST, VEC> dst(p.out, first, end, true);
 #pragma unroll
     for (int u = 0; u < PASSES; ++u) {
       const float4 t4 = *reinterpret_cast<const float4*>(es + (set * 16 + u * RPP + er) * LDE + ec);

@@ -158,3 +158,41 @@ int main() {
     program = tmp_path / "inside"
     subprocess.run(["g++", "-std=c++17", "-o", str(program), str(source)], check=True)
     assert subprocess.run([str(program)]).returncode == 0
+
+
+def test_rows_past_the_last_are_not_stored(tmp_path):
+    """The limits of the tiles' buffers, as compiled from ipc_mx.h: loads reach every element,
+    stores none past the last one, whatever the rows' length and the base's dword half."""
+    import re
+    import subprocess
+    from pathlib import Path
+
+    csrc = Path(__file__).resolve().parents[1] / "lich_amd" / "csrc"
+    body = re.search(r"inline long long mx_rows_bytes\(.*?\n}\n", (csrc / "ipc_mx.h").read_text(), re.S).group(0)
+    kernel = (csrc / "ipc_mx_gemm.h").read_text()
+    assert "mx_rows_bytes(first, end, ES, mis, store)" in kernel and "dst(p.out, first, end, true)" in kernel
+    source = tmp_path / "rows.cpp"
+    source.write_text(body + """
+int main() {
+  for (int M = 1; M <= 70; ++M)
+    for (int N = 1; N <= 70; ++N)
+      for (int half = 0; half < 2; ++half)  // the base's element within its dword
+        for (int row = 0; row < 128; row += 16)
+          for (int col = 0; col < N; col += 32) {
+            const long long first = (long long)row * N + col, end = (long long)M * N;
+            const unsigned mis = (unsigned)((first + half) * 2) & 2u;
+            const long long loads = mx_rows_bytes(first, end, 2, mis, false), stores = mx_rows_bytes(first, end, 2, mis, true);
+            if (loads % 4 || loads < stores || loads - stores > 2) return 1;
+            for (int r = 0; r < 16; ++r)
+              for (int c = col; c < N && c < col + 32; ++c) {
+                const unsigned at = (unsigned)(r * N + c - col) * 2u + mis;
+                if ((at < stores) != (row + r < M)) return 2;
+                if (row + r < M && at + 2 > loads) return 3;
+              }
+          }
+  return mx_rows_bytes(5, 9, 4, 0, false) == 16 && mx_rows_bytes(9, 5, 4, 0, true) == 0 ? 0 : 4;
+}
+""")
+    program = tmp_path / "rows"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-o", str(program), str(source)], check=True)
+    assert subprocess.run([str(program)]).returncode == 0
