@@ -192,8 +192,8 @@ __global__ void __launch_bounds__(WGM * WGN * WK * 64) ckpt_gemm_kernel(const Ck
   V fa[2][RM], fb[2][RN];
   auto stage = [&](int kt) -> unsigned char* { return ring + (kt & (STAGES - 1)) * STAGE; };
 
-  // prologue: stages 0 .. 2.  The last 1 .. 32 k are stage 0; a load that reaches past
-  // the operand's end there has all of its offset in the lane's, which is checked.
+  // prologue: stages 0 .. 2.  The last 1 .. 32 k are stage 0; what a load there has past
+  // the operand's end is 0, as it is where a whole stage's last row is shorter than a load.
   if (G == 1) {  // (no other stage: its loads take the operands' first values)
 #pragma unroll
     for (int q = 0; q < IA; ++q) oa[q] = 0;

@@ -15,7 +15,7 @@
 //     where a row ends inside one they bring the next row's first values, which no
 //     stored output reads.
 //   * The operands' last 1 .. 16 k come first, as stage 0, whose offsets are the
-//     lanes' own and checked against the operand's end; what the stage has no k
+//     lanes' own; loads past the operand's end give 0; what the stage has no k
 //     for is cleared in LDS before anything is read.  The loop knows whole stages inside
 //     the operands only.
 //   * CODES32 keeps X in 8 bits up to the fragment and evaluates f there, in every row
@@ -163,8 +163,7 @@ __global__ void __launch_bounds__(WGM * WGN * WK * 64) ckpt_gemm32_kernel(const 
     }
   };
 
-  // prologue: all stages of the ring but one.  The operands' last k, where a load may
-  // reach past the end, are stage 0: its whole offset is the lane's, which is checked.
+  // prologue: all stages of the ring but one.  The operands' last k are stage 0.
   const unsigned last_a = (unsigned)(K - tail) * step_a, last_b = (unsigned)(K - tail) * step_b;
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) {

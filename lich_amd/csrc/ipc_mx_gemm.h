@@ -25,7 +25,8 @@ namespace mx {
 typedef __attribute__((address_space(3))) void lds_void;
 
 // A buffer of `bytes` bytes: per-lane byte offsets of 32 bits plus a uniform one;
-// loads past the end give 0.
+// loads past the end give 0, dword by dword, the uniform offset counted (gfx950: lane
+// offset 0, uniform 64, 72 bytes: two dwords of the 16 bytes, then zeros).
 struct Rsrc {
   __amdgpu_buffer_rsrc_t r;
   __device__ __forceinline__ Rsrc(const void* base, unsigned bytes)

@@ -323,3 +323,11 @@ def test_no_storage_is_refused():
         save(fake, x8)
     with pytest.raises((ValueError, RuntimeError)):
         save(torch.zeros(64, 64).to_sparse().cuda(), x8)
+
+
+@pytest.mark.parametrize("storage,operand,unit", TYPES)
+@pytest.mark.parametrize("M,K,B", [(2, 33, 70), (4, 65, 2), (70, 34, 4), (2, 98, 2), (1, 17, 40), (40, 18, 1), (2, 33, 2), (1, 4001, 1),
+                                   (1000, 2049, 2), (1000, 1026, 1)])
+def test_gradient_of_rows_shorter_than_a_load(M, K, B, storage, operand, unit):
+    """Contractions whose last rows are too few for a load from the row before them."""
+    _gradient(M, K, B, storage, operand, unit, "silu")
