@@ -642,11 +642,12 @@ bool ckpt_products(int storage, int M, int K, int B) {
 }
 bool al4(const void* q) { return reinterpret_cast<uintptr_t>(q) % 4 == 0; }
 
-// Whether ipc_ckpt_gemm32.h can run a call of fp32 operands of these sizes.
+// Whether ipc_ckpt_gemm32.h can run a call of fp32 operands of these sizes (a weight update's
+// K and a 16-bit call's columns are too few by the other limits for mx_rows_fit to fail).
 bool ckpt_products32(int storage, int operand, int M, int K, int B) {
   const long long limit = 1LL << 29;
   return storage == IPC_DT_F32 && operand == IPC_DT_F32 && (long long)M * K < limit && (long long)M * B < limit &&
-         (long long)K * B < limit - (long long)K * 32;
+         (long long)K * B < limit - (long long)K * 32 && mx_rows_fit(B, 4);
 }
 
 // Whether a weight update of few samples streams W past rank-B sums (ipc_outer.hip).

@@ -53,6 +53,11 @@ __host__ __device__ inline long long mx_rows_bytes(long long first, long long en
   return store ? bytes : (bytes + 3) & ~3LL;
 }
 
+// Whether a tile epilogue's offsets from the first of 16 rows of N elements, rows past the
+// tensor's last one and a tile's columns included, fit 32 bits: past them such a row's
+// stores would come round to the tensor's start.
+inline bool mx_rows_fit(long long N, int element) { return (15 * N + 256) * element < (1LL << 32); }
+
 // axis 1: rows of x [R][C] are the packed rows; axis 0: its columns.
 hipError_t launch_mx_quantize(const void* x, void* codes, void* scales, int R, int C, int axis, int format,
                               int storage, int act, hipStream_t s);

@@ -331,3 +331,24 @@ def test_no_storage_is_refused():
 def test_gradient_of_rows_shorter_than_a_load(M, K, B, storage, operand, unit):
     """Contractions whose last rows are too few for a load from the row before them."""
     _gradient(M, K, B, storage, operand, unit, "silu")
+
+
+@pytest.mark.parametrize("M,K,B", [(1, 1, 2 ** 28 + 4), (3, 2, 2 ** 27)])
+def test_gradient_of_rows_past_two_to_the_26(M, K, B):
+    """A row's offsets times 16 pass 32 bits."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x, e = torch.randn(M, B, device="cuda", generator=g), torch.randn(K, B, device="cuda", generator=g)
+    w = torch.randn(K, M, device="cuda", generator=g)
+    save = mx.build_checkpoint_save(M, B)
+    x8, out = save.new_output(), torch.empty(M, B, device="cuda")
+    save(x, x8)
+    mx.build_checkpoint_gradient(M, K, B, "sigmoid")(w, e, x8, out)
+    mx.build_mx_dequantize(M, B, format="int8")(x8, x)
+    s = torch.sigmoid(x)
+    s.mul_(1 - s)
+    for row in range(M):  # f' in [0, 1 / 4] to a few units of 1, two products
+        want, size = torch.zeros(B, device="cuda"), torch.zeros(B, device="cuda")
+        for k in range(K):
+            want += w[k, row] * e[k]
+            size += (w[k, row] * e[k]).abs()
+        assert bool(((out[row] - s[row] * want).abs() <= 2.0 ** -20 * size + 2.0 ** -149).all())

@@ -196,3 +196,36 @@ int main() {
     program = tmp_path / "rows"
     subprocess.run(["g++", "-std=c++17", "-O1", "-o", str(program), str(source)], check=True)
     assert subprocess.run([str(program)]).returncode == 0
+
+
+def test_rows_past_the_last_do_not_come_round(tmp_path):
+    """Offsets of a tile's 16 rows in 32 bits, as compiled from ipc_mx.h: with as many columns as
+    are let through, no row past the tensor's end lands in it; with many more some do."""
+    import re
+    import subprocess
+    from pathlib import Path
+
+    csrc = Path(__file__).resolve().parents[1] / "lich_amd" / "csrc"
+    body = re.search(r"inline bool mx_rows_fit\(.*?}\n", (csrc / "ipc_mx.h").read_text(), re.S).group(0)
+    assert "mx_rows_fit(B, 4)" in (csrc / "ipc_abi.hip").read_text()
+    source = tmp_path / "fit.cpp"
+    source.write_text(body + """
+static bool round(long long N, int rows) {  // a dropped row's offset inside the first `rows` rows
+  for (int r = rows; r < 16; ++r)
+    for (int c = 0; c < 256; ++c)
+      if ((unsigned)((unsigned)r * (unsigned)N + c) * 4u < rows * N * 4) return true;
+  return false;
+}
+int main() {
+  long long most = 1;
+  while (mx_rows_fit(most + 1, 4)) most += 1 + (most < 71000000 ? 1000 : 0);
+  for (int rows = 1; rows < 8; ++rows)
+    if (rows * most < 1LL << 29 && round(most, rows)) return 1;
+  // sizes that the other limits let through: 2^26, one more row's offset; 2^28, the fifth row is the first
+  if (round(1 << 26, 1) || !mx_rows_fit(1 << 26, 4) || !round(1 << 28, 1) || mx_rows_fit(1 << 28, 4)) return 2;
+  return mx_rows_fit((1LL << 29) / 33, 4) && mx_rows_fit((1LL << 30) / 33, 2) && mx_rows_fit(1 << 24, 4) ? 0 : 3;
+}
+""")
+    program = tmp_path / "fit"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-o", str(program), str(source)], check=True)
+    assert subprocess.run([str(program)]).returncode == 0
