@@ -57,7 +57,8 @@ class CompactNet:
 
     def step(self, x: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
         """One training step on ``x [features, batch]`` and targets ``y [classes,
-        batch]``; returns the error ``y - x[0]`` before it."""
+        batch]``; returns the error ``y - x[0]`` before it.  The packed weights are
+        laid out anew by the next ``predict``."""
         state = x.to(self.dtype).contiguous()
         for l in range(len(self.w) - 1, -1, -1):
             self._save[l](state, self.kept[l])
@@ -65,6 +66,7 @@ class CompactNet:
             self._forward[l](state, self.w[l], out)
             state = out
         error = e = (y.to(self.dtype) - state).contiguous()
+        self.w4 = None
         for l in range(len(self.w)):
             below = None
             if l + 1 < len(self.w):  # before W[l] changes
@@ -75,7 +77,8 @@ class CompactNet:
         return error
 
     def pack(self) -> None:
-        """Lays the weights out in 4 bits for ``predict``."""
+        """Lays the weights out in 4 bits for ``predict``, which does so itself after a
+        ``step``; for a program that changes ``w``."""
         self.w4 = []
         for w in self.w:
             k = mx.build_mx_quantize(*w.shape, "identity", self.dtype)

@@ -98,3 +98,17 @@ def test_refusals():
         CompactNet((10, 20), 4, weights=[torch.zeros(10, 21)])
     with pytest.raises(ValueError, match="state"):
         FourBitSteps([torch.zeros(4, 2)], [torch.zeros(4, 4)])
+
+
+def test_answers_after_a_step():
+    """The weights of the last step answer, not those that an answer before it packed."""
+    w, x, y = _inputs(4)
+    xd, yd = x.float().cuda(), y.float().cuda()
+    net = CompactNet(DIMS, B, "tanh", rate=2.0, weights=w)
+    before = net.predict(xd)
+    for _ in range(2):
+        net.step(xd, yd)
+        got = net.predict(xd)
+        fresh = CompactNet(DIMS, B, "tanh", weights=[t.clone() for t in net.w])
+        assert torch.equal(got, fresh.predict(xd)) and not torch.equal(got, before)
+        before = got
