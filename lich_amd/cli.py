@@ -393,7 +393,10 @@ def compact_main(argv=None) -> int:
     p.add_argument("--seed", type=int, default=0)
     a = p.parse_args(argv)
     dtype = {"float16": torch.float16, "bfloat16": torch.bfloat16, "float32": torch.float32}[a.dtype]
-    dev, data = _device(), _dataset(a, a.subset)
+    data = _dataset(a, a.subset)
+    if len(data) < a.batch:
+        p.error(f"a batch of {a.batch} needs more than the {len(data)} samples there are")
+    dev = _device()
     _, net = compact.train(data, hidden=a.hidden, depth=a.depth, batch=a.batch, epochs=a.epochs, rate=a.rate,
                            activation=a.activation, dtype=dtype, seed=a.seed)
     images, labels = next(iter(data.batches(a.batch, shuffle=False)))

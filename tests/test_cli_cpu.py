@@ -88,3 +88,9 @@ def test_reference_command_follows_the_scripts_random_stream(capsys):
         assert int(rows[i][0]) == i
         assert abs(float(rows[i][1]) - m["energy"]) <= 1e-5 * m["energy"]
         assert abs(float(rows[i][2]) - m["max_abs_error"]) <= 1e-5 * m["max_abs_error"]
+
+
+def test_compact_refuses_fewer_samples_than_a_batch(capsys):
+    with pytest.raises(SystemExit) as refused:
+        cli.main(["compact", "--synthetic", "20", "--batch", "32"])
+    assert refused.value.code == 2 and "20 samples" in capsys.readouterr().err
