@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define IPC_ABI_VERSION 7
+#define IPC_ABI_VERSION 8
 
 /* status codes */
 #define IPC_OK 0
@@ -569,7 +569,9 @@ long long ipc_mx_predict_workspace_bytes(int K, int B, int storage);
  * storage, operand: as for ipc_weight_update and ipc_infer_update; the state is
  * widened in the kernels, exactly where the operand type is fp32 or bf16.  Larger
  * weight updates use a workspace lent by the caller (16-byte aligned,
- * ipc_ckpt_workspace_bytes bytes, 0: none), into which f(X) is widened once; state
+ * ipc_ckpt_weight_update_workspace_bytes bytes, 0: none), into which f(X) is widened
+ * once (ipc_ckpt_workspace_bytes, which knows no operand type: as many or, for few
+ * samples and other operands than the storage's, more than the call uses); state
  * gradients of 16-bit tensors with an odd M or B one of
  * ipc_ckpt_gradient_workspace_bytes bytes, into which those rows are laid out.
  * Without them slower kernels run.
@@ -581,6 +583,7 @@ int ipc_ckpt_gradient(const void* w_lower, const void* e_lower, const void* x_co
                       int M, int K, int B, int storage, int operand, int act, void* workspace,
                       long long workspace_bytes, void* stream);
 long long ipc_ckpt_gradient_workspace_bytes(int M, int K, int B, int storage);
+long long ipc_ckpt_weight_update_workspace_bytes(int act, int M, int K, int B, int storage, int operand);
 long long ipc_ckpt_workspace_bytes(int act, int M, int K, int B, int storage);
 
 void ipc_plan_destroy(ipc_plan* plan);

@@ -117,6 +117,7 @@ def _declare(lib):
         "ipc_ckpt_weight_update": ([vp, vp, vp, vp, i, i, i, f, i, i, i, vp, c_longlong, vp], i),
         "ipc_ckpt_gradient": ([vp, vp, vp, vp, vp, i, i, i, i, i, i, vp, c_longlong, vp], i),
         "ipc_ckpt_gradient_workspace_bytes": ([i, i, i, i], c_longlong),
+        "ipc_ckpt_weight_update_workspace_bytes": ([i, i, i, i, i, i], c_longlong),
         "ipc_ckpt_workspace_bytes": ([i, i, i, i, i], c_longlong),
         "ipc_mx_code_bytes": ([i, i, i], c_longlong),
         "ipc_mx_scale_bytes": ([i, i], c_longlong),

@@ -655,9 +655,14 @@ bool ckpt_products32(int storage, int operand, int M, int K, int B) {
 // 10.7, 3001 x 3101, 3 24.5 / 19.4, 1000 x 1531, 5 13.5 / 5.9, 4096 x 4096, 8 17.0 / 18.0, 16
 // 17.0 / 25.6; fp32 8192 x 8192, 1 97 / 78, 256 x 784, 4 4.1 / 3.7, 4096 x 4096, 8 28.4 / 23.4,
 // 16 28.3 / 29.2, and where W's rows are loaded value by value 3001 x 3101, 3 15.9 / 24.5.
-bool ckpt_outer(const void* w, int M, int K, int B, int storage, int operand) {
+// ckpt_few: by its sizes, which is all that a workspace query knows; an fp32 W that starts
+// off 16 bytes then runs from the codes.
+bool ckpt_few(int M, int K, int B, int storage, int operand) {
   if (storage != operand || M > 16 * 65535) return false;  // (16 rows a grid row)
-  return storage == IPC_DT_F32 ? B <= 8 && vec_ok(w, K, 4) : B <= 5;
+  return storage == IPC_DT_F32 ? B <= 8 && K % 4 == 0 : B <= 5;
+}
+bool ckpt_outer(const void* w, int M, int K, int B, int storage, int operand) {
+  return ckpt_few(M, K, B, storage, operand) && (storage != IPC_DT_F32 || al16(w));
 }
 
 // The weight update's workspace: f(X) widened once to the storage type.
@@ -669,7 +674,8 @@ bool ckpt_outer(const void* w, int M, int K, int B, int storage, int operand) {
 // their loaders: MI355X, bf16, us, loaders / products (relu; tanh): 512^2, 512 samples
 // 6.8 / 9.0; 8.3 / 9.8, 700^2, 512 10.4 / 9.7; 12.4 / 10.6, 1024^2, 1024 12.7 / 13.6; 17.4 /
 // 14.4, 1024 x 512, 2048 19.8 / 15.1; 27.1 / 15.7, 1536 x 1024, 320 15.8 / 9.7; 19.3 / 10.6.
-// Or (lengths those products cannot take) by the comparison of fp32.
+// Or (lengths those products cannot take) by the comparison of fp32.  fp32 storage with
+// 16-bit operands widens in the generic kernels' loaders and uses none.
 bool ckpt_weight_products(int act, int M, int K, int B, int storage) {
   const long long outputs = (long long)M * K;
   const bool cheap = act == IPC_ACT_IDENTITY || act == IPC_ACT_RELU;
@@ -685,6 +691,11 @@ long long ckpt_workspace_need(int act, int M, int K, int B, int storage) {
   const long long padded = mx_row_values(MX_INT8, B);
   if (ckpt_weight_products(act, M, K, B, storage)) return (K + (B % 2 ? (long long)M : 0LL)) * padded * 2;
   return s16_preact_rule(S16_WEIGHT, act, M, K, (long long)K * B) ? (long long)K * B * 2 : 0;
+}
+
+// What the call uses of it.
+long long ckpt_workspace_used(int act, int M, int K, int B, int storage, int operand) {
+  return storage != operand || ckpt_few(M, K, B, storage, operand) ? 0 : ckpt_workspace_need(act, M, K, B, storage);
 }
 
 // The state gradient's: rows of an odd length of W_lower [K][M] and E_lower [K][B] padded to
@@ -713,6 +724,11 @@ long long ipc_ckpt_workspace_bytes(int act, int M, int K, int B, int storage) {
   return ckpt_workspace_need(act, M, K, B, storage);
 }
 
+long long ipc_ckpt_weight_update_workspace_bytes(int act, int M, int K, int B, int storage, int operand) {
+  if (M < 1 || K < 1 || B < 1 || check_act(act) != IPC_OK || check_dtypes(storage, operand) != IPC_OK) return 0;
+  return ckpt_workspace_used(act, M, K, B, storage, operand);
+}
+
 int ipc_ckpt_weight_update(void* w, const void* e, const void* x_codes, const void* x_scales, int M, int K, int B,
                            float alpha, int storage, int operand, int act, void* workspace,
                            long long workspace_bytes, void* stream) {
@@ -730,7 +746,7 @@ int ipc_ckpt_weight_update(void* w, const void* e, const void* x_codes, const vo
     q.x_scales = static_cast<const unsigned char*>(x_scales);
     return launch_rc(launch_outer(q, storage, s), "ipc_ckpt_weight_update");
   }
-  const long long need = ckpt_workspace_need(act, M, K, B, storage);
+  const long long need = ckpt_workspace_used(act, M, K, B, storage, operand);
   const bool lent = need > 0 && workspace && workspace_bytes >= need;
   if (ckpt_products32(storage, operand, M, K, B)) {
     CkptProblem q{};

@@ -272,7 +272,8 @@ class MXPredictKernel(_MXProduct):
 class CheckpointWeightUpdateKernel(_Operator, _Kernel):
     """``k(W[M, K], E[M, B], X8, *, workspace=None)``: ``W += alpha E f(X)^T``, X [K, B] kept
     in 8 bits.  ``workspace`` (optional, caller-owned, ``new_workspace()``) lets a
-    large call evaluate f(X) once."""
+    large call evaluate f(X) once.  ``workspace_bytes`` is enough for it, in 16-bit storage also
+    where a call of few samples reads none and ``new_workspace()`` gives None."""
 
     workspace_bytes = 0
 
@@ -282,7 +283,12 @@ class CheckpointWeightUpdateKernel(_Operator, _Kernel):
         self._bind("ipc_ckpt_weight_update", (("W", (self.M, self.K), self.dtype), ("E", (self.M, self.B), self.dtype),
                                               _Packed("X", self.K, self.B, "int8")),
                    self.M, self.K, self.B, self.alpha, self.storage, self.operand, self.act, workspace=True)
-        self.workspace_bytes = int(nat.lib().ipc_ckpt_workspace_bytes(self.act, self.M, self.K, self.B, self.storage))
+        sizes = self.act, self.M, self.K, self.B, self.storage
+        self._used = int(nat.lib().ipc_ckpt_weight_update_workspace_bytes(*sizes, self.operand))
+        self.workspace_bytes = self._used if self.storage == nat.DT_F32 else int(nat.lib().ipc_ckpt_workspace_bytes(*sizes))
+
+    def new_workspace(self, device=None) -> torch.Tensor | None:
+        return super().new_workspace(device) if self._used else None
 
     def __call__(self, w, e, x8, *, workspace=None):
         rc = self._run(w, e, x8, workspace)

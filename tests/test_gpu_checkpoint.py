@@ -352,3 +352,19 @@ def test_gradient_of_rows_past_two_to_the_26(M, K, B):
             want += w[k, row] * e[k]
             size += (w[k, row] * e[k]).abs()
         assert bool(((out[row] - s[row] * want).abs() <= 2.0 ** -20 * size + 2.0 ** -149).all())
+
+
+@pytest.mark.parametrize("storage,operand,unit", TYPES)
+@pytest.mark.parametrize("M,K,B", [(1032, 1100, 1), (2052, 2052, 5), (2052, 2052, 6), (4096, 4096, 8), (4096, 4099, 8), (300, 300, 4),
+                                   (1100, 2050, 192), (4100, 4000, 64)])
+def test_the_workspace_asked_for_is_used(M, K, B, storage, operand, unit):
+    """A lent workspace is written where new_workspace() gives one, and nowhere else."""
+    k = mx.build_checkpoint_weight_update(M, K, B, "silu", DT[storage], operand_dtype=DT[operand])
+    x8, _ = _keep(torch.ones(K, B, dtype=torch.float64), storage)
+    w, e = torch.zeros(M, K, dtype=DT[storage], device="cuda"), torch.ones(M, B, dtype=DT[storage], device="cuda")
+    lent = torch.full((4 * K * 192 + 2 * M * 192,), 77, dtype=torch.uint8, device="cuda")
+    k(w, e, x8, workspace=lent)
+    own = k.new_workspace()
+    assert bool((lent == 77).all()) == (own is None)
+    if own is not None:
+        assert bool((lent[own.numel():] == 77).all())

@@ -229,3 +229,30 @@ int main() {
     program = tmp_path / "fit"
     subprocess.run(["g++", "-std=c++17", "-O1", "-o", str(program), str(source)], check=True)
     assert subprocess.run([str(program)]).returncode == 0
+
+
+@pytest.mark.parametrize("storage,operand,M,K,B,used", [
+    ("float32", "float16", 4096, 4096, 1024, 0), ("float32", "bfloat16", 4096, 4096, 1024, 0),
+    ("float32", "float32", 4096, 4096, 1024, 4 * 4096 * 1024), ("float32", "float32", 300, 300, 64, 0),
+    ("float32", "float32", 4096, 4096, 8, 0), ("float32", "float32", 4096, 4099, 8, 4 * 4099 * 32),
+    ("float32", "float32", 4096, 4096, 9, 4 * 4096 * 32),
+    ("bfloat16", "bfloat16", 8192, 8192, 1, 0), ("float16", "float16", 8192, 8192, 5, 0),
+    ("bfloat16", "bfloat16", 8192, 8192, 6, 2 * 8192 * 32), ("float16", "float16", 8192, 8192, 7, 2 * 2 * 8192 * 32),
+])
+def test_workspace_of_a_weight_update(storage, operand, M, K, B, used):
+    """0 where no call of these sizes and types reads one."""
+    lib, dts = nat.lib(), [nat.dtype_code(t) for t in (storage, operand)]
+    act = nat.act_code("silu")
+    assert lib.ipc_ckpt_weight_update_workspace_bytes(act, M, K, B, *dts) == used
+    assert lib.ipc_ckpt_workspace_bytes(act, M, K, B, dts[0]) >= used
+    k = mx.build_checkpoint_weight_update(M, K, B, "silu", storage, operand_dtype=operand)
+    assert k.workspace_bytes == used or (storage != "float32" and B <= 5)
+    if used == 0:
+        assert k.new_workspace() is None
+
+
+def test_workspace_queries_refuse():
+    need = nat.lib().ipc_ckpt_weight_update_workspace_bytes
+    assert need(4, 4096, 4096, 1024, 1, 1) > 0
+    for bad in ((4, 0, 4096, 1024, 1, 1), (9, 4096, 4096, 1024, 1, 1), (4, 4096, 4096, 1024, 3, 3), (4, 4096, 4096, 1024, 1, 2)):
+        assert need(*bad) == 0
