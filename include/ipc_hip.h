@@ -552,7 +552,8 @@ int ipc_mx_weight_update(void* w, const void* e_codes, const void* e_scales, con
 
 /* OUT [M][B] = W f(X) with W packed in IPC_MX_FP4 by rows and the states X [K][B]
  * in their storage type, which are not quantised: the forward pass of one
- * sample or a few (at most 1048560).  f(X) is carried to fp32 accuracy.  With a
+ * sample or a few (at most 1048560).  f(X) is carried to 2^-25 of its value for fp32
+ * states and to 2^-17 for 16-bit ones, the sum in fp32.  With a
  * workspace lent (16-byte aligned, ipc_mx_predict_workspace_bytes bytes, 0: none
  * used) f(X) is evaluated once, else in every workgroup. */
 int ipc_mx_predict(const void* x, const void* w_codes, const void* w_scales, void* out, int M, int K, int B,

@@ -7,10 +7,11 @@
 // and one scale byte, which the scaled conversions widen exactly to bf16.
 //
 // f(X) is evaluated once per workgroup and element and carried as a sum of bf16
-// terms, 3 for fp32 states and 2 for 16-bit ones (errors of 2^-25 and 2^-17), each
-// a matrix product of its own (v_mfma_f32_16x16x32_bf16): with W exact, the
-// result is that of an fp32 product.  The matrix units stay idle most of the
-// time, so the extra terms cost nothing that is waited for.
+// terms, each a matrix product of its own (v_mfma_f32_16x16x32_bf16), with W exact:
+// 3 terms for fp32 states (errors of 2^-25 of f(X): the result is that of an fp32
+// product), 2 for 16-bit ones (2^-17, a 64th of fp16's own rounding and a 512th of
+// bf16's).  The matrix units stay idle most of the time, so the extra terms cost
+// nothing that is waited for.
 //
 // The k order within a group is free as long as both operands agree: product j
 // of a group takes values 8 j .. 8 j + 7 of every lane's own block.
@@ -39,6 +40,15 @@ __device__ __forceinline__ bf16x8 widen8(unsigned w, float scale) {
   const bf16x2 a0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0), a1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1);
   const bf16x2 a2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2), a3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3);
   return bf16x8{a0[0], a0[1], a1[0], a1[1], a2[0], a2[1], a3[0], a3[1]};
+}
+
+// Term t of v, which keeps the rest.  The first one is finite, since a finite fp32 value
+// may round past the largest bf16; an infinity or NaN is the second, and has no rest.
+__device__ __forceinline__ bf16 take_term(int t, float& v) {
+  constexpr float MOST = 0x1.fep127f;
+  const bf16 h = cvt<bf16>(t == 0 ? __builtin_amdgcn_fmed3f(v, -MOST, MOST) : v);
+  v = t == 0 || __builtin_isfinite(to_f32(h)) ? v - to_f32(h) : 0.0f;
+  return h;
 }
 
 // The form without a workspace: RM tiles of 16 rows and 16 samples per workgroup.
@@ -102,11 +112,7 @@ __global__ void __launch_bounds__(MAX_WAVES * 64) mx_predict_kernel(const MxPred
     for (int i = 0; i < XI; ++i) {
       float v = kg * MX_GROUP + i * KPI + sk < K ? f[i] : 0.0f;  // past the contraction: zero, whatever f(0) is
 #pragma unroll
-      for (int t = 0; t < TERMS; ++t) {
-        const bf16 h = cvt<bf16>(v);
-        xs[(t * NP + sn) * XLD + i * KPI + sk] = h;
-        v = __builtin_isfinite(to_f32(h)) ? v - to_f32(h) : 0.0f;  // (an infinity has no rest)
-      }
+      for (int t = 0; t < TERMS; ++t) xs[(t * NP + sn) * XLD + i * KPI + sk] = take_term(t, v);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
@@ -160,9 +166,8 @@ __global__ void __launch_bounds__(256) mx_terms_kernel(const ST* __restrict__ x,
     bf16x8 h;
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
-      const bf16 b = cvt<bf16>(k + q < K ? v[q] : 0.0f);
-      h[q] = b;
-      v[q] = __builtin_isfinite(to_f32(b)) ? v[q] - to_f32(b) : 0.0f;  // (an infinity has no rest)
+      if (k + q >= K) v[q] = 0.0f;  // past the contraction: zero, whatever f(0) is
+      h[q] = take_term(t, v[q]);
     }
     *reinterpret_cast<bf16x8*>(to + (long long)t * 4 * rb * 32) = h;
   }

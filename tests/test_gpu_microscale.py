@@ -378,3 +378,49 @@ def test_fast_and_checked_calls_agree():
     for bad in ((x4.codes, x4.scales[:1]), (x4.codes.cpu(), x4.scales), [*x4], (x4.codes,)):
         with pytest.raises((ValueError, TypeError)):
             qx(x, bad)
+
+
+@pytest.mark.parametrize("M,K,B", [(40, 200, 1), (40, 200, 3), (8200, 200, 2), (40, 200, 12), (100, 1531, 17)])
+@pytest.mark.parametrize("size", [2.0 ** 127, 2.0 ** -100])
+def test_predict_of_states_near_the_ends_of_fp32(M, K, B, size):
+    """Finite states past the largest bf16 among them, zero weights in their way: the sum's
+    bound and that of the terms as for any other states."""
+    g = torch.Generator().manual_seed(K + B)
+    w = _rand(g, M, K, size=2.0 ** -16)
+    w[::3] = 0
+    x = (torch.rand(K, B, generator=g, dtype=torch.float64) * 2 - 1) * 2 * size
+    x[:4] = torch.tensor([1.0, -1.0, 1 - 2.0 ** -10, 1 - 2.0 ** -23], dtype=torch.float64)[:, None] * (2 - 2.0 ** -23) * size
+    x = x.float().double()
+    assert bool(x.isfinite().all())
+    wq = O.quantised(w, "fp4")
+    want = wq @ x
+    k = mx.build_mx_predict(M, K, B, "identity")
+    for workspace in (None, k.new_workspace()):
+        out = torch.full((M, B), 7.0, device="cuda")
+        k(_dev(x, "fp32"), _pack4(w), out, workspace=workspace)
+        _close(out, want, O.product_bound(wq, x, 3 * K) + 2.0 ** -21 * (wq.abs() @ x.abs()), "fp32")
+
+
+@pytest.mark.parametrize("storage", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("B", [1, 3, 12, 17])
+def test_predict_carries_infinities_and_nan(B, storage):
+    """They reach the outputs that a sum of products would give: infinite by a weight's sign,
+    NaN by a zero weight, by two of different signs, by NaN, and the others stay finite."""
+    M, K = 40, 200
+    g = torch.Generator().manual_seed(B)
+    w, x = _rand(g, M, K), _rand(g, K, B)
+    w[7, 96:128] = 0
+    x[100, 0] = float("inf")
+    if B > 1:
+        x[5, 1] = float("nan")
+        x[130, 2], x[150, 2] = float("inf"), float("-inf")
+    x = _up(x.to(DT[storage]))
+    wq = O.quantised(w, "fp4")
+    want = sum(wq[:, k:k + 1] * x[k:k + 1] for k in range(K))
+    k = mx.build_mx_predict(M, K, B, "identity", DT[storage])
+    for workspace in (None, k.new_workspace()):
+        out = torch.full((M, B), 7.0, dtype=DT[storage], device="cuda")
+        k(_dev(x, storage), _pack4(w), out, workspace=workspace)
+        got = _up(out)
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isfinite(), want.isfinite())
+        assert torch.equal(got[want.isinf()], want[want.isinf()])
