@@ -42,15 +42,19 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 // before each transposing read, whose address it cannot tell from theirs (the state
 // gradient's main loop then ran four times as long).  There is no register to wait
 // for; every wait is one of the kernel's own.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void to_lds16_unseen(i32x4 rsrc, unsigned char* lds, unsigned v, unsigned s) {
   const unsigned at = (unsigned)(unsigned long long)(lds_void*)lds;
-  // (m0 holds the place; a wait state lies between its write and its use.  The compiler
-  // sets it anew for each instruction of its own that reads it.)
+  // (m0 holds the place; a wait state lies between its write and its use.  Named as
+  // clobbered, so that the compiler sets it anew for an instruction of its own that reads
+  // it; it warns of any reserved register there.)
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
                : "s"(at), "v"(v), "s"(rsrc), "s"(s)
-               : "memory");
+               : "memory", "m0");
 }
+#pragma clang diagnostic pop
 // The buffer resource of `bytes` bytes at `base`, as words.
 __device__ __forceinline__ i32x4 rsrc_words(const void* base, unsigned bytes) {
   const unsigned long long a = reinterpret_cast<unsigned long long>(base);

@@ -38,13 +38,16 @@ namespace ipc {
 namespace mx {
 
 // 4 bytes a lane, as to_lds16_unseen.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void to_lds4_unseen(i32x4 rsrc, unsigned char* lds, unsigned v, unsigned s) {
   const unsigned at = (unsigned)(unsigned long long)(lds_void*)lds;
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
                :
                : "s"(at), "v"(v), "s"(rsrc), "s"(s)
-               : "memory");
+               : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 constexpr int K32 = 16;  // k of a stage
 

@@ -256,3 +256,17 @@ def test_workspace_queries_refuse():
     assert need(4, 4096, 4096, 1024, 1, 1) > 0
     for bad in ((4, 0, 4096, 1024, 1, 1), (9, 4096, 4096, 1024, 1, 1), (4, 4096, 4096, 1024, 3, 3), (4, 4096, 4096, 1024, 1, 2)):
         assert need(*bad) == 0
+
+
+def test_inline_assembly_names_m0():
+    """Whatever writes m0 says so."""
+    import re
+    from pathlib import Path
+
+    found = 0
+    for path in (Path(__file__).resolve().parents[1] / "lich_amd" / "csrc").iterdir():
+        for asm in re.findall(r"\basm\b[^;]*?\((.*?)\);", path.read_text(), re.S):
+            if re.search(r"mov_b32 m0,", asm):
+                found += 1
+                assert '"m0"' in asm.rsplit(":", 1)[1], path.name
+    assert found == 2
