@@ -424,3 +424,46 @@ def test_predict_carries_infinities_and_nan(B, storage):
         got = _up(out)
         assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isfinite(), want.isfinite())
         assert torch.equal(got[want.isinf()], want[want.isinf()])
+
+
+@pytest.mark.parametrize("fmt", ["fp4", "int8"])
+@pytest.mark.parametrize("storage", ["fp32", "bf16"])
+@pytest.mark.parametrize("axis", [0, 1])
+def test_quantize_at_the_bottom_of_the_range(axis, storage, fmt):
+    """Blocks under the smallest scale, 2^-126, whose values are subnormal floats: the codes of
+    the definition, and back the subnormals they stand for."""
+    g = torch.Generator().manual_seed(8)
+    x = _rand(g, 64, 160) * 2.0 ** torch.randint(-132, -122, (64, 5), generator=g).double().repeat_interleave(32, 1)
+    x[:8, :32] = torch.linspace(2.0 ** -128, 2.0 ** -126, 32, dtype=torch.float64)
+    x[8, :32] = 2.0 ** -128  # halfway to the first code
+    x[9, :32] = 2.0 ** -128 * (1 + 2.0 ** -7)
+    xd = _dev(x if axis == 1 else x.T.contiguous(), storage)
+    x = _up(xd if axis == 1 else xd.T.contiguous())
+    k = mx.build_mx_quantize(*xd.shape, "identity", DT[storage], format=fmt, axis=axis)
+    out = k.new_output()
+    k(xd, out)
+    codes, scales = O.pack(x, fmt)
+    assert bool((scales == 1).any()) and torch.equal(out.scales.cpu(), scales)
+    back = torch.empty(x.shape, dtype=DT[storage], device="cuda")
+    mx.build_mx_dequantize(*x.shape, DT[storage], format=fmt)(out, back)
+    want = O.quantised(x, fmt)
+    assert bool((want.abs() == 2.0 ** -127).any()) and torch.equal(_up(back), want.to(DT[storage]).double())
+
+
+@pytest.mark.parametrize("M,K,B", [(64, 160, 40), (1100, 160, 1025)])
+def test_products_read_the_bottom_of_the_range(M, K, B):
+    """Weights of 2^-127 to 2^-122 against states of 2^100: exact codes and scales in the product
+    and in the prediction."""
+    g = torch.Generator().manual_seed(M)
+    w = _rand(g, M, K) * 2.0 ** torch.randint(-127, -122, (M, K // 32), generator=g).double().repeat_interleave(32, 1)
+    x = _rand(g, B, K, size=2.0 ** 100)
+    wq, xq = O.quantised(w, "fp4"), O.quantised(x, "fp4").T.contiguous()
+    out = torch.full((M, B), 7.0, device="cuda")
+    mx.build_mx_forward(M, K, B)(_pack4(x), _pack4(w), out)
+    _close(out, wq @ xq, O.product_bound(wq, xq, K), "fp32")
+    predict = mx.build_mx_predict(M, K, B, "identity")
+    for workspace in (None, predict.new_workspace()):
+        out.fill_(7.0)
+        xs = x.T.contiguous().float()
+        predict(xs.cuda(), _pack4(w), out, workspace=workspace)
+        _close(out, wq @ xs.double(), O.product_bound(wq, xs.double(), 3 * K) + 2.0 ** -21 * (wq.abs() @ xs.double().abs()), "fp32")
