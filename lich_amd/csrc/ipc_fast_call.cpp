@@ -153,7 +153,7 @@ PyObject* call_run(PyObject* self, PyObject* const* argv, size_t nargsf, PyObjec
       if (!THPVariable_Check(o)) return refuse;
       try {
         const at::Tensor& t = THPVariable_Unpack(o);
-        if (!t.is_cuda() || !t.is_contiguous()) return refuse;
+        if (!t.is_cuda() || t.get_device() != device || !t.is_contiguous()) return refuse;
         a.workspace = t.data_ptr();
         a.bytes = (long long)t.nbytes();
       } catch (const std::exception&) {

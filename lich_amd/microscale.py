@@ -115,6 +115,10 @@ class _Operator:
     def _checked(self, rc: int, *given, workspace=None) -> None:
         if rc < 0:
             nat.check(rc)
+        flat = [t for g in (*given, workspace) for t in (g if isinstance(g, tuple) else (g,))]
+        devices = {t.device for t in flat if isinstance(t, torch.Tensor) and t.device.type == "cuda"}
+        if len(devices) > 1:
+            raise ValueError(f"tensors on different devices ({', '.join(sorted(map(str, devices)))})")
         pointers = []
         for o, t in zip(self._operands, given):
             pointers += o(t) if isinstance(o, _Packed) else (_pointer(t, *o),)

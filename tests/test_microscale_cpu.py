@@ -270,3 +270,27 @@ def test_inline_assembly_names_m0():
                 found += 1
                 assert '"m0"' in asm.rsplit(":", 1)[1], path.name
     assert found == 2
+
+
+def test_tensors_on_different_devices_are_refused():
+    """Also a workspace; tensors without storage, so that no such device is needed."""
+    from torch._subclasses import FakeTensorMode
+
+    def on(device, *shape, dtype=torch.float32):
+        with FakeTensorMode():
+            return torch.empty(shape, dtype=dtype, device=device)
+
+    def packed(k, device):
+        p = k._operands[1]
+        return mx.MXMatrix(on(device, *p.codes, dtype=p.dtype), on(device, *p.scales, dtype=torch.uint8))
+
+    k = mx.build_mx_predict(16, 256, 8, "relu")
+    good = on("cuda:0", 256, 8), packed(k, "cuda:0"), on("cuda:0", 16, 8)
+    for at, other in enumerate((on("cuda:1", 256, 8), packed(k, "cuda:1"), on("cuda:1", 16, 8))):
+        with pytest.raises(ValueError, match="different devices .*cuda:0, cuda:1"):
+            k(*good[:at], other, *good[at + 1:])
+    codes, scales = good[1]
+    with pytest.raises(ValueError, match="different devices"):
+        k(good[0], mx.MXMatrix(codes, packed(k, "cuda:1").scales), good[2])
+    with pytest.raises(ValueError, match="different devices"):
+        k(*good, workspace=on("cuda:1", k.workspace_bytes, dtype=torch.uint8))
