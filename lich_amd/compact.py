@@ -31,7 +31,9 @@ def _weights(dims, seed, device, dtype):
 
 class CompactNet:
     """``dims`` = (classes, hidden ..., features), ``dtype`` the type of states and
-    weights, ``rate`` the step of the mean gradient over a batch."""
+    weights, ``rate`` the step of the mean gradient over a batch.  ``weights`` are the
+    net's own from then on: where they have its type and device they are not copied,
+    and ``step`` updates them in place."""
 
     def __init__(self, dims, batch: int, activation: str = "relu", dtype=torch.float32, rate: float = 0.01, *,
                  device=None, seed: int = 0, weights=None):
@@ -59,6 +61,8 @@ class CompactNet:
         """One training step on ``x [features, batch]`` and targets ``y [classes,
         batch]``; returns the error ``y - x[0]`` before it.  The packed weights are
         laid out anew by the next ``predict``."""
+        if tuple(y.shape) != (self.dims[0], self.batch):
+            raise ValueError(f"targets have shape {tuple(y.shape)}, the net expects {(self.dims[0], self.batch)}")
         state = x.to(self.dtype).contiguous()
         for l in range(len(self.w) - 1, -1, -1):
             self._save[l](state, self.kept[l])
