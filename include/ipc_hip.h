@@ -568,7 +568,8 @@ long long ipc_mx_predict_workspace_bytes(int K, int B, int storage);
  *   ipc_ckpt_gradient       G = f'(X) W_lower^T E_lower
  *                           W_lower [K][M], E_lower [K][B], X and G [M][B]
  * storage, operand: as for ipc_weight_update and ipc_infer_update; the state is
- * widened in the kernels, exactly where the operand type is fp32 or bf16.  Larger
+ * widened in the kernels, exactly where the operand type is fp32 or bf16 (fp16: a
+ * state from 65280 on may be kept as 65536, which that type reads as infinity).  Larger
  * weight updates use a workspace lent by the caller (16-byte aligned,
  * ipc_ckpt_weight_update_workspace_bytes bytes, 0: none), into which f(X) is widened
  * once (ipc_ckpt_workspace_bytes, which knows no operand type: as many or, for few
