@@ -588,6 +588,53 @@ long long ipc_ckpt_gradient_workspace_bytes(int M, int K, int B, int storage);
 long long ipc_ckpt_weight_update_workspace_bytes(int act, int M, int K, int B, int storage, int operand);
 long long ipc_ckpt_workspace_bytes(int act, int M, int K, int B, int storage);
 
+/*
+ * Nets over tokens: an input of rows of a learnt table, an output of V words under a
+ * softmax.  No counterpart in the reference.  Ids and targets are 64-bit; one
+ * outside 0 .. V - 1 marks a padded place.
+ *
+ *   ipc_embedding         x[c D + d][b] = scale table[ids[c][b]][d], zeros for a padded
+ *                         place; ids [C][B], table [V][D], x [C D][B]
+ *   ipc_embedding_update  table[v][d] += alpha sum of g[c D + d][b] over the places of
+ *                         v; the sum in fp32 in a fixed order, one rounding of the table's
+ *                         value.  From 513 places on it sorts them in a workspace of
+ *                         ipc_embedding_update_workspace_bytes bytes (0: none).
+ */
+int ipc_embedding(const long long* ids, const void* table, void* x, int V, int D, int C, int B, float scale, int storage,
+                  void* stream);
+int ipc_embedding_update(void* table, const long long* ids, const void* g, int V, int D, int C, int B, float alpha,
+                         int storage, void* workspace, long long workspace_bytes, void* stream);
+long long ipc_embedding_update_workspace_bytes(int V, int D, int C, int B, int storage);
+
+/* out = m x / (1 - dropped / 65536), x and out [M][B] (out may be x).  rng: two 64-bit
+ * numbers in device memory, seed and step, read when the call runs, so that a captured
+ * call draws anew once they change.  Value i (row-major) is kept where the i % 8-th
+ * 16-bit half (lower half first) of the four words of Philox 4x32-10 under key `seed`
+ * and counter (i / 8, site, step) is at least `dropped`; others are 0 whatever they
+ * were.  The same call on an error is the backward pass. */
+int ipc_dropout(const void* x, const long long* rng, void* out, int M, int B, int dropped, int site, int storage,
+                void* stream);
+
+/*
+ * Softmax cross entropy, z = W f(X), x [D][B], w [V][D], targets [B]:
+ *   ipc_token_loss    loss[b] = log sum_v exp z[v][b] - z[targets[b]][b]
+ *   ipc_token_update  that, and with e = onehot - softmax(z), a descent direction:
+ *                     g = f'(X) W^T e (w as it was), then w += alpha e f(X)^T
+ * A padded column has loss 0, no share of w and zeros in g, whatever x holds there.  The
+ * logits are never kept: they are formed per piece of the vocabulary, and for the
+ * update formed again.  Sums are in fp32 in a fixed order; fp32 products are sums of
+ * bf16 ones exact to 2^-24; in 16-bit storage f(X) and e are rounded once to the type.
+ * Both need a workspace (16-byte aligned) of ipc_token_loss_workspace_bytes /
+ * ipc_token_update_workspace_bytes bytes (0: refused).  w of 16 bits with an even D
+ * lies on 4 bytes.
+ */
+int ipc_token_loss(const void* x, const void* w, const long long* targets, float* loss, int V, int D, int B, int storage,
+                   int act, void* workspace, long long workspace_bytes, void* stream);
+int ipc_token_update(const void* x, void* w, const long long* targets, float* loss, void* g, int V, int D, int B,
+                     float alpha, int storage, int act, void* workspace, long long workspace_bytes, void* stream);
+long long ipc_token_loss_workspace_bytes(int V, int D, int B, int storage, int act);
+long long ipc_token_update_workspace_bytes(int V, int D, int B, int storage, int act);
+
 void ipc_plan_destroy(ipc_plan* plan);
 
 #ifdef __cplusplus

@@ -129,6 +129,14 @@ def _declare(lib):
         "ipc_mx_weight_update": ([vp, vp, vp, vp, vp, i, i, i, f, i, vp], i),
         "ipc_mx_predict": ([vp, vp, vp, vp, i, i, i, i, i, vp, c_longlong, vp], i),
         "ipc_mx_predict_workspace_bytes": ([i, i, i], c_longlong),
+        "ipc_embedding": ([vp, vp, vp, i, i, i, i, f, i, vp], i),
+        "ipc_embedding_update": ([vp, vp, vp, i, i, i, i, f, i, vp, c_longlong, vp], i),
+        "ipc_embedding_update_workspace_bytes": ([i, i, i, i, i], c_longlong),
+        "ipc_dropout": ([vp, vp, vp, i, i, i, i, i, vp], i),
+        "ipc_token_loss": ([vp, vp, vp, vp, i, i, i, i, i, vp, c_longlong, vp], i),
+        "ipc_token_update": ([vp, vp, vp, vp, vp, i, i, i, f, i, i, vp, c_longlong, vp], i),
+        "ipc_token_loss_workspace_bytes": ([i, i, i, i, i], c_longlong),
+        "ipc_token_update_workspace_bytes": ([i, i, i, i, i], c_longlong),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)

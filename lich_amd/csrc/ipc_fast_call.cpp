@@ -99,7 +99,9 @@ const Kind kKinds[] = {
     KIND("ipc_mx_pred_err", 6, 4, false, 0, false),        KIND("ipc_mx_forward", 5, 4, false, 0, false),
     KIND("ipc_mx_infer_update", 6, 3, true, 2, false),     KIND("ipc_mx_weight_update", 5, 3, true, 1, false),
     KIND("ipc_mx_predict", 4, 5, false, 0, true),          KIND("ipc_ckpt_weight_update", 4, 3, true, 3, true),
-    KIND("ipc_ckpt_gradient", 5, 6, false, 0, true),
+    KIND("ipc_ckpt_gradient", 5, 6, false, 0, true),       KIND("ipc_embedding", 3, 4, true, 1, false),
+    KIND("ipc_embedding_update", 3, 4, true, 1, true),     KIND("ipc_dropout", 3, 5, false, 0, false),
+    KIND("ipc_token_loss", 4, 5, false, 0, true),          KIND("ipc_token_update", 5, 3, true, 2, true),
 };
 
 // ------------------------------------------------------------------ Call

@@ -1,0 +1,90 @@
+// ipc_token.h - nets over tokens: layouts, host structs and launchers.
+//
+//   embedding         X[c D + d][b] = scale TABLE[ids[c][b]][d]
+//   embedding update  TABLE[v][d] += alpha sum of G[c D + d][b] over the places (c, b) of v
+//   dropout           OUT = m X / (1 - p), m from a counter-based generator
+//   token loss        loss[b] = log sum_v exp z[v] - z[t_b], z = W f(X) column b
+//   token update      that, e = onehot - softmax(z), G = f'(X) W^T e, W += alpha e f(X)^T
+//
+// States are [features][batch], weights [out][in], ids and targets 64-bit.  An id or
+// target outside 0 .. V - 1 is a padded place.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace ipc {
+
+// ------------------------------------------------------------------ embedding
+struct EmbedProblem {
+  int V, D, C, B;
+  const long long* ids;  // [C][B]
+  const void* table;     // [V][D]
+  void* x;               // [C D][B]
+  float scale;
+  int vec_d, vec_b;      // rows of the table / of x allow 4-element accesses
+};
+hipError_t launch_embedding(const EmbedProblem& p, int storage, hipStream_t s);
+
+// Places are sorted by id, ties in their order; their rows of G, transposed once, are then
+// summed in runs of EMBED_RUN places, and sums that cross a run's end joined in order.
+constexpr int EMBED_RUN = 32;
+// From so many places on (below, one launch finds the places of an id itself).
+constexpr int EMBED_SORTED = 513;
+struct EmbedUpdate {
+  int V, D, C, B;
+  void* table;
+  const long long* ids;
+  const void* g;         // [C D][B]
+  float alpha;
+  int vec_d, vec_b;
+  // workspace (from EMBED_SORTED places on)
+  int* order;            // [N] place of each sorted position
+  int* key;              // [N + 1] its id; -1 from the first position without one on
+  void* rows;            // [N][D] G transposed
+  float* part;           // [runs][2][D] sums of ids that cross a run's start / end
+};
+struct EmbedLayout {
+  long long order, key, rows, part, bytes;
+};
+inline EmbedLayout embed_layout(int D, int C, int B, int element) {
+  auto up = [](long long v) { return (v + 255) & ~255LL; };
+  const long long n = (long long)C * B, runs = (n + EMBED_RUN - 1) / EMBED_RUN;
+  EmbedLayout l{};
+  l.key = up(n * 4);
+  l.rows = l.key + up((n + 1) * 4);
+  l.part = l.rows + up(n * D * element);
+  l.bytes = n < EMBED_SORTED ? 0 : l.part + up(runs * 2 * D * 4);
+  return l;
+}
+hipError_t launch_embedding_update(const EmbedUpdate& p, int storage, hipStream_t s);
+
+// -------------------------------------------------------------------- dropout
+struct DropoutProblem {
+  long long n;
+  const void* x;
+  const long long* rng;  // seed, step
+  void* out;
+  unsigned dropped;      // of 65536
+  unsigned site;
+  int vec;               // x and out on 16 bytes
+};
+hipError_t launch_dropout(const DropoutProblem& p, int storage, hipStream_t s);
+
+// -------------------------------------------------------------------- softmax
+struct TokenProblem {
+  int V, D, B;
+  const void* x;             // [D][B]
+  void* w;                   // [V][D]
+  const long long* targets;  // [B]
+  float* loss;               // [B]
+  void* g;                   // [D][B], or nullptr: the loss alone
+  float alpha;
+  int act;
+  unsigned char* workspace;
+};
+// 0: sizes that the kernels do not take
+long long token_workspace_bytes(int V, int D, int B, int storage, int act, bool update);
+hipError_t launch_token(const TokenProblem& p, int storage, hipStream_t s);
+
+}  // namespace ipc

@@ -1,0 +1,398 @@
+// ipc_token_embed.hip - rows of a learnt table as a net's input state, and their update.
+//
+//   X[c D + d][b] = scale TABLE[ids[c][b]][d]
+//   TABLE[v][d] += alpha sum over the places (c, b) of v of G[c D + d][b]
+//
+// Both move bytes and little else.  The table has a token's features next to each
+// other, a state has the samples there, so a block of 64 samples by 64 features turns
+// in LDS and both sides see runs of 128 bytes (16-bit).
+#include "ipc_device.h"
+#include "ipc_token.h"
+
+namespace ipc {
+namespace {
+
+template <typename ST> struct Four { ST v[4]; };
+
+template <typename ST>
+__device__ __forceinline__ void store4(ST* p, const ST (&v)[4]) {
+  typedef ST V __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<V*>(p) = V{v[0], v[1], v[2], v[3]};
+}
+
+// BT samples x DT features of one context place.
+template <typename ST, int BT>
+__global__ void __launch_bounds__(256) embed_kernel(const EmbedProblem p) {
+  constexpr int DT = BT == 1 ? 1024 : 4096 / BT, LD = DT + (BT == 1 ? 0 : 2);
+  __shared__ ST tile[BT * LD];
+  const int tiles_d = (p.D + DT - 1) / DT, tiles_b = (p.B + BT - 1) / BT;
+  const int td = blockIdx.x % tiles_d, tb = blockIdx.x / tiles_d % tiles_b, c = blockIdx.x / tiles_d / tiles_b;
+  const int d0 = td * DT, b0 = tb * BT, tid = threadIdx.x;
+  const ST* table = static_cast<const ST*>(p.table);
+  ST* x = static_cast<ST*>(p.x);
+#pragma unroll 4
+  for (int u = tid; u < BT * DT / 4; u += 256) {
+    const int r = u / (DT / 4), d = d0 + u % (DT / 4) * 4, b = b0 + r;
+    if (b >= p.B || d >= p.D) continue;
+    const long long id = p.ids[(long long)c * p.B + b];
+    const bool real = id >= 0 && id < p.V;
+    const ST* from = table + (real ? id : 0) * p.D + d;
+    float v[4] = {};
+    if (real) {
+      if (p.vec_d) {
+        load4(from, v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (d + i < p.D) v[i] = to_f32(from[i]);
+      }
+    }
+    ST o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = real ? cvt<ST>(v[i] * p.scale) : cvt<ST>(0.0f);
+    if constexpr (BT == 1) {  // (one sample: X is as long as the row)
+      ST* to = x + (long long)c * p.D + d;
+      if (p.vec_d && p.vec_b) {
+        store4(to, o);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (d + i < p.D) to[i] = o[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tile[r * LD + (d - d0) + i] = o[i];
+    }
+  }
+  if constexpr (BT > 1) {
+    __syncthreads();
+#pragma unroll 4
+    for (int u = tid; u < BT * DT / 4; u += 256) {
+      const int r = u % (BT / 4) * 4, d = u / (BT / 4), b = b0 + r;
+      if (b >= p.B || d0 + d >= p.D) continue;
+      ST o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = tile[(r + i) * LD + d];
+      ST* to = x + ((long long)c * p.D + d0 + d) * p.B + b;
+      if (p.vec_b) {
+        store4(to, o);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (b + i < p.B) to[i] = o[i];
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ update
+// Few places: a workgroup for each place and slab of features.  The first place of an id
+// sums all of its places in order, the others have nothing to do.
+template <typename ST>
+__global__ void __launch_bounds__(256) embed_few_kernel(const EmbedUpdate p) {
+  __shared__ int same[EMBED_SORTED];
+  __shared__ int count, earlier;
+  const int N = p.C * p.B, slabs = (p.D + 255) / 256, n = blockIdx.x / slabs, tid = threadIdx.x;
+  const int d = blockIdx.x % slabs * 256 + tid;
+  const long long id = p.ids[n];
+  if (id < 0 || id >= p.V) return;
+  if (tid == 0) earlier = 0;
+  __syncthreads();
+  for (int i = tid; i < n; i += 256)
+    if (p.ids[i] == id) earlier = 1;
+  __syncthreads();
+  if (earlier) return;
+  if (tid < 64) {  // one wave lists the places in order
+    int at = 0;
+    for (int i = n; i < N; i += 64) {
+      const bool hit = i + tid < N && p.ids[i + tid < N ? i + tid : N - 1] == id;
+      const unsigned long long m = __ballot(hit);
+      if (hit) same[at + __popcll(m & ((1ull << tid) - 1))] = i + tid;
+      at += __popcll(m);
+    }
+    if (tid == 0) count = at;
+  }
+  __syncthreads();
+  if (d >= p.D) return;
+  const ST* g = static_cast<const ST*>(p.g);
+  ST* t = static_cast<ST*>(p.table) + id * p.D + d;
+  const float old = to_f32(*t);
+  float sum = 0.0f;
+  const int many = count;
+#pragma unroll 4
+  for (int i = 0; i < many; ++i) {
+    const int at = same[i], c = at / p.B, b = at - c * p.B;
+    sum += to_f32(g[((long long)c * p.D + d) * p.B + b]);
+  }
+  *t = cvt<ST>(old + p.alpha * sum);
+}
+
+// Workgroups 0 .. ranges - 1: each owns a range of ids, reads all places in order twice and
+// writes its own, sorted, behind those of smaller ids (which it counts on the way, so
+// that no workgroup waits for another).  Each of the eight waves has an eighth of the
+// places, so that an id's places keep their order.  The other workgroups transpose G.
+constexpr int SORT_WAVES = 8;
+
+inline int sort_range(int V) {
+  const int r = (V / 256 + 64) / 64 * 64;
+  return r > 1024 ? 1024 : r;
+}
+
+template <typename ST>
+__device__ void transpose_rows(const EmbedUpdate& p, int block, ST* tile) {
+  constexpr int LD = 66;
+  const int tiles_d = (p.D + 63) / 64, tiles_b = (p.B + 63) / 64;
+  const int td = block % tiles_d, tb = block / tiles_d % tiles_b, c = block / tiles_d / tiles_b;
+  const int d0 = td * 64, b0 = tb * 64;
+  const ST* g = static_cast<const ST*>(p.g);
+  ST* rows = static_cast<ST*>(p.rows);
+  for (int u = threadIdx.x; u < 1024; u += SORT_WAVES * 64) {
+    const int d = u >> 4, b = (u & 15) * 4;
+    if (d0 + d >= p.D || b0 + b >= p.B) continue;
+    const ST* from = g + ((long long)c * p.D + d0 + d) * p.B + b0 + b;
+    ST v[4];
+    if (p.vec_b) {
+      const Four<ST> f = *reinterpret_cast<const Four<ST>*>(__builtin_assume_aligned(from, 4 * sizeof(ST)));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = f.v[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = b0 + b + i < p.B ? from[i] : cvt<ST>(0.0f);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) tile[d * LD + b + i] = v[i];
+  }
+  __syncthreads();
+  for (int u = threadIdx.x; u < 1024; u += SORT_WAVES * 64) {
+    const int b = u >> 4, d = (u & 15) * 4;
+    if (b0 + b >= p.B || d0 + d >= p.D) continue;
+    ST v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = tile[(d + i) * LD + b];
+    ST* to = rows + ((long long)c * p.B + b0 + b) * p.D + d0 + d;
+    if (p.D % 4 == 0) {  // (rows starts on 256 bytes)
+      store4(to, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (d0 + d + i < p.D) to[i] = v[i];
+    }
+  }
+}
+
+template <typename ST>
+__global__ void __launch_bounds__(SORT_WAVES * 64) embed_sort_kernel(const EmbedUpdate p, int ranges, int range) {
+  extern __shared__ __align__(16) int lds[];
+  if ((int)blockIdx.x >= ranges) {
+    transpose_rows<ST>(p, blockIdx.x - ranges, reinterpret_cast<ST*>(lds));
+    return;
+  }
+  __shared__ int before[SORT_WAVES], sums[SORT_WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int N = p.C * p.B, per = ((N + SORT_WAVES - 1) / SORT_WAVES + 63) / 64 * 64;
+  const int first = wave * per, last = first + per < N ? first + per : N;
+  const long long lo = (long long)blockIdx.x * range;
+  const long long hi = lo + range < p.V ? lo + range : p.V;
+  int* mine = lds + wave * range;
+  for (int i = tid; i < SORT_WAVES * range; i += SORT_WAVES * 64) lds[i] = 0;
+  __syncthreads();
+  int less = 0;
+#pragma unroll 4
+  for (int i = first + lane; i < last; i += 64) {
+    const long long id = p.ids[i];
+    less += id >= 0 && id < lo;
+    if (id >= lo && id < hi) atomicAdd(&mine[id - lo], 1);  // (a count: the order does not matter)
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) less += __shfl_xor(less, o);
+  if (lane == 0) before[wave] = less;
+  __syncthreads();
+  int base = 0;
+#pragma unroll
+  for (int w = 0; w < SORT_WAVES; ++w) base += before[w];
+  // where each id's places of each wave start: ids in order, then waves
+  for (int r0 = 0; r0 < range; r0 += SORT_WAVES * 64) {
+    const int r = r0 + tid;
+    int total = 0;
+    if (r < range)
+      for (int w = 0; w < SORT_WAVES; ++w) total += lds[w * range + r];
+    int scan = total;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(scan, o);
+      if (lane >= o) scan += v;
+    }
+    if (lane == 63) sums[wave] = scan;
+    __syncthreads();
+    int at = base + scan - total;
+    for (int w = 0; w < SORT_WAVES; ++w) {
+      if (w < wave) at += sums[w];
+      base += sums[w];
+    }
+    if (r < range)
+      for (int w = 0; w < SORT_WAVES; ++w) {
+        const int n = lds[w * range + r];
+        lds[w * range + r] = at;
+        at += n;
+      }
+    __syncthreads();
+  }
+  if (blockIdx.x == ranges - 1)  // behind the last place with an id
+    for (int i = base + tid; i <= N; i += SORT_WAVES * 64) p.key[i] = -1;
+  for (int i0 = first; i0 < last; i0 += 64) {
+    const int i = i0 + lane;
+    const long long id = i < last ? p.ids[i] : -1;
+    const bool in = id >= lo && id < hi;
+    const int own = in ? (int)(id - lo) : -1;
+    unsigned long long left = __ballot(in);
+    while (left) {  // one id after the other, its places in lane order
+      const int which = __shfl(own, __ffsll((unsigned long long)left) - 1);
+      const unsigned long long same = __ballot(own == which);
+      if (own == which) {
+        const int at = mine[which] + __popcll(same & ((1ull << lane) - 1));
+        p.order[at] = i;
+        p.key[at] = (int)id;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (lane == __ffsll(same) - 1) mine[which] += __popcll(same);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      left &= ~same;
+    }
+  }
+}
+
+// A run of EMBED_RUN sorted places, 4 features a thread.  Ids that begin and end in the
+// run are finished here; a sum that came over the run's start goes to part[run][0], one
+// that goes on past its end to part[run][1].
+template <typename ST>
+__device__ __forceinline__ void add_to_table(const EmbedUpdate& p, int id, int d, const float (&sum)[4]) {
+  ST* t = static_cast<ST*>(p.table) + (long long)id * p.D + d;
+  if (p.vec_d) {
+    float old[4];
+    ST o[4];
+    load4(t, old);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = cvt<ST>(old[i] + p.alpha * sum[i]);
+    store4(t, o);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (d + i < p.D) t[i] = cvt<ST>(to_f32(t[i]) + p.alpha * sum[i]);
+  }
+}
+
+template <typename ST>
+__global__ void __launch_bounds__(256) embed_run_kernel(const EmbedUpdate p) {
+  const int slabs = gridDim.y, run = blockIdx.x, N = p.C * p.B;
+  const int d = (blockIdx.y * blockDim.x + threadIdx.x) * 4;
+  const int first = run * EMBED_RUN, last = first + EMBED_RUN < N ? first + EMBED_RUN : N;
+  (void)slabs;
+  if (p.key[first] < 0 || d >= p.D) return;
+  const ST* rows = static_cast<const ST*>(p.rows);
+  const bool whole = p.D % 4 == 0;
+  int id = p.key[first];
+  bool over = first > 0 && p.key[first - 1] == id;  // came over the start
+  float sum[4] = {};
+  for (int i = first; i < last;) {
+    const int n = p.order[i];
+    const ST* from = rows + (long long)n * p.D + d;
+    float v[4] = {};
+    if (whole) {
+      load4(from, v);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (d + q < p.D) v[q] = to_f32(from[q]);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) sum[q] += v[q];
+    ++i;
+    const int next = p.key[i];
+    if (i < last && next == id) continue;
+    // the id's last place in this run
+    const bool on = next == id;
+    if (over || on) {
+      float* to = p.part + ((long long)run * 2 + (over ? 0 : 1)) * p.D + d;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (d + q < p.D) to[q] = sum[q];
+    } else {
+      add_to_table<ST>(p, id, d, sum);
+    }
+    if (next < 0 || i >= last) break;
+    id = next;
+    over = false;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) sum[q] = 0.0f;
+  }
+}
+
+// Sums that cross runs' ends, joined in order by the run they begin in.
+template <typename ST>
+__global__ void __launch_bounds__(256) embed_join_kernel(const EmbedUpdate p) {
+  const int run = blockIdx.x, N = p.C * p.B, runs = (N + EMBED_RUN - 1) / EMBED_RUN;
+  const int d = (blockIdx.y * blockDim.x + threadIdx.x) * 4;
+  const int first = run * EMBED_RUN, end = first + EMBED_RUN;
+  if (end >= N || d >= p.D) return;
+  const int id = p.key[end - 1];
+  if (id < 0 || p.key[end] != id) return;
+  if (p.key[first] == id && first > 0 && p.key[first - 1] == id) return;  // it began earlier
+  float sum[4] = {};
+  for (int r = run, slot = 1; r < runs; ++r, slot = 0) {
+    if (slot == 0 && p.key[r * EMBED_RUN] != id) break;
+    const float* from = p.part + ((long long)r * 2 + slot) * p.D + d;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (d + q < p.D) sum[q] += from[q];
+  }
+  add_to_table<ST>(p, id, d, sum);
+}
+
+template <typename ST>
+hipError_t run_embed(const EmbedProblem& p, hipStream_t s) {
+  auto blocks = [&](int bt, int dt) {
+    return dim3((unsigned)((long long)p.C * ((p.B + bt - 1) / bt) * ((p.D + dt - 1) / dt)));
+  };
+  if (p.B == 1) hipLaunchKernelGGL((embed_kernel<ST, 1>), blocks(1, 1024), dim3(256), 0, s, p);
+  else if (p.B <= 4) hipLaunchKernelGGL((embed_kernel<ST, 4>), blocks(4, 1024), dim3(256), 0, s, p);
+  else if (p.B <= 16) hipLaunchKernelGGL((embed_kernel<ST, 16>), blocks(16, 256), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((embed_kernel<ST, 64>), blocks(64, 64), dim3(256), 0, s, p);
+  return hipGetLastError();
+}
+
+template <typename ST>
+hipError_t run_update(const EmbedUpdate& p, hipStream_t s) {
+  const int N = p.C * p.B;
+  if (N < EMBED_SORTED) {
+    hipLaunchKernelGGL((embed_few_kernel<ST>), dim3((unsigned)(N * (long long)((p.D + 255) / 256))), dim3(256), 0, s, p);
+    return hipGetLastError();
+  }
+  const int range = sort_range(p.V), ranges = (int)(((long long)p.V + range - 1) / range);
+  const long long turns = (long long)p.C * ((p.B + 63) / 64) * ((p.D + 63) / 64);
+  const int turn_lds = 64 * 66 * (int)sizeof(ST), sort_lds = SORT_WAVES * range * 4;
+  hipLaunchKernelGGL((embed_sort_kernel<ST>), dim3((unsigned)(ranges + turns)), dim3(SORT_WAVES * 64),
+                     turn_lds > sort_lds ? turn_lds : sort_lds, s, p, ranges, range);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const int threads = p.D >= 1024 ? 256 : ((p.D + 3) / 4 + 63) / 64 * 64;
+  const dim3 grid((unsigned)((N + EMBED_RUN - 1) / EMBED_RUN), (unsigned)((p.D + 4 * threads - 1) / (4 * threads)));
+  hipLaunchKernelGGL((embed_run_kernel<ST>), grid, dim3(threads), 0, s, p);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((embed_join_kernel<ST>), grid, dim3(threads), 0, s, p);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_embedding(const EmbedProblem& p, int storage, hipStream_t s) {
+  if (storage == 0) return run_embed<float>(p, s);
+  return storage == 1 ? run_embed<f16>(p, s) : run_embed<bf16>(p, s);
+}
+
+hipError_t launch_embedding_update(const EmbedUpdate& p, int storage, hipStream_t s) {
+  if (storage == 0) return run_update<float>(p, s);
+  return storage == 1 ? run_update<f16>(p, s) : run_update<bf16>(p, s);
+}
+
+}  // namespace ipc

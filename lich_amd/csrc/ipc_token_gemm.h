@@ -1,0 +1,354 @@
+// ipc_token_gemm.h - the matrix products of a softmax over tokens (gfx950).
+//
+//   TOKEN_STATS   Z[v][n] = sum_d W[v][d] F[d][n], of which only each tile's largest value and
+//                 sum of exponentials a column are kept, and the target's logit
+//   TOKEN_ERROR   the same products again; e = onehot - softmax(Z), rounded to the operand
+//                 type and stored transposed, ET[n][v]
+//   TOKEN_GRAD    P[d][n] = sum_v W[v][d] e[v][n]     (a slice of the vocabulary a workgroup)
+//   TOKEN_WEIGHT  W[v][d] += alpha sum_n e[v][n] F[d][n]
+//
+// v_mfma_f32_32x32x16 tiles in the pipeline of ipc_ckpt_gemm.h: four stages of 32 k filled by
+// LDS-DMA loads, one barrier a stage, loads and the next fragments' reads between the
+// products.  B is k-contiguous in every product (F^T, ET, F lie as that asks); A is for
+// the first two (W), and k-rows read transposed for the others (W, ET), so that one
+// copy of W and one of the errors serve both products they appear in.
+//
+// fp32 tensors: every operand is the sum of three bf16 terms (24 bits, the type's own), and a
+// product the six term products above 2^-24 of it, smallest first; 233 TFLOP/s at
+// six times the 16-bit work against 154 of the fp32 matrix instruction's peak use.
+//
+// The accumulators of the first two lie with a column n a lane (and rows v in its
+// registers), so that a column's maximum and sum are the lane's own business up to one
+// exchange between the halves of a wave and one between waves; the others' with four
+// consecutive columns a lane, for the shared tile epilogue.
+#pragma once
+
+#include "ipc_ckpt_gemm.h"
+#include "ipc_token.h"
+
+namespace ipc {
+
+enum { TOKEN_STATS = 0, TOKEN_ERROR = 1, TOKEN_GRAD = 2, TOKEN_WEIGHT = 3 };
+
+// One product.  Rows start at multiples of 4 bytes; a and b with all their terms lie
+// below 2^31 bytes.
+struct TokenGemm {
+  int M, N, K;                     // K: of one term; A k-contiguous: of any length, else a multiple of 32
+  const void* a; long long lda;    // elements
+  const void* b; long long ldb;
+  long long a_bytes, b_bytes;      // buffers' ends (loads past them give 0)
+  unsigned a_term, b_term;         // bytes from one term to the next
+  int slices;                      // TOKEN_GRAD: of the contraction
+  void* out;                       // STATS: float2 [tile rows][N]; ERROR: ET; GRAD: [slices][M][N] fp32; WEIGHT: W
+  long long out_ld, out_term;      // ERROR: elements
+  int out_rows;                    // ERROR: of ET, N up to a multiple of 32
+  int add;                         // GRAD: out holds sums already
+  int vec;                         // WEIGHT: out allows 4-element accesses
+  float scal;                      // WEIGHT: alpha; ERROR: the errors' scale
+  // STATS, ERROR
+  const long long* targets; int first, V;  // first: of the piece's rows
+  float* target_logit;
+  const float2* stats;             // ERROR: of each column, largest logit and 1 / sum of exp(z - largest)
+};
+// storage: 0 (three bf16 terms), 1, 2
+hipError_t launch_token_stats(const TokenGemm& p, int storage, int bm, hipStream_t s);
+hipError_t launch_token_error(const TokenGemm& p, int storage, int bm, hipStream_t s);
+hipError_t launch_token_grad(const TokenGemm& p, int storage, int tile, hipStream_t s);
+hipError_t launch_token_weight(const TokenGemm& p, int storage, hipStream_t s);
+
+namespace token {
+
+using namespace mx;
+
+// a and b terms of product g of a contraction over three terms each, smallest first
+constexpr int PRODUCTS = 6;
+__device__ __forceinline__ unsigned term_of(unsigned packed, int g) { return (packed >> (2 * g)) & 3u; }
+constexpr unsigned TERMS_A = 2u | 1u << 2 | 0u << 4 | 1u << 6 | 0u << 8 | 0u << 10;
+constexpr unsigned TERMS_B = 0u | 1u << 2 | 2u << 4 | 0u << 6 | 1u << 8 | 0u << 10;
+
+template <bool EXACT>
+__device__ __forceinline__ float exp_of(float x) {
+  // the hardware exponential's relative error grows with |x| by 2^-24 a unit; 16-bit results do not see it
+  if constexpr (EXACT) return expf(x);
+  return __builtin_amdgcn_exp2f(x * 1.44269504f);
+}
+
+template <typename OT, bool SPLIT, int MODE, int BM, int BN, int WGM, int WGN>
+__global__ void __launch_bounds__(WGM * WGN * 64) token_gemm_kernel(const TokenGemm p) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  using MF = Mfma32<OT>;
+  typedef typename MF::operand V;
+  constexpr bool MN = MODE == TOKEN_GRAD || MODE == TOKEN_WEIGHT, COLUMNS = !MN;
+  constexpr int NW = WGM * WGN, WTM = BM / WGM, WTN = BN / WGN, RM = WTM / 32, RN = WTN / 32;
+  constexpr int A_BYTES = BM * 64, B_BYTES = BN * 64, STAGE = A_BYTES + B_BYTES;
+  constexpr int IA = A_BYTES / 1024 / NW, IB = B_BYTES / 1024 / NW, LPS = IA + IB;  // LDS-DMA loads per wave and stage
+  static_assert(IA * 1024 * NW == A_BYTES && IB * 1024 * NW == B_BYTES, "tile / waves");
+
+  // consecutive tiles per XCD, in supertiles of 8 x 4 (as in mx_tile_kernel); slices outermost
+  const int tn = (p.N + BN - 1) / BN, tm = (p.M + BM - 1) / BM;
+  const int b = blockIdx.x, per = gridDim.x >> 3, rem = gridDim.x & 7, xcd = b & 7;
+  const int t0 = xcd * per + (xcd < rem ? xcd : rem) + (b >> 3);
+  const int slice = MODE == TOKEN_GRAD ? t0 / (tm * tn) : 0, t = t0 - slice * tm * tn;
+  const int band = t / (8 * tn), rows = tm - band * 8 < 8 ? tm - band * 8 : 8, w8 = t - band * 8 * tn;
+  const int cs = w8 / (rows * 4), cols = tn - cs * 4 < 4 ? tn - cs * 4 : 4, w2 = w8 - cs * rows * 4;
+  const int m0 = (band * 8 + w2 / cols) * BM, n0 = (cs * 4 + w2 % cols) * BN;
+
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = w / WGN, wn = w % WGN, lr = lane & 31, lk = lane >> 5;
+  const int M = p.M, N = p.N, K = p.K, GS = (K + 31) / 32, tail = K - (GS - 1) * 32;
+  // stages of this workgroup: begin .. end - 1 of all products' one after the other
+  const int all = SPLIT ? PRODUCTS * GS : GS;
+  const int begin = MODE == TOKEN_GRAD ? (int)((long long)all * slice / p.slices) : 0;
+  const int end = MODE == TOKEN_GRAD ? (int)((long long)all * (slice + 1) / p.slices) : all;
+  const int G = end - begin;
+
+  const Rsrc ga(p.a, (unsigned)p.a_bytes), gb(p.b, (unsigned)p.b_bytes);
+  const i32x4 wa = rsrc_words(p.a, (unsigned)p.a_bytes), wb = rsrc_words(p.b, (unsigned)p.b_bytes);
+  // byte offset of this lane's 16 bytes of LDS-DMA instruction q of an operand
+  auto source = [&](bool mn, int q, int edge, int e0, int lim, long long ld) -> unsigned {
+    const int slot = (q * NW + w) * 64 + lane;
+    if (mn) {  // columns past the end: the last ones again or the next row's, never stored
+      const int cpr = edge / 8, r = slot / cpr, c = (slot % cpr) ^ (edge == 64 ? (r & 2) << 1 : (r & 3) << 2);
+      const int col = e0 + c * 8 < (int)ld ? e0 + c * 8 : (int)ld - 2;
+      return (unsigned)(r * ld + col) * 2u;
+    }
+    const int r = slot >> 2, c = (slot & 3) ^ ((r >> 2) & 3), row = e0 + r < lim ? e0 + r : lim - 1;
+    return (unsigned)(row * ld) * 2u + (unsigned)c * 16u;
+  };
+  unsigned oa[IA], ob[IB];
+#pragma unroll
+  for (int q = 0; q < IA; ++q) oa[q] = source(MN, q, BM, m0, M, p.lda);
+#pragma unroll
+  for (int q = 0; q < IB; ++q) ob[q] = source(false, q, BN, n0, N, p.ldb);
+  const unsigned step_a = MN ? (unsigned)p.lda * 64u : 64u;  // of a stage
+  // load q of a stage: uniform offsets sa, sb
+  auto load = [&](int q, unsigned char* st, unsigned sa, unsigned sb) {
+    unsigned char* at = q < IA ? st + (q * NW + w) * 1024 : st + A_BYTES + ((q - IA) * NW + w) * 1024;
+    const unsigned v = q < IA ? oa[q < IA ? q : 0] : ob[q < IA ? 0 : q - IA];
+    if constexpr (MN) to_lds16_unseen(q < IA ? wa : wb, at, v, q < IA ? sa : sb);
+    else (q < IA ? ga : gb).to_lds16(at, v, q < IA ? sa : sb);
+  };
+  // uniform offsets of stage kt (past the end: of the last, so that every step counts the
+  // same).  A k-contiguous A may end inside a stage: that one comes first, and what it has
+  // no k for is cleared.
+  unsigned sa, sb;
+  auto seek = [&](int kt) {
+    const int g = begin + (kt < G ? kt : G - 1);
+    if constexpr (SPLIT) {
+      const int product = g / GS, k = g - product * GS;
+      sa = (unsigned)k * step_a + term_of(TERMS_A, product) * p.a_term;
+      sb = (unsigned)k * 64u + term_of(TERMS_B, product) * p.b_term;
+    } else {
+      const int k = MN ? g : g == 0 ? GS - 1 : g - 1;
+      sa = (unsigned)k * step_a;
+      sb = (unsigned)k * 64u;
+    }
+  };
+
+  f32x16 acc[RM][RN];
+#pragma unroll
+  for (int i = 0; i < RM; ++i)
+#pragma unroll
+    for (int j = 0; j < RN; ++j)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
+
+  // fragments of 16 k (half s of a stage): row / column lr of a 32-wide block, k 8 lk .. + 7
+  const int g4 = lane >> 4, li = lane & 15;
+  const int tr_row = 8 * (g4 >> 1) + (li >> 2), tr_low = 2 * (g4 & 1) + ((li & 3) >> 1);
+  auto straight = [&](const unsigned char* blk, int e, int s) -> V {
+    return *reinterpret_cast<const V*>(blk + (e + lr) * 64 + ((((s * 2) | lk) ^ ((lr >> 2) & 3)) << 4));
+  };
+  auto turned = [&](const unsigned char* blk, int rowb, int e, int s) -> V {
+    const int chunk = (((e >> 5) ^ (rowb == 128 ? li >> 3 : li >> 2)) << 2) | tr_low;
+    const unsigned char* p0 = blk + (s * 16 + tr_row) * rowb + (chunk << 4) + (li & 1) * 8;
+    const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p0));
+    const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p0 + 4 * rowb));
+    return __builtin_bit_cast(V, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  V fa[2][RM], fb[2][RN];
+  auto read_a = [&](const unsigned char* st, int i, int s) -> V {
+    if constexpr (MN) return turned(st, BM * 2, wm * WTM + i * 32, s);
+    else return straight(st, wm * WTM + i * 32, s);
+  };
+  auto read_b = [&](const unsigned char* st, int j, int s) -> V { return straight(st + A_BYTES, wn * WTN + j * 32, s); };
+  auto stage = [&](int kt) -> unsigned char* { return smem + (kt & (STAGES - 1)) * STAGE; };
+
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) {
+    seek(s);
+#pragma unroll
+    for (int q = 0; q < LPS; ++q) load(q, stage(s), sa, sb);
+  }
+  wait_loads<2 * LPS>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  if (!SPLIT && !MN && tail < 32) {
+    unsigned short* h = reinterpret_cast<unsigned short*>(smem);
+    for (int i = tid; i < BM * 32; i += NW * 64)
+      if (((i & 31) ^ (((i >> 7) & 3) << 3)) >= tail) h[i] = 0;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  }
+#pragma unroll
+  for (int j = 0; j < RN; ++j) fb[0][j] = read_b(stage(0), j, 0);
+#pragma unroll
+  for (int i = 0; i < RM; ++i) fa[0][i] = read_a(stage(0), i, 0);
+
+  // half a step: the products of set S; the fragments of the next 16 k (half S ^ 1 of
+  // `next`) and half of stage kt + 3's loads between them
+  auto half = [&](auto SV, const unsigned char* next, unsigned char* fill) {
+    constexpr int S = decltype(SV)::value, O = S ^ 1;
+    constexpr int L0 = S == 0 ? 0 : (LPS + 1) / 2, L1 = S == 0 ? (LPS + 1) / 2 : LPS;
+    constexpr int NM = RM * RN, NR = RM + RN;
+#pragma unroll
+    for (int q = 0; q < NM; ++q) {
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+        if (r * NM / NR == q) {
+          if (r < RN) fb[O][r < RN ? r : 0] = read_b(next, r, O);
+          else fa[O][r < RN ? 0 : r - RN] = read_a(next, r - RN, O);
+        }
+#pragma unroll
+      for (int l = L0; l < L1; ++l)
+        if ((l - L0) * NM / (L1 - L0) == q) load(l, fill, sa, sb);
+      const int i = q / RN, j = q % RN;
+      acc[i][j] = COLUMNS ? MF::run(fa[S][i], fb[S][j], acc[i][j]) : MF::run(fb[S][j], fa[S][i], acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+#pragma unroll 1
+  for (int kt = 0; kt < G; ++kt) {
+    // stage kt + 1 of this wave has landed (kt + 2 may be in flight), then everybody's;
+    // everybody is done with stage kt - 1, which kt + 3 takes
+    wait_loads<LPS>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    seek(kt + 3);
+    half(std::integral_constant<int, 0>{}, stage(kt), stage(kt + 3));
+    half(std::integral_constant<int, 1>{}, stage(kt + 1), stage(kt + 3));
+  }
+  wait_loads<0>();  // no load may land in the epilogue's LDS
+
+  if constexpr (MODE == TOKEN_STATS) {
+    __syncthreads();
+    float2* red = reinterpret_cast<float2*>(smem);  // [WGM][BN]
+#pragma unroll
+    for (int j = 0; j < RN; ++j) {
+      const int c = wn * WTN + j * 32 + lr, n = n0 + c, mw = m0 + wm * WTM + 4 * lk;
+      const long long target = (n < N ? p.targets[n] : -1) - p.first;
+      float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < RM; ++i)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          const int m = mw + i * 32 + 8 * (q >> 2) + (q & 3);
+          if (m >= M) acc[i][j][q] = -__builtin_inff();
+          top = __builtin_fmaxf(top, acc[i][j][q]);
+          if (m == target && m < M) p.target_logit[n] = acc[i][j][q];
+        }
+      top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+      const float from = top == -__builtin_inff() ? 0.0f : top;  // (a column of -inf: no sum, and no NaN)
+#pragma unroll
+      for (int i = 0; i < RM; ++i)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) sum += exp_of<SPLIT>(acc[i][j][q] - from);
+      sum += __shfl_xor(sum, 32);
+      if (lk == 0) red[wm * BN + c] = make_float2(top, sum);
+    }
+    __syncthreads();
+    for (int c = tid; c < BN; c += NW * 64) {
+      if (n0 + c >= N) continue;
+      float2 v[WGM];
+      float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < WGM; ++i) {
+        v[i] = red[i * BN + c];
+        top = __builtin_fmaxf(top, v[i].x);
+      }
+#pragma unroll
+      for (int i = 0; i < WGM; ++i) sum += v[i].x == -__builtin_inff() ? v[i].y : v[i].y * exp_of<SPLIT>(v[i].x - top);
+      static_cast<float2*>(p.out)[(long long)(m0 / BM) * N + n0 + c] = make_float2(top, sum);
+    }
+  } else if constexpr (MODE == TOKEN_ERROR) {
+    __syncthreads();
+    constexpr int LD = WTM + 8, TERMS = SPLIT ? 3 : 1;  // (LDS rows of 2 WTM + 16 bytes)
+    unsigned short* es = reinterpret_cast<unsigned short*>(smem) + w * 32 * LD;
+    unsigned short* out = static_cast<unsigned short*>(p.out);
+#pragma unroll
+    for (int j = 0; j < RN; ++j) {
+      const int n = n0 + wn * WTN + j * 32 + lr, mw = m0 + wm * WTM + 4 * lk;
+      const long long id = n < N ? p.targets[n] : -1;
+      const bool real = id >= 0 && id < p.V;
+      const long long target = id - p.first;
+      const float2 st = real ? p.stats[n] : make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int i = 0; i < RM; ++i)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          const int m = mw + i * 32 + 8 * (q >> 2) + (q & 3);
+          const float e = (m == target ? 1.0f : 0.0f) - exp_of<SPLIT>(acc[i][j][q] - st.x) * st.y;
+          acc[i][j][q] = real && m < M ? e * p.scal : 0.0f;
+        }
+#pragma unroll
+      for (int term = 0; term < TERMS; ++term) {
+#pragma unroll
+        for (int i = 0; i < RM; ++i)
+#pragma unroll
+          for (int q = 0; q < 16; q += 4) {
+            unsigned short h[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const OT o = cvt<OT>(acc[i][j][q + u]);
+              h[u] = __builtin_bit_cast(unsigned short, o);
+              if (SPLIT) acc[i][j][q + u] -= to_f32(o);  // exact; NaN stays
+            }
+            *reinterpret_cast<uint2*>(es + lr * LD + i * 32 + 2 * q + 4 * lk) =
+                make_uint2(h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16);
+          }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        constexpr int LPR = WTM / 8, PASSES = 32 / (64 / LPR);  // lanes a row of ET, passes over 32
+#pragma unroll
+        for (int u = 0; u < PASSES; ++u) {
+          const int r = u * (64 / LPR) + lane / LPR, c = lane % LPR * 8;
+          const uint4 v = *reinterpret_cast<const uint4*>(es + r * LD + c);
+          const long long row = n0 + wn * WTN + j * 32 + r;
+          const int col = m0 + wm * WTM + c;
+          // rows and columns past the ends, up to ET's own (multiples of 32), get zeros
+          if (row < p.out_rows && col < p.out_ld)
+            *reinterpret_cast<uint4*>(out + term * p.out_term + row * p.out_ld + col) = v;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      }
+    }
+  } else {
+    typedef typename std::conditional<MODE == TOKEN_GRAD || SPLIT, float, OT>::type ST;
+    MxProblem e{};
+    e.M = M; e.N = N; e.scal = MODE == TOKEN_GRAD ? 1.0f : p.scal;
+    e.out = MODE == TOKEN_GRAD ? static_cast<float*>(p.out) + (long long)slice * M * N : p.out;
+    float* es = reinterpret_cast<float*>(smem) + w * 32 * (WTN + 4);
+    const int mw = m0 + wm * WTM, nw = n0 + wn * WTN;
+    if (MODE == TOKEN_GRAD && !p.add) tile_epilogue<ST, KIND_FWD, ACT_IDENTITY, true, RM, RN>(e, acc, es, mw, nw);
+    else if (MODE == TOKEN_GRAD || p.vec) tile_epilogue<ST, KIND_WEIGHT, ACT_IDENTITY, true, RM, RN>(e, acc, es, mw, nw);
+    else tile_epilogue<ST, KIND_WEIGHT, ACT_IDENTITY, false, RM, RN>(e, acc, es, mw, nw);
+  }
+}
+
+template <typename OT, bool SPLIT, int MODE, int BM, int BN, int WGM, int WGN>
+hipError_t run_tile(const TokenGemm& p, hipStream_t s) {
+  constexpr int NW = WGM * WGN, ring = STAGES * (BM + BN) * 64;
+  constexpr int epi = MODE == TOKEN_STATS ? WGM * BN * 8 : MODE == TOKEN_ERROR ? NW * 32 * (BM / WGM + 8) * 2 : NW * 32 * (BN / WGN + 4) * 4;
+  constexpr int smem = epi > ring ? epi : ring;
+  static_assert(smem <= 160 * 1024, "LDS");
+  const void* fn = reinterpret_cast<const void*>(&token_gemm_kernel<OT, SPLIT, MODE, BM, BN, WGM, WGN>);
+  const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != hipSuccess) return e;
+  const long long tiles = ((p.M + BM - 1LL) / BM) * ((p.N + BN - 1LL) / BN) * (MODE == TOKEN_GRAD ? p.slices : 1);
+  TokenGemm q = p;
+  void* args[] = {&q};
+  return hipLaunchKernel(fn, dim3((unsigned)tiles), dim3(NW * 64), args, smem, s);
+}
+
+}  // namespace token
+}  // namespace ipc

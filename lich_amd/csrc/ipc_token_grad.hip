@@ -1,0 +1,22 @@
+// ipc_token_grad.hip - the products that take a piece's errors: the state's gradient and W's update.
+#include "ipc_token_gemm.h"
+
+namespace ipc {
+namespace {
+
+template <typename OT, bool SPLIT>
+hipError_t grad(const TokenGemm& p, int tile, hipStream_t s) {
+  if (tile == 256) return token::run_tile<OT, SPLIT, TOKEN_GRAD, 256, 256, 2, 2>(p, s);
+  if (tile == 128 && p.N > 64) return token::run_tile<OT, SPLIT, TOKEN_GRAD, 128, 128, 2, 2>(p, s);
+  if (tile == 128) return token::run_tile<OT, SPLIT, TOKEN_GRAD, 128, 64, 2, 2>(p, s);
+  return token::run_tile<OT, SPLIT, TOKEN_GRAD, 64, 64, 2, 2>(p, s);
+}
+
+}  // namespace
+
+hipError_t launch_token_grad(const TokenGemm& p, int storage, int tile, hipStream_t s) {
+  if (storage == 0) return grad<bf16, true>(p, tile, s);
+  return storage == 1 ? grad<f16, false>(p, tile, s) : grad<bf16, false>(p, tile, s);
+}
+
+}  // namespace ipc

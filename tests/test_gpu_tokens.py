@@ -1,0 +1,205 @@
+"""Operators over tokens against their definitions in 64 bits.
+
+Tolerances: u is half a step of the storage type (bf16 2^-8, fp16 2^-11, fp32 2^-24), H = 2^-24 the
+fp32 arithmetic's.  Bounds are per element and worst case: a sum of n products of
+magnitudes summing to S is off by at most (n + 2) H S; the activations are within
+16 H of theirs, relative."""
+import pytest
+import torch
+
+from lich_amd import tokens
+from tests import token_oracle as O
+from tests.helpers import DEV, gen
+
+pytestmark = pytest.mark.gpu
+
+H = 2.0 ** -24
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def check(got, want, bound, what):
+    got, want, bound = got.detach().cpu().double(), want.cpu(), bound.cpu()
+    assert bool(torch.isfinite(got).all()), what
+    over = ((got - want).abs() - bound).max()
+    assert float(over) <= 0, f"{what}: {float(over):.3e} over a bound of {float(bound.max()):.3e} at most"
+
+
+def randn(shape, g, dtype, scale=1.0):
+    return (torch.randn(shape, generator=g) * scale).to(dtype)
+
+
+def some_ids(V, shape, g, padded=0.2):
+    """Ids with many repeats of a few, and padded places of three kinds."""
+    ids = torch.where(torch.rand(shape, generator=g) < 0.5, torch.randint(0, V, shape, generator=g),
+                      torch.randint(0, min(V, 3), shape, generator=g))
+    bad = torch.tensor([-1, V, 2 ** 40])[torch.randint(0, 3, shape, generator=g)]
+    return torch.where(torch.rand(shape, generator=g) < padded, bad, ids)
+
+
+# ------------------------------------------------------------------ embedding
+SIZES = [(1, 1, 1, 1), (5, 3, 1, 1), (7, 1030, 3, 1), (40, 17, 2, 3), (11, 1029, 1, 4), (64, 33, 5, 9), (100, 260, 2, 16),
+         (130, 65, 3, 17), (1000, 64, 8, 64), (333, 129, 4, 131), (3000, 131, 5, 301)]
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("V,D,C,B", SIZES)
+def test_embedding(V, D, C, B, name):
+    dt, g = TYPES[name], gen(V + D)
+    ids, table = some_ids(V, (C, B), g), randn((V, D), g, dt)
+    x = torch.full((C * D, B), float("nan"), dtype=dt, device=DEV)
+    tokens.build_embedding(V, D, C, B, dt, 1.7)(ids.to(DEV), table.to(DEV), x)
+    want = O.embedding(ids, table, torch.tensor(1.7, dtype=torch.float32).item())
+    # the product rounded to fp32, then to the type
+    check(x, want, (half_step(dt) + 2 * H) * want.abs() + 2.0 ** -25 * (dt == torch.float16), "x")
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("V,D,C,B", SIZES + [(3, 20, 1, 513), (1, 7, 2, 700), (70000, 5, 3, 1000), (600000, 4, 1, 520), (50, 1100, 1, 600)])
+def test_embedding_update(V, D, C, B, name):
+    dt, gn = TYPES[name], gen(V + D + 1)
+    ids, table, g = some_ids(V, (C, B), gn), randn((V, D), gn, dt), randn((C * D, B), gn, dt)
+    k = tokens.build_embedding_update(V, D, C, B, dt, 0.3)
+    assert (k.workspace_bytes > 0) == (C * B >= 513)
+    t = table.to(DEV)
+    k(t, ids.to(DEV), g.to(DEV), workspace=k.new_workspace(DEV))
+    total, size, many = O.embedding_sums(ids, g, V)
+    alpha = torch.tensor(0.3, dtype=torch.float32).item()
+    want = table.double() + alpha * total
+    bound = half_step(dt) * want.abs() + 2.0 ** -25 * (dt == torch.float16) + (many[:, None] + 4) * H * alpha * size + 4 * H * (table.double().abs() + want.abs())
+    check(t, want, bound * 1.01, "table")
+    unused = many == 0
+    assert torch.equal(t.cpu()[unused], table[unused])
+
+
+def test_embedding_update_gives_the_same_bits():
+    V, D, C, B = 1000, 96, 3, 700
+    g = gen(4)
+    ids, table, e = some_ids(V, (C, B), g).to(DEV), randn((V, D), g, torch.float32).to(DEV), randn((C * D, B), g, torch.float32).to(DEV)
+    k = tokens.build_embedding_update(V, D, C, B, "float32", 0.1)
+    got = []
+    for _ in range(3):
+        t = table.clone()
+        k(t, ids, e, workspace=k.new_workspace(DEV))
+        got.append(t)
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+
+
+def test_embedding_update_of_padded_places_only():
+    V, D, C, B = 100, 9, 2, 400
+    table = torch.randn((V, D), device=DEV)
+    t = table.clone()
+    k = tokens.build_embedding_update(V, D, C, B, "float32", 0.1)
+    k(t, torch.full((C, B), -1, device=DEV), torch.full((C * D, B), float("nan"), device=DEV), workspace=k.new_workspace(DEV))
+    assert torch.equal(t, table)
+
+
+# -------------------------------------------------------------------- dropout
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("M,B,p", [(1, 1, 0.5), (3, 5, 0.0), (7, 9, 0.1), (64, 33, 0.25), (129, 8, 0.9), (40, 64, 65535 / 65536)])
+def test_dropout(M, B, p, name):
+    dt, g = TYPES[name], gen(M + B)
+    seed, step, site = 0x123456789ABCDEF, -3, 7
+    x = randn((M, B), g, dt)
+    x[0, 0] = float("inf")
+    rng, xd = torch.tensor([seed, step], device=DEV), x.to(DEV)
+    out = torch.full_like(xd, float("nan"))
+    k = tokens.build_dropout(M, B, dt, p, site=site)
+    k(xd, rng, out)
+    dropped = round(p * 65536)
+    keep = O.kept(M * B, seed, step, site, dropped).reshape(M, B)
+    want = torch.where(keep, x.double() * 65536 / (65536 - dropped), torch.zeros((), dtype=torch.float64))
+    # share, product and result are rounded; at the type's end the result may be infinite
+    top = torch.finfo(dt).max
+    fine = want.abs() <= top
+    got = out.cpu().double()
+    assert torch.equal(got == 0, (want == 0) | ~keep)
+    assert bool(((got - want).abs()[fine] <= (half_step(dt) + 3 * H) * want.abs()[fine] + 2.0 ** -25 * (dt == torch.float16)).all())
+    assert bool(torch.isinf(got[~fine]).all())
+    k(xd, rng, xd)  # in place
+    assert torch.equal(torch.nan_to_num(xd), torch.nan_to_num(out))
+
+
+def test_dropout_of_a_view_off_16_bytes():
+    M, B = 33, 31
+    base = torch.randn(M * B + 1, device=DEV)
+    rng = torch.tensor([5, 6], device=DEV)
+    k = tokens.build_dropout(M, B, "float32", 0.5)
+    want, out = torch.empty((M, B), device=DEV), torch.full((M * B + 2,), 9.0, device=DEV)
+    k(base[1:].reshape(M, B).clone(), rng, want)
+    k(base[1:].reshape(M, B), rng, out[1:-1].reshape(M, B))
+    assert torch.equal(out[1:-1].reshape(M, B), want) and float(out[0]) == float(out[-1]) == 9.0
+
+
+# -------------------------------------------------------------------- softmax
+def softmax_bounds(r, w, dt, V, D, B, activation, alpha):
+    """Per element: what loss, G and W may be off by."""
+    u = half_step(dt)
+    # f rounded to the type (identity, relu: exact); fp32: three bf16 terms, six of nine products
+    df = (0.0 if activation in ("identity", "relu") and dt != torch.float32 else 17 * H if dt == torch.float32 else u + 17 * H)
+    products = 6 if dt == torch.float32 else 1
+    dz = (r["size"] * (df + (8 * H if dt == torch.float32 else 0) + (products * D + 4) * H)).max(0).values + 2.0 ** -25 * (dt == torch.float16) * w.double().abs().sum(1).max()
+    near = 2.0 ** -19  # exp and log: the exponent's own rounding, 2^-24 of at most 32 where a result counts
+    loss = 2 * dz + near * (1 + r["loss"].abs()) + (V + 64) * H
+    de = r["p"] * ((2 * dz).expm1() + near + (V + 64) * H) + (u if dt != torch.float32 else H) * r["e"].abs() + (2.0 ** -35 if dt == torch.float16 else H)
+    wa, n = w.double().abs(), (V + 64) * products
+    g = r["df"].abs() * (wa.T @ de + n * H * (wa.T @ r["e"].abs())) + (u + 20 * H) * r["g"].abs() + 16 * H * (wa.T @ r["e"].abs()) + 2.0 ** -25 * (dt == torch.float16)
+    fa = r["f"].abs()
+    dw = de @ fa.T + r["e"].abs() @ (fa * df).T + (B * products + 8) * H * (r["e"].abs() @ fa.T) + (2.0 ** -25 * (dt == torch.float16)) * r["e"].abs().sum(1, keepdim=True)
+    new = w.double() + alpha * r["dw"]
+    return loss, g * 1.01, (alpha * dw + (u + 2 * H) * new.abs() + 4 * H * w.double().abs() + 2.0 ** -25 * (dt == torch.float16)) * 1.01
+
+
+def softmax_case(V, D, B, dt, seed, padded=0.15, wscale=None):
+    g = gen(seed)
+    x, w = randn((D, B), g, dt), randn((V, D), g, dt, wscale if wscale is not None else 2.0 / D ** 0.5)
+    return x, w, some_ids(V, (B,), g, padded)
+
+
+def run_update(x, w, targets, activation, alpha):
+    (D, B), V, dt = x.shape, w.shape[0], x.dtype
+    k = tokens.build_token_update(V, D, B, activation, dt, alpha)
+    w = w.clone()
+    loss, g = torch.full((B,), float("nan"), device=DEV), torch.full((D, B), float("nan"), dtype=dt, device=DEV)
+    ws = k.new_workspace(DEV)
+    ws.fill_(255)  # (a NaN in every type)
+    k(x, w, targets, loss, g, workspace=ws)
+    return loss, g, w
+
+
+SOFTMAX = [(1, 1, 1), (2, 1, 1), (1, 5, 3), (10, 64, 128), (3, 33, 2), (17, 31, 65), (65, 40, 64), (257, 96, 33), (1000, 37, 130),
+           (130, 515, 77), (2001, 300, 257), (5003, 64, 300), (300, 1100, 1), (4100, 70, 5)]
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("V,D,B", SOFTMAX)
+def test_token_update(V, D, B, name):
+    dt = TYPES[name]
+    activation = ["identity", "relu", "tanh", "sigmoid", "silu", "gelu"][(V + D + B) % 6]
+    x, w, t = softmax_case(V, D, B, dt, V + D + B)
+    alpha = 0.25
+    loss, g, wn = run_update(x.to(DEV), w.to(DEV), t.to(DEV), activation, alpha)
+    r = O.softmax(x, w, t, activation)
+    bl, bg, bw = softmax_bounds(r, w, dt, V, D, B, activation, alpha)
+    check(loss, r["loss"], bl, "loss")
+    check(g, r["g"], bg, "g")
+    check(wn, w.double() + alpha * r["dw"], bw, "w")
+    padded = (t < 0) | (t >= V)
+    assert bool((loss.cpu()[padded] == 0).all()) and bool((g.cpu()[:, padded] == 0).all())
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("activation", ["identity", "relu", "tanh", "sigmoid", "silu", "gelu"])
+def test_token_loss(activation, name):
+    dt = TYPES[name]
+    for V, D, B in ((10, 64, 128), (999, 77, 3), (300, 130, 90)):
+        x, w, t = softmax_case(V, D, B, dt, V)
+        k = tokens.build_token_loss(V, D, B, activation, dt)
+        loss, wd = torch.full((B,), float("nan"), device=DEV), w.to(DEV)
+        k(x.to(DEV), wd, t.to(DEV), loss, workspace=k.new_workspace(DEV))
+        r = O.softmax(x, w, t, activation)
+        check(loss, r["loss"], softmax_bounds(r, w, dt, V, D, B, activation, 0.0)[0], "loss")
+        assert torch.equal(wd.cpu(), w)
