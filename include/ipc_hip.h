@@ -621,9 +621,11 @@ int ipc_dropout(const void* x, const long long* rng, void* out, int M, int B, in
  *   ipc_token_update  that, and with e = onehot - softmax(z), a descent direction:
  *                     g = f'(X) W^T e (w as it was), then w += alpha e f(X)^T
  * A padded column has loss 0, no share of w and zeros in g, whatever x holds there.  The
- * logits are never kept: they are formed per piece of the vocabulary, and for the
- * update formed again.  Sums are in fp32 in a fixed order; fp32 products are sums of
- * bf16 ones exact to 2^-24; in 16-bit storage f(X) and e are rounded once to the type.
+ * logits are never kept: they are formed in pieces of the vocabulary of at most 2^30 bytes
+ * of errors.  Sums are in fp32 in a fixed order; fp32 products are sums of bf16 ones
+ * exact to 2^-24, in which an infinite weight or state counts as the largest bf16; in 16-bit
+ * storage f(X) and e are rounded to the type (the loss knows f(X) to twice its digits, the
+ * update's to first order in what the rounding left).
  * Both need a workspace (16-byte aligned) of ipc_token_loss_workspace_bytes /
  * ipc_token_update_workspace_bytes bytes (0: refused).  w of 16 bits with an even D
  * lies on 4 bytes.

@@ -30,7 +30,6 @@ __global__ void __launch_bounds__(256) embed_kernel(const EmbedProblem p) {
   const int d0 = td * DT, b0 = tb * BT, tid = threadIdx.x;
   const ST* table = static_cast<const ST*>(p.table);
   ST* x = static_cast<ST*>(p.x);
-#pragma unroll 4
   for (int u = tid; u < BT * DT / 4; u += 256) {
     const int r = u / (DT / 4), d = d0 + u % (DT / 4) * 4, b = b0 + r;
     if (b >= p.B || d >= p.D) continue;
@@ -66,7 +65,6 @@ __global__ void __launch_bounds__(256) embed_kernel(const EmbedProblem p) {
   }
   if constexpr (BT > 1) {
     __syncthreads();
-#pragma unroll 4
     for (int u = tid; u < BT * DT / 4; u += 256) {
       const int r = u % (BT / 4) * 4, d = u / (BT / 4), b = b0 + r;
       if (b >= p.B || d0 + d >= p.D) continue;

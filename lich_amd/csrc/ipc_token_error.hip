@@ -1,27 +1,22 @@
-// ipc_token_error.hip - errors of a piece of the vocabulary.
+// ipc_token_error.hip - errors of a piece of the vocabulary, its logits formed again.
 #include "ipc_token_gemm.h"
 
 namespace ipc {
 namespace {
 
-template <int MODE, typename OT, bool SPLIT>
-hipError_t run(const TokenGemm& p, int bm, hipStream_t s) {
-  if (bm == 256) return token::run_tile<OT, SPLIT, MODE, 256, 256, 2, 2>(p, s);
-  if (bm == 128 && p.N > 64) return token::run_tile<OT, SPLIT, MODE, 128, 128, 2, 2>(p, s);
-  if (bm == 128) return token::run_tile<OT, SPLIT, MODE, 128, 64, 2, 2>(p, s);
-  return token::run_tile<OT, SPLIT, MODE, 64, 64, 2, 2>(p, s);
-}
-
-template <int MODE>
-hipError_t by_type(const TokenGemm& p, int storage, int bm, hipStream_t s) {
-  if (storage == 0) return run<MODE, bf16, true>(p, bm, s);
-  return storage == 1 ? run<MODE, f16, false>(p, bm, s) : run<MODE, bf16, false>(p, bm, s);
+template <typename OT, bool SPLIT>
+hipError_t run(const TokenGemm& p, int tile, hipStream_t s) {
+  if (tile == TILE_256) return token::run_tile<OT, SPLIT, TOKEN_ERROR, false, 256, 256, 2, 2>(p, s);
+  if (tile == TILE_128) return token::run_tile<OT, SPLIT, TOKEN_ERROR, false, 128, 128, 2, 2>(p, s);
+  if (tile == TILE_128_64) return token::run_tile<OT, SPLIT, TOKEN_ERROR, false, 128, 64, 2, 2>(p, s);
+  return token::run_tile<OT, SPLIT, TOKEN_ERROR, false, 64, 64, 2, 2>(p, s);
 }
 
 }  // namespace
 
-hipError_t launch_token_error(const TokenGemm& p, int storage, int bm, hipStream_t s) {
-  return by_type<TOKEN_ERROR>(p, storage, bm, s);
+hipError_t launch_token_error(const TokenGemm& p, int storage, int tile, hipStream_t s) {
+  if (storage == 0) return run<bf16, true>(p, tile, s);
+  return storage == 1 ? run<f16, false>(p, tile, s) : run<bf16, false>(p, tile, s);
 }
 
 }  // namespace ipc

@@ -2,6 +2,7 @@
 //
 //   TOKEN_STATS   Z[v][n] = sum_d W[v][d] F[d][n], of which only each tile's largest value and
 //                 sum of exponentials a column are kept, and the target's logit
+//   TOKEN_KEEP    that, and the exponentials, as KEPT[n][v] relative to their tile's largest
 //   TOKEN_ERROR   the same products again; e = onehot - softmax(Z), rounded to the operand
 //                 type and stored transposed, ET[n][v]
 //   TOKEN_GRAD    P[d][n] = sum_v W[v][d] e[v][n]     (a slice of the vocabulary a workgroup)
@@ -28,7 +29,14 @@
 
 namespace ipc {
 
-enum { TOKEN_STATS = 0, TOKEN_ERROR = 1, TOKEN_GRAD = 2, TOKEN_WEIGHT = 3 };
+enum { TOKEN_STATS = 0, TOKEN_KEEP = 1, TOKEN_ERROR = 2, TOKEN_GRAD = 3, TOKEN_WEIGHT = 4 };
+
+// Tiles of the first three: rows (of W) and columns of a workgroup, and the rows of a wave, whose
+// largest values and sums are kept (unit; two: with f(X) in two terms).
+enum { TILE_256 = 0, TILE_128 = 1, TILE_128_64 = 2, TILE_64 = 3 };
+inline int token_unit(int tile, bool two) {
+  return tile == TILE_256 ? 128 : tile == TILE_128 ? 64 : tile == TILE_128_64 ? (two ? 32 : 64) : 32;
+}
 
 // One product.  Rows start at multiples of 4 bytes; a and b with all their terms lie
 // below 2^31 bytes.
@@ -39,20 +47,22 @@ struct TokenGemm {
   long long a_bytes, b_bytes;      // buffers' ends (loads past them give 0)
   unsigned a_term, b_term;         // bytes from one term to the next
   int slices;                      // TOKEN_GRAD: of the contraction
-  void* out;                       // STATS: float2 [tile rows][N]; ERROR: ET; GRAD: [slices][M][N] fp32; WEIGHT: W
-  long long out_ld, out_term;      // ERROR: elements
-  int out_rows;                    // ERROR: of ET, N up to a multiple of 32
+  void* out;                       // STATS, KEEP: float2 [units][N]; ERROR: ET; GRAD: [slices][M][N] fp32; WEIGHT: W
+  void* kept;                      // KEEP: exponentials times 2^15 in fp16 (fp32: in fp32), layout of ET
+  long long out_ld, out_term;      // KEEP, ERROR: elements
+  int out_rows;                    // of ET, N up to a multiple of 32
   int add;                         // GRAD: out holds sums already
   int vec;                         // WEIGHT: out allows 4-element accesses
   float scal;                      // WEIGHT: alpha; ERROR: the errors' scale
-  // STATS, ERROR
+  // STATS, KEEP, ERROR
   const long long* targets; int first, V;  // first: of the piece's rows
   float* target_logit;
   const float2* stats;             // ERROR: of each column, largest logit and 1 / sum of exp(z - largest)
 };
 // storage: 0 (three bf16 terms), 1, 2
-hipError_t launch_token_stats(const TokenGemm& p, int storage, int bm, hipStream_t s);
-hipError_t launch_token_error(const TokenGemm& p, int storage, int bm, hipStream_t s);
+hipError_t launch_token_stats(const TokenGemm& p, int storage, int tile, bool two, hipStream_t s);
+hipError_t launch_token_keep(const TokenGemm& p, int storage, int tile, hipStream_t s);
+hipError_t launch_token_error(const TokenGemm& p, int storage, int tile, hipStream_t s);
 hipError_t launch_token_grad(const TokenGemm& p, int storage, int tile, hipStream_t s);
 hipError_t launch_token_weight(const TokenGemm& p, int storage, hipStream_t s);
 
@@ -73,25 +83,27 @@ __device__ __forceinline__ float exp_of(float x) {
   return __builtin_amdgcn_exp2f(x * 1.44269504f);
 }
 
-template <typename OT, bool SPLIT, int MODE, int BM, int BN, int WGM, int WGN>
+template <typename OT, bool SPLIT, int MODE, bool TWO, int BM, int BN, int WGM, int WGN>
 __global__ void __launch_bounds__(WGM * WGN * 64) token_gemm_kernel(const TokenGemm p) {
   extern __shared__ __align__(16) unsigned char smem[];
   using MF = Mfma32<OT>;
   typedef typename MF::operand V;
   constexpr bool MN = MODE == TOKEN_GRAD || MODE == TOKEN_WEIGHT, COLUMNS = !MN;
   constexpr int NW = WGM * WGN, WTM = BM / WGM, WTN = BN / WGN, RM = WTM / 32, RN = WTN / 32;
+  constexpr int RNC = TWO ? RN / 2 : RN, BNC = TWO ? BN / 2 : BN;  // blocks and columns of different n
   constexpr int A_BYTES = BM * 64, B_BYTES = BN * 64, STAGE = A_BYTES + B_BYTES;
+  static_assert(!TWO || (MODE == TOKEN_STATS && RN % 2 == 0), "two terms of f(X)");
   constexpr int IA = A_BYTES / 1024 / NW, IB = B_BYTES / 1024 / NW, LPS = IA + IB;  // LDS-DMA loads per wave and stage
   static_assert(IA * 1024 * NW == A_BYTES && IB * 1024 * NW == B_BYTES, "tile / waves");
 
   // consecutive tiles per XCD, in supertiles of 8 x 4 (as in mx_tile_kernel); slices outermost
-  const int tn = (p.N + BN - 1) / BN, tm = (p.M + BM - 1) / BM;
+  const int tn = (p.N + BNC - 1) / BNC, tm = (p.M + BM - 1) / BM;
   const int b = blockIdx.x, per = gridDim.x >> 3, rem = gridDim.x & 7, xcd = b & 7;
   const int t0 = xcd * per + (xcd < rem ? xcd : rem) + (b >> 3);
   const int slice = MODE == TOKEN_GRAD ? t0 / (tm * tn) : 0, t = t0 - slice * tm * tn;
   const int band = t / (8 * tn), rows = tm - band * 8 < 8 ? tm - band * 8 : 8, w8 = t - band * 8 * tn;
   const int cs = w8 / (rows * 4), cols = tn - cs * 4 < 4 ? tn - cs * 4 : 4, w2 = w8 - cs * rows * 4;
-  const int m0 = (band * 8 + w2 / cols) * BM, n0 = (cs * 4 + w2 % cols) * BN;
+  const int m0 = (band * 8 + w2 / cols) * BM, n0 = (cs * 4 + w2 % cols) * BNC;
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = w / WGN, wn = w % WGN, lr = lane & 31, lk = lane >> 5;
@@ -115,11 +127,18 @@ __global__ void __launch_bounds__(WGM * WGN * 64) token_gemm_kernel(const TokenG
     const int r = slot >> 2, c = (slot & 3) ^ ((r >> 2) & 3), row = e0 + r < lim ? e0 + r : lim - 1;
     return (unsigned)(row * ld) * 2u + (unsigned)c * 16u;
   };
+  // (TWO: the first half of a wave's columns holds f(X)'s leading term, the second half,
+  // the same columns, what is left of it)
+  auto source_two = [&](int q) -> unsigned {
+    const int slot = (q * NW + w) * 64 + lane, r = slot >> 2, c = (slot & 3) ^ ((r >> 2) & 3);
+    const int of = r / WTN, at = r % WTN, n = n0 + of * (WTN / 2) + at % (WTN / 2);
+    return (at >= WTN / 2 ? p.b_term : 0u) + (unsigned)((n < N ? n : N - 1) * p.ldb) * 2u + (unsigned)c * 16u;
+  };
   unsigned oa[IA], ob[IB];
 #pragma unroll
   for (int q = 0; q < IA; ++q) oa[q] = source(MN, q, BM, m0, M, p.lda);
 #pragma unroll
-  for (int q = 0; q < IB; ++q) ob[q] = source(false, q, BN, n0, N, p.ldb);
+  for (int q = 0; q < IB; ++q) ob[q] = TWO ? source_two(q) : source(false, q, BN, n0, N, p.ldb);
   const unsigned step_a = MN ? (unsigned)p.lda * 64u : 64u;  // of a stage
   // load q of a stage: uniform offsets sa, sb
   auto load = [&](int q, unsigned char* st, unsigned sa, unsigned sb) {
@@ -231,57 +250,109 @@ __global__ void __launch_bounds__(WGM * WGN * 64) token_gemm_kernel(const TokenG
   }
   wait_loads<0>();  // no load may land in the epilogue's LDS
 
-  if constexpr (MODE == TOKEN_STATS) {
-    __syncthreads();
-    float2* red = reinterpret_cast<float2*>(smem);  // [WGM][BN]
+  // Block column j of the accumulators, columns n across the lanes, as rows n of a matrix with
+  // v along its rows, through this wave's part of the LDS.  FORM 0: errors in the operand
+  // type (fp32: three terms); 1: exponentials in fp16 times 2^15; 2: in fp32.  Rows and
+  // columns past the ends, up to the matrix's own, hold what the accumulators do there.
+  auto store_columns = [&](auto form, int j) {
+    constexpr int FORM = decltype(form)::value;
+    typedef typename std::conditional<FORM == 2, float, unsigned short>::type U;
+    constexpr int LD = WTM + (FORM == 2 ? 4 : 8), TERMS = FORM == 0 && SPLIT ? 3 : 1, PER = 16 / sizeof(U);
+    U* es = reinterpret_cast<U*>(smem) + w * 32 * LD;
+    U* out = static_cast<U*>(FORM == 0 ? p.out : p.kept);
 #pragma unroll
-    for (int j = 0; j < RN; ++j) {
-      const int c = wn * WTN + j * 32 + lr, n = n0 + c, mw = m0 + wm * WTM + 4 * lk;
-      const long long target = (n < N ? p.targets[n] : -1) - p.first;
-      float top = -__builtin_inff(), sum = 0.0f;
+    for (int term = 0; term < TERMS; ++term) {
 #pragma unroll
       for (int i = 0; i < RM; ++i)
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          const int m = mw + i * 32 + 8 * (q >> 2) + (q & 3);
-          if (m >= M) acc[i][j][q] = -__builtin_inff();
-          top = __builtin_fmaxf(top, acc[i][j][q]);
-          if (m == target && m < M) p.target_logit[n] = acc[i][j][q];
+        for (int q = 0; q < 16; q += 4) {
+          U h[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const float v = acc[i][j][q + u];
+            if constexpr (FORM == 0) {
+              const OT o = cvt<OT>(v);
+              h[u] = __builtin_bit_cast(unsigned short, o);
+              if (SPLIT) acc[i][j][q + u] = v - to_f32(o);  // exact; NaN stays
+            } else if constexpr (FORM == 1) {
+              h[u] = __builtin_bit_cast(unsigned short, cvt<f16>(v * 32768.0f));
+            } else {
+              h[u] = v;
+            }
+          }
+          typedef U U4 __attribute__((ext_vector_type(4)));
+          *reinterpret_cast<U4*>(es + lr * LD + i * 32 + 2 * q + 4 * lk) = U4{h[0], h[1], h[2], h[3]};
         }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      constexpr int LPR = WTM / PER, RPP = 64 / LPR, PASSES = 32 / RPP;  // lanes a row, rows a pass
+#pragma unroll
+      for (int u = 0; u < PASSES; ++u) {
+        const int r = u * RPP + lane / LPR, c = lane % LPR * PER;
+        const uint4 v = *reinterpret_cast<const uint4*>(es + r * LD + c);
+        const long long row = n0 + wn * WTN + j * 32 + r;
+        const int col = m0 + wm * WTM + c;
+        if (row < p.out_rows && col < p.out_ld) *reinterpret_cast<uint4*>(out + term * p.out_term + row * p.out_ld + col) = v;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+  };
+  if constexpr (TWO) {
+#pragma unroll
+    for (int i = 0; i < RM; ++i)
+#pragma unroll
+      for (int j = 0; j < RNC; ++j)
+#pragma unroll
+        for (int q = 0; q < 16; ++q)  // (an infinite weight times the rest of f(X), of either sign, is no matter)
+          acc[i][j][q] += __builtin_isinf(acc[i][j][q]) ? 0.0f : acc[i][j + RNC][q];
+  }
+  if constexpr (MODE == TOKEN_STATS || MODE == TOKEN_KEEP) {
+    if constexpr (MODE == TOKEN_KEEP) __syncthreads();
+    const int mw = m0 + wm * WTM;
+#pragma unroll
+    for (int j = 0; j < RNC; ++j) {
+      const int n = n0 + wn * WTN / (TWO ? 2 : 1) + j * 32 + lr;
+      if (m0 + BM > M) {
+#pragma unroll
+        for (int i = 0; i < RM; ++i)
+#pragma unroll
+          for (int q = 0; q < 16; ++q)
+            if (mw + i * 32 + 8 * (q >> 2) + 4 * lk + (q & 3) >= M) acc[i][j][q] = -__builtin_inff();
+      }
+      const long long to = (n < N ? p.targets[n] : -1) - p.first - mw;
+      const int target = to >= 0 && to < WTM && to < M - mw ? (int)to - 4 * lk : -1;
+      if (__any(target >= 0)) {
+#pragma unroll
+        for (int i = 0; i < RM; ++i)
+#pragma unroll
+          for (int q = 0; q < 16; ++q)
+            if (target == i * 32 + 8 * (q >> 2) + (q & 3)) p.target_logit[n] = acc[i][j][q];
+      }
+      float top = acc[0][j][0], sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < RM; ++i)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) top = __builtin_fmaxf(top, acc[i][j][q]);
       top = __builtin_fmaxf(top, __shfl_xor(top, 32));
       const float from = top == -__builtin_inff() ? 0.0f : top;  // (a column of -inf: no sum, and no NaN)
 #pragma unroll
       for (int i = 0; i < RM; ++i)
 #pragma unroll
-        for (int q = 0; q < 16; ++q) sum += exp_of<SPLIT>(acc[i][j][q] - from);
+        for (int q = 0; q < 16; ++q) {
+          acc[i][j][q] = exp_of<SPLIT>(acc[i][j][q] - from);
+          sum += acc[i][j][q];
+        }
       sum += __shfl_xor(sum, 32);
-      if (lk == 0) red[wm * BN + c] = make_float2(top, sum);
-    }
-    __syncthreads();
-    for (int c = tid; c < BN; c += NW * 64) {
-      if (n0 + c >= N) continue;
-      float2 v[WGM];
-      float top = -__builtin_inff(), sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < WGM; ++i) {
-        v[i] = red[i * BN + c];
-        top = __builtin_fmaxf(top, v[i].x);
-      }
-#pragma unroll
-      for (int i = 0; i < WGM; ++i) sum += v[i].x == -__builtin_inff() ? v[i].y : v[i].y * exp_of<SPLIT>(v[i].x - top);
-      static_cast<float2*>(p.out)[(long long)(m0 / BM) * N + n0 + c] = make_float2(top, sum);
+      if (lk == 0 && n < N && mw < M) static_cast<float2*>(p.out)[(long long)(mw / WTM) * N + n] = make_float2(top, sum);
+      if constexpr (MODE == TOKEN_KEEP) store_columns(std::integral_constant<int, SPLIT ? 2 : 1>{}, j);
     }
   } else if constexpr (MODE == TOKEN_ERROR) {
     __syncthreads();
-    constexpr int LD = WTM + 8, TERMS = SPLIT ? 3 : 1;  // (LDS rows of 2 WTM + 16 bytes)
-    unsigned short* es = reinterpret_cast<unsigned short*>(smem) + w * 32 * LD;
-    unsigned short* out = static_cast<unsigned short*>(p.out);
 #pragma unroll
     for (int j = 0; j < RN; ++j) {
       const int n = n0 + wn * WTN + j * 32 + lr, mw = m0 + wm * WTM + 4 * lk;
       const long long id = n < N ? p.targets[n] : -1;
       const bool real = id >= 0 && id < p.V;
-      const long long target = id - p.first;
+      const int target = real && id - p.first < M ? (int)(id - p.first) : -1;
       const float2 st = real ? p.stats[n] : make_float2(0.0f, 0.0f);
 #pragma unroll
       for (int i = 0; i < RM; ++i)
@@ -291,36 +362,7 @@ __global__ void __launch_bounds__(WGM * WGN * 64) token_gemm_kernel(const TokenG
           const float e = (m == target ? 1.0f : 0.0f) - exp_of<SPLIT>(acc[i][j][q] - st.x) * st.y;
           acc[i][j][q] = real && m < M ? e * p.scal : 0.0f;
         }
-#pragma unroll
-      for (int term = 0; term < TERMS; ++term) {
-#pragma unroll
-        for (int i = 0; i < RM; ++i)
-#pragma unroll
-          for (int q = 0; q < 16; q += 4) {
-            unsigned short h[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const OT o = cvt<OT>(acc[i][j][q + u]);
-              h[u] = __builtin_bit_cast(unsigned short, o);
-              if (SPLIT) acc[i][j][q + u] -= to_f32(o);  // exact; NaN stays
-            }
-            *reinterpret_cast<uint2*>(es + lr * LD + i * 32 + 2 * q + 4 * lk) =
-                make_uint2(h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16);
-          }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        constexpr int LPR = WTM / 8, PASSES = 32 / (64 / LPR);  // lanes a row of ET, passes over 32
-#pragma unroll
-        for (int u = 0; u < PASSES; ++u) {
-          const int r = u * (64 / LPR) + lane / LPR, c = lane % LPR * 8;
-          const uint4 v = *reinterpret_cast<const uint4*>(es + r * LD + c);
-          const long long row = n0 + wn * WTN + j * 32 + r;
-          const int col = m0 + wm * WTM + c;
-          // rows and columns past the ends, up to ET's own (multiples of 32), get zeros
-          if (row < p.out_rows && col < p.out_ld)
-            *reinterpret_cast<uint4*>(out + term * p.out_term + row * p.out_ld + col) = v;
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      }
+      store_columns(std::integral_constant<int, 0>{}, j);
     }
   } else {
     typedef typename std::conditional<MODE == TOKEN_GRAD || SPLIT, float, OT>::type ST;
@@ -335,16 +377,19 @@ __global__ void __launch_bounds__(WGM * WGN * 64) token_gemm_kernel(const TokenG
   }
 }
 
-template <typename OT, bool SPLIT, int MODE, int BM, int BN, int WGM, int WGN>
+template <typename OT, bool SPLIT, int MODE, bool TWO, int BM, int BN, int WGM, int WGN>
 hipError_t run_tile(const TokenGemm& p, hipStream_t s) {
   constexpr int NW = WGM * WGN, ring = STAGES * (BM + BN) * 64;
-  constexpr int epi = MODE == TOKEN_STATS ? WGM * BN * 8 : MODE == TOKEN_ERROR ? NW * 32 * (BM / WGM + 8) * 2 : NW * 32 * (BN / WGN + 4) * 4;
+  constexpr int epi = MODE == TOKEN_STATS ? 0
+                      : MODE == TOKEN_ERROR || (MODE == TOKEN_KEEP && !SPLIT) ? NW * 32 * (BM / WGM + 8) * 2
+                      : MODE == TOKEN_KEEP ? NW * 32 * (BM / WGM + 4) * 4 : NW * 32 * (BN / WGN + 4) * 4;
   constexpr int smem = epi > ring ? epi : ring;
   static_assert(smem <= 160 * 1024, "LDS");
-  const void* fn = reinterpret_cast<const void*>(&token_gemm_kernel<OT, SPLIT, MODE, BM, BN, WGM, WGN>);
-  const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const void* fn = reinterpret_cast<const void*>(&token_gemm_kernel<OT, SPLIT, MODE, TWO, BM, BN, WGM, WGN>);
+  static const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != hipSuccess) return e;
-  const long long tiles = ((p.M + BM - 1LL) / BM) * ((p.N + BN - 1LL) / BN) * (MODE == TOKEN_GRAD ? p.slices : 1);
+  constexpr int BNC = TWO ? BN / 2 : BN;
+  const long long tiles = ((p.M + BM - 1LL) / BM) * ((p.N + BNC - 1LL) / BNC) * (MODE == TOKEN_GRAD ? p.slices : 1);
   TokenGemm q = p;
   void* args[] = {&q};
   return hipLaunchKernel(fn, dim3((unsigned)tiles), dim3(NW * 64), args, smem, s);

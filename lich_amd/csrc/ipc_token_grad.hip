@@ -6,10 +6,10 @@ namespace {
 
 template <typename OT, bool SPLIT>
 hipError_t grad(const TokenGemm& p, int tile, hipStream_t s) {
-  if (tile == 256) return token::run_tile<OT, SPLIT, TOKEN_GRAD, 256, 256, 2, 2>(p, s);
-  if (tile == 128 && p.N > 64) return token::run_tile<OT, SPLIT, TOKEN_GRAD, 128, 128, 2, 2>(p, s);
-  if (tile == 128) return token::run_tile<OT, SPLIT, TOKEN_GRAD, 128, 64, 2, 2>(p, s);
-  return token::run_tile<OT, SPLIT, TOKEN_GRAD, 64, 64, 2, 2>(p, s);
+  if (tile == 256) return token::run_tile<OT, SPLIT, TOKEN_GRAD, false, 256, 256, 2, 2>(p, s);
+  if (tile == 128 && p.N > 64) return token::run_tile<OT, SPLIT, TOKEN_GRAD, false, 128, 128, 2, 2>(p, s);
+  if (tile == 128) return token::run_tile<OT, SPLIT, TOKEN_GRAD, false, 128, 64, 2, 2>(p, s);
+  return token::run_tile<OT, SPLIT, TOKEN_GRAD, false, 64, 64, 2, 2>(p, s);
 }
 
 }  // namespace

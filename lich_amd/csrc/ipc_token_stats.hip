@@ -4,24 +4,21 @@
 namespace ipc {
 namespace {
 
-template <int MODE, typename OT, bool SPLIT>
-hipError_t run(const TokenGemm& p, int bm, hipStream_t s) {
-  if (bm == 256) return token::run_tile<OT, SPLIT, MODE, 256, 256, 2, 2>(p, s);
-  if (bm == 128 && p.N > 64) return token::run_tile<OT, SPLIT, MODE, 128, 128, 2, 2>(p, s);
-  if (bm == 128) return token::run_tile<OT, SPLIT, MODE, 128, 64, 2, 2>(p, s);
-  return token::run_tile<OT, SPLIT, MODE, 64, 64, 2, 2>(p, s);
-}
-
-template <int MODE>
-hipError_t by_type(const TokenGemm& p, int storage, int bm, hipStream_t s) {
-  if (storage == 0) return run<MODE, bf16, true>(p, bm, s);
-  return storage == 1 ? run<MODE, f16, false>(p, bm, s) : run<MODE, bf16, false>(p, bm, s);
+template <typename OT, bool SPLIT, bool TWO>
+hipError_t run(const TokenGemm& p, int tile, hipStream_t s) {
+  constexpr int M = TWO ? 4 : 2, N = TWO ? 1 : 2;  // (two terms: both in one wave)
+  if (tile == TILE_256) return token::run_tile<OT, SPLIT, TOKEN_STATS, TWO, 256, 256, 2, 2>(p, s);
+  if (tile == TILE_128) return token::run_tile<OT, SPLIT, TOKEN_STATS, TWO, 128, 128, 2, 2>(p, s);
+  if (tile == TILE_128_64) return token::run_tile<OT, SPLIT, TOKEN_STATS, TWO, 128, 64, M, N>(p, s);
+  return token::run_tile<OT, SPLIT, TOKEN_STATS, TWO, 64, 64, 2, N>(p, s);
 }
 
 }  // namespace
 
-hipError_t launch_token_stats(const TokenGemm& p, int storage, int bm, hipStream_t s) {
-  return by_type<TOKEN_STATS>(p, storage, bm, s);
+hipError_t launch_token_stats(const TokenGemm& p, int storage, int tile, bool two, hipStream_t s) {
+  if (storage == 0) return run<bf16, true, false>(p, tile, s);
+  if (two) return storage == 1 ? run<f16, false, true>(p, tile, s) : run<bf16, false, true>(p, tile, s);
+  return storage == 1 ? run<f16, false, false>(p, tile, s) : run<bf16, false, false>(p, tile, s);
 }
 
 }  // namespace ipc
