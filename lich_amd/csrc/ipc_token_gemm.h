@@ -83,8 +83,8 @@ __device__ __forceinline__ float exp_of(float x) {
   return __builtin_amdgcn_exp2f(x * 1.44269504f);
 }
 
-template <typename OT, bool SPLIT, int MODE, bool TWO, int BM, int BN, int WGM, int WGN>
-__global__ void __launch_bounds__(WGM * WGN * 64) token_gemm_kernel(const TokenGemm p) {
+template <typename OT, bool SPLIT, int MODE, bool TWO, int BM, int BN, int WGM, int WGN, int ST, int PER_CU>
+__global__ void __launch_bounds__(WGM * WGN * 64, WGM * WGN / 4 * PER_CU) token_gemm_kernel(const TokenGemm p) {
   extern __shared__ __align__(16) unsigned char smem[];
   using MF = Mfma32<OT>;
   typedef typename MF::operand V;
@@ -191,15 +191,14 @@ __global__ void __launch_bounds__(WGM * WGN * 64) token_gemm_kernel(const TokenG
     else return straight(st, wm * WTM + i * 32, s);
   };
   auto read_b = [&](const unsigned char* st, int j, int s) -> V { return straight(st + A_BYTES, wn * WTN + j * 32, s); };
-  auto stage = [&](int kt) -> unsigned char* { return smem + (kt & (STAGES - 1)) * STAGE; };
 
 #pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) {
+  for (int s = 0; s < ST - 1; ++s) {
     seek(s);
 #pragma unroll
-    for (int q = 0; q < LPS; ++q) load(q, stage(s), sa, sb);
+    for (int q = 0; q < LPS; ++q) load(q, smem + s * STAGE, sa, sb);
   }
-  wait_loads<2 * LPS>();
+  wait_loads<(ST - 2) * LPS>();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   if (!SPLIT && !MN && tail < 32) {
@@ -211,12 +210,12 @@ __global__ void __launch_bounds__(WGM * WGN * 64) token_gemm_kernel(const TokenG
     asm volatile("" ::: "memory");
   }
 #pragma unroll
-  for (int j = 0; j < RN; ++j) fb[0][j] = read_b(stage(0), j, 0);
+  for (int j = 0; j < RN; ++j) fb[0][j] = read_b(smem, j, 0);
 #pragma unroll
-  for (int i = 0; i < RM; ++i) fa[0][i] = read_a(stage(0), i, 0);
+  for (int i = 0; i < RM; ++i) fa[0][i] = read_a(smem, i, 0);
 
   // half a step: the products of set S; the fragments of the next 16 k (half S ^ 1 of
-  // `next`) and half of stage kt + 3's loads between them
+  // `next`) and half of a later stage's loads between them
   auto half = [&](auto SV, const unsigned char* next, unsigned char* fill) {
     constexpr int S = decltype(SV)::value, O = S ^ 1;
     constexpr int L0 = S == 0 ? 0 : (LPS + 1) / 2, L1 = S == 0 ? (LPS + 1) / 2 : LPS;
@@ -237,19 +236,34 @@ __global__ void __launch_bounds__(WGM * WGN * 64) token_gemm_kernel(const TokenG
       __builtin_amdgcn_sched_barrier(0);
     }
   };
+  int at = 0;  // place of stage kt
 #pragma unroll 1
   for (int kt = 0; kt < G; ++kt) {
-    // stage kt + 1 of this wave has landed (kt + 2 may be in flight), then everybody's;
-    // everybody is done with stage kt - 1, which kt + 3 takes
-    wait_loads<LPS>();
+    // stage kt + 1 of this wave has landed (later ones may be in flight), then everybody's;
+    // everybody is done with stage kt - 1, whose place the last one loaded takes
+    wait_loads<(ST - 3) * LPS>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    seek(kt + 3);
-    half(std::integral_constant<int, 0>{}, stage(kt), stage(kt + 3));
-    half(std::integral_constant<int, 1>{}, stage(kt + 1), stage(kt + 3));
+    seek(kt + ST - 1);
+    unsigned char* here = smem + at * STAGE;
+    unsigned char* fill = smem + (at == 0 ? ST - 1 : at - 1) * STAGE;
+    at = at + 1 == ST ? 0 : at + 1;
+    half(std::integral_constant<int, 0>{}, here, fill);
+    half(std::integral_constant<int, 1>{}, smem + at * STAGE, fill);
   }
   wait_loads<0>();  // no load may land in the epilogue's LDS
 
+  // Rows past the last.  (The limit is made anew each time: the compiler would keep a
+  // mask of every row, thousands of scalar registers.)
+  auto mask_rows = [&](int j, float with) {
+    int left = M - m0 - wm * WTM - 4 * lk;
+    asm("" : "+v"(left));
+#pragma unroll
+    for (int i = 0; i < RM; ++i)
+#pragma unroll
+      for (int q = 0; q < 16; ++q)
+        if (i * 32 + 8 * (q >> 2) + (q & 3) >= left) acc[i][j][q] = with;
+  };
   // Block column j of the accumulators, columns n across the lanes, as rows n of a matrix with
   // v along its rows, through this wave's part of the LDS.  FORM 0: errors in the operand
   // type (fp32: three terms); 1: exponentials in fp16 times 2^15; 2: in fp32.  Rows and
@@ -311,21 +325,18 @@ __global__ void __launch_bounds__(WGM * WGN * 64) token_gemm_kernel(const TokenG
 #pragma unroll
     for (int j = 0; j < RNC; ++j) {
       const int n = n0 + wn * WTN / (TWO ? 2 : 1) + j * 32 + lr;
-      if (m0 + BM > M) {
-#pragma unroll
-        for (int i = 0; i < RM; ++i)
-#pragma unroll
-          for (int q = 0; q < 16; ++q)
-            if (mw + i * 32 + 8 * (q >> 2) + 4 * lk + (q & 3) >= M) acc[i][j][q] = -__builtin_inff();
-      }
+      if (m0 + BM > M) mask_rows(j, -__builtin_inff());
+      // the target's place among this lane's rows of the column
       const long long to = (n < N ? p.targets[n] : -1) - p.first - mw;
-      const int target = to >= 0 && to < WTM && to < M - mw ? (int)to - 4 * lk : -1;
-      if (__any(target >= 0)) {
+      const int own = (int)to - 4 * lk;
+      const bool hit = to >= 0 && to < WTM && to < M - mw && (own & 4) == 0;
+      if (__any(hit)) {
+        float z = 0.0f;
 #pragma unroll
         for (int i = 0; i < RM; ++i)
 #pragma unroll
-          for (int q = 0; q < 16; ++q)
-            if (target == i * 32 + 8 * (q >> 2) + (q & 3)) p.target_logit[n] = acc[i][j][q];
+          for (int q = 0; q < 16; ++q) z = own == i * 32 + 8 * (q >> 2) + (q & 3) ? acc[i][j][q] : z;
+        if (hit) p.target_logit[n] = z;
       }
       float top = acc[0][j][0], sum = 0.0f;
 #pragma unroll
@@ -344,48 +355,55 @@ __global__ void __launch_bounds__(WGM * WGN * 64) token_gemm_kernel(const TokenG
       sum += __shfl_xor(sum, 32);
       if (lk == 0 && n < N && mw < M) static_cast<float2*>(p.out)[(long long)(mw / WTM) * N + n] = make_float2(top, sum);
       if constexpr (MODE == TOKEN_KEEP) store_columns(std::integral_constant<int, SPLIT ? 2 : 1>{}, j);
+      __builtin_amdgcn_sched_barrier(0);
     }
   } else if constexpr (MODE == TOKEN_ERROR) {
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < RN; ++j) {
-      const int n = n0 + wn * WTN + j * 32 + lr, mw = m0 + wm * WTM + 4 * lk;
-      const long long id = n < N ? p.targets[n] : -1;
+      const int n = n0 + wn * WTN + j * 32 + lr, mw = m0 + wm * WTM;
+      const long long id = n < N ? p.targets[n] : -1, to = id - p.first - mw;
       const bool real = id >= 0 && id < p.V;
-      const int target = real && id - p.first < M ? (int)(id - p.first) : -1;
+      const int own = (int)to - 4 * lk;
+      const bool hit = real && to >= 0 && to < WTM && (own & 4) == 0;
       const float2 st = real ? p.stats[n] : make_float2(0.0f, 0.0f);
+      const float share = -st.y * p.scal;
 #pragma unroll
       for (int i = 0; i < RM; ++i)
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          const int m = mw + i * 32 + 8 * (q >> 2) + (q & 3);
-          const float e = (m == target ? 1.0f : 0.0f) - exp_of<SPLIT>(acc[i][j][q] - st.x) * st.y;
-          acc[i][j][q] = real && m < M ? e * p.scal : 0.0f;
-        }
+        for (int q = 0; q < 16; ++q) acc[i][j][q] = real ? exp_of<SPLIT>(acc[i][j][q] - st.x) * share : 0.0f;
+      if (__any(hit)) {
+#pragma unroll
+        for (int i = 0; i < RM; ++i)
+#pragma unroll
+          for (int q = 0; q < 16; ++q) acc[i][j][q] += hit && own == i * 32 + 8 * (q >> 2) + (q & 3) ? p.scal : 0.0f;
+      }
+      if (m0 + BM > M) mask_rows(j, 0.0f);
       store_columns(std::integral_constant<int, 0>{}, j);
+      __builtin_amdgcn_sched_barrier(0);
     }
   } else {
-    typedef typename std::conditional<MODE == TOKEN_GRAD || SPLIT, float, OT>::type ST;
+    typedef typename std::conditional<MODE == TOKEN_GRAD || SPLIT, float, OT>::type TT;
     MxProblem e{};
     e.M = M; e.N = N; e.scal = MODE == TOKEN_GRAD ? 1.0f : p.scal;
     e.out = MODE == TOKEN_GRAD ? static_cast<float*>(p.out) + (long long)slice * M * N : p.out;
     float* es = reinterpret_cast<float*>(smem) + w * 32 * (WTN + 4);
     const int mw = m0 + wm * WTM, nw = n0 + wn * WTN;
-    if (MODE == TOKEN_GRAD && !p.add) tile_epilogue<ST, KIND_FWD, ACT_IDENTITY, true, RM, RN>(e, acc, es, mw, nw);
-    else if (MODE == TOKEN_GRAD || p.vec) tile_epilogue<ST, KIND_WEIGHT, ACT_IDENTITY, true, RM, RN>(e, acc, es, mw, nw);
-    else tile_epilogue<ST, KIND_WEIGHT, ACT_IDENTITY, false, RM, RN>(e, acc, es, mw, nw);
+    if (MODE == TOKEN_GRAD && !p.add) tile_epilogue<TT, KIND_FWD, ACT_IDENTITY, true, RM, RN>(e, acc, es, mw, nw);
+    else if (MODE == TOKEN_GRAD || p.vec) tile_epilogue<TT, KIND_WEIGHT, ACT_IDENTITY, true, RM, RN>(e, acc, es, mw, nw);
+    else tile_epilogue<TT, KIND_WEIGHT, ACT_IDENTITY, false, RM, RN>(e, acc, es, mw, nw);
   }
 }
 
-template <typename OT, bool SPLIT, int MODE, bool TWO, int BM, int BN, int WGM, int WGN>
+template <typename OT, bool SPLIT, int MODE, bool TWO, int BM, int BN, int WGM, int WGN, int ST = 4, int PER_CU = 1>
 hipError_t run_tile(const TokenGemm& p, hipStream_t s) {
-  constexpr int NW = WGM * WGN, ring = STAGES * (BM + BN) * 64;
+  constexpr int NW = WGM * WGN, ring = ST * (BM + BN) * 64;
   constexpr int epi = MODE == TOKEN_STATS ? 0
                       : MODE == TOKEN_ERROR || (MODE == TOKEN_KEEP && !SPLIT) ? NW * 32 * (BM / WGM + 8) * 2
                       : MODE == TOKEN_KEEP ? NW * 32 * (BM / WGM + 4) * 4 : NW * 32 * (BN / WGN + 4) * 4;
   constexpr int smem = epi > ring ? epi : ring;
   static_assert(smem <= 160 * 1024, "LDS");
-  const void* fn = reinterpret_cast<const void*>(&token_gemm_kernel<OT, SPLIT, MODE, TWO, BM, BN, WGM, WGN>);
+  const void* fn = reinterpret_cast<const void*>(&token_gemm_kernel<OT, SPLIT, MODE, TWO, BM, BN, WGM, WGN, ST, PER_CU>);
   static const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != hipSuccess) return e;
   constexpr int BNC = TWO ? BN / 2 : BN;

@@ -7,7 +7,7 @@ namespace {
 template <typename OT, bool SPLIT>
 hipError_t weight(const TokenGemm& p, hipStream_t s) {
   auto tiles = [&](long long e) { return ((p.M + e - 1) / e) * ((p.N + e - 1) / e); };
-  if (tiles(256) >= 160) return token::run_tile<OT, SPLIT, TOKEN_WEIGHT, false, 256, 256, 2, 2>(p, s);
+  if (tiles(256) >= 160) return token::run_tile<OT, SPLIT, TOKEN_WEIGHT, false, 256, 256, 2, 4>(p, s);
   if (tiles(128) > 128) return token::run_tile<OT, SPLIT, TOKEN_WEIGHT, false, 128, 128, 2, 2>(p, s);
   return token::run_tile<OT, SPLIT, TOKEN_WEIGHT, false, 64, 64, 2, 2>(p, s);
 }
