@@ -28,7 +28,7 @@ hipError_t launch_embedding(const EmbedProblem& p, int storage, hipStream_t s);
 
 // Places are sorted by id, ties in their order; their rows of G, transposed once, are then
 // summed in runs of EMBED_RUN places, and sums that cross a run's end joined in order.
-constexpr int EMBED_RUN = 32;
+constexpr int EMBED_RUN = 16;
 // From so many places on (below, one launch finds the places of an id itself).
 constexpr int EMBED_SORTED = 513;
 struct EmbedUpdate {

@@ -127,53 +127,62 @@ __global__ void __launch_bounds__(256) embed_few_kernel(const EmbedUpdate p) {
 
 // Workgroups 0 .. ranges - 1: each owns a range of ids, reads all places in order twice and
 // writes its own, sorted, behind those of smaller ids (which it counts on the way, so
-// that no workgroup waits for another).  Each of the eight waves has an eighth of the
-// places, so that an id's places keep their order.  The other workgroups transpose G.
-constexpr int SORT_WAVES = 8;
+// that no workgroup waits for another).  Each of the sixteen waves has a sixteenth of the
+// places, so that an id's places keep their order; up to 8192 places stay in its registers
+// between the two readings.  The other workgroups transpose G.
+constexpr int SORT_WAVES = 16, SORT_HELD = 8;
 
 inline int sort_range(int V) {
   const int r = (V / 256 + 64) / 64 * 64;
-  return r > 1024 ? 1024 : r;
+  return r > 512 ? 512 : r;
 }
 
+// A block of G, 64 features by TURN samples, so that each thread has several loads in flight.
+template <typename ST> constexpr int TURN = sizeof(ST) == 4 ? 128 : 256;
 template <typename ST>
 __device__ void transpose_rows(const EmbedUpdate& p, int block, ST* tile) {
-  constexpr int LD = 66;
-  const int tiles_d = (p.D + 63) / 64, tiles_b = (p.B + 63) / 64;
+  constexpr int W = TURN<ST>, LD = W + 2, EACH = 64 * W / 4 / (SORT_WAVES * 64);
+  const int tiles_d = (p.D + 63) / 64, tiles_b = (p.B + W - 1) / W;
   const int td = block % tiles_d, tb = block / tiles_d % tiles_b, c = block / tiles_d / tiles_b;
-  const int d0 = td * 64, b0 = tb * 64;
+  const int d0 = td * 64, b0 = tb * W;
   const ST* g = static_cast<const ST*>(p.g);
   ST* rows = static_cast<ST*>(p.rows);
-  for (int u = threadIdx.x; u < 1024; u += SORT_WAVES * 64) {
-    const int d = u >> 4, b = (u & 15) * 4;
+  ST v[EACH][4];
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int u = e * SORT_WAVES * 64 + threadIdx.x, d = u / (W / 4), b = u % (W / 4) * 4;
     if (d0 + d >= p.D || b0 + b >= p.B) continue;
     const ST* from = g + ((long long)c * p.D + d0 + d) * p.B + b0 + b;
-    ST v[4];
     if (p.vec_b) {
       const Four<ST> f = *reinterpret_cast<const Four<ST>*>(__builtin_assume_aligned(from, 4 * sizeof(ST)));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = f.v[i];
+      for (int i = 0; i < 4; ++i) v[e][i] = f.v[i];
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = b0 + b + i < p.B ? from[i] : cvt<ST>(0.0f);
+      for (int i = 0; i < 4; ++i) v[e][i] = b0 + b + i < p.B ? from[i] : cvt<ST>(0.0f);
     }
+  }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) tile[d * LD + b + i] = v[i];
+  for (int e = 0; e < EACH; ++e) {
+    const int u = e * SORT_WAVES * 64 + threadIdx.x, d = u / (W / 4), b = u % (W / 4) * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) tile[d * LD + b + i] = v[e][i];
   }
   __syncthreads();
-  for (int u = threadIdx.x; u < 1024; u += SORT_WAVES * 64) {
-    const int b = u >> 4, d = (u & 15) * 4;
-    if (b0 + b >= p.B || d0 + d >= p.D) continue;
-    ST v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = tile[(d + i) * LD + b];
+  for (int e = 0; e < EACH; ++e) {
+    const int u = e * SORT_WAVES * 64 + threadIdx.x, b = u >> 4, d = (u & 15) * 4;
+    if (b0 + b >= p.B || d0 + d >= p.D) continue;
+    ST o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = tile[(d + i) * LD + b];
     ST* to = rows + ((long long)c * p.B + b0 + b) * p.D + d0 + d;
     if (p.D % 4 == 0) {  // (rows starts on 256 bytes)
-      store4(to, v);
+      store4(to, o);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (d0 + d + i < p.D) to[i] = v[i];
+        if (d0 + d + i < p.D) to[i] = o[i];
     }
   }
 }
@@ -195,12 +204,26 @@ __global__ void __launch_bounds__(SORT_WAVES * 64) embed_sort_kernel(const Embed
   for (int i = tid; i < SORT_WAVES * range; i += SORT_WAVES * 64) lds[i] = 0;
   __syncthreads();
   int less = 0;
-#pragma unroll 4
-  for (int i = first + lane; i < last; i += 64) {
-    const long long id = p.ids[i];
-    less += id >= 0 && id < lo;
-    if (id >= lo && id < hi) atomicAdd(&mine[id - lo], 1);  // (a count: the order does not matter)
-  }
+  // 64 SORT_HELD places from i0 on: ids relative to the range, -1 below it or padded, `range` or more above
+  unsigned held[SORT_HELD];
+  auto fetch = [&](int i0, bool count) {
+    long long id[SORT_HELD];
+#pragma unroll
+    for (int u = 0; u < SORT_HELD; ++u) {
+      const int i = i0 + u * 64 + lane;
+      id[u] = i < last ? p.ids[i] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < SORT_HELD; ++u) {
+      const bool in = id[u] >= lo && id[u] < hi;
+      held[u] = in ? (unsigned)(id[u] - lo) : ~0u;
+      if (count) {
+        less += id[u] >= 0 && id[u] < lo;
+        if (in) atomicAdd(&mine[held[u]], 1);  // (a count: the order does not matter)
+      }
+    }
+  };
+  for (int i0 = first; i0 < last; i0 += 64 * SORT_HELD) fetch(i0, true);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) less += __shfl_xor(less, o);
   if (lane == 0) before[wave] = less;
@@ -237,24 +260,26 @@ __global__ void __launch_bounds__(SORT_WAVES * 64) embed_sort_kernel(const Embed
   }
   if (blockIdx.x == ranges - 1)  // behind the last place with an id
     for (int i = base + tid; i <= N; i += SORT_WAVES * 64) p.key[i] = -1;
-  for (int i0 = first; i0 < last; i0 += 64) {
-    const int i = i0 + lane;
-    const long long id = i < last ? p.ids[i] : -1;
-    const bool in = id >= lo && id < hi;
-    const int own = in ? (int)(id - lo) : -1;
-    unsigned long long left = __ballot(in);
-    while (left) {  // one id after the other, its places in lane order
-      const int which = __shfl(own, __ffsll((unsigned long long)left) - 1);
-      const unsigned long long same = __ballot(own == which);
-      if (own == which) {
-        const int at = mine[which] + __popcll(same & ((1ull << lane) - 1));
-        p.order[at] = i;
-        p.key[at] = (int)id;
+  for (int i0 = first; i0 < last; i0 += 64 * SORT_HELD) {
+    if (last - first > 64 * SORT_HELD) fetch(i0, false);
+#pragma unroll
+    for (int u = 0; u < SORT_HELD; ++u) {
+      const unsigned own = held[u];
+      unsigned long long left = __ballot(own != ~0u);
+      while (left) {  // one id after the other, its places in lane order
+        const unsigned which = __builtin_amdgcn_readlane(own, __ffsll((unsigned long long)left) - 1);
+        const unsigned long long same = __ballot(own == which);
+        const int at = mine[which];
+        if (own == which) {
+          const int to = at + __popcll(same & ((1ull << lane) - 1));
+          p.order[to] = i0 + u * 64 + lane;
+          p.key[to] = (int)(lo + which);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (lane == 0) mine[which] = at + __popcll(same);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        left &= ~same;
       }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      if (lane == __ffsll(same) - 1) mine[which] += __popcll(same);
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      left &= ~same;
     }
   }
 }
@@ -262,63 +287,71 @@ __global__ void __launch_bounds__(SORT_WAVES * 64) embed_sort_kernel(const Embed
 // A run of EMBED_RUN sorted places, 4 features a thread.  Ids that begin and end in the
 // run are finished here; a sum that came over the run's start goes to part[run][0], one
 // that goes on past its end to part[run][1].
+// (values as they lie: widened when used, so that many rows can be in flight)
 template <typename ST>
-__device__ __forceinline__ void add_to_table(const EmbedUpdate& p, int id, int d, const float (&sum)[4]) {
-  ST* t = static_cast<ST*>(p.table) + (long long)id * p.D + d;
-  if (p.vec_d) {
-    float old[4];
-    ST o[4];
-    load4(t, old);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = cvt<ST>(old[i] + p.alpha * sum[i]);
-    store4(t, o);
+__device__ __forceinline__ void get_row(const ST* from, int left, bool whole, Four<ST>& v) {
+  if (whole) {
+    v = *reinterpret_cast<const Four<ST>*>(__builtin_assume_aligned(from, 4 * sizeof(ST)));
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (d + i < p.D) t[i] = cvt<ST>(to_f32(t[i]) + p.alpha * sum[i]);
+    for (int q = 0; q < 4; ++q) v.v[q] = q < left ? from[q] : cvt<ST>(0.0f);
   }
+}
+template <typename ST>
+__device__ __forceinline__ void put_row(ST* to, int left, bool whole, const float (&v)[4]) {
+  ST o[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) o[q] = cvt<ST>(v[q]);
+  if (whole) {
+    store4(to, o);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q < left) to[q] = o[q];
+  }
+}
+template <typename ST>
+__device__ __forceinline__ void add_to_row(ST* to, int left, bool whole, const Four<ST>& old, float alpha, const float (&sum)[4]) {
+  float v[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) v[q] = to_f32(old.v[q]) + alpha * sum[q];
+  put_row(to, left, whole, v);
 }
 
 template <typename ST>
 __global__ void __launch_bounds__(256) embed_run_kernel(const EmbedUpdate p) {
-  const int slabs = gridDim.y, run = blockIdx.x, N = p.C * p.B;
-  const int d = (blockIdx.y * blockDim.x + threadIdx.x) * 4;
-  const int first = run * EMBED_RUN, last = first + EMBED_RUN < N ? first + EMBED_RUN : N;
-  (void)slabs;
-  if (p.key[first] < 0 || d >= p.D) return;
+  const int run = blockIdx.x, N = p.C * p.B, lane = threadIdx.x & 63;
+  const int d = (blockIdx.y * blockDim.x + threadIdx.x) * 4, first = run * EMBED_RUN;
+  // lane i: the id of the place before the run's i-th, and the i-th's row of G
+  const int at = first - 1 + lane;
+  const int keys = at >= 0 && at <= N ? p.key[at] : -1;
+  const int orders = lane < EMBED_RUN && first + lane < N ? p.order[first + lane] : 0;
+  auto key = [&](int i) { return __builtin_amdgcn_readlane(keys, i + 1); };
+  if (key(0) < 0 || d >= p.D) return;
   const ST* rows = static_cast<const ST*>(p.rows);
-  const bool whole = p.D % 4 == 0;
-  int id = p.key[first];
-  bool over = first > 0 && p.key[first - 1] == id;  // came over the start
+  ST* table = static_cast<ST*>(p.table);
+  const bool whole = p.D % 4 == 0, vec = p.vec_d != 0;  // (rows and part start on 256 bytes)
+  const int left = p.D - d;
+  // every row of G and of the table, none stored before all are read (a place without an id: any row)
+  Four<ST> v[EMBED_RUN], old[EMBED_RUN];
+#pragma unroll
+  for (int u = 0; u < EMBED_RUN; ++u) {
+    const int id = key(u);
+    get_row(rows + (long long)(id < 0 ? 0 : __builtin_amdgcn_readlane(orders, u)) * p.D + d, left, whole, v[u]);
+    get_row(table + (long long)(id < 0 ? 0 : id) * p.D + d, left, vec, old[u]);
+  }
+  bool over = key(-1) == key(0);  // its sum came over the start
   float sum[4] = {};
-  for (int i = first; i < last;) {
-    const int n = p.order[i];
-    const ST* from = rows + (long long)n * p.D + d;
-    float v[4] = {};
-    if (whole) {
-      load4(from, v);
-    } else {
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (d + q < p.D) v[q] = to_f32(from[q]);
-    }
+  for (int u = 0; u < EMBED_RUN; ++u) {
+    const int id = key(u);
+    if (id < 0) return;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) sum[q] += v[q];
-    ++i;
-    const int next = p.key[i];
-    if (i < last && next == id) continue;
-    // the id's last place in this run
-    const bool on = next == id;
-    if (over || on) {
-      float* to = p.part + ((long long)run * 2 + (over ? 0 : 1)) * p.D + d;
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (d + q < p.D) to[q] = sum[q];
-    } else {
-      add_to_table<ST>(p, id, d, sum);
-    }
-    if (next < 0 || i >= last) break;
-    id = next;
+    for (int q = 0; q < 4; ++q) sum[q] += to_f32(v[u].v[q]);
+    const bool on = key(u + 1) == id;
+    if (on && u + 1 < EMBED_RUN) continue;
+    if (over || on) put_row(p.part + ((long long)run * 2 + (over ? 0 : 1)) * p.D + d, left, whole, sum);  // the run's first and ended, or its last and not
+    else add_to_row(table + (long long)id * p.D + d, left, vec, old[u], p.alpha, sum);
     over = false;
 #pragma unroll
     for (int q = 0; q < 4; ++q) sum[q] = 0.0f;
@@ -329,21 +362,35 @@ __global__ void __launch_bounds__(256) embed_run_kernel(const EmbedUpdate p) {
 template <typename ST>
 __global__ void __launch_bounds__(256) embed_join_kernel(const EmbedUpdate p) {
   const int run = blockIdx.x, N = p.C * p.B, runs = (N + EMBED_RUN - 1) / EMBED_RUN;
-  const int d = (blockIdx.y * blockDim.x + threadIdx.x) * 4;
+  const int d = (blockIdx.y * blockDim.x + threadIdx.x) * 4, lane = threadIdx.x & 63;
   const int first = run * EMBED_RUN, end = first + EMBED_RUN;
-  if (end >= N || d >= p.D) return;
+  if (end >= N) return;
   const int id = p.key[end - 1];
   if (id < 0 || p.key[end] != id) return;
-  if (p.key[first] == id && first > 0 && p.key[first - 1] == id) return;  // it began earlier
-  float sum[4] = {};
-  for (int r = run, slot = 1; r < runs; ++r, slot = 0) {
-    if (slot == 0 && p.key[r * EMBED_RUN] != id) break;
-    const float* from = p.part + ((long long)r * 2 + slot) * p.D + d;
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (d + q < p.D) sum[q] += from[q];
+  if (first > 0 && p.key[first] == id && p.key[first - 1] == id) return;  // it began earlier
+  int more = 0;  // runs it goes on into
+  for (int r = run + 1;; r += 64) {
+    const unsigned long long other = __ballot(r + lane >= runs || p.key[(long long)(r + lane < runs ? r + lane : 0) * EMBED_RUN] != id);
+    more += other ? __ffsll(other) - 1 : 64;
+    if (other) break;
   }
-  add_to_table<ST>(p, id, d, sum);
+  if (d >= p.D) return;
+  const int left = p.D - d;
+  const bool whole = p.D % 4 == 0;
+  ST* row = static_cast<ST*>(p.table) + (long long)id * p.D + d;
+  float sum[4] = {};
+  Four<ST> old;
+  get_row(row, left, p.vec_d != 0, old);
+  const float* from = p.part + ((long long)run * 2 + 1) * p.D + d;
+#pragma unroll 8
+  for (int r = 0; r <= more; ++r) {
+    // (its own second sum, then the later runs' first ones: 1, 3, 5, ... rows on)
+    Four<float> v;
+    get_row(from + (r == 0 ? 0 : 2 * r - 1) * (long long)p.D, left, whole, v);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) sum[q] += v.v[q];
+  }
+  add_to_row(row, left, p.vec_d != 0, old, p.alpha, sum);
 }
 
 template <typename ST>
@@ -366,8 +413,8 @@ hipError_t run_update(const EmbedUpdate& p, hipStream_t s) {
     return hipGetLastError();
   }
   const int range = sort_range(p.V), ranges = (int)(((long long)p.V + range - 1) / range);
-  const long long turns = (long long)p.C * ((p.B + 63) / 64) * ((p.D + 63) / 64);
-  const int turn_lds = 64 * 66 * (int)sizeof(ST), sort_lds = SORT_WAVES * range * 4;
+  const long long turns = (long long)p.C * ((p.B + TURN<ST> - 1) / TURN<ST>) * ((p.D + 63) / 64);
+  const int turn_lds = 64 * (TURN<ST> + 2) * (int)sizeof(ST), sort_lds = SORT_WAVES * range * 4;
   hipLaunchKernelGGL((embed_sort_kernel<ST>), dim3((unsigned)(ranges + turns)), dim3(SORT_WAVES * 64),
                      turn_lds > sort_lds ? turn_lds : sort_lds, s, p, ranges, range);
   hipError_t e = hipGetLastError();
