@@ -9,9 +9,11 @@
     python -m lich_amd.cli steady-state [--dims 784 64 64 10] [...]
     python -m lich_amd.cli toolchain
     python -m lich_amd.cli compact [--synthetic 4096] [--hidden 64 --depth 2] [...]
+    python -m lich_amd.cli tokens [--text FILE [--words N] | --synthetic 20000] [...]
 
 ``compact`` (no counterpart in the reference) trains with 8-bit states and answers
-with 4-bit weights.  Each other subcommand takes the arguments of the reference script it replaces
+with 4-bit weights; ``tokens`` (nor this) does so on a text, predicting each token
+from those before it.  Each other subcommand takes the arguments of the reference script it replaces
 (``smoke.py``, ``validate_reference.py``, ``autotune.py``, ``train_mnist.py``,
 ``train_paper_efficiency.py``, ``thermal_bench.py``,
 ``benchmark_stage2_4_steady_state.py``, ``toolchain_probe.py``).  Differences:
@@ -417,6 +419,47 @@ def compact_main(argv=None) -> int:
     return 0
 
 
+# ------------------------------------------------------------------- tokens
+def tokens_main(argv=None) -> int:
+    """A net over the tokens of a text (``lich_amd.token_net``): training, then the losses of the
+    last batch and the tokens that its 4-bit weights predict."""
+    from . import token_net
+    from .data import load_tokens, synthetic_tokens
+
+    p = argparse.ArgumentParser(prog="lich_amd.cli tokens")
+    p.add_argument("--text", default=None, help="a text file; its bytes are the tokens")
+    p.add_argument("--words", type=int, default=0, help="tokens are the commonest N words instead")
+    p.add_argument("--synthetic", type=int, default=0, help="N seeded synthetic tokens instead of a file")
+    p.add_argument("--vocab", type=int, default=256, help="vocabulary of the synthetic tokens")
+    p.add_argument("--context", type=int, default=4)
+    p.add_argument("--width", type=int, default=32, help="features of a token")
+    p.add_argument("--hidden", type=int, default=64)
+    p.add_argument("--depth", type=int, default=1, help="number of hidden layers")
+    p.add_argument("--batch", type=int, default=128)
+    p.add_argument("--epochs", type=int, default=4)
+    p.add_argument("--rate", type=float, default=0.5)
+    p.add_argument("--dropout", type=float, default=0.0)
+    p.add_argument("--activation", default="tanh")
+    p.add_argument("--dtype", choices=["float16", "bfloat16", "float32"], default="float32")
+    p.add_argument("--seed", type=int, default=0)
+    a = p.parse_args(argv)
+    if (a.text is None) == (a.synthetic <= 0):
+        p.error("either --text FILE or --synthetic N")
+    dtype = {"float16": torch.float16, "bfloat16": torch.bfloat16, "float32": torch.float32}[a.dtype]
+    data = load_tokens(a.text, words=a.words) if a.text else synthetic_tokens(a.synthetic, vocab=a.vocab, seed=a.seed)
+    if len(data) < 1 or data.vocab < 1:
+        p.error("the text is empty")
+    dev = _device()
+    _, net = token_net.train(data, context=a.context, width=a.width, hidden=(a.hidden,) * a.depth, batch=a.batch,
+                             epochs=a.epochs, rate=a.rate, p=a.dropout, activation=a.activation, dtype=dtype, seed=a.seed)
+    ids, targets = (t.to(dev) for t in next(iter(data.batches(a.batch, a.context, shuffle=False))))
+    real = targets >= 0
+    loss = float(net.losses(ids, targets).sum()) / max(int(real.sum()), 1)
+    right = float(((net.predict(ids).float().argmax(0) == targets) & real).sum()) / max(int(real.sum()), 1)
+    print(f"first {int(real.sum())} places: loss={loss:.4f}, predicted with 4-bit weights {right:.4f}", flush=True)
+    return 0
+
+
 def _autotune(argv):
     from .autotune import main
     return main(argv)
@@ -429,7 +472,7 @@ def _train(argv):
 
 COMMANDS = {"smoke": smoke_main, "reference": reference_main, "autotune": _autotune, "train-mnist": _train,
             "efficiency": efficiency_main, "thermal-bench": thermal_main, "steady-state": steady_main,
-            "toolchain": toolchain_main, "compact": compact_main}
+            "toolchain": toolchain_main, "compact": compact_main, "tokens": tokens_main}
 
 
 def main(argv=None) -> int:

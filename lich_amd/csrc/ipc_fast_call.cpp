@@ -17,6 +17,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/DeviceGuard.h>
 #include <torch/csrc/Device.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
@@ -176,10 +177,14 @@ PyObject* call_run(PyObject* self, PyObject* const* argv, size_t nargsf, PyObjec
   Py_DECREF(refuse);
   if (PyErr_Occurred()) return nullptr;
   int rc;
+  HANDLE_TH_ERRORS
+  // (the stream's own device: the default stream's handle names none)
+  const c10::OptionalDeviceGuard guard(c10::Device(c10::kCUDA, device));
   Py_BEGIN_ALLOW_THREADS
   rc = k.enter(a);
   Py_END_ALLOW_THREADS
   return PyLong_FromLong(rc);
+  END_HANDLE_TH_ERRORS
 }
 
 PyObject* call_new(PyTypeObject* type, PyObject* args, PyObject*) {

@@ -11,6 +11,7 @@ with an asynchronous, double-buffered H2D pipeline is an open item of its
 * ``synthetic_dataset`` is a seeded, MNIST-shaped stand-in with a learnable
   class structure (one prototype image per class plus noise) for machines
   without the files;
+* ``TokenDataset`` gives contexts and targets of a text (``load_tokens``, ``synthetic_tokens``);
 * ``BatchStager`` copies batches into two pinned host slots, issues their
   H2D copies on a side stream and lays them out on the device as the
   ``[features, B]`` input and ``[classes, B]`` one-hot target, so batch i+1
@@ -144,6 +145,65 @@ def synthetic_dataset(n: int, *, seed: int = 0, num_classes: int = 10, shape: tu
     img = protos[labels] + noise * (rng.random((int(n),) + tuple(shape), dtype=np.float32) - 0.5)
     img = np.clip(np.rint(np.clip(img, 0.0, 1.0) * 255.0), 0, 255).astype(np.uint8)
     return ArrayDataset(img, labels, num_classes, f"synthetic(seed={seed})")
+
+
+@dataclass
+class TokenDataset:
+    """A text as int64 tokens ``[N]`` of a vocabulary; -1 where a word is not in it."""
+
+    tokens: np.ndarray
+    vocab: int
+    names: list | None = None
+
+    def __len__(self) -> int:
+        return int(len(self.tokens))
+
+    def batches(self, batch: int, context: int, *, shuffle: bool = True, seed: int = 0,
+                epoch: int = 0) -> Iterator[tuple[torch.Tensor, torch.Tensor]]:
+        """(ids ``[context, batch]``, targets ``[batch]``): the tokens before each place and the one at
+        it, in a seeded order per epoch; -1 before the text begins and for what the
+        last batch lacks."""
+        n, context = len(self), int(context)
+        text = np.concatenate([np.full(context, -1, dtype=np.int64), np.asarray(self.tokens, dtype=np.int64)])
+        order = np.random.default_rng([int(seed), int(epoch)]).permutation(n) if shuffle else np.arange(n)
+        for s in range(0, n, batch):
+            at = order[s:s + batch]
+            ids = np.full((context, batch), -1, dtype=np.int64)
+            targets = np.full(batch, -1, dtype=np.int64)
+            ids[:, :len(at)] = text[at[None, :] + np.arange(context)[:, None]]
+            targets[:len(at)] = text[at + context]
+            yield torch.from_numpy(ids), torch.from_numpy(targets)
+
+
+def load_tokens(path: str | Path, *, words: int = 0) -> TokenDataset:
+    """A text file's bytes as tokens, or with ``words`` its whitespace-separated words, the
+    commonest ``words`` of them numbered by falling count (others -1)."""
+    raw = Path(path).read_bytes()
+    if words <= 0:
+        return TokenDataset(np.frombuffer(raw, dtype=np.uint8).astype(np.int64), 256)
+    found = raw.decode("utf-8", "replace").split()
+    counts: dict[str, int] = {}
+    for w in found:
+        counts[w] = counts.get(w, 0) + 1
+    names = sorted(counts, key=lambda w: (-counts[w], w))[:int(words)]
+    number = {w: i for i, w in enumerate(names)}
+    return TokenDataset(np.array([number.get(w, -1) for w in found], dtype=np.int64), len(names), names)
+
+
+def synthetic_tokens(n: int, *, vocab: int = 256, seed: int = 0, noise: float = 0.2) -> TokenDataset:
+    """A seeded text with a structure to learn: each token is followed by one of its own, a fixed
+    permutation, except for a share of random ones whose frequency falls with their rank."""
+    rng = np.random.default_rng(int(seed))
+    follows = rng.permutation(vocab)
+    ranks = np.floor(np.exp(rng.random(n) * np.log(vocab + 1.0))).astype(np.int64) - 1
+    ranks = np.clip(ranks, 0, vocab - 1)
+    stray = rng.random(n) < noise
+    out = np.empty(n, dtype=np.int64)
+    last = 0
+    for i in range(n):
+        last = int(ranks[i]) if stray[i] else int(follows[last])
+        out[i] = last
+    return TokenDataset(out, vocab)
 
 
 class BatchStager:

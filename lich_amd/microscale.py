@@ -124,7 +124,8 @@ class _Operator:
             pointers += o(t) if isinstance(o, _Packed) else (_pointer(t, *o),)
         first = given[0] if isinstance(given[0], torch.Tensor) else given[0][0]
         lent = _Kernel._ws(workspace) if self._lends else ()
-        nat.check(self._entry(*pointers, *self._constants, *lent, nat.current_stream_handle(first.get_device())))
+        with torch.cuda.device(first.device):  # (the default stream's handle names no device)
+            nat.check(self._entry(*pointers, *self._constants, *lent, nat.current_stream_handle(first.get_device())))
 
 
 def _no_fast_call(*_) -> int:
