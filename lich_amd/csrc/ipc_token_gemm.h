@@ -15,8 +15,8 @@
 // copy of W and one of the errors serve both products they appear in.
 //
 // fp32 tensors: every operand is the sum of three bf16 terms (24 bits, the type's own), and a
-// product the six term products above 2^-24 of it, smallest first; 233 TFLOP/s at
-// six times the 16-bit work against 154 of the fp32 matrix instruction's peak use.
+// product the six term products above 2^-24 of it, smallest first, from one stage that holds
+// all terms.  Six times the 16-bit work, but the fp32 matrix instruction takes sixteen.
 //
 // The accumulators of the first two lie with a column n a lane (and rows v in its
 // registers), so that a column's maximum and sum are the lane's own business up to one
@@ -64,17 +64,31 @@ hipError_t launch_token_stats(const TokenGemm& p, int storage, int tile, bool tw
 hipError_t launch_token_keep(const TokenGemm& p, int storage, int tile, hipStream_t s);
 hipError_t launch_token_error(const TokenGemm& p, int storage, int tile, hipStream_t s);
 hipError_t launch_token_grad(const TokenGemm& p, int storage, int tile, hipStream_t s);
-hipError_t launch_token_weight(const TokenGemm& p, int storage, hipStream_t s);
+
+// The state's gradient from its slices, G = f'(X) sum, zeros in padded columns, and what
+// the loss is off by for f(X)'s rounding (fixes: [token_fix_rows][B], or nullptr).
+struct TokenFinish {
+  int D, B, V, slices, act;
+  const float* part;  // [slices][D][B]
+  const void* x;
+  const long long* targets;
+  void* g;
+  float scale;
+  float* fixes;
+  int vec;            // x and g allow 4-element accesses
+};
+inline int token_fix_rows(int D, bool vec) { return vec ? (D + 15) / 16 : (D + 3) / 4; }
+hipError_t launch_token_finish(const TokenFinish& p, int storage, hipStream_t s);
+// W's update, and (f) the gradient's last step, which needs no more than that does: in one
+// launch where both are small.
+hipError_t launch_token_weight(const TokenGemm& p, const TokenFinish* f, int storage, hipStream_t s);
 
 namespace token {
 
 using namespace mx;
 
-// a and b terms of product g of a contraction over three terms each, smallest first
-constexpr int PRODUCTS = 6;
-__device__ __forceinline__ unsigned term_of(unsigned packed, int g) { return (packed >> (2 * g)) & 3u; }
-constexpr unsigned TERMS_A = 2u | 1u << 2 | 0u << 4 | 1u << 6 | 0u << 8 | 0u << 10;
-constexpr unsigned TERMS_B = 0u | 1u << 2 | 2u << 4 | 0u << 6 | 1u << 8 | 0u << 10;
+// a and b terms of the products of three terms each, smallest first
+constexpr int PRODUCTS = 6, TERM_A[PRODUCTS] = {2, 1, 0, 1, 0, 0}, TERM_B[PRODUCTS] = {0, 1, 2, 0, 1, 0};
 
 template <bool EXACT>
 __device__ __forceinline__ float exp_of(float x) {
@@ -83,22 +97,22 @@ __device__ __forceinline__ float exp_of(float x) {
   return __builtin_amdgcn_exp2f(x * 1.44269504f);
 }
 
-template <typename OT, bool SPLIT, int MODE, bool TWO, int BM, int BN, int WGM, int WGN, int ST, int PER_CU>
-__global__ void __launch_bounds__(WGM * WGN * 64, WGM * WGN / 4 * PER_CU) token_gemm_kernel(const TokenGemm p) {
-  extern __shared__ __align__(16) unsigned char smem[];
+// Workgroup `block` of `blocks` of a product.
+template <typename OT, bool SPLIT, int MODE, bool TWO, int BM, int BN, int WGM, int WGN, int ST>
+__device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* smem, int block, int blocks) {
   using MF = Mfma32<OT>;
   typedef typename MF::operand V;
   constexpr bool MN = MODE == TOKEN_GRAD || MODE == TOKEN_WEIGHT, COLUMNS = !MN;
   constexpr int NW = WGM * WGN, WTM = BM / WGM, WTN = BN / WGN, RM = WTM / 32, RN = WTN / 32;
   constexpr int RNC = TWO ? RN / 2 : RN, BNC = TWO ? BN / 2 : BN;  // blocks and columns of different n
-  constexpr int A_BYTES = BM * 64, B_BYTES = BN * 64, STAGE = A_BYTES + B_BYTES;
+  constexpr int TERMS = SPLIT ? 3 : 1, A_BYTES = BM * 64, B_BYTES = BN * 64, STAGE = TERMS * (A_BYTES + B_BYTES);
   static_assert(!TWO || (MODE == TOKEN_STATS && RN % 2 == 0), "two terms of f(X)");
-  constexpr int IA = A_BYTES / 1024 / NW, IB = B_BYTES / 1024 / NW, LPS = IA + IB;  // LDS-DMA loads per wave and stage
+  constexpr int IA = A_BYTES / 1024 / NW, IB = B_BYTES / 1024 / NW, LPS = TERMS * (IA + IB);  // LDS-DMA loads per wave and stage
   static_assert(IA * 1024 * NW == A_BYTES && IB * 1024 * NW == B_BYTES, "tile / waves");
 
   // consecutive tiles per XCD, in supertiles of 8 x 4 (as in mx_tile_kernel); slices outermost
   const int tn = (p.N + BNC - 1) / BNC, tm = (p.M + BM - 1) / BM;
-  const int b = blockIdx.x, per = gridDim.x >> 3, rem = gridDim.x & 7, xcd = b & 7;
+  const int b = block, per = blocks >> 3, rem = blocks & 7, xcd = b & 7;
   const int t0 = xcd * per + (xcd < rem ? xcd : rem) + (b >> 3);
   const int slice = MODE == TOKEN_GRAD ? t0 / (tm * tn) : 0, t = t0 - slice * tm * tn;
   const int band = t / (8 * tn), rows = tm - band * 8 < 8 ? tm - band * 8 : 8, w8 = t - band * 8 * tn;
@@ -108,10 +122,9 @@ __global__ void __launch_bounds__(WGM * WGN * 64, WGM * WGN / 4 * PER_CU) token_
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = w / WGN, wn = w % WGN, lr = lane & 31, lk = lane >> 5;
   const int M = p.M, N = p.N, K = p.K, GS = (K + 31) / 32, tail = K - (GS - 1) * 32;
-  // stages of this workgroup: begin .. end - 1 of all products' one after the other
-  const int all = SPLIT ? PRODUCTS * GS : GS;
-  const int begin = MODE == TOKEN_GRAD ? (int)((long long)all * slice / p.slices) : 0;
-  const int end = MODE == TOKEN_GRAD ? (int)((long long)all * (slice + 1) / p.slices) : all;
+  // stages of this workgroup: begin .. end - 1
+  const int begin = MODE == TOKEN_GRAD ? (int)((long long)GS * slice / p.slices) : 0;
+  const int end = MODE == TOKEN_GRAD ? (int)((long long)GS * (slice + 1) / p.slices) : GS;
   const int G = end - begin;
 
   const Rsrc ga(p.a, (unsigned)p.a_bytes), gb(p.b, (unsigned)p.b_bytes);
@@ -140,12 +153,14 @@ __global__ void __launch_bounds__(WGM * WGN * 64, WGM * WGN / 4 * PER_CU) token_
 #pragma unroll
   for (int q = 0; q < IB; ++q) ob[q] = TWO ? source_two(q) : source(false, q, BN, n0, N, p.ldb);
   const unsigned step_a = MN ? (unsigned)p.lda * 64u : 64u;  // of a stage
-  // load q of a stage: uniform offsets sa, sb
+  // load q of a stage: uniform offsets sa, sb; the terms of A, then those of B
   auto load = [&](int q, unsigned char* st, unsigned sa, unsigned sb) {
-    unsigned char* at = q < IA ? st + (q * NW + w) * 1024 : st + A_BYTES + ((q - IA) * NW + w) * 1024;
-    const unsigned v = q < IA ? oa[q < IA ? q : 0] : ob[q < IA ? 0 : q - IA];
-    if constexpr (MN) to_lds16_unseen(q < IA ? wa : wb, at, v, q < IA ? sa : sb);
-    else (q < IA ? ga : gb).to_lds16(at, v, q < IA ? sa : sb);
+    const bool of_a = q < TERMS * IA;
+    const int r = of_a ? q : q - TERMS * IA, each = of_a ? IA : IB, term = r / each, i = r % each;
+    unsigned char* at = st + (of_a ? term * A_BYTES : TERMS * A_BYTES + term * B_BYTES) + (i * NW + w) * 1024;
+    const unsigned v = of_a ? oa[of_a ? i : 0] : ob[of_a ? 0 : i], o = of_a ? sa + term * p.a_term : sb + term * p.b_term;
+    if constexpr (MN) to_lds16_unseen(of_a ? wa : wb, at, v, o);
+    else (of_a ? ga : gb).to_lds16(at, v, o);
   };
   // uniform offsets of stage kt (past the end: of the last, so that every step counts the
   // same).  A k-contiguous A may end inside a stage: that one comes first, and what it has
@@ -153,15 +168,9 @@ __global__ void __launch_bounds__(WGM * WGN * 64, WGM * WGN / 4 * PER_CU) token_
   unsigned sa, sb;
   auto seek = [&](int kt) {
     const int g = begin + (kt < G ? kt : G - 1);
-    if constexpr (SPLIT) {
-      const int product = g / GS, k = g - product * GS;
-      sa = (unsigned)k * step_a + term_of(TERMS_A, product) * p.a_term;
-      sb = (unsigned)k * 64u + term_of(TERMS_B, product) * p.b_term;
-    } else {
-      const int k = MN ? g : g == 0 ? GS - 1 : g - 1;
-      sa = (unsigned)k * step_a;
-      sb = (unsigned)k * 64u;
-    }
+    const int k = MN || SPLIT ? g : g == 0 ? GS - 1 : g - 1;
+    sa = (unsigned)k * step_a;
+    sb = (unsigned)k * 64u;
   };
 
   f32x16 acc[RM][RN];
@@ -185,12 +194,19 @@ __global__ void __launch_bounds__(WGM * WGN * 64, WGM * WGN / 4 * PER_CU) token_
     const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p0 + 4 * rowb));
     return __builtin_bit_cast(V, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
   };
-  V fa[2][RM], fb[2][RN];
-  auto read_a = [&](const unsigned char* st, int i, int s) -> V {
-    if constexpr (MN) return turned(st, BM * 2, wm * WTM + i * 32, s);
-    else return straight(st, wm * WTM + i * 32, s);
+  V fa[2][TERMS][RM], fb[2][TERMS][RN];
+  // part r of a half stage's fragments
+  auto fetch = [&](int r, const unsigned char* st, int s, int set) {
+    const int term = r / (RM + RN), i = r % (RM + RN);
+    if (i < RN) {
+      fb[set][term][i < RN ? i : 0] = straight(st + TERMS * A_BYTES + term * B_BYTES, wn * WTN + i * 32, s);
+    } else {
+      const unsigned char* blk = st + term * A_BYTES;
+      const int e = wm * WTM + (i - RN) * 32;
+      if constexpr (MN) fa[set][term][i < RN ? 0 : i - RN] = turned(blk, BM * 2, e, s);
+      else fa[set][term][i < RN ? 0 : i - RN] = straight(blk, e, s);
+    }
   };
-  auto read_b = [&](const unsigned char* st, int j, int s) -> V { return straight(st + A_BYTES, wn * WTN + j * 32, s); };
 
 #pragma unroll
   for (int s = 0; s < ST - 1; ++s) {
@@ -210,29 +226,25 @@ __global__ void __launch_bounds__(WGM * WGN * 64, WGM * WGN / 4 * PER_CU) token_
     asm volatile("" ::: "memory");
   }
 #pragma unroll
-  for (int j = 0; j < RN; ++j) fb[0][j] = read_b(smem, j, 0);
-#pragma unroll
-  for (int i = 0; i < RM; ++i) fa[0][i] = read_a(smem, i, 0);
+  for (int r = 0; r < TERMS * (RM + RN); ++r) fetch(r, smem, 0, 0);
 
   // half a step: the products of set S; the fragments of the next 16 k (half S ^ 1 of
   // `next`) and half of a later stage's loads between them
   auto half = [&](auto SV, const unsigned char* next, unsigned char* fill) {
     constexpr int S = decltype(SV)::value, O = S ^ 1;
     constexpr int L0 = S == 0 ? 0 : (LPS + 1) / 2, L1 = S == 0 ? (LPS + 1) / 2 : LPS;
-    constexpr int NM = RM * RN, NR = RM + RN;
+    constexpr int EACH = RM * RN, NM = (SPLIT ? PRODUCTS : 1) * EACH, NR = TERMS * (RM + RN);
 #pragma unroll
     for (int q = 0; q < NM; ++q) {
 #pragma unroll
       for (int r = 0; r < NR; ++r)
-        if (r * NM / NR == q) {
-          if (r < RN) fb[O][r < RN ? r : 0] = read_b(next, r, O);
-          else fa[O][r < RN ? 0 : r - RN] = read_a(next, r - RN, O);
-        }
+        if (r * NM / NR == q) fetch(r, next, O, O);
 #pragma unroll
       for (int l = L0; l < L1; ++l)
         if ((l - L0) * NM / (L1 - L0) == q) load(l, fill, sa, sb);
-      const int i = q / RN, j = q % RN;
-      acc[i][j] = COLUMNS ? MF::run(fa[S][i], fb[S][j], acc[i][j]) : MF::run(fb[S][j], fa[S][i], acc[i][j]);
+      const int i = q % EACH / RN, j = q % RN;
+      const V a = fa[S][SPLIT ? TERM_A[q / EACH] : 0][i], b = fb[S][SPLIT ? TERM_B[q / EACH] : 0][j];
+      acc[i][j] = COLUMNS ? MF::run(a, b, acc[i][j]) : MF::run(b, a, acc[i][j]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -395,22 +407,33 @@ __global__ void __launch_bounds__(WGM * WGN * 64, WGM * WGN / 4 * PER_CU) token_
   }
 }
 
-template <typename OT, bool SPLIT, int MODE, bool TWO, int BM, int BN, int WGM, int WGN, int ST = 4, int PER_CU = 1>
-hipError_t run_tile(const TokenGemm& p, hipStream_t s) {
-  constexpr int NW = WGM * WGN, ring = ST * (BM + BN) * 64;
+template <typename OT, bool SPLIT, int MODE, bool TWO, int BM, int BN, int WGM, int WGN, int ST>
+__global__ void __launch_bounds__(WGM * WGN * 64) token_gemm_kernel(const TokenGemm p) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  product_tile<OT, SPLIT, MODE, TWO, BM, BN, WGM, WGN, ST>(p, smem, blockIdx.x, gridDim.x);
+}
+
+template <bool SPLIT, int MODE, int BM, int BN, int WGM, int WGN, int ST>
+constexpr int tile_lds() {
+  constexpr int NW = WGM * WGN, ring = ST * (SPLIT ? 3 : 1) * (BM + BN) * 64;
   constexpr int epi = MODE == TOKEN_STATS ? 0
                       : MODE == TOKEN_ERROR || (MODE == TOKEN_KEEP && !SPLIT) ? NW * 32 * (BM / WGM + 8) * 2
                       : MODE == TOKEN_KEEP ? NW * 32 * (BM / WGM + 4) * 4 : NW * 32 * (BN / WGN + 4) * 4;
-  constexpr int smem = epi > ring ? epi : ring;
+  return epi > ring ? epi : ring;
+}
+
+template <typename OT, bool SPLIT, int MODE, bool TWO, int BM, int BN, int WGM, int WGN, int ST = 4>
+hipError_t run_tile(const TokenGemm& p, hipStream_t s) {
+  constexpr int smem = tile_lds<SPLIT, MODE, BM, BN, WGM, WGN, ST>();
   static_assert(smem <= 160 * 1024, "LDS");
-  const void* fn = reinterpret_cast<const void*>(&token_gemm_kernel<OT, SPLIT, MODE, TWO, BM, BN, WGM, WGN, ST, PER_CU>);
+  const void* fn = reinterpret_cast<const void*>(&token_gemm_kernel<OT, SPLIT, MODE, TWO, BM, BN, WGM, WGN, ST>);
   static const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != hipSuccess) return e;
   constexpr int BNC = TWO ? BN / 2 : BN;
   const long long tiles = ((p.M + BM - 1LL) / BM) * ((p.N + BNC - 1LL) / BNC) * (MODE == TOKEN_GRAD ? p.slices : 1);
   TokenGemm q = p;
   void* args[] = {&q};
-  return hipLaunchKernel(fn, dim3((unsigned)tiles), dim3(NW * 64), args, smem, s);
+  return hipLaunchKernel(fn, dim3((unsigned)tiles), dim3(WGM * WGN * 64), args, smem, s);
 }
 
 }  // namespace token

@@ -8,10 +8,10 @@
 //    whatever they hold (so that nothing of them reaches W).
 // 2. Every piece of the vocabulary: the largest logit and sum of exponentials of each wave's
 //    rows.
-// 3. A column's parts joined: its loss, largest logit and 1 / sum.
+// 3. A column's parts joined: its loss, largest logit and 1 / sum (with one piece, by step 4).
 // 4. Every piece: its errors in 16 bits (fp32: three terms), its share of W^T e, and its
 //    rows of W, which nothing reads any more.
-// 5. The shares added in order, times f'(X).
+// 5. The shares added in order, times f'(X) (small: in the launch that updates W).
 //
 // Errors: a vocabulary whose errors fit one piece (1 GiB) has its exponentials kept there by step
 // 2, relative to their part's largest, and scaled in place: three products.  A
@@ -70,12 +70,12 @@ bool make_plan(int V, int D, int B, int storage, int act, bool update, Plan& o) 
   auto tiles = [&](long long m, long long n, long long e) { return ((m + e - 1) / e) * ((n + e - 1) / e); };
   const long long columns = o.two ? 2LL * B : B;
   if (columns <= 64) o.tile = o.rows >= 32768 ? TILE_128_64 : TILE_64;
-  else o.tile = tiles(o.rows, columns, 256) >= 192 ? TILE_256 : tiles(o.rows, columns, 128) > 128 ? TILE_128 : TILE_64;
+  else o.tile = storage != DT_F32 && tiles(o.rows, columns, 256) >= 192 ? TILE_256 : tiles(o.rows, columns, 128) > 128 ? TILE_128 : TILE_64;
   o.unit = token_unit(o.tile, o.two);
-  o.grad_tile = D >= 256 && B >= 256 ? 256 : D > 64 ? 128 : 64;
+  o.grad_tile = storage != DT_F32 && D >= 256 && B >= 256 ? 256 : D > 64 ? 128 : 64;
   const long long gt = o.grad_tile == 256 ? tiles(D, B, 256)
                        : o.grad_tile == 128 ? (D + 127LL) / 128 * (B > 64 ? (B + 127LL) / 128 : 1) : tiles(D, B, 64);
-  const long long stages = (long long)(o.terms == 3 ? token::PRODUCTS : 1) * (o.Vp / 32);
+  const long long stages = o.Vp / 32;
   o.slices = (int)std::max<long long>(1, std::min({256 / gt, stages / 8, 64LL}));
   long long at = 0;
   auto take = [&](long long bytes) {
@@ -93,7 +93,7 @@ bool make_plan(int V, int D, int B, int storage, int act, bool update, Plan& o) 
     o.et = take((long long)o.terms * o.Bk * o.Vp * 2);
     o.part = take(4LL * o.slices * D * B);
     o.kept = storage != DT_F32 ? o.et : o.keep ? take(4LL * o.Bk * o.Vp) : 0;
-    o.fixes = o.fix ? take(4LL * B * ((D + 31) / 32)) : 0;
+    o.fixes = o.fix ? take(4LL * B * token_fix_rows(D, false)) : 0;
   }
   o.bytes = at;
   return true;
@@ -125,36 +125,38 @@ __device__ __forceinline__ unsigned short term(float& v, bool again) {
   return __builtin_bit_cast(unsigned short, o);
 }
 
+// (TERMS 2: the loss alone, whose second term is what the first leaves of f(X))
 template <typename ST, typename OT, int TERMS, int ACT>
-__global__ void __launch_bounds__(256) token_states_kernel(const States p) {
-  // (TERMS 2: the loss alone, whose second term is what the first leaves of f(X))
-  __shared__ unsigned short tile[64][66];
-  const int tiles_n = (p.Bk + 63) / 64, d0 = blockIdx.x / tiles_n * 64, n0 = blockIdx.x % tiles_n * 64;
-  const int tid = threadIdx.x, c = tid & 63, n = n0 + c;
+__device__ __forceinline__ void lay_states(const States& p, int block) {
+  __shared__ unsigned short tile[32][34];
+  const int tiles_n = p.Bk / 32, d0 = block / tiles_n * 32, n0 = block % tiles_n * 32;
+  const int c = threadIdx.x & 31, r = threadIdx.x >> 5, n = n0 + c;
   const long long id = n < p.B ? p.targets[n] : -1;
   const bool real = id >= 0 && id < p.V;
-  float v[16];
+  float v[4];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int d = d0 + i * 4 + (tid >> 6);
-    v[i] = real && d < p.D ? act_t<ACT>(to_f32(static_cast<const ST*>(p.x)[(long long)d * p.B + n])) : 0.0f;
+  for (int i = 0; i < 4; ++i) {
+    const int d = d0 + i * 8 + r;
+    v[i] = n < p.B && d < p.D ? to_f32(static_cast<const ST*>(p.x)[(long long)d * p.B + n]) : 0.0f;
   }
 #pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = real && d0 + i * 8 + r < p.D ? act_t<ACT>(v[i]) : 0.0f;
+#pragma unroll
   for (int t = 0; t < TERMS; ++t) {
+    if (t > 0) __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int r = i * 4 + (tid >> 6), d = d0 + r;
+    for (int i = 0; i < 4; ++i) {
+      const int d = d0 + i * 8 + r;
       const unsigned short h = term<OT>(v[i], TERMS > 1);
-      tile[r][c] = h;
-      if (p.f && d < p.D && n < p.Bk) p.f[((long long)t * p.D + d) * p.Bk + n] = h;
+      tile[i * 8 + r][c] = h;
+      if (p.f && d < p.D) p.f[((long long)t * p.D + d) * p.Bk + n] = h;
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int r = i * 4 + (tid >> 6), row = n0 + r, d = d0 + c;
-      if (row < p.B && d < p.Dp) p.ft[((long long)t * p.B + row) * p.Dp + d] = tile[c][r];
+    for (int i = 0; i < 4; ++i) {
+      const int row = n0 + i * 8 + r;
+      if (row < p.B) p.ft[((long long)t * p.B + row) * p.Dp + d0 + c] = tile[c][i * 8 + r];
     }
-    __syncthreads();
   }
 }
 
@@ -166,8 +168,8 @@ struct Rows {
   unsigned short* out;
 };
 template <typename ST, typename OT, int TERMS>
-__global__ void __launch_bounds__(256) token_rows_kernel(const Rows p) {
-  const long long at = ((long long)blockIdx.x * 256 + threadIdx.x) * 4, count = (long long)p.padded * p.Dp;
+__device__ __forceinline__ void lay_rows(const Rows& p, unsigned block) {
+  const long long at = ((long long)block * 256 + threadIdx.x) * 4, count = (long long)p.padded * p.Dp;
   if (at >= count) return;
   const int r = (int)(at / p.Dp), d = (int)(at - (long long)r * p.Dp);
   const ST* from = static_cast<const ST*>(p.w) + (long long)r * p.D + d;
@@ -183,6 +185,13 @@ __global__ void __launch_bounds__(256) token_rows_kernel(const Rows p) {
   }
 }
 
+// Workgroups 0 .. states - 1: f(X); the others: rows of W.
+template <typename ST, typename OT, int TERMS, int ACT>
+__global__ void __launch_bounds__(256) token_lay_kernel(const States x, const Rows w, unsigned states) {
+  if (blockIdx.x < states) lay_states<ST, OT, TERMS, ACT>(x, blockIdx.x);
+  else lay_rows<ST, OT, TERMS>(w, blockIdx.x - states);
+}
+
 // ---------------------------------------------------------------- a column's tiles
 struct Columns {
   int B, V, tiles;
@@ -196,18 +205,17 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
   const float top = __builtin_fmaxf(a.x, b.x), none = -__builtin_inff();
   return make_float2(top, (a.x == none ? a.y : a.y * expf(a.x - top)) + (b.x == none ? b.y : b.y * expf(b.x - top)));
 }
-// 16 columns a workgroup, 64 threads each
-__global__ void __launch_bounds__(1024) token_columns_kernel(const Columns p) {
-  __shared__ float2 red[64][16];
-  const int c = threadIdx.x & 15, g = threadIdx.x >> 4, n = blockIdx.x * 16 + c;
+// `across` columns a workgroup (a power of two, 16 at most), 1024 / across threads each
+__global__ void __launch_bounds__(1024) token_columns_kernel(const Columns p, int across) {
+  __shared__ float2 red[1024];
+  const int c = threadIdx.x & (across - 1), each = 1024 / across, g = threadIdx.x / across, n = blockIdx.x * across + c;
   float2 v = make_float2(-__builtin_inff(), 0.0f);
   if (n < p.B)
-    for (int t = g; t < p.tiles; t += 64) v = join(v, p.part[(long long)t * p.B + n]);
-  red[g][c] = v;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
+    for (int t = g; t < p.tiles; t += each) v = join(v, p.part[(long long)t * p.B + n]);
+  red[threadIdx.x] = v;
+  for (int o = each / 2; o > 0; o >>= 1) {
     __syncthreads();
-    if (g < o) red[g][c] = v = join(v, red[g + o][c]);
+    if (g < o) red[threadIdx.x] = v = join(v, red[threadIdx.x + o * across]);
   }
   if (g != 0 || n >= p.B) return;
   const long long id = p.targets[n];
@@ -215,56 +223,14 @@ __global__ void __launch_bounds__(1024) token_columns_kernel(const Columns p) {
   p.norm[n] = make_float2(v.x, 1.0f / v.y);
 }
 
-// ------------------------------------------------------------------ G
-struct Grad {
-  int D, B, V, slices;
-  const float* part;  // [slices][D][B]
-  const void* x;
-  const long long* targets;
-  void* g;
-  float scale;
-  float* fixes;       // [(D + 31) / 32][B], or nullptr
-};
-// 32 rows of 64 columns a workgroup
-template <typename ST, int ACT>
-__global__ void __launch_bounds__(256) token_gradient_kernel(const Grad p) {
-  __shared__ float red[4][64];
-  const int tiles_n = (p.B + 63) / 64, d0 = blockIdx.x / tiles_n * 32, c = threadIdx.x & 63, r = threadIdx.x >> 6;
-  const int n = blockIdx.x % tiles_n * 64 + c;
-  const long long count = (long long)p.D * p.B;
-  const long long id = n < p.B ? p.targets[n] : -1;
-  const bool real = id >= 0 && id < p.V;
-  float fix = 0.0f;
-  if (n < p.B) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int d = d0 + i * 4 + r;
-      if (d >= p.D) break;
-      const long long at = (long long)d * p.B + n;
-      float sum = 0.0f;
-#pragma unroll 4
-      for (int s = 0; s < p.slices; ++s) sum += p.part[s * count + at];
-      const float x = to_f32(static_cast<const ST*>(p.x)[at]);
-      sum *= p.scale;
-      static_cast<ST*>(p.g)[at] = cvt<ST>(real ? dact_t<ACT>(x) * sum : 0.0f);
-      if (p.fixes && real) {
-        const float f = act_t<ACT>(x);
-        fix += sum * (f - to_f32(cvt<ST>(f)));
-      }
-    }
-  }
-  if (!p.fixes) return;
-  red[r][c] = fix;
-  __syncthreads();
-  if (r == 0 && n < p.B) p.fixes[(long long)(d0 / 32) * p.B + n] = red[0][c] + red[1][c] + red[2][c] + red[3][c];
-}
-
+// ---------------------------------------------------------------- the loss
 // loss -= the fixes, in order; 16 columns a workgroup, 16 threads each
 __global__ void __launch_bounds__(256) token_fix_kernel(const float* fixes, int rows, int B, float* loss) {
   __shared__ float red[16][16];
   const int c = threadIdx.x & 15, g = threadIdx.x >> 4, n = blockIdx.x * 16 + c;
   float sum = 0.0f;
   if (n < B)
+#pragma unroll 8
     for (int i = g; i < rows; i += 16) sum += fixes[(long long)i * B + n];
   red[g][c] = sum;
   __syncthreads();
@@ -275,61 +241,86 @@ __global__ void __launch_bounds__(256) token_fix_kernel(const float* fixes, int 
 }
 
 // ------------------------------------------------------------------ errors
-// Kept exponentials into errors, in place (fp32: into three terms).  Eight of a row a thread;
-// its columns up to Vp and rows up to Bk, zeros past the ends and in padded rows.
+// Kept exponentials into errors, in place (fp32: into three terms): a column (a row of ET, up
+// to Vp) a workgroup, which joins the column's parts itself, up to ERROR_RUN values; of longer
+// ones 2048 values, their columns joined before.  Zeros past the ends and in padded rows, up
+// to Bk.  us, joining here / before: V = 10007, B = 77 fp32 9.6 / 4.7 + 5.4; V = 32000, B = 1024
+// bf16 34.8 / 6.3 + 27.0; V = 128000, B = 2048 341 / 14.6 + 226.
+constexpr int ERROR_RUN = 8192;
 struct Errors {
-  int V, B, Vp, Bk, unit;
-  const void* kept;   // [Bk][Vp]
+  int V, B, Vp, Bk, unit, units;
+  const void* kept;     // [Bk][Vp]
   unsigned short* et;
-  const float2* part;
+  const float2* part;   // [units][B]
+  const float* logit;
+  float* loss;
   const float2* norm;
-  const float* loss;
   const long long* targets;
   float scale;
 };
-template <typename OT, int TERMS>
+template <typename OT, int TERMS, bool JOIN>
 __global__ void __launch_bounds__(256) token_errors_kernel(const Errors p) {
-  const int per = p.Vp / 8;
-  const unsigned at = blockIdx.x * 256u + threadIdx.x, n = at / (unsigned)per;
-  const int v = (int)(at - n * (unsigned)per) * 8;
-  if (n >= (unsigned)p.Bk) return;
-  const long long place = (long long)n * p.Vp + v;
-  const long long id = n < (unsigned)p.B ? p.targets[n] : -1;
-  float e[8] = {};
-  if (id >= 0 && id < p.V && v < p.V) {
-    const float2 norm = p.norm[n];
-    const float part = p.part[(long long)(v / p.unit) * p.B + n].x;
-    const float share = -p.scale * norm.y * (part == -__builtin_inff() ? 0.0f : expf(part - norm.x));
-    if constexpr (TERMS == 1) {
-      const f16x8 h = *reinterpret_cast<const f16x8*>(static_cast<const unsigned short*>(p.kept) + place);
+  __shared__ float2 red[4];
+  const int runs = JOIN ? 1 : (p.Vp + 2047) / 2048, n = blockIdx.x / runs, tid = threadIdx.x;
+  const int first = blockIdx.x % runs * 2048, last = JOIN ? p.Vp : min(first + 2048, p.Vp);
+  const long long id = n < p.B ? p.targets[n] : -1;
+  const bool real = id >= 0 && id < p.V;  // (the same for the whole workgroup)
+  float2 all = make_float2(-__builtin_inff(), 0.0f);  // y: 1 / sum
+  float loss = 0.0f;
+  if constexpr (JOIN) {
+    if (real) {
+      for (int t = tid; t < p.units; t += 256) all = join(all, p.part[(long long)t * p.B + n]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = (float)h[i] * (1.0f / 32768.0f) * share;
-    } else {
-      const float4* k = reinterpret_cast<const float4*>(static_cast<const float*>(p.kept) + place);
-      const float4 a = k[0], b = k[1];
-      e[0] = a.x; e[1] = a.y; e[2] = a.z; e[3] = a.w; e[4] = b.x; e[5] = b.y; e[6] = b.z; e[7] = b.w;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] *= share;
+      for (int o = 32; o > 0; o >>= 1) all = join(all, make_float2(__shfl_xor(all.x, o), __shfl_xor(all.y, o)));
+      if ((tid & 63) == 0) red[tid >> 6] = all;
+      __syncthreads();
+      all = join(join(red[0], red[1]), join(red[2], red[3]));
+      loss = logf(all.y) + (all.x - p.logit[n]);
+      all.y = 1.0f / all.y;
     }
-    if (v + 8 > p.V) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (v + i >= p.V) e[i] = 0.0f;
-    }
-    if (id >= v && id < v + 8) {
-      const float own = -expm1f(-p.loss[n]) * p.scale;  // 1 - p without its cancellation
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (id == v + i) e[i] = own;
-    }
+    if (tid == 0 && n < p.B) p.loss[n] = loss;
+  } else if (real) {
+    all = p.norm[n];
+    loss = p.loss[n];
   }
+  const float norm = -p.scale * all.y;
+  for (int v = first + tid * 8; v < last; v += 256 * 8) {
+    const long long place = (long long)n * p.Vp + v;
+    float e[8] = {};
+    if (real && v < p.V) {
+      const float part = p.part[(long long)(v / p.unit) * p.B + n].x;
+      const float share = norm * (part == -__builtin_inff() ? 0.0f : expf(part - all.x));
+      if constexpr (TERMS == 1) {
+        const f16x8 h = *reinterpret_cast<const f16x8*>(static_cast<const unsigned short*>(p.kept) + place);
 #pragma unroll
-  for (int t = 0; t < TERMS; ++t) {
-    unsigned short h[8];
+        for (int i = 0; i < 8; ++i) e[i] = (float)h[i] * (1.0f / 32768.0f) * share;
+      } else {
+        const float4* k = reinterpret_cast<const float4*>(static_cast<const float*>(p.kept) + place);
+        const float4 a = k[0], b = k[1];
+        e[0] = a.x; e[1] = a.y; e[2] = a.z; e[3] = a.w; e[4] = b.x; e[5] = b.y; e[6] = b.z; e[7] = b.w;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = term<OT>(e[i], TERMS > 1);
-    *reinterpret_cast<uint4*>(p.et + (long long)t * p.Bk * p.Vp + place) =
-        make_uint4(h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16, h[4] | (unsigned)h[5] << 16, h[6] | (unsigned)h[7] << 16);
+        for (int i = 0; i < 8; ++i) e[i] *= share;
+      }
+      if (v + 8 > p.V) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (v + i >= p.V) e[i] = 0.0f;
+      }
+      if (id >= v && id < v + 8) {
+        const float own = -expm1f(-loss) * p.scale;  // 1 - p without its cancellation
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (id == v + i) e[i] = own;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < TERMS; ++t) {
+      unsigned short h[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] = term<OT>(e[i], TERMS > 1);
+      *reinterpret_cast<uint4*>(p.et + (long long)t * p.Bk * p.Vp + place) =
+          make_uint4(h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16, h[4] | (unsigned)h[5] << 16, h[6] | (unsigned)h[7] << 16);
+    }
   }
 }
 
@@ -341,13 +332,20 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
   unsigned char* ws = p.workspace;
   auto at = [&](long long offset) { return reinterpret_cast<unsigned short*>(ws + offset); };
   const States st{p.D, p.B, p.V, o.Dp, o.Bk, p.x, p.targets, update ? at(o.f) : nullptr, at(o.ft)};
-  const unsigned state_tiles = (unsigned)((o.Dp + 63LL) / 64 * ((o.Bk + 63LL) / 64));
+  const unsigned state_tiles = (unsigned)((long long)(o.Dp / 32) * (o.Bk / 32));
   constexpr bool inexact = TERMS == 1 && ACT != ACT_IDENTITY && ACT != ACT_RELU;
-  if (inexact && !update) hipLaunchKernelGGL((token_states_kernel<ST, OT, inexact ? 2 : TERMS, ACT>), dim3(state_tiles), dim3(256), 0, s, st);
-  else hipLaunchKernelGGL((token_states_kernel<ST, OT, TERMS, ACT>), dim3(state_tiles), dim3(256), 0, s, st);
-
-  hipError_t e = hipGetLastError();
+  hipError_t e = hipSuccess;
   auto rows_of = [&](int first) { return std::min(o.rows, p.V - first); };
+  // the piece's rows of W where they are laid out, and (states: workgroups) f(X)
+  auto lay_out = [&](int first, unsigned states) {
+    const int rows = rows_of(first), padded = (rows + 31) / 32 * 32;
+    const Rows r{rows, padded, p.D, o.Dp, static_cast<const ST*>(p.w) + (long long)first * p.D, at(o.ws)};
+    const long long fours = o.copy ? (long long)padded * o.Dp / 4 : 0;
+    const dim3 grid(states + (unsigned)((fours + 255) / 256)), block(256);
+    if (inexact && !update) hipLaunchKernelGGL((token_lay_kernel<ST, OT, inexact ? 2 : TERMS, ACT>), grid, block, 0, s, st, r, states);
+    else hipLaunchKernelGGL((token_lay_kernel<ST, OT, TERMS, ACT>), grid, block, 0, s, st, r, states);
+    if (e == hipSuccess) e = hipGetLastError();
+  };
   // the piece's rows of W, as an operand of the products
   auto weights = [&](int first, TokenGemm& q, bool lay) {
     const int rows = rows_of(first), padded = (rows + 31) / 32 * 32;
@@ -356,12 +354,7 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
       q.a = w; q.lda = p.D; q.a_bytes = (long long)rows * p.D * 2; q.a_term = 0;
       return;
     }
-    if (lay) {
-      const Rows r{rows, padded, p.D, o.Dp, w, at(o.ws)};
-      const long long fours = (long long)padded * o.Dp / 4;
-      hipLaunchKernelGGL((token_rows_kernel<ST, OT, TERMS>), dim3((unsigned)((fours + 255) / 256)), dim3(256), 0, s, r);
-      if (e == hipSuccess) e = hipGetLastError();
-    }
+    if (lay) lay_out(first, 0);
     q.a = at(o.ws); q.lda = o.Dp;
     q.a_term = (unsigned)(padded * o.Dp * 2);
     q.a_bytes = (long long)TERMS * padded * o.Dp * 2;
@@ -376,8 +369,10 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
     return q;
   };
   float2* part = reinterpret_cast<float2*>(ws + o.stats);
+  lay_out(0, state_tiles);
+  if (e != hipSuccess) return e;
   for (int first = 0; first < p.V && e == hipSuccess; first += o.rows) {
-    TokenGemm q = logits(first, true);
+    TokenGemm q = logits(first, first > 0);
     if (e != hipSuccess) return e;
     q.out = part + (long long)(first / o.unit) * p.B;
     if (o.keep) {
@@ -388,21 +383,33 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
     }
   }
   if (e != hipSuccess) return e;
-  const Columns c{p.B, p.V, (p.V + o.unit - 1) / o.unit, part, reinterpret_cast<const float*>(ws + o.logit), p.targets, p.loss,
-                  reinterpret_cast<float2*>(ws + o.norm)};
-  hipLaunchKernelGGL(token_columns_kernel, dim3((unsigned)((p.B + 15) / 16)), dim3(1024), 0, s, c);
-  e = hipGetLastError();
-  if (!update || e != hipSuccess) return e;
+  const int units = (p.V + o.unit - 1) / o.unit;
+  const bool joined = o.keep && o.Vp <= ERROR_RUN;  // with the errors
+  if (!joined) {
+    const Columns c{p.B, p.V, units, part, reinterpret_cast<const float*>(ws + o.logit), p.targets, p.loss,
+                    reinterpret_cast<float2*>(ws + o.norm)};
+    int across = 16;
+    while (across > 1 && across / 2 >= p.B) across /= 2;
+    hipLaunchKernelGGL(token_columns_kernel, dim3((unsigned)((p.B + across - 1) / across)), dim3(1024), 0, s, c, across);
+    e = hipGetLastError();
+    if (!update || e != hipSuccess) return e;
+  }
 
   // fp16: errors below its smallest normal number matter (1 / V), so they are kept times 2^10
   const float scale = storage == DT_F16 ? 1024.0f : 1.0f;
+  float* fixes = o.fix ? reinterpret_cast<float*>(ws + o.fixes) : nullptr;
+  const int vec_state = p.B % 4 == 0 && reinterpret_cast<uintptr_t>(p.x) % (4 * sizeof(ST)) == 0 &&
+                        reinterpret_cast<uintptr_t>(p.g) % (4 * sizeof(ST)) == 0;
+  const TokenFinish finish{p.D, p.B, p.V, o.slices, p.act, reinterpret_cast<const float*>(ws + o.part), p.x, p.targets, p.g,
+                           1.0f / scale, fixes, vec_state};
   for (int first = 0; first < p.V; first += o.rows) {
     const int rows = rows_of(first), Vp = (rows + 31) / 32 * 32;
     if (o.keep) {
-      const Errors er{p.V, p.B, Vp, o.Bk, o.unit, ws + o.kept, at(o.et), part, reinterpret_cast<const float2*>(ws + o.norm),
-                      p.loss, p.targets, scale};
-      const long long eights = (long long)o.Bk * Vp / 8;
-      hipLaunchKernelGGL((token_errors_kernel<OT, TERMS>), dim3((unsigned)((eights + 255) / 256)), dim3(256), 0, s, er);
+      const Errors er{p.V, p.B, Vp, o.Bk, o.unit, units, ws + o.kept, at(o.et), part, reinterpret_cast<const float*>(ws + o.logit),
+                      p.loss, reinterpret_cast<const float2*>(ws + o.norm), p.targets, scale};
+      const dim3 grid((unsigned)((long long)o.Bk * (joined ? 1 : (Vp + 2047) / 2048)));
+      if (joined) hipLaunchKernelGGL((token_errors_kernel<OT, TERMS, true>), grid, dim3(256), 0, s, er);
+      else hipLaunchKernelGGL((token_errors_kernel<OT, TERMS, false>), grid, dim3(256), 0, s, er);
       e = hipGetLastError();
     } else {
       TokenGemm q = logits(first, o.rows < p.V);  // (one piece: its rows are laid out already)
@@ -426,16 +433,11 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
     u.out = static_cast<ST*>(p.w) + (long long)first * p.D;
     u.vec = p.D % 4 == 0 && reinterpret_cast<uintptr_t>(p.w) % (4 * sizeof(ST)) == 0;
     u.scal = p.alpha / scale;
-    e = launch_token_weight(u, storage, s);
+    e = launch_token_weight(u, first + rows == p.V ? &finish : nullptr, storage, s);
     if (e != hipSuccess) return e;
   }
-  float* fixes = o.fix ? reinterpret_cast<float*>(ws + o.fixes) : nullptr;
-  const Grad gr{p.D, p.B, p.V, o.slices, reinterpret_cast<const float*>(ws + o.part), p.x, p.targets, p.g, 1.0f / scale, fixes};
-  const int bands = (p.D + 31) / 32;
-  hipLaunchKernelGGL((token_gradient_kernel<ST, ACT>), dim3((unsigned)((long long)bands * ((p.B + 63) / 64))), dim3(256), 0, s, gr);
-  e = hipGetLastError();
-  if (!fixes || e != hipSuccess) return e;
-  hipLaunchKernelGGL(token_fix_kernel, dim3((unsigned)((p.B + 15) / 16)), dim3(256), 0, s, fixes, bands, p.B, p.loss);
+  if (!fixes) return e;
+  hipLaunchKernelGGL(token_fix_kernel, dim3((unsigned)((p.B + 15) / 16)), dim3(256), 0, s, fixes, token_fix_rows(p.D, vec_state), p.B, p.loss);
   return hipGetLastError();
 }
 
