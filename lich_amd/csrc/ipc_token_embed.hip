@@ -287,82 +287,70 @@ __global__ void __launch_bounds__(SORT_WAVES * 64) embed_sort_kernel(const Embed
 // A run of EMBED_RUN sorted places, 4 features a thread.  Ids that begin and end in the
 // run are finished here; a sum that came over the run's start goes to part[run][0], one
 // that goes on past its end to part[run][1].
-// (values as they lie: widened when used, so that many rows can be in flight)
-template <typename ST>
-__device__ __forceinline__ void get_row(const ST* from, int left, bool whole, Four<ST>& v) {
-  if (whole) {
-    v = *reinterpret_cast<const Four<ST>*>(__builtin_assume_aligned(from, 4 * sizeof(ST)));
-  } else {
+// W features a thread: 4 where rows and the table are aligned for it, else 1.  Values stay as they
+// lie until used, so that many rows can be in flight.
+template <typename ST, int W> struct alignas(W * sizeof(ST)) Piece { ST v[W]; };
+template <int W, typename ST>
+__device__ __forceinline__ Piece<ST, W> get_piece(const ST* from) { return *reinterpret_cast<const Piece<ST, W>*>(from); }
+template <int W, typename ST>
+__device__ __forceinline__ void put_piece(ST* to, const float (&v)[W]) {
+  Piece<ST, W> o;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v.v[q] = q < left ? from[q] : cvt<ST>(0.0f);
-  }
+  for (int q = 0; q < W; ++q) o.v[q] = cvt<ST>(v[q]);
+  *reinterpret_cast<Piece<ST, W>*>(to) = o;
 }
-template <typename ST>
-__device__ __forceinline__ void put_row(ST* to, int left, bool whole, const float (&v)[4]) {
-  ST o[4];
+template <int W, typename ST>
+__device__ __forceinline__ void add_to_piece(ST* to, const Piece<ST, W>& old, float alpha, const float (&sum)[W]) {
+  float v[W];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) o[q] = cvt<ST>(v[q]);
-  if (whole) {
-    store4(to, o);
-  } else {
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (q < left) to[q] = o[q];
-  }
-}
-template <typename ST>
-__device__ __forceinline__ void add_to_row(ST* to, int left, bool whole, const Four<ST>& old, float alpha, const float (&sum)[4]) {
-  float v[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) v[q] = to_f32(old.v[q]) + alpha * sum[q];
-  put_row(to, left, whole, v);
+  for (int q = 0; q < W; ++q) v[q] = to_f32(old.v[q]) + alpha * sum[q];
+  put_piece<W>(to, v);
 }
 
-template <typename ST>
+template <typename ST, int W>
 __global__ void __launch_bounds__(256) embed_run_kernel(const EmbedUpdate p) {
   const int run = blockIdx.x, N = p.C * p.B, lane = threadIdx.x & 63;
-  const int d = (blockIdx.y * blockDim.x + threadIdx.x) * 4, first = run * EMBED_RUN;
+  const int d = (blockIdx.y * blockDim.x + threadIdx.x) * W, first = run * EMBED_RUN;
   // lane i: the id of the place before the run's i-th, and the i-th's row of G
   const int at = first - 1 + lane;
   const int keys = at >= 0 && at <= N ? p.key[at] : -1;
   const int orders = lane < EMBED_RUN && first + lane < N ? p.order[first + lane] : 0;
   auto key = [&](int i) { return __builtin_amdgcn_readlane(keys, i + 1); };
   if (key(0) < 0 || d >= p.D) return;
-  const ST* rows = static_cast<const ST*>(p.rows);
-  ST* table = static_cast<ST*>(p.table);
-  const bool whole = p.D % 4 == 0, vec = p.vec_d != 0;  // (rows and part start on 256 bytes)
-  const int left = p.D - d;
+  const ST* rows = static_cast<const ST*>(p.rows) + d;
+  ST* table = static_cast<ST*>(p.table) + d;
   // every row of G and of the table, none stored before all are read (a place without an id: any row)
-  Four<ST> v[EMBED_RUN], old[EMBED_RUN];
+  Piece<ST, W> v[EMBED_RUN], old[EMBED_RUN];
 #pragma unroll
   for (int u = 0; u < EMBED_RUN; ++u) {
     const int id = key(u);
-    get_row(rows + (long long)(id < 0 ? 0 : __builtin_amdgcn_readlane(orders, u)) * p.D + d, left, whole, v[u]);
-    get_row(table + (long long)(id < 0 ? 0 : id) * p.D + d, left, vec, old[u]);
+    v[u] = get_piece<W>(rows + (long long)(id < 0 ? 0 : __builtin_amdgcn_readlane(orders, u)) * p.D);
+    old[u] = get_piece<W>(table + (long long)(id < 0 ? 0 : id) * p.D);
   }
   bool over = key(-1) == key(0);  // its sum came over the start
-  float sum[4] = {};
+  float sum[W] = {};
 #pragma unroll
   for (int u = 0; u < EMBED_RUN; ++u) {
     const int id = key(u);
     if (id < 0) return;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) sum[q] += to_f32(v[u].v[q]);
+    for (int q = 0; q < W; ++q) sum[q] += to_f32(v[u].v[q]);
     const bool on = key(u + 1) == id;
     if (on && u + 1 < EMBED_RUN) continue;
-    if (over || on) put_row(p.part + ((long long)run * 2 + (over ? 0 : 1)) * p.D + d, left, whole, sum);  // the run's first and ended, or its last and not
-    else add_to_row(table + (long long)id * p.D + d, left, vec, old[u], p.alpha, sum);
+    // the run's first and ended, or its last and not: a part
+    if (over || on) put_piece<W>(p.part + ((long long)run * 2 + (over ? 0 : 1)) * p.D + d, sum);
+    else add_to_piece<W>(table + (long long)id * p.D, old[u], p.alpha, sum);
     over = false;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) sum[q] = 0.0f;
+    for (int q = 0; q < W; ++q) sum[q] = 0.0f;
   }
 }
 
 // Sums that cross runs' ends, joined in order by the run they begin in.
-template <typename ST>
+template <typename ST, int W>
 __global__ void __launch_bounds__(256) embed_join_kernel(const EmbedUpdate p) {
   const int run = blockIdx.x, N = p.C * p.B, runs = (N + EMBED_RUN - 1) / EMBED_RUN;
-  const int d = (blockIdx.y * blockDim.x + threadIdx.x) * 4, lane = threadIdx.x & 63;
+  const int d = (blockIdx.y * blockDim.x + threadIdx.x) * W, lane = threadIdx.x & 63;
   const int first = run * EMBED_RUN, end = first + EMBED_RUN;
   if (end >= N) return;
   const int id = p.key[end - 1];
@@ -375,22 +363,29 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const EmbedUpdate p) {
     if (other) break;
   }
   if (d >= p.D) return;
-  const int left = p.D - d;
-  const bool whole = p.D % 4 == 0;
   ST* row = static_cast<ST*>(p.table) + (long long)id * p.D + d;
-  float sum[4] = {};
-  Four<ST> old;
-  get_row(row, left, p.vec_d != 0, old);
+  const Piece<ST, W> old = get_piece<W>(row);
+  float sum[W] = {};
   const float* from = p.part + ((long long)run * 2 + 1) * p.D + d;
 #pragma unroll 8
   for (int r = 0; r <= more; ++r) {
     // (its own second sum, then the later runs' first ones: 1, 3, 5, ... rows on)
-    Four<float> v;
-    get_row(from + (r == 0 ? 0 : 2 * r - 1) * (long long)p.D, left, whole, v);
+    const Piece<float, W> v = get_piece<W>(from + (r == 0 ? 0 : 2 * r - 1) * (long long)p.D);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) sum[q] += v.v[q];
+    for (int q = 0; q < W; ++q) sum[q] += v.v[q];
   }
-  add_to_row(row, left, p.vec_d != 0, old, p.alpha, sum);
+  add_to_piece<W>(row, old, p.alpha, sum);
+}
+
+template <typename ST, int W>
+hipError_t run_sums(const EmbedUpdate& p, hipStream_t s) {
+  const int N = p.C * p.B, lanes = (p.D + W - 1) / W, threads = lanes >= 256 ? 256 : (lanes + 63) / 64 * 64;
+  const dim3 grid((unsigned)((N + EMBED_RUN - 1) / EMBED_RUN), (unsigned)((lanes + threads - 1) / threads));
+  hipLaunchKernelGGL((embed_run_kernel<ST, W>), grid, dim3(threads), 0, s, p);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((embed_join_kernel<ST, W>), grid, dim3(threads), 0, s, p);
+  return hipGetLastError();
 }
 
 template <typename ST>
@@ -417,15 +412,9 @@ hipError_t run_update(const EmbedUpdate& p, hipStream_t s) {
   const int turn_lds = 64 * (TURN<ST> + 2) * (int)sizeof(ST), sort_lds = SORT_WAVES * range * 4;
   hipLaunchKernelGGL((embed_sort_kernel<ST>), dim3((unsigned)(ranges + turns)), dim3(SORT_WAVES * 64),
                      turn_lds > sort_lds ? turn_lds : sort_lds, s, p, ranges, range);
-  hipError_t e = hipGetLastError();
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const int threads = p.D >= 1024 ? 256 : ((p.D + 3) / 4 + 63) / 64 * 64;
-  const dim3 grid((unsigned)((N + EMBED_RUN - 1) / EMBED_RUN), (unsigned)((p.D + 4 * threads - 1) / (4 * threads)));
-  hipLaunchKernelGGL((embed_run_kernel<ST>), grid, dim3(threads), 0, s, p);
-  e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((embed_join_kernel<ST>), grid, dim3(threads), 0, s, p);
-  return hipGetLastError();
+  return p.vec_d ? run_sums<ST, 4>(p, s) : run_sums<ST, 1>(p, s);
 }
 
 }  // namespace
