@@ -132,14 +132,18 @@ __global__ void __launch_bounds__(256) embed_few_kernel(const EmbedUpdate p) {
 // between the two readings.  The other workgroups transpose G.
 constexpr int SORT_WAVES = 16, SORT_HELD = 8;
 
-inline int sort_range(int V) {
-  const int r = (V / 256 + 64) / 64 * 64;
+// Ids of a range, at most 512: a workgroup for each 32 places, up to one a CU.  (Few ids each:
+// a wave places the ids that it meets among 64 places one after the other; 8192 places of 64
+// ids in one range: 56 us, in 64: 11.  But few workgroups for few places: 1505 places of 1531
+// ids, 256 ranges 10.6 us, 24 6.2.)
+inline int sort_range(int V, int N) {
+  const int most = N / 32 < 256 ? N / 32 : 256, r = (V + most - 1) / most;
   return r > 512 ? 512 : r;
 }
 
 // A block of G, 64 features by TURN samples, so that each thread has several loads in flight.
 template <typename ST> constexpr int TURN = sizeof(ST) == 4 ? 128 : 256;
-template <typename ST>
+template <typename ST, bool VEC>
 __device__ void transpose_rows(const EmbedUpdate& p, int block, ST* tile) {
   constexpr int W = TURN<ST>, LD = W + 2, EACH = 64 * W / 4 / (SORT_WAVES * 64);
   const int tiles_d = (p.D + 63) / 64, tiles_b = (p.B + W - 1) / W;
@@ -153,7 +157,7 @@ __device__ void transpose_rows(const EmbedUpdate& p, int block, ST* tile) {
     const int u = e * SORT_WAVES * 64 + threadIdx.x, d = u / (W / 4), b = u % (W / 4) * 4;
     if (d0 + d >= p.D || b0 + b >= p.B) continue;
     const ST* from = g + ((long long)c * p.D + d0 + d) * p.B + b0 + b;
-    if (p.vec_b) {
+    if constexpr (VEC) {
       const Four<ST> f = *reinterpret_cast<const Four<ST>*>(__builtin_assume_aligned(from, 4 * sizeof(ST)));
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[e][i] = f.v[i];
@@ -177,7 +181,7 @@ __device__ void transpose_rows(const EmbedUpdate& p, int block, ST* tile) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = tile[(d + i) * LD + b];
     ST* to = rows + ((long long)c * p.B + b0 + b) * p.D + d0 + d;
-    if (p.D % 4 == 0) {  // (rows starts on 256 bytes)
+    if constexpr (VEC) {  // (rows starts on 256 bytes)
       store4(to, o);
     } else {
 #pragma unroll
@@ -187,11 +191,11 @@ __device__ void transpose_rows(const EmbedUpdate& p, int block, ST* tile) {
   }
 }
 
-template <typename ST>
+template <typename ST, bool VEC>
 __global__ void __launch_bounds__(SORT_WAVES * 64) embed_sort_kernel(const EmbedUpdate p, int ranges, int range) {
   extern __shared__ __align__(16) int lds[];
   if ((int)blockIdx.x >= ranges) {
-    transpose_rows<ST>(p, blockIdx.x - ranges, reinterpret_cast<ST*>(lds));
+    transpose_rows<ST, VEC>(p, blockIdx.x - ranges, reinterpret_cast<ST*>(lds));
     return;
   }
   __shared__ int before[SORT_WAVES], sums[SORT_WAVES];
@@ -262,9 +266,15 @@ __global__ void __launch_bounds__(SORT_WAVES * 64) embed_sort_kernel(const Embed
     for (int i = base + tid; i <= N; i += SORT_WAVES * 64) p.key[i] = -1;
   for (int i0 = first; i0 < last; i0 += 64 * SORT_HELD) {
     if (last - first > 64 * SORT_HELD) fetch(i0, false);
+    unsigned many = 0;  // bit u: the u-th 64 have some in the range
 #pragma unroll
-    for (int u = 0; u < SORT_HELD; ++u) {
-      const unsigned own = held[u];
+    for (int u = 0; u < SORT_HELD; ++u) many |= __any(held[u] != ~0u) ? 1u << u : 0u;
+#pragma unroll 1
+    for (; many; many &= many - 1) {
+      const int u = __ffs(many) - 1;
+      unsigned own = held[0];
+#pragma unroll
+      for (int q = 1; q < SORT_HELD; ++q) own = u == q ? held[q] : own;
       unsigned long long left = __ballot(own != ~0u);
       while (left) {  // one id after the other, its places in lane order
         const unsigned which = __builtin_amdgcn_readlane(own, __ffsll((unsigned long long)left) - 1);
@@ -407,11 +417,13 @@ hipError_t run_update(const EmbedUpdate& p, hipStream_t s) {
     hipLaunchKernelGGL((embed_few_kernel<ST>), dim3((unsigned)(N * (long long)((p.D + 255) / 256))), dim3(256), 0, s, p);
     return hipGetLastError();
   }
-  const int range = sort_range(p.V), ranges = (int)(((long long)p.V + range - 1) / range);
+  const int range = sort_range(p.V, N), ranges = (int)(((long long)p.V + range - 1) / range);
   const long long turns = (long long)p.C * ((p.B + TURN<ST> - 1) / TURN<ST>) * ((p.D + 63) / 64);
   const int turn_lds = 64 * (TURN<ST> + 2) * (int)sizeof(ST), sort_lds = SORT_WAVES * range * 4;
-  hipLaunchKernelGGL((embed_sort_kernel<ST>), dim3((unsigned)(ranges + turns)), dim3(SORT_WAVES * 64),
-                     turn_lds > sort_lds ? turn_lds : sort_lds, s, p, ranges, range);
+  const dim3 grid((unsigned)(ranges + turns)), block(SORT_WAVES * 64);
+  const int lds = turn_lds > sort_lds ? turn_lds : sort_lds;
+  if (p.vec_b && p.D % 4 == 0) hipLaunchKernelGGL((embed_sort_kernel<ST, true>), grid, block, lds, s, p, ranges, range);
+  else hipLaunchKernelGGL((embed_sort_kernel<ST, false>), grid, block, lds, s, p, ranges, range);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   return p.vec_d ? run_sums<ST, 4>(p, s) : run_sums<ST, 1>(p, s);
