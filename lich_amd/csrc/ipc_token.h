@@ -86,9 +86,8 @@ struct TokenProblem {
 // 0: sizes that the kernels do not take
 long long token_workspace_bytes(int V, int D, int B, int storage, int act, bool update);
 hipError_t launch_token(const TokenProblem& p, int storage, hipStream_t s);
-// A small one in one workgroup, without a workspace: up to so many V D B.
-constexpr long long kTokenSmall = 1 << 18;
-bool token_small(int V, int D, int B, bool update);
+// A small one in one workgroup, without a workspace.
+bool token_small(int V, int D, int B);
 hipError_t launch_token_small(const TokenProblem& p, int storage, hipStream_t s);
 
 }  // namespace ipc

@@ -436,5 +436,16 @@ hipError_t run_tile(const TokenGemm& p, hipStream_t s) {
   return hipLaunchKernel(fn, dim3((unsigned)tiles), dim3(WGM * WGN * 64), args, smem, s);
 }
 
+// 64 x 64 tiles: as many stages as leave two workgroups a CU (fp32: one, or two of three stages
+// where there are more workgroups than CUs), since a step of few workgroups is as long as
+// a load takes over the stages in flight.
+template <typename OT, bool SPLIT, int MODE, bool TWO, int WGM, int WGN>
+hipError_t run_narrow(const TokenGemm& p, hipStream_t s) {
+  constexpr int BNC = TWO ? 32 : 64;
+  const long long tiles = ((p.M + 63LL) / 64) * ((p.N + BNC - 1LL) / BNC) * (MODE == TOKEN_GRAD ? p.slices : 1);
+  if (SPLIT && tiles > 256) return run_tile<OT, SPLIT, MODE, TWO, 64, 64, WGM, WGN, 3>(p, s);
+  return run_tile<OT, SPLIT, MODE, TWO, 64, 64, WGM, WGN, SPLIT ? 6 : 8>(p, s);
+}
+
 }  // namespace token
 }  // namespace ipc

@@ -10,8 +10,8 @@ hipError_t run(const TokenGemm& p, int tile, hipStream_t s) {
     if (tile == TILE_256) return token::run_tile<OT, SPLIT, TOKEN_KEEP, false, 256, 256, 2, 4>(p, s);
   }
   if (tile == TILE_128) return token::run_tile<OT, SPLIT, TOKEN_KEEP, false, 128, 128, 2, 2, SPLIT ? 3 : 4>(p, s);
-  if (tile == TILE_128_64) return token::run_tile<OT, SPLIT, TOKEN_KEEP, false, 128, 64, 2, 2>(p, s);
-  return token::run_tile<OT, SPLIT, TOKEN_KEEP, false, 64, 64, 2, 2, SPLIT ? 3 : 4>(p, s);
+  if (tile == TILE_128_64) return token::run_tile<OT, SPLIT, TOKEN_KEEP, false, 128, 64, 2, 2, SPLIT ? 4 : 6>(p, s);
+  return token::run_narrow<OT, SPLIT, TOKEN_KEEP, false, 2, 2>(p, s);
 }
 
 }  // namespace

@@ -164,10 +164,12 @@ __global__ void __launch_bounds__(kThreads) token_small_kernel(const TokenProble
 
 }  // namespace
 
-bool token_small(int V, int D, int B, bool update) {
-  (void)update;
-  return (long long)V * D <= 1 << 16 && (long long)D * B <= 1 << 16 && (long long)V * B <= 1 << 16 &&
-         (long long)V * D * B <= kTokenSmall && small_lds(V, D, B) <= kLds;
+// One workgroup is slow at anything long: us, in one / the launches of the general path, fp32:
+// 10 x 64 x 128 (V, D, B) 11.5 / 21.6; 64 x 64 x 64 18 / 23.6; 10 x 256 x 100 30.6 / 26.
+bool token_small(int V, int D, int B) {
+  constexpr long long most = 1 << 14;
+  return (long long)V * D <= most && (long long)D * B <= most && (long long)V * B <= most &&
+         (long long)V * D * B <= 1 << 18 && small_lds(V, D, B) <= kLds;
 }
 
 template <typename ST, int ACT>

@@ -461,7 +461,7 @@ long long token_workspace_bytes(int V, int D, int B, int storage, int act, bool 
 }
 
 hipError_t launch_token(const TokenProblem& p, int storage, hipStream_t s) {
-  if (token_small(p.V, p.D, p.B, p.g != nullptr)) return launch_token_small(p, storage, s);
+  if (token_small(p.V, p.D, p.B)) return launch_token_small(p, storage, s);
   if (storage == DT_F32) return by_act<float, bf16, 3>(p, storage, s);
   return storage == DT_F16 ? by_act<f16, f16, 1>(p, storage, s) : by_act<bf16, bf16, 1>(p, storage, s);
 }

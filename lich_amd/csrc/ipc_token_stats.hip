@@ -11,8 +11,8 @@ hipError_t run(const TokenGemm& p, int tile, hipStream_t s) {
     if (tile == TILE_256) return token::run_tile<OT, SPLIT, TOKEN_STATS, TWO, 256, 256, 2, 4>(p, s);
   }
   if (tile == TILE_128) return token::run_tile<OT, SPLIT, TOKEN_STATS, TWO, 128, 128, 2, 2, SPLIT ? 3 : 4>(p, s);
-  if (tile == TILE_128_64) return token::run_tile<OT, SPLIT, TOKEN_STATS, TWO, 128, 64, M, N>(p, s);
-  return token::run_tile<OT, SPLIT, TOKEN_STATS, TWO, 64, 64, 2, N, SPLIT ? 3 : 4>(p, s);
+  if (tile == TILE_128_64) return token::run_tile<OT, SPLIT, TOKEN_STATS, TWO, 128, 64, M, N, SPLIT ? 4 : 6>(p, s);
+  return token::run_narrow<OT, SPLIT, TOKEN_STATS, TWO, 2, N>(p, s);
 }
 
 }  // namespace
