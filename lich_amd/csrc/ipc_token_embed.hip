@@ -320,13 +320,14 @@ __device__ __forceinline__ void add_to_piece(ST* to, const Piece<ST, W>& old, fl
 template <typename ST, int W>
 __global__ void __launch_bounds__(256) embed_run_kernel(const EmbedUpdate p) {
   const int run = blockIdx.x, N = p.C * p.B, lane = threadIdx.x & 63;
-  const int d = (blockIdx.y * blockDim.x + threadIdx.x) * W, first = run * EMBED_RUN;
+  // (threads past the last feature go along with the first: their lanes hold places too)
+  const int mine = (blockIdx.y * blockDim.x + threadIdx.x) * W, d = mine < p.D ? mine : 0, first = run * EMBED_RUN;
   // lane i: the id of the place before the run's i-th, and the i-th's row of G
   const int at = first - 1 + lane;
   const int keys = at >= 0 && at <= N ? p.key[at] : -1;
   const int orders = lane < EMBED_RUN && first + lane < N ? p.order[first + lane] : 0;
   auto key = [&](int i) { return __builtin_amdgcn_readlane(keys, i + 1); };
-  if (key(0) < 0 || d >= p.D) return;
+  if (key(0) < 0) return;
   const ST* rows = static_cast<const ST*>(p.rows) + d;
   ST* table = static_cast<ST*>(p.table) + d;
   // every row of G and of the table, none stored before all are read (a place without an id: any row)
@@ -348,7 +349,8 @@ __global__ void __launch_bounds__(256) embed_run_kernel(const EmbedUpdate p) {
     const bool on = key(u + 1) == id;
     if (on && u + 1 < EMBED_RUN) continue;
     // the run's first and ended, or its last and not: a part
-    if (over || on) put_piece<W>(p.part + ((long long)run * 2 + (over ? 0 : 1)) * p.D + d, sum);
+    if (mine >= p.D) {
+    } else if (over || on) put_piece<W>(p.part + ((long long)run * 2 + (over ? 0 : 1)) * p.D + d, sum);
     else add_to_piece<W>(table + (long long)id * p.D, old[u], p.alpha, sum);
     over = false;
 #pragma unroll

@@ -189,7 +189,7 @@ __device__ __forceinline__ void lay_rows(const Rows& p, unsigned block) {
 template <typename ST, typename OT, int TERMS, int ACT>
 __global__ void __launch_bounds__(256) token_lay_kernel(const States x, const Rows w, unsigned states) {
   if (blockIdx.x < states) lay_states<ST, OT, TERMS, ACT>(x, blockIdx.x);
-  else lay_rows<ST, OT, TERMS>(w, blockIdx.x - states);
+  else lay_rows<ST, OT, TERMS == 2 ? 1 : TERMS>(w, blockIdx.x - states);  // (W has no second term)
 }
 
 // ---------------------------------------------------------------- a column's tiles

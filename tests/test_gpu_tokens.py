@@ -363,3 +363,63 @@ def test_calls_in_a_graph_and_on_another_stream(name):
             for a, b in ((s.table, eager.table), (s.w, eager.w), (s.x, eager.x), (s.g, eager.g), (s.loss, eager.loss), (s.after, eager.after)):
                 assert torch.equal(a, b), step
     assert float(eager.loss.mean()) != float(eager.after.mean())
+
+
+# --------------------------------------------------- nothing written beside the tensors
+class Fenced:
+    """Tensors inside one larger buffer with a known value between and behind them."""
+
+    def __init__(self, parts, room):
+        offsets, at = [], room
+        for shape, dtype in parts:
+            size = torch.empty((), dtype=dtype).element_size()
+            n = 1
+            for v in shape:
+                n *= v
+            at = -(-at // 256) * 256
+            offsets.append((at, n * size))
+            at += n * size + room
+        self.buffer = torch.full((at,), 0x5A, dtype=torch.uint8, device=DEV)
+        self.views = [self.buffer[o:o + b].view(dtype).reshape(shape) for (o, b), (shape, dtype) in zip(offsets, parts)]
+        self.mine = torch.zeros(at, dtype=torch.bool, device=DEV)
+        for o, b in offsets:
+            self.mine[o:o + b] = True
+
+    def intact(self):
+        return bool((self.buffer[~self.mine] == 0x5A).all())
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("activation", ["identity", "tanh"])
+@pytest.mark.parametrize("V,D,B", [(2, 1, 1), (10, 64, 128), (999, 77, 3), (300, 131, 90), (26240, 1, 70), (7001, 65, 1), (700, 200, 300),
+                                   (164, 2, 188), (5000, 35, 520)])
+def test_softmax_calls_stay_inside_their_tensors(V, D, B, activation, name):
+    """Also inside the workspace's stated size; room behind each as large as the workspace itself."""
+    dt = TYPES[name]
+    x, w, t = softmax_case(V, D, B, dt, V + D)
+    k, score = tokens.build_token_update(V, D, B, activation, dt, 0.1), tokens.build_token_loss(V, D, B, activation, dt)
+    for call, inputs in ((k, 5), (score, 4)):
+        f = Fenced([((D, B), dt), ((V, D), dt), ((B,), torch.int64), ((B,), torch.float32), ((D, B), dt),
+                    ((call.workspace_bytes,), torch.uint8)], max(4096, call.workspace_bytes))
+        for view, value in zip(f.views, (x, w, t)):
+            view.copy_(value)
+        call(*f.views[:inputs], workspace=f.views[5])
+        assert f.intact()
+        assert bool(torch.isfinite(f.views[3]).all())
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("V,D,C,B", [(5, 3, 1, 1), (130, 65, 3, 17), (47, 2, 12, 290), (300, 1, 3, 500), (3000, 131, 5, 301), (70, 64, 3, 400)])
+def test_embedding_calls_stay_inside_their_tensors(V, D, C, B, name):
+    dt, g = TYPES[name], gen(V)
+    k = tokens.build_embedding_update(V, D, C, B, dt, 0.1)
+    f = Fenced([((V, D), dt), ((C, B), torch.int64), ((C * D, B), dt), ((k.workspace_bytes,), torch.uint8)], max(4096, k.workspace_bytes))
+    f.views[0].copy_(randn((V, D), g, dt))
+    f.views[1].copy_(some_ids(V, (C, B), g))
+    tokens.build_embedding(V, D, C, B, dt, 2.0)(f.views[1], f.views[0], f.views[2])
+    assert f.intact()
+    k(f.views[0], f.views[1], f.views[2], workspace=f.views[3])
+    assert f.intact()
+    rng = torch.tensor([1, 2], device=DEV)
+    tokens.build_dropout(C * D, B, dt, 0.3)(f.views[2], rng, f.views[2])
+    assert f.intact()
