@@ -58,6 +58,9 @@ inline EmbedLayout embed_layout(int D, int C, int B, int element) {
   return l;
 }
 hipError_t launch_embedding_update(const EmbedUpdate& p, int storage, hipStream_t s);
+// Places of N ids sorted by id, ties in their order: order [N], key [N + 1] as in EmbedUpdate; slot
+// [V]: the first sorted position of each id, -1 of those that do not occur.
+hipError_t launch_sort_places(const long long* ids, int N, int V, int* order, int* key, int* slot, hipStream_t s);
 
 // -------------------------------------------------------------------- dropout
 struct DropoutProblem {

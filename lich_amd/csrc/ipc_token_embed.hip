@@ -137,7 +137,7 @@ constexpr int SORT_WAVES = 16, SORT_HELD = 8;
 // ids in one range: 56 us, in 64: 11.  But few workgroups for few places: 1505 places of 1531
 // ids, 256 ranges 10.6 us, 24 6.2.)
 inline int sort_range(int V, int N) {
-  const int most = N / 32 < 256 ? N / 32 : 256, r = (V + most - 1) / most;
+  const int most = N < 64 ? 1 : N / 32 < 256 ? N / 32 : 256, r = (V + most - 1) / most;
   return r > 512 ? 512 : r;
 }
 
@@ -191,19 +191,15 @@ __device__ void transpose_rows(const EmbedUpdate& p, int block, ST* tile) {
   }
 }
 
-template <typename ST, bool VEC>
-__global__ void __launch_bounds__(SORT_WAVES * 64) embed_sort_kernel(const EmbedUpdate p, int ranges, int range) {
-  extern __shared__ __align__(16) int lds[];
-  if ((int)blockIdx.x >= ranges) {
-    transpose_rows<ST, VEC>(p, blockIdx.x - ranges, reinterpret_cast<ST*>(lds));
-    return;
-  }
+// Range `block` of `ranges`; lds: SORT_WAVES * range.
+__device__ __forceinline__ void sort_places(const long long* ids, int N, int V, int* order, int* key, int* slot, int* lds, int block,
+                                            int ranges, int range) {
   __shared__ int before[SORT_WAVES], sums[SORT_WAVES];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int N = p.C * p.B, per = ((N + SORT_WAVES - 1) / SORT_WAVES + 63) / 64 * 64;
+  const int per = ((N + SORT_WAVES - 1) / SORT_WAVES + 63) / 64 * 64;
   const int first = wave * per, last = first + per < N ? first + per : N;
-  const long long lo = (long long)blockIdx.x * range;
-  const long long hi = lo + range < p.V ? lo + range : p.V;
+  const long long lo = (long long)block * range;
+  const long long hi = lo + range < V ? lo + range : V;
   int* mine = lds + wave * range;
   for (int i = tid; i < SORT_WAVES * range; i += SORT_WAVES * 64) lds[i] = 0;
   __syncthreads();
@@ -215,7 +211,7 @@ __global__ void __launch_bounds__(SORT_WAVES * 64) embed_sort_kernel(const Embed
 #pragma unroll
     for (int u = 0; u < SORT_HELD; ++u) {
       const int i = i0 + u * 64 + lane;
-      id[u] = i < last ? p.ids[i] : -1;
+      id[u] = i < last ? ids[i] : -1;
     }
 #pragma unroll
     for (int u = 0; u < SORT_HELD; ++u) {
@@ -254,6 +250,7 @@ __global__ void __launch_bounds__(SORT_WAVES * 64) embed_sort_kernel(const Embed
       if (w < wave) at += sums[w];
       base += sums[w];
     }
+    if (slot && r < range && lo + r < V) slot[lo + r] = total > 0 ? at : -1;
     if (r < range)
       for (int w = 0; w < SORT_WAVES; ++w) {
         const int n = lds[w * range + r];
@@ -262,8 +259,8 @@ __global__ void __launch_bounds__(SORT_WAVES * 64) embed_sort_kernel(const Embed
       }
     __syncthreads();
   }
-  if (blockIdx.x == ranges - 1)  // behind the last place with an id
-    for (int i = base + tid; i <= N; i += SORT_WAVES * 64) p.key[i] = -1;
+  if (block == ranges - 1)  // behind the last place with an id
+    for (int i = base + tid; i <= N; i += SORT_WAVES * 64) key[i] = -1;
   for (int i0 = first; i0 < last; i0 += 64 * SORT_HELD) {
     if (last - first > 64 * SORT_HELD) fetch(i0, false);
     unsigned many = 0;  // bit u: the u-th 64 have some in the range
@@ -282,8 +279,8 @@ __global__ void __launch_bounds__(SORT_WAVES * 64) embed_sort_kernel(const Embed
         const int at = mine[which];
         if (own == which) {
           const int to = at + __popcll(same & ((1ull << lane) - 1));
-          p.order[to] = i0 + u * 64 + lane;
-          p.key[to] = (int)(lo + which);
+          order[to] = i0 + u * 64 + lane;
+          key[to] = (int)(lo + which);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         if (lane == 0) mine[which] = at + __popcll(same);
@@ -292,6 +289,19 @@ __global__ void __launch_bounds__(SORT_WAVES * 64) embed_sort_kernel(const Embed
       }
     }
   }
+}
+
+template <typename ST, bool VEC>
+__global__ void __launch_bounds__(SORT_WAVES * 64) embed_sort_kernel(const EmbedUpdate p, int ranges, int range) {
+  extern __shared__ __align__(16) int lds[];
+  if ((int)blockIdx.x >= ranges) transpose_rows<ST, VEC>(p, blockIdx.x - ranges, reinterpret_cast<ST*>(lds));
+  else sort_places(p.ids, p.C * p.B, p.V, p.order, p.key, nullptr, lds, blockIdx.x, ranges, range);
+}
+
+__global__ void __launch_bounds__(SORT_WAVES * 64) sort_places_kernel(const long long* ids, int N, int V, int* order, int* key, int* slot,
+                                                                      int ranges, int range) {
+  extern __shared__ __align__(16) int lds[];
+  sort_places(ids, N, V, order, key, slot, lds, blockIdx.x, ranges, range);
 }
 
 // A run of EMBED_RUN sorted places, 4 features a thread.  Ids that begin and end in the
@@ -436,6 +446,13 @@ hipError_t run_update(const EmbedUpdate& p, hipStream_t s) {
 hipError_t launch_embedding(const EmbedProblem& p, int storage, hipStream_t s) {
   if (storage == 0) return run_embed<float>(p, s);
   return storage == 1 ? run_embed<f16>(p, s) : run_embed<bf16>(p, s);
+}
+
+hipError_t launch_sort_places(const long long* ids, int N, int V, int* order, int* key, int* slot, hipStream_t s) {
+  const int range = sort_range(V, N), ranges = (int)(((long long)V + range - 1) / range);
+  hipLaunchKernelGGL(sort_places_kernel, dim3((unsigned)ranges), dim3(SORT_WAVES * 64), SORT_WAVES * range * 4, s, ids, N, V, order, key, slot,
+                     ranges, range);
+  return hipGetLastError();
 }
 
 hipError_t launch_embedding_update(const EmbedUpdate& p, int storage, hipStream_t s) {

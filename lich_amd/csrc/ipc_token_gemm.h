@@ -2,7 +2,7 @@
 //
 //   TOKEN_STATS   Z[v][n] = sum_d W[v][d] F[d][n], of which only each tile's largest value and
 //                 sum of exponentials a column are kept, and the target's logit
-//   TOKEN_KEEP    that, and the exponentials, as KEPT[n][v] relative to their tile's largest
+//   TOKEN_KEEP    that, and the exponentials, as KEPT[n][v] relative to their wave's largest
 //   TOKEN_ERROR   the same products again; e = onehot - softmax(Z), rounded to the operand
 //                 type and stored transposed, ET[n][v]
 //   TOKEN_GRAD    P[d][n] = sum_v W[v][d] e[v][n]     (a slice of the vocabulary a workgroup)
@@ -57,11 +57,15 @@ struct TokenGemm {
   // STATS, KEEP, ERROR
   const long long* targets; int first, V;  // first: of the piece's rows
   float* target_logit;
+  const float* loss;               // ERROR
+  const int* slot;                 // WEIGHT, or nullptr: of each row, its row in hot (-1: none), which the sum begins with
+  const float* hot; int hot_ld;
   const float2* stats;             // ERROR: of each column, largest logit and 1 / sum of exp(z - largest)
 };
 // storage: 0 (three bf16 terms), 1, 2
 hipError_t launch_token_stats(const TokenGemm& p, int storage, int tile, bool two, hipStream_t s);
-hipError_t launch_token_keep(const TokenGemm& p, int storage, int tile, hipStream_t s);
+// two: f(X) in two terms, the exponentials kept in fp32
+hipError_t launch_token_keep(const TokenGemm& p, int storage, int tile, bool two, hipStream_t s);
 hipError_t launch_token_error(const TokenGemm& p, int storage, int tile, hipStream_t s);
 hipError_t launch_token_grad(const TokenGemm& p, int storage, int tile, hipStream_t s);
 
@@ -81,13 +85,14 @@ inline int token_fix_rows(int D, bool vec) { return vec ? (D + 15) / 16 : (D + 3
 hipError_t launch_token_finish(const TokenFinish& p, int storage, hipStream_t s);
 // W's update, and (f) the gradient's last step, which needs no more than that does: in one
 // launch where both are small.
-hipError_t launch_token_weight(const TokenGemm& p, const TokenFinish* f, int storage, hipStream_t s);
+// terms: of both operands in 16-bit storage, 1 or 2
+hipError_t launch_token_weight(const TokenGemm& p, const TokenFinish* f, int storage, int terms, hipStream_t s);
 
 namespace token {
 
 using namespace mx;
 
-// a and b terms of the products of three terms each, smallest first
+// a and b terms of the products of three terms each, smallest first (of two terms: the last three)
 constexpr int PRODUCTS = 6, TERM_A[PRODUCTS] = {2, 1, 0, 1, 0, 0}, TERM_B[PRODUCTS] = {0, 1, 2, 0, 1, 0};
 
 template <bool EXACT>
@@ -97,16 +102,20 @@ __device__ __forceinline__ float exp_of(float x) {
   return __builtin_amdgcn_exp2f(x * 1.44269504f);
 }
 
+// The error at the target, 1 - p, without its cancellation.
+__device__ __forceinline__ float target_error(float loss, float scale) { return -expm1f(-loss) * scale; }
+
 // Workgroup `block` of `blocks` of a product.
-template <typename OT, bool SPLIT, int MODE, bool TWO, int BM, int BN, int WGM, int WGN, int ST>
+template <typename OT, int TERMS, int MODE, bool TWO, int BM, int BN, int WGM, int WGN, int ST>
 __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* smem, int block, int blocks) {
   using MF = Mfma32<OT>;
   typedef typename MF::operand V;
   constexpr bool MN = MODE == TOKEN_GRAD || MODE == TOKEN_WEIGHT, COLUMNS = !MN;
   constexpr int NW = WGM * WGN, WTM = BM / WGM, WTN = BN / WGN, RM = WTM / 32, RN = WTN / 32;
   constexpr int RNC = TWO ? RN / 2 : RN, BNC = TWO ? BN / 2 : BN;  // blocks and columns of different n
-  constexpr int TERMS = SPLIT ? 3 : 1, A_BYTES = BM * 64, B_BYTES = BN * 64, STAGE = TERMS * (A_BYTES + B_BYTES);
-  static_assert(!TWO || (MODE == TOKEN_STATS && RN % 2 == 0), "two terms of f(X)");
+  constexpr bool SPLIT = TERMS == 3, FINE = SPLIT || (MODE == TOKEN_KEEP && TWO);  // FINE: kept in fp32
+  constexpr int A_BYTES = BM * 64, B_BYTES = BN * 64, STAGE = TERMS * (A_BYTES + B_BYTES);
+  static_assert(!TWO || ((MODE == TOKEN_STATS || MODE == TOKEN_KEEP) && TERMS == 1 && RN % 2 == 0), "two terms of f(X)");
   constexpr int IA = A_BYTES / 1024 / NW, IB = B_BYTES / 1024 / NW, LPS = TERMS * (IA + IB);  // LDS-DMA loads per wave and stage
   static_assert(IA * 1024 * NW == A_BYTES && IB * 1024 * NW == B_BYTES, "tile / waves");
 
@@ -180,6 +189,25 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
     for (int j = 0; j < RN; ++j)
 #pragma unroll
       for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
+  if constexpr (MODE == TOKEN_WEIGHT && TERMS == 1) {  // what the targets' rows begin with
+    if (p.slot) {
+#pragma unroll
+      for (int i = 0; i < RM; ++i) {
+        const int m = m0 + wm * WTM + i * 32 + lr, at = m < M ? p.slot[m] : -1;
+        if (!__any(at >= 0)) continue;
+#pragma unroll
+        for (int j = 0; j < RN; ++j)
+#pragma unroll
+          for (int q = 0; q < 16; q += 4) {
+            const int n = n0 + wn * WTN + j * 32 + 2 * q + 4 * lk;
+            if (at >= 0 && n < p.hot_ld) {
+              const float4 v = *reinterpret_cast<const float4*>(p.hot + (long long)at * p.hot_ld + n);
+              acc[i][j][q] = v.x; acc[i][j][q + 1] = v.y; acc[i][j][q + 2] = v.z; acc[i][j][q + 3] = v.w;
+            }
+          }
+      }
+    }
+  }
 
   // fragments of 16 k (half s of a stage): row / column lr of a 32-wide block, k 8 lk .. + 7
   const int g4 = lane >> 4, li = lane & 15;
@@ -233,7 +261,7 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
   auto half = [&](auto SV, const unsigned char* next, unsigned char* fill) {
     constexpr int S = decltype(SV)::value, O = S ^ 1;
     constexpr int L0 = S == 0 ? 0 : (LPS + 1) / 2, L1 = S == 0 ? (LPS + 1) / 2 : LPS;
-    constexpr int EACH = RM * RN, NM = (SPLIT ? PRODUCTS : 1) * EACH, NR = TERMS * (RM + RN);
+    constexpr int EACH = RM * RN, FIRST = TERMS == 3 ? 0 : TERMS == 2 ? 3 : 5, NM = (PRODUCTS - FIRST) * EACH, NR = TERMS * (RM + RN);
 #pragma unroll
     for (int q = 0; q < NM; ++q) {
 #pragma unroll
@@ -243,7 +271,7 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
       for (int l = L0; l < L1; ++l)
         if ((l - L0) * NM / (L1 - L0) == q) load(l, fill, sa, sb);
       const int i = q % EACH / RN, j = q % RN;
-      const V a = fa[S][SPLIT ? TERM_A[q / EACH] : 0][i], b = fb[S][SPLIT ? TERM_B[q / EACH] : 0][j];
+      const V a = fa[S][TERM_A[FIRST + q / EACH]][i], b = fb[S][TERM_B[FIRST + q / EACH]][j];
       acc[i][j] = COLUMNS ? MF::run(a, b, acc[i][j]) : MF::run(b, a, acc[i][j]);
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -283,11 +311,11 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
   auto store_columns = [&](auto form, int j) {
     constexpr int FORM = decltype(form)::value;
     typedef typename std::conditional<FORM == 2, float, unsigned short>::type U;
-    constexpr int LD = WTM + (FORM == 2 ? 4 : 8), TERMS = FORM == 0 && SPLIT ? 3 : 1, PER = 16 / sizeof(U);
+    constexpr int LD = WTM + (FORM == 2 ? 4 : 8), PARTS = FORM == 0 && SPLIT ? 3 : 1, PER = 16 / sizeof(U);
     U* es = reinterpret_cast<U*>(smem) + w * 32 * LD;
     U* out = static_cast<U*>(FORM == 0 ? p.out : p.kept);
 #pragma unroll
-    for (int term = 0; term < TERMS; ++term) {
+    for (int term = 0; term < PARTS; ++term) {
 #pragma unroll
       for (int i = 0; i < RM; ++i)
 #pragma unroll
@@ -315,7 +343,7 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
       for (int u = 0; u < PASSES; ++u) {
         const int r = u * RPP + lane / LPR, c = lane % LPR * PER;
         const uint4 v = *reinterpret_cast<const uint4*>(es + r * LD + c);
-        const long long row = n0 + wn * WTN + j * 32 + r;
+        const long long row = n0 + wn * WTN / (TWO ? 2 : 1) + j * 32 + r;
         const int col = m0 + wm * WTM + c;
         if (row < p.out_rows && col < p.out_ld) *reinterpret_cast<uint4*>(out + term * p.out_term + row * p.out_ld + col) = v;
       }
@@ -361,12 +389,12 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
       for (int i = 0; i < RM; ++i)
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
-          acc[i][j][q] = exp_of<SPLIT>(acc[i][j][q] - from);
+          acc[i][j][q] = exp_of<FINE>(acc[i][j][q] - from);
           sum += acc[i][j][q];
         }
       sum += __shfl_xor(sum, 32);
       if (lk == 0 && n < N && mw < M) static_cast<float2*>(p.out)[(long long)(mw / WTM) * N + n] = make_float2(top, sum);
-      if constexpr (MODE == TOKEN_KEEP) store_columns(std::integral_constant<int, SPLIT ? 2 : 1>{}, j);
+      if constexpr (MODE == TOKEN_KEEP) store_columns(std::integral_constant<int, FINE ? 2 : 1>{}, j);
       __builtin_amdgcn_sched_barrier(0);
     }
   } else if constexpr (MODE == TOKEN_ERROR) {
@@ -379,7 +407,7 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
       const int own = (int)to - 4 * lk;
       const bool hit = real && to >= 0 && to < WTM && (own & 4) == 0;
       const float2 st = real ? p.stats[n] : make_float2(0.0f, 0.0f);
-      const float share = -st.y * p.scal;
+      const float share = -st.y * p.scal, at_target = real ? target_error(p.loss[n], p.scal) : 0.0f;
 #pragma unroll
       for (int i = 0; i < RM; ++i)
 #pragma unroll
@@ -388,7 +416,8 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
 #pragma unroll
         for (int i = 0; i < RM; ++i)
 #pragma unroll
-          for (int q = 0; q < 16; ++q) acc[i][j][q] += hit && own == i * 32 + 8 * (q >> 2) + (q & 3) ? p.scal : 0.0f;
+          for (int q = 0; q < 16; ++q)
+            acc[i][j][q] = hit && own == i * 32 + 8 * (q >> 2) + (q & 3) ? at_target : acc[i][j][q];
       }
       if (m0 + BM > M) mask_rows(j, 0.0f);
       store_columns(std::integral_constant<int, 0>{}, j);
@@ -407,26 +436,26 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
   }
 }
 
-template <typename OT, bool SPLIT, int MODE, bool TWO, int BM, int BN, int WGM, int WGN, int ST>
+template <typename OT, int TERMS, int MODE, bool TWO, int BM, int BN, int WGM, int WGN, int ST>
 __global__ void __launch_bounds__(WGM * WGN * 64) token_gemm_kernel(const TokenGemm p) {
   extern __shared__ __align__(16) unsigned char smem[];
-  product_tile<OT, SPLIT, MODE, TWO, BM, BN, WGM, WGN, ST>(p, smem, blockIdx.x, gridDim.x);
+  product_tile<OT, TERMS, MODE, TWO, BM, BN, WGM, WGN, ST>(p, smem, blockIdx.x, gridDim.x);
 }
 
-template <bool SPLIT, int MODE, int BM, int BN, int WGM, int WGN, int ST>
+template <int TERMS, int MODE, bool TWO, int BM, int BN, int WGM, int WGN, int ST>
 constexpr int tile_lds() {
-  constexpr int NW = WGM * WGN, ring = ST * (SPLIT ? 3 : 1) * (BM + BN) * 64;
+  constexpr int NW = WGM * WGN, ring = ST * TERMS * (BM + BN) * 64;
   constexpr int epi = MODE == TOKEN_STATS ? 0
-                      : MODE == TOKEN_ERROR || (MODE == TOKEN_KEEP && !SPLIT) ? NW * 32 * (BM / WGM + 8) * 2
+                      : MODE == TOKEN_ERROR || (MODE == TOKEN_KEEP && TERMS == 1 && !TWO) ? NW * 32 * (BM / WGM + 8) * 2
                       : MODE == TOKEN_KEEP ? NW * 32 * (BM / WGM + 4) * 4 : NW * 32 * (BN / WGN + 4) * 4;
   return epi > ring ? epi : ring;
 }
 
-template <typename OT, bool SPLIT, int MODE, bool TWO, int BM, int BN, int WGM, int WGN, int ST = 4>
+template <typename OT, int TERMS, int MODE, bool TWO, int BM, int BN, int WGM, int WGN, int ST = 4>
 hipError_t run_tile(const TokenGemm& p, hipStream_t s) {
-  constexpr int smem = tile_lds<SPLIT, MODE, BM, BN, WGM, WGN, ST>();
+  constexpr int smem = tile_lds<TERMS, MODE, TWO, BM, BN, WGM, WGN, ST>();
   static_assert(smem <= 160 * 1024, "LDS");
-  const void* fn = reinterpret_cast<const void*>(&token_gemm_kernel<OT, SPLIT, MODE, TWO, BM, BN, WGM, WGN, ST>);
+  const void* fn = reinterpret_cast<const void*>(&token_gemm_kernel<OT, TERMS, MODE, TWO, BM, BN, WGM, WGN, ST>);
   static const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != hipSuccess) return e;
   constexpr int BNC = TWO ? BN / 2 : BN;
@@ -439,12 +468,12 @@ hipError_t run_tile(const TokenGemm& p, hipStream_t s) {
 // 64 x 64 tiles: as many stages as leave two workgroups a CU (fp32: one, or two of three stages
 // where there are more workgroups than CUs), since a step of few workgroups is as long as
 // a load takes over the stages in flight.
-template <typename OT, bool SPLIT, int MODE, bool TWO, int WGM, int WGN>
+template <typename OT, int TERMS, int MODE, bool TWO, int WGM, int WGN>
 hipError_t run_narrow(const TokenGemm& p, hipStream_t s) {
   constexpr int BNC = TWO ? 32 : 64;
   const long long tiles = ((p.M + 63LL) / 64) * ((p.N + BNC - 1LL) / BNC) * (MODE == TOKEN_GRAD ? p.slices : 1);
-  if (SPLIT && tiles > 256) return run_tile<OT, SPLIT, MODE, TWO, 64, 64, WGM, WGN, 3>(p, s);
-  return run_tile<OT, SPLIT, MODE, TWO, 64, 64, WGM, WGN, SPLIT ? 6 : 8>(p, s);
+  if (TERMS == 3 && tiles > 256) return run_tile<OT, TERMS, MODE, TWO, 64, 64, WGM, WGN, 3>(p, s);
+  return run_tile<OT, TERMS, MODE, TWO, 64, 64, WGM, WGN, TERMS == 3 ? 6 : 8 / TERMS>(p, s);
 }
 
 }  // namespace token

@@ -4,21 +4,21 @@
 namespace ipc {
 namespace {
 
-template <typename OT, bool SPLIT>
+template <typename OT, int TERMS>
 hipError_t grad(const TokenGemm& p, int tile, hipStream_t s) {
-  if constexpr (!SPLIT) {
-    if (tile == 256) return token::run_tile<OT, SPLIT, TOKEN_GRAD, false, 256, 256, 2, 2>(p, s);
+  if constexpr (TERMS == 1) {
+    if (tile == 256) return token::run_tile<OT, TERMS, TOKEN_GRAD, false, 256, 256, 2, 2>(p, s);
   }
-  if (tile >= 128 && p.N > 64) return token::run_tile<OT, SPLIT, TOKEN_GRAD, false, 128, 128, 2, 2, SPLIT ? 3 : 4>(p, s);
-  if (tile == 128) return token::run_tile<OT, SPLIT, TOKEN_GRAD, false, 128, 64, 2, 2, SPLIT ? 4 : 6>(p, s);
-  return token::run_narrow<OT, SPLIT, TOKEN_GRAD, false, 2, 2>(p, s);
+  if (tile >= 128 && p.N > 64) return token::run_tile<OT, TERMS, TOKEN_GRAD, false, 128, 128, 2, 2, TERMS == 3 ? 3 : 4>(p, s);
+  if (tile == 128) return token::run_tile<OT, TERMS, TOKEN_GRAD, false, 128, 64, 2, 2, TERMS == 3 ? 4 : 6>(p, s);
+  return token::run_narrow<OT, TERMS, TOKEN_GRAD, false, 2, 2>(p, s);
 }
 
 }  // namespace
 
 hipError_t launch_token_grad(const TokenGemm& p, int storage, int tile, hipStream_t s) {
-  if (storage == 0) return grad<bf16, true>(p, tile, s);
-  return storage == 1 ? grad<f16, false>(p, tile, s) : grad<bf16, false>(p, tile, s);
+  if (storage == 0) return grad<bf16, 3>(p, tile, s);
+  return storage == 1 ? grad<f16, 1>(p, tile, s) : grad<bf16, 1>(p, tile, s);
 }
 
 }  // namespace ipc

@@ -20,11 +20,19 @@
 // not much dearer below.  Kept in fp16 times 2^15: 2^-12 of the value, down to 2^-29 of the
 // part's largest, and so finer than the error's own rounding except where both are fp16's.
 //
-// f(X) in 16 bits, where it is not exact there (all but identity and relu): the loss, which is
-// fp32, would be off by the logits' 2^-9 (2^-12).  The loss alone takes f(X) in two terms, both
-// in one tile, so that W is read once.  The update corrects it to first order instead,
-// by the gradient that it has: loss -= sum_d (W^T e)_d (f - rounded f)_d; what is left
-// is half the variance of the logits' rounding, 3e-6 of a loss for bf16 logits of deviation 3.
+// In 16 bits errors and, but for identity and relu, f(X) do not fit the operand type.  What
+// the results lose by it, and what is done:
+//   * G is rounded to the type itself: nothing.
+//   * the loss is fp32 and would be off by the logits' rounding, 2^-9 (2^-12).  The loss alone
+//     takes f(X) in two terms, both in one tile, so that W is read once.
+//   * W: a sum that is 2^-9 off rounds a weight in a few hundred of a target's row the other
+//     way, and the next loss differs by 1e-5 .. 1e-3.
+//   Small updates (kFineErrors, kFineWork: launches, not products, are their time) have f(X) and e in
+//   two terms and the exponentials in fp32: all of it is good to 2^-16 and better.  Large ones
+//   correct the loss to first order by the gradient that they have, loss -= sum_d (W^T e)_d (f - rounded
+//   f)_d (left: half the variance of the logits' rounding, 3e-6 of a loss for bf16 logits of deviation
+//   3), and make the errors at the targets, the ones near 1, good in fp32 (token_hot_kernel; left in the next
+//   loss: 2e-7 .. 2e-5).
 #include <algorithm>
 
 #include "ipc_token_gemm.h"
@@ -34,17 +42,22 @@ namespace {
 
 constexpr long long kPieceBytes = 1LL << 30;  // of a piece's errors, and of its rows of W where those are laid out
 constexpr long long kOperand = (1LL << 31) - 1;
+// 16-bit updates of at most so many errors and multiplications are `fine`.
+constexpr long long kFineErrors = 1LL << 23, kFineWork = 1LL << 31;
 
 struct Plan {
   int terms, Dp, Bk;
   bool copy;          // W laid out per piece: fp32, or 16-bit rows of an odd length
-  bool two;           // the loss alone: f(X) in two terms
-  bool fix;           // the update: the loss corrected
+  bool two;           // the logits with f(X) in two terms
+  bool fine;          // the update in 16 bits, small: errors and f(X) in two terms
+  bool mend;          // the update in 16 bits, large: targets' errors made good in fp32
+  bool fix;           // and the loss corrected
+  int ft_terms, f_terms, e_terms;
   bool keep;          // one piece, its exponentials kept
   int rows, Vp;       // of a piece (the last may have fewer), ET's row length
   int tile, unit;     // of the logits
   int grad_tile, slices;
-  long long f, ft, et, kept, ws, part, stats, logit, norm, fixes, bytes;  // offsets in the workspace
+  long long f, ft, et, kept, ws, part, stats, logit, norm, fixes, order, key, slot, hot, bytes;  // offsets in the workspace
 };
 
 bool make_plan(int V, int D, int B, int storage, int act, bool update, Plan& o) {
@@ -56,17 +69,23 @@ bool make_plan(int V, int D, int B, int storage, int act, bool update, Plan& o) 
   o.Bk = (int)up(B, 32);
   o.copy = storage == DT_F32 || D % 2 != 0;
   const bool inexact = storage != DT_F32 && act != ACT_IDENTITY && act != ACT_RELU;
-  o.two = inexact && !update;
-  o.fix = inexact && update;
-  const long long state = (long long)o.terms * o.Dp * o.Bk * 2;
-  if (state * (o.two ? 2 : 1) > kOperand) return false;
-  const long long row_w = 2LL * (o.copy ? o.terms * o.Dp : D), row_e = update ? 2LL * o.terms * o.Bk : 1;
+  const long long work = (long long)V * B;
+  o.fine = update && storage != DT_F32 && work <= kFineErrors && work * D <= kFineWork;
+  o.mend = update && storage != DT_F32 && !o.fine;
+  o.fix = inexact && o.mend;
+  o.two = o.fine || (inexact && !update);
+  o.ft_terms = storage == DT_F32 ? 3 : o.two || o.fix ? 2 : 1;
+  o.f_terms = o.e_terms = storage == DT_F32 ? 3 : o.fine ? 2 : 1;
+  const long long state = 2LL * o.Dp * o.Bk;
+  if (state * o.ft_terms > kOperand) return false;
+  const long long row_w = 2LL * (o.copy ? o.terms * o.Dp : D), row_e = update ? 2LL * o.e_terms * o.Bk : 1;
   long long rows = std::min((o.copy ? kPieceBytes : kOperand) / row_w, kPieceBytes / row_e) / 256 * 256;
   if (rows < 256) rows = 256;
   if (rows * std::max(row_w, row_e) > kOperand && std::min<long long>(rows, up(V, 32)) * std::max(row_w, row_e) > kOperand) return false;
   o.rows = (int)std::min<long long>(rows, V);
   o.Vp = (int)up(o.rows, 32);
   o.keep = update && o.rows == V && (storage != DT_F32 || (long long)o.Bk * o.Vp * 10 <= kPieceBytes);
+  if (o.fine && !o.keep) return false;  // (never: its errors are few)
   auto tiles = [&](long long m, long long n, long long e) { return ((m + e - 1) / e) * ((n + e - 1) / e); };
   const long long columns = o.two ? 2LL * B : B;
   if (columns <= 64) o.tile = o.rows >= 32768 ? TILE_128_64 : TILE_64;
@@ -83,30 +102,36 @@ bool make_plan(int V, int D, int B, int storage, int act, bool update, Plan& o) 
     at += up(bytes, 256);
     return here;
   };
-  o.ft = take(o.two ? 2 * state : state);
+  o.ft = take(state * o.ft_terms);
   o.logit = take(4LL * B);
   o.norm = take(8LL * B);
   o.stats = take(8LL * B * (((long long)V + o.unit - 1) / o.unit));
   if (o.copy) o.ws = take((long long)o.terms * o.Vp * o.Dp * 2);
   if (update) {
-    o.f = take(state);
-    o.et = take((long long)o.terms * o.Bk * o.Vp * 2);
+    o.f = take(state * o.f_terms);
+    o.et = take((long long)o.e_terms * o.Bk * o.Vp * 2);
     o.part = take(4LL * o.slices * D * B);
-    o.kept = storage != DT_F32 ? o.et : o.keep ? take(4LL * o.Bk * o.Vp) : 0;
+    o.kept = o.e_terms == 1 ? o.et : o.keep ? take(4LL * o.Bk * o.Vp) : 0;
     o.fixes = o.fix ? take(4LL * B * token_fix_rows(D, false)) : 0;
+    if (o.mend) {
+      o.order = take(4LL * B);
+      o.key = take(4LL * (B + 1));
+      o.slot = take(4LL * V);
+      o.hot = take(4LL * B * o.Dp);
+    }
   }
   o.bytes = at;
   return true;
 }
 
 // ------------------------------------------------------------------ f(X)
-// F [T][D][Bk] and FT [T][B][Dp] of X [D][B] in the operand type (T terms), zeros past
+// F [f_terms][D][Bk] and FT [T][B][Dp] of X [D][B] in the operand type (T terms), zeros past
 // the ends and in padded columns.
 struct States {
-  int D, B, V, Dp, Bk;
+  int D, B, V, Dp, Bk, f_terms;
   const void* x;
   const long long* targets;
-  unsigned short* f;  // or nullptr
+  unsigned short* f;  // its first f_terms terms, or nullptr
   unsigned short* ft;
 };
 
@@ -125,7 +150,6 @@ __device__ __forceinline__ unsigned short term(float& v, bool again) {
   return __builtin_bit_cast(unsigned short, o);
 }
 
-// (TERMS 2: the loss alone, whose second term is what the first leaves of f(X))
 template <typename ST, typename OT, int TERMS, int ACT>
 __device__ __forceinline__ void lay_states(const States& p, int block) {
   __shared__ unsigned short tile[32][34];
@@ -149,7 +173,7 @@ __device__ __forceinline__ void lay_states(const States& p, int block) {
       const int d = d0 + i * 8 + r;
       const unsigned short h = term<OT>(v[i], TERMS > 1);
       tile[i * 8 + r][c] = h;
-      if (p.f && d < p.D) p.f[((long long)t * p.D + d) * p.Bk + n] = h;
+      if (p.f && t < p.f_terms && d < p.D) p.f[((long long)t * p.D + d) * p.Bk + n] = h;
     }
     __syncthreads();
 #pragma unroll
@@ -189,7 +213,7 @@ __device__ __forceinline__ void lay_rows(const Rows& p, unsigned block) {
 template <typename ST, typename OT, int TERMS, int ACT>
 __global__ void __launch_bounds__(256) token_lay_kernel(const States x, const Rows w, unsigned states) {
   if (blockIdx.x < states) lay_states<ST, OT, TERMS, ACT>(x, blockIdx.x);
-  else lay_rows<ST, OT, TERMS == 2 ? 1 : TERMS>(w, blockIdx.x - states);  // (W has no second term)
+  else lay_rows<ST, OT, std::is_same<ST, float>::value ? 3 : 1>(w, blockIdx.x - states);  // (whatever terms f(X) has)
 }
 
 // ---------------------------------------------------------------- a column's tiles
@@ -241,7 +265,7 @@ __global__ void __launch_bounds__(256) token_fix_kernel(const float* fixes, int 
 }
 
 // ------------------------------------------------------------------ errors
-// Kept exponentials into errors, in place (fp32: into three terms): a column (a row of ET, up
+// Kept exponentials into errors, in place, or from fp32 into two or three terms: a column (a row of ET, up
 // to Vp) a workgroup, which joins the column's parts itself, up to ERROR_RUN values; of longer
 // ones 2048 values, their columns joined before.  Zeros past the ends and in padded rows, up
 // to Bk.  us, joining here / before: V = 10007, B = 77 fp32 9.6 / 4.7 + 5.4; V = 32000, B = 1024
@@ -307,7 +331,7 @@ __global__ void __launch_bounds__(256) token_errors_kernel(const Errors p) {
           if (v + i >= p.V) e[i] = 0.0f;
       }
       if (id >= v && id < v + 8) {
-        const float own = -expm1f(-loss) * p.scale;  // 1 - p without its cancellation
+        const float own = token::target_error(loss, p.scale);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           if (id == v + i) e[i] = own;
@@ -324,6 +348,58 @@ __global__ void __launch_bounds__(256) token_errors_kernel(const Errors p) {
   }
 }
 
+// ---------------------------------------------------------------- targets' rows
+// What rounding e and f to 16 bits leaves out of the sum e f^T where e is near 1, at the
+// targets: hot[p][d] = sum over the columns n of sorted positions p .. of one target of
+// (e - rounded e) rounded f + e (f - rounded f), for the first position p of each target.
+// (Elsewhere e is a probability, whose rounding counts as little.  Without this a weight in a
+// few hundred of a target's row rounds the other way, and the next loss differs by 1e-5 .. 1e-3.)
+// A workgroup has 256 features of a position: four groups of 64 lanes take every fourth column.
+struct Hot {
+  int B, D, Dp, terms;
+  const int* order;
+  const int* key;
+  const unsigned short* ft;  // [terms][B][Dp]
+  const float* loss;
+  float* hot;                // [B][Dp]
+  float scale;
+};
+template <typename OT>
+__global__ void __launch_bounds__(256) token_hot_kernel(const Hot p) {
+  __shared__ float4 red[4][64];
+  const int slabs = (p.Dp + 255) / 256, at = blockIdx.x / slabs, lane = threadIdx.x & 63, group = threadIdx.x >> 6;
+  const int d = blockIdx.x % slabs * 256 + lane * 4;
+  const int id = p.key[at];
+  if (id < 0 || (at > 0 && p.key[at - 1] == id)) return;
+  int many = 0;  // columns of this target
+  for (int i = at;; i += 64) {
+    const unsigned long long other = __ballot(p.key[i + lane < p.B ? i + lane : p.B] != id);
+    many += other ? __ffsll(other) - 1 : 64;
+    if (other) break;
+  }
+  float sum[4] = {};
+  const int from = d < p.Dp ? d : 0;
+#pragma unroll 4
+  for (int i = group; i < many; i += 4) {
+    const int n = p.order[at + i];
+    const float e = token::target_error(p.loss[n], p.scale), left = e - to_f32(cvt<OT>(e));
+    float f[4], g[4] = {};
+    load4(reinterpret_cast<const OT*>(p.ft) + (long long)n * p.Dp + from, f);
+    if (p.terms > 1) load4(reinterpret_cast<const OT*>(p.ft) + ((long long)p.B + n) * p.Dp + from, g);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) sum[q] += left * f[q] + e * g[q];
+  }
+  red[group][lane] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+  __syncthreads();
+  if (group != 0 || d >= p.Dp) return;
+  float4 all = red[0][lane];
+#pragma unroll
+  for (int g = 1; g < 4; ++g) {
+    all.x += red[g][lane].x; all.y += red[g][lane].y; all.z += red[g][lane].z; all.w += red[g][lane].w;
+  }
+  *reinterpret_cast<float4*>(p.hot + (long long)at * p.Dp + d) = all;
+}
+
 template <typename ST, typename OT, int TERMS, int ACT>
 hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
   const bool update = p.g != nullptr;
@@ -331,9 +407,8 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
   if (!make_plan(p.V, p.D, p.B, storage, p.act, update, o)) return hipErrorInvalidValue;
   unsigned char* ws = p.workspace;
   auto at = [&](long long offset) { return reinterpret_cast<unsigned short*>(ws + offset); };
-  const States st{p.D, p.B, p.V, o.Dp, o.Bk, p.x, p.targets, update ? at(o.f) : nullptr, at(o.ft)};
+  const States st{p.D, p.B, p.V, o.Dp, o.Bk, o.f_terms, p.x, p.targets, update ? at(o.f) : nullptr, at(o.ft)};
   const unsigned state_tiles = (unsigned)((long long)(o.Dp / 32) * (o.Bk / 32));
-  constexpr bool inexact = TERMS == 1 && ACT != ACT_IDENTITY && ACT != ACT_RELU;
   hipError_t e = hipSuccess;
   auto rows_of = [&](int first) { return std::min(o.rows, p.V - first); };
   // the piece's rows of W where they are laid out, and (states: workgroups) f(X)
@@ -342,7 +417,7 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
     const Rows r{rows, padded, p.D, o.Dp, static_cast<const ST*>(p.w) + (long long)first * p.D, at(o.ws)};
     const long long fours = o.copy ? (long long)padded * o.Dp / 4 : 0;
     const dim3 grid(states + (unsigned)((fours + 255) / 256)), block(256);
-    if (inexact && !update) hipLaunchKernelGGL((token_lay_kernel<ST, OT, inexact ? 2 : TERMS, ACT>), grid, block, 0, s, st, r, states);
+    if (TERMS == 1 && o.ft_terms == 2) hipLaunchKernelGGL((token_lay_kernel<ST, OT, TERMS == 1 ? 2 : TERMS, ACT>), grid, block, 0, s, st, r, states);
     else hipLaunchKernelGGL((token_lay_kernel<ST, OT, TERMS, ACT>), grid, block, 0, s, st, r, states);
     if (e == hipSuccess) e = hipGetLastError();
   };
@@ -363,7 +438,7 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
     TokenGemm q{};
     weights(first, q, lay);
     q.M = rows_of(first); q.N = p.B; q.K = o.copy ? o.Dp : p.D;
-    q.b = at(o.ft); q.ldb = o.Dp; q.b_term = (unsigned)(p.B * o.Dp * 2); q.b_bytes = (long long)(o.two ? 2 : TERMS) * p.B * o.Dp * 2;
+    q.b = at(o.ft); q.ldb = o.Dp; q.b_term = (unsigned)(p.B * o.Dp * 2); q.b_bytes = (long long)o.ft_terms * p.B * o.Dp * 2;
     q.targets = p.targets; q.first = first; q.V = p.V;
     q.target_logit = reinterpret_cast<float*>(ws + o.logit);
     return q;
@@ -377,7 +452,7 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
     q.out = part + (long long)(first / o.unit) * p.B;
     if (o.keep) {
       q.kept = ws + o.kept; q.out_ld = o.Vp; q.out_rows = o.Bk;
-      e = launch_token_keep(q, storage, o.tile, s);
+      e = launch_token_keep(q, storage, o.tile, o.two, s);
     } else {
       e = launch_token_stats(q, storage, o.tile, o.two, s);
     }
@@ -402,22 +477,34 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
                         reinterpret_cast<uintptr_t>(p.g) % (4 * sizeof(ST)) == 0;
   const TokenFinish finish{p.D, p.B, p.V, o.slices, p.act, reinterpret_cast<const float*>(ws + o.part), p.x, p.targets, p.g,
                            1.0f / scale, fixes, vec_state};
+  auto make_good = [&] {  // once the losses are known
+    int *order = reinterpret_cast<int*>(ws + o.order), *key = reinterpret_cast<int*>(ws + o.key);
+    e = launch_sort_places(p.targets, p.B, p.V, order, key, reinterpret_cast<int*>(ws + o.slot), s);
+    if (e != hipSuccess) return;
+    const Hot h{p.B, p.D, o.Dp, o.ft_terms, order, key, at(o.ft), p.loss, reinterpret_cast<float*>(ws + o.hot), scale};
+    hipLaunchKernelGGL((token_hot_kernel<OT>), dim3((unsigned)((long long)p.B * ((o.Dp + 255) / 256))), dim3(256), 0, s, h);
+    e = hipGetLastError();
+  };
   for (int first = 0; first < p.V; first += o.rows) {
     const int rows = rows_of(first), Vp = (rows + 31) / 32 * 32;
     if (o.keep) {
       const Errors er{p.V, p.B, Vp, o.Bk, o.unit, units, ws + o.kept, at(o.et), part, reinterpret_cast<const float*>(ws + o.logit),
                       p.loss, reinterpret_cast<const float2*>(ws + o.norm), p.targets, scale};
       const dim3 grid((unsigned)((long long)o.Bk * (joined ? 1 : (Vp + 2047) / 2048)));
-      if (joined) hipLaunchKernelGGL((token_errors_kernel<OT, TERMS, true>), grid, dim3(256), 0, s, er);
-      else hipLaunchKernelGGL((token_errors_kernel<OT, TERMS, false>), grid, dim3(256), 0, s, er);
+      constexpr int MORE = TERMS == 3 ? 3 : 2;
+      if (o.e_terms == 1 && joined) hipLaunchKernelGGL((token_errors_kernel<OT, TERMS, true>), grid, dim3(256), 0, s, er);
+      else if (o.e_terms == 1) hipLaunchKernelGGL((token_errors_kernel<OT, TERMS, false>), grid, dim3(256), 0, s, er);
+      else if (joined) hipLaunchKernelGGL((token_errors_kernel<OT, MORE, true>), grid, dim3(256), 0, s, er);
+      else hipLaunchKernelGGL((token_errors_kernel<OT, MORE, false>), grid, dim3(256), 0, s, er);
       e = hipGetLastError();
     } else {
       TokenGemm q = logits(first, o.rows < p.V);  // (one piece: its rows are laid out already)
       if (e != hipSuccess) return e;
       q.stats = reinterpret_cast<const float2*>(ws + o.norm);
-      q.out = at(o.et); q.out_ld = Vp; q.out_rows = o.Bk; q.out_term = (long long)o.Bk * Vp; q.scal = scale;
+      q.out = at(o.et); q.out_ld = Vp; q.out_rows = o.Bk; q.out_term = (long long)o.Bk * Vp; q.scal = scale; q.loss = p.loss;
       e = launch_token_error(q, storage, o.tile, s);
     }
+    if (e == hipSuccess && o.mend && first == 0) make_good();
     if (e != hipSuccess) return e;
     TokenGemm g{};
     weights(first, g, false);
@@ -427,13 +514,18 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
     e = launch_token_grad(g, storage, o.grad_tile, s);
     if (e != hipSuccess) return e;
     TokenGemm u{};
-    u.a = at(o.et); u.lda = Vp; u.a_term = g.b_term; u.a_bytes = g.b_bytes;
-    u.b = at(o.f); u.ldb = o.Bk; u.b_term = (unsigned)(p.D * o.Bk * 2); u.b_bytes = (long long)TERMS * p.D * o.Bk * 2;
+    u.a = at(o.et); u.lda = Vp; u.a_term = g.b_term; u.a_bytes = (long long)o.e_terms * o.Bk * Vp * 2;
+    u.b = at(o.f); u.ldb = o.Bk; u.b_term = (unsigned)(p.D * o.Bk * 2); u.b_bytes = (long long)o.f_terms * p.D * o.Bk * 2;
     u.M = rows; u.N = p.D; u.K = o.Bk;
     u.out = static_cast<ST*>(p.w) + (long long)first * p.D;
     u.vec = p.D % 4 == 0 && reinterpret_cast<uintptr_t>(p.w) % (4 * sizeof(ST)) == 0;
     u.scal = p.alpha / scale;
-    e = launch_token_weight(u, first + rows == p.V ? &finish : nullptr, storage, s);
+    if (o.mend) {
+      u.slot = reinterpret_cast<const int*>(ws + o.slot) + first;
+      u.hot = reinterpret_cast<const float*>(ws + o.hot);
+      u.hot_ld = o.Dp;
+    }
+    e = launch_token_weight(u, first + rows == p.V ? &finish : nullptr, storage, o.f_terms, s);
     if (e != hipSuccess) return e;
   }
   if (!fixes) return e;
