@@ -189,23 +189,15 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
     for (int j = 0; j < RN; ++j)
 #pragma unroll
       for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
-  if constexpr (MODE == TOKEN_WEIGHT && TERMS == 1) {  // what the targets' rows begin with
-    if (p.slot) {
+  // TOKEN_WEIGHT: what the targets' rows begin with.  Asked for ahead of the operands, used
+  // once those are on their way.
+  constexpr bool HOT = MODE == TOKEN_WEIGHT && TERMS == 1;
+  int slot[HOT ? RM : 1];
+  if constexpr (HOT) {
 #pragma unroll
-      for (int i = 0; i < RM; ++i) {
-        const int m = m0 + wm * WTM + i * 32 + lr, at = m < M ? p.slot[m] : -1;
-        if (!__any(at >= 0)) continue;
-#pragma unroll
-        for (int j = 0; j < RN; ++j)
-#pragma unroll
-          for (int q = 0; q < 16; q += 4) {
-            const int n = n0 + wn * WTN + j * 32 + 2 * q + 4 * lk;
-            if (at >= 0 && n < p.hot_ld) {
-              const float4 v = *reinterpret_cast<const float4*>(p.hot + (long long)at * p.hot_ld + n);
-              acc[i][j][q] = v.x; acc[i][j][q + 1] = v.y; acc[i][j][q + 2] = v.z; acc[i][j][q + 3] = v.w;
-            }
-          }
-      }
+    for (int i = 0; i < RM; ++i) {
+      const int m = m0 + wm * WTM + i * 32 + lr;
+      slot[i] = p.slot && m < M ? p.slot[m] : -1;
     }
   }
 
@@ -241,6 +233,24 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
     seek(s);
 #pragma unroll
     for (int q = 0; q < LPS; ++q) load(q, smem + s * STAGE, sa, sb);
+  }
+  if constexpr (HOT) {
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+      if (slot[i] >= 0) {
+        const float* row = p.hot + (long long)slot[i] * p.hot_ld;
+#pragma unroll
+        for (int j = 0; j < RN; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int n = n0 + wn * WTN + j * 32 + 8 * q + 4 * lk;
+            const float4 v = *reinterpret_cast<const float4*>(row + (n < p.hot_ld ? n : 0));
+            acc[i][j][4 * q] = v.x; acc[i][j][4 * q + 1] = v.y; acc[i][j][4 * q + 2] = v.z; acc[i][j][4 * q + 3] = v.w;
+          }
+      }
+    }
+    // (a wait that the compiler knows of: it would else wait for these loads in every step)
+    __builtin_amdgcn_s_waitcnt(vm_wait<0>());
   }
   wait_loads<(ST - 2) * LPS>();
   __builtin_amdgcn_s_barrier();
@@ -472,7 +482,9 @@ template <typename OT, int TERMS, int MODE, bool TWO, int WGM, int WGN>
 hipError_t run_narrow(const TokenGemm& p, hipStream_t s) {
   constexpr int BNC = TWO ? 32 : 64;
   const long long tiles = ((p.M + 63LL) / 64) * ((p.N + BNC - 1LL) / BNC) * (MODE == TOKEN_GRAD ? p.slices : 1);
-  if (TERMS == 3 && tiles > 256) return run_tile<OT, TERMS, MODE, TWO, 64, 64, WGM, WGN, 3>(p, s);
+  if constexpr (TERMS == 3) {
+    if (tiles > 256) return run_tile<OT, TERMS, MODE, TWO, 64, 64, WGM, WGN, 3>(p, s);
+  }
   return run_tile<OT, TERMS, MODE, TWO, 64, 64, WGM, WGN, TERMS == 3 ? 6 : 8 / TERMS>(p, s);
 }
 

@@ -94,8 +94,12 @@ hipError_t weight_finish(const TokenGemm& p, const TokenFinish& f, hipStream_t s
 template <typename OT, int TERMS>
 hipError_t weight(const TokenGemm& p, const TokenFinish* f, int storage, hipStream_t s) {
   auto tiles = [&](long long e) { return ((p.M + e - 1) / e) * ((p.N + e - 1) / e); };
-  if (tiles(128) <= 128 && f)
-    return TERMS == 3 && tiles(64) > 256 ? weight_finish<OT, TERMS, 3>(p, *f, s) : weight_finish<OT, TERMS, TERMS == 3 ? 6 : 8 / TERMS>(p, *f, s);
+  if (tiles(128) <= 128 && f) {
+    if constexpr (TERMS == 3) {
+      if (tiles(64) > 256) return weight_finish<OT, TERMS, 3>(p, *f, s);
+    }
+    return weight_finish<OT, TERMS, TERMS == 3 ? 6 : 8 / TERMS>(p, *f, s);
+  }
   if (f) {
     const hipError_t e = launch_token_finish(*f, storage, s);
     if (e != hipSuccess) return e;
