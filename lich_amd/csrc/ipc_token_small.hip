@@ -164,12 +164,16 @@ __global__ void __launch_bounds__(kThreads) token_small_kernel(const TokenProble
 
 }  // namespace
 
-// One workgroup is slow at anything long: us, in one / the launches of the general path, fp32:
-// 10 x 64 x 128 (V, D, B) 11.5 / 21.6; 64 x 64 x 64 18 / 23.6; 10 x 256 x 100 30.6 / 26.
+// One workgroup is slow at anything long: the steps that its threads take one after the other are
+// counted.  us, in one / in the launches of the general path, fp32: 10 x 64 x 128 (V, D, B; 82
+// steps) 11.5 / 21.6; 64 x 64 x 64 (152) 18 / 23.6; 10 x 256 x 100 (225) 30.6 / 26; 1844 x 4 x 1 (1877) 76 / 22.
 bool token_small(int V, int D, int B) {
   constexpr long long most = 1 << 14;
-  return (long long)V * D <= most && (long long)D * B <= most && (long long)V * B <= most &&
-         (long long)V * D * B <= 1 << 18 && small_lds(V, D, B) <= kLds;
+  if ((long long)V * D > most || (long long)D * B > most || (long long)V * B > most || small_lds(V, D, B) > kLds) return false;
+  auto rounds = [](long long items) { return (items + kThreads - 1) / kThreads; };
+  const long long logits = rounds((V + 3LL) / 4 * B) * ((D + 3) / 4), gradient = rounds((D + 3LL) / 4 * B) * V,
+                  update = rounds((long long)V * D) * ((B + 3) / 4), fill = rounds((long long)V * (D + 4)) + 2 * rounds((D + 3LL) / 4 * B);
+  return logits + gradient + update + fill <= 192;
 }
 
 template <typename ST, int ACT>

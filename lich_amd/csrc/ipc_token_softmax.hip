@@ -88,8 +88,10 @@ bool make_plan(int V, int D, int B, int storage, int act, bool update, Plan& o) 
   if (o.fine && !o.keep) return false;  // (never: its errors are few)
   auto tiles = [&](long long m, long long n, long long e) { return ((m + e - 1) / e) * ((n + e - 1) / e); };
   const long long columns = o.two ? 2LL * B : B;
+  // (the largest tile that gives the CUs one each; fp32: us, 64 wide / 128 x 64, 4000 x 4000 x 512 update 355 / 336,
+  // 10007 x 515 x 77 77 / 72)
   if (columns <= 64) o.tile = o.rows >= 32768 ? TILE_128_64 : TILE_64;
-  else o.tile = storage != DT_F32 && tiles(o.rows, columns, 256) >= 192 ? TILE_256 : tiles(o.rows, columns, 128) > 128 ? TILE_128 : TILE_64;
+  else o.tile = storage != DT_F32 && tiles(o.rows, columns, 256) >= 192 ? TILE_256 : tiles(o.rows, columns, 128) > 128 ? TILE_128 : storage == DT_F32 && (o.rows + 127LL) / 128 * ((columns + 63) / 64) >= 128 ? TILE_128_64 : TILE_64;
   o.unit = token_unit(o.tile, o.two);
   o.grad_tile = storage != DT_F32 && D >= 256 && B >= 256 ? 256 : D > 64 ? 128 : 64;
   const long long gt = o.grad_tile == 256 ? tiles(D, B, 256)
