@@ -32,10 +32,11 @@ namespace ipc {
 enum { TOKEN_STATS = 0, TOKEN_KEEP = 1, TOKEN_ERROR = 2, TOKEN_GRAD = 3, TOKEN_WEIGHT = 4 };
 
 // Tiles of the first three: rows (of W) and columns of a workgroup, and the rows of a wave, whose
-// largest values and sums are kept (unit; two: with f(X) in two terms).
+// largest values and sums are kept (unit; ways: terms of f(X), side by side in a tile; with three
+// TILE_128_64 and TILE_64 alone, each 96 columns wide).
 enum { TILE_256 = 0, TILE_128 = 1, TILE_128_64 = 2, TILE_64 = 3 };
-inline int token_unit(int tile, bool two) {
-  return tile == TILE_256 ? 128 : tile == TILE_128 ? 64 : tile == TILE_128_64 ? (two ? 32 : 64) : 32;
+inline int token_unit(int tile, int ways) {
+  return tile == TILE_256 ? 128 : tile == TILE_128 ? 64 : tile == TILE_128_64 ? (ways == 2 ? 32 : 64) : 32;
 }
 
 // One product.  Rows start at multiples of 4 bytes; a and b with all their terms lie
@@ -63,9 +64,9 @@ struct TokenGemm {
   const float2* stats;             // ERROR: of each column, largest logit and 1 / sum of exp(z - largest)
 };
 // storage: 0 (three bf16 terms), 1, 2
-hipError_t launch_token_stats(const TokenGemm& p, int storage, int tile, bool two, hipStream_t s);
-// two: f(X) in two terms, the exponentials kept in fp32
-hipError_t launch_token_keep(const TokenGemm& p, int storage, int tile, bool two, hipStream_t s);
+// ways: terms of f(X); more than one: the exponentials kept in fp32
+hipError_t launch_token_stats(const TokenGemm& p, int storage, int tile, int ways, hipStream_t s);
+hipError_t launch_token_keep(const TokenGemm& p, int storage, int tile, int ways, hipStream_t s);
 hipError_t launch_token_error(const TokenGemm& p, int storage, int tile, hipStream_t s);
 hipError_t launch_token_grad(const TokenGemm& p, int storage, int tile, hipStream_t s);
 
@@ -85,7 +86,7 @@ inline int token_fix_rows(int D, bool vec) { return vec ? (D + 15) / 16 : (D + 3
 hipError_t launch_token_finish(const TokenFinish& p, int storage, hipStream_t s);
 // W's update, and (f) the gradient's last step, which needs no more than that does: in one
 // launch where both are small.
-// terms: of both operands in 16-bit storage, 1 or 2
+// terms: of both operands in 16-bit storage, 1, 2 (fp16) or 3 (bf16)
 hipError_t launch_token_weight(const TokenGemm& p, const TokenFinish* f, int storage, int terms, hipStream_t s);
 
 namespace token {
@@ -94,6 +95,10 @@ using namespace mx;
 
 // a and b terms of the products of three terms each, smallest first (of two terms: the last three)
 constexpr int PRODUCTS = 6, TERM_A[PRODUCTS] = {2, 1, 0, 1, 0, 0}, TERM_B[PRODUCTS] = {0, 1, 2, 0, 1, 0};
+
+// (three terms of bf16 are fp32's, but where a launcher says otherwise)
+template <typename OT, int TERMS>
+using storage_of = typename std::conditional<TERMS == 3, float, OT>::type;
 
 template <bool EXACT>
 __device__ __forceinline__ float exp_of(float x) {
@@ -106,16 +111,17 @@ __device__ __forceinline__ float exp_of(float x) {
 __device__ __forceinline__ float target_error(float loss, float scale) { return -expm1f(-loss) * scale; }
 
 // Workgroup `block` of `blocks` of a product.
-template <typename OT, int TERMS, int MODE, bool TWO, int BM, int BN, int WGM, int WGN, int ST>
+// WT: the type of W, which TOKEN_WEIGHT writes.
+template <typename OT, int TERMS, int MODE, int WAYS, int BM, int BN, int WGM, int WGN, int ST, typename WT>
 __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* smem, int block, int blocks) {
   using MF = Mfma32<OT>;
   typedef typename MF::operand V;
   constexpr bool MN = MODE == TOKEN_GRAD || MODE == TOKEN_WEIGHT, COLUMNS = !MN;
   constexpr int NW = WGM * WGN, WTM = BM / WGM, WTN = BN / WGN, RM = WTM / 32, RN = WTN / 32;
-  constexpr int RNC = TWO ? RN / 2 : RN, BNC = TWO ? BN / 2 : BN;  // blocks and columns of different n
-  constexpr bool SPLIT = TERMS == 3, FINE = SPLIT || (MODE == TOKEN_KEEP && TWO);  // FINE: kept in fp32
+  constexpr int RNC = RN / WAYS, BNC = BN / WAYS, WTC = WTN / WAYS;  // blocks and columns of different n
+  constexpr bool SPLIT = TERMS == 3, FINE = SPLIT || (MODE == TOKEN_KEEP && WAYS > 1);  // FINE: kept in fp32
   constexpr int A_BYTES = BM * 64, B_BYTES = BN * 64, STAGE = TERMS * (A_BYTES + B_BYTES);
-  static_assert(!TWO || ((MODE == TOKEN_STATS || MODE == TOKEN_KEEP) && TERMS == 1 && RN % 2 == 0), "two terms of f(X)");
+  static_assert(WAYS == 1 || ((MODE == TOKEN_STATS || MODE == TOKEN_KEEP) && TERMS == 1 && RN % WAYS == 0), "terms of f(X)");
   constexpr int IA = A_BYTES / 1024 / NW, IB = B_BYTES / 1024 / NW, LPS = TERMS * (IA + IB);  // LDS-DMA loads per wave and stage
   static_assert(IA * 1024 * NW == A_BYTES && IB * 1024 * NW == B_BYTES, "tile / waves");
 
@@ -149,18 +155,18 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
     const int r = slot >> 2, c = (slot & 3) ^ ((r >> 2) & 3), row = e0 + r < lim ? e0 + r : lim - 1;
     return (unsigned)(row * ld) * 2u + (unsigned)c * 16u;
   };
-  // (TWO: the first half of a wave's columns holds f(X)'s leading term, the second half,
-  // the same columns, what is left of it)
-  auto source_two = [&](int q) -> unsigned {
+  // (WAYS > 1: the first of as many parts of a wave's columns holds f(X)'s leading term, the
+  // others, the same columns, the next ones)
+  auto source_ways = [&](int q) -> unsigned {
     const int slot = (q * NW + w) * 64 + lane, r = slot >> 2, c = (slot & 3) ^ ((r >> 2) & 3);
-    const int of = r / WTN, at = r % WTN, n = n0 + of * (WTN / 2) + at % (WTN / 2);
-    return (at >= WTN / 2 ? p.b_term : 0u) + (unsigned)((n < N ? n : N - 1) * p.ldb) * 2u + (unsigned)c * 16u;
+    const int of = r / WTN, at = r % WTN, n = n0 + of * WTC + at % WTC;
+    return at / WTC * p.b_term + (unsigned)((n < N ? n : N - 1) * p.ldb) * 2u + (unsigned)c * 16u;
   };
   unsigned oa[IA], ob[IB];
 #pragma unroll
   for (int q = 0; q < IA; ++q) oa[q] = source(MN, q, BM, m0, M, p.lda);
 #pragma unroll
-  for (int q = 0; q < IB; ++q) ob[q] = TWO ? source_two(q) : source(false, q, BN, n0, N, p.ldb);
+  for (int q = 0; q < IB; ++q) ob[q] = WAYS > 1 ? source_ways(q) : source(false, q, BN, n0, N, p.ldb);
   const unsigned step_a = MN ? (unsigned)p.lda * 64u : 64u;  // of a stage
   // load q of a stage: uniform offsets sa, sb; the terms of A, then those of B
   auto load = [&](int q, unsigned char* st, unsigned sa, unsigned sb) {
@@ -353,28 +359,31 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
       for (int u = 0; u < PASSES; ++u) {
         const int r = u * RPP + lane / LPR, c = lane % LPR * PER;
         const uint4 v = *reinterpret_cast<const uint4*>(es + r * LD + c);
-        const long long row = n0 + wn * WTN / (TWO ? 2 : 1) + j * 32 + r;
+        const long long row = n0 + wn * WTC + j * 32 + r;
         const int col = m0 + wm * WTM + c;
         if (row < p.out_rows && col < p.out_ld) *reinterpret_cast<uint4*>(out + term * p.out_term + row * p.out_ld + col) = v;
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
   };
-  if constexpr (TWO) {
+  if constexpr (WAYS > 1) {
 #pragma unroll
     for (int i = 0; i < RM; ++i)
 #pragma unroll
       for (int j = 0; j < RNC; ++j)
 #pragma unroll
-        for (int q = 0; q < 16; ++q)  // (an infinite weight times the rest of f(X), of either sign, is no matter)
-          acc[i][j][q] += __builtin_isinf(acc[i][j][q]) ? 0.0f : acc[i][j + RNC][q];
+        for (int q = 0; q < 16; ++q) {  // (an infinite weight times the rest of f(X), of either sign, is no matter)
+          float rest = acc[i][j + RNC][q];
+          if constexpr (WAYS == 3) rest += acc[i][j + 2 * RNC][q];
+          acc[i][j][q] += __builtin_isinf(acc[i][j][q]) ? 0.0f : rest;
+        }
   }
   if constexpr (MODE == TOKEN_STATS || MODE == TOKEN_KEEP) {
     if constexpr (MODE == TOKEN_KEEP) __syncthreads();
     const int mw = m0 + wm * WTM;
 #pragma unroll
     for (int j = 0; j < RNC; ++j) {
-      const int n = n0 + wn * WTN / (TWO ? 2 : 1) + j * 32 + lr;
+      const int n = n0 + wn * WTC + j * 32 + lr;
       if (m0 + BM > M) mask_rows(j, -__builtin_inff());
       // the target's place among this lane's rows of the column
       const long long to = (n < N ? p.targets[n] : -1) - p.first - mw;
@@ -434,7 +443,7 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
       __builtin_amdgcn_sched_barrier(0);
     }
   } else {
-    typedef typename std::conditional<MODE == TOKEN_GRAD || SPLIT, float, OT>::type TT;
+    typedef typename std::conditional<MODE == TOKEN_GRAD, float, WT>::type TT;
     MxProblem e{};
     e.M = M; e.N = N; e.scal = MODE == TOKEN_GRAD ? 1.0f : p.scal;
     e.out = MODE == TOKEN_GRAD ? static_cast<float*>(p.out) + (long long)slice * M * N : p.out;
@@ -446,29 +455,29 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
   }
 }
 
-template <typename OT, int TERMS, int MODE, bool TWO, int BM, int BN, int WGM, int WGN, int ST>
+template <typename OT, int TERMS, int MODE, int WAYS, int BM, int BN, int WGM, int WGN, int ST, typename WT>
 __global__ void __launch_bounds__(WGM * WGN * 64) token_gemm_kernel(const TokenGemm p) {
   extern __shared__ __align__(16) unsigned char smem[];
-  product_tile<OT, TERMS, MODE, TWO, BM, BN, WGM, WGN, ST>(p, smem, blockIdx.x, gridDim.x);
+  product_tile<OT, TERMS, MODE, WAYS, BM, BN, WGM, WGN, ST, WT>(p, smem, blockIdx.x, gridDim.x);
 }
 
-template <int TERMS, int MODE, bool TWO, int BM, int BN, int WGM, int WGN, int ST>
+template <int TERMS, int MODE, int WAYS, int BM, int BN, int WGM, int WGN, int ST>
 constexpr int tile_lds() {
   constexpr int NW = WGM * WGN, ring = ST * TERMS * (BM + BN) * 64;
   constexpr int epi = MODE == TOKEN_STATS ? 0
-                      : MODE == TOKEN_ERROR || (MODE == TOKEN_KEEP && TERMS == 1 && !TWO) ? NW * 32 * (BM / WGM + 8) * 2
+                      : MODE == TOKEN_ERROR || (MODE == TOKEN_KEEP && TERMS == 1 && WAYS == 1) ? NW * 32 * (BM / WGM + 8) * 2
                       : MODE == TOKEN_KEEP ? NW * 32 * (BM / WGM + 4) * 4 : NW * 32 * (BN / WGN + 4) * 4;
   return epi > ring ? epi : ring;
 }
 
-template <typename OT, int TERMS, int MODE, bool TWO, int BM, int BN, int WGM, int WGN, int ST = 4>
+template <typename OT, int TERMS, int MODE, int WAYS, int BM, int BN, int WGM, int WGN, int ST = 4, typename WT = storage_of<OT, TERMS>>
 hipError_t run_tile(const TokenGemm& p, hipStream_t s) {
-  constexpr int smem = tile_lds<TERMS, MODE, TWO, BM, BN, WGM, WGN, ST>();
+  constexpr int smem = tile_lds<TERMS, MODE, WAYS, BM, BN, WGM, WGN, ST>();
   static_assert(smem <= 160 * 1024, "LDS");
-  const void* fn = reinterpret_cast<const void*>(&token_gemm_kernel<OT, TERMS, MODE, TWO, BM, BN, WGM, WGN, ST>);
+  const void* fn = reinterpret_cast<const void*>(&token_gemm_kernel<OT, TERMS, MODE, WAYS, BM, BN, WGM, WGN, ST, WT>);
   static const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != hipSuccess) return e;
-  constexpr int BNC = TWO ? BN / 2 : BN;
+  constexpr int BNC = BN / WAYS;
   const long long tiles = ((p.M + BM - 1LL) / BM) * ((p.N + BNC - 1LL) / BNC) * (MODE == TOKEN_GRAD ? p.slices : 1);
   TokenGemm q = p;
   void* args[] = {&q};
@@ -478,14 +487,14 @@ hipError_t run_tile(const TokenGemm& p, hipStream_t s) {
 // 64 x 64 tiles: as many stages as leave two workgroups a CU (fp32: one, or two of three stages
 // where there are more workgroups than CUs), since a step of few workgroups is as long as
 // a load takes over the stages in flight.
-template <typename OT, int TERMS, int MODE, bool TWO, int WGM, int WGN>
+template <typename OT, int TERMS, int MODE, int WAYS, int WGM, int WGN, typename WT = storage_of<OT, TERMS>>
 hipError_t run_narrow(const TokenGemm& p, hipStream_t s) {
-  constexpr int BNC = TWO ? 32 : 64;
+  constexpr int BNC = 64 / WAYS;
   const long long tiles = ((p.M + 63LL) / 64) * ((p.N + BNC - 1LL) / BNC) * (MODE == TOKEN_GRAD ? p.slices : 1);
   if constexpr (TERMS == 3) {
-    if (tiles > 256) return run_tile<OT, TERMS, MODE, TWO, 64, 64, WGM, WGN, 3>(p, s);
+    if (tiles > 256) return run_tile<OT, TERMS, MODE, WAYS, 64, 64, WGM, WGN, 3, WT>(p, s);
   }
-  return run_tile<OT, TERMS, MODE, TWO, 64, 64, WGM, WGN, TERMS == 3 ? 6 : 8 / TERMS>(p, s);
+  return run_tile<OT, TERMS, MODE, WAYS, 64, 64, WGM, WGN, TERMS == 3 ? 6 : 8 / TERMS, WT>(p, s);
 }
 
 }  // namespace token

@@ -7,11 +7,11 @@ namespace {
 template <typename OT, int TERMS>
 hipError_t grad(const TokenGemm& p, int tile, hipStream_t s) {
   if constexpr (TERMS == 1) {
-    if (tile == 256) return token::run_tile<OT, TERMS, TOKEN_GRAD, false, 256, 256, 2, 2>(p, s);
+    if (tile == 256) return token::run_tile<OT, TERMS, TOKEN_GRAD, 1, 256, 256, 2, 2>(p, s);
   }
-  if (tile >= 128 && p.N > 64) return token::run_tile<OT, TERMS, TOKEN_GRAD, false, 128, 128, 2, 2, TERMS == 3 ? 3 : 4>(p, s);
-  if (tile == 128) return token::run_tile<OT, TERMS, TOKEN_GRAD, false, 128, 64, 2, 2, TERMS == 3 ? 4 : 6>(p, s);
-  return token::run_narrow<OT, TERMS, TOKEN_GRAD, false, 2, 2>(p, s);
+  if (tile >= 128 && p.N > 64) return token::run_tile<OT, TERMS, TOKEN_GRAD, 1, 128, 128, 2, 2, TERMS == 3 ? 3 : 4>(p, s);
+  if (tile == 128) return token::run_tile<OT, TERMS, TOKEN_GRAD, 1, 128, 64, 2, 2, TERMS == 3 ? 4 : 6>(p, s);
+  return token::run_narrow<OT, TERMS, TOKEN_GRAD, 1, 2, 2>(p, s);
 }
 
 }  // namespace

@@ -24,11 +24,11 @@
 // the results lose by it, and what is done:
 //   * G is rounded to the type itself: nothing.
 //   * the loss is fp32 and would be off by the logits' rounding, 2^-9 (2^-12).  The loss alone
-//     takes f(X) in two terms, both in one tile, so that W is read once.
+//     takes f(X) in two terms (small calls in bf16: three), all in one tile, so that W is read once.
 //   * W: a sum that is 2^-9 off rounds a weight in a few hundred of a target's row the other
 //     way, and the next loss differs by 1e-5 .. 1e-3.
 //   Small updates (kFineErrors, kFineWork: launches, not products, are their time) have f(X) and e in
-//   two terms and the exponentials in fp32: all of it is good to 2^-16 and better.  Large ones
+//   two terms, three in bf16, and the exponentials in fp32: all of it is good to 2^-22 and better.  Large ones
 //   correct the loss to first order by the gradient that they have, loss -= sum_d (W^T e)_d (f - rounded
 //   f)_d (left: half the variance of the logits' rounding, 3e-6 of a loss for bf16 logits of deviation
 //   3), and make the errors at the targets, the ones near 1, good in fp32 (token_hot_kernel; left in the next
@@ -48,8 +48,8 @@ constexpr long long kFineErrors = 1LL << 23, kFineWork = 1LL << 31;
 struct Plan {
   int terms, Dp, Bk;
   bool copy;          // W laid out per piece: fp32, or 16-bit rows of an odd length
-  bool two;           // the logits with f(X) in two terms
-  bool fine;          // the update in 16 bits, small: errors and f(X) in two terms
+  int ways;           // terms of f(X) in the logits, in 16 bits
+  bool fine;          // the update in 16 bits, small: errors and f(X) in `ways` terms
   bool mend;          // the update in 16 bits, large: targets' errors made good in fp32
   bool fix;           // and the loss corrected
   int ft_terms, f_terms, e_terms;
@@ -70,12 +70,14 @@ bool make_plan(int V, int D, int B, int storage, int act, bool update, Plan& o) 
   o.copy = storage == DT_F32 || D % 2 != 0;
   const bool inexact = storage != DT_F32 && act != ACT_IDENTITY && act != ACT_RELU;
   const long long work = (long long)V * B;
-  o.fine = update && storage != DT_F32 && work <= kFineErrors && work * D <= kFineWork;
+  const bool few = storage != DT_F32 && work <= kFineErrors && work * D <= kFineWork;
+  const int most = storage == DT_BF16 ? 3 : 2;
+  o.fine = update && few;
   o.mend = update && storage != DT_F32 && !o.fine;
   o.fix = inexact && o.mend;
-  o.two = o.fine || (inexact && !update);
-  o.ft_terms = storage == DT_F32 ? 3 : o.two || o.fix ? 2 : 1;
-  o.f_terms = o.e_terms = storage == DT_F32 ? 3 : o.fine ? 2 : 1;
+  o.ways = o.fine || (inexact && !update) ? few ? most : 2 : 1;
+  o.ft_terms = storage == DT_F32 ? 3 : o.fix ? 2 : o.ways;
+  o.f_terms = o.e_terms = storage == DT_F32 ? 3 : o.fine ? most : 1;
   const long long state = 2LL * o.Dp * o.Bk;
   if (state * o.ft_terms > kOperand) return false;
   const long long row_w = 2LL * (o.copy ? o.terms * o.Dp : D), row_e = update ? 2LL * o.e_terms * o.Bk : 1;
@@ -87,12 +89,13 @@ bool make_plan(int V, int D, int B, int storage, int act, bool update, Plan& o) 
   o.keep = update && o.rows == V && (storage != DT_F32 || (long long)o.Bk * o.Vp * 10 <= kPieceBytes);
   if (o.fine && !o.keep) return false;  // (never: its errors are few)
   auto tiles = [&](long long m, long long n, long long e) { return ((m + e - 1) / e) * ((n + e - 1) / e); };
-  const long long columns = o.two ? 2LL * B : B;
+  const long long columns = (long long)o.ways * B;
   // (the largest tile that gives the CUs one each; fp32: us, 64 wide / 128 x 64, 4000 x 4000 x 512 update 355 / 336,
   // 10007 x 515 x 77 77 / 72)
-  if (columns <= 64) o.tile = o.rows >= 32768 ? TILE_128_64 : TILE_64;
+  if (o.ways == 3) o.tile = (o.rows + 127LL) / 128 * ((B + 31LL) / 32) >= 256 ? TILE_128_64 : TILE_64;
+  else if (columns <= 64) o.tile = o.rows >= 32768 ? TILE_128_64 : TILE_64;
   else o.tile = storage != DT_F32 && tiles(o.rows, columns, 256) >= 192 ? TILE_256 : tiles(o.rows, columns, 128) > 128 ? TILE_128 : storage == DT_F32 && (o.rows + 127LL) / 128 * ((columns + 63) / 64) >= 128 ? TILE_128_64 : TILE_64;
-  o.unit = token_unit(o.tile, o.two);
+  o.unit = token_unit(o.tile, o.ways);
   o.grad_tile = storage != DT_F32 && D >= 256 && B >= 256 ? 256 : D > 64 ? 128 : 64;
   const long long gt = o.grad_tile == 256 ? tiles(D, B, 256)
                        : o.grad_tile == 128 ? (D + 127LL) / 128 * (B > 64 ? (B + 127LL) / 128 : 1) : tiles(D, B, 64);
@@ -419,7 +422,8 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
     const Rows r{rows, padded, p.D, o.Dp, static_cast<const ST*>(p.w) + (long long)first * p.D, at(o.ws)};
     const long long fours = o.copy ? (long long)padded * o.Dp / 4 : 0;
     const dim3 grid(states + (unsigned)((fours + 255) / 256)), block(256);
-    if (TERMS == 1 && o.ft_terms == 2) hipLaunchKernelGGL((token_lay_kernel<ST, OT, TERMS == 1 ? 2 : TERMS, ACT>), grid, block, 0, s, st, r, states);
+    if (o.ft_terms == 2) hipLaunchKernelGGL((token_lay_kernel<ST, OT, TERMS == 1 ? 2 : TERMS, ACT>), grid, block, 0, s, st, r, states);
+    else if (o.ft_terms == 3) hipLaunchKernelGGL((token_lay_kernel<ST, OT, std::is_same<OT, bf16>::value ? 3 : TERMS, ACT>), grid, block, 0, s, st, r, states);
     else hipLaunchKernelGGL((token_lay_kernel<ST, OT, TERMS, ACT>), grid, block, 0, s, st, r, states);
     if (e == hipSuccess) e = hipGetLastError();
   };
@@ -454,9 +458,9 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
     q.out = part + (long long)(first / o.unit) * p.B;
     if (o.keep) {
       q.kept = ws + o.kept; q.out_ld = o.Vp; q.out_rows = o.Bk;
-      e = launch_token_keep(q, storage, o.tile, o.two, s);
+      e = launch_token_keep(q, storage, o.tile, o.ways, s);
     } else {
-      e = launch_token_stats(q, storage, o.tile, o.two, s);
+      e = launch_token_stats(q, storage, o.tile, o.ways, s);
     }
   }
   if (e != hipSuccess) return e;
@@ -493,7 +497,7 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
       const Errors er{p.V, p.B, Vp, o.Bk, o.unit, units, ws + o.kept, at(o.et), part, reinterpret_cast<const float*>(ws + o.logit),
                       p.loss, reinterpret_cast<const float2*>(ws + o.norm), p.targets, scale};
       const dim3 grid((unsigned)((long long)o.Bk * (joined ? 1 : (Vp + 2047) / 2048)));
-      constexpr int MORE = TERMS == 3 ? 3 : 2;
+      constexpr int MORE = std::is_same<OT, bf16>::value ? 3 : 2;
       if (o.e_terms == 1 && joined) hipLaunchKernelGGL((token_errors_kernel<OT, TERMS, true>), grid, dim3(256), 0, s, er);
       else if (o.e_terms == 1) hipLaunchKernelGGL((token_errors_kernel<OT, TERMS, false>), grid, dim3(256), 0, s, er);
       else if (joined) hipLaunchKernelGGL((token_errors_kernel<OT, MORE, true>), grid, dim3(256), 0, s, er);

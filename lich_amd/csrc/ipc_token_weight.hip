@@ -68,20 +68,20 @@ __global__ void __launch_bounds__(256) token_finish_kernel(const TokenFinish p) 
   finish<ST>(p, red, blockIdx.x);
 }
 
-template <typename OT, int TERMS, int ST>
+template <typename OT, int TERMS, int ST, typename WT>
 __global__ void __launch_bounds__(256) token_weight_finish_kernel(const TokenGemm p, const TokenFinish f, unsigned first) {
   extern __shared__ __align__(16) unsigned char smem[];
   if (blockIdx.x < first) {
-    finish<typename std::conditional<TERMS == 3, float, OT>::type>(f, reinterpret_cast<float*>(smem), blockIdx.x);
+    finish<WT>(f, reinterpret_cast<float*>(smem), blockIdx.x);
     return;
   }
-  token::product_tile<OT, TERMS, TOKEN_WEIGHT, false, 64, 64, 2, 2, ST>(p, smem, blockIdx.x - first, gridDim.x - first);
+  token::product_tile<OT, TERMS, TOKEN_WEIGHT, 1, 64, 64, 2, 2, ST, WT>(p, smem, blockIdx.x - first, gridDim.x - first);
 }
 
-template <typename OT, int TERMS, int ST>
+template <typename OT, int TERMS, int ST, typename WT>
 hipError_t weight_finish(const TokenGemm& p, const TokenFinish& f, hipStream_t s) {
-  constexpr int smem = token::tile_lds<TERMS, TOKEN_WEIGHT, false, 64, 64, 2, 2, ST>();
-  const void* fn = reinterpret_cast<const void*>(&token_weight_finish_kernel<OT, TERMS, ST>);
+  constexpr int smem = token::tile_lds<TERMS, TOKEN_WEIGHT, 1, 64, 64, 2, 2, ST>();
+  const void* fn = reinterpret_cast<const void*>(&token_weight_finish_kernel<OT, TERMS, ST, WT>);
   static const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != hipSuccess) return e;
   TokenGemm q = p;
@@ -91,24 +91,24 @@ hipError_t weight_finish(const TokenGemm& p, const TokenFinish& f, hipStream_t s
   return hipLaunchKernel(fn, dim3(first + (unsigned)(((p.M + 63LL) / 64) * ((p.N + 63LL) / 64))), dim3(256), args, smem, s);
 }
 
-template <typename OT, int TERMS>
+template <typename OT, int TERMS, typename WT>
 hipError_t weight(const TokenGemm& p, const TokenFinish* f, int storage, hipStream_t s) {
   auto tiles = [&](long long e) { return ((p.M + e - 1) / e) * ((p.N + e - 1) / e); };
   if (tiles(128) <= 128 && f) {
     if constexpr (TERMS == 3) {
-      if (tiles(64) > 256) return weight_finish<OT, TERMS, 3>(p, *f, s);
+      if (tiles(64) > 256) return weight_finish<OT, TERMS, 3, WT>(p, *f, s);
     }
-    return weight_finish<OT, TERMS, TERMS == 3 ? 6 : 8 / TERMS>(p, *f, s);
+    return weight_finish<OT, TERMS, TERMS == 3 ? 6 : 8 / TERMS, WT>(p, *f, s);
   }
   if (f) {
     const hipError_t e = launch_token_finish(*f, storage, s);
     if (e != hipSuccess) return e;
   }
   if constexpr (TERMS == 1) {
-    if (tiles(256) >= 160) return token::run_tile<OT, TERMS, TOKEN_WEIGHT, false, 256, 256, 2, 4>(p, s);
+    if (tiles(256) >= 160) return token::run_tile<OT, TERMS, TOKEN_WEIGHT, 1, 256, 256, 2, 4>(p, s);
   }
-  if (tiles(128) > 128) return token::run_tile<OT, TERMS, TOKEN_WEIGHT, false, 128, 128, 2, 2, TERMS == 3 ? 3 : 4>(p, s);
-  return token::run_narrow<OT, TERMS, TOKEN_WEIGHT, false, 2, 2>(p, s);
+  if (tiles(128) > 128) return token::run_tile<OT, TERMS, TOKEN_WEIGHT, 1, 128, 128, 2, 2, TERMS == 3 ? 3 : 4, WT>(p, s);
+  return token::run_narrow<OT, TERMS, TOKEN_WEIGHT, 1, 2, 2, WT>(p, s);
 }
 
 }  // namespace
@@ -122,9 +122,9 @@ hipError_t launch_token_finish(const TokenFinish& p, int storage, hipStream_t s)
 }
 
 hipError_t launch_token_weight(const TokenGemm& p, const TokenFinish* f, int storage, int terms, hipStream_t s) {
-  if (storage == 0) return weight<bf16, 3>(p, f, storage, s);
-  if (terms == 2) return storage == 1 ? weight<f16, 2>(p, f, storage, s) : weight<bf16, 2>(p, f, storage, s);
-  return storage == 1 ? weight<f16, 1>(p, f, storage, s) : weight<bf16, 1>(p, f, storage, s);
+  if (storage == 0) return weight<bf16, 3, float>(p, f, storage, s);
+  if (storage == 1) return terms == 2 ? weight<f16, 2, f16>(p, f, storage, s) : weight<f16, 1, f16>(p, f, storage, s);
+  return terms == 3 ? weight<bf16, 3, bf16>(p, f, storage, s) : weight<bf16, 1, bf16>(p, f, storage, s);
 }
 
 }  // namespace ipc
