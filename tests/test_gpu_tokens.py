@@ -230,6 +230,41 @@ def test_token_update_in_pieces(V, D, B, name):
     check(wn, w.double() + 2.0 * r["dw"], bw, "w")
 
 
+# Weights in 16 bits are the roundings of sums that are good to a few H, where an operand rounded to
+# 16 bits would leave u: a weight may differ from the exact sum's rounding only where that
+# lies within the sums' bound of a tie.  e: of small calls as fp32, of large ones (the last two) that of the
+# targets alone; the others are probabilities of a large vocabulary.  Sums over the
+# vocabulary are trees of parts: 256 H.
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+@pytest.mark.parametrize("V,D,B,activation", [(400, 6, 9, "relu"), (3000, 8, 12, "gelu"), (90, 7, 40, "silu"), (524301, 8, 17, "relu"),
+                                              (700001, 6, 13, "tanh")])
+def test_weights_round_as_the_exact_sums(V, D, B, activation, name):
+    dt, alpha = TYPES[name], 0.25
+    u, half, few = half_step(dt), dt == torch.float16, V * B <= 1 << 23
+    x, w, t = softmax_case(V, D, B, dt, V + D)
+    got = run_update(x.to(DEV), w.to(DEV), t.to(DEV), activation, alpha)[2].cpu()
+    r = O.softmax(x, w, t, activation)
+    hot = torch.zeros((V, B), dtype=torch.bool)
+    real = (t >= 0) & (t < V)
+    hot[t[real], real.nonzero()[:, 0]] = True
+    exact = activation in ("identity", "relu")
+    fa, ea, p, small = r["f"].abs(), r["e"].abs(), r["p"], 2.0 ** -25 * half
+    fine_df = 0.0 if exact else 18 * H + (0.0 if few else u * u)
+    logit_df = fine_df if few else 0.0 if exact else u + 17 * H
+    dz = (r["size"] * (logit_df + (3 * D + 4) * H)).max(0).values + small * w.double().abs().sum(1).max()
+    de = p * ((2 * dz).expm1() + 8 * H * (1 + p.clamp(min=1e-300).log().abs()) + 256 * H) + 4 * H * ea + 2.0 ** -34 * half + 2.0 ** -38 * (not few)
+    if not few:
+        de = de + torch.where(hot, 0.0, (u + 2.0 ** -11) * ea)
+    left = torch.where(hot | few, fine_df, 0.0 if exact else u + 17 * H)
+    new = w.double() + alpha * r["dw"]
+    bound = alpha * (de @ fa.T + (ea * left) @ fa.T + (3 * B + 10) * H * (ea @ fa.T) + small * ea.sum(1, keepdim=True)) + 2 * H * (new.abs() + (alpha * r["dw"]).abs())
+    low, high = (new - bound).to(dt), (new + bound).to(dt)
+    assert bool(((got >= low) & (got <= high)).all()), int(((got < low) | (got > high)).sum())
+    # (operands rounded to 16 bits would not pass, but where they are e of nearly 1 and an exact f)
+    plain = (w.double() + alpha * (r["e"].to(dt).double() @ r["f"].to(dt).double().T)).to(dt)
+    assert bool(((plain < low) | (plain > high)).any()) or (not few and exact)
+
+
 @pytest.mark.parametrize("name", TYPES)
 @pytest.mark.parametrize("V,D,B", [(10, 64, 128), (1000, 37, 130), (2001, 300, 257), (33000, 40, 7)])
 def test_padded_columns_hold_anything(V, D, B, name):
