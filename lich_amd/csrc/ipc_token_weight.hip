@@ -68,47 +68,54 @@ __global__ void __launch_bounds__(256) token_finish_kernel(const TokenFinish p) 
   finish<ST>(p, red, blockIdx.x);
 }
 
-template <typename OT, int TERMS, int ST, typename WT>
+// Workgroups 0 .. first - 1: the gradient's last step; the others: W.
+template <typename OT, int TERMS, int E, int ST, typename WT>
 __global__ void __launch_bounds__(256) token_weight_finish_kernel(const TokenGemm p, const TokenFinish f, unsigned first) {
   extern __shared__ __align__(16) unsigned char smem[];
   if (blockIdx.x < first) {
     finish<WT>(f, reinterpret_cast<float*>(smem), blockIdx.x);
     return;
   }
-  token::product_tile<OT, TERMS, TOKEN_WEIGHT, 1, 64, 64, 2, 2, ST, WT>(p, smem, blockIdx.x - first, gridDim.x - first);
+  token::product_tile<OT, TERMS, TOKEN_WEIGHT, 1, E, E, 2, 2, ST, WT>(p, smem, blockIdx.x - first, gridDim.x - first);
 }
 
-template <typename OT, int TERMS, int ST, typename WT>
-hipError_t weight_finish(const TokenGemm& p, const TokenFinish& f, hipStream_t s) {
-  constexpr int smem = token::tile_lds<TERMS, TOKEN_WEIGHT, 1, 64, 64, 2, 2, ST>();
-  const void* fn = reinterpret_cast<const void*>(&token_weight_finish_kernel<OT, TERMS, ST, WT>);
+// With the gradient's last step, if there is one (its 256 threads are those of a workgroup here).
+template <typename OT, int TERMS, int E, int ST, typename WT>
+hipError_t weight_finish(const TokenGemm& p, const TokenFinish* f, hipStream_t s) {
+  if (!f) return token::run_tile<OT, TERMS, TOKEN_WEIGHT, 1, E, E, 2, 2, ST, WT>(p, s);
+  constexpr int smem = token::tile_lds<TERMS, TOKEN_WEIGHT, 1, E, E, 2, 2, ST>();
+  const void* fn = reinterpret_cast<const void*>(&token_weight_finish_kernel<OT, TERMS, E, ST, WT>);
   static const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != hipSuccess) return e;
   TokenGemm q = p;
-  TokenFinish g = f;
+  TokenFinish g = *f;
   unsigned first = finish_blocks(g);
   void* args[] = {&q, &g, &first};
-  return hipLaunchKernel(fn, dim3(first + (unsigned)(((p.M + 63LL) / 64) * ((p.N + 63LL) / 64))), dim3(256), args, smem, s);
+  return hipLaunchKernel(fn, dim3(first + (unsigned)(((p.M + E - 1LL) / E) * ((p.N + E - 1LL) / E))), dim3(256), args, smem, s);
 }
 
 template <typename OT, int TERMS, typename WT>
 hipError_t weight(const TokenGemm& p, const TokenFinish* f, int storage, hipStream_t s) {
   auto tiles = [&](long long e) { return ((p.M + e - 1) / e) * ((p.N + e - 1) / e); };
-  if (tiles(128) <= 128 && f) {
-    if constexpr (TERMS == 3) {
-      if (tiles(64) > 256) return weight_finish<OT, TERMS, 3, WT>(p, *f, s);
-    }
-    return weight_finish<OT, TERMS, TERMS == 3 ? 6 : 8 / TERMS, WT>(p, *f, s);
-  }
-  if (f) {
+  const bool large = TERMS == 1 && tiles(256) >= 160;
+  // (many of the last step's workgroups would wait for LDS that they do not use: us, in one launch / two, fp32
+  // 4000 x 4000 x 512 343 / 339, bf16 20000 x 128 x 256 63 / 69)
+  if (f && (large || finish_blocks(*f) > 512)) {
     const hipError_t e = launch_token_finish(*f, storage, s);
     if (e != hipSuccess) return e;
+    f = nullptr;
   }
   if constexpr (TERMS == 1) {
-    if (tiles(256) >= 160) return token::run_tile<OT, TERMS, TOKEN_WEIGHT, 1, 256, 256, 2, 4>(p, s);
+    if (large) return token::run_tile<OT, TERMS, TOKEN_WEIGHT, 1, 256, 256, 2, 4>(p, s);
   }
-  if (tiles(128) > 128) return token::run_tile<OT, TERMS, TOKEN_WEIGHT, 1, 128, 128, 2, 2, TERMS == 3 ? 3 : 4, WT>(p, s);
-  return token::run_narrow<OT, TERMS, TOKEN_WEIGHT, 1, 2, 2, WT>(p, s);
+  // (narrow tiles where wide ones are mostly padding and a product is a few steps: us, 128 / 64 wide, fp32 10007 x 515 x 77
+  // 73 / 70, 50000 x 64 x 16 62 / 54; where they are not, 32000 x 4096 x 4 241 / 265)
+  const int wide = (p.N + 127) / 128 * 128, narrow = (p.N + 63) / 64 * 64;
+  if (tiles(128) > 128 && !(wide - wide / 16 > narrow && (p.K <= 128 || p.N <= 64))) return weight_finish<OT, TERMS, 128, TERMS == 3 ? 3 : 4, WT>(p, f, s);
+  if constexpr (TERMS == 3) {
+    if (tiles(64) > 256) return weight_finish<OT, TERMS, 64, 3, WT>(p, f, s);
+  }
+  return weight_finish<OT, TERMS, 64, TERMS == 3 ? 6 : 8 / TERMS, WT>(p, f, s);
 }
 
 }  // namespace
