@@ -96,7 +96,8 @@ bool make_plan(int V, int D, int B, int storage, int act, bool update, Plan& o) 
   else if (columns <= 64) o.tile = o.rows >= 32768 ? TILE_128_64 : TILE_64;
   else o.tile = storage != DT_F32 && tiles(o.rows, columns, 256) >= 192 ? TILE_256 : tiles(o.rows, columns, 128) > 128 ? TILE_128 : storage == DT_F32 && (o.rows + 127LL) / 128 * ((columns + 63) / 64) >= 128 ? TILE_128_64 : TILE_64;
   o.unit = token_unit(o.tile, o.ways);
-  o.grad_tile = storage != DT_F32 && D >= 256 && B >= 256 ? 256 : D > 64 ? 128 : 64;
+  // (few tiles: narrow ones, with longer slices: us, fp32 10007 x 515 x 77 70.4 / 70.0, bf16 1000 x 1000 x 128 35.7 / 34.2)
+  o.grad_tile = storage != DT_F32 && D >= 256 && B >= 256 ? 256 : D > 64 && tiles(D, B, 128) > 8 ? 128 : 64;
   const long long gt = o.grad_tile == 256 ? tiles(D, B, 256)
                        : o.grad_tile == 128 ? (D + 127LL) / 128 * (B > 64 ? (B + 127LL) / 128 : 1) : tiles(D, B, 64);
   const long long stages = o.Vp / 32;
