@@ -72,22 +72,28 @@ bool make_plan(int V, int D, int B, int storage, int act, bool update, Plan& o) 
   const long long work = (long long)V * B;
   const bool few = storage != DT_F32 && work <= kFineErrors && work * D <= kFineWork;
   const int most = storage == DT_BF16 ? 3 : 2;
-  o.fine = update && few;
-  o.mend = update && storage != DT_F32 && !o.fine;
-  o.fix = inexact && o.mend;
-  o.ways = o.fine || (inexact && !update) ? few ? most : 2 : 1;
-  o.ft_terms = storage == DT_F32 ? 3 : o.fix ? 2 : o.ways;
-  o.f_terms = o.e_terms = storage == DT_F32 ? 3 : o.fine ? most : 1;
   const long long state = 2LL * o.Dp * o.Bk;
-  if (state * o.ft_terms > kOperand) return false;
-  const long long row_w = 2LL * (o.copy ? o.terms * o.Dp : D), row_e = update ? 2LL * o.e_terms * o.Bk : 1;
-  long long rows = std::min((o.copy ? kPieceBytes : kOperand) / row_w, kPieceBytes / row_e) / 256 * 256;
-  if (rows < 256) rows = 256;
-  if (rows * std::max(row_w, row_e) > kOperand && std::min<long long>(rows, up(V, 32)) * std::max(row_w, row_e) > kOperand) return false;
-  o.rows = (int)std::min<long long>(rows, V);
+  // the rows of a piece, 0 for sizes that the kernels do not take
+  auto pieces = [&](bool fine) -> long long {
+    o.fine = fine;
+    o.mend = update && storage != DT_F32 && !fine;
+    o.fix = inexact && o.mend;
+    o.ways = fine || (inexact && !update) ? few && state * most <= kOperand ? most : 2 : 1;
+    o.ft_terms = storage == DT_F32 ? 3 : o.fix ? 2 : o.ways;
+    o.f_terms = o.e_terms = storage == DT_F32 ? 3 : fine ? most : 1;
+    if (state * o.ft_terms > kOperand) return 0;
+    const long long row_w = 2LL * (o.copy ? o.terms * o.Dp : D), row_e = update ? 2LL * o.e_terms * o.Bk : 1;
+    long long rows = std::min((o.copy ? kPieceBytes : kOperand) / row_w, kPieceBytes / row_e) / 256 * 256;
+    if (rows < 256) rows = 256;
+    rows = std::min<long long>(rows, V);
+    return up(rows, 32) * std::max(row_w, row_e) > kOperand ? 0 : rows;
+  };
+  long long rows = pieces(update && few);
+  if (o.fine && rows < V) rows = pieces(false);  // (weights of more than a piece: not a small call)
+  if (rows == 0) return false;
+  o.rows = (int)rows;
   o.Vp = (int)up(o.rows, 32);
   o.keep = update && o.rows == V && (storage != DT_F32 || (long long)o.Bk * o.Vp * 10 <= kPieceBytes);
-  if (o.fine && !o.keep) return false;  // (never: its errors are few)
   auto tiles = [&](long long m, long long n, long long e) { return ((m + e - 1) / e) * ((n + e - 1) / e); };
   const long long columns = (long long)o.ways * B;
   // (the largest tile that gives the CUs one each; fp32: us, 64 wide / 128 x 64, 4000 x 4000 x 512 update 355 / 336,

@@ -98,7 +98,7 @@ class TokenNet(CompactNet):
 def train(dataset, *, context=4, width=32, hidden=(64,), batch=128, epochs=4, rate=0.5, p=0.0, activation="tanh",
           dtype=torch.float32, seed=0, device=None, log=print):
     """Trains a ``TokenNet`` on a ``TokenDataset``; returns (records, net)."""
-    device = torch.device(device or "cuda", 0)
+    device = torch.device("cuda", 0) if device is None else torch.device(device)
     net = TokenNet(dataset.vocab, context, width, hidden, batch, activation, dtype, rate, p, device=device, seed=seed)
     records = []
     for epoch in range(epochs):

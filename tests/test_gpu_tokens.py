@@ -265,6 +265,23 @@ def test_weights_round_as_the_exact_sums(V, D, B, activation, name):
     assert bool(((plain < low) | (plain > high)).any()) or (not few and exact)
 
 
+# weights of more than a piece under few columns
+@pytest.mark.parametrize("V,D,B,name", [(300001, 2001, 1, "bf16"), (600001, 2000, 2, "f16")])
+def test_token_update_of_a_large_table_and_one_sample(V, D, B, name):
+    dt = TYPES[name]
+    g = torch.Generator(device=DEV).manual_seed(V)
+    x, t = torch.randn((D, B), generator=g, device=DEV).to(dt), torch.tensor([V - 1, 5][:B], device=DEV)
+    w = torch.empty((V, D), dtype=dt, device=DEV).normal_(generator=g).mul_(2.0 / D ** 0.5)
+    loss, gx, wn = run_update(x, w, t, "silu", 0.5)
+    r = O.softmax(x, w, t, "silu")
+    bl, bg, bw = softmax_bounds(r, w, dt, V, D, B, "silu", 0.5)
+    check(loss, r["loss"], bl, "loss")
+    check(gx, r["g"], bg, "g")
+    for rows in (slice(0, 2000), slice(V // 2, V // 2 + 2000), slice(V - 2000, V)):
+        check(wn[rows], w[rows].double() + 0.5 * r["dw"][rows], bw[rows], "w")
+    assert bool(torch.isfinite(wn).all())
+
+
 @pytest.mark.parametrize("name", TYPES)
 @pytest.mark.parametrize("V,D,B", [(10, 64, 128), (1000, 37, 130), (2001, 300, 257), (33000, 40, 7)])
 def test_padded_columns_hold_anything(V, D, B, name):

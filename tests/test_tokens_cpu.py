@@ -61,6 +61,16 @@ def test_workspaces():
     assert update(1 << 20, 64, 4096, 2, 0) < 3 << 30
 
 
+@pytest.mark.parametrize("storage", [0, 1, 2])
+@pytest.mark.parametrize("V,D,B", [(300001, 2001, 1), (700001, 2000, 1), (1 << 20, 2047, 1), (1, 1, 1 << 22), (2, 8, 1 << 21), (1, 60, 8000000)])
+def test_calls_of_few_products_over_large_tensors_are_taken(V, D, B, storage):
+    """A vocabulary whose weights take more than a piece, and states that do not fit in three terms."""
+    lib = nat.lib()
+    fits = storage != 0 or D * B < 1 << 28
+    assert (lib.ipc_token_update_workspace_bytes(V, D, B, storage, 2) > 0) == fits
+    assert (lib.ipc_token_loss_workspace_bytes(V, D, B, storage, 2) > 0) == fits
+
+
 def test_builders_refuse():
     for bad in (dict(p=1.0), dict(p=-0.1), dict(p=1 - 2.0 ** -18), dict(p=float("nan")), dict(site=-1), dict(site=2 ** 31)):
         with pytest.raises(ValueError):
