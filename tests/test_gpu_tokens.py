@@ -134,6 +134,39 @@ def test_dropout_of_a_view_off_16_bytes():
     assert torch.equal(out[1:-1].reshape(M, B), want) and float(out[0]) == float(out[-1]) == 9.0
 
 
+# ------------------------------------------- tensors of more than 2^32 bytes
+def test_rows_behind_four_gigabytes():
+    V, D, C, B = 1100000, 1944, 2, 300
+    table = torch.empty((V, D), dtype=torch.bfloat16, device=DEV)
+    last = 700
+    table[:last].normal_()
+    table[-last:].normal_()
+    ids = torch.cat([torch.randint(0, last, (1, B), device=DEV), torch.randint(V - last, V, (1, B), device=DEV)])
+    x = torch.empty((C * D, B), dtype=torch.bfloat16, device=DEV)
+    tokens.build_embedding(V, D, C, B, "bfloat16", 1.0)(ids, table, x)
+    assert torch.equal(x.reshape(C, D, B).transpose(1, 2), table[ids])
+    far, near = table[-last:].clone(), table[:last].clone()
+    k = tokens.build_embedding_update(V, D, C, B, "bfloat16", 0.5)
+    k(table, ids, x, workspace=k.new_workspace(DEV))
+    for part, old, rows in ((ids[0], near, table[:last]), (ids[1] - (V - last), far, table[-last:])):
+        want = old.clone()
+        small = tokens.build_embedding_update(last, D, 1, B, "bfloat16", 0.5)
+        # (the same sums in other runs: one more rounding each of at most 300 fp32 additions)
+        small(want, part.reshape(1, B), old[part].t().contiguous(), workspace=small.new_workspace(DEV))
+        assert bool(((want.double() - rows.double()).abs() <= 2 * half_step(torch.bfloat16) * rows.double().abs() + 2.0 ** -12).all())
+
+
+def test_dropout_behind_four_gigabytes():
+    M, B = 40001, 53001
+    x = torch.empty((M, B), dtype=torch.bfloat16, device=DEV)
+    x[-1] = 1.0
+    tokens.build_dropout(M, B, "bfloat16", 0.5, site=3)(x, torch.tensor([9, 8], device=DEV), x)
+    got = x[-1].cpu()
+    for i in (M * B - 1, M * B - 100, M * B - B):
+        word = O.philox((i // 8, 3, 8, 0), (9, 0))[i % 8 // 2]
+        assert float(got[i - (M - 1) * B]) == (2.0 if (word >> (16 * (i % 2))) & 0xFFFF >= 32768 else 0.0)
+
+
 # -------------------------------------------------------------------- softmax
 def softmax_bounds(r, w, dt, V, D, B, activation, alpha, update=True):
     """Per element: what loss, G and W may be off by."""
