@@ -30,26 +30,39 @@ __global__ void __launch_bounds__(256) embed_kernel(const EmbedProblem p) {
   const int d0 = td * DT, b0 = tb * BT, tid = threadIdx.x;
   const ST* table = static_cast<const ST*>(p.table);
   ST* x = static_cast<ST*>(p.x);
-  for (int u = tid; u < BT * DT / 4; u += 256) {
-    const int r = u / (DT / 4), d = d0 + u % (DT / 4) * 4, b = b0 + r;
-    if (b >= p.B || d >= p.D) continue;
-    const long long id = p.ids[(long long)c * p.B + b];
-    const bool real = id >= 0 && id < p.V;
-    const ST* from = table + (real ? id : 0) * p.D + d;
-    float v[4] = {};
-    if (real) {
-      if (p.vec_d) {
-        load4(from, v);
-      } else {
+  // every id, then every row's part, then the rest: two waits for memory in all
+  constexpr int EACH = BT * DT / 1024;
+  long long id[EACH];
+  Four<ST> v[EACH];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (d + i < p.D) v[i] = to_f32(from[i]);
-      }
+  for (int e = 0; e < EACH; ++e) {
+    const int b = b0 + (e * 256 + tid) / (DT / 4);
+    id[e] = b < p.B ? p.ids[(long long)c * p.B + b] : -1;
+  }
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int d = d0 + (e * 256 + tid) % (DT / 4) * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[e].v[i] = cvt<ST>(0.0f);
+    if (id[e] < 0 || id[e] >= p.V || d >= p.D) continue;
+    const ST* from = table + id[e] * p.D + d;
+    if (p.vec_d) {
+      v[e] = *reinterpret_cast<const Four<ST>*>(__builtin_assume_aligned(from, 4 * sizeof(ST)));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (d + i < p.D) v[e].v[i] = from[i];
     }
+  }
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int u = e * 256 + tid, r = u / (DT / 4), d = d0 + u % (DT / 4) * 4;
+    const bool real = id[e] >= 0 && id[e] < p.V;
     ST o[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = real ? cvt<ST>(v[i] * p.scale) : cvt<ST>(0.0f);
+    for (int i = 0; i < 4; ++i) o[i] = real ? cvt<ST>(to_f32(v[e].v[i]) * p.scale) : cvt<ST>(0.0f);
     if constexpr (BT == 1) {  // (one sample: X is as long as the row)
+      if (d >= p.D) continue;
       ST* to = x + (long long)c * p.D + d;
       if (p.vec_d && p.vec_b) {
         store4(to, o);
