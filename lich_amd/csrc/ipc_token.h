@@ -89,6 +89,10 @@ struct TokenProblem {
 // 0: sizes that the kernels do not take
 long long token_workspace_bytes(int V, int D, int B, int storage, int act, bool update);
 hipError_t launch_token(const TokenProblem& p, int storage, hipStream_t s);
+// A few samples, W as it lies.
+bool token_few(int V, int D, int B, int storage);
+long long token_few_workspace_bytes(int V, int D, int B, int storage, bool update);
+hipError_t launch_token_few(const TokenProblem& p, int storage, hipStream_t s);
 // A small one in one workgroup, without a workspace.
 bool token_small(int V, int D, int B);
 hipError_t launch_token_small(const TokenProblem& p, int storage, hipStream_t s);

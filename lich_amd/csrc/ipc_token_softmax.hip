@@ -561,12 +561,14 @@ hipError_t by_act(const TokenProblem& p, int storage, hipStream_t s) {
 }  // namespace
 
 long long token_workspace_bytes(int V, int D, int B, int storage, int act, bool update) {
+  if (token_few(V, D, B, storage)) return token_few_workspace_bytes(V, D, B, storage, update);
   Plan o;
   return make_plan(V, D, B, storage, act, update, o) ? o.bytes : 0;
 }
 
 hipError_t launch_token(const TokenProblem& p, int storage, hipStream_t s) {
   if (token_small(p.V, p.D, p.B)) return launch_token_small(p, storage, s);
+  if (token_few(p.V, p.D, p.B, storage)) return launch_token_few(p, storage, s);
   if (storage == DT_F32) return by_act<float, bf16, 3>(p, storage, s);
   return storage == DT_F16 ? by_act<f16, f16, 1>(p, storage, s) : by_act<bf16, bf16, 1>(p, storage, s);
 }

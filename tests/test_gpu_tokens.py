@@ -298,8 +298,27 @@ def test_weights_round_as_the_exact_sums(V, D, B, activation, name):
     assert bool(((plain < low) | (plain > high)).any()) or (not few and exact)
 
 
+# a few samples: every number of them, rows that end inside 16 bytes, one piece of a row or many
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("V,D,B", [(9, 8, 1), (1000, 9, 2), (700, 15, 1), (257, 129, 3), (40, 513, 4), (6001, 701, 3), (2500, 2055, 4), (513, 520, 5),
+                                   (90, 1021, 7), (3, 300, 8), (33, 36000, 1), (20000, 16, 2)])
+def test_a_few_samples(V, D, B, name):
+    dt = TYPES[name]
+    activation = ["tanh", "identity", "gelu", "relu", "silu", "sigmoid"][(V + D + B) % 6]
+    x, w, t = softmax_case(V, D, B, dt, V + D + B, padded=0.0 if B == 1 else 0.3)
+    loss, g, wn = run_update(x.to(DEV), w.to(DEV), t.to(DEV), activation, 0.25)
+    r = O.softmax(x, w, t, activation)
+    bl, bg, bw = softmax_bounds(r, w, dt, V, D, B, activation, 0.25)
+    check(loss, r["loss"], bl, "loss")
+    check(g, r["g"], bg, "g")
+    check(wn, w.double() + 0.25 * r["dw"], bw, "w")
+    k, alone = tokens.build_token_loss(V, D, B, activation, dt), torch.full((B,), float("nan"), device=DEV)
+    k(x.to(DEV), w.to(DEV), t.to(DEV), alone, workspace=k.new_workspace(DEV))
+    check(alone, r["loss"], softmax_bounds(r, w, dt, V, D, B, activation, 0.0, False)[0], "the loss alone")
+
+
 # weights of more than a piece under few columns
-@pytest.mark.parametrize("V,D,B,name", [(300001, 2001, 1, "bf16"), (600001, 2000, 2, "f16")])
+@pytest.mark.parametrize("V,D,B,name", [(300001, 2001, 1, "bf16"), (600001, 2000, 2, "f16"), (14001, 40001, 1, "bf16"), (30000, 40000, 1, "f16")])
 def test_token_update_of_a_large_table_and_one_sample(V, D, B, name):
     dt = TYPES[name]
     g = torch.Generator(device=DEV).manual_seed(V)
@@ -477,7 +496,7 @@ class Fenced:
 @pytest.mark.parametrize("name", TYPES)
 @pytest.mark.parametrize("activation", ["identity", "tanh"])
 @pytest.mark.parametrize("V,D,B", [(2, 1, 1), (10, 64, 128), (999, 77, 3), (300, 131, 90), (26240, 1, 70), (7001, 65, 1), (700, 200, 300),
-                                   (164, 2, 188), (5000, 35, 520)])
+                                   (164, 2, 188), (5000, 35, 520), (1000, 9, 2), (6001, 701, 3), (520, 130, 8)])
 def test_softmax_calls_stay_inside_their_tensors(V, D, B, activation, name):
     """Also inside the workspace's stated size; room behind each as large as the workspace itself."""
     dt = TYPES[name]

@@ -62,7 +62,7 @@ def test_workspaces():
 
 
 @pytest.mark.parametrize("storage", [0, 1, 2])
-@pytest.mark.parametrize("V,D,B", [(300001, 2001, 1), (700001, 2000, 1), (1 << 20, 2047, 1), (1, 1, 1 << 22), (2, 8, 1 << 21), (1, 60, 8000000)])
+@pytest.mark.parametrize("V,D,B", [(300001, 2001, 1), (14001, 40001, 1), (30000, 40000, 1), (700001, 2000, 1), (1 << 20, 2047, 1), (1, 1, 1 << 22), (2, 8, 1 << 21), (1, 60, 8000000)])
 def test_calls_of_few_products_over_large_tensors_are_taken(V, D, B, storage):
     """A vocabulary whose weights take more than a piece, and states that do not fit in three terms."""
     lib = nat.lib()
