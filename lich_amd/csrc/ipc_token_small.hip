@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(kThreads) token_small_kernel(const TokenProble
     const int v = i / B * 4, b = i % B;
     float z[4] = {};
     int d = 0;
-#pragma unroll 1
+#pragma unroll 4
     for (; d + 4 <= D; d += 4) {
       const float g[4] = {f[d * RB + b], f[(d + 1) * RB + b], f[(d + 2) * RB + b], f[(d + 3) * RB + b]};
 #pragma unroll
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(kThreads) token_small_kernel(const TokenProble
 
 // One workgroup is slow at anything long: the steps that its threads take one after the other are
 // counted.  us, in one / in the launches of the general path, fp32: 10 x 64 x 128 (V, D, B; 82
-// steps) 11.5 / 21.6; 64 x 64 x 64 (152) 18 / 23.6; 10 x 256 x 100 (225) 30.6 / 26; 1844 x 4 x 1 (1877) 76 / 22.
+// steps) 11.3 / 21.6; 64 x 64 x 64 (152) 18 / 23.6; 10 x 256 x 100 (225) 30.6 / 26; 1844 x 4 x 1 (1877) 76 / 22.
 bool token_small(int V, int D, int B) {
   constexpr long long most = 1 << 14;
   if ((long long)V * D > most || (long long)D * B > most || (long long)V * B > most || small_lds(V, D, B) > kLds) return false;
