@@ -620,12 +620,17 @@ int ipc_dropout(const void* x, const long long* rng, void* out, int M, int B, in
  *   ipc_token_loss    loss[b] = log sum_v exp z[v][b] - z[targets[b]][b]
  *   ipc_token_update  that, and with e = onehot - softmax(z), a descent direction:
  *                     g = f'(X) W^T e (w as it was), then w += alpha e f(X)^T
- * A padded column has loss 0, no share of w and zeros in g, whatever x holds there.  The
- * logits are never kept: they are formed in pieces of the vocabulary of at most 2^30 bytes
- * of errors.  Sums are in fp32 in a fixed order; fp32 products are sums of bf16 ones
- * exact to 2^-24, in which an infinite weight or state counts as the largest bf16; in 16-bit
- * storage f(X) and e are rounded to the type (the loss knows f(X) to twice its digits, the
- * update's to first order in what the rounding left).
+ * A padded column has loss 0, no share of w and zeros in g, whatever x holds there.  What
+ * is kept of the logits is bounded: errors of pieces of the vocabulary of at most 2^30
+ * bytes each, and for at most 8 samples the logits.  Sums are in fp32 in a fixed order.
+ *   - at most 8 samples in fp32, 2 in 16 bits (4 where w has 2^22 values and more): fp32 products
+ *     of the values as they are;
+ *   - fp32: products of three bf16 terms each, exact to 2^-24, in which an infinite weight
+ *     or state counts as the largest bf16;
+ *   - 16 bits: w as it is; the loss alone takes f(X) in two terms of the type, a small call
+ *     (at most 2^23 errors and 2^31 multiplications) f(X) and e in two fp16 or three bf16 terms.  A
+ *     larger update rounds both to the type once, makes the sums of the targets' rows
+ *     good in fp32 and corrects the loss to first order in what f(X)'s rounding left.
  * Both need a workspace (16-byte aligned) of ipc_token_loss_workspace_bytes /
  * ipc_token_update_workspace_bytes bytes (0: refused).  w of 16 bits with an even D
  * lies on 4 bytes.

@@ -5,7 +5,14 @@
 //
 // Both move bytes and little else.  The table has a token's features next to each
 // other, a state has the samples there, so a block of 64 samples by 64 features turns
-// in LDS and both sides see runs of 128 bytes (16-bit).
+// in LDS and both sides see runs of 128 bytes (16-bit).  512 features of 8 x 1024 places,
+// bf16: 5.7 us, 2.1 TB/s of 12 MB that need be moved, 2.3 of it the launch.
+//
+// The update sorts the places by id, so that every sum has one owner and one order
+// (atomics would add in any), in three launches: sort, with G transposed beside it (12.5 us; the
+// sort alone 8.6, each of 256 workgroups reading all 8192 ids), sums of 16 places (6.5), sums that
+// cross those (4.6).  Together 23 us for 8192 places of 512 features in bf16, where 15 MB
+// take 3: launches and the waits for memory between dependent steps.
 #include "ipc_device.h"
 #include "ipc_token.h"
 

@@ -8,6 +8,8 @@
 // how many launches stand beside them: once for the loss (logits and each workgroup's
 // largest and sum, then these joined), twice read and once written for the update, whose
 // second pass takes the gradient's share of a row of W before it writes the new row.
+// 32000 x 4096 bf16, one sample: logits 41.7 us (6.3 TB/s), the loss 55 in all with W cold; update
+// 134, where three passes of W take 154 at a copy's rate (part of W is still in the cache).
 #include <algorithm>
 
 #include "ipc_token_gemm.h"

@@ -12,6 +12,7 @@
 // 4. Every piece: its errors in 16 bits (fp32: three terms), its share of W^T e, and its
 //    rows of W, which nothing reads any more.
 // 5. The shares added in order, times f'(X) (small: in the launch that updates W).
+// A small output layer has ipc_token_small.hip, a few samples ipc_token_few.hip.
 //
 // Errors: a vocabulary whose errors fit one piece (1 GiB) has its exponentials kept there by step
 // 2, relative to their part's largest, and scaled in place: three products.  A

@@ -12,8 +12,9 @@ column of a state.
 * ``build_dropout``: a mask from a counter-based generator, never stored; the
   same call on an error is the backward pass.
 * ``build_token_loss``, ``build_token_update``: softmax cross entropy of the
-  output layer over the vocabulary in pieces, the logits never kept; the update
-  also gives the state's error direction and changes the weights.
+  output layer over the vocabulary in pieces, whose logits are kept for a few
+  samples at most; the update also gives the state's error direction and changes
+  the weights.
 
 Each builder returns a callable that validates its tensors and enqueues on
 torch's current stream, as in ``lich_amd.kernels``; nothing is allocated or
