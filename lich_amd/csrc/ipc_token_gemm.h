@@ -8,10 +8,10 @@
 //   TOKEN_GRAD    P[d][n] = sum_v W[v][d] e[v][n]     (a slice of the vocabulary a workgroup)
 //   TOKEN_WEIGHT  W[v][d] += alpha sum_n e[v][n] F[d][n]
 //
-// v_mfma_f32_32x32x16 tiles in the pipeline of ipc_ckpt_gemm.h: four stages of 32 k filled by
+// v_mfma_f32_32x32x16 tiles in the pipeline of ipc_ckpt_gemm.h: three to eight stages of 32 k filled by
 // LDS-DMA loads, one barrier a stage, loads and the next fragments' reads between the
 // products.  B is k-contiguous in every product (F^T, ET, F lie as that asks); A is for
-// the first two (W), and k-rows read transposed for the others (W, ET), so that one
+// the first three (W), and k-rows read transposed for the others (W, ET), so that one
 // copy of W and one of the errors serve both products they appear in.
 //
 // fp32 tensors: every operand is the sum of three bf16 terms (24 bits, the type's own), and a
@@ -25,7 +25,7 @@
 // workgroup to cover (256 x 128 tiles of three stages, two a CU: TOKEN_WEIGHT 1130-1170).  Matrix
 // units are busy 63, 81 and 66 % of the CUs' cycles.
 //
-// The accumulators of the first two lie with a column n a lane (and rows v in its
+// The accumulators of the first three lie with a column n a lane (and rows v in its
 // registers), so that a column's maximum and sum are the lane's own business up to one
 // exchange between the halves of a wave and one between waves; the others' with four
 // consecutive columns a lane, for the shared tile epilogue.

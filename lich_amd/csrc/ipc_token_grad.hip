@@ -1,4 +1,4 @@
-// ipc_token_grad.hip - the products that take a piece's errors: the state's gradient and W's update.
+// ipc_token_grad.hip - the state's gradient from a piece's errors, the vocabulary cut into slices.
 #include "ipc_token_gemm.h"
 
 namespace ipc {
