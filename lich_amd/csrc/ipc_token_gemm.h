@@ -23,7 +23,8 @@
 // The main loop of a 256 x 256 tile runs at 1.17 PFLOP/s, 0.92 us a stage; beside it stand
 // 9 us a tile of first loads and epilogue, which the LDS that a tile fills leaves no second
 // workgroup to cover (256 x 128 tiles of three stages, two a CU: TOKEN_WEIGHT 1130-1170).  Matrix
-// units are busy 63, 81 and 66 % of the CUs' cycles.
+// units are busy 63, 81 and 66 % of the CUs' cycles, and power holds them: over zeros the whole
+// update takes 2650 us, not 3190.
 //
 // The accumulators of the first three lie with a column n a lane (and rows v in its
 // registers), so that a column's maximum and sum are the lane's own business up to one
