@@ -5,6 +5,7 @@
 //   TOKEN_KEEP    that, and the exponentials, as KEPT[n][v] relative to their wave's largest
 //   TOKEN_ERROR   the same products again; e = onehot - softmax(Z), rounded to the operand
 //                 type and stored transposed, ET[n][v]
+//   TOKEN_ONE     a vocabulary within one tile: losses and errors (as many terms as f(X) has) at once
 //   TOKEN_GRAD    P[d][n] = sum_v W[v][d] e[v][n]     (a slice of the vocabulary a workgroup)
 //   TOKEN_WEIGHT  W[v][d] += alpha sum_n e[v][n] F[d][n]
 //
@@ -37,7 +38,7 @@
 
 namespace ipc {
 
-enum { TOKEN_STATS = 0, TOKEN_KEEP = 1, TOKEN_ERROR = 2, TOKEN_GRAD = 3, TOKEN_WEIGHT = 4 };
+enum { TOKEN_STATS = 0, TOKEN_KEEP = 1, TOKEN_ERROR = 2, TOKEN_GRAD = 3, TOKEN_WEIGHT = 4, TOKEN_ONE = 5 };
 
 // Tiles of the first three: rows (of W) and columns of a workgroup, and the rows of a wave, whose
 // largest values and sums are kept (unit; ways: terms of f(X), side by side in a tile; with three
@@ -62,10 +63,10 @@ struct TokenGemm {
   int out_rows;                    // of ET, N up to a multiple of 32
   int add;                         // GRAD: out holds sums already
   int vec;                         // WEIGHT: out allows 4-element accesses
-  float scal;                      // WEIGHT: alpha; ERROR: the errors' scale
-  // STATS, KEEP, ERROR
+  float scal;                      // WEIGHT: alpha; ERROR, ONE: the errors' scale
+  // STATS, KEEP, ERROR, ONE
   const long long* targets; int first, V;  // first: of the piece's rows
-  float* target_logit;
+  float* target_logit;             // ONE: the losses
   const float* loss;               // ERROR
   const int* slot;                 // WEIGHT, or nullptr: of each row, its row in hot (-1: none), which the sum begins with
   const float* hot; int hot_ld;
@@ -75,6 +76,9 @@ struct TokenGemm {
 // ways: terms of f(X); more than one: the exponentials kept in fp32
 hipError_t launch_token_stats(const TokenGemm& p, int storage, int tile, int ways, hipStream_t s);
 hipError_t launch_token_keep(const TokenGemm& p, int storage, int tile, int ways, hipStream_t s);
+// M at most TOKEN_ONE_ROWS
+constexpr int TOKEN_ONE_ROWS = 128;
+hipError_t launch_token_one(const TokenGemm& p, int storage, int ways, hipStream_t s);
 hipError_t launch_token_error(const TokenGemm& p, int storage, int tile, hipStream_t s);
 hipError_t launch_token_grad(const TokenGemm& p, int storage, int tile, hipStream_t s);
 
@@ -127,9 +131,9 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
   constexpr bool MN = MODE == TOKEN_GRAD || MODE == TOKEN_WEIGHT, COLUMNS = !MN;
   constexpr int NW = WGM * WGN, WTM = BM / WGM, WTN = BN / WGN, RM = WTM / 32, RN = WTN / 32;
   constexpr int RNC = RN / WAYS, BNC = BN / WAYS, WTC = WTN / WAYS;  // blocks and columns of different n
-  constexpr bool SPLIT = TERMS == 3, FINE = SPLIT || (MODE == TOKEN_KEEP && WAYS > 1);  // FINE: kept in fp32
+  constexpr bool SPLIT = TERMS == 3, FINE = SPLIT || ((MODE == TOKEN_KEEP || MODE == TOKEN_ONE) && WAYS > 1);  // FINE: kept in fp32
   constexpr int A_BYTES = BM * 64, B_BYTES = BN * 64, STAGE = TERMS * (A_BYTES + B_BYTES);
-  static_assert(WAYS == 1 || ((MODE == TOKEN_STATS || MODE == TOKEN_KEEP) && TERMS == 1 && RN % WAYS == 0), "terms of f(X)");
+  static_assert(WAYS == 1 || ((MODE == TOKEN_STATS || MODE == TOKEN_KEEP || MODE == TOKEN_ONE) && TERMS == 1 && RN % WAYS == 0), "terms of f(X)");
   constexpr int IA = A_BYTES / 1024 / NW, IB = B_BYTES / 1024 / NW, LPS = TERMS * (IA + IB);  // LDS-DMA loads per wave and stage
   static_assert(IA * 1024 * NW == A_BYTES && IB * 1024 * NW == B_BYTES, "tile / waves");
 
@@ -330,12 +334,12 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
   };
   // Block column j of the accumulators, columns n across the lanes, as rows n of a matrix with
   // v along its rows, through this wave's part of the LDS.  FORM 0: errors in the operand
-  // type (fp32: three terms); 1: exponentials in fp16 times 2^15; 2: in fp32.  Rows and
+  // type (fp32: three terms; ONE: as many as f(X) has); 1: exponentials in fp16 times 2^15; 2: in fp32.  Rows and
   // columns past the ends, up to the matrix's own, hold what the accumulators do there.
   auto store_columns = [&](auto form, int j) {
     constexpr int FORM = decltype(form)::value;
     typedef typename std::conditional<FORM == 2, float, unsigned short>::type U;
-    constexpr int LD = WTM + (FORM == 2 ? 4 : 8), PARTS = FORM == 0 && SPLIT ? 3 : 1, PER = 16 / sizeof(U);
+    constexpr int LD = WTM + (FORM == 2 ? 4 : 8), PARTS = FORM != 0 ? 1 : SPLIT ? 3 : WAYS, PER = 16 / sizeof(U);
     U* es = reinterpret_cast<U*>(smem) + w * 32 * LD;
     U* out = static_cast<U*>(FORM == 0 ? p.out : p.kept);
 #pragma unroll
@@ -351,7 +355,7 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
             if constexpr (FORM == 0) {
               const OT o = cvt<OT>(v);
               h[u] = __builtin_bit_cast(unsigned short, o);
-              if (SPLIT) acc[i][j][q + u] = v - to_f32(o);  // exact; NaN stays
+              if (PARTS > 1) acc[i][j][q + u] = v - to_f32(o);  // exact; NaN stays
             } else if constexpr (FORM == 1) {
               h[u] = __builtin_bit_cast(unsigned short, cvt<f16>(v * 32768.0f));
             } else {
@@ -424,6 +428,76 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
       if constexpr (MODE == TOKEN_KEEP) store_columns(std::integral_constant<int, FINE ? 2 : 1>{}, j);
       __builtin_amdgcn_sched_barrier(0);
     }
+  } else if constexpr (MODE == TOKEN_ONE) {
+    // of each column the largest logit and sum of a wave's rows, and its target's logit
+    float2* stat = reinterpret_cast<float2*>(smem + NW * 32 * (WTM + 8) * 2);  // [WGM][BNC]
+    float* own_logit = reinterpret_cast<float*>(stat + WGM * BNC);
+    __syncthreads();
+    const int mw = m0 + wm * WTM;
+#pragma unroll
+    for (int j = 0; j < RNC; ++j) {
+      const int c = wn * WTC + j * 32 + lr, n = n0 + c;
+      if (m0 + BM > M) mask_rows(j, -__builtin_inff());
+      const long long to = (n < N ? p.targets[n] : -1) - mw;
+      const int own = (int)to - 4 * lk;
+      if (to >= 0 && to < WTM && to < M - mw && (own & 4) == 0) {
+        float z = 0.0f;
+#pragma unroll
+        for (int i = 0; i < RM; ++i)
+#pragma unroll
+          for (int q = 0; q < 16; ++q) z = own == i * 32 + 8 * (q >> 2) + (q & 3) ? acc[i][j][q] : z;
+        own_logit[c] = z;
+      }
+      float top = acc[0][j][0], sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < RM; ++i)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) top = __builtin_fmaxf(top, acc[i][j][q]);
+      top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+      const float from = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+      for (int i = 0; i < RM; ++i)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          acc[i][j][q] = exp_of<true>(acc[i][j][q] - from);
+          sum += acc[i][j][q];
+        }
+      sum += __shfl_xor(sum, 32);
+      if (lk == 0) stat[wm * BNC + c] = make_float2(top, sum);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < RNC; ++j) {
+      const int c = wn * WTC + j * 32 + lr, n = n0 + c;
+      const long long id = n < N ? p.targets[n] : -1, to = id - mw;
+      const bool real = id >= 0 && id < p.V;
+      const int own = (int)to - 4 * lk;
+      const bool hit = real && to >= 0 && to < WTM && (own & 4) == 0;
+      float top = stat[c].x, sum = 0.0f;
+#pragma unroll
+      for (int i = 1; i < WGM; ++i) top = __builtin_fmaxf(top, stat[i * BNC + c].x);
+      float of_wave = 0.0f;
+#pragma unroll
+      for (int i = 0; i < WGM; ++i) {
+        const float2 part = stat[i * BNC + c];
+        const float by = part.x == -__builtin_inff() ? 0.0f : expf(part.x - top);
+        sum += part.x == -__builtin_inff() ? part.y : part.y * by;
+        if (i == wm) of_wave = by;
+      }
+      const float loss = real ? logf(sum) + (top - own_logit[c]) : 0.0f, share = -of_wave / sum * p.scal;
+      if (wm == 0 && lk == 0 && n < N) p.target_logit[n] = loss;
+      const float at_target = target_error(loss, p.scal);
+#pragma unroll
+      for (int i = 0; i < RM; ++i)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          const float v = real ? acc[i][j][q] * share : 0.0f;
+          acc[i][j][q] = hit && own == i * 32 + 8 * (q >> 2) + (q & 3) ? at_target : v;
+        }
+      if (m0 + BM > M) mask_rows(j, 0.0f);
+      store_columns(std::integral_constant<int, 0>{}, j);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   } else if constexpr (MODE == TOKEN_ERROR) {
     __syncthreads();
 #pragma unroll
@@ -473,6 +547,7 @@ template <int TERMS, int MODE, int WAYS, int BM, int BN, int WGM, int WGN, int S
 constexpr int tile_lds() {
   constexpr int NW = WGM * WGN, ring = ST * TERMS * (BM + BN) * 64;
   constexpr int epi = MODE == TOKEN_STATS ? 0
+                      : MODE == TOKEN_ONE ? NW * 32 * (BM / WGM + 8) * 2 + (WGM * 8 + 4) * (BN / WAYS)
                       : MODE == TOKEN_ERROR || (MODE == TOKEN_KEEP && TERMS == 1 && WAYS == 1) ? NW * 32 * (BM / WGM + 8) * 2
                       : MODE == TOKEN_KEEP ? NW * 32 * (BM / WGM + 4) * 4 : NW * 32 * (BN / WGN + 4) * 4;
   return epi > ring ? epi : ring;

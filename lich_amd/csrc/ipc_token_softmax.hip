@@ -8,7 +8,8 @@
 //    whatever they hold (so that nothing of them reaches W).
 // 2. Every piece of the vocabulary: the largest logit and sum of exponentials of each wave's
 //    rows.
-// 3. A column's parts joined: its loss, largest logit and 1 / sum (with one piece, by step 4).
+// 3. A column's parts joined: its loss, largest logit and 1 / sum (with one piece, by step 4; a vocabulary
+//    that one tile holds: steps 2 to 4 are one).
 // 4. Every piece: its errors in 16 bits (fp32: three terms), its share of W^T e, and its
 //    rows of W, which nothing reads any more.
 // 5. The shares added in order, times f'(X) (small: in the launch that updates W).
@@ -55,6 +56,7 @@ struct Plan {
   bool fix;           // and the loss corrected
   int ft_terms, f_terms, e_terms;
   bool keep;          // one piece, its exponentials kept
+  bool one;           // and one tile: errors at once
   int rows, Vp;       // of a piece (the last may have fewer), ET's row length
   int tile, unit;     // of the logits
   int grad_tile, slices;
@@ -95,6 +97,9 @@ bool make_plan(int V, int D, int B, int storage, int act, bool update, Plan& o) 
   o.rows = (int)rows;
   o.Vp = (int)up(o.rows, 32);
   o.keep = update && o.rows == V && (storage != DT_F32 || (long long)o.Bk * o.Vp * 10 <= kPieceBytes);
+  // (a launch less against half as many workgroups at long sums: us, at once / kept first, bf16 64 x 300 x 200 21.7 / 25.8,
+  // fp32 128 x 512 x 4000 89 / 98, 26 x 2000 x 30 36.6 / 40.7; 128 x 1000 x 100 39 / 37, 100 x 4001 x 16 77 / 64)
+  o.one = o.keep && !o.mend && (V <= TOKEN_ONE_ROWS / 2 || (V <= TOKEN_ONE_ROWS && D <= 512));
   auto tiles = [&](long long m, long long n, long long e) { return ((m + e - 1) / e) * ((n + e - 1) / e); };
   const long long columns = (long long)o.ways * B;
   // (the largest tile that gives the CUs one each; fp32: us, 64 wide / 128 x 64, 4000 x 4000 x 512 update 355 / 336,
@@ -124,7 +129,7 @@ bool make_plan(int V, int D, int B, int storage, int act, bool update, Plan& o) 
     o.f = take(state * o.f_terms);
     o.et = take((long long)o.e_terms * o.Bk * o.Vp * 2);
     o.part = take(4LL * o.slices * D * B);
-    o.kept = o.e_terms == 1 ? o.et : o.keep ? take(4LL * o.Bk * o.Vp) : 0;
+    o.kept = o.e_terms == 1 ? o.et : o.keep && !o.one ? take(4LL * o.Bk * o.Vp) : 0;
     o.fixes = o.fix ? take(4LL * B * token_fix_rows(D, false)) : 0;
     if (o.mend) {
       o.order = take(4LL * B);
@@ -458,13 +463,19 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
     return q;
   };
   float2* part = reinterpret_cast<float2*>(ws + o.stats);
+  // fp16: errors below its smallest normal number matter (1 / V), so they are kept times 2^10
+  const float scale = storage == DT_F16 ? 1024.0f : 1.0f;
   lay_out(0, state_tiles);
   if (e != hipSuccess) return e;
   for (int first = 0; first < p.V && e == hipSuccess; first += o.rows) {
     TokenGemm q = logits(first, first > 0);
     if (e != hipSuccess) return e;
     q.out = part + (long long)(first / o.unit) * p.B;
-    if (o.keep) {
+    if (o.one) {
+      q.out = at(o.et); q.out_ld = o.Vp; q.out_rows = o.Bk; q.out_term = (long long)o.Bk * o.Vp; q.scal = scale;
+      q.target_logit = p.loss;
+      e = launch_token_one(q, storage, o.ways, s);
+    } else if (o.keep) {
       q.kept = ws + o.kept; q.out_ld = o.Vp; q.out_rows = o.Bk;
       e = launch_token_keep(q, storage, o.tile, o.ways, s);
     } else {
@@ -474,7 +485,7 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
   if (e != hipSuccess) return e;
   const int units = (p.V + o.unit - 1) / o.unit;
   const bool joined = o.keep && o.Vp <= ERROR_RUN;  // with the errors
-  if (!joined) {
+  if (!joined && !o.one) {
     const Columns c{p.B, p.V, units, part, reinterpret_cast<const float*>(ws + o.logit), p.targets, p.loss,
                     reinterpret_cast<float2*>(ws + o.norm)};
     int across = 16;
@@ -484,8 +495,6 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
     if (!update || e != hipSuccess) return e;
   }
 
-  // fp16: errors below its smallest normal number matter (1 / V), so they are kept times 2^10
-  const float scale = storage == DT_F16 ? 1024.0f : 1.0f;
   float* fixes = o.fix ? reinterpret_cast<float*>(ws + o.fixes) : nullptr;
   const int vec_state = p.B % 4 == 0 && reinterpret_cast<uintptr_t>(p.x) % (4 * sizeof(ST)) == 0 &&
                         reinterpret_cast<uintptr_t>(p.g) % (4 * sizeof(ST)) == 0;
@@ -501,7 +510,7 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
   };
   for (int first = 0; first < p.V; first += o.rows) {
     const int rows = rows_of(first), Vp = (rows + 31) / 32 * 32;
-    if (o.keep) {
+    if (o.keep && !o.one) {
       const Errors er{p.V, p.B, Vp, o.Bk, o.unit, units, ws + o.kept, at(o.et), part, reinterpret_cast<const float*>(ws + o.logit),
                       p.loss, reinterpret_cast<const float2*>(ws + o.norm), p.targets, scale};
       const dim3 grid((unsigned)((long long)o.Bk * (joined ? 1 : (Vp + 2047) / 2048)));
@@ -511,7 +520,7 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
       else if (joined) hipLaunchKernelGGL((token_errors_kernel<OT, MORE, true>), grid, dim3(256), 0, s, er);
       else hipLaunchKernelGGL((token_errors_kernel<OT, MORE, false>), grid, dim3(256), 0, s, er);
       e = hipGetLastError();
-    } else {
+    } else if (!o.keep) {
       TokenGemm q = logits(first, o.rows < p.V);  // (one piece: its rows are laid out already)
       if (e != hipSuccess) return e;
       q.stats = reinterpret_cast<const float2*>(ws + o.norm);

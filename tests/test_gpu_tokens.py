@@ -317,6 +317,24 @@ def test_a_few_samples(V, D, B, name):
     check(alone, r["loss"], softmax_bounds(r, w, dt, V, D, B, activation, 0.0, False)[0], "the loss alone")
 
 
+# a vocabulary within one tile, and the first that is not
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("V,D,B", [(64, 300, 200), (63, 33, 1000), (2, 3001, 40), (100, 90, 65), (128, 512, 33), (127, 7, 700), (128, 513, 40), (129, 60, 70),
+                                   (1, 400, 100)])
+def test_a_vocabulary_within_a_tile(V, D, B, name):
+    dt = TYPES[name]
+    activation = ["silu", "sigmoid", "tanh", "identity", "gelu", "relu"][(V + D + B) % 6]
+    x, w, t = softmax_case(V, D, B, dt, V + D + B, padded=0.2)
+    loss, g, wn = run_update(x.to(DEV), w.to(DEV), t.to(DEV), activation, 0.25)
+    r = O.softmax(x, w, t, activation)
+    bl, bg, bw = softmax_bounds(r, w, dt, V, D, B, activation, 0.25)
+    check(loss, r["loss"], bl, "loss")
+    check(g, r["g"], bg, "g")
+    check(wn, w.double() + 0.25 * r["dw"], bw, "w")
+    padded = (t < 0) | (t >= V)
+    assert bool((loss.cpu()[padded] == 0).all()) and bool((g.cpu()[:, padded] == 0).all())
+
+
 # weights of more than a piece under few columns
 @pytest.mark.parametrize("V,D,B,name", [(300001, 2001, 1, "bf16"), (600001, 2000, 2, "f16"), (14001, 40001, 1, "bf16"), (30000, 40000, 1, "f16")])
 def test_token_update_of_a_large_table_and_one_sample(V, D, B, name):
@@ -496,7 +514,7 @@ class Fenced:
 @pytest.mark.parametrize("name", TYPES)
 @pytest.mark.parametrize("activation", ["identity", "tanh"])
 @pytest.mark.parametrize("V,D,B", [(2, 1, 1), (10, 64, 128), (999, 77, 3), (300, 131, 90), (26240, 1, 70), (7001, 65, 1), (700, 200, 300),
-                                   (164, 2, 188), (5000, 35, 520), (1000, 9, 2), (6001, 701, 3), (520, 130, 8)])
+                                   (164, 2, 188), (5000, 35, 520), (1000, 9, 2), (6001, 701, 3), (520, 130, 8), (100, 90, 65), (33, 100, 300)])
 def test_softmax_calls_stay_inside_their_tensors(V, D, B, activation, name):
     """Also inside the workspace's stated size; room behind each as large as the workspace itself."""
     dt = TYPES[name]
