@@ -7,6 +7,7 @@
 //                 type and stored transposed, ET[n][v]
 //   TOKEN_ONE     a vocabulary within one tile: losses and errors (as many terms as f(X) has) at once
 //   TOKEN_GRAD    P[d][n] = sum_v W[v][d] e[v][n]     (a slice of the vocabulary a workgroup)
+//   TOKEN_STATE   that of a whole vocabulary, times f'(X): the state's gradient
 //   TOKEN_WEIGHT  W[v][d] += alpha sum_n e[v][n] F[d][n]
 //
 // v_mfma_f32_32x32x16 tiles in the pipeline of ipc_ckpt_gemm.h: three to eight stages of 32 k filled by
@@ -38,7 +39,7 @@
 
 namespace ipc {
 
-enum { TOKEN_STATS = 0, TOKEN_KEEP = 1, TOKEN_ERROR = 2, TOKEN_GRAD = 3, TOKEN_WEIGHT = 4, TOKEN_ONE = 5 };
+enum { TOKEN_STATS = 0, TOKEN_KEEP = 1, TOKEN_ERROR = 2, TOKEN_GRAD = 3, TOKEN_WEIGHT = 4, TOKEN_ONE = 5, TOKEN_STATE = 6 };
 
 // Tiles of the first three: rows (of W) and columns of a workgroup, and the rows of a wave, whose
 // largest values and sums are kept (unit; ways: terms of f(X), side by side in a tile; with three
@@ -63,8 +64,9 @@ struct TokenGemm {
   int out_rows;                    // of ET, N up to a multiple of 32
   int add;                         // GRAD: out holds sums already
   int vec;                         // WEIGHT: out allows 4-element accesses
-  float scal;                      // WEIGHT: alpha; ERROR, ONE: the errors' scale
-  // STATS, KEEP, ERROR, ONE
+  float scal;                      // WEIGHT: alpha; ERROR, ONE: the errors' scale; STATE: 1 / that
+  const void* x; int act;          // STATE: of its type and layout, G's
+  // STATS, KEEP, ERROR, ONE, STATE (targets and V)
   const long long* targets; int first, V;  // first: of the piece's rows
   float* target_logit;             // ONE: the losses
   const float* loss;               // ERROR
@@ -100,6 +102,9 @@ hipError_t launch_token_finish(const TokenFinish& p, int storage, hipStream_t s)
 // launch where both are small.
 // terms: of both operands in 16-bit storage, 1, 2 (fp16) or 3 (bf16)
 hipError_t launch_token_weight(const TokenGemm& p, const TokenFinish* f, int storage, int terms, hipStream_t s);
+// The state's gradient (g, TOKEN_STATE) from W's copy and W's update (u) in one launch.
+hipError_t launch_token_tail(const TokenGemm& g, const TokenGemm& u, int storage, hipStream_t s);
+inline long long token_tail_tiles(int V, int D, int B) { return (D + 63LL) / 64 * ((B + 63LL) / 64 + (V + 63LL) / 64); }
 
 namespace token {
 
@@ -123,12 +128,12 @@ __device__ __forceinline__ float exp_of(float x) {
 __device__ __forceinline__ float target_error(float loss, float scale) { return -expm1f(-loss) * scale; }
 
 // Workgroup `block` of `blocks` of a product.
-// WT: the type of W, which TOKEN_WEIGHT writes.
+// WT: the type of W, which TOKEN_WEIGHT writes, and of the state.
 template <typename OT, int TERMS, int MODE, int WAYS, int BM, int BN, int WGM, int WGN, int ST, typename WT>
 __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* smem, int block, int blocks) {
   using MF = Mfma32<OT>;
   typedef typename MF::operand V;
-  constexpr bool MN = MODE == TOKEN_GRAD || MODE == TOKEN_WEIGHT, COLUMNS = !MN;
+  constexpr bool MN = MODE == TOKEN_GRAD || MODE == TOKEN_WEIGHT || MODE == TOKEN_STATE, COLUMNS = !MN;
   constexpr int NW = WGM * WGN, WTM = BM / WGM, WTN = BN / WGN, RM = WTM / 32, RN = WTN / 32;
   constexpr int RNC = RN / WAYS, BNC = BN / WAYS, WTC = WTN / WAYS;  // blocks and columns of different n
   constexpr bool SPLIT = TERMS == 3, FINE = SPLIT || ((MODE == TOKEN_KEEP || MODE == TOKEN_ONE) && WAYS > 1);  // FINE: kept in fp32
@@ -524,6 +529,25 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
       store_columns(std::integral_constant<int, 0>{}, j);
       __builtin_amdgcn_sched_barrier(0);
     }
+  } else if constexpr (MODE == TOKEN_STATE) {
+    static_assert(RM == 1 && RN == 1, "a block a wave");
+    __syncthreads();
+    float* es = reinterpret_cast<float*>(smem) + w * 32 * 36;
+#pragma unroll
+    for (int q = 0; q < 16; q += 4)
+      *reinterpret_cast<float4*>(es + lr * 36 + 2 * q + 4 * lk) = make_float4(acc[0][0][q], acc[0][0][q + 1], acc[0][0][q + 2], acc[0][0][q + 3]);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int n = n0 + wn * WTN + lr;
+    const long long id = n < N ? p.targets[n] : -1;
+    const bool real = id >= 0 && id < p.V;
+#pragma unroll 1
+    for (int r = lk; r < 32; r += 2) {
+      const int d = m0 + wm * WTM + r;
+      if (d >= M || n >= N) continue;
+      const long long here = (long long)d * N + n;
+      const float v = act_df(p.act, to_f32(static_cast<const WT*>(p.x)[here])) * (es[r * 36 + lr] * p.scal);
+      static_cast<WT*>(p.out)[here] = cvt<WT>(real ? v : 0.0f);
+    }
   } else {
     typedef typename std::conditional<MODE == TOKEN_GRAD, float, WT>::type TT;
     MxProblem e{};
@@ -547,6 +571,7 @@ template <int TERMS, int MODE, int WAYS, int BM, int BN, int WGM, int WGN, int S
 constexpr int tile_lds() {
   constexpr int NW = WGM * WGN, ring = ST * TERMS * (BM + BN) * 64;
   constexpr int epi = MODE == TOKEN_STATS ? 0
+                      : MODE == TOKEN_STATE ? NW * 32 * 36 * 4
                       : MODE == TOKEN_ONE ? NW * 32 * (BM / WGM + 8) * 2 + (WGM * 8 + 4) * (BN / WAYS)
                       : MODE == TOKEN_ERROR || (MODE == TOKEN_KEEP && TERMS == 1 && WAYS == 1) ? NW * 32 * (BM / WGM + 8) * 2
                       : MODE == TOKEN_KEEP ? NW * 32 * (BM / WGM + 4) * 4 : NW * 32 * (BN / WGN + 4) * 4;

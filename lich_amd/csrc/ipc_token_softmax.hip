@@ -49,7 +49,7 @@ constexpr long long kFineErrors = 1LL << 23, kFineWork = 1LL << 31;
 
 struct Plan {
   int terms, Dp, Bk;
-  bool copy;          // W laid out per piece: fp32, or 16-bit rows of an odd length
+  bool copy;          // W laid out per piece: fp32, 16-bit rows of an odd length, or for `tail`
   int ways;           // terms of f(X) in the logits, in 16 bits
   bool fine;          // the update in 16 bits, small: errors and f(X) in `ways` terms
   bool mend;          // the update in 16 bits, large: targets' errors made good in fp32
@@ -57,6 +57,7 @@ struct Plan {
   int ft_terms, f_terms, e_terms;
   bool keep;          // one piece, its exponentials kept
   bool one;           // and one tile: errors at once
+  bool tail;          // the gradient and W's update in one launch, from W's copy
   int rows, Vp;       // of a piece (the last may have fewer), ET's row length
   int tile, unit;     // of the logits
   int grad_tile, slices;
@@ -70,11 +71,12 @@ bool make_plan(int V, int D, int B, int storage, int act, bool update, Plan& o) 
   if (D > (1 << 26) || B > (1 << 26)) return false;
   o.Dp = (int)up(D, 32);
   o.Bk = (int)up(B, 32);
-  o.copy = storage == DT_F32 || D % 2 != 0;
   const bool inexact = storage != DT_F32 && act != ACT_IDENTITY && act != ACT_RELU;
   const long long work = (long long)V * B;
   const bool few = storage != DT_F32 && work <= kFineErrors && work * D <= kFineWork;
   const int most = storage == DT_BF16 ? 3 : 2;
+  const bool tail = update && (few || storage == DT_F32) && V <= 480 && (long long)V * D <= 1 << 20 && token_tail_tiles(V, D, B) <= 256;
+  o.copy = storage == DT_F32 || D % 2 != 0 || tail;
   const long long state = 2LL * o.Dp * o.Bk;
   // the rows of a piece, 0 for sizes that the kernels do not take
   auto pieces = [&](bool fine) -> long long {
@@ -114,6 +116,7 @@ bool make_plan(int V, int D, int B, int storage, int act, bool update, Plan& o) 
                        : o.grad_tile == 128 ? (D + 127LL) / 128 * (B > 64 ? (B + 127LL) / 128 : 1) : tiles(D, B, 64);
   const long long stages = o.Vp / 32;
   o.slices = (int)std::max<long long>(1, std::min({256 / gt, stages / 8, 64LL}));
+  o.tail = tail && o.keep && !o.mend && o.slices == 1;
   long long at = 0;
   auto take = [&](long long bytes) {
     const long long here = at;
@@ -128,7 +131,7 @@ bool make_plan(int V, int D, int B, int storage, int act, bool update, Plan& o) 
   if (update) {
     o.f = take(state * o.f_terms);
     o.et = take((long long)o.e_terms * o.Bk * o.Vp * 2);
-    o.part = take(4LL * o.slices * D * B);
+    o.part = o.tail ? 0 : take(4LL * o.slices * D * B);
     o.kept = o.e_terms == 1 ? o.et : o.keep && !o.one ? take(4LL * o.Bk * o.Vp) : 0;
     o.fixes = o.fix ? take(4LL * B * token_fix_rows(D, false)) : 0;
     if (o.mend) {
@@ -534,7 +537,7 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
     g.M = p.D; g.N = p.B; g.K = Vp;
     g.b = at(o.et); g.ldb = Vp; g.b_term = (unsigned)((long long)o.Bk * Vp * 2); g.b_bytes = (long long)TERMS * o.Bk * Vp * 2;
     g.slices = o.slices; g.out = ws + o.part; g.add = first > 0;
-    e = launch_token_grad(g, storage, o.grad_tile, s);
+    if (!o.tail) e = launch_token_grad(g, storage, o.grad_tile, s);
     if (e != hipSuccess) return e;
     TokenGemm u{};
     u.a = at(o.et); u.lda = Vp; u.a_term = g.b_term; u.a_bytes = (long long)o.e_terms * o.Bk * Vp * 2;
@@ -543,6 +546,10 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
     u.out = static_cast<ST*>(p.w) + (long long)first * p.D;
     u.vec = p.D % 4 == 0 && reinterpret_cast<uintptr_t>(p.w) % (4 * sizeof(ST)) == 0;
     u.scal = p.alpha / scale;
+    if (o.tail) {
+      g.out = p.g; g.x = p.x; g.act = p.act; g.targets = p.targets; g.V = p.V; g.scal = 1.0f / scale;
+      return launch_token_tail(g, u, storage, s);
+    }
     if (o.mend) {
       u.slot = reinterpret_cast<const int*>(ws + o.slot) + first;
       u.hot = reinterpret_cast<const float*>(ws + o.hot);
