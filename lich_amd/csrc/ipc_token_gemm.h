@@ -57,7 +57,7 @@ struct TokenGemm {
   const void* b; long long ldb;
   long long a_bytes, b_bytes;      // buffers' ends (loads past them give 0)
   unsigned a_term, b_term;         // bytes from one term to the next
-  int slices;                      // TOKEN_GRAD: of the contraction
+  int slices;                      // GRAD (and WEIGHT, see launch_token_tail): of the contraction
   void* out;                       // STATS, KEEP: float2 [units][N]; ERROR: ET; GRAD: [slices][M][N] fp32; WEIGHT: W
   void* kept;                      // KEEP: exponentials times 2^15 in fp16 (fp32: in fp32), layout of ET
   long long out_ld, out_term;      // KEEP, ERROR: elements
@@ -102,8 +102,9 @@ hipError_t launch_token_finish(const TokenFinish& p, int storage, hipStream_t s)
 // launch where both are small.
 // terms: of both operands in 16-bit storage, 1, 2 (fp16) or 3 (bf16)
 hipError_t launch_token_weight(const TokenGemm& p, const TokenFinish* f, int storage, int terms, hipStream_t s);
-// The state's gradient (g, TOKEN_STATE) from W's copy and W's update (u) in one launch.
-hipError_t launch_token_tail(const TokenGemm& g, const TokenGemm& u, int storage, hipStream_t s);
+// The state's gradient (g, TOKEN_STATE) from W's copy and W's update (u) in one launch.  u.slices > 1: u's
+// contraction cut into as many, whose sums ([slices][M][N] at part) a second launch adds to W.
+hipError_t launch_token_tail(const TokenGemm& g, const TokenGemm& u, float* part, int storage, hipStream_t s);
 inline long long token_tail_tiles(int V, int D, int B) { return (D + 63LL) / 64 * ((B + 63LL) / 64 + (V + 63LL) / 64); }
 
 namespace token {

@@ -58,6 +58,7 @@ struct Plan {
   bool keep;          // one piece, its exponentials kept
   bool one;           // and one tile: errors at once
   bool tail;          // the gradient and W's update in one launch, from W's copy
+  int cut;            // slices of the batch in that
   int rows, Vp;       // of a piece (the last may have fewer), ET's row length
   int tile, unit;     // of the logits
   int grad_tile, slices;
@@ -117,6 +118,10 @@ bool make_plan(int V, int D, int B, int storage, int act, bool update, Plan& o) 
   const long long stages = o.Vp / 32;
   o.slices = (int)std::max<long long>(1, std::min({256 / gt, stages / 8, 64LL}));
   o.tail = tail && o.keep && !o.mend && o.slices == 1;
+  // (W's product: as many slices of eight steps and more as give every CU a workgroup, three at least: us, cut / whole, bf16
+  // 6 x 73 x 3026 21.7 / 45, 329 x 3 x 4059 40 / 66, 26 x 40 x 2000 21.3 / 29.2; two: 256 x 256 x 512 27.2 / 25.6)
+  o.cut = (int)std::min<long long>(o.Bk / 256, (256 - tiles(D, B, 64)) / tiles(V, D, 64));
+  if (o.cut < 3) o.cut = 1;
   long long at = 0;
   auto take = [&](long long bytes) {
     const long long here = at;
@@ -131,7 +136,7 @@ bool make_plan(int V, int D, int B, int storage, int act, bool update, Plan& o) 
   if (update) {
     o.f = take(state * o.f_terms);
     o.et = take((long long)o.e_terms * o.Bk * o.Vp * 2);
-    o.part = o.tail ? 0 : take(4LL * o.slices * D * B);
+    o.part = o.tail ? o.cut > 1 ? take(4LL * o.cut * V * D) : 0 : take(4LL * o.slices * D * B);
     o.kept = o.e_terms == 1 ? o.et : o.keep && !o.one ? take(4LL * o.Bk * o.Vp) : 0;
     o.fixes = o.fix ? take(4LL * B * token_fix_rows(D, false)) : 0;
     if (o.mend) {
@@ -548,7 +553,8 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
     u.scal = p.alpha / scale;
     if (o.tail) {
       g.out = p.g; g.x = p.x; g.act = p.act; g.targets = p.targets; g.V = p.V; g.scal = 1.0f / scale;
-      return launch_token_tail(g, u, storage, s);
+      u.slices = o.cut;
+      return launch_token_tail(g, u, reinterpret_cast<float*>(ws + o.part), storage, s);
     }
     if (o.mend) {
       u.slot = reinterpret_cast<const int*>(ws + o.slot) + first;

@@ -319,7 +319,7 @@ def test_a_few_samples(V, D, B, name):
 
 # a vocabulary within one tile, and the first that is not
 @pytest.mark.parametrize("name", TYPES)
-@pytest.mark.parametrize("V,D,B", [(64, 300, 200), (63, 33, 1000), (2, 3001, 40), (100, 90, 65), (128, 512, 33), (127, 7, 700), (128, 513, 40), (129, 60, 70),
+@pytest.mark.parametrize("V,D,B", [(64, 300, 200), (63, 33, 1000), (2, 3001, 40), (100, 90, 65), (128, 512, 33), (127, 7, 700), (128, 513, 40), (129, 60, 70), (6, 73, 3026), (329, 3, 2059), (480, 33, 900),
                                    (1, 400, 100)])
 def test_a_vocabulary_within_a_tile(V, D, B, name):
     dt = TYPES[name]
