@@ -631,6 +631,8 @@ int ipc_dropout(const void* x, const long long* rng, void* out, int M, int B, in
  *     (at most 2^23 errors and 2^31 multiplications) f(X) and e in two fp16 or three bf16 terms.  A
  *     larger update rounds both to the type once, makes the sums of the targets' rows
  *     good in fp32 and corrects the loss to first order in what f(X)'s rounding left.
+ * A word whose weights give it logits far below the others' has no share of anything; infinite
+ * weights are for the loss alone (g takes 0 times infinity where they are not the largest bf16).
  * Both need a workspace (16-byte aligned) of ipc_token_loss_workspace_bytes /
  * ipc_token_update_workspace_bytes bytes (0: refused).  w of 16 bits with an even D
  * lies on 4 bytes.

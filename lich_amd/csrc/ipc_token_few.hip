@@ -122,6 +122,14 @@ __global__ void __launch_bounds__(kWaves * 64) token_few_logits_kernel(const Few
       Sixteen<ST> in[R];
 #pragma unroll
       for (int i = 0; i < R; ++i) in[i] = get(rows[i] + (d < whole ? d : p.D - P));
+      if (d >= whole) {  // (what whole pieces have is no number here: 0 times infinity)
+#pragma unroll
+        for (int q = 0; q < P - 1; ++q)
+          if (q < P - (p.D - whole)) {
+#pragma unroll
+            for (int i = 0; i < R; ++i) in[i].v[q] = cvt<ST>(0.0f);
+          }
+      }
 #pragma unroll
       for (int s = 0; s < TB; ++s) {
         float4 g[P / 4];

@@ -393,6 +393,62 @@ def test_words_masked_by_their_weights(name):
 
 
 @pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("V,D,B", [(12, 9, 30), (300, 50, 2), (70000, 70, 1), (100, 60, 90), (5000, 40, 11)])
+def test_words_masked_by_their_weights_in_every_size(V, D, B, name):
+    dt, some = TYPES[name], V - V // 3
+    x, w, t = softmax_case(V, D, B, dt, 5, padded=0.0)
+    t = t % some
+    for low in (torch.finfo(dt).min / 64, -float("inf")):
+        wm = w.clone()
+        wm[some:] = low
+        k = tokens.build_token_loss(V, D, B, "sigmoid", dt)
+        loss = torch.full((B,), float("nan"), device=DEV)
+        k(x.to(DEV), wm.to(DEV), t.to(DEV), loss, workspace=k.new_workspace(DEV))
+        r = O.softmax(x, w[:some], t, "sigmoid")
+        check(loss, r["loss"], softmax_bounds(r, w[:some], dt, V, D, B, "sigmoid", 0.0, False)[0], "loss")
+    wm[some:] = torch.finfo(dt).min / 64
+    loss, g, wn = run_update(x.to(DEV), wm.to(DEV), t.to(DEV), "sigmoid", 0.5)
+    bl, bg, _ = softmax_bounds(r, w[:some], dt, V, D, B, "sigmoid", 0.5)
+    check(loss, r["loss"], bl, "loss")
+    check(g, r["g"], bg, "g")
+    assert torch.equal(wn[some:].cpu(), wm[some:])
+
+
+@pytest.mark.parametrize("name", TYPES)
+def test_calls_of_few_samples_in_a_graph(name):
+    """A few samples, one tile, slices of a long batch: replays that share a workspace give the eager bits."""
+    dt = TYPES[name]
+    cases = []
+    for V, D, B in ((900, 70, 2), (100, 60, 90), (20, 40, 1000)):
+        x, w, t = (v.to(DEV) for v in softmax_case(V, D, B, dt, V))
+        k = tokens.build_token_update(V, D, B, "tanh", dt, 0.3)
+        cases.append((k, x, w, t))
+    ws = torch.empty(max(k.workspace_bytes for k, *_ in cases), dtype=torch.uint8, device=DEV)
+
+    def new():
+        return [(w.clone(), torch.empty(x.shape[1], device=DEV), torch.empty_like(x)) for _, x, w, _ in cases]
+
+    def run(state):
+        for (k, x, _, t), (w, loss, g) in zip(cases, state):
+            k(x, w, t, loss, g, workspace=ws)
+
+    eager, kept, side = new(), new(), torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        run(new())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        run(kept)
+    for _ in range(3):
+        run(eager)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(eager, kept):
+            assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+@pytest.mark.parametrize("name", TYPES)
 def test_large_and_confident_logits(name):
     """Logits of a few hundred, columns whose target has all the probability."""
     dt, V, D, B = TYPES[name], 400, 64, 65
