@@ -5,7 +5,8 @@
 //   TOKEN_KEEP    that, and the exponentials, as KEPT[n][v] relative to their wave's largest
 //   TOKEN_ERROR   the same products again; e = onehot - softmax(Z), rounded to the operand
 //                 type and stored transposed, ET[n][v]
-//   TOKEN_ONE     a vocabulary within one tile: losses and errors (as many terms as f(X) has) at once
+//   TOKEN_ONE     a vocabulary within one tile: losses and errors (as many terms as f(X) has; none where
+//                 the output has no rows) at once
 //   TOKEN_GRAD    P[d][n] = sum_v W[v][d] e[v][n]     (a slice of the vocabulary a workgroup)
 //   TOKEN_STATE   that of a whole vocabulary, times f'(X): the state's gradient
 //   TOKEN_WEIGHT  W[v][d] += alpha sum_n e[v][n] F[d][n]

@@ -56,7 +56,7 @@ struct Plan {
   bool fix;           // and the loss corrected
   int ft_terms, f_terms, e_terms;
   bool keep;          // one piece, its exponentials kept
-  bool one;           // and one tile: errors at once
+  bool one;           // one tile: losses (and errors) at once
   bool tail;          // the gradient and W's update in one launch, from W's copy
   int cut;            // slices of the batch in that
   int rows, Vp;       // of a piece (the last may have fewer), ET's row length
@@ -76,6 +76,10 @@ bool make_plan(int V, int D, int B, int storage, int act, bool update, Plan& o) 
   const long long work = (long long)V * B;
   const bool few = storage != DT_F32 && work <= kFineErrors && work * D <= kFineWork;
   const int most = storage == DT_BF16 ? 3 : 2;
+  // (V within a tile: a launch less against half as many workgroups at long sums: us, at once / kept first, bf16
+  // 64 x 300 x 200 update 21.7 / 25.8, fp32 128 x 512 x 4000 89 / 98, 26 x 2000 x 30 36.6 / 40.7; 128 x 1000 x 100 39 / 37,
+  // 100 x 4001 x 16 77 / 64; the loss alone, 64 x 300 x 200 11.6 / 13.7, 100 x 90 x 64 12.8 / 11.9)
+  const bool within = V <= TOKEN_ONE_ROWS / 2 || (update && V <= TOKEN_ONE_ROWS && D <= 512);
   const bool tail = update && (few || storage == DT_F32) && V <= 480 && (long long)V * D <= 1 << 20 && token_tail_tiles(V, D, B) <= 256;
   o.copy = storage == DT_F32 || D % 2 != 0 || tail;
   const long long state = 2LL * o.Dp * o.Bk;
@@ -100,9 +104,7 @@ bool make_plan(int V, int D, int B, int storage, int act, bool update, Plan& o) 
   o.rows = (int)rows;
   o.Vp = (int)up(o.rows, 32);
   o.keep = update && o.rows == V && (storage != DT_F32 || (long long)o.Bk * o.Vp * 10 <= kPieceBytes);
-  // (a launch less against half as many workgroups at long sums: us, at once / kept first, bf16 64 x 300 x 200 21.7 / 25.8,
-  // fp32 128 x 512 x 4000 89 / 98, 26 x 2000 x 30 36.6 / 40.7; 128 x 1000 x 100 39 / 37, 100 x 4001 x 16 77 / 64)
-  o.one = o.keep && !o.mend && (V <= TOKEN_ONE_ROWS / 2 || (V <= TOKEN_ONE_ROWS && D <= 512));
+  o.one = within && (update ? o.keep && !o.mend : o.rows == V && (storage == DT_F32 || (few && o.ways == most)));
   auto tiles = [&](long long m, long long n, long long e) { return ((m + e - 1) / e) * ((n + e - 1) / e); };
   const long long columns = (long long)o.ways * B;
   // (the largest tile that gives the CUs one each; fp32: us, 64 wide / 128 x 64, 4000 x 4000 x 512 update 355 / 336,
@@ -480,7 +482,10 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
     if (e != hipSuccess) return e;
     q.out = part + (long long)(first / o.unit) * p.B;
     if (o.one) {
-      q.out = at(o.et); q.out_ld = o.Vp; q.out_rows = o.Bk; q.out_term = (long long)o.Bk * o.Vp; q.scal = scale;
+      q.scal = scale;
+      if (update) {
+        q.out = at(o.et); q.out_ld = o.Vp; q.out_rows = o.Bk; q.out_term = (long long)o.Bk * o.Vp;
+      }
       q.target_logit = p.loss;
       e = launch_token_one(q, storage, o.ways, s);
     } else if (o.keep) {
@@ -500,8 +505,8 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
     while (across > 1 && across / 2 >= p.B) across /= 2;
     hipLaunchKernelGGL(token_columns_kernel, dim3((unsigned)((p.B + across - 1) / across)), dim3(1024), 0, s, c, across);
     e = hipGetLastError();
-    if (!update || e != hipSuccess) return e;
   }
+  if (!update || e != hipSuccess) return e;
 
   float* fixes = o.fix ? reinterpret_cast<float*>(ws + o.fixes) : nullptr;
   const int vec_state = p.B % 4 == 0 && reinterpret_cast<uintptr_t>(p.x) % (4 * sizeof(ST)) == 0 &&

@@ -331,8 +331,12 @@ def test_a_vocabulary_within_a_tile(V, D, B, name):
     check(loss, r["loss"], bl, "loss")
     check(g, r["g"], bg, "g")
     check(wn, w.double() + 0.25 * r["dw"], bw, "w")
+    k, alone = tokens.build_token_loss(V, D, B, activation, dt), torch.full((B,), float("nan"), device=DEV)
+    k(x.to(DEV), w.to(DEV), t.to(DEV), alone, workspace=k.new_workspace(DEV))
+    check(alone, r["loss"], softmax_bounds(r, w, dt, V, D, B, activation, 0.0, False)[0], "the loss alone")
     padded = (t < 0) | (t >= V)
-    assert bool((loss.cpu()[padded] == 0).all()) and bool((g.cpu()[:, padded] == 0).all())
+    for got in (loss, alone, g):
+        assert bool((got.cpu()[..., padded] == 0).all())
 
 
 # weights of more than a piece under few columns
