@@ -382,47 +382,52 @@ __global__ void __launch_bounds__(256) token_errors_kernel(const Errors p) {
 // (e - rounded e) rounded f + e (f - rounded f), for the first position p of each target.
 // (Elsewhere e is a probability, whose rounding counts as little.  Without this a weight in a
 // few hundred of a target's row rounds the other way, and the next loss differs by 1e-5 .. 1e-3.)
-// A workgroup has 256 features of a position: four groups of 64 lanes take every fourth column.
+// A workgroup has 256 features of a position: HOT_GROUPS waves take every so many-th column.  (Words
+// are not drawn evenly: the commonest has a tenth of the columns.  128000 words, 2048 samples of 2048 features,
+// fp16: 26 us.)
+constexpr int HOT_GROUPS = 4;
 struct Hot {
-  int B, D, Dp, terms;
+  int B, D, Dp;
   const int* order;
   const int* key;
-  const unsigned short* ft;  // [terms][B][Dp]
+  const unsigned short* ft;  // [TWO ? 2 : 1][B][Dp]
   const float* loss;
   float* hot;                // [B][Dp]
   float scale;
 };
-template <typename OT>
-__global__ void __launch_bounds__(256) token_hot_kernel(const Hot p) {
-  __shared__ float4 red[4][64];
-  const int slabs = (p.Dp + 255) / 256, at = blockIdx.x / slabs, lane = threadIdx.x & 63, group = threadIdx.x >> 6;
-  const int d = blockIdx.x % slabs * 256 + lane * 4;
+template <typename OT, bool TWO>
+__global__ void __launch_bounds__(HOT_GROUPS * 64) token_hot_kernel(const Hot p) {
+  __shared__ float4 red[HOT_GROUPS][64];
+  const int slabs = (p.Dp + 255) / 256, at = blockIdx.x / slabs, lane = threadIdx.x & 63;
+  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d = blockIdx.x % slabs * 256 + lane * 4;
   const int id = p.key[at];
   if (id < 0 || (at > 0 && p.key[at - 1] == id)) return;
-  int many = 0;  // columns of this target
-  for (int i = at;; i += 64) {
-    const unsigned long long other = __ballot(p.key[i + lane < p.B ? i + lane : p.B] != id);
-    many += other ? __ffsll(other) - 1 : 64;
-    if (other) break;
-  }
   float sum[4] = {};
-  const int from = d < p.Dp ? d : 0;
-#pragma unroll 4
-  for (int i = group; i < many; i += 4) {
-    const int n = p.order[at + i];
-    const float e = token::target_error(p.loss[n], p.scale), left = e - to_f32(cvt<OT>(e));
-    float f[4], g[4] = {};
-    load4(reinterpret_cast<const OT*>(p.ft) + (long long)n * p.Dp + from, f);
-    if (p.terms > 1) load4(reinterpret_cast<const OT*>(p.ft) + ((long long)p.B + n) * p.Dp + from, g);
+  const OT* ft = reinterpret_cast<const OT*>(p.ft) + (d < p.Dp ? d : 0);
+  for (int i = at;; i += 64) {
+    // 64 columns of this target, fewer at its end: a lane each for their places and errors
+    const unsigned long long other = __ballot(p.key[i + lane < p.B ? i + lane : p.B] != id);
+    const int many = other ? __ffsll(other) - 1 : 64, mine = lane < many ? p.order[i + lane] : 0;
+    const float e = token::target_error(p.loss[mine], p.scale), left = e - to_f32(cvt<OT>(e));
+#pragma unroll 8
+    for (int c = group; c < many; c += HOT_GROUPS) {
+      const long long n = __builtin_amdgcn_readlane(mine, c);
+      const float all = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(e), c));
+      const float rest = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(left), c));
+      float f[4], g[4] = {};
+      load4(ft + n * p.Dp, f);
+      if constexpr (TWO) load4(ft + (p.B + n) * p.Dp, g);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) sum[q] += left * f[q] + e * g[q];
+      for (int q = 0; q < 4; ++q) sum[q] += TWO ? rest * f[q] + all * g[q] : rest * f[q];
+    }
+    if (other) break;
   }
   red[group][lane] = make_float4(sum[0], sum[1], sum[2], sum[3]);
   __syncthreads();
   if (group != 0 || d >= p.Dp) return;
   float4 all = red[0][lane];
 #pragma unroll
-  for (int g = 1; g < 4; ++g) {
+  for (int g = 1; g < HOT_GROUPS; ++g) {
     all.x += red[g][lane].x; all.y += red[g][lane].y; all.z += red[g][lane].z; all.w += red[g][lane].w;
   }
   *reinterpret_cast<float4*>(p.hot + (long long)at * p.Dp + d) = all;
@@ -517,8 +522,10 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
     int *order = reinterpret_cast<int*>(ws + o.order), *key = reinterpret_cast<int*>(ws + o.key);
     e = launch_sort_places(p.targets, p.B, p.V, order, key, reinterpret_cast<int*>(ws + o.slot), s);
     if (e != hipSuccess) return;
-    const Hot h{p.B, p.D, o.Dp, o.ft_terms, order, key, at(o.ft), p.loss, reinterpret_cast<float*>(ws + o.hot), scale};
-    hipLaunchKernelGGL((token_hot_kernel<OT>), dim3((unsigned)((long long)p.B * ((o.Dp + 255) / 256))), dim3(256), 0, s, h);
+    const Hot h{p.B, p.D, o.Dp, order, key, at(o.ft), p.loss, reinterpret_cast<float*>(ws + o.hot), scale};
+    const dim3 grid((unsigned)((long long)p.B * ((o.Dp + 255) / 256))), block(HOT_GROUPS * 64);
+    if (o.ft_terms == 2) hipLaunchKernelGGL((token_hot_kernel<OT, true>), grid, block, 0, s, h);
+    else hipLaunchKernelGGL((token_hot_kernel<OT, false>), grid, block, 0, s, h);
     e = hipGetLastError();
   };
   for (int first = 0; first < p.V; first += o.rows) {
