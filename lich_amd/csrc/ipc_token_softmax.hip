@@ -46,6 +46,9 @@ constexpr long long kPieceBytes = 1LL << 30;  // of a piece's errors, and of its
 constexpr long long kOperand = (1LL << 31) - 1;
 // 16-bit updates of at most so many errors and multiplications are `fine`.
 constexpr long long kFineErrors = 1LL << 23, kFineWork = 1LL << 31;
+// And in bf16 those of few words: there probabilities are not small, and rounding them to 8 bits leaves the
+// next loss 2e-5 .. 5e-5 off (600 x 8000 x 1000, 1201 x 4040 x 2744; fine: under 1e-6).
+constexpr int kFineWords = 2048;
 
 struct Plan {
   int terms, Dp, Bk;
@@ -74,7 +77,7 @@ bool make_plan(int V, int D, int B, int storage, int act, bool update, Plan& o) 
   o.Bk = (int)up(B, 32);
   const bool inexact = storage != DT_F32 && act != ACT_IDENTITY && act != ACT_RELU;
   const long long work = (long long)V * B;
-  const bool few = storage != DT_F32 && work <= kFineErrors && work * D <= kFineWork;
+  const bool few = storage != DT_F32 && work <= kFineErrors && (work * D <= kFineWork || (update && storage == DT_BF16 && V <= kFineWords));
   const int most = storage == DT_BF16 ? 3 : 2;
   // (V within a tile: a launch less against half as many workgroups at long sums: us, at once / kept first, bf16
   // 64 x 300 x 200 update 21.7 / 25.8, fp32 128 x 512 x 4000 89 / 98, 26 x 2000 x 30 36.6 / 40.7; 128 x 1000 x 100 39 / 37,
