@@ -339,6 +339,20 @@ def test_a_vocabulary_within_a_tile(V, D, B, name):
         assert bool((got.cpu()[..., padded] == 0).all())
 
 
+# large products: few words (bf16 as small calls), targets' rows made good, the widest tiles
+@pytest.mark.parametrize("V,D,B,name", [(600, 4000, 1000, "bf16"), (601, 3999, 1001, "f16"), (3000, 1500, 600, "bf16"), (6000, 700, 1030, "f16"),
+                                        (4000, 500, 1000, "f16"), (2000, 1030, 500, "f32")])
+def test_token_update_of_large_products(V, D, B, name):
+    dt = TYPES[name]
+    x, w, t = (v.to(DEV) for v in softmax_case(V, D, B, dt, V + D + B))
+    loss, g, wn = run_update(x, w, t, "gelu", 0.5)
+    r = O.softmax(x, w, t, "gelu")
+    bl, bg, bw = softmax_bounds(r, w, dt, V, D, B, "gelu", 0.5)
+    check(loss, r["loss"], bl, "loss")
+    check(g, r["g"], bg, "g")
+    check(wn, w.double() + 0.5 * r["dw"], bw, "w")
+
+
 # weights of more than a piece under few columns
 @pytest.mark.parametrize("V,D,B,name", [(300001, 2001, 1, "bf16"), (600001, 2000, 2, "f16"), (14001, 40001, 1, "bf16"), (30000, 40000, 1, "f16")])
 def test_token_update_of_a_large_table_and_one_sample(V, D, B, name):
