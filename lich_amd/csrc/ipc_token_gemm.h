@@ -37,18 +37,11 @@
 
 #include "ipc_ckpt_gemm.h"
 #include "ipc_token.h"
+#include "ipc_token_plan.h"
 
 namespace ipc {
 
 enum { TOKEN_STATS = 0, TOKEN_KEEP = 1, TOKEN_ERROR = 2, TOKEN_GRAD = 3, TOKEN_WEIGHT = 4, TOKEN_ONE = 5, TOKEN_STATE = 6 };
-
-// Tiles of the first three: rows (of W) and columns of a workgroup, and the rows of a wave, whose
-// largest values and sums are kept (unit; ways: terms of f(X), side by side in a tile; with three
-// TILE_128_64 and TILE_64 alone, each 96 columns wide).
-enum { TILE_256 = 0, TILE_128 = 1, TILE_128_64 = 2, TILE_64 = 3 };
-inline int token_unit(int tile, int ways) {
-  return tile == TILE_256 ? 128 : tile == TILE_128 ? 64 : tile == TILE_128_64 ? (ways == 2 ? 32 : 64) : 32;
-}
 
 // One product.  Rows start at multiples of 4 bytes; a and b with all their terms lie
 // below 2^31 bytes.
@@ -76,11 +69,10 @@ struct TokenGemm {
   const float2* stats;             // ERROR: of each column, largest logit and 1 / sum of exp(z - largest)
 };
 // storage: 0 (three bf16 terms), 1, 2
-// ways: terms of f(X); more than one: the exponentials kept in fp32
+// ways: terms of f(X), as many as token_ways has (ONE: 1, 2, 3 by storage); more than one: the exponentials kept in fp32
 hipError_t launch_token_stats(const TokenGemm& p, int storage, int tile, int ways, hipStream_t s);
 hipError_t launch_token_keep(const TokenGemm& p, int storage, int tile, int ways, hipStream_t s);
 // M at most TOKEN_ONE_ROWS
-constexpr int TOKEN_ONE_ROWS = 128;
 hipError_t launch_token_one(const TokenGemm& p, int storage, int ways, hipStream_t s);
 hipError_t launch_token_error(const TokenGemm& p, int storage, int tile, hipStream_t s);
 hipError_t launch_token_grad(const TokenGemm& p, int storage, int tile, hipStream_t s);
@@ -97,7 +89,6 @@ struct TokenFinish {
   float* fixes;
   int vec;            // x and g allow 4-element accesses
 };
-inline int token_fix_rows(int D, bool vec) { return vec ? (D + 15) / 16 : (D + 3) / 4; }
 hipError_t launch_token_finish(const TokenFinish& p, int storage, hipStream_t s);
 // W's update, and (f) the gradient's last step, which needs no more than that does: in one
 // launch where both are small.
@@ -106,7 +97,6 @@ hipError_t launch_token_weight(const TokenGemm& p, const TokenFinish* f, int sto
 // The state's gradient (g, TOKEN_STATE) from W's copy and W's update (u) in one launch.  u.slices > 1: u's
 // contraction cut into as many, whose sums ([slices][M][N] at part) a second launch adds to W.
 hipError_t launch_token_tail(const TokenGemm& g, const TokenGemm& u, float* part, int storage, hipStream_t s);
-inline long long token_tail_tiles(int V, int D, int B) { return (D + 63LL) / 64 * ((B + 63LL) / 64 + (V + 63LL) / 64); }
 
 namespace token {
 

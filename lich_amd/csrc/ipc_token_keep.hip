@@ -23,6 +23,7 @@ hipError_t run(const TokenGemm& p, int tile, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_token_keep(const TokenGemm& p, int storage, int tile, int ways, hipStream_t s) {
+  if (!token_ways(storage, ways, true)) return hipErrorInvalidValue;
   if (storage == 0) return run<bf16, 3, 1>(p, tile, s);
   if (storage == 1) return ways == 2 ? run<f16, 1, 2>(p, tile, s) : run<f16, 1, 1>(p, tile, s);
   return ways == 3 ? run<bf16, 1, 3>(p, tile, s) : run<bf16, 1, 1>(p, tile, s);

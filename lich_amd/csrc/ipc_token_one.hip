@@ -15,6 +15,7 @@ hipError_t run(const TokenGemm& p, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_token_one(const TokenGemm& p, int storage, int ways, hipStream_t s) {
+  if (ways != (storage == 0 ? 1 : storage == 1 ? 2 : 3)) return hipErrorInvalidValue;
   if (storage == 0) return run<bf16, 3, 1>(p, s);
   return storage == 1 ? run<f16, 1, 2>(p, s) : run<bf16, 1, 3>(p, s);
 }

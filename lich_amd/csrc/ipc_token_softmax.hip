@@ -29,131 +29,16 @@
 //     takes f(X) in two terms (small calls in bf16: three), all in one tile, so that W is read once.
 //   * W: a sum that is 2^-9 off rounds a weight in a few hundred of a target's row the other
 //     way, and the next loss differs by 1e-5 .. 1e-3.
-//   Small updates (kFineErrors, kFineWork: launches, not products, are their time) have f(X) and e in
+//   Small updates (TOKEN_FINE_ERRORS, TOKEN_FINE_WORK: launches, not products, are their time) have f(X) and e in
 //   two terms, three in bf16, and the exponentials in fp32: all of it is good to 2^-22 and better.  Large ones
 //   correct the loss to first order by the gradient that they have, loss -= sum_d (W^T e)_d (f - rounded
 //   f)_d (left: half the variance of the logits' rounding, 3e-6 of a loss for bf16 logits of deviation
 //   3), and make the errors at the targets, the ones near 1, good in fp32 (token_hot_kernel; left in the next
 //   loss: 2e-7 .. 2e-5).
-#include <algorithm>
-
 #include "ipc_token_gemm.h"
 
 namespace ipc {
 namespace {
-
-constexpr long long kPieceBytes = 1LL << 30;  // of a piece's errors, and of its rows of W where those are laid out
-constexpr long long kOperand = (1LL << 31) - 1;
-// 16-bit updates of at most so many errors and multiplications are `fine`.
-constexpr long long kFineErrors = 1LL << 23, kFineWork = 1LL << 31;
-// And in bf16 those of few words: there probabilities are not small, and rounding them to 8 bits leaves the
-// next loss 2e-5 .. 5e-5 off (600 x 8000 x 1000, 1201 x 4040 x 2744; fine: under 1e-6).
-constexpr int kFineWords = 2048;
-
-struct Plan {
-  int terms, Dp, Bk;
-  bool copy;          // W laid out per piece: fp32, 16-bit rows of an odd length, or for `tail`
-  int ways;           // terms of f(X) in the logits, in 16 bits
-  bool fine;          // the update in 16 bits, small: errors and f(X) in `ways` terms
-  bool mend;          // the update in 16 bits, large: targets' errors made good in fp32
-  bool fix;           // and the loss corrected
-  int ft_terms, f_terms, e_terms;
-  bool keep;          // one piece, its exponentials kept
-  bool one;           // one tile: losses (and errors) at once
-  bool tail;          // the gradient and W's update in one launch, from W's copy
-  int cut;            // slices of the batch in that
-  int rows, Vp;       // of a piece (the last may have fewer), ET's row length
-  int tile, unit;     // of the logits
-  int grad_tile, slices;
-  long long f, ft, et, kept, ws, part, stats, logit, norm, fixes, order, key, slot, hot, bytes;  // offsets in the workspace
-};
-
-bool make_plan(int V, int D, int B, int storage, int act, bool update, Plan& o) {
-  auto up = [](long long v, long long m) { return (v + m - 1) / m * m; };
-  o = Plan{};
-  o.terms = storage == DT_F32 ? 3 : 1;
-  if (D > (1 << 26) || B > (1 << 26)) return false;
-  o.Dp = (int)up(D, 32);
-  o.Bk = (int)up(B, 32);
-  const bool inexact = storage != DT_F32 && act != ACT_IDENTITY && act != ACT_RELU;
-  const long long work = (long long)V * B;
-  const bool few = storage != DT_F32 && work <= kFineErrors && (work * D <= kFineWork || (update && storage == DT_BF16 && V <= kFineWords));
-  const int most = storage == DT_BF16 ? 3 : 2;
-  // (V within a tile: a launch less against half as many workgroups at long sums: us, at once / kept first, bf16
-  // 64 x 300 x 200 update 21.7 / 25.8, fp32 128 x 512 x 4000 89 / 98, 26 x 2000 x 30 36.6 / 40.7; 128 x 1000 x 100 39 / 37,
-  // 100 x 4001 x 16 77 / 64; the loss alone, 64 x 300 x 200 11.6 / 13.7, 100 x 90 x 64 12.8 / 11.9)
-  const bool within = V <= TOKEN_ONE_ROWS / 2 || (update && V <= TOKEN_ONE_ROWS && D <= 512);
-  const bool tail = update && (few || storage == DT_F32) && V <= 480 && (long long)V * D <= 1 << 20 && token_tail_tiles(V, D, B) <= 256;
-  o.copy = storage == DT_F32 || D % 2 != 0 || tail;
-  const long long state = 2LL * o.Dp * o.Bk;
-  // the rows of a piece, 0 for sizes that the kernels do not take
-  auto pieces = [&](bool fine) -> long long {
-    o.fine = fine;
-    o.mend = update && storage != DT_F32 && !fine;
-    o.fix = inexact && o.mend;
-    o.ways = fine || (inexact && !update) ? few && state * most <= kOperand ? most : 2 : 1;
-    o.ft_terms = storage == DT_F32 ? 3 : o.fix ? 2 : o.ways;
-    o.f_terms = o.e_terms = storage == DT_F32 ? 3 : fine ? most : 1;
-    if (state * o.ft_terms > kOperand) return 0;
-    const long long row_w = 2LL * (o.copy ? o.terms * o.Dp : D), row_e = update ? 2LL * o.e_terms * o.Bk : 1;
-    long long rows = std::min((o.copy ? kPieceBytes : kOperand) / row_w, kPieceBytes / row_e) / 256 * 256;
-    if (rows < 256) rows = 256;
-    rows = std::min<long long>(rows, V);
-    return up(rows, 32) * std::max(row_w, row_e) > kOperand ? 0 : rows;
-  };
-  long long rows = pieces(update && few);
-  if (o.fine && rows < V) rows = pieces(false);  // (weights of more than a piece: not a small call)
-  if (rows == 0) return false;
-  o.rows = (int)rows;
-  o.Vp = (int)up(o.rows, 32);
-  o.keep = update && o.rows == V && (storage != DT_F32 || (long long)o.Bk * o.Vp * 10 <= kPieceBytes);
-  o.one = within && (update ? o.keep && !o.mend : o.rows == V && (storage == DT_F32 || (few && o.ways == most)));
-  auto tiles = [&](long long m, long long n, long long e) { return ((m + e - 1) / e) * ((n + e - 1) / e); };
-  const long long columns = (long long)o.ways * B;
-  // (the largest tile that gives the CUs one each; fp32: us, 64 wide / 128 x 64, 4000 x 4000 x 512 update 355 / 336,
-  // 10007 x 515 x 77 77 / 72)
-  if (o.ways == 3) o.tile = (o.rows + 127LL) / 128 * ((B + 31LL) / 32) >= 256 ? TILE_128_64 : TILE_64;
-  else if (columns <= 64) o.tile = o.rows >= 32768 ? TILE_128_64 : TILE_64;
-  else o.tile = storage != DT_F32 && tiles(o.rows, columns, 256) >= 192 ? TILE_256 : tiles(o.rows, columns, 128) > 128 ? TILE_128 : storage == DT_F32 && (o.rows + 127LL) / 128 * ((columns + 63) / 64) >= 128 ? TILE_128_64 : TILE_64;
-  o.unit = token_unit(o.tile, o.ways);
-  // (few tiles: narrow ones, with longer slices: us, fp32 10007 x 515 x 77 70.4 / 70.0, bf16 1000 x 1000 x 128 35.7 / 34.2)
-  o.grad_tile = storage != DT_F32 && D >= 256 && B >= 256 ? 256 : D > 64 && tiles(D, B, 128) > 8 ? 128 : 64;
-  const long long gt = o.grad_tile == 256 ? tiles(D, B, 256)
-                       : o.grad_tile == 128 ? (D + 127LL) / 128 * (B > 64 ? (B + 127LL) / 128 : 1) : tiles(D, B, 64);
-  const long long stages = o.Vp / 32;
-  o.slices = (int)std::max<long long>(1, std::min({256 / gt, stages / 8, 64LL}));
-  o.tail = tail && o.keep && !o.mend && o.slices == 1;
-  // (W's product: as many slices of eight steps and more as give every CU a workgroup, three at least: us, cut / whole, bf16
-  // 6 x 73 x 3026 21.7 / 45, 329 x 3 x 4059 40 / 66, 26 x 40 x 2000 21.3 / 29.2; two: 256 x 256 x 512 27.2 / 25.6)
-  o.cut = (int)std::min<long long>(o.Bk / 256, (256 - tiles(D, B, 64)) / tiles(V, D, 64));
-  if (o.cut < 3) o.cut = 1;
-  long long at = 0;
-  auto take = [&](long long bytes) {
-    const long long here = at;
-    at += up(bytes, 256);
-    return here;
-  };
-  o.ft = take(state * o.ft_terms);
-  o.logit = take(4LL * B);
-  o.norm = take(8LL * B);
-  o.stats = take(8LL * B * (((long long)V + o.unit - 1) / o.unit));
-  if (o.copy) o.ws = take((long long)o.terms * o.Vp * o.Dp * 2);
-  if (update) {
-    o.f = take(state * o.f_terms);
-    o.et = take((long long)o.e_terms * o.Bk * o.Vp * 2);
-    o.part = o.tail ? o.cut > 1 ? take(4LL * o.cut * V * D) : 0 : take(4LL * o.slices * D * B);
-    o.kept = o.e_terms == 1 ? o.et : o.keep && !o.one ? take(4LL * o.Bk * o.Vp) : 0;
-    o.fixes = o.fix ? take(4LL * B * token_fix_rows(D, false)) : 0;
-    if (o.mend) {
-      o.order = take(4LL * B);
-      o.key = take(4LL * (B + 1));
-      o.slot = take(4LL * V);
-      o.hot = take(4LL * B * o.Dp);
-    }
-  }
-  o.bytes = at;
-  return true;
-}
 
 // ------------------------------------------------------------------ f(X)
 // F [f_terms][D][Bk] and FT [T][B][Dp] of X [D][B] in the operand type (T terms), zeros past
@@ -439,8 +324,8 @@ __global__ void __launch_bounds__(HOT_GROUPS * 64) token_hot_kernel(const Hot p)
 template <typename ST, typename OT, int TERMS, int ACT>
 hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
   const bool update = p.g != nullptr;
-  Plan o;
-  if (!make_plan(p.V, p.D, p.B, storage, p.act, update, o)) return hipErrorInvalidValue;
+  TokenPlan o;
+  if (!plan_token(p.V, p.D, p.B, storage, p.act, update, o)) return hipErrorInvalidValue;
   unsigned char* ws = p.workspace;
   auto at = [&](long long offset) { return reinterpret_cast<unsigned short*>(ws + offset); };
   const States st{p.D, p.B, p.V, o.Dp, o.Bk, o.f_terms, p.x, p.targets, update ? at(o.f) : nullptr, at(o.ft)};
@@ -600,8 +485,8 @@ hipError_t by_act(const TokenProblem& p, int storage, hipStream_t s) {
 
 long long token_workspace_bytes(int V, int D, int B, int storage, int act, bool update) {
   if (token_few(V, D, B, storage)) return token_few_workspace_bytes(V, D, B, storage, update);
-  Plan o;
-  return make_plan(V, D, B, storage, act, update, o) ? o.bytes : 0;
+  TokenPlan o;
+  return plan_token(V, D, B, storage, act, update, o) ? o.bytes : 0;
 }
 
 hipError_t launch_token(const TokenProblem& p, int storage, hipStream_t s) {
