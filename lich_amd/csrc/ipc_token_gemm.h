@@ -51,7 +51,7 @@ struct TokenGemm {
   const void* b; long long ldb;
   long long a_bytes, b_bytes;      // buffers' ends (loads past them give 0)
   unsigned a_term, b_term;         // bytes from one term to the next
-  int slices;                      // GRAD (and WEIGHT, see launch_token_tail): of the contraction
+  int slices;                      // GRAD (and WEIGHT, see launch_token_tail): of the contraction, a stage of 32 each at least
   void* out;                       // STATS, KEEP: float2 [units][N]; ERROR: ET; GRAD: [slices][M][N] fp32; WEIGHT: W
   void* kept;                      // KEEP: exponentials times 2^15 in fp16 (fp32: in fp32), layout of ET
   long long out_ld, out_term;      // KEEP, ERROR: elements

@@ -17,6 +17,7 @@ hipError_t grad(const TokenGemm& p, int tile, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_token_grad(const TokenGemm& p, int storage, int tile, hipStream_t s) {
+  if (p.slices < 1 || p.slices > p.K / 32) return hipErrorInvalidValue;  // (a slice without a stage has no first one to load)
   if (storage == 0) return grad<bf16, 3>(p, tile, s);
   return storage == 1 ? grad<f16, 1>(p, tile, s) : grad<bf16, 1>(p, tile, s);
 }

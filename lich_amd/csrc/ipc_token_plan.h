@@ -140,4 +140,8 @@ inline bool plan_token(int V, int D, int B, int storage, int act, bool update, T
   return true;
 }
 
+// Of the gradient's contraction over a piece of `rows` rows: as many slices as a whole piece has, but of one stage of
+// 32 at least.  (A later piece adds to the first so many sums; the others have theirs.)
+inline int token_piece_slices(const TokenPlan& o, int rows) { return std::min(o.slices, (rows + 31) / 32); }
+
 }  // namespace ipc

@@ -441,7 +441,7 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
     weights(first, g, false);
     g.M = p.D; g.N = p.B; g.K = Vp;
     g.b = at(o.et); g.ldb = Vp; g.b_term = (unsigned)((long long)o.Bk * Vp * 2); g.b_bytes = (long long)TERMS * o.Bk * Vp * 2;
-    g.slices = o.slices; g.out = ws + o.part; g.add = first > 0;
+    g.slices = token_piece_slices(o, rows); g.out = ws + o.part; g.add = first > 0;
     if (!o.tail) e = launch_token_grad(g, storage, o.grad_tile, s);
     if (e != hipSuccess) return e;
     TokenGemm u{};

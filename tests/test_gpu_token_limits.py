@@ -41,3 +41,9 @@ def check_update(x, w, t, activation, alpha):
                                                    (300, 16384, 24576, "silu", "bf16"), (40, 20000, 20000, "tanh", "f16"), (3, 30000, 20000, "relu", "f16")])
 def test_updates_of_large_states(V, D, B, activation, name):
     check_update(*large_case(V, D, B, TYPES[name]), activation, 0.5)
+
+
+# vocabularies in pieces whose last one has fewer stages of 32 rows than a whole one has slices
+@pytest.mark.parametrize("V,D,B,name", [(524298, 64, 1000, "bf16"), (524289, 8, 1000, "f16"), (131073, 300, 4096, "f16"), (21770, 8192, 64, "f32"), (91793, 1949, 118, "f32")])
+def test_short_last_pieces(V, D, B, name):
+    check_update(*large_case(V, D, B, TYPES[name]), "tanh", 0.5)

@@ -12,7 +12,7 @@ F32, F16, BF16 = 0, 1, 2
 IDENTITY, TANH = 0, 2
 OPERAND = 2 ** 31 - 1
 FIELDS = ("taken terms Dp Bk copy ways fine mend fix ft_terms f_terms e_terms keep one tail cut rows Vp tile unit grad_tile "
-          "slices f ft et kept ws part stats bytes").split()
+          "slices f ft et kept ws part stats bytes last last_slices").split()
 
 
 class Plan:
@@ -27,7 +27,7 @@ class Plan:
 def plans(tmp_path_factory):
     """plans(cases): the accepted ones of (V, D, B, storage, activation, update)."""
     at = tmp_path_factory.mktemp("plan")
-    values = ", (long long)o.".join(["(long long)taken"] + FIELDS[1:])
+    values = ", (long long)o.".join(["(long long)taken"] + FIELDS[1:-2]) + ", last, ipc::token_piece_slices(o, last)"
     (at / "plan.cpp").write_text("""
 #include <cstdio>
 namespace ipc { enum { DT_F32 = 0, DT_F16 = 1, DT_BF16 = 2 }; enum { ACT_IDENTITY = 0, ACT_RELU = 1 }; }
@@ -37,6 +37,7 @@ int main() {
   while (scanf("%%d %%d %%d %%d %%d %%d", &V, &D, &B, &storage, &act, &update) == 6) {
     ipc::TokenPlan o;
     const bool taken = ipc::plan_token(V, D, B, storage, act, update != 0, o);
+    const int last = taken ? (V - 1) %% o.rows + 1 : 0;  // rows of the last piece
     const long long all[] = {%s};
     for (long long v : all) printf("%%lld ", v);
     printf("\\n");
@@ -121,3 +122,25 @@ def test_updates_whose_states_fit_in_two_terms_alone(plans, V, D, B):
     """bf16, few words: not in three terms, so not as a small call."""
     p, = plans([(V, D, B, BF16, TANH, 1)])
     assert (p.fine, p.mend, p.ways, p.ft_terms, p.f_terms, p.e_terms) == (0, 1, 1, 2, 1, 1)
+
+
+def slices_of(p):
+    """First stage and the one behind the last of each slice of the last piece, as product_tile has them."""
+    stages = (p.last + 31) // 32
+    return [(stages * s // p.last_slices, stages * (s + 1) // p.last_slices) for s in range(p.last_slices)]
+
+
+def test_every_slice_of_every_piece_has_a_stage(plans, accepted):
+    """A whole piece has eight stages a slice and more; the last one may be of a single row."""
+    in_pieces = [(V, D, B, storage, TANH, 1) for V in (151936, 256128, 262144, 131073, 524298, 21770, 91793) for D in (64, 1024, 1949, 2048, 4096, 4192, 8192)
+                 for B in (9, 64, 118, 128, 256, 1000, 4096) for storage in (F32, F16, BF16) if V * D <= OPERAND]
+    short = 0
+    for p in plans(in_pieces) + [p for p in accepted if p.update]:
+        if p.tail:
+            continue
+        assert 1 <= p.slices <= max(1, p.Vp // 32 // 8), p.case
+        assert 1 <= p.last_slices <= p.slices, p.case
+        for begin, end in slices_of(p):
+            assert 0 <= begin < end <= (p.last + 31) // 32, p.case
+        short += p.rows < p.V and p.last_slices < p.slices
+    assert short > 20
