@@ -75,7 +75,8 @@ hipError_t launch_token_keep(const TokenGemm& p, int storage, int tile, int ways
 // M at most TOKEN_ONE_ROWS
 hipError_t launch_token_one(const TokenGemm& p, int storage, int ways, hipStream_t s);
 hipError_t launch_token_error(const TokenGemm& p, int storage, int tile, hipStream_t s);
-hipError_t launch_token_grad(const TokenGemm& p, int storage, int tile, hipStream_t s);
+// ways: terms of the errors, 1 or (16 bits) 2
+hipError_t launch_token_grad(const TokenGemm& p, int storage, int tile, int ways, hipStream_t s);
 
 // The state's gradient from its slices, G = f'(X) sum, zeros in padded columns, and what
 // the loss is off by for f(X)'s rounding (fixes: [token_fix_rows][B], or nullptr).
@@ -94,7 +95,7 @@ hipError_t launch_token_finish(const TokenFinish& p, int storage, hipStream_t s)
 // launch where both are small.
 // terms: of both operands in 16-bit storage, 1, 2 (fp16) or 3 (bf16)
 hipError_t launch_token_weight(const TokenGemm& p, const TokenFinish* f, int storage, int terms, hipStream_t s);
-// The state's gradient (g, TOKEN_STATE) from W's copy and W's update (u) in one launch.  u.slices > 1: u's
+// The state's gradient (g, TOKEN_STATE; in 16 bits with two terms of the errors) from W's copy and W's update (u) in one launch.  u.slices > 1: u's
 // contraction cut into as many, whose sums ([slices][M][N] at part) a second launch adds to W.
 hipError_t launch_token_tail(const TokenGemm& g, const TokenGemm& u, float* part, int storage, hipStream_t s);
 
@@ -130,7 +131,7 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
   constexpr int RNC = RN / WAYS, BNC = BN / WAYS, WTC = WTN / WAYS;  // blocks and columns of different n
   constexpr bool SPLIT = TERMS == 3, FINE = SPLIT || ((MODE == TOKEN_KEEP || MODE == TOKEN_ONE) && WAYS > 1);  // FINE: kept in fp32
   constexpr int A_BYTES = BM * 64, B_BYTES = BN * 64, STAGE = TERMS * (A_BYTES + B_BYTES);
-  static_assert(WAYS == 1 || ((MODE == TOKEN_STATS || MODE == TOKEN_KEEP || MODE == TOKEN_ONE) && TERMS == 1 && RN % WAYS == 0), "terms of f(X)");
+  static_assert(WAYS == 1 || (MODE != TOKEN_ERROR && MODE != TOKEN_WEIGHT && TERMS == 1 && RN % WAYS == 0), "terms of B");
   constexpr int IA = A_BYTES / 1024 / NW, IB = B_BYTES / 1024 / NW, LPS = TERMS * (IA + IB);  // LDS-DMA loads per wave and stage
   static_assert(IA * 1024 * NW == A_BYTES && IB * 1024 * NW == B_BYTES, "tile / waves");
 
@@ -164,7 +165,7 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
     const int r = slot >> 2, c = (slot & 3) ^ ((r >> 2) & 3), row = e0 + r < lim ? e0 + r : lim - 1;
     return (unsigned)(row * ld) * 2u + (unsigned)c * 16u;
   };
-  // (WAYS > 1: the first of as many parts of a wave's columns holds f(X)'s leading term, the
+  // (WAYS > 1: the first of as many parts of a wave's columns holds B's leading term, the
   // others, the same columns, the next ones)
   auto source_ways = [&](int q) -> unsigned {
     const int slot = (q * NW + w) * 64 + lane, r = slot >> 2, c = (slot & 3) ^ ((r >> 2) & 3);
@@ -381,7 +382,7 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
 #pragma unroll
       for (int j = 0; j < RNC; ++j)
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {  // (an infinite weight times the rest of f(X), of either sign, is no matter)
+        for (int q = 0; q < 16; ++q) {  // (an infinite weight times the rest, of either sign, is no matter)
           float rest = acc[i][j + RNC][q];
           if constexpr (WAYS == 3) rest += acc[i][j + 2 * RNC][q];
           acc[i][j][q] += __builtin_isinf(acc[i][j][q]) ? 0.0f : rest;
@@ -522,14 +523,14 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
       __builtin_amdgcn_sched_barrier(0);
     }
   } else if constexpr (MODE == TOKEN_STATE) {
-    static_assert(RM == 1 && RN == 1, "a block a wave");
+    static_assert(RM == 1 && RNC == 1, "a block a wave");
     __syncthreads();
     float* es = reinterpret_cast<float*>(smem) + w * 32 * 36;
 #pragma unroll
     for (int q = 0; q < 16; q += 4)
       *reinterpret_cast<float4*>(es + lr * 36 + 2 * q + 4 * lk) = make_float4(acc[0][0][q], acc[0][0][q + 1], acc[0][0][q + 2], acc[0][0][q + 3]);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    const int n = n0 + wn * WTN + lr;
+    const int n = n0 + wn * WTC + lr;
     const long long id = n < N ? p.targets[n] : -1;
     const bool real = id >= 0 && id < p.V;
 #pragma unroll 1
@@ -545,11 +546,16 @@ __device__ __forceinline__ void product_tile(const TokenGemm& p, unsigned char* 
     MxProblem e{};
     e.M = M; e.N = N; e.scal = MODE == TOKEN_GRAD ? 1.0f : p.scal;
     e.out = MODE == TOKEN_GRAD ? static_cast<float*>(p.out) + (long long)slice * M * N : p.out;
-    float* es = reinterpret_cast<float*>(smem) + w * 32 * (WTN + 4);
-    const int mw = m0 + wm * WTM, nw = n0 + wn * WTN;
-    if (MODE == TOKEN_GRAD && !p.add) tile_epilogue<TT, KIND_FWD, ACT_IDENTITY, true, RM, RN>(e, acc, es, mw, nw);
-    else if (MODE == TOKEN_GRAD || p.vec) tile_epilogue<TT, KIND_WEIGHT, ACT_IDENTITY, true, RM, RN>(e, acc, es, mw, nw);
-    else tile_epilogue<TT, KIND_WEIGHT, ACT_IDENTITY, false, RM, RN>(e, acc, es, mw, nw);
+    float* es = reinterpret_cast<float*>(smem) + w * 32 * (WTC + 4);
+    const int mw = m0 + wm * WTM, nw = n0 + wn * WTC;
+    f32x16 sum[RM][RNC];
+#pragma unroll
+    for (int i = 0; i < RM; ++i)
+#pragma unroll
+      for (int j = 0; j < RNC; ++j) sum[i][j] = acc[i][j];
+    if (MODE == TOKEN_GRAD && !p.add) tile_epilogue<TT, KIND_FWD, ACT_IDENTITY, true, RM, RNC>(e, sum, es, mw, nw);
+    else if (MODE == TOKEN_GRAD || p.vec) tile_epilogue<TT, KIND_WEIGHT, ACT_IDENTITY, true, RM, RNC>(e, sum, es, mw, nw);
+    else tile_epilogue<TT, KIND_WEIGHT, ACT_IDENTITY, false, RM, RNC>(e, sum, es, mw, nw);
   }
 }
 

@@ -41,7 +41,7 @@ struct TokenPlan {
   int cut;            // slices of the batch in that
   int rows, Vp;       // of a piece (the last may have fewer), ET's row length
   int tile, unit;     // of the logits
-  int grad_tile, slices;
+  int grad_tile, grad_ways, slices;  // of the gradient; its terms of the errors
   long long f, ft, et, kept, ws, part, stats, logit, norm, fixes, order, key, slot, hot, bytes;  // offsets in the workspace
 };
 
@@ -103,7 +103,8 @@ inline bool plan_token(int V, int D, int B, int storage, int act, bool update, T
   o.unit = token_unit(o.tile, o.ways);
   // (few tiles: narrow ones, with longer slices: us, fp32 10007 x 515 x 77 70.4 / 70.0, bf16 1000 x 1000 x 128 35.7 / 34.2)
   o.grad_tile = storage != DT_F32 && D >= 256 && B >= 256 ? 256 : D > 64 && tiles(D, B, 128) > 8 ? 128 : 64;
-  const long long gt = o.grad_tile == 256 ? tiles(D, B, 256)
+  o.grad_ways = o.fine ? 2 : 1;
+  const long long gt = o.grad_tile == 256 ? (D + 255LL) / 256 * ((B + 256 / o.grad_ways - 1LL) / (256 / o.grad_ways))
                        : o.grad_tile == 128 ? (D + 127LL) / 128 * (B > 64 ? (B + 127LL) / 128 : 1) : tiles(D, B, 64);
   const long long stages = o.Vp / 32;
   o.slices = (int)std::max<long long>(1, std::min({256 / gt, stages / 8, 64LL}));

@@ -24,7 +24,9 @@
 //
 // In 16 bits errors and, but for identity and relu, f(X) do not fit the operand type.  What
 // the results lose by it, and what is done:
-//   * G is rounded to the type itself: nothing.
+//   * G is rounded to the type itself, but a target's error, rounded once, would be off by as much for the whole
+//     column, and half of its values would be next to the right ones.  Small updates multiply two terms of the errors
+//     (2^-16, 2^-22) with W.
 //   * the loss is fp32 and would be off by the logits' rounding, 2^-9 (2^-12).  The loss alone
 //     takes f(X) in two terms (small calls in bf16: three), all in one tile, so that W is read once.
 //   * W: a sum that is 2^-9 off rounds a weight in a few hundred of a target's row the other
@@ -440,9 +442,9 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
     TokenGemm g{};
     weights(first, g, false);
     g.M = p.D; g.N = p.B; g.K = Vp;
-    g.b = at(o.et); g.ldb = Vp; g.b_term = (unsigned)((long long)o.Bk * Vp * 2); g.b_bytes = (long long)TERMS * o.Bk * Vp * 2;
+    g.b = at(o.et); g.ldb = Vp; g.b_term = (unsigned)((long long)o.Bk * Vp * 2); g.b_bytes = (long long)o.e_terms * o.Bk * Vp * 2;
     g.slices = token_piece_slices(o, rows); g.out = ws + o.part; g.add = first > 0;
-    if (!o.tail) e = launch_token_grad(g, storage, o.grad_tile, s);
+    if (!o.tail) e = launch_token_grad(g, storage, o.grad_tile, o.grad_ways, s);
     if (e != hipSuccess) return e;
     TokenGemm u{};
     u.a = at(o.et); u.lda = Vp; u.a_term = g.b_term; u.a_bytes = (long long)o.e_terms * o.Bk * Vp * 2;

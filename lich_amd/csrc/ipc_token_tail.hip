@@ -6,18 +6,23 @@
 namespace ipc {
 namespace {
 
+// The gradient's tile: 64 columns, in 16 bits (GT = 1) with two terms of the errors side by side.
+template <int GT> constexpr int kWays = GT == 1 ? 2 : 1;
+template <int GT> constexpr int kWide = 64 * kWays<GT>;
+template <int GT> constexpr int kStages = GT == 3 ? 6 : 8;
+
 // CUT: W's product as slices (of the form of TOKEN_GRAD: both read A by rows of the contraction)
 template <typename OT, int GT, int UT, bool CUT, typename WT>
 __global__ void __launch_bounds__(256) token_tail_kernel(const TokenGemm g, const TokenGemm u, unsigned first) {
   extern __shared__ __align__(16) unsigned char smem[];
   constexpr int UM = CUT ? TOKEN_GRAD : TOKEN_WEIGHT;
-  if (blockIdx.x < first) token::product_tile<OT, GT, TOKEN_STATE, 1, 64, 64, 2, 2, GT == 3 ? 6 : 8, WT>(g, smem, blockIdx.x, first);
+  if (blockIdx.x < first) token::product_tile<OT, GT, TOKEN_STATE, kWays<GT>, 64, kWide<GT>, 2, 2, kStages<GT>, WT>(g, smem, blockIdx.x, first);
   else token::product_tile<OT, UT, UM, 1, 64, 64, 2, 2, UT == 3 ? 6 : 4, WT>(u, smem, blockIdx.x - first, gridDim.x - first);
 }
 
 template <typename OT, int GT, int UT, bool CUT, typename WT>
 hipError_t products(const TokenGemm& g, const TokenGemm& u, hipStream_t s) {
-  constexpr int a = token::tile_lds<GT, TOKEN_STATE, 1, 64, 64, 2, 2, GT == 3 ? 6 : 8>(), b = token::tile_lds<UT, TOKEN_WEIGHT, 1, 64, 64, 2, 2, UT == 3 ? 6 : 4>();
+  constexpr int a = token::tile_lds<GT, TOKEN_STATE, kWays<GT>, 64, kWide<GT>, 2, 2, kStages<GT>>(), b = token::tile_lds<UT, TOKEN_WEIGHT, 1, 64, 64, 2, 2, UT == 3 ? 6 : 4>();
   constexpr int smem = a > b ? a : b;
   const void* fn = reinterpret_cast<const void*>(&token_tail_kernel<OT, GT, UT, CUT, WT>);
   static const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, smem);

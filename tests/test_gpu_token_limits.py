@@ -5,7 +5,7 @@ import torch
 
 from tests import token_oracle as O
 from tests.helpers import DEV
-from tests.test_gpu_tokens import TYPES, run_update, softmax_bounds
+from tests.test_gpu_tokens import H, TYPES, half_step, run_update, softmax_bounds, softmax_case
 
 pytestmark = pytest.mark.gpu
 
@@ -34,6 +34,37 @@ def check_update(x, w, t, activation, alpha):
     check(wn, w.double() + alpha * r["dw"], bw, "w")
     padded = t < 0
     assert bool((loss[padded] == 0).all()) and bool((g[:, padded] == 0).all())
+
+
+# G in 16 bits is the rounding of a sum that is good to a few H, where errors rounded to 16 bits would leave u in a whole
+# column: it may differ from the exact sum's rounding only where that lies within the sum's bound of a tie.  e, per element:
+# p's own error (the logits' two or three terms of f(X), exp, the sum of V exponentials in a tree of parts, as for the weights
+# of test_gpu_tokens.py) and what is left of two terms, u^2 of it.  A matrix instruction adds 16 products to a sum at once:
+# D / 16 steps of three terms in a logit, V / 16 of two in G, and within a step's products 16 H.
+def gradient_bounds(r, x, w, V, D, dt):
+    u, half = half_step(dt), dt == torch.float16
+    exact, small, wa, ea = not bool((r["f"].to(dt).double() != r["f"]).any()), 2.0 ** -25 * half, w.double().abs(), r["e"].abs()
+    dz = (r["size"] * ((0.0 if exact else 18 * H) + (3 * D / 16 + 64) * H)).max(0).values + small * 2.0 ** -11 * wa.sum(1).max()
+    de = r["p"] * ((2 * dz).expm1() + 8 * H * (1 + r["p"].clamp(min=1e-300).log().abs()) + 256 * H) + (u * u + 4 * H) * ea + 2.0 ** -34 * half
+    return r["df"].abs() * (wa.T @ de + (V / 8 + 64) * H * (wa.T @ ea)) + 16 * H * (wa.T @ ea) + 2 * H * r["g"].abs()
+
+
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+@pytest.mark.parametrize("V,D,B,activation", [(2, 200, 400, "relu"), (90, 70, 40, "tanh"), (400, 60, 90, "identity"), (100, 600, 70, "gelu"), (300, 130, 40, "relu"),
+                                              (700, 90, 130, "silu"), (600, 300, 300, "relu"), (3000, 8, 12, "tanh"), (500, 400, 20, "sigmoid"),
+                                              (700, 1100, 70, "relu"), (600, 1200, 33, "identity")])
+def test_state_gradients_round_as_the_exact_sums(V, D, B, activation, name):
+    dt = TYPES[name]
+    x, w, t = softmax_case(V, D, B, dt, V + D)
+    got = run_update(x.to(DEV), w.to(DEV), t.to(DEV), activation, 0.25)[1].cpu()
+    r = O.softmax(x, w, t, activation)
+    bound = gradient_bounds(r, x, w, V, D, dt)
+    low, high = (r["g"] - bound).to(dt), (r["g"] + bound).to(dt)
+    assert bool(((got >= low) & (got <= high)).all()), int(((got < low) | (got > high)).sum())
+    # (errors rounded to 16 bits would not pass; but at D = 1200 a logit's bound, 289 H of magnitudes of 44 in all, lets p
+    # be off by 2^-9 of itself, more than fp16's half step)
+    plain = (r["df"] * (w.double().T @ r["e"].to(dt).double())).to(dt)
+    assert D > 1000 or bool(((plain < low) | (plain > high)).any())
 
 
 # states that fit an operand in two terms but not in three; the last three in fp16, which takes two

@@ -11,7 +11,7 @@ ROOT = Path(__file__).resolve().parents[1]
 F32, F16, BF16 = 0, 1, 2
 IDENTITY, TANH = 0, 2
 OPERAND = 2 ** 31 - 1
-FIELDS = ("taken terms Dp Bk copy ways fine mend fix ft_terms f_terms e_terms keep one tail cut rows Vp tile unit grad_tile "
+FIELDS = ("taken terms Dp Bk copy ways fine mend fix ft_terms f_terms e_terms keep one tail cut rows Vp tile unit grad_tile grad_ways "
           "slices f ft et kept ws part stats bytes last last_slices").split()
 
 
@@ -86,12 +86,12 @@ def test_as_many_terms_are_laid_out_as_multiplied(accepted):
     for p in accepted:
         if p.storage == F32:
             assert (p.ways, p.ft_terms, p.terms, p.fine, p.mend) == (1, 3, 3, 0, 0), p.case
-            assert not p.update or p.f_terms == p.e_terms == 3, p.case
+            assert not p.update or (p.f_terms == p.e_terms == 3 and p.grad_ways == 1), p.case
             continue
         assert p.ft_terms >= p.ways, p.case
         if p.update:
             assert p.f_terms <= p.ft_terms and p.f_terms == p.e_terms, p.case
-            assert p.fine != p.mend, p.case
+            assert p.fine != p.mend and p.grad_ways == 1 + p.fine, p.case
             most = 2 if p.storage == F16 else 3
             assert (p.ways, p.ft_terms, p.f_terms) == ((most,) * 3 if p.fine else (1, 2 if p.fix else 1, 1)), p.case
 
