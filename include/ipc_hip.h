@@ -630,8 +630,8 @@ int ipc_dropout(const void* x, const long long* rng, void* out, int M, int B, in
  *   - 16 bits: w as it is; the loss alone takes f(X) in two terms of the type, a small call
  *     (at most 2^23 errors and 2^31 multiplications; of bf16 updates of up to 2048 words any number
  *     of these) f(X) and e in two fp16 or three bf16 terms (e for g in two).  A
- *     larger update rounds both to the type once, makes the sums of the targets' rows
- *     good in fp32 and corrects the loss to first order in what f(X)'s rounding left.
+ *     larger update rounds both to the type once, makes the targets' share of w's and g's
+ *     sums good in fp32 and corrects the loss to first order in what f(X)'s rounding left.
  * A word whose weights give it logits far below the others' has no share of anything; infinite
  * weights are for the loss alone (g takes 0 times infinity where they are not the largest bf16).
  * Both need a workspace (16-byte aligned) of ipc_token_loss_workspace_bytes /

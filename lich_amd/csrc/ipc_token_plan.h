@@ -32,7 +32,7 @@ struct TokenPlan {
   bool copy;          // W laid out per piece: fp32, 16-bit rows of an odd length, or for `tail`
   int ways;           // terms of f(X) in the logits, in 16 bits
   bool fine;          // the update in 16 bits, small: errors and f(X) in `ways` terms
-  bool mend;          // the update in 16 bits, large: targets' errors made good in fp32
+  bool mend;          // the update in 16 bits, large: targets' errors made good in fp32 (for G in a slice of its own)
   bool fix;           // and the loss corrected
   int ft_terms, f_terms, e_terms;
   bool keep;          // one piece, its exponentials kept
@@ -127,7 +127,7 @@ inline bool plan_token(int V, int D, int B, int storage, int act, bool update, T
   if (update) {
     o.f = take(state * o.f_terms);
     o.et = take((long long)o.e_terms * o.Bk * o.Vp * 2);
-    o.part = o.tail ? o.cut > 1 ? take(4LL * o.cut * V * D) : 0 : take(4LL * o.slices * D * B);
+    o.part = o.tail ? o.cut > 1 ? take(4LL * o.cut * V * D) : 0 : take(4LL * (o.slices + (o.mend ? 1 : 0)) * D * B);
     o.kept = o.e_terms == 1 ? o.et : o.keep && !o.one ? take(4LL * o.Bk * o.Vp) : 0;
     o.fixes = o.fix ? take(4LL * B * token_fix_rows(D, false)) : 0;
     if (o.mend) {

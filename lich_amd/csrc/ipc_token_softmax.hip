@@ -26,7 +26,7 @@
 // the results lose by it, and what is done:
 //   * G is rounded to the type itself, but a target's error, rounded once, would be off by as much for the whole
 //     column, and half of its values would be next to the right ones.  Small updates multiply two terms of the errors
-//     (2^-16, 2^-22) with W.
+//     (2^-16, 2^-22) with W; large ones add the target's row of W times what rounding left of its error to G's sums.
 //   * the loss is fp32 and would be off by the logits' rounding, 2^-9 (2^-12).  The loss alone
 //     takes f(X) in two terms (small calls in bf16: three), all in one tile, so that W is read once.
 //   * W: a sum that is 2^-9 off rounds a weight in a few hundred of a target's row the other
@@ -285,11 +285,61 @@ struct Hot {
   float* hot;                // [B][Dp]
   float scale;
 };
+
+// And out of W^T e: rest[d][n] = (e - rounded e) W[t_n][d], 64 features by 64 columns a workgroup, turned in LDS.
+struct Rest {
+  int V, D, B;
+  const void* w;
+  const long long* targets;
+  const float* loss;
+  float* rest;  // [D][B]
+  float scale;
+};
+template <typename OT>
+__device__ __forceinline__ void rest_of_targets(const Rest& p, int block) {
+  constexpr int WAVES = HOT_GROUPS, EACH = 64 / WAVES;
+  __shared__ float tile[64][65], left[64];
+  const int tiles_d = (p.D + 63) / 64, d0 = block % tiles_d * 64, n0 = block / tiles_d * 64;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const OT* w = static_cast<const OT*>(p.w) + (d0 + lane < p.D ? d0 + lane : 0);
+  // a wave has 16 columns, a lane of it the target and error of one
+  const int mine = n0 + wave * EACH + (lane & (EACH - 1));
+  long long id = mine < p.B ? p.targets[mine] : -1;
+  if (id >= p.V) id = -1;
+  const int row = (int)id;
+  if (lane < EACH) {
+    const float e = id < 0 ? 0.0f : token::target_error(p.loss[mine], p.scale);
+    left[wave * EACH + lane] = e - to_f32(cvt<OT>(e));
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  OT v[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int r = __builtin_amdgcn_readlane(row, i);
+    v[i] = w[(long long)(r < 0 ? 0 : r) * p.D];
+  }
+#pragma unroll
+  for (int i = 0; i < EACH; ++i)  // (a padded column: none, whatever its row would hold)
+    tile[wave * EACH + i][lane] = __builtin_amdgcn_readlane(row, i) < 0 ? 0.0f : to_f32(v[i]) * left[wave * EACH + i];
+  __syncthreads();
+  if (n0 + lane >= p.B) return;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int d = wave * EACH + i;
+    if (d0 + d < p.D) p.rest[(long long)(d0 + d) * p.B + n0 + lane] = tile[lane][d];
+  }
+}
+
+// Workgroups 0 .. first - 1: G's part; the others: W's.
 template <typename OT, bool TWO>
-__global__ void __launch_bounds__(HOT_GROUPS * 64) token_hot_kernel(const Hot p) {
+__global__ void __launch_bounds__(HOT_GROUPS * 64) token_hot_kernel(const Hot p, const Rest q, unsigned first) {
+  if (blockIdx.x < first) {
+    rest_of_targets<OT>(q, blockIdx.x);
+    return;
+  }
   __shared__ float4 red[HOT_GROUPS][64];
-  const int slabs = (p.Dp + 255) / 256, at = blockIdx.x / slabs, lane = threadIdx.x & 63;
-  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d = blockIdx.x % slabs * 256 + lane * 4;
+  const int slabs = (p.Dp + 255) / 256, block = blockIdx.x - first, at = block / slabs, lane = threadIdx.x & 63;
+  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d = block % slabs * 256 + lane * 4;
   const int id = p.key[at];
   if (id < 0 || (at > 0 && p.key[at - 1] == id)) return;
   float sum[4] = {};
@@ -406,16 +456,19 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
   float* fixes = o.fix ? reinterpret_cast<float*>(ws + o.fixes) : nullptr;
   const int vec_state = p.B % 4 == 0 && reinterpret_cast<uintptr_t>(p.x) % (4 * sizeof(ST)) == 0 &&
                         reinterpret_cast<uintptr_t>(p.g) % (4 * sizeof(ST)) == 0;
-  const TokenFinish finish{p.D, p.B, p.V, o.slices, p.act, reinterpret_cast<const float*>(ws + o.part), p.x, p.targets, p.g,
+  const TokenFinish finish{p.D, p.B, p.V, o.slices + (o.mend ? 1 : 0), p.act, reinterpret_cast<const float*>(ws + o.part), p.x, p.targets, p.g,
                            1.0f / scale, fixes, vec_state};
   auto make_good = [&] {  // once the losses are known
     int *order = reinterpret_cast<int*>(ws + o.order), *key = reinterpret_cast<int*>(ws + o.key);
     e = launch_sort_places(p.targets, p.B, p.V, order, key, reinterpret_cast<int*>(ws + o.slot), s);
     if (e != hipSuccess) return;
     const Hot h{p.B, p.D, o.Dp, order, key, at(o.ft), p.loss, reinterpret_cast<float*>(ws + o.hot), scale};
-    const dim3 grid((unsigned)((long long)p.B * ((o.Dp + 255) / 256))), block(HOT_GROUPS * 64);
-    if (o.ft_terms == 2) hipLaunchKernelGGL((token_hot_kernel<OT, true>), grid, block, 0, s, h);
-    else hipLaunchKernelGGL((token_hot_kernel<OT, false>), grid, block, 0, s, h);
+    // (the slice behind the products')
+    const Rest r{p.V, p.D, p.B, p.w, p.targets, p.loss, reinterpret_cast<float*>(ws + o.part) + (long long)o.slices * p.D * p.B, scale};
+    const unsigned rests = (unsigned)(((p.D + 63LL) / 64) * ((p.B + 63LL) / 64));
+    const dim3 grid(rests + (unsigned)((long long)p.B * ((o.Dp + 255) / 256))), block(HOT_GROUPS * 64);
+    if (o.ft_terms == 2) hipLaunchKernelGGL((token_hot_kernel<OT, true>), grid, block, 0, s, h, r, rests);
+    else hipLaunchKernelGGL((token_hot_kernel<OT, false>), grid, block, 0, s, h, r, rests);
     e = hipGetLastError();
   };
   for (int first = 0; first < p.V; first += o.rows) {

@@ -67,6 +67,32 @@ def test_state_gradients_round_as_the_exact_sums(V, D, B, activation, name):
     assert D > 1000 or bool(((plain < low) | (plain > high)).any())
 
 
+# Large updates: the target's error in fp32, the others, probabilities of a large vocabulary, rounded to the type (and kept as
+# fp16 times 2^15 of their part's largest): a_v each at most, of either sign, so that a sum of them passes 8 sqrt(sum a_v^2 W^2)
+# once in 10^13 (Hoeffding's bound).  f(X) is exact here.
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+@pytest.mark.parametrize("V,D,B,activation", [(524301, 8, 17, "relu"), (700001, 5, 13, "identity"), (5000, 33, 1700, "relu"), (6000, 300, 1500, "relu")])
+def test_state_gradients_of_large_updates(V, D, B, activation, name):
+    dt = TYPES[name]
+    u, half = half_step(dt), dt == torch.float16
+    x, w, t = (v.to(DEV) for v in softmax_case(V, D, B, dt, V + D))
+    got = run_update(x, w, t, activation, 0.25)[1]
+    r = O.softmax(x, w, t, activation)
+    hot = torch.zeros((V, B), dtype=torch.bool, device=DEV)
+    real = (t >= 0) & (t < V)
+    hot[t[real], real.nonzero()[:, 0]] = True
+    wa, p = w.double().abs(), r["p"]
+    dz = (r["size"] * (D / 16 + 64) * H).max(0).values
+    de = p * ((2 * dz).expm1() + 8 * H * (1 + p.clamp(min=1e-300).log().abs()) + 256 * H) + 4 * H * r["e"].abs()
+    rounded = torch.where(hot, 0.0, (u + 2.0 ** -11) * p + 2.0 ** -38 + 2.0 ** -35 * half)
+    back = wa.T @ de + 8 * ((wa ** 2).T @ rounded ** 2).sqrt() + (V / 16 + 64) * H * (wa.T @ r["e"].abs())
+    bound = r["df"].abs() * back + 2 * H * r["g"].abs()
+    low, high = (r["g"] - bound).to(dt), (r["g"] + bound).to(dt)
+    assert bool(((got >= low) & (got <= high)).all()), int(((got < low) | (got > high)).sum())
+    plain = (r["df"] * (w.double().T @ r["e"].to(dt).double())).to(dt)
+    assert V > 10000 or bool(((plain < low) | (plain > high)).any())
+
+
 # states that fit an operand in two terms but not in three; the last three in fp16, which takes two
 @pytest.mark.parametrize("V,D,B,activation,name", [(200, 10000, 40000, "tanh", "bf16"), (2, 8200, 50000, "relu", "bf16"), (1, 500, 800000, "gelu", "bf16"),
                                                    (300, 16384, 24576, "silu", "bf16"), (40, 20000, 20000, "tanh", "f16"), (3, 30000, 20000, "relu", "f16")])
