@@ -625,15 +625,15 @@ int ipc_dropout(const void* x, const long long* rng, void* out, int M, int B, in
  * bytes each, and for at most 8 samples the logits.  Sums are in fp32 in a fixed order.
  *   - at most 8 samples in fp32, 2 in 16 bits (4 where w has 2^22 values and more): fp32 products
  *     of the values as they are;
- *   - fp32: products of three bf16 terms each, exact to 2^-24, in which an infinite weight
- *     or state counts as the largest bf16;
+ *   - fp32: products of three bf16 terms each, exact to 2^-24;
  *   - 16 bits: w as it is; the loss alone takes f(X) in two terms of the type, a small call
  *     (at most 2^23 errors and 2^31 multiplications; of bf16 updates of up to 2048 words any number
  *     of these) f(X) and e in two fp16 or three bf16 terms (e for g in two).  A
  *     larger update rounds both to the type once, makes the targets' share of w's and g's
  *     sums good in fp32 and corrects the loss to first order in what f(X)'s rounding left.
- * A word whose weights give it logits far below the others' has no share of anything; infinite
- * weights are for the loss alone (g takes 0 times infinity where they are not the largest bf16).
+ * A word whose weights give it logits far below the others' has no share of anything.  Infinite weights and states
+ * multiply as numbers do, whatever the sizes: a logit of -infinity has no share, one of infinity or NaN makes its
+ * column's loss NaN.  Infinite weights are for the loss alone: g takes 0 times infinity.
  * Both need a workspace (16-byte aligned) of ipc_token_loss_workspace_bytes /
  * ipc_token_update_workspace_bytes bytes (0: refused).  w of 16 bits with an even D
  * lies on 4 bytes.

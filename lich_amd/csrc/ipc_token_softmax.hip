@@ -54,18 +54,30 @@ struct States {
 };
 
 // v as the operand's bits; of a sum of terms (`again`), what is left of it.  The first
-// term stays finite, of infinities too (the largest, and nothing left): the products of an
-// infinity with the other operand's terms, of either sign, would make a NaN of it.
+// term of a finite value stays finite; an infinite one's others are 0.
 template <typename OT>
 __device__ __forceinline__ unsigned short term(float& v, bool again) {
   OT o = cvt<OT>(v);
   if (again) {
     const bool inf = __builtin_isinf(v);
-    if (__builtin_isinf(to_f32(o)))
+    if (!inf && __builtin_isinf(to_f32(o)))
       o = __builtin_bit_cast(OT, (unsigned short)((v > 0.0f ? 0u : 0x8000u) | (std::is_same<OT, bf16>::value ? 0x7f7fu : 0x7bffu)));
     v = inf ? 0.0f : v - to_f32(o);
   }
   return __builtin_bit_cast(unsigned short, o);
+}
+// The same of f(X) in fp32, cut off towards zero (eight bits a term, so three are all 24): a value's terms have its
+// sign, those with nothing left too (2^-126), so that an infinite weight's products with them are all the
+// infinity that its product with the value is.  What the three products left out come to grows from 6e-9 of a logit to
+// 1.8e-8, where the fp32 sums of the others are 1e-7 off.
+__device__ __forceinline__ unsigned short inner_term(float& v) {
+  if (v != v) return __builtin_bit_cast(unsigned short, cvt<bf16>(v));
+  const unsigned bits = __builtin_bit_cast(unsigned, v) & 0xffff0000u;
+  if (v != 0.0f) {
+    const float left = v - __builtin_bit_cast(float, bits);
+    v = __builtin_fabsf(left) >= 0x1p-126f ? left : __builtin_copysignf(0x1p-126f, v);  // (of infinity NaN is left)
+  }
+  return (unsigned short)(bits >> 16);
 }
 
 template <typename ST, typename OT, int TERMS, int ACT>
@@ -89,7 +101,9 @@ __device__ __forceinline__ void lay_states(const States& p, int block) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int d = d0 + i * 8 + r;
-      const unsigned short h = term<OT>(v[i], TERMS > 1);
+      unsigned short h;
+      if constexpr (std::is_same<ST, float>::value) h = inner_term(v[i]);
+      else h = term<OT>(v[i], TERMS > 1);
       tile[i * 8 + r][c] = h;
       if (p.f && t < p.f_terms && d < p.D) p.f[((long long)t * p.D + d) * p.Bk + n] = h;
     }

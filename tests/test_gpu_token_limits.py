@@ -3,6 +3,7 @@ pieces, against their definitions in 64 bits on the device (bounds: those of tes
 import pytest
 import torch
 
+from lich_amd import tokens
 from tests import token_oracle as O
 from tests.helpers import DEV
 from tests.test_gpu_tokens import H, TYPES, half_step, run_update, softmax_bounds, softmax_case
@@ -91,6 +92,41 @@ def test_state_gradients_of_large_updates(V, D, B, activation, name):
     assert bool(((got >= low) & (got <= high)).all()), int(((got < low) | (got > high)).sum())
     plain = (r["df"] * (w.double().T @ r["e"].to(dt).double())).to(dt)
     assert V > 10000 or bool(((plain < low) | (plain > high)).any())
+
+
+# Infinities by the definition, in every form that a call takes by its size: a small layer, few samples, one tile, tiles and pieces of
+# exponentials.  A weight of -inf gives a logit of the sign of its state: -inf, a masked word, or inf, a loss of NaN.
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("activation", ["identity", "tanh"])
+@pytest.mark.parametrize("V,D,B", [(10, 20, 30), (700, 70, 2), (60, 33, 90), (300, 50, 40), (1000, 600, 130), (5000, 17, 260)])
+def test_infinities(V, D, B, activation, name):
+    dt = TYPES[name]
+    x, w, t = softmax_case(V, D, B, dt, V + D + B, padded=0.1)
+    t[0], t[1] = 1, V - 1
+    some = w.clone()
+    some[V - 1, 3] = -float("inf")
+    many = x.clone()
+    many[5, 0] = float("inf")
+    up = w.clone()
+    up[2] = float("inf")
+    for states, weights in ((x, some), (many, w), (x, up)):
+        if states is many and activation == "tanh":
+            continue  # (f is finite)
+        want = O.softmax(states, weights, t, activation)["loss"]
+        k, loss = tokens.build_token_loss(V, D, B, activation, dt), torch.zeros(B, device=DEV)
+        k(states.to(DEV), weights.to(DEV), t.to(DEV), loss, workspace=k.new_workspace(DEV))
+        got = loss.cpu().double()
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got == float("inf"), want == float("inf"))
+        if states is many:
+            trained, g, _ = run_update(states.to(DEV), weights.to(DEV), t.to(DEV), activation, 0.25)
+            assert bool(trained[0].isnan()) and bool(trained[1:].isfinite().all()) and bool(g[:, 1:].isfinite().all())
+        fine = want.isfinite()
+        assert bool(fine.any()) or weights is up
+        # (what a masked word adds is 0; its row is left out of the bounds)
+        kept = weights.clone()
+        kept[weights.isinf()] = 0.0
+        r = O.softmax(x, kept, t, activation)
+        assert bool(((got - want).abs() <= softmax_bounds(r, kept, dt, V, D, B, activation, 0.0, False)[0])[fine].all())
 
 
 # states that fit an operand in two terms but not in three; the last three in fp16, which takes two
