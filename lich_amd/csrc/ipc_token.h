@@ -57,6 +57,31 @@ inline EmbedLayout embed_layout(int D, int C, int B, int element) {
   l.bytes = n < EMBED_SORTED ? 0 : l.part + up(runs * 2 * D * 4);
   return l;
 }
+// Ids of a range of the sort, at most 512: a workgroup for each 32 places, up to one a CU.  (Few ids each:
+// a wave places the ids that it meets among 64 places one after the other; 8192 places of 64
+// ids in one range: 56 us, in 64: 11.  But few workgroups for few places: 1505 places of 1531
+// ids, 256 ranges 10.6 us, 24 6.2.)
+inline int sort_range(int V, int N) {
+  const int most = N < 64 ? 1 : N / 32 < 256 ? N / 32 : 256, r = (V + most - 1LL) / most < 512 ? (int)((V + most - 1LL) / most) : 512;
+  return r;
+}
+// Samples of a block that the sort's launch turns (by 64 features).
+constexpr int embed_turn(int element) { return element == 4 ? 128 : 256; }
+// Workgroups of the lookup: of 256 threads each for a block of samples by features of a place.
+inline long long embed_blocks(int D, int C, int B) {
+  const int bt = B == 1 ? 1 : B <= 4 ? 4 : B <= 16 ? 16 : 64, dt = bt == 1 ? 1024 : 4096 / bt;
+  return (long long)C * ((B + bt - 1LL) / bt) * ((D + dt - 1LL) / dt);
+}
+// Whether the calls' launches stay below 2^32 work-items.
+inline bool embed_fits(int V, int D, int C, int B, int element) {
+  constexpr long long most = (1LL << 32) - 1;
+  const long long n = (long long)C * B;
+  if (256 * embed_blocks(D, C, B) > most) return false;
+  if (n < EMBED_SORTED) return true;
+  const int range = sort_range(V, (int)n), turn = embed_turn(element);
+  const long long sorts = ((long long)V + range - 1) / range + (long long)C * ((B + turn - 1LL) / turn) * ((D + 63LL) / 64);
+  return 1024 * sorts <= most && 256 * ((n + EMBED_RUN - 1) / EMBED_RUN) <= most;
+}
 hipError_t launch_embedding_update(const EmbedUpdate& p, int storage, hipStream_t s);
 // Places of N ids sorted by id, ties in their order: order [N], key [N + 1] as in EmbedUpdate; slot
 // [V]: the first sorted position of each id, -1 of those that do not occur.

@@ -16,6 +16,8 @@ int check_embedding(int V, int D, int C, int B, int storage) {
     return fail(IPC_ERR_SHAPE, "dimensions must be >= 1 (V=%d D=%d C=%d B=%d)", V, D, C, B);
   if ((long long)V * D > kMaxElems || (long long)C * B > kMaxElems || (long long)C * B * D > kMaxElems)
     return fail(IPC_ERR_SHAPE, "table or state too large (V=%d D=%d C=%d B=%d)", V, D, C, B);
+  if (!embed_fits(V, D, C, B, elem_size(storage)))
+    return fail(IPC_ERR_SHAPE, "too large for a launch (V=%d D=%d C=%d B=%d)", V, D, C, B);
   return ok();
 }
 
@@ -33,7 +35,7 @@ int check_token(const void* x, const void* w, const void* targets, const void* l
   TRY(check_act(act));
   TRY(check_dims(V, D, B, 1));
   if (token_workspace_bytes(V, D, B, storage, act, update) == 0)
-    return fail(IPC_ERR_SHAPE, "states too large (D=%d B=%d)", D, B);
+    return fail(IPC_ERR_SHAPE, "too large (V=%d D=%d B=%d)", V, D, B);
   TRY(check_ptr(x, "x", elem_size(storage)));
   TRY(check_ptr(w, "w", elem_size(storage)));
   if (storage != IPC_DT_F32 && D % 2 == 0 && reinterpret_cast<uintptr_t>(w) % 4)

@@ -152,17 +152,8 @@ __global__ void __launch_bounds__(256) embed_few_kernel(const EmbedUpdate p) {
 // between the two readings.  The other workgroups transpose G.
 constexpr int SORT_WAVES = 16, SORT_HELD = 8;
 
-// Ids of a range, at most 512: a workgroup for each 32 places, up to one a CU.  (Few ids each:
-// a wave places the ids that it meets among 64 places one after the other; 8192 places of 64
-// ids in one range: 56 us, in 64: 11.  But few workgroups for few places: 1505 places of 1531
-// ids, 256 ranges 10.6 us, 24 6.2.)
-inline int sort_range(int V, int N) {
-  const int most = N < 64 ? 1 : N / 32 < 256 ? N / 32 : 256, r = (V + most - 1) / most;
-  return r > 512 ? 512 : r;
-}
-
 // A block of G, 64 features by TURN samples, so that each thread has several loads in flight.
-template <typename ST> constexpr int TURN = sizeof(ST) == 4 ? 128 : 256;
+template <typename ST> constexpr int TURN = embed_turn(sizeof(ST));
 template <typename ST, bool VEC>
 __device__ void transpose_rows(const EmbedUpdate& p, int block, ST* tile) {
   constexpr int W = TURN<ST>, LD = W + 2, EACH = 64 * W / 4 / (SORT_WAVES * 64);
@@ -445,13 +436,11 @@ hipError_t run_sums(const EmbedUpdate& p, hipStream_t s) {
 
 template <typename ST>
 hipError_t run_embed(const EmbedProblem& p, hipStream_t s) {
-  auto blocks = [&](int bt, int dt) {
-    return dim3((unsigned)((long long)p.C * ((p.B + bt - 1) / bt) * ((p.D + dt - 1) / dt)));
-  };
-  if (p.B == 1) hipLaunchKernelGGL((embed_kernel<ST, 1>), blocks(1, 1024), dim3(256), 0, s, p);
-  else if (p.B <= 4) hipLaunchKernelGGL((embed_kernel<ST, 4>), blocks(4, 1024), dim3(256), 0, s, p);
-  else if (p.B <= 16) hipLaunchKernelGGL((embed_kernel<ST, 16>), blocks(16, 256), dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((embed_kernel<ST, 64>), blocks(64, 64), dim3(256), 0, s, p);
+  const dim3 grid((unsigned)embed_blocks(p.D, p.C, p.B)), block(256);
+  if (p.B == 1) hipLaunchKernelGGL((embed_kernel<ST, 1>), grid, block, 0, s, p);
+  else if (p.B <= 4) hipLaunchKernelGGL((embed_kernel<ST, 4>), grid, block, 0, s, p);
+  else if (p.B <= 16) hipLaunchKernelGGL((embed_kernel<ST, 16>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((embed_kernel<ST, 64>), grid, block, 0, s, p);
   return hipGetLastError();
 }
 

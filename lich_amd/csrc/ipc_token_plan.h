@@ -27,6 +27,14 @@ constexpr long long TOKEN_FINE_ERRORS = 1LL << 23, TOKEN_FINE_WORK = 1LL << 31;
 // next loss 2e-5 .. 5e-5 off (600 x 8000 x 1000, 1201 x 4040 x 2744; fine: under 1e-6).
 constexpr int TOKEN_FINE_WORDS = 2048;
 
+// A column's errors in one workgroup, up to so many; of more, one for each 2048.
+constexpr int TOKEN_ERROR_RUN = 8192;
+inline long long token_error_blocks(int Bk, int Vp) { return (long long)Bk * (Vp <= TOKEN_ERROR_RUN ? 1 : (Vp + 2047) / 2048); }
+// Workgroups of the launch that makes the targets' errors good, for G and for W.
+inline long long token_rest_blocks(int D, int B) { return (D + 63LL) / 64 * ((B + 63LL) / 64); }
+inline long long token_hot_blocks(int Dp, int B) { return (long long)B * ((Dp + 255) / 256); }
+constexpr long long TOKEN_LAUNCH = (1LL << 32) - 1;  // work-items of a launch
+
 struct TokenPlan {
   int terms, Dp, Bk;
   bool copy;          // W laid out per piece: fp32, 16-bit rows of an odd length, or for `tail`
@@ -113,6 +121,9 @@ inline bool plan_token(int V, int D, int B, int storage, int act, bool update, T
   // 6 x 73 x 3026 21.7 / 45, 329 x 3 x 4059 40 / 66, 26 x 40 x 2000 21.3 / 29.2; two: 256 x 256 x 512 27.2 / 25.6)
   o.cut = (int)std::min<long long>(o.Bk / 256, (256 - tiles(D, B, 64)) / tiles(V, D, 64));
   if (o.cut < 3) o.cut = 1;
+  // (the other launches have fewer work-items than an operand has bytes)
+  if (o.keep && !o.one && 256 * token_error_blocks(o.Bk, o.Vp) > TOKEN_LAUNCH) return false;
+  if (o.mend && (256 * (token_rest_blocks(D, B) + token_hot_blocks(o.Dp, B)) > TOKEN_LAUNCH || 2LL * V + 1024 > TOKEN_LAUNCH)) return false;
   long long at = 0;
   auto take = [&](long long bytes) {
     const long long here = at;

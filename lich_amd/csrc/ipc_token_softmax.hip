@@ -198,11 +198,10 @@ __global__ void __launch_bounds__(256) token_fix_kernel(const float* fixes, int 
 
 // ------------------------------------------------------------------ errors
 // Kept exponentials into errors, in place, or from fp32 into two or three terms: a column (a row of ET, up
-// to Vp) a workgroup, which joins the column's parts itself, up to ERROR_RUN values; of longer
+// to Vp) a workgroup, which joins the column's parts itself, up to TOKEN_ERROR_RUN values; of longer
 // ones 2048 values, their columns joined before.  Zeros past the ends and in padded rows, up
 // to Bk.  us, joining here / before: V = 10007, B = 77 fp32 9.6 / 4.7 + 5.4; V = 32000, B = 1024
 // bf16 34.8 / 6.3 + 27.0; V = 128000, B = 2048 341 / 14.6 + 226.
-constexpr int ERROR_RUN = 8192;
 struct Errors {
   int V, B, Vp, Bk, unit, units;
   const void* kept;     // [Bk][Vp]
@@ -456,7 +455,7 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
   }
   if (e != hipSuccess) return e;
   const int units = (p.V + o.unit - 1) / o.unit;
-  const bool joined = o.keep && o.Vp <= ERROR_RUN;  // with the errors
+  const bool joined = o.keep && o.Vp <= TOKEN_ERROR_RUN;  // with the errors
   if (!joined && !o.one) {
     const Columns c{p.B, p.V, units, part, reinterpret_cast<const float*>(ws + o.logit), p.targets, p.loss,
                     reinterpret_cast<float2*>(ws + o.norm)};
@@ -479,8 +478,8 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
     const Hot h{p.B, p.D, o.Dp, order, key, at(o.ft), p.loss, reinterpret_cast<float*>(ws + o.hot), scale};
     // (the slice behind the products')
     const Rest r{p.V, p.D, p.B, p.w, p.targets, p.loss, reinterpret_cast<float*>(ws + o.part) + (long long)o.slices * p.D * p.B, scale};
-    const unsigned rests = (unsigned)(((p.D + 63LL) / 64) * ((p.B + 63LL) / 64));
-    const dim3 grid(rests + (unsigned)((long long)p.B * ((o.Dp + 255) / 256))), block(HOT_GROUPS * 64);
+    const unsigned rests = (unsigned)token_rest_blocks(p.D, p.B);
+    const dim3 grid(rests + (unsigned)token_hot_blocks(o.Dp, p.B)), block(HOT_GROUPS * 64);
     if (o.ft_terms == 2) hipLaunchKernelGGL((token_hot_kernel<OT, true>), grid, block, 0, s, h, r, rests);
     else hipLaunchKernelGGL((token_hot_kernel<OT, false>), grid, block, 0, s, h, r, rests);
     e = hipGetLastError();
@@ -490,7 +489,7 @@ hipError_t run(const TokenProblem& p, int storage, hipStream_t s) {
     if (o.keep && !o.one) {
       const Errors er{p.V, p.B, Vp, o.Bk, o.unit, units, ws + o.kept, at(o.et), part, reinterpret_cast<const float*>(ws + o.logit),
                       p.loss, reinterpret_cast<const float2*>(ws + o.norm), p.targets, scale};
-      const dim3 grid((unsigned)((long long)o.Bk * (joined ? 1 : (Vp + 2047) / 2048)));
+      const dim3 grid((unsigned)token_error_blocks(o.Bk, Vp));
       constexpr int MORE = std::is_same<OT, bf16>::value ? 3 : 2;
       if (o.e_terms == 1 && joined) hipLaunchKernelGGL((token_errors_kernel<OT, TERMS, true>), grid, dim3(256), 0, s, er);
       else if (o.e_terms == 1) hipLaunchKernelGGL((token_errors_kernel<OT, TERMS, false>), grid, dim3(256), 0, s, er);

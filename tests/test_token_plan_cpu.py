@@ -7,6 +7,8 @@ from pathlib import Path
 
 import pytest
 
+from lich_amd import _native as nat
+
 ROOT = Path(__file__).resolve().parents[1]
 F32, F16, BF16 = 0, 1, 2
 IDENTITY, TANH = 0, 2
@@ -144,3 +146,36 @@ def test_every_slice_of_every_piece_has_a_stage(plans, accepted):
             assert 0 <= begin < end <= (p.last + 31) // 32, p.case
         short += p.rows < p.V and p.last_slices < p.slices
     assert short > 20
+
+
+P = 4096  # a fake, aligned, non-null address; never dereferenced (validation fails first)
+
+
+@pytest.mark.parametrize("V,D,C,B", [(10, 1, 1 << 24, 1), (10, 1, 1 << 24, 3), (5, 2, 1 << 25, 17), (100, 1, 1, 1 << 30), (100, 1, 2, 1 << 29)])
+def test_embeddings_of_too_many_places_for_a_launch_are_refused(V, D, C, B):
+    """2^32 work-items and more: before any of an update's launches has run."""
+    lib, big = nat.lib(), 1 << 50
+    for storage in (F32, F16, BF16):
+        if B < 1 << 29:
+            assert lib.ipc_embedding(P, P, P, V, D, C, B, 1.0, storage, None) == nat.ERR_SHAPE and "launch" in nat.last_error()
+        assert lib.ipc_embedding_update(P, P, P, V, D, C, B, 1.0, storage, P, big, None) == nat.ERR_SHAPE and "launch" in nat.last_error()
+        assert lib.ipc_embedding_update_workspace_bytes(V, D, C, B, storage) == 0
+
+
+def test_updates_of_too_many_samples_for_a_launch_are_refused(plans):
+    lib = nat.lib()
+    for V, D, B in ((1, 8, 1 << 24), (3, 30, 20000000), (100, 2, 17000000)):
+        for storage in (F16, BF16):
+            assert lib.ipc_token_update_workspace_bytes(V, D, B, storage, TANH) == 0
+            assert lib.ipc_token_update(P, P, P, P, P, V, D, B, 1.0, storage, TANH, P, 1 << 50, None) == nat.ERR_SHAPE
+            assert "too large" in nat.last_error()
+    assert len(plans([(1, 8, 1 << 24, BF16, IDENTITY, 0), (1, 60, 8000000, BF16, TANH, 1)])) == 2
+
+
+def test_no_launch_has_too_many_work_items(accepted):
+    for p in accepted:
+        if p.keep and not p.one:
+            runs = 1 if p.Vp <= 8192 else (p.Vp + 2047) // 2048
+            assert 256 * p.Bk * runs < 1 << 32, p.case
+        if p.mend:
+            assert 256 * (-(-p.D // 64) * -(-p.B // 64) + p.B * -(-p.Dp // 256)) < 1 << 32, p.case
