@@ -630,7 +630,7 @@ int ipc_dropout(const void* x, const long long* rng, void* out, int M, int B, in
  *     (at most 2^23 errors and 2^31 multiplications; of bf16 updates of up to 2048 words any number
  *     of these) f(X) and e in two fp16 or three bf16 terms (e for g in two).  A
  *     larger update rounds both to the type once, makes the targets' share of w's and g's
- *     sums good in fp32 and corrects the loss to first order in what f(X)'s rounding left.
+ *     sums good in fp32 and corrects the loss to first order in what f(X)'s rounding left (not below 0).
  * A word whose weights give it logits far below the others' has no share of anything.  Infinite weights and states
  * multiply as numbers do, whatever the sizes: a logit of -infinity has no share, one of infinity or NaN makes its
  * column's loss NaN.  Infinite weights are for the loss alone: g takes 0 times infinity.

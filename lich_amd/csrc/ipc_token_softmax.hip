@@ -180,7 +180,8 @@ __global__ void __launch_bounds__(1024) token_columns_kernel(const Columns p, in
 }
 
 // ---------------------------------------------------------------- the loss
-// loss -= the fixes, in order; 16 columns a workgroup, 16 threads each
+// loss -= the fixes, in order; 16 columns a workgroup, 16 threads each.  (Not below 0, where to first order it may
+// be once logits of a thousand and more are off by some.)
 __global__ void __launch_bounds__(256) token_fix_kernel(const float* fixes, int rows, int B, float* loss) {
   __shared__ float red[16][16];
   const int c = threadIdx.x & 15, g = threadIdx.x >> 4, n = blockIdx.x * 16 + c;
@@ -193,7 +194,8 @@ __global__ void __launch_bounds__(256) token_fix_kernel(const float* fixes, int 
   if (g != 0 || n >= B) return;
 #pragma unroll
   for (int i = 1; i < 16; ++i) sum += red[i][c];
-  loss[n] -= sum;
+  sum = loss[n] - sum;
+  loss[n] = sum < 0.0f ? 0.0f : sum;
 }
 
 // ------------------------------------------------------------------ errors

@@ -129,6 +129,20 @@ def test_infinities(V, D, B, activation, name):
         assert bool(((got - want).abs() <= softmax_bounds(r, kept, dt, V, D, B, activation, 0.0, False)[0])[fine].all())
 
 
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+def test_losses_of_huge_logits_are_not_negative(name):
+    """Logits of thousands, which rounding f(X) moves by some: a loss corrected to first order stays a loss."""
+    dt, V, D, B = TYPES[name], 9000, 300, 2000
+    x, w, t = (v.to(DEV) for v in softmax_case(V, D, B, dt, 4, padded=0.0, wscale=600.0 if name == "f16" else 100.0))
+    t[:] = (w.double() @ torch.tanh(x.double())).argmax(0)
+    loss = run_update(x, w, t, "tanh", 0.0)[0]
+    assert bool(torch.isfinite(loss).all()) and float(loss.min()) >= 0.0
+    want = O.softmax(x, w, t, "tanh")["loss"]
+    off = (w.double() @ (torch.tanh(x.double()) - torch.tanh(x.double()).to(dt).double())).abs().amax(0)
+    # (rounding moves the logits by `off` at most, and a loss by twice that; the correction moves it by as much again)
+    assert bool(((loss.double() - want).abs() <= 4 * off + 2.0 ** -10).all())
+
+
 # states that fit an operand in two terms but not in three; the last three in fp16, which takes two
 @pytest.mark.parametrize("V,D,B,activation,name", [(200, 10000, 40000, "tanh", "bf16"), (2, 8200, 50000, "relu", "bf16"), (1, 500, 800000, "gelu", "bf16"),
                                                    (300, 16384, 24576, "silu", "bf16"), (40, 20000, 20000, "tanh", "f16"), (3, 30000, 20000, "relu", "f16")])
