@@ -634,7 +634,7 @@ int ipc_dropout(const void* x, const long long* rng, void* out, int M, int B, in
  * A word whose weights give it logits far below the others' has no share of anything.  Infinite weights and states
  * multiply as numbers do, whatever the sizes: a logit of -infinity has no share, one of infinity or NaN makes its
  * column's loss NaN.  Infinite weights are for the loss alone: g takes 0 times infinity.
- * Both need a workspace (16-byte aligned) of ipc_token_loss_workspace_bytes /
+ * V D, V B and D B lie below 2^31.  Both need a workspace (16-byte aligned) of ipc_token_loss_workspace_bytes /
  * ipc_token_update_workspace_bytes bytes (0: refused).  w of 16 bits with an even D
  * lies on 4 bytes.
  */

@@ -27,7 +27,8 @@ struct EmbedProblem {
 hipError_t launch_embedding(const EmbedProblem& p, int storage, hipStream_t s);
 
 // Places are sorted by id, ties in their order; their rows of G, transposed once, are then
-// summed in runs of EMBED_RUN places, and sums that cross a run's end joined in order.
+// summed in runs of EMBED_RUN places, and sums that cross a run's end joined: in order, or by up to four groups of
+// threads that have a part of the runs each.  The order is the same every time.
 constexpr int EMBED_RUN = 16;
 // From so many places on (below, one launch finds the places of an id itself).
 constexpr int EMBED_SORTED = 513;

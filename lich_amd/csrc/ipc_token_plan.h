@@ -24,7 +24,11 @@ constexpr long long TOKEN_OPERAND = (1LL << 31) - 1;                  // of an o
 // 16-bit updates of at most so many errors and multiplications are `fine`.
 constexpr long long TOKEN_FINE_ERRORS = 1LL << 23, TOKEN_FINE_WORK = 1LL << 31;
 // And in bf16 those of few words: there probabilities are not small, and rounding them to 8 bits leaves the
-// next loss 2e-5 .. 5e-5 off (600 x 8000 x 1000, 1201 x 4040 x 2744; fine: under 1e-6).
+// next loss off in its fifth digit.  The next loss's error and us, one term / fine, 4000 features, 1024 samples: 2048 words
+// 1.9e-5 / 7.6e-7, 159 / 235; 4096 8.5e-6 / 3.3e-7, 194 / 423; 8192 5.8e-6 / 8.4e-7, 301 / 798.  4000 samples: 512 words
+// 2.3e-5 / 1.4e-6, 288 / 400; 2048 1.0e-5 / 1.5e-6, 436 / 977.  From 2048 words on, or with more errors, one term keeps the loss
+// to five digits and a fine update costs twice the time.  (600 x 8000 x 1000 and 1201 x 4040 x 2744 with one: 5e-5 and
+// 4e-5.)  In fp16 one term leaves 3.4e-6 at 512 words, 2.0e-6 at 2048.
 constexpr int TOKEN_FINE_WORDS = 2048;
 
 // A column's errors in one workgroup, up to so many; of more, one for each 2048.

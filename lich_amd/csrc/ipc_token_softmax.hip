@@ -36,7 +36,8 @@
 //   correct the loss to first order by the gradient that they have, loss -= sum_d (W^T e)_d (f - rounded
 //   f)_d (left: half the variance of the logits' rounding, 3e-6 of a loss for bf16 logits of deviation
 //   3), and make the errors at the targets, the ones near 1, good in fp32 (token_hot_kernel; left in the next
-//   loss: 2e-7 .. 2e-5).
+//   loss: up to 2e-5 in bf16, 3e-6 in fp16, most with few words).  Other errors are probabilities, each rounded
+//   once: where a net gives one of them most of a column, that column of G is off by up to its rounding.
 #include "ipc_token_gemm.h"
 
 namespace ipc {
@@ -289,7 +290,7 @@ __global__ void __launch_bounds__(256) token_errors_kernel(const Errors p) {
 // few hundred of a target's row rounds the other way, and the next loss differs by 1e-5 .. 1e-3.)
 // A workgroup has 256 features of a position: HOT_GROUPS waves take every so many-th column.  (Words
 // are not drawn evenly: the commonest has a tenth of the columns.  128000 words, 2048 samples of 2048 features,
-// fp16: 26 us.)
+// fp16: 26 us; with G's part 33.)
 constexpr int HOT_GROUPS = 4;
 struct Hot {
   int B, D, Dp;

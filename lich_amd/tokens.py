@@ -59,7 +59,7 @@ class EmbeddingKernel(_TokenKernel):
 
 class EmbeddingUpdateKernel(_TokenKernel):
     """``k(TABLE[V, D], IDS[C, B], G[C * D, B], *, workspace)``: ``TABLE[v] += alpha * sum of G's
-    columns at the places of v``, the sum in fp32 in the places' order, one rounding.
+    columns at the places of v``, the sum in fp32 in a fixed order, one rounding.
     ``workspace`` (caller-owned, ``new_workspace()``) is needed where
     ``workspace_bytes`` is not 0."""
 
