@@ -179,3 +179,10 @@ def test_no_launch_has_too_many_work_items(accepted):
             assert 256 * p.Bk * runs < 1 << 32, p.case
         if p.mend:
             assert 256 * (-(-p.D // 64) * -(-p.B // 64) + p.B * -(-p.Dp // 256)) < 1 << 32, p.case
+
+
+@pytest.mark.parametrize("storage", [F32, F16, BF16])
+def test_pieces_bound_what_a_large_vocabulary_takes(plans, storage):
+    """Errors and laid-out weights of a piece 1 GiB each, whatever the vocabulary."""
+    got = plans((V, 64, B, storage, TANH, 1) for V, B in ((1 << 19, 4095), (1 << 20, 2047), (1 << 24, 127), (1 << 24, 33)))
+    assert len(got) == 4 and all(p.rows < p.V and 1 << 30 < p.bytes < 3 << 30 for p in got), [(p.case, p.rows, p.bytes) for p in got]
