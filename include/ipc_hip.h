@@ -625,7 +625,7 @@ int ipc_dropout(const void* x, const long long* rng, void* out, int M, int B, in
  * bytes each, and for at most 8 samples the logits.  Sums are in fp32 in a fixed order.
  *   - at most 8 samples in fp32, 2 in 16 bits (4 where w has 2^22 values and more): fp32 products
  *     of the values as they are;
- *   - fp32: products of three bf16 terms each, exact to 2^-24;
+ *   - fp32: products of three bf16 terms each, exact to 2^-24 (with f(X) 2^-22);
  *   - 16 bits: w as it is; the loss alone takes f(X) in two terms of the type, a small call
  *     (at most 2^23 errors and 2^31 multiplications; of bf16 updates of up to 2048 words any number
  *     of these) f(X) and e in two fp16 or three bf16 terms (e for g in two).  A

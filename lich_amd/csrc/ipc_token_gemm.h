@@ -18,7 +18,7 @@
 // copy of W and one of the errors serve both products they appear in.
 //
 // fp32 tensors: every operand is the sum of three bf16 terms (24 bits, the type's own), and a
-// product the six term products above 2^-24 of it, smallest first, from one stage that holds
+// product the six term products above 2^-24 of it (2^-22 with f(X), whose terms are cut off), smallest first, from one stage that holds
 // all terms.  Six times the 16-bit work, but the fp32 matrix instruction takes sixteen.
 //
 // What they reach (fp16, 128000 words, 2048 features, 2048 samples, 1.07 PFLOP each; a library's

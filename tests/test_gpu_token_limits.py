@@ -154,3 +154,120 @@ def test_updates_of_large_states(V, D, B, activation, name):
 @pytest.mark.parametrize("V,D,B,name", [(524298, 64, 1000, "bf16"), (524289, 8, 1000, "f16"), (131073, 300, 4096, "f16"), (21770, 8192, 64, "f32"), (91793, 1949, 118, "f32")])
 def test_short_last_pieces(V, D, B, name):
     check_update(*large_case(V, D, B, TYPES[name]), "tanh", 0.5)
+
+
+def off(t, by):
+    """The same values `by` elements behind a 256-byte boundary."""
+    base = torch.zeros(t.numel() + by, dtype=t.dtype, device=DEV)
+    view = base[by:].view(t.shape)
+    view.copy_(t)
+    return view
+
+
+# every form of a call: a small layer, few samples, one tile, two launches at the end, slices, large products, two pieces
+FORMS = [(10, 64, 128), (900, 72, 2), (60, 34, 92), (300, 52, 40), (20, 40, 1000), (1000, 600, 130), (3001, 36, 64), (6000, 300, 1500), (9000, 33, 1000), (524298, 8, 1000)]
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("V,D,B", FORMS)
+def test_softmax_calls_on_tensors_off_their_boundaries(V, D, B, name):
+    """The same bits; a loss corrected by sums of other parts within 8 H of what the sums hold."""
+    dt = TYPES[name]
+    x, w, t = large_case(V, D, B, dt)
+    k = tokens.build_token_update(V, D, B, "tanh", dt, 0.3)
+    score = tokens.build_token_loss(V, D, B, "tanh", dt)
+    ws, ws2 = k.new_workspace(DEV), score.new_workspace(DEV)
+    got = []
+    for by in (0, 1, 2, 3, 6):
+        by_w = by if dt == torch.float32 or D % 2 else by // 2 * 2  # (rows of an even length lie on 4 bytes)
+        a, v, loss, g, alone = off(x, by), off(w, by_w), off(torch.zeros(B, device=DEV), by), off(torch.zeros_like(x), by + 1), off(torch.zeros(B, device=DEV), by)
+        score(a, v, t, alone, workspace=ws2)
+        k(a, v, t, loss, g, workspace=ws)
+        got.append((alone, g, v, loss))
+    for other in got[1:]:
+        assert all(torch.equal(p, q) for p, q in zip(got[0][:3], other[:3]))
+        assert float((got[0][3] - other[3]).abs().max()) <= 8 * H * 64
+    assert bool(torch.isfinite(got[0][3]).all())
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("V,D,C,B", [(50, 64, 3, 1), (50, 64, 3, 4), (50, 64, 3, 40), (700, 36, 2, 300), (700, 131, 1, 600)])
+def test_embedding_calls_on_tensors_off_their_boundaries(V, D, C, B, name):
+    dt = TYPES[name]
+    g = torch.Generator(device=DEV).manual_seed(V + D)
+    table, e = torch.randn((V, D), generator=g, device=DEV).to(dt), torch.randn((C * D, B), generator=g, device=DEV).to(dt)
+    ids = torch.randint(-1, V, (C, B), generator=g, device=DEV)
+    look, learn = tokens.build_embedding(V, D, C, B, dt, 1.5), tokens.build_embedding_update(V, D, C, B, dt, 0.1)
+    ws, got = learn.new_workspace(DEV), []
+    for by in (0, 1, 2, 3, 6):
+        x, rows = off(torch.zeros_like(e), by + 1), off(table, by)
+        look(off(ids, by), rows, x)
+        learn(rows, ids, off(e, by), workspace=ws)
+        got.append((x, rows))
+    for other in got[1:]:
+        assert all(torch.equal(p, q) for p, q in zip(got[0], other))
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("V,D,B", FORMS)
+def test_targets_that_are_all_padded(V, D, B, name):
+    dt = TYPES[name]
+    x, w, _ = large_case(V, D, B, dt)
+    x[0] = float("nan")
+    loss, g, wn = run_update(x, w, torch.full((B,), -1, device=DEV), "gelu", 0.5)
+    assert bool((loss == 0).all()) and bool((g == 0).all()) and torch.equal(wn, w)
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("V,D,B", FORMS[5:])
+def test_large_calls_in_a_graph(V, D, B, name):
+    """Replays between eager calls, both in one workspace, give the eager bits."""
+    dt = TYPES[name]
+    x, w, t = large_case(V, D, B, dt)
+    k = tokens.build_token_update(V, D, B, "silu", dt, 0.3)
+    ws = k.new_workspace(DEV)
+
+    def new():
+        return w.clone(), torch.empty(B, device=DEV), torch.empty_like(x)
+
+    eager, kept, side = new(), new(), torch.cuda.Stream()
+    warm = new()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        k(x, warm[0], t, *warm[1:], workspace=ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        k(x, kept[0], t, *kept[1:], workspace=ws)
+    for _ in range(3):
+        k(x, eager[0], t, *eager[1:], workspace=ws)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(eager, kept))
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("V,D,B", FORMS[3:9])
+def test_one_target_in_every_column(V, D, B, name):
+    x, w, t = large_case(V, D, B, TYPES[name])
+    check_update(x, w, torch.full_like(t, V - 1), "relu", 0.25 / B)
+
+
+@pytest.mark.parametrize("name", TYPES)
+def test_calls_on_two_streams_at_once(name):
+    """Each with a workspace of its own."""
+    dt, V, D, B = TYPES[name], 6000, 300, 1500
+    x, w, t = large_case(V, D, B, dt)
+    k = tokens.build_token_update(V, D, B, "gelu", dt, 0.3)
+    want = run_update(x, w, t, "gelu", 0.3)
+    streams, calls = [torch.cuda.Stream() for _ in range(3)], []
+    for _ in streams:
+        calls.append((k.new_workspace(DEV), w.clone(), torch.empty(B, device=DEV), torch.empty_like(x)))
+    torch.cuda.synchronize()
+    for s, (ws, v, loss, g) in zip(streams, calls):
+        with torch.cuda.stream(s):
+            k(x, v, t, loss, g, workspace=ws)
+    torch.cuda.synchronize()
+    for _, v, loss, g in calls:
+        assert torch.equal(v, want[2]) and torch.equal(loss, want[0]) and torch.equal(g, want[1])
